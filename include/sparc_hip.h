@@ -579,6 +579,97 @@ sparc_status sparc_rms_norm_backward(int64_t rows, int64_t cols, int32_t io_dtyp
                                      const float* rstd, const void* dy, void* dx, float* dweight, void* workspace,
                                      size_t workspace_bytes, sparc_stream_t stream);
 
+/* ---- Layer norm ------------------------------------------------------------
+ * x, y [rows, cols] in io_dtype, any cols > 0; weight, bias [cols] in
+ * param_dtype (io_dtype, or F32 beside BF16 I/O), each NULL where there is
+ * none; mean, rstd [rows] fp32, written where given (both or neither; the
+ * backward needs them).  Per row, in fp32 arithmetic: mu = mean(x), rstd =
+ * 1 / sqrt(mean((x - mu)^2) + eps), y = (x - mu) rstd weight + bias.  Pointers
+ * are aligned to their values; 16-byte alignment (and cols a multiple of 16
+ * bytes) takes the widest accesses.  No counterpart in the reference, which
+ * ships the layer, not a network: torch.nn.LayerNorm's formula. */
+sparc_status sparc_layer_norm_forward(int64_t rows, int64_t cols, int32_t io_dtype, int32_t param_dtype, const void* x,
+                                      const void* weight, const void* bias, float eps, void* y, float* mean,
+                                      float* rstd, sparc_stream_t stream);
+
+/* Workspace bytes of sparc_layer_norm_backward (0: invalid shape). */
+size_t sparc_layer_norm_workspace_bytes(int64_t rows, int64_t cols);
+
+/* Backward of sparc_layer_norm_forward given its mean and rstd and dy [rows,
+ * cols] (io_dtype): with xhat = (x - mean) rstd and g = dy weight, dx = rstd
+ * (g - mean(g) - xhat mean(g xhat)) (io_dtype), dweight [cols] = the sum over
+ * rows of dy xhat and dbias [cols] = the sum over rows of dy (param_dtype),
+ * summed in fp32 in a fixed order and rounded once.  dx, dweight, dbias:
+ * written where given.  Without dweight and dbias the workspace may be NULL;
+ * with rows = 0 they are zero and every row tensor may be NULL. */
+sparc_status sparc_layer_norm_backward(int64_t rows, int64_t cols, int32_t io_dtype, int32_t param_dtype,
+                                       const void* x, const void* weight, const float* mean, const float* rstd,
+                                       const void* dy, void* dx, void* dweight, void* dbias, void* workspace,
+                                       size_t workspace_bytes, sparc_stream_t stream);
+
+/* ---- Embedding -------------------------------------------------------------
+ * tokens [n] of id_bytes 4 or 8 (int32, int64); weight [vocab, dim] and y [n,
+ * dim] in io_dtype: y[i] = scale weight[tokens[i]], rounded once.  An id
+ * outside [0, vocab) gives a row of NaN.  No counterpart in the reference,
+ * which ships the layer, not a network (the same holds for the gradient
+ * clipping and the beam step below). */
+sparc_status sparc_embedding_forward(int64_t n, int64_t vocab, int64_t dim, int32_t io_dtype, int32_t id_bytes,
+                                     const void* tokens, const void* weight, float scale, void* y,
+                                     sparc_stream_t stream);
+
+/* Workspace bytes of sparc_embedding_backward (0: invalid shape). */
+size_t sparc_embedding_workspace_bytes(int64_t n, int64_t vocab, int64_t dim);
+
+/* dweight [vocab, dim] (io_dtype, every row written) = scale times the sum of
+ * dy[i] over the i with tokens[i] = v, in fp32, rounded once; the tokens are
+ * sorted and the sums have a fixed order, so equal calls give equal bits.
+ * Positions of padding_id (-1: none) and of ids outside [0, vocab) take no
+ * part.  workspace: 16-byte aligned. */
+sparc_status sparc_embedding_backward(int64_t n, int64_t vocab, int64_t dim, int32_t io_dtype, int32_t id_bytes,
+                                      const void* tokens, int64_t padding_id, const void* dy, float scale,
+                                      void* dweight, void* workspace, size_t workspace_bytes, sparc_stream_t stream);
+
+/* ---- Gradient norm and clipping ---------------------------------------------
+ * count tensors (host arrays, read during the call): tensors[i] points to
+ * sizes[i] values of dtypes[i] (sparc_dtype) on the device.  norm [1] fp32 = the
+ * L2 norm over all values, accumulated in fp64 in a fixed order (0 without
+ * values).  sparc_clip_grad_norm then multiplies every value by max_norm /
+ * (norm + 1e-6) where that is below 1 (or NaN), and writes nothing otherwise. */
+size_t sparc_grad_norm_workspace_bytes(int64_t count);
+sparc_status sparc_grad_norm(int64_t count, void* const* tensors, const int64_t* sizes, const int32_t* dtypes,
+                             float* norm, void* workspace, size_t workspace_bytes, sparc_stream_t stream);
+sparc_status sparc_clip_grad_norm(int64_t count, void* const* tensors, const int64_t* sizes, const int32_t* dtypes,
+                                  float max_norm, float* norm, void* workspace, size_t workspace_bytes,
+                                  sparc_stream_t stream);
+
+/* ---- Beam search -------------------------------------------------------------
+ * One step over batch rows of ``beams`` (1 to 32) hypotheses.  logits: batch *
+ * beams rows of vocab values (io_dtype), row_stride values apart; scores
+ * [batch, beams] fp32 log-probabilities, -inf for an empty beam; finished
+ * [batch, beams] bytes or NULL.  The candidates of a beam are score + (x -
+ * lse), lse the row's log-sum-exp, in fp32; a finished beam has (eos_id, score)
+ * and -inf for every other token.  The best ``beams`` of a batch row's beams *
+ * vocab candidates, in descending order and ties to the lowest beam * vocab +
+ * token, give tokens, parents (int64) and new_scores; new_finished (or NULL) is
+ * the parent's flag or token == eos_id.  eos_id -1: beams do not finish.  A
+ * beam whose logits are all -inf has -inf candidates; a NaN or +inf logit makes
+ * all its candidates NaN, which rank above every number.  beams * vocab below
+ * 2^31. */
+size_t sparc_beam_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab);
+sparc_status sparc_beam_step(int64_t batch, int64_t beams, int64_t vocab, int64_t row_stride, int32_t io_dtype,
+                             const void* logits, const float* scores, const uint8_t* finished, int64_t eos_id,
+                             int64_t* tokens, int64_t* parents, float* new_scores, uint8_t* new_finished,
+                             void* workspace, size_t workspace_bytes, sparc_stream_t stream);
+
+/* count planes (host arrays, read during the call) of batch * beams contiguous
+ * rows of row_bytes[i] bytes (an even number): dst row b * beams + k = src row b
+ * * beams + parents[b, k] (device, int64).  dst[i] is src[i] (in place) or does
+ * not overlap any plane of the call.  A parent outside [0, beams) fills its rows
+ * with one bits (NaN). */
+sparc_status sparc_reorder_states(int64_t batch, int64_t beams, int64_t count, const void* const* src,
+                                  void* const* dst, const int64_t* row_bytes, const int64_t* parents,
+                                  sparc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -61,6 +61,18 @@ EXPORTED_SYMBOLS = (
     "sparc_rms_norm_forward",
     "sparc_rms_norm_workspace_bytes",
     "sparc_rms_norm_backward",
+    "sparc_layer_norm_forward",
+    "sparc_layer_norm_workspace_bytes",
+    "sparc_layer_norm_backward",
+    "sparc_embedding_forward",
+    "sparc_embedding_workspace_bytes",
+    "sparc_embedding_backward",
+    "sparc_grad_norm_workspace_bytes",
+    "sparc_grad_norm",
+    "sparc_clip_grad_norm",
+    "sparc_beam_workspace_bytes",
+    "sparc_beam_step",
+    "sparc_reorder_states",
     "sparc_last_error",
     "sparc_version",
 )
@@ -85,6 +97,7 @@ _lib = None
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int32
+_F32 = ctypes.c_float
 _SZ = ctypes.c_size_t
 
 
@@ -172,6 +185,30 @@ def load() -> ctypes.CDLL:
         lib.sparc_rms_norm_workspace_bytes.restype = _SZ
         lib.sparc_rms_norm_backward.argtypes = [_I64, _I64, _I32] + [_P] * 7 + [_SZ, _P]
         lib.sparc_rms_norm_backward.restype = ctypes.c_int
+        lib.sparc_layer_norm_forward.argtypes = [_I64, _I64, _I32, _I32, _P, _P, _P, _F32, _P, _P, _P, _P]
+        lib.sparc_layer_norm_forward.restype = ctypes.c_int
+        lib.sparc_layer_norm_workspace_bytes.argtypes = [_I64, _I64]
+        lib.sparc_layer_norm_workspace_bytes.restype = _SZ
+        lib.sparc_layer_norm_backward.argtypes = [_I64, _I64, _I32, _I32] + [_P] * 9 + [_SZ, _P]
+        lib.sparc_layer_norm_backward.restype = ctypes.c_int
+        lib.sparc_embedding_forward.argtypes = [_I64, _I64, _I64, _I32, _I32, _P, _P, _F32, _P, _P]
+        lib.sparc_embedding_forward.restype = ctypes.c_int
+        lib.sparc_embedding_workspace_bytes.argtypes = [_I64, _I64, _I64]
+        lib.sparc_embedding_workspace_bytes.restype = _SZ
+        lib.sparc_embedding_backward.argtypes = [_I64, _I64, _I64, _I32, _I32, _P, _I64, _P, _F32, _P, _P, _SZ, _P]
+        lib.sparc_embedding_backward.restype = ctypes.c_int
+        lib.sparc_grad_norm_workspace_bytes.argtypes = [_I64]
+        lib.sparc_grad_norm_workspace_bytes.restype = _SZ
+        lib.sparc_grad_norm.argtypes = [_I64, _P, _P, _P, _P, _P, _SZ, _P]
+        lib.sparc_grad_norm.restype = ctypes.c_int
+        lib.sparc_clip_grad_norm.argtypes = [_I64, _P, _P, _P, _F32, _P, _P, _SZ, _P]
+        lib.sparc_clip_grad_norm.restype = ctypes.c_int
+        lib.sparc_beam_workspace_bytes.argtypes = [_I64, _I64, _I64]
+        lib.sparc_beam_workspace_bytes.restype = _SZ
+        lib.sparc_beam_step.argtypes = [_I64, _I64, _I64, _I64, _I32, _P, _P, _P, _I64] + [_P] * 5 + [_SZ, _P]
+        lib.sparc_beam_step.restype = ctypes.c_int
+        lib.sparc_reorder_states.argtypes = [_I64, _I64, _I64, _P, _P, _P, _P, _P]
+        lib.sparc_reorder_states.restype = ctypes.c_int
         lib.sparc_last_error.argtypes = []
         lib.sparc_last_error.restype = ctypes.c_char_p
         lib.sparc_version.argtypes = []

@@ -1,0 +1,520 @@
+// Embedding lookup with scaling, and the table's gradient by sorted tokens.
+//
+//   forward   y[n] = scale W[t_n]
+//   backward  dW[v] = scale sum over n with t_n = v of dy[n], for every row v
+//
+// Rows in the I/O type, sums in fp32 rounded once.  An id outside [0, vocab)
+// gives a row of NaN and takes no part in the gradient; the padding row gets a
+// gradient of zero.
+//
+// The backward sorts the token positions by id (a stable radix sort of
+// 32-bit keys, digits of up to 9 bits: two passes up to 2^18 ids), so that the
+// positions of one id stand together in their order in the batch.  Pieces of
+// kPiece sorted positions are then summed side by side, whatever the ids'
+// frequencies: a run of equal ids inside a piece is written to its row at
+// once; a run that crosses pieces leaves one fp32 partial row per piece,
+// joined in order by a second kernel.  Every sum has a fixed order, so dW does
+// not depend on timing, and every row of dW is written exactly once: rows
+// without tokens are cleared by further workgroups of the summing kernel.
+
+#include "common.h"
+#include "sparc_hip.h"
+
+namespace sparc {
+namespace {
+
+constexpr int kPiece = 16;          // sorted positions per piece
+constexpr int kSortThreads = 256;   // 4 waves per sort tile
+constexpr int kSortWaves = kSortThreads / 64;
+constexpr int kMaxDigits = 512;     // 9 bits
+constexpr int kJoinWaves = 16;
+constexpr uint32_t kNone = 0xffffffffu;
+
+// Scaled copies of table rows.  A group of lpr lanes (a power of two up to 64)
+// takes one block of lpr * V columns of one token.
+template <typename IO, int V>
+__global__ void __launch_bounds__(256)
+embed_fwd_kernel(int64_t N, int64_t vocab, int D, int lpr, int blocks, const void* tokens, int wide_ids, const void* w,
+                 float scale, void* y) {
+  const int gl = threadIdx.x & (lpr - 1);
+  const int64_t per = 256 / lpr;
+  const int64_t jobs = N * blocks;
+  for (int64_t job = blockIdx.x * per + threadIdx.x / lpr; job < jobs; job += gridDim.x * per) {
+    const int64_t n = blocks == 1 ? job : job / blocks;
+    const int c = (static_cast<int>(job - n * blocks) * lpr + gl) * V;
+    if (c >= D) continue;
+    const int64_t id = wide_ids ? static_cast<const int64_t*>(tokens)[n] : static_cast<const int32_t*>(tokens)[n];
+    float v[V];
+    if (id >= 0 && id < vocab) {
+      unpack<IO, V>(load_raw<IO, V>(w, id * D + c), v);
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] *= scale;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = __uint_as_float(0x7fc00000u);
+    }
+    store_raw<IO, V>(y, n * D + c, pack<IO, V>(v));
+  }
+}
+
+// ---------------------------------------------------------------------------
+// the sort
+// ---------------------------------------------------------------------------
+// The key of a position: its id, or vocab (behind every row) where it takes no
+// part in the gradient.
+__device__ __forceinline__ uint32_t token_key(const void* tokens, int wide_ids, int64_t n, int64_t vocab, int64_t pad) {
+  const int64_t id = wide_ids ? static_cast<const int64_t*>(tokens)[n] : static_cast<const int32_t*>(tokens)[n];
+  return static_cast<uint32_t>(id >= 0 && id < vocab && id != pad ? id : vocab);
+}
+
+struct SortPass {
+  const void* tokens;     // the first pass reads ids, later ones keys
+  int wide_ids;
+  int64_t vocab, pad;
+  const uint32_t* keys_in;
+  const uint32_t* pos_in;
+  uint32_t* keys_out;
+  uint32_t* pos_out;
+  uint32_t* counts;       // [tiles][digits] of this pass
+  uint8_t* touched;       // [vocab]: cleared by the first count, set by the last scatter
+  int64_t n;
+  int shift, bits;
+  int first, last;
+};
+
+// Digit counts of each tile of kSortThreads * ITEMS positions
+template <int ITEMS>
+__global__ void __launch_bounds__(kSortThreads)
+sort_count_kernel(SortPass p) {
+  __shared__ uint32_t hist[kMaxDigits];
+  const int digits = 1 << p.bits;
+  for (int d = threadIdx.x; d < digits; d += kSortThreads) hist[d] = 0;
+  if (p.first) {
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kSortThreads;
+    for (int64_t v = static_cast<int64_t>(blockIdx.x) * kSortThreads + threadIdx.x; v < p.vocab; v += step)
+      p.touched[v] = 0;
+  }
+  __syncthreads();
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * (kSortThreads * ITEMS);
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int64_t n = base + i * kSortThreads + threadIdx.x;
+    if (n < p.n) {
+      const uint32_t key = p.first ? token_key(p.tokens, p.wide_ids, n, p.vocab, p.pad) : p.keys_in[n];
+      atomicAdd(&hist[(key >> p.shift) & (digits - 1)], 1u);
+    }
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < digits; d += kSortThreads) p.counts[static_cast<int64_t>(blockIdx.x) * digits + d] = hist[d];
+}
+
+// Moves each tile's positions behind all positions of smaller digits and those
+// of its own digit in earlier tiles.  A wave ranks its 64 * ITEMS consecutive
+// positions 64 at a time: the lanes of equal digit are found by one ballot per
+// digit bit, and a counter per wave and digit in LDS carries the rank on.
+template <int ITEMS>
+__global__ void __launch_bounds__(kSortThreads)
+sort_scatter_kernel(SortPass p) {
+  __shared__ uint32_t cnt[kSortWaves][kMaxDigits];  // counts, then the waves' first places
+  __shared__ uint32_t start[kMaxDigits];            // this tile's first place of each digit
+  __shared__ uint32_t wsum[kSortWaves];
+  const int digits = 1 << p.bits;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int d = threadIdx.x; d < digits; d += kSortThreads) {
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) cnt[w][d] = 0;
+  }
+  // a thread's digits: 2 t and 2 t + 1, so that a scan over threads is one over digits
+  uint32_t before[2] = {0, 0}, total[2] = {0, 0};
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int d = 2 * threadIdx.x + k;
+    if (d < digits) {
+      for (int tile = 0; tile < static_cast<int>(gridDim.x); ++tile) {
+        const uint32_t c = p.counts[static_cast<int64_t>(tile) * digits + d];
+        if (tile < static_cast<int>(blockIdx.x)) before[k] += c;
+        total[k] += c;
+      }
+    }
+  }
+  uint32_t sum = total[0] + total[1];
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t up = __shfl_up(sum, o);
+    if (lane >= o) sum += up;
+  }
+  if (lane == 63) wsum[wave] = sum;
+  __syncthreads();
+  uint32_t base = sum - total[0] - total[1];
+  for (int w = 0; w < wave; ++w) base += wsum[w];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int d = 2 * threadIdx.x + k;
+    if (d < digits) start[d] = base + before[k];
+    base += total[k];
+  }
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kSortThreads * ITEMS) + wave * (64 * ITEMS) + lane;
+  uint32_t key[ITEMS], rank[ITEMS];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int64_t n = first + i * 64;
+    key[i] = n < p.n ? (p.first ? token_key(p.tokens, p.wide_ids, n, p.vocab, p.pad) : p.keys_in[n]) : 0u;
+  }
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const bool valid = first + i * 64 < p.n;
+    const uint32_t d = (key[i] >> p.shift) & (digits - 1);
+    uint64_t same = __ballot(valid);
+    for (int b = 0; b < p.bits; ++b) {
+      const uint64_t one = __ballot((d >> b) & 1u);
+      same &= (d >> b) & 1u ? one : ~one;
+    }
+    const uint32_t below = __popcll(same & ((uint64_t(1) << lane) - 1));
+    const uint32_t old = cnt[wave][d];
+    rank[i] = old + below;
+    wave_lds_fence();
+    if (valid && below == 0) cnt[wave][d] = old + __popcll(same);
+    wave_lds_fence();
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < digits; d += kSortThreads) {
+    uint32_t at = start[d];
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) {
+      const uint32_t c = cnt[w][d];
+      cnt[w][d] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int64_t n = first + i * 64;
+    if (n < p.n) {
+      const uint32_t to = cnt[wave][(key[i] >> p.shift) & (digits - 1)] + rank[i];
+      p.keys_out[to] = key[i];
+      p.pos_out[to] = p.first ? static_cast<uint32_t>(n) : p.pos_in[n];
+      if (p.last && key[i] < static_cast<uint32_t>(p.vocab)) p.touched[key[i]] = 1;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// the sums
+// ---------------------------------------------------------------------------
+template <typename IO, int V>
+__device__ __forceinline__ void write_row(void* dw, int64_t index, const float (&acc)[V], float scale) {
+  float o[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) o[i] = acc[i] * scale;
+  store_raw<IO, V>(dw, index, pack<IO, V>(o));
+}
+
+// Workgroups below sum_groups: pieces of sorted positions, a group of lpr lanes
+// per piece and block of lpr * V columns.  part: [pieces][2][D] fp32, the
+// partial sums of a run that goes on from the piece before (0) and of one that
+// begins here and goes on into the next (1).  The others clear rows of dW that
+// no token names.
+template <typename IO, int V>
+__global__ void __launch_bounds__(256)
+embed_sum_kernel(int64_t N, int64_t vocab, int D, int lpr, int blocks, int64_t sum_groups, const uint32_t* keys,
+                 const uint32_t* pos, const uint8_t* touched, const void* dy, float scale, float* part, void* dw) {
+  const int gl = threadIdx.x & (lpr - 1);
+  const int64_t per = 256 / lpr;
+  if (blockIdx.x >= sum_groups) {
+    const int64_t jobs = vocab * blocks, step = (gridDim.x - sum_groups) * per;
+    for (int64_t job = (blockIdx.x - sum_groups) * per + threadIdx.x / lpr; job < jobs; job += step) {
+      const int64_t v = blocks == 1 ? job : job / blocks;
+      const int c = (static_cast<int>(job - v * blocks) * lpr + gl) * V;
+      if (c < D && !touched[v]) {
+        float z[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) z[i] = 0.0f;
+        store_raw<IO, V>(dw, v * D + c, pack<IO, V>(z));
+      }
+    }
+    return;
+  }
+  const int64_t pieces = (N + kPiece - 1) / kPiece, jobs = pieces * blocks;
+  for (int64_t job = blockIdx.x * per + threadIdx.x / lpr; job < jobs; job += sum_groups * per) {
+    const int64_t piece = blocks == 1 ? job : job / blocks;
+    const int c = (static_cast<int>(job - piece * blocks) * lpr + gl) * V;
+    if (c >= D) continue;
+    const int64_t p0 = piece * kPiece;
+    const int n = N - p0 < kPiece ? static_cast<int>(N - p0) : kPiece;
+    uint32_t key[kPiece];
+    typename Raw<IO, V>::T raw[kPiece];
+#pragma unroll
+    for (int i = 0; i < kPiece; ++i) key[i] = i < n ? keys[p0 + i] : kNone;
+    const uint32_t prev = p0 > 0 ? keys[p0 - 1] : kNone;
+    const uint32_t next = p0 + n < N ? keys[p0 + n] : kNone;
+#pragma unroll
+    for (int i = 0; i < kPiece; ++i) {
+      if (key[i] < static_cast<uint32_t>(vocab)) raw[i] = load_raw<IO, V>(dy, static_cast<int64_t>(pos[p0 + i]) * D + c);
+    }
+    float acc[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = 0.0f;
+    bool head = prev == key[0];  // the run in hand goes on from the piece before
+#pragma unroll
+    for (int i = 0; i < kPiece; ++i) {
+      if (key[i] < static_cast<uint32_t>(vocab)) {  // what follows is vocab or kNone only
+        float v[V];
+        unpack<IO, V>(raw[i], v);
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] += v[k];
+        const uint32_t after = i + 1 < kPiece && i + 1 < n ? key[i + 1 < kPiece ? i + 1 : i] : next;
+        const bool end = i + 1 == n;
+        if (end || after != key[i]) {
+          if (head || after == key[i]) {
+            float* to = part + ((piece * 2 + (head ? 0 : 1)) * D + c);
+#pragma unroll
+            for (int k = 0; k < V; ++k) to[k] = acc[k];
+          } else {
+            write_row<IO, V>(dw, static_cast<int64_t>(key[i]) * D + c, acc, scale);
+          }
+          head = false;
+#pragma unroll
+          for (int k = 0; k < V; ++k) acc[k] = 0.0f;
+        }
+      }
+    }
+  }
+}
+
+// Joins the runs that begin in piece blockIdx.x and go on behind it: the first
+// piece's partial sum, then the later ones' in order, kJoinWaves slices of them
+// side by side.  blockIdx.y: a block of 64 columns.
+template <typename IO>
+__global__ void __launch_bounds__(64 * kJoinWaves)
+embed_join_kernel(int64_t N, int64_t vocab, int D, const uint32_t* keys, float scale, const float* part, void* dw) {
+  __shared__ float red[kJoinWaves][64];
+  const int64_t pieces = (N + kPiece - 1) / kPiece;
+  for (int64_t piece = blockIdx.x; piece + 1 < pieces; piece += gridDim.x) {
+    const int64_t p0 = piece * kPiece, p1 = p0 + kPiece;
+    const uint32_t key = keys[p1 - 1];
+    if (key >= static_cast<uint32_t>(vocab) || keys[p1] != key) continue;          // nothing crosses
+    if (p0 > 0 && keys[p0] == key && keys[p0 - 1] == key) continue;                // it began earlier
+    // the run's end: the first position behind p1 with a larger key
+    int64_t lo = p1, hi = N;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) / 2;
+      if (keys[mid] <= key) lo = mid + 1; else hi = mid;
+    }
+    const int64_t last = (lo - 1) / kPiece, count = last - piece;  // pieces behind this one
+    const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
+    const int64_t each = (count + kJoinWaves - 1) / kJoinWaves;
+    const int64_t a = piece + 1 + slice * each, b = a + each < last + 1 ? a + each : last + 1;
+    for (int c0 = blockIdx.y * 64; c0 < D; c0 += gridDim.y * 64) {
+      const int c = c0 + lane;
+      float s = 0.0f;
+      if (c < D) {
+        if (slice == 0) s = part[(piece * 2 + 1) * D + c];
+        float u[8];
+        int64_t q = a;
+        for (; q + 8 <= b; q += 8) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) u[k] = part[(q + k) * 2 * D + c];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) s += u[k];
+        }
+        for (; q < b; ++q) s += part[q * 2 * D + c];
+      }
+      red[slice][lane] = s;
+      __syncthreads();
+      if (slice == 0 && c < D) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kJoinWaves; ++k) sum += red[k][lane];
+        store1<IO>(dw, static_cast<int64_t>(key) * D + c, sum * scale);
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+sparc_status em_fail(sparc_status s, const char* msg) {
+  snprintf(error_buffer(), 512, "%s", msg);
+  return s;
+}
+sparc_status em_launched(const char* what) {
+  const hipError_t e = hipGetLastError();
+  if (e == hipSuccess) return SPARC_OK;
+  snprintf(error_buffer(), 512, "%s: %s", what, hipGetErrorString(e));
+  return SPARC_EHIP;
+}
+
+sparc_status em_check(int64_t n, int64_t vocab, int64_t dim, int32_t io, int32_t id_bytes) {
+  if (n < 0 || vocab <= 0 || dim <= 0) return em_fail(SPARC_EINVAL, "embedding: n >= 0, vocab > 0 and dim > 0 required");
+  if (io != SPARC_F32 && io != SPARC_BF16) return em_fail(SPARC_EINVAL, "embedding: unknown io_dtype");
+  if (id_bytes != 4 && id_bytes != 8) return em_fail(SPARC_EINVAL, "embedding: ids are 32- or 64-bit integers");
+  if (n > (int64_t(1) << 30) || vocab > (int64_t(1) << 30) || dim > (int64_t(1) << 24) ||
+      n > (int64_t(1) << 46) / dim || vocab > (int64_t(1) << 46) / dim)
+    return em_fail(SPARC_EINVAL, "embedding: too large");
+  return SPARC_OK;
+}
+
+struct Sort {
+  int bits, passes, digit_bits, items;
+  int64_t tiles;
+};
+Sort sort_of(int64_t n, int64_t vocab) {
+  Sort s;
+  s.bits = 1;
+  while ((vocab >> s.bits) > 0) ++s.bits;  // keys 0 .. vocab
+  s.passes = (s.bits + 8) / 9;
+  s.digit_bits = (s.bits + s.passes - 1) / s.passes;
+  s.items = n <= 65536 ? 8 : 32;  // at most 32 tiles' counts to add up, then tiles four times the size
+  s.tiles = (n + kSortThreads * s.items - 1) / (kSortThreads * s.items);
+  if (s.tiles < 1) s.tiles = 1;  // without tokens, one tile clears the flags
+  return s;
+}
+size_t up256(size_t b) { return (b + 255) / 256 * 256; }
+
+// lanes per row and column blocks per row
+void em_groups(int64_t dim, int v, int& lpr, int& blocks) {
+  const int64_t vecs = (dim + v - 1) / v;
+  lpr = 1;
+  while (lpr < 64 && lpr < vecs) lpr <<= 1;
+  blocks = static_cast<int>((vecs + lpr - 1) / lpr);
+}
+unsigned em_grid(int64_t jobs, int lpr) {
+  const int64_t g = (jobs * lpr + 255) / 256;
+  return static_cast<unsigned>(g < 1 ? 1 : (g < (1 << 20) ? g : (1 << 20)));
+}
+int em_vec(int64_t dim, size_t es, const void* a, const void* b) {
+  for (int v = static_cast<int>(16 / es); v > 1; v /= 2)
+    if (dim % v == 0 && reinterpret_cast<uintptr_t>(a) % (v * es) == 0 && reinterpret_cast<uintptr_t>(b) % (v * es) == 0)
+      return v;
+  return 1;
+}
+template <int N> using Int = std::integral_constant<int, N>;
+template <typename IO, typename F>
+void em_dispatch(int v, F&& f) {
+  if constexpr (sizeof(IO) == 2) {
+    if (v == 8) return f(Int<8>{});
+  }
+  if (v == 4) return f(Int<4>{});
+  if (v == 2) return f(Int<2>{});
+  f(Int<1>{});
+}
+
+template <typename IO>
+void em_forward(hipStream_t st, int64_t n, int64_t vocab, int64_t dim, const void* tokens, int id_bytes, const void* w,
+                float scale, void* y) {
+  em_dispatch<IO>(em_vec(dim, sizeof(IO), w, y), [&](auto V) {
+    int lpr, blocks;
+    em_groups(dim, V(), lpr, blocks);
+    hipLaunchKernelGGL((embed_fwd_kernel<IO, V()>), dim3(em_grid(n * blocks, lpr)), dim3(256), 0, st, n, vocab,
+                       static_cast<int>(dim), lpr, blocks, tokens, id_bytes == 8, w, scale, y);
+  });
+}
+
+template <int ITEMS>
+void em_sort_pass(hipStream_t st, int64_t tiles, const SortPass& p) {
+  hipLaunchKernelGGL((sort_count_kernel<ITEMS>), dim3(static_cast<unsigned>(tiles)), dim3(kSortThreads), 0, st, p);
+  hipLaunchKernelGGL((sort_scatter_kernel<ITEMS>), dim3(static_cast<unsigned>(tiles)), dim3(kSortThreads), 0, st, p);
+}
+
+template <typename IO>
+void em_sums(hipStream_t st, int64_t n, int64_t vocab, int64_t dim, const uint32_t* keys, const uint32_t* pos,
+             const uint8_t* touched, const void* dy, float scale, float* part, void* dw) {
+  const int64_t pieces = (n + kPiece - 1) / kPiece;
+  em_dispatch<IO>(em_vec(dim, sizeof(IO), dy, dw), [&](auto V) {
+    int lpr, blocks;
+    em_groups(dim, V(), lpr, blocks);
+    const unsigned sum_groups = em_grid(pieces * blocks, lpr);
+    const unsigned clear = em_grid(vocab * blocks, lpr), most = 4096;
+    hipLaunchKernelGGL((embed_sum_kernel<IO, V()>), dim3(sum_groups + (clear < most ? clear : most)), dim3(256), 0, st,
+                       n, vocab, static_cast<int>(dim), lpr, blocks, static_cast<int64_t>(sum_groups), keys, pos,
+                       touched, dy, scale, part, dw);
+  });
+  if (pieces > 1) {
+    const int64_t blocks = (dim + 63) / 64;
+    const dim3 grid(static_cast<unsigned>(pieces < (1 << 18) ? pieces : (1 << 18)),
+                    static_cast<unsigned>(blocks < 64 ? blocks : 64));
+    hipLaunchKernelGGL((embed_join_kernel<IO>), grid, dim3(64 * kJoinWaves), 0, st, n, vocab, static_cast<int>(dim),
+                       keys, scale, part, dw);
+  }
+}
+
+}  // namespace
+}  // namespace sparc
+
+// ===========================================================================
+// C ABI
+// ===========================================================================
+extern "C" {
+
+sparc_status sparc_embedding_forward(int64_t n, int64_t vocab, int64_t dim, int32_t io_dtype, int32_t id_bytes,
+                                     const void* tokens, const void* weight, float scale, void* y,
+                                     sparc_stream_t stream) {
+  using namespace sparc;
+  if (sparc_status s = em_check(n, vocab, dim, io_dtype, id_bytes)) return s;
+  if (n == 0) return SPARC_OK;
+  if (!tokens || !weight || !y) return em_fail(SPARC_EINVAL, "embedding forward: NULL pointer");
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (io_dtype == SPARC_F32) em_forward<float>(st, n, vocab, dim, tokens, id_bytes, weight, scale, y);
+  else em_forward<sparc::bf16>(st, n, vocab, dim, tokens, id_bytes, weight, scale, y);
+  return em_launched("embedding forward");
+}
+
+size_t sparc_embedding_workspace_bytes(int64_t n, int64_t vocab, int64_t dim) {
+  using namespace sparc;
+  if (em_check(n, vocab, dim, SPARC_F32, 8)) return 0;
+  const Sort s = sort_of(n, vocab);
+  const int64_t pieces = (n + kPiece - 1) / kPiece;
+  return 4 * up256(n * sizeof(uint32_t)) + up256(s.tiles * (size_t(1) << s.digit_bits) * sizeof(uint32_t)) +
+         up256(vocab) + up256(static_cast<size_t>(pieces) * 2 * dim * sizeof(float)) + 256;
+}
+
+sparc_status sparc_embedding_backward(int64_t n, int64_t vocab, int64_t dim, int32_t io_dtype, int32_t id_bytes,
+                                      const void* tokens, int64_t padding_id, const void* dy, float scale,
+                                      void* dweight, void* workspace, size_t workspace_bytes, sparc_stream_t stream) {
+  using namespace sparc;
+  if (sparc_status s = em_check(n, vocab, dim, io_dtype, id_bytes)) return s;
+  if (!dweight || (n > 0 && (!tokens || !dy))) return em_fail(SPARC_EINVAL, "embedding backward: NULL pointer");
+  if (!workspace || workspace_bytes < sparc_embedding_workspace_bytes(n, vocab, dim))
+    return em_fail(SPARC_EWORKSPACE, "embedding backward: workspace missing or too small");
+  if (reinterpret_cast<uintptr_t>(workspace) % 16)
+    return em_fail(SPARC_EINVAL, "embedding backward: the workspace must be 16-byte aligned");
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const Sort s = sort_of(n, vocab);
+  char* at = static_cast<char*>(workspace);
+  auto take = [&](size_t bytes) { char* p = at; at += up256(bytes); return p; };
+  uint32_t* keys[2] = {reinterpret_cast<uint32_t*>(take(n * 4)), reinterpret_cast<uint32_t*>(take(n * 4))};
+  uint32_t* pos[2] = {reinterpret_cast<uint32_t*>(take(n * 4)), reinterpret_cast<uint32_t*>(take(n * 4))};
+  uint32_t* counts = reinterpret_cast<uint32_t*>(take(s.tiles * (size_t(1) << s.digit_bits) * 4));
+  uint8_t* touched = reinterpret_cast<uint8_t*>(take(vocab));
+  float* part = reinterpret_cast<float*>(at);
+  int cur = 0;
+  for (int k = 0; k < s.passes; ++k) {
+    SortPass p{};
+    p.tokens = tokens;
+    p.wide_ids = id_bytes == 8;
+    p.vocab = vocab;
+    p.pad = padding_id;
+    p.keys_in = keys[cur ^ 1];
+    p.pos_in = pos[cur ^ 1];
+    p.keys_out = keys[cur];
+    p.pos_out = pos[cur];
+    p.counts = counts;
+    p.touched = touched;
+    p.n = n;
+    p.shift = k * s.digit_bits;
+    p.bits = s.digit_bits;
+    p.first = k == 0;
+    p.last = k == s.passes - 1;
+    if (s.items == 8) em_sort_pass<8>(st, s.tiles, p);
+    else em_sort_pass<32>(st, s.tiles, p);
+    cur ^= 1;
+  }
+  if (io_dtype == SPARC_F32) em_sums<float>(st, n, vocab, dim, keys[cur ^ 1], pos[cur ^ 1], touched, dy, scale, part, dweight);
+  else em_sums<sparc::bf16>(st, n, vocab, dim, keys[cur ^ 1], pos[cur ^ 1], touched, dy, scale, part, dweight);
+  return em_launched("embedding backward");
+}
+
+}  // extern "C"

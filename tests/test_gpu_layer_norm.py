@@ -1,0 +1,167 @@
+"""layer_norm on the GPU against float64: outputs and gradients over widths of
+every form (lanes of 1 to 16 bytes, one to sixteen waves per row, rows read
+again), types, strides and alignments.
+
+Tolerances, from the arithmetic: fp32 sums over a row of D values in registers
+and across lanes add at most some 32 + log2(D) roundings of 2^-24, and a fixed
+number of further operations follows, so fp32 results are held to 2^-17 of the
+largest; bf16 results are one rounding (2^-8) of such a value.  Sums over R rows
+add sqrt(R) such terms in partial sums."""
+import pytest
+import torch
+
+import sparc_amd
+from oracle import lm_oracle as L
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def _case(rows, D, dtype, pdtype, seed, mean=0.4):
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(rows, D, generator=g) * 1.7 + mean).to(dtype)
+    w = (1.0 + 0.3 * torch.randn(D, generator=g)).to(pdtype)
+    b = (0.2 * torch.randn(D, generator=g)).to(pdtype)
+    dy = torch.randn(rows, D, generator=g).to(dtype)
+    return x, w, b, dy
+
+
+def _close(got, want, what, scale=1.0):
+    """Within 2^-17 of the largest value, and one rounding of bf16 results."""
+    assert got.shape == want.shape, what
+    want = want.double()
+    off = (got.detach().cpu().double() - want).abs()
+    bound = scale * 2.0 ** -17 * want.abs().max().clamp_min(1e-30)
+    if got.dtype == BF16:
+        bound = bound + want.abs() * 2.0 ** -8
+    worst = (off - bound).max().item()
+    assert worst <= 0.0, f"{what}: {worst:.3g} over the bound, largest {want.abs().max():.3g}"
+
+
+def _check(rows, D, dtype, pdtype, weight=True, bias=True, seed=0):
+    x, w, b, dy = _case(rows, D, dtype, pdtype, seed)
+    w, b = w if weight else None, b if bias else None
+    leaves = [t.cuda().requires_grad_() for t in (x, w, b) if t is not None]
+    at = iter(leaves)
+    args = [next(at) if t is not None else None for t in (x, w, b)]
+    y = sparc_amd.layer_norm(*args, eps=1e-5)
+    grads = torch.autograd.grad(y, leaves, dy.cuda())
+    _close(y, L.layer_norm(x, w, b, 1e-5), "y")
+    dx, dw, db = L.layer_norm_grads(x, w, 1e-5, dy)
+    want = [dx] + ([dw] if weight else []) + ([db] if bias else [])
+    for got, ref, name in zip(grads, want, ("dx", "first parameter", "second parameter")):
+        _close(got, ref, name, scale=1.0 if name == "dx" else 4.0)
+    with torch.no_grad():  # the form without saved statistics: the same values
+        assert torch.equal(sparc_amd.layer_norm(*[None if a is None else a.detach() for a in args]), y)
+
+
+@pytest.mark.parametrize("dtype,pdtype", [(F32, F32), (BF16, BF16), (BF16, F32)], ids=["f32", "bf16", "bf16_f32"])
+@pytest.mark.parametrize("D", [1, 2, 7, 64, 200, 513, 768, 1001, 1024, 1536, 2050, 4096, 5000])
+def test_widths(D, dtype, pdtype):
+    print(f"[case] layer norm D={D} {dtype} {pdtype}", flush=True)
+    _check(37, D, dtype, pdtype, seed=D)
+
+
+@pytest.mark.parametrize("D,dtype", [(8193, F32), (16384, F32), (16388, F32), (24576, BF16), (24577, BF16),
+                                     (16386, BF16), (40000, BF16)])
+def test_wide_rows(D, dtype):
+    print(f"[case] layer norm D={D} {dtype}", flush=True)
+    _check(5, D, dtype, F32, seed=D)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 63, 1023, 1024, 4500])
+def test_row_counts(rows):
+    print(f"[case] layer norm rows={rows}", flush=True)
+    _check(rows, 96, BF16, BF16, seed=rows)
+    _check(rows, 97, F32, F32, seed=rows)
+
+
+@pytest.mark.parametrize("weight,bias", [(False, False), (True, False), (False, True)])
+def test_without_parameters(weight, bias):
+    print(f"[case] layer norm weight={weight} bias={bias}", flush=True)
+    _check(19, 264, F32, F32, weight, bias)
+    _check(19, 264, BF16, F32, weight, bias)
+
+
+def test_no_rows():
+    print("[case] layer norm without rows", flush=True)
+    x = torch.zeros(0, 12, device="cuda", requires_grad=True)
+    w, b = torch.ones(12, device="cuda", requires_grad=True), torch.ones(12, device="cuda", requires_grad=True)
+    y = sparc_amd.layer_norm(x, w, b)
+    dx, dw, db = torch.autograd.grad(y.sum(), [x, w, b])
+    assert y.shape == dx.shape == (0, 12) and not dw.any() and not db.any()
+
+
+def test_strides_and_alignment():
+    """A transposed input, an incoming gradient that is an expanded row, and
+    tensors that begin off a 16-byte boundary."""
+    print("[case] layer norm strides", flush=True)
+    x, w, b, dy = _case(40, 96, BF16, BF16, 3)
+    xt = x.t().contiguous().cuda().t()
+    assert not xt.is_contiguous()
+    xt.requires_grad_()
+    wd, bd = (torch.cat((t.new_zeros(1), t)).cuda()[1:].requires_grad_() for t in (w, b))
+    y = sparc_amd.layer_norm(xt, wd, bd)
+    row = dy[:1].cuda().expand(40, 96)
+    got = torch.autograd.grad(y, [xt, wd, bd], row)
+    _close(y, L.layer_norm(x, w, b, 1e-5), "y")
+    for a, ref, name in zip(got, L.layer_norm_grads(x, w, 1e-5, dy[:1].expand(40, 96)), ("dx", "dw", "db")):
+        _close(a, ref, name, scale=4.0)
+
+
+def test_large_mean_keeps_its_precision():
+    """A mean of 1000 standard deviations: the differences from it, and so the
+    variance, are off by the mean's own rounding (1000 2^-24 of a deviation),
+    not by that of squares."""
+    print("[case] layer norm large mean", flush=True)
+    x, w, b, _ = _case(16, 1000, F32, F32, 4, mean=0.0)
+    x = x + 1700.0
+    y = sparc_amd.layer_norm(x.cuda(), w.cuda(), b.cuda())
+    want = L.layer_norm(x, w, b, 1e-5)
+    assert (y.cpu().double() - want).abs().max() <= 4 * 1000 * 2.0 ** -24 * want.abs().max()
+
+
+def test_constant_rows_and_nan():
+    """A constant row has no variance: y is the bias; NaN stays in its row."""
+    print("[case] layer norm constant rows, NaN", flush=True)
+    x = torch.full((3, 320), 2.5, device="cuda")
+    x[1] = torch.randn(320)
+    x[1, 7] = float("nan")
+    b = torch.randn(320, device="cuda")
+    y = sparc_amd.layer_norm(x, torch.ones(320, device="cuda"), b)
+    assert torch.equal(y[0], b) and torch.equal(y[2], b) and y[1].isnan().all()
+
+
+def test_gradient_against_differences():
+    """<gradient, u> against (L(p + h u) - L(p - h u)) / 2h of the kernel's own
+    forward, L = <dy, y> in fp64.  y is off by up to 2^-20 per value, at random:
+    over sqrt(n) values of |dy| ~ 1 and 1 / 2h = 64 that is 0.01; the formula's
+    third derivative adds h^2 ~ 6e-5 of the gradient."""
+    print("[case] layer norm differences", flush=True)
+    x, w, b, dy = (t.cuda() for t in _case(24, 500, F32, F32, 6))
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    grads = torch.autograd.grad(sparc_amd.layer_norm(*leaves), leaves, dy)
+    g = torch.Generator().manual_seed(1)
+    h = 2.0 ** -7
+    for at, (leaf, grad) in enumerate(zip(leaves, grads)):
+        u = torch.randn(leaf.shape, generator=g).cuda()
+        loss = []
+        for s in (1, -1):
+            args = [t.detach() + s * h * u if i == at else t.detach() for i, t in enumerate(leaves)]
+            loss.append((sparc_amd.layer_norm(*args).double() * dy.double()).sum())
+        diff, want = float(loss[0] - loss[1]) / (2 * h), float((grad.double() * u.double()).sum())
+        assert abs(diff - want) <= 0.01 + 1e-3 * float(grad.norm() * u.norm()) / leaf.numel() ** 0.5 + 1e-3 * abs(want)
+
+
+def test_equal_calls_give_equal_bits_on_any_stream():
+    print("[case] layer norm determinism", flush=True)
+    x, w, b, dy = (t.cuda() for t in _case(3000, 768, BF16, BF16, 8))
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    first = torch.autograd.grad(sparc_amd.layer_norm(*leaves), leaves, dy)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = torch.autograd.grad(sparc_amd.layer_norm(*leaves), leaves, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(p, q) for p, q in zip(first, again))
