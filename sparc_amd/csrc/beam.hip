@@ -21,8 +21,7 @@
 // sorted and merged into the list by bitonic exchanges.  The bound starts at
 // the (K + 1)-th largest of the lanes' first values, so few candidates follow.
 
-#include "common.h"
-#include "sparc_hip.h"
+#include "rows.h"
 
 namespace sparc {
 namespace {
@@ -32,7 +31,15 @@ constexpr int kScanWaves = 4;      // waves (spans) per scan workgroup
 constexpr int kJoinWaves = 8;
 constexpr int kMaxSpans = 64;      // per row: a lane each when they are joined
 constexpr int kMinSpan = 2048;     // logits per span at least
-constexpr int kMaxPlanes = 96;     // state planes per launch: 2.5 KB of kernel arguments
+constexpr int kAhead = 4;          // vectors a lane reads at once
+constexpr int kMaxPlanes = 96;     // state planes per launch: 2.3 KB of kernel arguments
+
+// Values per span: whole rounds of 64 vectors
+template <int VEC>
+__host__ __device__ __forceinline__ int64_t span_values(int64_t V, int spans) {
+  const int64_t round = 64 * VEC, rounds = (V + round - 1) / round;
+  return (rounds + spans - 1) / spans * round;
+}
 
 // ---------------------------------------------------------------------------
 // keys
@@ -54,30 +61,60 @@ __device__ __forceinline__ uint64_t make_key(float x, uint32_t index) {
 __device__ __forceinline__ uint32_t key_index(uint64_t key) { return 0xffffffffu - static_cast<uint32_t>(key); }
 __device__ __forceinline__ float key_value(uint64_t key) { return unordered(static_cast<uint32_t>(key >> 32)); }
 
+// the key of one lane (the same for all) in every lane
 __device__ __forceinline__ uint64_t lane_key(uint64_t key, int lane) {
-  return (static_cast<uint64_t>(__shfl(static_cast<uint32_t>(key >> 32), lane)) << 32) |
-         __shfl(static_cast<uint32_t>(key), lane);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(key >> 32), lane);
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(key), lane);
+  return (static_cast<uint64_t>(hi) << 32) | lo;
 }
-__device__ __forceinline__ uint64_t xor_key(uint64_t key, int mask) {
-  return (static_cast<uint64_t>(__shfl_xor(static_cast<uint32_t>(key >> 32), mask)) << 32) |
-         __shfl_xor(static_cast<uint32_t>(key), mask);
-}
-__device__ __forceinline__ uint64_t exchange(uint64_t key, int mask, bool larger) {
-  const uint64_t other = xor_key(key, mask);
-  return (other > key) == larger ? other : key;
-}
-// the wave's 64 keys in descending (or ascending) order of the lanes
-template <bool DESCENDING>
-__device__ __forceinline__ uint64_t sort_keys(uint64_t key, int lane) {
-#pragma unroll
-  for (int size = 2; size <= 64; size <<= 1) {
-#pragma unroll
-    for (int m = size / 2; m > 0; m >>= 1) {
-      const bool up = (lane & size) == 0 || size == 64;  // this block of ``size`` lanes in the asked order
-      key = exchange(key, m, ((lane & m) == 0) == (up == DESCENDING));
+// Two lanes' words that are M apart: in both of them a and b are the two words,
+// in some order.  DPP and the row swaps only: no trip through LDS.
+template <int M>
+__device__ __forceinline__ void pair_words(uint32_t x, uint32_t& a, uint32_t& b) {
+  if constexpr (M == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    a = r[0];
+    b = r[1];
+  } else if constexpr (M == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    a = r[0];
+    b = r[1];
+  } else {
+    a = x;
+    if constexpr (M == 8) {
+      b = __builtin_amdgcn_update_dpp(0, static_cast<int>(x), kDppRowRor + 8, 0xF, 0xF, true);
+    } else if constexpr (M == 4) {  // banks 1 and 3 read lane - 4, banks 0 and 2 lane + 4
+      const int t = __builtin_amdgcn_update_dpp(0, static_cast<int>(x), kDppRowShr + 4, 0xF, 0xA, false);
+      b = __builtin_amdgcn_update_dpp(t, static_cast<int>(x), kDppRowShl + 4, 0xF, 0x5, false);
+    } else {
+      static_assert(M == 1 || M == 2, "a power of two up to 32");
+      b = __builtin_amdgcn_update_dpp(0, static_cast<int>(x), M == 1 ? kDppXor1 : kDppXor2, 0xF, 0xF, true);
     }
   }
+}
+// the larger or the smaller of the keys of this lane and the one M apart
+template <int M>
+__device__ __forceinline__ uint64_t exchange(uint64_t key, bool larger) {
+  uint32_t ah, al, bh, bl;
+  pair_words<M>(static_cast<uint32_t>(key >> 32), ah, bh);
+  pair_words<M>(static_cast<uint32_t>(key), al, bl);
+  const uint64_t a = (static_cast<uint64_t>(ah) << 32) | al, b = (static_cast<uint64_t>(bh) << 32) | bl;
+  return (b > a) == larger ? b : a;
+}
+// a bitonic sequence of 2 M lanes into order: the larger keys to the lanes
+// whose bit M is 0 where ``down``
+template <int M>
+__device__ __forceinline__ uint64_t merge_keys(uint64_t key, int lane, bool down) {
+  key = exchange<M>(key, ((lane & M) == 0) == down);
+  if constexpr (M > 1) key = merge_keys<M / 2>(key, lane, down);
   return key;
+}
+// the wave's 64 keys in descending (or ascending) order of the lanes
+template <bool DESCENDING, int SIZE = 64>
+__device__ __forceinline__ uint64_t sort_keys(uint64_t key, int lane) {
+  if constexpr (SIZE > 2) key = sort_keys<DESCENDING, SIZE / 2>(key, lane);
+  const bool asked = SIZE == 64 || (lane & SIZE) == 0;  // else this block of lanes the other way round
+  return merge_keys<SIZE / 2>(key, lane, asked == DESCENDING);
 }
 
 // ---------------------------------------------------------------------------
@@ -105,10 +142,7 @@ struct TopList {
   }
   __device__ __forceinline__ void merge(uint64_t cand, int lane) {
     cand = sort_keys<false>(cand, lane);
-    uint64_t k = list > cand ? list : cand;  // the 64 largest of both, bitonic
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) k = exchange(k, m, (lane & m) == 0);
-    list = k;
+    list = merge_keys<32>(list > cand ? list : cand, lane, true);  // the 64 largest of both, bitonic
     const uint64_t b = lane_key(list, want - 1);
     if (b > bound) bound = b;
   }
@@ -142,57 +176,39 @@ struct TopList {
 // ---------------------------------------------------------------------------
 // the scan of the logits
 // ---------------------------------------------------------------------------
-// A row in 16-byte vectors from the last aligned address at or before its
-// start: vector j holds the elements j VEC - shift + i.
+// A row in vectors of 16 bytes, at any alignment of its values
 template <typename IO>
 struct Row {
-  static constexpr int VEC = 16 / sizeof(IO);
-  const void* base;
-  int64_t V;
-  int shift;
-  int64_t vectors;
+  const void* logits;
+  int64_t offset, V;
 
-  __device__ __forceinline__ Row(const void* logits, int64_t offset, int64_t v) {
-    base = static_cast<const IO*>(logits) + offset;
-    V = v;
-    shift = static_cast<int>(reinterpret_cast<uintptr_t>(base) % 16 / sizeof(IO));
-    vectors = (v + shift + VEC - 1) / VEC;
-  }
-  // the elements of vector j, -inf where it reaches past the row; the first
-  // element's index is returned
-  __device__ __forceinline__ int64_t load(int64_t j, int64_t end, float (&x)[VEC]) const {
-    const int64_t at = j * VEC - shift;
-    if (j < end && at >= 0 && at + VEC <= V) {
-      unpack<IO, VEC>(load_raw<IO, VEC>(base, at), x);
+  // the values from ``at`` on, -inf behind the row
+  __device__ __forceinline__ void load(int64_t at, float (&x)[kVec<IO>]) const {
+    const int64_t left = V - at;
+    if (left >= kVec<IO>) {
+      unpack<IO, kVec<IO>>(load_vec<IO>(logits, offset + at, kVec<IO>), x);
     } else {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) x[i] = j < end && at + i >= 0 && at + i < V ? load1<IO>(base, at + i) : -INFINITY;
+      for (int i = 0; i < kVec<IO>; ++i) x[i] = i < left ? load1<IO>(logits, offset + at + i) : -INFINITY;
     }
-    return at;
+  }
+  // the keys of the values from ``at`` on into the list, by make(value)
+  template <typename F>
+  __device__ __forceinline__ void push(TopList& top, int64_t at, const float (&x)[kVec<IO>], int lane, F&& make) const {
+#pragma unroll
+    for (int i = 0; i < kVec<IO>; ++i)
+      top.push(at + i < V ? make_key(make(x[i]), static_cast<uint32_t>(at + i)) : 0, lane);
+  }
+  template <typename F>
+  __device__ __forceinline__ uint64_t largest(uint64_t k, int64_t at, const float (&x)[kVec<IO>], F&& make) const {
+#pragma unroll
+    for (int i = 0; i < kVec<IO>; ++i) {
+      const uint64_t key = at + i < V ? make_key(make(x[i]), static_cast<uint32_t>(at + i)) : 0;
+      k = key > k ? key : k;
+    }
+    return k;
   }
 };
-
-// The span's largest values by make(x): every value whose key passes the bound
-template <typename IO, typename F>
-__device__ __forceinline__ void push_vector(TopList& top, const Row<IO>& row, int64_t at, int64_t j, int64_t end,
-                                            const float (&x)[Row<IO>::VEC], int lane, F&& make) {
-#pragma unroll
-  for (int i = 0; i < Row<IO>::VEC; ++i) {
-    const bool in = j < end && at + i >= 0 && at + i < row.V;
-    top.push(in ? make_key(make(x[i]), static_cast<uint32_t>(at + i)) : 0, lane);
-  }
-}
-template <typename IO, typename F>
-__device__ __forceinline__ void start_list(TopList& top, const Row<IO>& row, int64_t at, int64_t j, int64_t end,
-                                           const float (&x)[Row<IO>::VEC], int lane, F&& make) {
-  uint64_t k = 0;
-#pragma unroll
-  for (int i = 0; i < Row<IO>::VEC; ++i) {
-    const uint64_t key = j < end && at + i >= 0 && at + i < row.V ? make_key(make(x[i]), static_cast<uint32_t>(at + i)) : 0;
-    k = key > k ? key : k;
-  }
-  top.start(k, lane);
-}
 
 // parts: [rows][spans] (maximum, sum of exp(x - maximum)); tops: [rows][spans][want] keys
 template <typename IO>
@@ -200,34 +216,62 @@ __global__ void __launch_bounds__(64 * kScanWaves)
 beam_scan_kernel(int64_t rows, int64_t V, int64_t ld, int spans, int want, const void* logits, float2* parts,
                  uint64_t* tops) {
   __shared__ uint64_t buf[kScanWaves][128];
-  constexpr int VEC = Row<IO>::VEC;
+  constexpr int VEC = kVec<IO>;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t job = static_cast<int64_t>(blockIdx.x) * kScanWaves + wave;
   if (job >= rows * spans) return;  // no workgroup barrier below
   const int64_t r = job / spans;
   const int span = static_cast<int>(job - r * spans);
-  const Row<IO> row(logits, r * ld, V);
-  const int64_t per = (row.vectors + spans - 1) / spans;
-  const int64_t begin = span * per, end = begin + per < row.vectors ? begin + per : row.vectors;
+  const Row<IO> row{logits, r * ld, V};
+  const int64_t begin = span * span_values<VEC>(V, spans);
+  int64_t end = begin + span_values<VEC>(V, spans);
+  end = end < V ? end : V;
   TopList top;
   top.init(buf[wave], want);
   const auto same = [](float v) { return v; };
   float m = -INFINITY, s = 0.0f;
-  for (int64_t j0 = begin; j0 < end; j0 += 64) {
-    const int64_t j = j0 + lane;
-    float x[VEC];
-    const int64_t at = row.load(j, end, x);
-    float big = x[0];
+  for (int64_t at0 = begin; at0 < end; at0 += kAhead * 64 * VEC) {  // spans are whole numbers of 64 vectors
+    float x[kAhead][VEC], big[kAhead];
 #pragma unroll
-    for (int i = 1; i < VEC; ++i) big = fmaxf(big, x[i]);
-    if (j0 == begin) start_list<IO>(top, row, at, j, end, x, lane, same);
-    // no value of any lane passes the bound: the usual case
-    if (__any(!(big < key_value(top.bound)))) push_vector<IO>(top, row, at, j, end, x, lane, same);
-    const float mn = fmaxf(m, big);
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t at = at0 + (u * 64 + lane) * VEC;
+      if (at0 + u * 64 * VEC < end) {
+        row.load(at, x[u]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) x[u][i] = -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      big[u] = x[u][0];
+#pragma unroll
+      for (int i = 1; i < VEC; ++i) big[u] = fmaxf(big[u], x[u][i]);
+    }
+    if (at0 == begin) {
+      uint64_t k = 0;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (at0 + u * 64 * VEC < end) k = row.largest(k, at0 + (u * 64 + lane) * VEC, x[u], same);
+      top.start(k, lane);
+    }
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      mn = fmaxf(mn, big[u]);
+      // seldom: a value of some lane may pass the bound
+      if (at0 + u * 64 * VEC < end && __any(!(big[u] < key_value(top.bound))))
+        row.push(top, at0 + (u * 64 + lane) * VEC, x[u], lane, same);
+    }
     const float ref = mn == -INFINITY ? 0.0f : mn;  // nothing but -inf so far: exp gives 0
     float add = 0.0f;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) add += fast_exp(x[i] - ref);
+    for (int u = 0; u < kAhead; ++u) {
+      float e = 0.0f;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) e += fast_exp(x[u][i] - ref);
+      add += e;
+    }
     s = fmaf(s, fast_exp(m - ref), add);
     m = mn;
   }
@@ -315,13 +359,14 @@ beam_join_kernel(BeamStep p) {
           again = again || score(left == low ? next_below<IO>(low) : left) == score(low);
         }
         if (again) {
-          const Row<IO> row(p.logits, (b * K + k) * p.ld, p.V);
+          const Row<IO> row{p.logits, (b * K + k) * p.ld, p.V};
           top.init(buf[wave], keep);
-          for (int64_t j0 = 0; j0 < row.vectors; j0 += 64) {
-            float x[Row<IO>::VEC];
-            const int64_t at = row.load(j0 + lane, row.vectors, x);
-            if (j0 == 0) start_list<IO>(top, row, at, lane, row.vectors, x, lane, score);
-            push_vector<IO>(top, row, at, j0 + lane, row.vectors, x, lane, score);
+          for (int64_t at0 = 0; at0 < p.V; at0 += 64 * kVec<IO>) {
+            float x[kVec<IO>];
+            const int64_t at = at0 + lane * kVec<IO>;
+            row.load(at, x);
+            if (at0 == 0) top.start(row.largest(0, at, x, score), lane);
+            row.push(top, at, x, lane, score);
           }
           top.finish(lane);
           if (lane < keep) mine = make_key(key_value(top.list), flat + key_index(top.list));
@@ -362,52 +407,72 @@ struct Planes {
   const void* src[kMaxPlanes];
   void* dst[kMaxPlanes];
   int64_t row_bytes[kMaxPlanes];
-  uint32_t first[kMaxPlanes + 1];  // first tile of each plane: 256 accesses of a row
-  int count;
 };
 template <int B> struct Bytes;
-template <> struct Bytes<16> { using T = uint4; };
+template <> struct Bytes<16> { typedef uint32_t T __attribute__((ext_vector_type(4))); };
 template <> struct Bytes<4> { using T = uint32_t; };
 template <> struct Bytes<2> { using T = uint16_t; };
 
-// A thread moves one access of B bytes of all K rows of a batch row: it reads
-// them all before it writes, so src and dst may be the same.  KM >= K.  A
-// parent outside the beams fills its row with ones (NaN).
+// In place, plane blockIdx.y: a thread moves one access of B bytes of all K
+// rows of a batch row and reads them all before it writes.  Rows that stay are
+// left alone.  KM >= K.  A parent outside the beams fills its row with ones
+// (NaN).
 template <int B, int KM>
 __global__ void __launch_bounds__(256)
-reorder_kernel(Planes pl, int K, int64_t batch, const int64_t* parents) {
+reorder_in_place_kernel(Planes pl, int K, int64_t batch, const int64_t* parents) {
   using T = typename Bytes<B>::T;
-  const uint32_t tiles = pl.first[pl.count];
-  const int64_t jobs = batch * tiles;
+  const int64_t rb = pl.row_bytes[blockIdx.y], tiles = (rb + 256 * B - 1) / (256 * B), jobs = batch * tiles;
+  char* const plane = static_cast<char*>(pl.dst[blockIdx.y]);
   for (int64_t job = blockIdx.x; job < jobs; job += gridDim.x) {
-    const int64_t b = job / tiles;
-    const uint32_t tile = static_cast<uint32_t>(job - b * tiles);
-    int lo = 0, hi = pl.count - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) / 2;
-      if (pl.first[mid] <= tile) lo = mid; else hi = mid - 1;
-    }
-    const int64_t rb = pl.row_bytes[lo];
-    const int64_t at = (static_cast<int64_t>(tile - pl.first[lo]) * 256 + threadIdx.x) * B;
+    const int64_t b = job / tiles, at = ((job - b * tiles) * 256 + threadIdx.x) * B;
     if (at >= rb) continue;
-    const char* src = static_cast<const char*>(pl.src[lo]) + b * K * rb + at;
-    char* dst = static_cast<char*>(pl.dst[lo]) + b * K * rb + at;
-    const bool in_place = src == dst;
+    char* const col = plane + b * K * rb + at;
+    int p[KM];
+#pragma unroll
+    for (int k = 0; k < KM; ++k) {
+      const int64_t from = k < K ? parents[b * K + k] : k;
+      p[k] = from >= 0 && from < K ? static_cast<int>(from) : -1;
+    }
     T v[KM];
 #pragma unroll
     for (int k = 0; k < KM; ++k) {
-      if (k < K) {
-        const int64_t p = parents[b * K + k];
-        if (p >= 0 && p < K) {
-          if (!(in_place && p == k)) v[k] = *reinterpret_cast<const T*>(src + p * rb);
-        } else {
-          __builtin_memset(&v[k], 0xff, B);
-        }
+      if (k < K && p[k] != k) {
+        if (p[k] >= 0) v[k] = *reinterpret_cast<const T*>(col + p[k] * rb);
+        else v[k] = ~T(0);
       }
     }
 #pragma unroll
-    for (int k = 0; k < KM; ++k) {
-      if (k < K && !(in_place && parents[b * K + k] == k)) *reinterpret_cast<T*>(dst + k * rb) = v[k];
+    for (int k = 0; k < KM; ++k)
+      if (k < K && p[k] != k) *reinterpret_cast<T*>(col + k * rb) = v[k];
+  }
+}
+
+// To other memory, plane blockIdx.y: a workgroup copies kCopy accesses per
+// thread of one row.
+constexpr int kCopy = 4;
+template <int B>
+__global__ void __launch_bounds__(256)
+reorder_copy_kernel(Planes pl, int K, int64_t batch, const int64_t* parents) {
+  using T = typename Bytes<B>::T;
+  const int64_t rb = pl.row_bytes[blockIdx.y], tile = 256 * B * kCopy, tiles = (rb + tile - 1) / tile;
+  const char* const from = static_cast<const char*>(pl.src[blockIdx.y]);
+  char* const to = static_cast<char*>(pl.dst[blockIdx.y]);
+  const int64_t jobs = batch * K * tiles;
+  for (int64_t job = blockIdx.x; job < jobs; job += gridDim.x) {
+    const int64_t row = job / tiles, at = (job - row * tiles) * tile + threadIdx.x * B;
+    const int64_t p = parents[row];
+    const char* const src = from + ((row / K) * K + p) * rb;
+    T v[kCopy];
+#pragma unroll
+    for (int i = 0; i < kCopy; ++i) {
+      const int64_t o = at + i * 256 * B;
+      v[i] = ~T(0);
+      if (p >= 0 && p < K && o < rb) v[i] = *reinterpret_cast<const T*>(src + o);
+    }
+#pragma unroll
+    for (int i = 0; i < kCopy; ++i) {
+      const int64_t o = at + i * 256 * B;
+      if (o < rb) *reinterpret_cast<T*>(to + row * rb + o) = v[i];
     }
   }
 }
@@ -415,22 +480,11 @@ reorder_kernel(Planes pl, int K, int64_t batch, const int64_t* parents) {
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-sparc_status bm_fail(sparc_status s, const char* msg) {
-  snprintf(error_buffer(), 512, "%s", msg);
-  return s;
-}
-sparc_status bm_launched(const char* what) {
-  const hipError_t e = hipGetLastError();
-  if (e == hipSuccess) return SPARC_OK;
-  snprintf(error_buffer(), 512, "%s: %s", what, hipGetErrorString(e));
-  return SPARC_EHIP;
-}
-
 sparc_status bm_check(int64_t batch, int64_t beams, int64_t vocab) {
   if (batch < 0 || beams < 1 || beams > kMaxBeams || vocab < 1)
-    return bm_fail(SPARC_EINVAL, "beam step: batch >= 0, 1 to 32 beams and vocab > 0 required");
+    return op_fail(SPARC_EINVAL, "beam step: batch >= 0, 1 to 32 beams and vocab > 0 required");
   if (batch > (int64_t(1) << 22) / beams || vocab > INT32_MAX / beams)
-    return bm_fail(SPARC_EINVAL, "beam step: too large");
+    return op_fail(SPARC_EINVAL, "beam step: too large");
   return SPARC_OK;
 }
 // Spans per row: about 8192 waves in all (32 per CU), none shorter than kMinSpan
@@ -440,16 +494,18 @@ int spans_of(int64_t rows, int64_t vocab) {
   s = s < most ? s : most;
   return static_cast<int>(s < 1 ? 1 : (s < kMaxSpans ? s : kMaxSpans));
 }
-size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
 template <int B>
-void launch_reorder(hipStream_t st, const Planes& pl, int K, int64_t batch, const int64_t* parents) {
-  const int64_t jobs = batch * pl.first[pl.count];
-  const dim3 grid(static_cast<unsigned>(jobs < (1 << 20) ? jobs : (1 << 20))), block(256);
-  if (K <= 4) hipLaunchKernelGGL((reorder_kernel<B, 4>), grid, block, 0, st, pl, K, batch, parents);
-  else if (K <= 8) hipLaunchKernelGGL((reorder_kernel<B, 8>), grid, block, 0, st, pl, K, batch, parents);
-  else if (K <= 16) hipLaunchKernelGGL((reorder_kernel<B, 16>), grid, block, 0, st, pl, K, batch, parents);
-  else hipLaunchKernelGGL((reorder_kernel<B, 32>), grid, block, 0, st, pl, K, batch, parents);
+void launch_reorder(hipStream_t st, const Planes& pl, int count, int64_t widest, bool in_place, int K, int64_t batch,
+                    const int64_t* parents) {
+  const int64_t tile = 256 * B * (in_place ? 1 : kCopy), tiles = (widest + tile - 1) / tile;
+  const int64_t jobs = tiles * batch * (in_place ? 1 : K);
+  const dim3 grid(op_grid(jobs), count), block(256);
+  if (!in_place) hipLaunchKernelGGL((reorder_copy_kernel<B>), grid, block, 0, st, pl, K, batch, parents);
+  else if (K <= 4) hipLaunchKernelGGL((reorder_in_place_kernel<B, 4>), grid, block, 0, st, pl, K, batch, parents);
+  else if (K <= 8) hipLaunchKernelGGL((reorder_in_place_kernel<B, 8>), grid, block, 0, st, pl, K, batch, parents);
+  else if (K <= 16) hipLaunchKernelGGL((reorder_in_place_kernel<B, 16>), grid, block, 0, st, pl, K, batch, parents);
+  else hipLaunchKernelGGL((reorder_in_place_kernel<B, 32>), grid, block, 0, st, pl, K, batch, parents);
 }
 
 int plane_access(const void* src, const void* dst, int64_t row_bytes) {
@@ -478,16 +534,16 @@ sparc_status sparc_beam_step(int64_t batch, int64_t beams, int64_t vocab, int64_
                              void* workspace, size_t workspace_bytes, sparc_stream_t stream) {
   using namespace sparc;
   if (sparc_status s = bm_check(batch, beams, vocab)) return s;
-  if (io_dtype != SPARC_F32 && io_dtype != SPARC_BF16) return bm_fail(SPARC_EINVAL, "beam step: unknown io_dtype");
-  if (row_stride < vocab) return bm_fail(SPARC_EINVAL, "beam step: row_stride below vocab");
-  if (eos_id < -1 || eos_id >= vocab) return bm_fail(SPARC_EINVAL, "beam step: eos_id outside the vocabulary");
-  if (finished && eos_id < 0) return bm_fail(SPARC_EINVAL, "beam step: finished beams need an eos_id");
+  if (io_dtype != SPARC_F32 && io_dtype != SPARC_BF16) return op_fail(SPARC_EINVAL, "beam step: unknown io_dtype");
+  if (row_stride < vocab) return op_fail(SPARC_EINVAL, "beam step: row_stride below vocab");
+  if (eos_id < -1 || eos_id >= vocab) return op_fail(SPARC_EINVAL, "beam step: eos_id outside the vocabulary");
+  if (finished && eos_id < 0) return op_fail(SPARC_EINVAL, "beam step: finished beams need an eos_id");
   if (batch == 0) return SPARC_OK;
-  if (!logits || !scores || !tokens || !parents || !new_scores) return bm_fail(SPARC_EINVAL, "beam step: NULL pointer");
+  if (!logits || !scores || !tokens || !parents || !new_scores) return op_fail(SPARC_EINVAL, "beam step: NULL pointer");
   if (!workspace || workspace_bytes < sparc_beam_workspace_bytes(batch, beams, vocab))
-    return bm_fail(SPARC_EWORKSPACE, "beam step: workspace missing or too small");
+    return op_fail(SPARC_EWORKSPACE, "beam step: workspace missing or too small");
   if (reinterpret_cast<uintptr_t>(workspace) % 8)
-    return bm_fail(SPARC_EINVAL, "beam step: the workspace must be 8-byte aligned");
+    return op_fail(SPARC_EINVAL, "beam step: the workspace must be 8-byte aligned");
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const int64_t rows = batch * beams;
   const int spans = spans_of(rows, vocab), want = static_cast<int>(beams) + 1;
@@ -519,7 +575,7 @@ sparc_status sparc_beam_step(int64_t batch, int64_t beams, int64_t vocab, int64_
     hipLaunchKernelGGL((beam_scan_kernel<sparc::bf16>), grid, block, 0, st, rows, vocab, row_stride, spans, want, logits, parts, tops);
     hipLaunchKernelGGL((beam_join_kernel<sparc::bf16>), join, jblock, 0, st, p);
   }
-  return bm_launched("beam step");
+  return op_launched("beam step");
 }
 
 sparc_status sparc_reorder_states(int64_t batch, int64_t beams, int64_t count, const void* const* src,
@@ -527,38 +583,42 @@ sparc_status sparc_reorder_states(int64_t batch, int64_t beams, int64_t count, c
                                   sparc_stream_t stream) {
   using namespace sparc;
   if (batch < 0 || beams < 1 || beams > kMaxBeams || count < 0 || batch > (int64_t(1) << 22) / beams)
-    return bm_fail(SPARC_EINVAL, "reorder states: batch >= 0, 1 to 32 beams and count >= 0 required");
+    return op_fail(SPARC_EINVAL, "reorder states: batch >= 0, 1 to 32 beams and count >= 0 required");
   if (batch == 0 || count == 0) return SPARC_OK;
-  if (!src || !dst || !row_bytes || !parents) return bm_fail(SPARC_EINVAL, "reorder states: NULL pointer");
+  if (!src || !dst || !row_bytes || !parents) return op_fail(SPARC_EINVAL, "reorder states: NULL pointer");
   for (int64_t i = 0; i < count; ++i) {
     if (row_bytes[i] < 0 || row_bytes[i] % 2 || row_bytes[i] > (int64_t(1) << 31))
-      return bm_fail(SPARC_EINVAL, "reorder states: rows of an even number of bytes up to 2^31 required");
-    if (row_bytes[i] > 0 && (!src[i] || !dst[i])) return bm_fail(SPARC_EINVAL, "reorder states: NULL plane");
+      return op_fail(SPARC_EINVAL, "reorder states: rows of an even number of bytes up to 2^31 required");
+    if (row_bytes[i] > 0 && (!src[i] || !dst[i])) return op_fail(SPARC_EINVAL, "reorder states: NULL plane");
     if ((reinterpret_cast<uintptr_t>(src[i]) | reinterpret_cast<uintptr_t>(dst[i])) % 2)
-      return bm_fail(SPARC_EINVAL, "reorder states: planes must be 2-byte aligned");
+      return op_fail(SPARC_EINVAL, "reorder states: planes must be 2-byte aligned");
   }
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   Planes pl;
-  for (const int access : {16, 4, 2}) {  // planes of one access width share launches
-    for (int64_t at = 0; at < count;) {
-      pl.count = 0;
-      uint32_t tiles = 0;
-      for (; at < count && pl.count < kMaxPlanes && tiles < (1u << 30); ++at) {
-        if (row_bytes[at] == 0 || plane_access(src[at], dst[at], row_bytes[at]) != access) continue;
-        pl.src[pl.count] = src[at];
-        pl.dst[pl.count] = dst[at];
-        pl.row_bytes[pl.count] = row_bytes[at];
-        pl.first[pl.count++] = tiles;
-        tiles += static_cast<uint32_t>((row_bytes[at] + 256 * access - 1) / (256 * access));
+  // planes of one access width, in place or not, share launches
+  for (const bool in_place : {false, true}) {
+    for (const int access : {16, 4, 2}) {
+      for (int64_t at = 0; at < count;) {
+        int n = 0;
+        int64_t widest = 0;
+        for (; at < count && n < kMaxPlanes; ++at) {
+          if (row_bytes[at] == 0 || (src[at] == dst[at]) != in_place ||
+              plane_access(src[at], dst[at], row_bytes[at]) != access)
+            continue;
+          pl.src[n] = src[at];
+          pl.dst[n] = dst[at];
+          pl.row_bytes[n++] = row_bytes[at];
+          widest = row_bytes[at] > widest ? row_bytes[at] : widest;
+        }
+        if (n == 0) break;
+        const int K = static_cast<int>(beams);
+        if (access == 16) launch_reorder<16>(st, pl, n, widest, in_place, K, batch, parents);
+        else if (access == 4) launch_reorder<4>(st, pl, n, widest, in_place, K, batch, parents);
+        else launch_reorder<2>(st, pl, n, widest, in_place, K, batch, parents);
       }
-      pl.first[pl.count] = tiles;
-      if (pl.count == 0) break;
-      if (access == 16) launch_reorder<16>(st, pl, static_cast<int>(beams), batch, parents);
-      else if (access == 4) launch_reorder<4>(st, pl, static_cast<int>(beams), batch, parents);
-      else launch_reorder<2>(st, pl, static_cast<int>(beams), batch, parents);
     }
   }
-  return bm_launched("reorder states");
+  return op_launched("reorder states");
 }
 
 }  // extern "C"

@@ -17,8 +17,7 @@
 // not depend on timing, and every row of dW is written exactly once: rows
 // without tokens are cleared by further workgroups of the summing kernel.
 
-#include "common.h"
-#include "sparc_hip.h"
+#include "rows.h"
 
 namespace sparc {
 namespace {
@@ -27,15 +26,17 @@ constexpr int kPiece = 16;          // sorted positions per piece
 constexpr int kSortThreads = 256;   // 4 waves per sort tile
 constexpr int kSortWaves = kSortThreads / 64;
 constexpr int kMaxDigits = 512;     // 9 bits
-constexpr int kJoinWaves = 16;
+constexpr int kJoinWaves = 16;      // pieces per join workgroup
+constexpr int kLongRun = 64;        // pieces of a run that a whole join workgroup adds up
 constexpr uint32_t kNone = 0xffffffffu;
 
 // Scaled copies of table rows.  A group of lpr lanes (a power of two up to 64)
-// takes one block of lpr * V columns of one token.
-template <typename IO, int V>
+// takes one block of lpr 16-byte vectors of one token.
+template <typename IO>
 __global__ void __launch_bounds__(256)
 embed_fwd_kernel(int64_t N, int64_t vocab, int D, int lpr, int blocks, const void* tokens, int wide_ids, const void* w,
                  float scale, void* y) {
+  constexpr int V = kVec<IO>;
   const int gl = threadIdx.x & (lpr - 1);
   const int64_t per = 256 / lpr;
   const int64_t jobs = N * blocks;
@@ -46,14 +47,14 @@ embed_fwd_kernel(int64_t N, int64_t vocab, int D, int lpr, int blocks, const voi
     const int64_t id = wide_ids ? static_cast<const int64_t*>(tokens)[n] : static_cast<const int32_t*>(tokens)[n];
     float v[V];
     if (id >= 0 && id < vocab) {
-      unpack<IO, V>(load_raw<IO, V>(w, id * D + c), v);
+      unpack<IO, V>(load_vec<IO>(w, id * D + c, D - c), v);
 #pragma unroll
       for (int i = 0; i < V; ++i) v[i] *= scale;
     } else {
 #pragma unroll
       for (int i = 0; i < V; ++i) v[i] = __uint_as_float(0x7fc00000u);
     }
-    store_raw<IO, V>(y, n * D + c, pack<IO, V>(v));
+    store_vec<IO>(y, n * D + c, D - c, pack<IO, V>(v));
   }
 }
 
@@ -126,14 +127,22 @@ sort_scatter_kernel(SortPass p) {
   }
   // a thread's digits: 2 t and 2 t + 1, so that a scan over threads is one over digits
   uint32_t before[2] = {0, 0}, total[2] = {0, 0};
+  if (2 * static_cast<int>(threadIdx.x) < digits) {
+    const uint2* counts = reinterpret_cast<const uint2*>(p.counts) + threadIdx.x;
+    const int tiles = gridDim.x, mine = blockIdx.x;
+    for (int t0 = 0; t0 < tiles; t0 += 16) {
+      uint2 c[16];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int d = 2 * threadIdx.x + k;
-    if (d < digits) {
-      for (int tile = 0; tile < static_cast<int>(gridDim.x); ++tile) {
-        const uint32_t c = p.counts[static_cast<int64_t>(tile) * digits + d];
-        if (tile < static_cast<int>(blockIdx.x)) before[k] += c;
-        total[k] += c;
+      for (int k = 0; k < 16; ++k)
+        c[k] = t0 + k < tiles ? counts[static_cast<int64_t>(t0 + k) * (digits / 2)] : make_uint2(0, 0);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        total[0] += c[k].x;
+        total[1] += c[k].y;
+        if (t0 + k < mine) {
+          before[0] += c[k].x;
+          before[1] += c[k].y;
+        }
       }
     }
   }
@@ -202,36 +211,34 @@ sort_scatter_kernel(SortPass p) {
 // ---------------------------------------------------------------------------
 // the sums
 // ---------------------------------------------------------------------------
-template <typename IO, int V>
-__device__ __forceinline__ void write_row(void* dw, int64_t index, const float (&acc)[V], float scale) {
-  float o[V];
+template <typename IO>
+__device__ __forceinline__ void write_row(void* dw, int64_t row, int D, int c, const float (&acc)[kVec<IO>],
+                                          float scale) {
+  float o[kVec<IO>];
 #pragma unroll
-  for (int i = 0; i < V; ++i) o[i] = acc[i] * scale;
-  store_raw<IO, V>(dw, index, pack<IO, V>(o));
+  for (int i = 0; i < kVec<IO>; ++i) o[i] = acc[i] * scale;
+  store_vec<IO>(dw, row * D + c, D - c, pack<IO, kVec<IO>>(o));
 }
 
 // Workgroups below sum_groups: pieces of sorted positions, a group of lpr lanes
-// per piece and block of lpr * V columns.  part: [pieces][2][D] fp32, the
+// per piece and block of lpr 16-byte vectors.  part: [pieces][2][D] fp32, the
 // partial sums of a run that goes on from the piece before (0) and of one that
 // begins here and goes on into the next (1).  The others clear rows of dW that
 // no token names.
-template <typename IO, int V>
+template <typename IO>
 __global__ void __launch_bounds__(256)
 embed_sum_kernel(int64_t N, int64_t vocab, int D, int lpr, int blocks, int64_t sum_groups, const uint32_t* keys,
                  const uint32_t* pos, const uint8_t* touched, const void* dy, float scale, float* part, void* dw) {
+  constexpr int V = kVec<IO>;
   const int gl = threadIdx.x & (lpr - 1);
   const int64_t per = 256 / lpr;
   if (blockIdx.x >= sum_groups) {
     const int64_t jobs = vocab * blocks, step = (gridDim.x - sum_groups) * per;
+    const Vec<IO> zero = {};
     for (int64_t job = (blockIdx.x - sum_groups) * per + threadIdx.x / lpr; job < jobs; job += step) {
       const int64_t v = blocks == 1 ? job : job / blocks;
       const int c = (static_cast<int>(job - v * blocks) * lpr + gl) * V;
-      if (c < D && !touched[v]) {
-        float z[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) z[i] = 0.0f;
-        store_raw<IO, V>(dw, v * D + c, pack<IO, V>(z));
-      }
+      if (c < D && !touched[v]) store_vec<IO>(dw, v * D + c, D - c, zero);
     }
     return;
   }
@@ -243,14 +250,15 @@ embed_sum_kernel(int64_t N, int64_t vocab, int D, int lpr, int blocks, int64_t s
     const int64_t p0 = piece * kPiece;
     const int n = N - p0 < kPiece ? static_cast<int>(N - p0) : kPiece;
     uint32_t key[kPiece];
-    typename Raw<IO, V>::T raw[kPiece];
+    Vec<IO> raw[kPiece];
 #pragma unroll
     for (int i = 0; i < kPiece; ++i) key[i] = i < n ? keys[p0 + i] : kNone;
     const uint32_t prev = p0 > 0 ? keys[p0 - 1] : kNone;
     const uint32_t next = p0 + n < N ? keys[p0 + n] : kNone;
 #pragma unroll
     for (int i = 0; i < kPiece; ++i) {
-      if (key[i] < static_cast<uint32_t>(vocab)) raw[i] = load_raw<IO, V>(dy, static_cast<int64_t>(pos[p0 + i]) * D + c);
+      if (key[i] < static_cast<uint32_t>(vocab))
+        raw[i] = load_vec<IO>(dy, static_cast<int64_t>(pos[p0 + i]) * D + c, D - c);
     }
     float acc[V];
 #pragma unroll
@@ -267,11 +275,12 @@ embed_sum_kernel(int64_t N, int64_t vocab, int D, int lpr, int blocks, int64_t s
         const bool end = i + 1 == n;
         if (end || after != key[i]) {
           if (head || after == key[i]) {
-            float* to = part + ((piece * 2 + (head ? 0 : 1)) * D + c);
+            const int64_t to = (piece * 2 + (head ? 0 : 1)) * D + c;
 #pragma unroll
-            for (int k = 0; k < V; ++k) to[k] = acc[k];
+            for (int q = 0; q < V; q += 4)
+              store_vec<float>(part, to + q, D - c - q, make_float4(acc[q], acc[q + 1], acc[q + 2], acc[q + 3]));
           } else {
-            write_row<IO, V>(dw, static_cast<int64_t>(key[i]) * D + c, acc, scale);
+            write_row<IO>(dw, key[i], D, c, acc, scale);
           }
           head = false;
 #pragma unroll
@@ -282,78 +291,115 @@ embed_sum_kernel(int64_t N, int64_t vocab, int D, int lpr, int blocks, int64_t s
   }
 }
 
-// Joins the runs that begin in piece blockIdx.x and go on behind it: the first
-// piece's partial sum, then the later ones' in order, kJoinWaves slices of them
-// side by side.  blockIdx.y: a block of 64 columns.
+// s += the rows a, a + 1, ... below b of the running partial sums, 4 columns
+__device__ __forceinline__ void add_parts(float (&s)[4], const float* part, int64_t a, int64_t b, int D, int c) {
+  int64_t q = a;
+  for (; q + 8 <= b; q += 8) {
+    float4 u[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) u[k] = load_vec<float>(part, (q + k) * 2 * D + c, D - c);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) { s[0] += u[k].x; s[1] += u[k].y; s[2] += u[k].z; s[3] += u[k].w; }
+  }
+  for (; q < b; ++q) {
+    const float4 u = load_vec<float>(part, q * 2 * D + c, D - c);
+    s[0] += u.x; s[1] += u.y; s[2] += u.z; s[3] += u.w;
+  }
+}
+
+// Joins the runs that cross pieces, a wave per piece: where a run begins in its
+// piece and goes on behind it, the piece's own partial sum, then the later
+// pieces' in order.  Runs over more than kLongRun pieces are left to the whole
+// workgroup, which adds kJoinWaves slices of them side by side.  blockIdx.y: a
+// block of 256 columns.
 template <typename IO>
 __global__ void __launch_bounds__(64 * kJoinWaves)
 embed_join_kernel(int64_t N, int64_t vocab, int D, const uint32_t* keys, float scale, const float* part, void* dw) {
-  __shared__ float red[kJoinWaves][64];
+  __shared__ float4 red[kJoinWaves][64];
+  __shared__ int64_t long_first[kJoinWaves], long_last[kJoinWaves];
+  __shared__ uint32_t long_key[kJoinWaves];
   const int64_t pieces = (N + kPiece - 1) / kPiece;
-  for (int64_t piece = blockIdx.x; piece + 1 < pieces; piece += gridDim.x) {
-    const int64_t p0 = piece * kPiece, p1 = p0 + kPiece;
-    const uint32_t key = keys[p1 - 1];
-    if (key >= static_cast<uint32_t>(vocab) || keys[p1] != key) continue;          // nothing crosses
-    if (p0 > 0 && keys[p0] == key && keys[p0 - 1] == key) continue;                // it began earlier
-    // the run's end: the first position behind p1 with a larger key
-    int64_t lo = p1, hi = N;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) / 2;
-      if (keys[mid] <= key) lo = mid + 1; else hi = mid;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  for (int64_t piece0 = static_cast<int64_t>(blockIdx.x) * kJoinWaves; piece0 + 1 < pieces;
+       piece0 += static_cast<int64_t>(gridDim.x) * kJoinWaves) {
+    const int64_t piece = piece0 + wave, p0 = piece * kPiece, p1 = p0 + kPiece;
+    bool begins = piece + 1 < pieces;
+    uint32_t key = kNone;
+    if (begins) {
+      key = keys[p1 - 1];
+      // it crosses, and does not come from an earlier piece
+      begins = key < static_cast<uint32_t>(vocab) && keys[p1] == key &&
+               !(p0 > 0 && keys[p0] == key && keys[p0 - 1] == key);
     }
-    const int64_t last = (lo - 1) / kPiece, count = last - piece;  // pieces behind this one
-    const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
-    const int64_t each = (count + kJoinWaves - 1) / kJoinWaves;
-    const int64_t a = piece + 1 + slice * each, b = a + each < last + 1 ? a + each : last + 1;
-    for (int c0 = blockIdx.y * 64; c0 < D; c0 += gridDim.y * 64) {
-      const int c = c0 + lane;
-      float s = 0.0f;
-      if (c < D) {
-        if (slice == 0) s = part[(piece * 2 + 1) * D + c];
-        float u[8];
-        int64_t q = a;
-        for (; q + 8 <= b; q += 8) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) u[k] = part[(q + k) * 2 * D + c];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) s += u[k];
+    int64_t last = piece;
+    if (begins) {
+      // pieces that begin with the key, 64 at a time: they are consecutive
+      for (;;) {
+        const int64_t q = last + 1 + lane;
+        const uint64_t same = __ballot(q < pieces && keys[q * kPiece] == key);
+        const int more = __popcll(same);
+        last += more;
+        if (more < 64) break;
+      }
+    }
+    const bool is_long = begins && last - piece > kLongRun;
+    if (lane == 0) {
+      long_first[wave] = is_long ? piece : -1;
+      long_last[wave] = last;
+      long_key[wave] = key;
+    }
+    if (begins && !is_long) {
+      for (int c = (blockIdx.y * 64 + lane) * 4; c < D; c += gridDim.y * 256) {
+        const float4 own = load_vec<float>(part, (piece * 2 + 1) * D + c, D - c);
+        float s[4] = {own.x, own.y, own.z, own.w};
+        add_parts(s, part, piece + 1, last + 1, D, c);
+        for (int i = 0; i < 4 && c + i < D; ++i) store1<IO>(dw, static_cast<int64_t>(key) * D + c + i, s[i] * scale);
+      }
+    }
+    __syncthreads();
+    for (int w = 0; w < kJoinWaves; ++w) {
+      const int64_t first = long_first[w];
+      if (first < 0) continue;  // uniform over the workgroup
+      const int64_t end = long_last[w] + 1, each = (end - first - 1 + kJoinWaves - 1) / kJoinWaves;
+      const int64_t a = first + 1 + wave * each, b = a + each < end ? a + each : end;
+      for (int c0 = blockIdx.y * 256; c0 < D; c0 += gridDim.y * 256) {
+        const int c = c0 + lane * 4;
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (c < D) {
+          if (wave == 0) {
+            const float4 own = load_vec<float>(part, (first * 2 + 1) * D + c, D - c);
+            s[0] = own.x; s[1] = own.y; s[2] = own.z; s[3] = own.w;
+          }
+          add_parts(s, part, a, b, D, c);
         }
-        for (; q < b; ++q) s += part[q * 2 * D + c];
+        red[wave][lane] = make_float4(s[0], s[1], s[2], s[3]);
+        __syncthreads();
+        if (wave == 0 && c < D) {
+          float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          for (int k = 0; k < kJoinWaves; ++k) {
+            const float4 u = red[k][lane];
+            t[0] += u.x; t[1] += u.y; t[2] += u.z; t[3] += u.w;
+          }
+          for (int i = 0; i < 4 && c + i < D; ++i)
+            store1<IO>(dw, static_cast<int64_t>(long_key[w]) * D + c + i, t[i] * scale);
+        }
+        __syncthreads();
       }
-      red[slice][lane] = s;
-      __syncthreads();
-      if (slice == 0 && c < D) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kJoinWaves; ++k) sum += red[k][lane];
-        store1<IO>(dw, static_cast<int64_t>(key) * D + c, sum * scale);
-      }
-      __syncthreads();
     }
+    __syncthreads();
   }
 }
 
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-sparc_status em_fail(sparc_status s, const char* msg) {
-  snprintf(error_buffer(), 512, "%s", msg);
-  return s;
-}
-sparc_status em_launched(const char* what) {
-  const hipError_t e = hipGetLastError();
-  if (e == hipSuccess) return SPARC_OK;
-  snprintf(error_buffer(), 512, "%s: %s", what, hipGetErrorString(e));
-  return SPARC_EHIP;
-}
-
 sparc_status em_check(int64_t n, int64_t vocab, int64_t dim, int32_t io, int32_t id_bytes) {
-  if (n < 0 || vocab <= 0 || dim <= 0) return em_fail(SPARC_EINVAL, "embedding: n >= 0, vocab > 0 and dim > 0 required");
-  if (io != SPARC_F32 && io != SPARC_BF16) return em_fail(SPARC_EINVAL, "embedding: unknown io_dtype");
-  if (id_bytes != 4 && id_bytes != 8) return em_fail(SPARC_EINVAL, "embedding: ids are 32- or 64-bit integers");
+  if (n < 0 || vocab <= 0 || dim <= 0) return op_fail(SPARC_EINVAL, "embedding: n >= 0, vocab > 0 and dim > 0 required");
+  if (io != SPARC_F32 && io != SPARC_BF16) return op_fail(SPARC_EINVAL, "embedding: unknown io_dtype");
+  if (id_bytes != 4 && id_bytes != 8) return op_fail(SPARC_EINVAL, "embedding: ids are 32- or 64-bit integers");
   if (n > (int64_t(1) << 30) || vocab > (int64_t(1) << 30) || dim > (int64_t(1) << 24) ||
       n > (int64_t(1) << 46) / dim || vocab > (int64_t(1) << 46) / dim)
-    return em_fail(SPARC_EINVAL, "embedding: too large");
+    return op_fail(SPARC_EINVAL, "embedding: too large");
   return SPARC_OK;
 }
 
@@ -372,45 +418,24 @@ Sort sort_of(int64_t n, int64_t vocab) {
   if (s.tiles < 1) s.tiles = 1;  // without tokens, one tile clears the flags
   return s;
 }
-size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
-// lanes per row and column blocks per row
+// Lanes per row and blocks per row: the widest group that leaves at most an
+// eighth of its lanes idle (96 vectors: 3 blocks of 32 lanes, not 2 of 64)
 void em_groups(int64_t dim, int v, int& lpr, int& blocks) {
   const int64_t vecs = (dim + v - 1) / v;
-  lpr = 1;
-  while (lpr < 64 && lpr < vecs) lpr <<= 1;
+  lpr = 64;
+  while (lpr > 1 && (vecs + lpr - 1) / lpr * lpr * 8 > vecs * 9) lpr >>= 1;
   blocks = static_cast<int>((vecs + lpr - 1) / lpr);
 }
-unsigned em_grid(int64_t jobs, int lpr) {
-  const int64_t g = (jobs * lpr + 255) / 256;
-  return static_cast<unsigned>(g < 1 ? 1 : (g < (1 << 20) ? g : (1 << 20)));
-}
-int em_vec(int64_t dim, size_t es, const void* a, const void* b) {
-  for (int v = static_cast<int>(16 / es); v > 1; v /= 2)
-    if (dim % v == 0 && reinterpret_cast<uintptr_t>(a) % (v * es) == 0 && reinterpret_cast<uintptr_t>(b) % (v * es) == 0)
-      return v;
-  return 1;
-}
-template <int N> using Int = std::integral_constant<int, N>;
-template <typename IO, typename F>
-void em_dispatch(int v, F&& f) {
-  if constexpr (sizeof(IO) == 2) {
-    if (v == 8) return f(Int<8>{});
-  }
-  if (v == 4) return f(Int<4>{});
-  if (v == 2) return f(Int<2>{});
-  f(Int<1>{});
-}
+unsigned em_grid(int64_t jobs, int lpr) { return op_grid((jobs * lpr + 255) / 256); }
 
 template <typename IO>
 void em_forward(hipStream_t st, int64_t n, int64_t vocab, int64_t dim, const void* tokens, int id_bytes, const void* w,
                 float scale, void* y) {
-  em_dispatch<IO>(em_vec(dim, sizeof(IO), w, y), [&](auto V) {
-    int lpr, blocks;
-    em_groups(dim, V(), lpr, blocks);
-    hipLaunchKernelGGL((embed_fwd_kernel<IO, V()>), dim3(em_grid(n * blocks, lpr)), dim3(256), 0, st, n, vocab,
-                       static_cast<int>(dim), lpr, blocks, tokens, id_bytes == 8, w, scale, y);
-  });
+  int lpr, blocks;
+  em_groups(dim, kVec<IO>, lpr, blocks);
+  hipLaunchKernelGGL((embed_fwd_kernel<IO>), dim3(em_grid(n * blocks, lpr)), dim3(256), 0, st, n, vocab,
+                     static_cast<int>(dim), lpr, blocks, tokens, id_bytes == 8, w, scale, y);
 }
 
 template <int ITEMS>
@@ -423,19 +448,17 @@ template <typename IO>
 void em_sums(hipStream_t st, int64_t n, int64_t vocab, int64_t dim, const uint32_t* keys, const uint32_t* pos,
              const uint8_t* touched, const void* dy, float scale, float* part, void* dw) {
   const int64_t pieces = (n + kPiece - 1) / kPiece;
-  em_dispatch<IO>(em_vec(dim, sizeof(IO), dy, dw), [&](auto V) {
-    int lpr, blocks;
-    em_groups(dim, V(), lpr, blocks);
-    const unsigned sum_groups = em_grid(pieces * blocks, lpr);
-    const unsigned clear = em_grid(vocab * blocks, lpr), most = 4096;
-    hipLaunchKernelGGL((embed_sum_kernel<IO, V()>), dim3(sum_groups + (clear < most ? clear : most)), dim3(256), 0, st,
-                       n, vocab, static_cast<int>(dim), lpr, blocks, static_cast<int64_t>(sum_groups), keys, pos,
-                       touched, dy, scale, part, dw);
-  });
+  int lpr, blocks;
+  em_groups(dim, kVec<IO>, lpr, blocks);
+  const unsigned sum_groups = em_grid(pieces * blocks, lpr);
+  const unsigned clear = em_grid(vocab * blocks, lpr), most = 4096;
+  hipLaunchKernelGGL((embed_sum_kernel<IO>), dim3(sum_groups + (clear < most ? clear : most)), dim3(256), 0, st, n,
+                     vocab, static_cast<int>(dim), lpr, blocks, static_cast<int64_t>(sum_groups), keys, pos, touched,
+                     dy, scale, part, dw);
   if (pieces > 1) {
-    const int64_t blocks = (dim + 63) / 64;
-    const dim3 grid(static_cast<unsigned>(pieces < (1 << 18) ? pieces : (1 << 18)),
-                    static_cast<unsigned>(blocks < 64 ? blocks : 64));
+    const int64_t groups = (pieces + kJoinWaves - 1) / kJoinWaves, columns = (dim + 255) / 256;
+    const dim3 grid(static_cast<unsigned>(groups < (1 << 18) ? groups : (1 << 18)),
+                    static_cast<unsigned>(columns < 64 ? columns : 64));
     hipLaunchKernelGGL((embed_join_kernel<IO>), grid, dim3(64 * kJoinWaves), 0, st, n, vocab, static_cast<int>(dim),
                        keys, scale, part, dw);
   }
@@ -455,11 +478,11 @@ sparc_status sparc_embedding_forward(int64_t n, int64_t vocab, int64_t dim, int3
   using namespace sparc;
   if (sparc_status s = em_check(n, vocab, dim, io_dtype, id_bytes)) return s;
   if (n == 0) return SPARC_OK;
-  if (!tokens || !weight || !y) return em_fail(SPARC_EINVAL, "embedding forward: NULL pointer");
+  if (!tokens || !weight || !y) return op_fail(SPARC_EINVAL, "embedding forward: NULL pointer");
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (io_dtype == SPARC_F32) em_forward<float>(st, n, vocab, dim, tokens, id_bytes, weight, scale, y);
   else em_forward<sparc::bf16>(st, n, vocab, dim, tokens, id_bytes, weight, scale, y);
-  return em_launched("embedding forward");
+  return op_launched("embedding forward");
 }
 
 size_t sparc_embedding_workspace_bytes(int64_t n, int64_t vocab, int64_t dim) {
@@ -476,11 +499,11 @@ sparc_status sparc_embedding_backward(int64_t n, int64_t vocab, int64_t dim, int
                                       void* dweight, void* workspace, size_t workspace_bytes, sparc_stream_t stream) {
   using namespace sparc;
   if (sparc_status s = em_check(n, vocab, dim, io_dtype, id_bytes)) return s;
-  if (!dweight || (n > 0 && (!tokens || !dy))) return em_fail(SPARC_EINVAL, "embedding backward: NULL pointer");
+  if (!dweight || (n > 0 && (!tokens || !dy))) return op_fail(SPARC_EINVAL, "embedding backward: NULL pointer");
   if (!workspace || workspace_bytes < sparc_embedding_workspace_bytes(n, vocab, dim))
-    return em_fail(SPARC_EWORKSPACE, "embedding backward: workspace missing or too small");
+    return op_fail(SPARC_EWORKSPACE, "embedding backward: workspace missing or too small");
   if (reinterpret_cast<uintptr_t>(workspace) % 16)
-    return em_fail(SPARC_EINVAL, "embedding backward: the workspace must be 16-byte aligned");
+    return op_fail(SPARC_EINVAL, "embedding backward: the workspace must be 16-byte aligned");
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const Sort s = sort_of(n, vocab);
   char* at = static_cast<char*>(workspace);
@@ -514,7 +537,7 @@ sparc_status sparc_embedding_backward(int64_t n, int64_t vocab, int64_t dim, int
   }
   if (io_dtype == SPARC_F32) em_sums<float>(st, n, vocab, dim, keys[cur ^ 1], pos[cur ^ 1], touched, dy, scale, part, dweight);
   else em_sums<sparc::bf16>(st, n, vocab, dim, keys[cur ^ 1], pos[cur ^ 1], touched, dy, scale, part, dweight);
-  return em_launched("embedding backward");
+  return op_launched("embedding backward");
 }
 
 }  // extern "C"

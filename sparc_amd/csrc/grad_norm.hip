@@ -11,8 +11,7 @@
 // order, so the norm does not depend on timing and no launch stands between;
 // where nothing is clipped they read nothing more.
 
-#include "common.h"
-#include "sparc_hip.h"
+#include "rows.h"
 
 namespace sparc {
 namespace {
@@ -30,48 +29,130 @@ struct TensorList {
   int count;
 };
 
-// The piece's tensor: the last one whose first piece is not behind it
-__device__ __forceinline__ int tensor_of(const TensorList& l, uint32_t piece) {
-  int lo = 0, hi = l.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (l.first[mid] <= piece) lo = mid; else hi = mid - 1;
+// A launch's list in LDS: one trip to the kernel arguments for all threads,
+// where a search among them would make one for each of its steps.
+struct ListInLds {
+  void* data[kMaxTensors];
+  int64_t size[kMaxTensors];
+  uint32_t first[kMaxTensors + 1];
+  uint8_t bf16_values[kMaxTensors];
+
+  __device__ __forceinline__ void load(const TensorList& l) {
+    for (int i = threadIdx.x; i <= l.count; i += kThreads) {
+      first[i] = l.first[i];
+      if (i < l.count) {
+        data[i] = l.data[i];
+        size[i] = l.size[i];
+        bf16_values[i] = l.bf16_values[i];
+      }
+    }
+    __syncthreads();
   }
-  return lo;
+  // the piece's tensor: the last one whose first piece is not behind it
+  __device__ __forceinline__ int tensor_of(uint32_t piece, int count) const {
+    int lo = 0, hi = count - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (first[mid] <= piece) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+  }
+  // f(first byte, end, whether bf16) for a piece
+  template <typename F>
+  __device__ __forceinline__ void piece(uint32_t p, int count, F&& f) const {
+    const int t = __builtin_amdgcn_readfirstlane(tensor_of(p, count));
+    const int64_t lo = static_cast<int64_t>(p - first[t]) * kPieceValues;
+    const int64_t hi = lo + kPieceValues < size[t] ? lo + kPieceValues : size[t];
+    const bool narrow = bf16_values[t];
+    const int size_of = narrow ? 2 : 4;
+    const uintptr_t base = reinterpret_cast<uintptr_t>(data[t]);
+    f(base + lo * size_of, base + hi * size_of, narrow);
+  }
+};
+
+// Values at an address out of the list: said to be global memory, which the
+// compiler cannot know of an address that it reads from LDS
+template <typename IO> struct GlobalTypes;
+template <> struct GlobalTypes<float> {
+  typedef __attribute__((address_space(1))) float One;
+  typedef uint32_t V4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(1))) V4 Four;
+};
+template <> struct GlobalTypes<bf16> {
+  typedef __attribute__((address_space(1))) uint16_t One;
+  typedef uint32_t V4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(1))) V4 Four;
+};
+template <typename IO>
+__device__ __forceinline__ float load_value(uintptr_t at) {
+  const auto v = *reinterpret_cast<const typename GlobalTypes<IO>::One*>(at);
+  if constexpr (sizeof(IO) == 4) return v;
+  else return bf16_bits_to_float(v);
+}
+template <typename IO>
+__device__ __forceinline__ void store_value(uintptr_t at, float v) {
+  auto* p = reinterpret_cast<typename GlobalTypes<IO>::One*>(at);
+  if constexpr (sizeof(IO) == 4) *p = v;
+  else *p = pack_bf16(v);
+}
+template <typename IO>
+__device__ __forceinline__ void load_values(uintptr_t at, Vec<IO>& v) {
+  const auto u = *reinterpret_cast<const typename GlobalTypes<IO>::Four*>(at);
+  __builtin_memcpy(&v, &u, 16);
+}
+template <typename IO>
+__device__ __forceinline__ void store_values(uintptr_t at, const Vec<IO>& v) {
+  typename GlobalTypes<IO>::V4 u;
+  __builtin_memcpy(&u, &v, 16);
+  *reinterpret_cast<typename GlobalTypes<IO>::Four*>(at) = u;
 }
 
-// f(values, first index, count) over [lo, hi) of an array: whole 16-byte
-// accesses from the first aligned value on, single values before and behind
-template <typename IO, typename F1, typename FV>
-__device__ __forceinline__ void for_piece(const void* base, int64_t lo, int64_t hi, F1&& one, FV&& vec) {
-  constexpr int V = 16 / sizeof(IO);
-  const uintptr_t at = reinterpret_cast<uintptr_t>(base) + static_cast<uintptr_t>(lo) * sizeof(IO);
-  int64_t a = lo + static_cast<int64_t>(((16 - at % 16) % 16) / sizeof(IO));
-  if (a > hi) a = hi;
-  const int64_t nv = (hi - a) / V;
-  if (lo + threadIdx.x < a) one(lo + threadIdx.x);
-  for (int64_t v = threadIdx.x; v < nv; v += kThreads) vec(a + v * V);
-  const int64_t b = a + nv * V;
-  if (b + threadIdx.x < hi) one(b + threadIdx.x);
+// Walks the bytes [at, end) of an array: four(a) for kInFlight whole 16-byte
+// vectors a, a + 16 kThreads, ..., vec(a) for each of the others, one(a) for the
+// values before the first aligned vector and behind the last
+constexpr int kInFlight = 4;
+template <typename IO, typename F1, typename FV, typename F4>
+__device__ __forceinline__ void for_piece(uintptr_t at, uintptr_t end, F1&& one, FV&& vec, F4&& four) {
+  constexpr uintptr_t kStep = 16 * kThreads;
+  uintptr_t a = (at + 15) / 16 * 16;
+  if (a > end) a = end;
+  const uintptr_t b = a + (end - a) / 16 * 16, t = threadIdx.x;
+  if (at + t * sizeof(IO) < a) one(at + t * sizeof(IO));
+  uintptr_t v = a + 16 * t;
+  for (; v + (kInFlight - 1) * kStep < b; v += kInFlight * kStep) four(v);
+  for (; v < b; v += kStep) vec(v);
+  if (b + t * sizeof(IO) < end) one(b + t * sizeof(IO));
 }
 
 template <typename IO>
-__device__ __forceinline__ void add_squares(const void* base, int64_t lo, int64_t hi, double& s0, double& s1) {
-  constexpr int V = 16 / sizeof(IO);
+__device__ __forceinline__ void add_vec(const Vec<IO>& raw, double& s0, double& s1) {
+  float v[kVec<IO>];
+  unpack<IO, kVec<IO>>(raw, v);
+#pragma unroll
+  for (int k = 0; k < kVec<IO>; k += 2) {
+    s0 = fma(static_cast<double>(v[k]), static_cast<double>(v[k]), s0);
+    s1 = fma(static_cast<double>(v[k + 1]), static_cast<double>(v[k + 1]), s1);
+  }
+}
+template <typename IO>
+__device__ __forceinline__ void add_squares(uintptr_t at, uintptr_t end, double& s0, double& s1) {
   for_piece<IO>(
-      base, lo, hi,
-      [&](int64_t i) {
-        const double v = load1<IO>(base, i);
+      at, end,
+      [&](uintptr_t a) {
+        const double v = load_value<IO>(a);
         s0 = fma(v, v, s0);
       },
-      [&](int64_t i) {
-        float v[V];
-        unpack<IO, V>(load_raw<IO, V>(base, i), v);
+      [&](uintptr_t a) {
+        Vec<IO> r;
+        load_values<IO>(a, r);
+        add_vec<IO>(r, s0, s1);
+      },
+      [&](uintptr_t a) {
+        Vec<IO> r[kInFlight];
 #pragma unroll
-        for (int k = 0; k < V; k += 2) {
-          s0 = fma(static_cast<double>(v[k]), static_cast<double>(v[k]), s0);
-          s1 = fma(static_cast<double>(v[k + 1]), static_cast<double>(v[k + 1]), s1);
-        }
+        for (int i = 0; i < kInFlight; ++i) load_values<IO>(a + i * 16 * kThreads, r[i]);
+#pragma unroll
+        for (int i = 0; i < kInFlight; ++i) add_vec<IO>(r[i], s0, s1);
       });
 }
 
@@ -90,14 +171,15 @@ __device__ __forceinline__ double group_total(double v, double* red) {
 __global__ void __launch_bounds__(kThreads)
 sum_squares_kernel(TensorList l, double* part) {
   __shared__ double red[kThreads / 64];
+  __shared__ ListInLds list;
+  list.load(l);
   double s0 = 0.0, s1 = 0.0;
   const uint32_t pieces = l.first[l.count];
   for (uint32_t p = blockIdx.x; p < pieces; p += gridDim.x) {
-    const int t = tensor_of(l, p);
-    const int64_t lo = static_cast<int64_t>(p - l.first[t]) * kPieceValues;
-    const int64_t hi = lo + kPieceValues < l.size[t] ? lo + kPieceValues : l.size[t];
-    if (l.bf16_values[t]) add_squares<bf16>(l.data[t], lo, hi, s0, s1);
-    else add_squares<float>(l.data[t], lo, hi, s0, s1);
+    list.piece(p, l.count, [&](uintptr_t at, uintptr_t end, bool narrow) {
+      if (narrow) add_squares<bf16>(at, end, s0, s1);
+      else add_squares<float>(at, end, s0, s1);
+    });
   }
   const double s = group_total(s0 + s1, red);
   if (threadIdx.x == 0) part[blockIdx.x] = s;
@@ -118,16 +200,28 @@ norm_kernel(const double* part, int n, float* norm) {
 }
 
 template <typename IO>
-__device__ __forceinline__ void scale_piece(void* base, int64_t lo, int64_t hi, float f) {
-  constexpr int V = 16 / sizeof(IO);
-  for_piece<IO>(
-      base, lo, hi, [&](int64_t i) { store1<IO>(base, i, load1<IO>(base, i) * f); },
-      [&](int64_t i) {
-        float v[V];
-        unpack<IO, V>(load_raw<IO, V>(base, i), v);
+__device__ __forceinline__ Vec<IO> scaled(const Vec<IO>& raw, float f) {
+  float v[kVec<IO>];
+  unpack<IO, kVec<IO>>(raw, v);
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[k] *= f;
-        store_raw<IO, V>(base, i, pack<IO, V>(v));
+  for (int k = 0; k < kVec<IO>; ++k) v[k] *= f;
+  return pack<IO, kVec<IO>>(v);
+}
+template <typename IO>
+__device__ __forceinline__ void scale_piece(uintptr_t at, uintptr_t end, float f) {
+  for_piece<IO>(
+      at, end, [&](uintptr_t a) { store_value<IO>(a, load_value<IO>(a) * f); },
+      [&](uintptr_t a) {
+        Vec<IO> r;
+        load_values<IO>(a, r);
+        store_values<IO>(a, scaled<IO>(r, f));
+      },
+      [&](uintptr_t a) {
+        Vec<IO> r[kInFlight];
+#pragma unroll
+        for (int i = 0; i < kInFlight; ++i) load_values<IO>(a + i * 16 * kThreads, r[i]);
+#pragma unroll
+        for (int i = 0; i < kInFlight; ++i) store_values<IO>(a + i * 16 * kThreads, scaled<IO>(r[i], f));
       });
 }
 
@@ -138,31 +232,21 @@ clip_kernel(TensorList l, const double* part, int n, float max_norm, float* norm
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = v;
   const float f = max_norm / (v + 1e-6f);
   if (f >= 1.0f) return;  // a NaN goes on, into every value
+  __shared__ ListInLds list;
+  list.load(l);
   const uint32_t pieces = l.first[l.count];
   for (uint32_t q = blockIdx.x; q < pieces; q += gridDim.x) {
     const uint32_t p = pieces - 1 - q;  // the last read are the likeliest in the caches
-    const int t = tensor_of(l, p);
-    const int64_t lo = static_cast<int64_t>(p - l.first[t]) * kPieceValues;
-    const int64_t hi = lo + kPieceValues < l.size[t] ? lo + kPieceValues : l.size[t];
-    if (l.bf16_values[t]) scale_piece<bf16>(l.data[t], lo, hi, f);
-    else scale_piece<float>(l.data[t], lo, hi, f);
+    list.piece(p, l.count, [&](uintptr_t at, uintptr_t end, bool narrow) {
+      if (narrow) scale_piece<bf16>(at, end, f);
+      else scale_piece<float>(at, end, f);
+    });
   }
 }
 
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-sparc_status gn_fail(sparc_status s, const char* msg) {
-  snprintf(error_buffer(), 512, "%s", msg);
-  return s;
-}
-sparc_status gn_launched(const char* what) {
-  const hipError_t e = hipGetLastError();
-  if (e == hipSuccess) return SPARC_OK;
-  snprintf(error_buffer(), 512, "%s: %s", what, hipGetErrorString(e));
-  return SPARC_EHIP;
-}
-
 // The next list of up to kMaxTensors tensors with values, from ``at`` on; where
 // they begin again is returned
 int64_t next_list(int64_t count, void* const* data, const int64_t* sizes, const int32_t* dtypes, int64_t at,
@@ -187,17 +271,17 @@ unsigned list_groups(const TensorList& l) {
 
 sparc_status gn_check(int64_t count, void* const* data, const int64_t* sizes, const int32_t* dtypes) {
   if (count < 0 || count > (int64_t(1) << 24) || (count > 0 && (!data || !sizes || !dtypes)))
-    return gn_fail(SPARC_EINVAL, "gradient norm: bad tensor list");
+    return op_fail(SPARC_EINVAL, "gradient norm: bad tensor list");
   int64_t total = 0;
   for (int64_t i = 0; i < count; ++i) {
     if (sizes[i] < 0 || sizes[i] > (int64_t(1) << 40) - total)  // 2^26 pieces in all
-      return gn_fail(SPARC_EINVAL, "gradient norm: bad tensor size");
+      return op_fail(SPARC_EINVAL, "gradient norm: bad tensor size");
     total += sizes[i];
     if (dtypes[i] != SPARC_F32 && dtypes[i] != SPARC_BF16)
-      return gn_fail(SPARC_EINVAL, "gradient norm: unknown dtype");
-    if (sizes[i] > 0 && !data[i]) return gn_fail(SPARC_EINVAL, "gradient norm: NULL tensor");
+      return op_fail(SPARC_EINVAL, "gradient norm: unknown dtype");
+    if (sizes[i] > 0 && !data[i]) return op_fail(SPARC_EINVAL, "gradient norm: NULL tensor");
     if (reinterpret_cast<uintptr_t>(data[i]) % (dtypes[i] == SPARC_BF16 ? 2 : 4))
-      return gn_fail(SPARC_EINVAL, "gradient norm: a tensor is not aligned to its values");
+      return op_fail(SPARC_EINVAL, "gradient norm: a tensor is not aligned to its values");
   }
   return SPARC_OK;
 }
@@ -234,16 +318,16 @@ sparc_status sparc_grad_norm(int64_t count, void* const* tensors, const int64_t*
                              float* norm, void* workspace, size_t workspace_bytes, sparc_stream_t stream) {
   using namespace sparc;
   if (sparc_status s = gn_check(count, tensors, sizes, dtypes)) return s;
-  if (!norm) return gn_fail(SPARC_EINVAL, "gradient norm: NULL pointer");
+  if (!norm) return op_fail(SPARC_EINVAL, "gradient norm: NULL pointer");
   if (!workspace || workspace_bytes < sparc_grad_norm_workspace_bytes(count))
-    return gn_fail(SPARC_EWORKSPACE, "gradient norm: workspace missing or too small");
+    return op_fail(SPARC_EWORKSPACE, "gradient norm: workspace missing or too small");
   if (reinterpret_cast<uintptr_t>(workspace) % 8)
-    return gn_fail(SPARC_EINVAL, "gradient norm: the workspace must be 8-byte aligned");
+    return op_fail(SPARC_EINVAL, "gradient norm: the workspace must be 8-byte aligned");
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   double* part = static_cast<double*>(workspace);
   const int n = launch_sums(st, count, tensors, sizes, dtypes, part);
   hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(kThreads), 0, st, part, n, norm);
-  return gn_launched("gradient norm");
+  return op_launched("gradient norm");
 }
 
 sparc_status sparc_clip_grad_norm(int64_t count, void* const* tensors, const int64_t* sizes, const int32_t* dtypes,
@@ -251,12 +335,12 @@ sparc_status sparc_clip_grad_norm(int64_t count, void* const* tensors, const int
                                   sparc_stream_t stream) {
   using namespace sparc;
   if (sparc_status s = gn_check(count, tensors, sizes, dtypes)) return s;
-  if (!(max_norm >= 0.0f)) return gn_fail(SPARC_EINVAL, "gradient clipping: max_norm must be >= 0");
-  if (!norm) return gn_fail(SPARC_EINVAL, "gradient clipping: NULL pointer");
+  if (!(max_norm >= 0.0f)) return op_fail(SPARC_EINVAL, "gradient clipping: max_norm must be >= 0");
+  if (!norm) return op_fail(SPARC_EINVAL, "gradient clipping: NULL pointer");
   if (!workspace || workspace_bytes < sparc_grad_norm_workspace_bytes(count))
-    return gn_fail(SPARC_EWORKSPACE, "gradient clipping: workspace missing or too small");
+    return op_fail(SPARC_EWORKSPACE, "gradient clipping: workspace missing or too small");
   if (reinterpret_cast<uintptr_t>(workspace) % 8)
-    return gn_fail(SPARC_EINVAL, "gradient clipping: the workspace must be 8-byte aligned");
+    return op_fail(SPARC_EINVAL, "gradient clipping: the workspace must be 8-byte aligned");
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   double* part = static_cast<double*>(workspace);
   const int n = launch_sums(st, count, tensors, sizes, dtypes, part);
@@ -270,7 +354,7 @@ sparc_status sparc_clip_grad_norm(int64_t count, void* const* tensors, const int
     any = true;
   }
   if (!any) hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(kThreads), 0, st, part, 0, norm);
-  return gn_launched("gradient clipping");
+  return op_launched("gradient clipping");
 }
 
 }  // extern "C"

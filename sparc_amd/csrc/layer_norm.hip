@@ -9,16 +9,17 @@
 // from registers, so a large mean costs no precision.
 //
 // A row is held in registers by the waves that own it: one wave, or a
-// workgroup of 4 or 16 waves for wider rows, each lane NCH pieces of V
-// consecutive columns.  V is the widest access that cols and the pointers'
-// alignment allow, up to 16 bytes.  Rows too wide for that are read again for
-// each pass over them (the *_wide kernels).  The backward keeps the columns'
-// sums of dy xhat and dy in registers over the rows that its waves walk, and
-// writes one partial row per workgroup; a second kernel adds the partial rows
-// in a fixed order, so the parameters' gradients do not depend on timing.
+// workgroup of 4 or 16 waves for wider rows, each lane NCH vectors of 16 bytes
+// (at any alignment; a width that is no multiple ends in a shorter one).  Rows
+// too wide for that are read again for each pass over them (the *_wide
+// kernels).  The backward keeps the columns' sums of dy xhat and dy in
+// registers over the rows that its waves walk, beside the weight (in LDS for
+// the widest rows, whose registers are full), reads the next row while it works
+// on one, and writes one partial row per workgroup; a second kernel adds the
+// partial rows in a fixed order, so the parameters' gradients do not depend on
+// timing.
 
-#include "common.h"
-#include "sparc_hip.h"
+#include "rows.h"
 
 namespace sparc {
 namespace {
@@ -26,21 +27,6 @@ namespace {
 constexpr int kRowWaves = 4;       // forward, one wave per row: rows per workgroup (1 with few rows)
 constexpr int kBwdRowWaves = 8;    // backward, one wave per row: rows in flight per workgroup
 constexpr int64_t kFewRows = 1024; // below this a forward workgroup holds one row: one per CU before two
-
-// N values of type T into fp32, in pieces of at most 16 bytes
-template <typename T, int N>
-__device__ __forceinline__ void load_f32(const void* base, int64_t index, float (&o)[N]) {
-  if constexpr (sizeof(T) * N <= 16) {
-    unpack<T, N>(load_raw<T, N>(base, index), o);
-  } else {
-    constexpr int H = N / 2;
-    float a[H], b[H];
-    load_f32<T, H>(base, index, a);
-    load_f32<T, H>(base, index + H, b);
-#pragma unroll
-    for (int i = 0; i < H; ++i) { o[i] = a[i]; o[H + i] = b[i]; }
-  }
-}
 
 // Sums of N values over the W waves that share a row, in every lane.  red: two
 // buffers used in turn (``turn``), so that one barrier per call is enough.
@@ -66,24 +52,26 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float (*red)[N][W], int&
   }
 }
 
-template <typename IO, typename PT, int V, int NCH, int W>
+// WHOLE: D is a multiple of the vector, so that no element needs a mask
+template <typename IO, typename PT, int NCH, int W, bool WHOLE>
 __global__ void __launch_bounds__(W == 1 ? 64 * kRowWaves : 64 * W)
 layer_norm_fwd_kernel(int64_t R, int D, const void* x, const void* w, const void* b, float eps, void* y, float* mean,
                       float* rstd) {
+  constexpr int V = kVec<IO>;
   __shared__ float red[2][1][W];
   int turn = 0;
   const int t = W == 1 ? (threadIdx.x & 63) : threadIdx.x;
   const int64_t per = W == 1 ? blockDim.x >> 6 : 1;
   const int64_t first = W == 1 ? blockIdx.x * per + (threadIdx.x >> 6) : blockIdx.x;
+  const float inv_d = 1.0f / static_cast<float>(D);
   for (int64_t row = first; row < R; row += gridDim.x * per) {  // uniform over the waves of a row
     const int64_t base = row * D;
-    typename Raw<IO, V>::T raw[NCH];
+    Vec<IO> raw[NCH];
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       const int c = (k * 64 * W + t) * V;
-      if (c < D) raw[k] = load_raw<IO, V>(x, base + c);
+      if (c < D) raw[k] = load_vec<IO>(x, base + c, WHOLE ? V : D - c);
     }
-    const float inv_d = 1.0f / static_cast<float>(D);
     float s[1] = {0.0f};
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
@@ -99,11 +87,15 @@ layer_norm_fwd_kernel(int64_t R, int D, const void* x, const void* w, const void
     s[0] = 0.0f;
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      if ((k * 64 * W + t) * V < D) {
+      const int c = (k * 64 * W + t) * V;
+      if (c < D) {
         float v[V];
         unpack<IO, V>(raw[k], v);
 #pragma unroll
-        for (int i = 0; i < V; ++i) s[0] = fmaf(v[i] - mu, v[i] - mu, s[0]);
+        for (int i = 0; i < V; ++i) {
+          const float d = WHOLE || i < D - c ? v[i] - mu : 0.0f;
+          s[0] = fmaf(d, d, s[0]);
+        }
       }
     }
     row_sums<1, W>(s, red, turn);
@@ -116,76 +108,106 @@ layer_norm_fwd_kernel(int64_t R, int D, const void* x, const void* w, const void
     for (int k = 0; k < NCH; ++k) {
       const int c = (k * 64 * W + t) * V;
       if (c < D) {
+        const int n = WHOLE ? V : D - c;
         float v[V], o[V];
         unpack<IO, V>(raw[k], v);
 #pragma unroll
         for (int i = 0; i < V; ++i) o[i] = (v[i] - mu) * r;
         if (w) {
           float p[V];
-          load_f32<PT, V>(w, c, p);
+          load_f32<PT, V>(w, c, n, p);
 #pragma unroll
           for (int i = 0; i < V; ++i) o[i] *= p[i];
         }
         if (b) {
           float p[V];
-          load_f32<PT, V>(b, c, p);
+          load_f32<PT, V>(b, c, n, p);
 #pragma unroll
           for (int i = 0; i < V; ++i) o[i] += p[i];
         }
-        store_raw<IO, V>(y, base + c, pack<IO, V>(o));
+        store_vec<IO>(y, base + c, n, pack<IO, V>(o));
       }
     }
   }
 }
 
-template <typename IO, typename PT, int V, int NCH, int W>
+template <typename IO, typename PT, int NCH, int W, bool WHOLE>
 __global__ void __launch_bounds__(W == 1 ? 64 * kBwdRowWaves : 64 * W)
 layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const float* mean, const float* rstd,
                       const void* dy, void* dx, float* dw_part, float* db_part) {
+  constexpr int V = kVec<IO>;
   constexpr int kRows = W == 1 ? kBwdRowWaves : 1;  // rows a workgroup works on at once
+  constexpr int NP = V / kVec<PT>;                  // parameter vectors per vector of a row
+  constexpr bool kWeightInLds = W == 16;
+  // the next row into registers of its own while this one is worked on; with
+  // more than 16 columns per lane there are none left for it, and each vector
+  // of the next row is read once this row's is done with
+  constexpr bool kAhead = NCH * V <= 16;
   __shared__ float red[2][2][W];
+  __shared__ Vec<PT> w_lds[kWeightInLds ? NCH * 64 * W * NP : 1];
   int turn = 0;
   const int t = W == 1 ? (threadIdx.x & 63) : threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
-  using RawT = typename Raw<IO, V>::T;
-  RawT xr[NCH], dr[NCH];
+  Vec<IO> xr[NCH], dr[NCH];
+  Vec<PT> wr[kWeightInLds ? 1 : NCH][NP];
   float aw[NCH][V], ab[NCH][V];
 #pragma unroll
   for (int k = 0; k < NCH; ++k) {
+    const int c = (k * 64 * W + t) * V;
 #pragma unroll
     for (int i = 0; i < V; ++i) { aw[k][i] = 0.0f; ab[k][i] = 0.0f; }
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {  // without a weight: ones
+      float ones[kVec<PT>];
+#pragma unroll
+      for (int i = 0; i < kVec<PT>; ++i) ones[i] = 1.0f;
+      Vec<PT> p = pack<PT, kVec<PT>>(ones);
+      if (w && c < D) p = load_vec<PT>(w, c + q * kVec<PT>, WHOLE ? kVec<PT> : D - c - q * kVec<PT>);
+      if constexpr (kWeightInLds) w_lds[(k * 64 * W + t) * NP + q] = p;  // read back by this thread only
+      else wr[k][q] = p;
+    }
   }
+  const auto weight = [&](int k, float (&p)[V]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {
+      float f[kVec<PT>];
+      if constexpr (kWeightInLds) unpack<PT, kVec<PT>>(w_lds[(k * 64 * W + t) * NP + q], f);
+      else unpack<PT, kVec<PT>>(wr[k][q], f);
+#pragma unroll
+      for (int i = 0; i < kVec<PT>; ++i) p[q * kVec<PT> + i] = f[i];
+    }
+  };
   const float inv_d = 1.0f / static_cast<float>(D);
   int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + (W == 1 ? wave : 0);
-  auto load_row = [&](int64_t at, RawT (&xo)[NCH], RawT (&dyo)[NCH]) __attribute__((always_inline)) {
+  const auto load_row = [&](int64_t at, Vec<IO> (&xo)[NCH], Vec<IO> (&dyo)[NCH]) __attribute__((always_inline)) {
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       const int c = (k * 64 * W + t) * V;
       if (c < D) {
-        xo[k] = load_raw<IO, V>(x, at * D + c);
-        dyo[k] = load_raw<IO, V>(dy, at * D + c);
+        xo[k] = load_vec<IO>(x, at * D + c, WHOLE ? V : D - c);
+        dyo[k] = load_vec<IO>(dy, at * D + c, WHOLE ? V : D - c);
       }
     }
   };
   if (row < R) load_row(row, xr, dr);
   for (; row < R; row += step) {  // uniform over the waves of a row
-    RawT xn[NCH], dn[NCH];
-    if (row + step < R) load_row(row + step, xn, dn);
+    Vec<IO> xn[kAhead ? NCH : 1], dn[kAhead ? NCH : 1];
+    if constexpr (kAhead) {
+      if (row + step < R) load_row(row + step, xn, dn);
+    }
     const float mu = mean[row], r = rstd[row];
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      const int c = (k * 64 * W + t) * V;
-      if (c < D) {
+      if ((k * 64 * W + t) * V < D) {  // behind a short vector dy is zero
         float xv[V], dv[V], p[V];
         unpack<IO, V>(xr[k], xv);
         unpack<IO, V>(dr[k], dv);
-        if (w) load_f32<PT, V>(w, c, p);
+        weight(k, p);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float xh = (xv[i] - mu) * r;
-          const float g = w ? dv[i] * p[i] : dv[i];
+          const float xh = (xv[i] - mu) * r, g = dv[i] * p[i];
           s[0] += g;
           s[1] = fmaf(g, xh, s[1]);
           aw[k][i] = fmaf(dv[i], xh, aw[k][i]);
@@ -195,54 +217,57 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
     }
     row_sums<2, W>(s, red, turn);
     const float m0 = s[0] * inv_d, m1 = s[1] * inv_d;
-    if (dx) {
-#pragma unroll
-      for (int k = 0; k < NCH; ++k) {
-        const int c = (k * 64 * W + t) * V;
-        if (c < D) {
-          float xv[V], dv[V], p[V], o[V];
-          unpack<IO, V>(xr[k], xv);
-          unpack<IO, V>(dr[k], dv);
-          if (w) load_f32<PT, V>(w, c, p);
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float xh = (xv[i] - mu) * r;
-            const float g = w ? dv[i] * p[i] : dv[i];
-            o[i] = r * (fmaf(-xh, m1, g) - m0);
-          }
-          store_raw<IO, V>(dx, row * D + c, pack<IO, V>(o));
-        }
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < NCH; ++k) { xr[k] = xn[k]; dr[k] = dn[k]; }
-  }
-  // one partial row per workgroup; with a wave per row, its waves' sums are
-  // added first, wave 0, 1, 2, ...
-  auto write = [&](float (&a)[NCH][V], float* part) __attribute__((always_inline)) {
-    __shared__ float lds[W == 1 ? kBwdRowWaves - 1 : 1][64 * V];
-    float* out = part + static_cast<int64_t>(blockIdx.x) * D;
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       const int c = (k * 64 * W + t) * V;
-      if constexpr (W == 1) {
-        if (wave > 0) {
+      if (c < D) {
+        const int n = WHOLE ? V : D - c;
+        if (dx) {
+          float xv[V], dv[V], p[V], o[V];
+          unpack<IO, V>(xr[k], xv);
+          unpack<IO, V>(dr[k], dv);
+          weight(k, p);
 #pragma unroll
-          for (int i = 0; i < V; ++i) lds[wave - 1][i * 64 + t] = a[k][i];
-        }
-        __syncthreads();
-        if (wave == 0) {
-          for (int v = 0; v < kBwdRowWaves - 1; ++v) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) a[k][i] += lds[v][i * 64 + t];
+          for (int i = 0; i < V; ++i) {
+            const float xh = (xv[i] - mu) * r;
+            o[i] = r * (fmaf(-xh, m1, dv[i] * p[i]) - m0);
           }
+          store_vec<IO>(dx, row * D + c, n, pack<IO, V>(o));
+        }
+        if constexpr (kAhead) {
+          xr[k] = xn[k];
+          dr[k] = dn[k];
+        } else if (row + step < R) {
+          xr[k] = load_vec<IO>(x, (row + step) * D + c, n);
+          dr[k] = load_vec<IO>(dy, (row + step) * D + c, n);
         }
       }
-      if ((W > 1 || wave == 0) && c < D) {
+    }
+  }
+  // one partial row per workgroup; with a wave per row, its waves' sums are
+  // added first, wave 0, 1, 2, ...
+  __shared__ float4 lds[W == 1 ? kBwdRowWaves - 1 : 1][V / 4][64];
+  const auto write = [&](float (&a)[NCH][V], float* part) __attribute__((always_inline)) {
+    const int64_t out = static_cast<int64_t>(blockIdx.x) * D;
 #pragma unroll
-        for (int i = 0; i < V; ++i) out[c + i] = a[k][i];
+    for (int k = 0; k < NCH; ++k) {
+      const int c = (k * 64 * W + t) * V;
+#pragma unroll
+      for (int q = 0; q < V / 4; ++q) {
+        float4 u = make_float4(a[k][4 * q], a[k][4 * q + 1], a[k][4 * q + 2], a[k][4 * q + 3]);
+        if constexpr (W == 1) {
+          if (wave > 0) lds[wave - 1][q][t] = u;
+          __syncthreads();
+          if (wave == 0) {
+            for (int v = 0; v < kBwdRowWaves - 1; ++v) {
+              const float4 o = lds[v][q][t];
+              u.x += o.x; u.y += o.y; u.z += o.z; u.w += o.w;
+            }
+          }
+          __syncthreads();
+        }
+        if ((W > 1 || wave == 0) && c + 4 * q < D) store_vec<float>(part, out + c + 4 * q, D - c - 4 * q, u);
       }
-      if constexpr (W == 1) __syncthreads();
     }
   };
   if (dw_part) write(aw, dw_part);
@@ -325,112 +350,63 @@ layer_norm_params_wide_kernel(int64_t R, int64_t D, const void* x, const float* 
   if (db_part) db_part[blockIdx.y * D + c] = ab;
 }
 
-// out[c] = sum over the n partial rows: 64 columns by 16 slices of rows per
-// workgroup, the slices added in order.  blockIdx.y: dw, db.
-template <typename PT>
+// out[c] = sum over the n partial rows: CW columns by 1024 / CW slices of rows
+// per workgroup, the slices added in order.  blockIdx.y: dw, db.
+template <typename PT, int CW>
 __global__ void __launch_bounds__(1024)
 layer_norm_reduce_kernel(int n, int64_t D, const float* dw_part, const float* db_part, void* dw, void* db) {
-  __shared__ float red[16][64];
+  constexpr int S = 1024 / CW;
+  __shared__ float red[S][CW];
   const float* part = blockIdx.y ? db_part : dw_part;
   void* out = blockIdx.y ? db : dw;
   if (!out) return;  // uniform over the workgroup
-  const int cl = threadIdx.x & 63, slice = threadIdx.x >> 6;
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + cl;
+  const int cl = threadIdx.x & (CW - 1), slice = threadIdx.x / CW;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * CW + cl;
   float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   if (c < D) {
     int r = slice;
-    for (; r + 48 < n; r += 64) {
+    for (; r + 3 * S < n; r += 4 * S) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) a[k] += part[(r + 16 * k) * D + c];
+      for (int k = 0; k < 4; ++k) a[k] += part[(r + k * S) * D + c];
     }
-    for (; r < n; r += 16) a[0] += part[r * D + c];
+    for (; r < n; r += S) a[0] += part[r * D + c];
   }
   red[slice][cl] = (a[0] + a[1]) + (a[2] + a[3]);
   __syncthreads();
-  if (slice == 0 && c < D) {
-    float s = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) s += red[k][cl];
-    store1<PT>(out, c, s);
+  for (int h = S / 2; h > 0; h >>= 1) {
+    if (slice < h) red[slice][cl] += red[slice + h][cl];
+    __syncthreads();
   }
+  if (slice == 0 && c < D) store1<PT>(out, c, red[0][cl]);
 }
 
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-sparc_status ln_fail(sparc_status s, const char* msg) {
-  snprintf(error_buffer(), 512, "%s", msg);
-  return s;
-}
-sparc_status ln_launched(const char* what) {
-  const hipError_t e = hipGetLastError();
-  if (e == hipSuccess) return SPARC_OK;
-  snprintf(error_buffer(), 512, "%s: %s", what, hipGetErrorString(e));
-  return SPARC_EHIP;
-}
-
-// Workgroups of a launch over rows: at most 2^20, which loop (a launch holds
-// less than 2^32 threads per dimension).
-unsigned ln_grid(int64_t groups) { return static_cast<unsigned>(groups < (1 << 20) ? groups : (1 << 20)); }
-
-// Columns per access: cols has to be a multiple, and the row pointers (and the
-// parameters, 16 bytes at a time at most) aligned to it.
-int ln_vec(int64_t D, size_t es, size_t ps, const void* const* rows, int n_rows, const void* const* params,
-           int n_params) {
-  const int widest = static_cast<int>(16 / es);
-  for (int v = widest; v > 1; v = v == 8 ? 2 : 1) {
-    bool ok = D % v == 0;
-    for (int i = 0; i < n_rows; ++i) ok = ok && reinterpret_cast<uintptr_t>(rows[i]) % (v * es) == 0;
-    const size_t pa = v * ps < 16 ? v * ps : 16;
-    for (int i = 0; i < n_params; ++i) ok = ok && reinterpret_cast<uintptr_t>(params[i]) % pa == 0;
-    if (ok) return v;
-  }
-  return 1;
-}
-
-template <int N> using Int = std::integral_constant<int, N>;
-
-// f(V, NCH, W) for the narrowest form that holds a row of D columns in
-// registers: up to 16 columns per lane with 1 or 4 waves, 32 with 16 (the
+// f(NCH, W) for the narrowest form that holds a row of D columns in registers:
+// up to 16 columns per lane with 1 or 4 waves, 32 (16 in fp32) with 16 (the
 // backward holds two fp32 sums per column beside two rows of x and dy).
 // False: wider than that.
-template <int V, typename F>
-bool ln_form(int64_t D, F&& f) {
-  constexpr int P = 64 * V;  // columns per wave and piece
-  const auto fits = [&](int nch, int w) { return D <= static_cast<int64_t>(P) * nch * w; };
-  if constexpr (V >= 4) {
-    if (fits(1, 1)) f(Int<V>{}, Int<1>{}, Int<1>{});
-    else if (fits(2, 1)) f(Int<V>{}, Int<2>{}, Int<1>{});
-    else if (V == 4 && fits(3, 1)) f(Int<V>{}, Int<3>{}, Int<1>{});
-    else if (V == 4 && fits(4, 1)) f(Int<V>{}, Int<4>{}, Int<1>{});
-    else if (fits(1, 4)) f(Int<V>{}, Int<1>{}, Int<4>{});
-    else if (fits(2, 4)) f(Int<V>{}, Int<2>{}, Int<4>{});
-    else if (V == 4 && fits(4, 4)) f(Int<V>{}, Int<4>{}, Int<4>{});
-    else if (fits(1, 16)) f(Int<V>{}, Int<1>{}, Int<16>{});
-    else if (fits(2, 16)) f(Int<V>{}, Int<2>{}, Int<16>{});
-    else if (fits(3, 16)) f(Int<V>{}, Int<3>{}, Int<16>{});
-    else if (fits(4, 16)) f(Int<V>{}, Int<4>{}, Int<16>{});
-    else return false;
-  } else {
-    if (fits(4, 1)) f(Int<V>{}, Int<4>{}, Int<1>{});
-    else if (fits(8, 1)) f(Int<V>{}, Int<8>{}, Int<1>{});
-    else if (fits(4, 4)) f(Int<V>{}, Int<4>{}, Int<4>{});
-    else if (fits(8, 4)) f(Int<V>{}, Int<8>{}, Int<4>{});
-    else if (fits(4, 16)) f(Int<V>{}, Int<4>{}, Int<16>{});
-    else if (fits(8, 16)) f(Int<V>{}, Int<8>{}, Int<16>{});
-    else return false;
-  }
-  return true;
-}
 template <typename IO, typename F>
-bool ln_dispatch(int v, int64_t D, F&& f) {
-  if constexpr (sizeof(IO) == 2) {
-    if (v == 8) return ln_form<8>(D, f);
-    if (v == 2) return ln_form<2>(D, f);
-  } else {
-    if (v == 4) return ln_form<4>(D, f);
+bool ln_form(int64_t D, F&& f) {
+  constexpr int64_t P = 64 * kVec<IO>;  // columns per wave and vector
+  if (D <= P) return f(Int<1>{}, Int<1>{}), true;
+  if (D <= 2 * P) return f(Int<2>{}, Int<1>{}), true;
+  if constexpr (sizeof(IO) == 4) {
+    if (D <= 3 * P) return f(Int<3>{}, Int<1>{}), true;
+    if (D <= 4 * P) return f(Int<4>{}, Int<1>{}), true;
   }
-  return ln_form<1>(D, f);
+  if (D <= 4 * P) return f(Int<1>{}, Int<4>{}), true;
+  if (D <= 8 * P) return f(Int<2>{}, Int<4>{}), true;
+  if constexpr (sizeof(IO) == 4) {
+    if (D <= 16 * P) return f(Int<4>{}, Int<4>{}), true;
+  }
+  if (D <= 16 * P) return f(Int<1>{}, Int<16>{}), true;
+  if (D <= 32 * P) return f(Int<2>{}, Int<16>{}), true;
+  if (D <= 48 * P) return f(Int<3>{}, Int<16>{}), true;
+  if (D <= 64 * P) return f(Int<4>{}, Int<16>{}), true;
+  return false;
 }
 
 // Workgroups of the backward = partial rows: enough to fill the GPU (256 CUs
@@ -443,53 +419,68 @@ int64_t bwd_groups(int64_t R, int rows_at_once, int waves) {
 constexpr int64_t kMostPartials = 1024;  // the largest bwd_groups (W = 4)
 constexpr int64_t kWideSlices = 64;
 
+template <typename PT>
+void launch_reduce(hipStream_t st, int64_t n, int64_t D, const float* dw_part, const float* db_part, void* dw,
+                   void* db) {
+  // few columns: 16 of them per workgroup, so that more workgroups share the rows
+  if (D < 8192)
+    hipLaunchKernelGGL((layer_norm_reduce_kernel<PT, 16>), dim3(static_cast<unsigned>((D + 15) / 16), 2), dim3(1024), 0,
+                       st, static_cast<int>(n), D, dw_part, db_part, dw, db);
+  else
+    hipLaunchKernelGGL((layer_norm_reduce_kernel<PT, 64>), dim3(static_cast<unsigned>((D + 63) / 64), 2), dim3(1024), 0,
+                       st, static_cast<int>(n), D, dw_part, db_part, dw, db);
+}
+
 sparc_status ln_check(int64_t rows, int64_t cols, int32_t io, int32_t pt) {
-  if (rows < 0 || cols <= 0) return ln_fail(SPARC_EINVAL, "layer norm: rows >= 0 and cols > 0 required");
-  if (io != SPARC_F32 && io != SPARC_BF16) return ln_fail(SPARC_EINVAL, "layer norm: unknown io_dtype");
+  if (rows < 0 || cols <= 0) return op_fail(SPARC_EINVAL, "layer norm: rows >= 0 and cols > 0 required");
+  if (io != SPARC_F32 && io != SPARC_BF16) return op_fail(SPARC_EINVAL, "layer norm: unknown io_dtype");
   if (pt != SPARC_F32 && pt != io)
-    return ln_fail(SPARC_EINVAL, "layer norm: parameters are in the I/O type, or fp32 beside bf16 I/O");
+    return op_fail(SPARC_EINVAL, "layer norm: parameters are in the I/O type, or fp32 beside bf16 I/O");
   if (rows > INT32_MAX || cols > (int64_t(1) << 28) || rows > (int64_t(1) << 46) / cols)
-    return ln_fail(SPARC_EINVAL, "layer norm: too large");
+    return op_fail(SPARC_EINVAL, "layer norm: too large");
   return SPARC_OK;
 }
 
 template <typename IO, typename PT>
 sparc_status ln_forward(hipStream_t st, int64_t R, int64_t D, const void* x, const void* w, const void* b, float eps,
                         void* y, float* mean, float* rstd) {
-  const void* rows[2] = {x, y};
-  const void* params[2] = {w, b};
-  const int v = ln_vec(D, sizeof(IO), sizeof(PT), rows, 2, params, 2);
-  const bool held = ln_dispatch<IO>(v, D, [&](auto V, auto NCH, auto W) {
+  const bool held = ln_form<IO>(D, [&](auto NCH, auto W) {
     const int per = W() > 1 ? 1 : (R < kFewRows ? 1 : kRowWaves);
-    const dim3 grid(ln_grid((R + per - 1) / per)), block(64 * (W() > 1 ? W() : per));
-    hipLaunchKernelGGL((layer_norm_fwd_kernel<IO, PT, V(), NCH(), W()>), grid, block, 0, st, R, static_cast<int>(D), x,
-                       w, b, eps, y, mean, rstd);
+    const dim3 grid(op_grid((R + per - 1) / per)), block(64 * (W() > 1 ? W() : per));
+    if (D % kVec<IO> == 0)
+      hipLaunchKernelGGL((layer_norm_fwd_kernel<IO, PT, NCH(), W(), true>), grid, block, 0, st, R, static_cast<int>(D),
+                         x, w, b, eps, y, mean, rstd);
+    else
+      hipLaunchKernelGGL((layer_norm_fwd_kernel<IO, PT, NCH(), W(), false>), grid, block, 0, st, R,
+                         static_cast<int>(D), x, w, b, eps, y, mean, rstd);
   });
   if (!held)
-    hipLaunchKernelGGL((layer_norm_fwd_wide_kernel<IO, PT>), dim3(ln_grid(R)), dim3(kWideThreads), 0, st, D, x, w, b,
+    hipLaunchKernelGGL((layer_norm_fwd_wide_kernel<IO, PT>), dim3(op_grid(R)), dim3(kWideThreads), 0, st, D, x, w, b,
                        eps, y, mean, rstd, R);
-  return ln_launched("layer norm forward");
+  return op_launched("layer norm forward");
 }
 
 template <typename IO, typename PT>
 sparc_status ln_backward(hipStream_t st, int64_t R, int64_t D, const void* x, const void* w, const float* mean,
                          const float* rstd, const void* dy, void* dx, void* dw, void* db, float* ws) {
-  const void* rows[3] = {x, dy, dx};
-  const void* params[1] = {w};
-  const int v = ln_vec(D, sizeof(IO), sizeof(PT), rows, 3, params, 1);
   float* dw_part = dw ? ws : nullptr;
   float* db_part = db ? ws : nullptr;  // behind dw's partial rows where there are any
   int64_t n = 0;
-  const bool held = ln_dispatch<IO>(v, D, [&](auto V, auto NCH, auto W) {
+  const bool held = ln_form<IO>(D, [&](auto NCH, auto W) {
     const int waves = W() > 1 ? W() : kBwdRowWaves;
     n = bwd_groups(R, W() > 1 ? 1 : kBwdRowWaves, waves);
     if (dw && db) db_part = ws + n * D;
-    hipLaunchKernelGGL((layer_norm_bwd_kernel<IO, PT, V(), NCH(), W()>), dim3(static_cast<unsigned>(n)),
-                       dim3(64 * waves), 0, st, R, static_cast<int>(D), x, w, mean, rstd, dy, dx, dw_part, db_part);
+    const dim3 grid(static_cast<unsigned>(n)), block(64 * waves);
+    if (D % kVec<IO> == 0)
+      hipLaunchKernelGGL((layer_norm_bwd_kernel<IO, PT, NCH(), W(), true>), grid, block, 0, st, R, static_cast<int>(D),
+                         x, w, mean, rstd, dy, dx, dw_part, db_part);
+    else
+      hipLaunchKernelGGL((layer_norm_bwd_kernel<IO, PT, NCH(), W(), false>), grid, block, 0, st, R,
+                         static_cast<int>(D), x, w, mean, rstd, dy, dx, dw_part, db_part);
   });
   if (!held) {
     if (dx)
-      hipLaunchKernelGGL((layer_norm_dx_wide_kernel<IO, PT>), dim3(ln_grid(R)), dim3(kWideThreads), 0, st, D, x, w,
+      hipLaunchKernelGGL((layer_norm_dx_wide_kernel<IO, PT>), dim3(op_grid(R)), dim3(kWideThreads), 0, st, D, x, w,
                          mean, rstd, dy, dx, R);
     if (dw || db) {
       n = R < kWideSlices ? R : kWideSlices;
@@ -499,13 +490,10 @@ sparc_status ln_backward(hipStream_t st, int64_t R, int64_t D, const void* x, co
                          x, mean, rstd, dy, dw_part, db_part);
     }
   }
-  if (sparc_status s = ln_launched("layer norm backward")) return s;
-  if (dw || db) {
-    hipLaunchKernelGGL((layer_norm_reduce_kernel<PT>), dim3(static_cast<unsigned>((D + 63) / 64), 2), dim3(1024), 0, st,
-                       static_cast<int>(n), D, dw_part, db_part, dw, db);
-    return ln_launched("layer norm backward");
-  }
-  return SPARC_OK;
+  if (sparc_status s = op_launched("layer norm backward")) return s;
+  if (!dw && !db) return SPARC_OK;
+  launch_reduce<PT>(st, n, D, dw_part, db_part, dw, db);
+  return op_launched("layer norm backward");
 }
 
 }  // namespace
@@ -521,10 +509,10 @@ sparc_status sparc_layer_norm_forward(int64_t rows, int64_t cols, int32_t io_dty
                                       float* rstd, sparc_stream_t stream) {
   using namespace sparc;
   if (sparc_status s = ln_check(rows, cols, io_dtype, param_dtype)) return s;
-  if (!(eps >= 0.0f)) return ln_fail(SPARC_EINVAL, "layer norm forward: eps must be >= 0");
+  if (!(eps >= 0.0f)) return op_fail(SPARC_EINVAL, "layer norm forward: eps must be >= 0");
   if (rows == 0) return SPARC_OK;
   if (!x || !y || !mean != !rstd)
-    return ln_fail(SPARC_EINVAL, "layer norm forward: NULL pointer (mean and rstd come together)");
+    return op_fail(SPARC_EINVAL, "layer norm forward: NULL pointer (mean and rstd come together)");
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (io_dtype == SPARC_F32) return ln_forward<float, float>(st, rows, cols, x, weight, bias, eps, y, mean, rstd);
   if (param_dtype == SPARC_F32)
@@ -549,20 +537,15 @@ sparc_status sparc_layer_norm_backward(int64_t rows, int64_t cols, int32_t io_dt
   if (!dx && !dweight && !dbias) return SPARC_OK;
   if (rows == 0) {  // the parameters' gradients are sums over no rows
     if (!dweight && !dbias) return SPARC_OK;
-    const dim3 grid(static_cast<unsigned>((cols + 63) / 64), 2);
-    if (param_dtype == SPARC_F32)
-      hipLaunchKernelGGL((layer_norm_reduce_kernel<float>), grid, dim3(1024), 0, st, 0, cols, nullptr, nullptr, dweight,
-                         dbias);
-    else
-      hipLaunchKernelGGL((layer_norm_reduce_kernel<sparc::bf16>), grid, dim3(1024), 0, st, 0, cols, nullptr, nullptr,
-                         dweight, dbias);
-    return ln_launched("layer norm backward");
+    if (param_dtype == SPARC_F32) launch_reduce<float>(st, 0, cols, nullptr, nullptr, dweight, dbias);
+    else launch_reduce<sparc::bf16>(st, 0, cols, nullptr, nullptr, dweight, dbias);
+    return op_launched("layer norm backward");
   }
-  if (!x || !mean || !rstd || !dy) return ln_fail(SPARC_EINVAL, "layer norm backward: NULL pointer");
+  if (!x || !mean || !rstd || !dy) return op_fail(SPARC_EINVAL, "layer norm backward: NULL pointer");
   if ((dweight || dbias) && (!workspace || workspace_bytes < sparc_layer_norm_workspace_bytes(rows, cols)))
-    return ln_fail(SPARC_EWORKSPACE, "layer norm backward: workspace missing or too small");
+    return op_fail(SPARC_EWORKSPACE, "layer norm backward: workspace missing or too small");
   if (reinterpret_cast<uintptr_t>(workspace) % sizeof(float))
-    return ln_fail(SPARC_EINVAL, "layer norm backward: the workspace must be 4-byte aligned");
+    return op_fail(SPARC_EINVAL, "layer norm backward: the workspace must be 4-byte aligned");
   float* ws = static_cast<float*>(workspace);
   if (io_dtype == SPARC_F32)
     return ln_backward<float, float>(st, rows, cols, x, weight, mean, rstd, dy, dx, dweight, dbias, ws);
