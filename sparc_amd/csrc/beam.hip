@@ -19,7 +19,10 @@
 // its index, so keys are distinct and compare as (value, lower index).
 // Candidates above the list's bound are gathered in LDS; 64 at a time they are
 // sorted and merged into the list by bitonic exchanges.  The bound starts at
-// the (K + 1)-th largest of the lanes' first values, so few candidates follow.
+// the (K + 1)-th largest of the maxima of the lanes' first values, those of all
+// waves of a workgroup together where they share a row, so few candidates
+// follow: most vectors cost a maximum and a comparison beside their
+// exponentials.
 
 #include "rows.h"
 
@@ -34,11 +37,11 @@ constexpr int kMinSpan = 2048;     // logits per span at least
 constexpr int kAhead = 4;          // vectors a lane reads at once
 constexpr int kMaxPlanes = 96;     // state planes per launch: 2.3 KB of kernel arguments
 
-// Values per span: whole rounds of 64 vectors
-template <int VEC>
-__host__ __device__ __forceinline__ int64_t span_values(int64_t V, int spans) {
-  const int64_t round = 64 * VEC, rounds = (V + round - 1) / round;
-  return (rounds + spans - 1) / spans * round;
+// Vectors per span: whole rounds of 64
+template <typename IO>
+__device__ __forceinline__ int64_t span_vectors(int64_t V, int spans) {
+  const int64_t rounds = (V / kVec<IO> + 63) / 64;
+  return (rounds + spans - 1) / spans * 64;
 }
 
 // ---------------------------------------------------------------------------
@@ -101,17 +104,24 @@ __device__ __forceinline__ uint64_t exchange(uint64_t key, bool larger) {
   const uint64_t a = (static_cast<uint64_t>(ah) << 32) | al, b = (static_cast<uint64_t>(bh) << 32) | bl;
   return (b > a) == larger ? b : a;
 }
+template <int M>
+__device__ __forceinline__ uint32_t exchange(uint32_t x, bool larger) {
+  uint32_t a, b;
+  pair_words<M>(x, a, b);
+  const uint32_t most = a > b ? a : b, least = a > b ? b : a;
+  return larger ? most : least;
+}
 // a bitonic sequence of 2 M lanes into order: the larger keys to the lanes
 // whose bit M is 0 where ``down``
-template <int M>
-__device__ __forceinline__ uint64_t merge_keys(uint64_t key, int lane, bool down) {
+template <int M, typename T>
+__device__ __forceinline__ T merge_keys(T key, int lane, bool down) {
   key = exchange<M>(key, ((lane & M) == 0) == down);
   if constexpr (M > 1) key = merge_keys<M / 2>(key, lane, down);
   return key;
 }
 // the wave's 64 keys in descending (or ascending) order of the lanes
-template <bool DESCENDING, int SIZE = 64>
-__device__ __forceinline__ uint64_t sort_keys(uint64_t key, int lane) {
+template <bool DESCENDING, int SIZE = 64, typename T>
+__device__ __forceinline__ T sort_keys(T key, int lane) {
   if constexpr (SIZE > 2) key = sort_keys<DESCENDING, SIZE / 2>(key, lane);
   const bool asked = SIZE == 64 || (lane & SIZE) == 0;  // else this block of lanes the other way round
   return merge_keys<SIZE / 2>(key, lane, asked == DESCENDING);
@@ -123,28 +133,47 @@ __device__ __forceinline__ uint64_t sort_keys(uint64_t key, int lane) {
 struct TopList {
   uint64_t list;   // lane i: the i-th largest key so far, 0: none
   uint64_t bound;  // keys at or below it cannot be among the ``want`` largest
+  float low;       // nor can later values at or below it (NaN: any can)
   uint32_t held;   // candidates in the buffer (wave-uniform)
   int want;
   uint64_t* buf;   // 128 keys of LDS of this wave
 
   __device__ __forceinline__ void init(uint64_t* b, int w) {
     list = 0;
-    bound = 0;
     held = 0;
     want = w;
     buf = b;
+    set_bound(0);
   }
-  // the first keys of all lanes: ``want`` of them are at least as large as the
-  // want-th largest of the lanes' largest
-  __device__ __forceinline__ void start(uint64_t lane_largest, int lane) {
-    const uint64_t k = lane_key(sort_keys<true>(lane_largest, lane), want - 1);
-    bound = k ? k - 1 : 0;
+  __device__ __forceinline__ void set_bound(uint64_t b) {
+    bound = b;
+    const uint32_t o = static_cast<uint32_t>(b >> 32);
+    low = unordered(o == 0x7fffffffu ? o - 1 : o);  // not -0, which is not below 0
+  }
+  // largest: the ordered bits of the largest of each lane's first values (0:
+  // none).  ``want`` values at least are not below the want-th largest of them,
+  // here of the lanes of this wave and, with ``shared`` (LDS of a whole
+  // workgroup, every wave of which calls this), of the other waves.
+  __device__ __forceinline__ void start(uint32_t largest, int lane, uint32_t (*shared)[64] = nullptr, int wave = 0,
+                                        int waves = 1) {
+    uint32_t v = sort_keys<true>(largest, lane);
+    if (shared) {
+      shared[wave][lane] = v;
+      __syncthreads();
+      for (int o = 0; o < waves; ++o) {
+        if (o == wave) continue;
+        const uint32_t other = shared[o][63 - lane];
+        v = merge_keys<32>(other > v ? other : v, lane, true);  // the 64 largest of both
+      }
+    }
+    const uint64_t t = __builtin_amdgcn_readlane(v, want - 1);
+    set_bound(t ? (t << 32) - 1 : 0);
   }
   __device__ __forceinline__ void merge(uint64_t cand, int lane) {
     cand = sort_keys<false>(cand, lane);
     list = merge_keys<32>(list > cand ? list : cand, lane, true);  // the 64 largest of both, bitonic
     const uint64_t b = lane_key(list, want - 1);
-    if (b > bound) bound = b;
+    if (b > bound) set_bound(b);
   }
   // a key per lane, 0: none; every lane of the wave calls it
   __device__ __forceinline__ void push(uint64_t key, int lane) {
@@ -176,111 +205,173 @@ struct TopList {
 // ---------------------------------------------------------------------------
 // the scan of the logits
 // ---------------------------------------------------------------------------
-// A row in vectors of 16 bytes, at any alignment of its values
+// Value i of a vector, i differing between lanes (an array indexed by it would
+// go through memory)
+template <typename IO>
+__device__ __forceinline__ float pick(const Vec<IO>& r, int i) {
+  if constexpr (sizeof(IO) == 4) {
+    const float a = i & 1 ? r.y : r.x, b = i & 1 ? r.w : r.z;
+    return i & 2 ? b : a;
+  } else {
+    const uint32_t a = i & 2 ? r.y : r.x, b = i & 2 ? r.w : r.z, c = i & 4 ? b : a;
+    return __uint_as_float(i & 1 ? c & 0xffff0000u : c << 16);
+  }
+}
+
+// A row of V logits in whole vectors of 16 bytes, at any alignment, and the
+// V % VEC values behind them.
 template <typename IO>
 struct Row {
+  static constexpr int VEC = kVec<IO>;
   const void* logits;
   int64_t offset, V;
 
-  // the values from ``at`` on, -inf behind the row
-  __device__ __forceinline__ void load(int64_t at, float (&x)[kVec<IO>]) const {
-    const int64_t left = V - at;
-    if (left >= kVec<IO>) {
-      unpack<IO, kVec<IO>>(load_vec<IO>(logits, offset + at, kVec<IO>), x);
+  __device__ __forceinline__ int64_t vectors() const { return V / VEC; }
+  __device__ __forceinline__ Vec<IO> load(int64_t j) const { return load_vec<IO>(logits, offset + j * VEC, VEC); }
+  // the values behind the vectors, one per lane, -inf in the other lanes
+  __device__ __forceinline__ float rest(int lane, int64_t& at) const {
+    at = vectors() * VEC + lane;
+    return at < V ? load1<IO>(logits, offset + at) : -INFINITY;
+  }
+  // Those of a vector's values that may pass the list's bound into the list, by
+  // make(value); ``in``: this lane has a vector; ``all``: every value.  Few
+  // lanes hold any such value, so every turn takes one from each lane that does,
+  // not one place of all lanes.
+  template <typename F>
+  __device__ __forceinline__ void push(TopList& top, bool in, int64_t j, const Vec<IO>& raw, bool all, int lane,
+                                       F&& make) const {
+    uint32_t pass = 0;
+    {
+      float x[VEC];
+      unpack<IO, VEC>(raw, x);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) pass |= in && (all || !(x[i] <= top.low)) ? 1u << i : 0u;
+    }
+    while (__any(pass != 0)) {
+      const int i = __ffs(static_cast<int>(pass)) - 1;
+      top.push(pass ? make_key(make(pick<IO>(raw, i)), static_cast<uint32_t>(j * VEC + i)) : 0, lane);
+      pass &= pass - 1;
+    }
+  }
+};
+
+constexpr float kLog2E = 1.4426950408889634f;       // rounded to fp32
+constexpr float kLog2ELow = 1.9259629911e-8f;       // and what is left of it
+constexpr float kHuge = 1e38f;                      // beyond it x log2(e) may overflow
+
+// A lane's maximum m and sum s of 2^(x log2(e) - m log2(e)), the product of m
+// rounded: one fused multiply-add and one exponential per value.
+struct SumExp {
+  float m, s;
+
+  // ``in``: the values count
+  template <int N>
+  __device__ __forceinline__ void add(const float (&x)[N], float big, bool in) {
+#pragma clang fp contract(off)  // m log2(e) rounds the same way each time it is formed
+    const float mn = in ? fmaxf(m, big) : m;
+    const float ref = mn == -INFINITY ? 0.0f : mn;  // nothing but -inf so far: every power is 0
+    float sum = 0.0f;
+    if (__any(fabsf(ref) > kHuge)) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) sum += fast_exp(x[i] - ref);
+      s = fmaf(s, fast_exp(m - ref), in ? sum : 0.0f);
     } else {
+      const float r = ref * kLog2E;
 #pragma unroll
-      for (int i = 0; i < kVec<IO>; ++i) x[i] = i < left ? load1<IO>(logits, offset + at + i) : -INFINITY;
+      for (int i = 0; i < N; ++i) sum += __builtin_amdgcn_exp2f(fmaf(x[i], kLog2E, -r));
+      s = fmaf(s, __builtin_amdgcn_exp2f(m * kLog2E - r), in ? sum : 0.0f);
     }
+    m = mn;
   }
-  // the keys of the values from ``at`` on into the list, by make(value)
-  template <typename F>
-  __device__ __forceinline__ void push(TopList& top, int64_t at, const float (&x)[kVec<IO>], int lane, F&& make) const {
+  // The maximum over the wave, and the sum of e^(x - maximum) over it: the
+  // maximum's product with log2(e) is taken to twice fp32's precision here, so
+  // that what the lanes' products were rounded by does not stay in the sum.
+  __device__ __forceinline__ void join(float& all, float& sum) const {
+#pragma clang fp contract(off)
+    all = m;
 #pragma unroll
-    for (int i = 0; i < kVec<IO>; ++i)
-      top.push(at + i < V ? make_key(make(x[i]), static_cast<uint32_t>(at + i)) : 0, lane);
-  }
-  template <typename F>
-  __device__ __forceinline__ uint64_t largest(uint64_t k, int64_t at, const float (&x)[kVec<IO>], F&& make) const {
-#pragma unroll
-    for (int i = 0; i < kVec<IO>; ++i) {
-      const uint64_t key = at + i < V ? make_key(make(x[i]), static_cast<uint32_t>(at + i)) : 0;
-      k = key > k ? key : k;
+    for (int o = 32; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor(all, o));
+    const float ref = all == -INFINITY ? 0.0f : all;
+    float f;
+    if (fabsf(ref) > kHuge) {
+      f = fast_exp(m - ref);
+    } else {
+      const float r = ref * kLog2E;
+      f = __builtin_amdgcn_exp2f((m * kLog2E - r) - fmaf(ref, kLog2ELow, fmaf(ref, kLog2E, -r)));
     }
-    return k;
+    sum = group_sum(m == -INFINITY ? s : s * f, 64);  // s: 0, or NaN
   }
 };
 
 // parts: [rows][spans] (maximum, sum of exp(x - maximum)); tops: [rows][spans][want] keys
 template <typename IO>
-__global__ void __launch_bounds__(64 * kScanWaves)
+__global__ void __launch_bounds__(64 * kScanWaves, 4)
 beam_scan_kernel(int64_t rows, int64_t V, int64_t ld, int spans, int want, const void* logits, float2* parts,
                  uint64_t* tops) {
   __shared__ uint64_t buf[kScanWaves][128];
+  __shared__ uint32_t first[kScanWaves][64];
   constexpr int VEC = kVec<IO>;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t job = static_cast<int64_t>(blockIdx.x) * kScanWaves + wave;
-  if (job >= rows * spans) return;  // no workgroup barrier below
+  const bool together = spans % kScanWaves == 0;  // the workgroup's waves share a row: they meet once
+  if (job >= rows * spans) return;                // not where they do
   const int64_t r = job / spans;
   const int span = static_cast<int>(job - r * spans);
   const Row<IO> row{logits, r * ld, V};
-  const int64_t begin = span * span_values<VEC>(V, spans);
-  int64_t end = begin + span_values<VEC>(V, spans);
-  end = end < V ? end : V;
+  const int64_t per = span_vectors<IO>(V, spans), begin = span * per;
+  const int64_t end = begin + per < row.vectors() ? begin + per : row.vectors();
   TopList top;
   top.init(buf[wave], want);
   const auto same = [](float v) { return v; };
-  float m = -INFINITY, s = 0.0f;
-  for (int64_t at0 = begin; at0 < end; at0 += kAhead * 64 * VEC) {  // spans are whole numbers of 64 vectors
-    float x[kAhead][VEC], big[kAhead];
+  SumExp acc{-INFINITY, 0.0f};
+  // Loads past the span's end repeat its last vector: without a branch around
+  // them the wave waits for the one it needs, not for all that it has issued.
+  const auto load = [&](int64_t j) { return row.load(j < end ? j : end - 1); };
+  Vec<IO> raw[kAhead] = {};
+  if (begin < end) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) raw[u] = load(begin + u * 64 + lane);
+  }
+  uint32_t largest = 0;
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) {
+    float x[VEC], big;
+    unpack<IO, VEC>(raw[u], x);
+    big = x[0];
+#pragma unroll
+    for (int i = 1; i < VEC; ++i) big = fmaxf(big, x[i]);
+    const uint32_t o = begin + u * 64 + lane < end ? ordered(big) : 0;
+    largest = o > largest ? o : largest;
+  }
+  top.start(largest, lane, together ? first : nullptr, wave, kScanWaves);
+  for (int64_t j0 = begin; j0 < end; j0 += kAhead * 64) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int64_t at = at0 + (u * 64 + lane) * VEC;
-      if (at0 + u * 64 * VEC < end) {
-        row.load(at, x[u]);
-      } else {
+      const int64_t j = j0 + u * 64 + lane;
+      const bool in = j < end;
+      const Vec<IO> now = raw[u];
+      // the vector of the next round, while this one is worked on
+      raw[u] = load(j + kAhead * 64);
+      float x[VEC];
+      unpack<IO, VEC>(now, x);
+      float big = x[0];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) x[u][i] = -INFINITY;
-      }
+      for (int i = 1; i < VEC; ++i) big = fmaxf(big, x[i]);
+      if (__any(in && !(big <= top.low))) row.push(top, in, j, now, false, lane, same);
+      acc.add(x, big, in);
     }
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      big[u] = x[u][0];
-#pragma unroll
-      for (int i = 1; i < VEC; ++i) big[u] = fmaxf(big[u], x[u][i]);
-    }
-    if (at0 == begin) {
-      uint64_t k = 0;
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (at0 + u * 64 * VEC < end) k = row.largest(k, at0 + (u * 64 + lane) * VEC, x[u], same);
-      top.start(k, lane);
-    }
-    float mn = m;
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      mn = fmaxf(mn, big[u]);
-      // seldom: a value of some lane may pass the bound
-      if (at0 + u * 64 * VEC < end && __any(!(big[u] < key_value(top.bound))))
-        row.push(top, at0 + (u * 64 + lane) * VEC, x[u], lane, same);
-    }
-    const float ref = mn == -INFINITY ? 0.0f : mn;  // nothing but -inf so far: exp gives 0
-    float add = 0.0f;
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      float e = 0.0f;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) e += fast_exp(x[u][i] - ref);
-      add += e;
-    }
-    s = fmaf(s, fast_exp(m - ref), add);
-    m = mn;
+  }
+  if (span == spans - 1 && V % VEC != 0) {
+    int64_t at;
+    const float x = row.rest(lane, at);
+    top.push(at < V ? make_key(x, static_cast<uint32_t>(at)) : 0, lane);
+    const float one[1] = {x};
+    acc.add(one, x, true);
   }
   top.finish(lane);
-  float all = m;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor(all, o));
-  s = group_sum(s * fast_exp(m - (all == -INFINITY ? 0.0f : all)), 64);
-  if (lane == 0) parts[job] = make_float2(all, s);
+  float all, sum;
+  acc.join(all, sum);
+  if (lane == 0) parts[job] = make_float2(all, sum);
   if (lane < want) tops[job * want + lane] = top.list;
 }
 
@@ -348,7 +439,7 @@ beam_join_kernel(BeamStep p) {
         const uint64_t* tops = p.tops + r * n;
         for (int i0 = 0; i0 < n; i0 += 64) {
           const uint64_t key = i0 + lane < n ? tops[i0 + lane] : 0;
-          if (i0 == 0) top.start(key, lane);
+          if (i0 == 0) top.start(static_cast<uint32_t>(key >> 32), lane);
           top.push(key, lane);
         }
         top.finish(lane);
@@ -361,13 +452,15 @@ beam_join_kernel(BeamStep p) {
         if (again) {
           const Row<IO> row{p.logits, (b * K + k) * p.ld, p.V};
           top.init(buf[wave], keep);
-          for (int64_t at0 = 0; at0 < p.V; at0 += 64 * kVec<IO>) {
-            float x[kVec<IO>];
-            const int64_t at = at0 + lane * kVec<IO>;
-            row.load(at, x);
-            if (at0 == 0) top.start(row.largest(0, at, x, score), lane);
-            row.push(top, at, x, lane, score);
+          for (int64_t j0 = 0; j0 < row.vectors(); j0 += 64) {
+            const bool in = j0 + lane < row.vectors();
+            Vec<IO> raw = {};
+            if (in) raw = row.load(j0 + lane);
+            row.push(top, in, j0 + lane, raw, true, lane, score);
           }
+          int64_t at;
+          const float x = row.rest(lane, at);
+          top.push(at < p.V ? make_key(score(x), static_cast<uint32_t>(at)) : 0, lane);
           top.finish(lane);
           if (lane < keep) mine = make_key(key_value(top.list), flat + key_index(top.list));
         } else if (lane < keep) {
@@ -384,7 +477,7 @@ beam_join_kernel(BeamStep p) {
   const int n = K * (K + 1);
   for (int i0 = 0; i0 < n; i0 += 64) {
     const uint64_t key = i0 + lane < n ? cand[i0 + lane] : 0;
-    if (i0 == 0) top.start(key, lane);
+    if (i0 == 0) top.start(static_cast<uint32_t>(key >> 32), lane);
     top.push(key, lane);
   }
   top.finish(lane);
@@ -487,12 +580,14 @@ sparc_status bm_check(int64_t batch, int64_t beams, int64_t vocab) {
     return op_fail(SPARC_EINVAL, "beam step: too large");
   return SPARC_OK;
 }
-// Spans per row: about 8192 waves in all (32 per CU), none shorter than kMinSpan
+// Spans per row: about 4096 waves in all (16 per CU, what their registers
+// allow), none shorter than kMinSpan
 int spans_of(int64_t rows, int64_t vocab) {
-  int64_t s = 8192 / (rows > 0 ? rows : 1);
+  int64_t s = 4096 / (rows > 0 ? rows : 1);
   const int64_t most = (vocab + kMinSpan - 1) / kMinSpan;
   s = s < most ? s : most;
-  return static_cast<int>(s < 1 ? 1 : (s < kMaxSpans ? s : kMaxSpans));
+  s = s < 1 ? 1 : (s < kMaxSpans ? s : kMaxSpans);
+  return static_cast<int>(s < kScanWaves ? s : s / kScanWaves * kScanWaves);  // whole workgroups per row
 }
 
 template <int B>

@@ -61,13 +61,6 @@ embed_fwd_kernel(int64_t N, int64_t vocab, int D, int lpr, int blocks, const voi
 // ---------------------------------------------------------------------------
 // the sort
 // ---------------------------------------------------------------------------
-// The key of a position: its id, or vocab (behind every row) where it takes no
-// part in the gradient.
-__device__ __forceinline__ uint32_t token_key(const void* tokens, int wide_ids, int64_t n, int64_t vocab, int64_t pad) {
-  const int64_t id = wide_ids ? static_cast<const int64_t*>(tokens)[n] : static_cast<const int32_t*>(tokens)[n];
-  return static_cast<uint32_t>(id >= 0 && id < vocab && id != pad ? id : vocab);
-}
-
 struct SortPass {
   const void* tokens;     // the first pass reads ids, later ones keys
   int wide_ids;
@@ -81,6 +74,32 @@ struct SortPass {
   int64_t n;
   int shift, bits;
   int first, last;
+
+  // The keys of ITEMS positions from ``at`` on, ``step`` apart, all read at
+  // once.  A key is the position's id, or vocab (behind every row) where it
+  // takes no part in the gradient; past the end it repeats the last one's.
+  template <int ITEMS>
+  __device__ __forceinline__ void load_keys(int64_t at, int64_t step, uint32_t (&key)[ITEMS]) const {
+    int64_t i[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) i[k] = at + k * step < n ? at + k * step : n - 1;
+    if (!first) {
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k) key[k] = keys_in[i[k]];
+      return;
+    }
+    int64_t id[ITEMS];
+    if (wide_ids) {
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k) id[k] = static_cast<const int64_t*>(tokens)[i[k]];
+    } else {
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k) id[k] = static_cast<const int32_t*>(tokens)[i[k]];
+    }
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+      key[k] = static_cast<uint32_t>(id[k] >= 0 && id[k] < vocab && id[k] != pad ? id[k] : vocab);
+  }
 };
 
 // Digit counts of each tile of kSortThreads * ITEMS positions
@@ -96,14 +115,13 @@ sort_count_kernel(SortPass p) {
       p.touched[v] = 0;
   }
   __syncthreads();
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * (kSortThreads * ITEMS);
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * (kSortThreads * ITEMS) + threadIdx.x;
+  if (p.n > 0) {
+    uint32_t key[ITEMS];
+    p.load_keys<ITEMS>(base, kSortThreads, key);
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
-    const int64_t n = base + i * kSortThreads + threadIdx.x;
-    if (n < p.n) {
-      const uint32_t key = p.first ? token_key(p.tokens, p.wide_ids, n, p.vocab, p.pad) : p.keys_in[n];
-      atomicAdd(&hist[(key >> p.shift) & (digits - 1)], 1u);
-    }
+    for (int i = 0; i < ITEMS; ++i)
+      if (base + i * kSortThreads < p.n) atomicAdd(&hist[(key[i] >> p.shift) & (digits - 1)], 1u);
   }
   __syncthreads();
   for (int d = threadIdx.x; d < digits; d += kSortThreads) p.counts[static_cast<int64_t>(blockIdx.x) * digits + d] = hist[d];
@@ -121,6 +139,16 @@ sort_scatter_kernel(SortPass p) {
   __shared__ uint32_t wsum[kSortWaves];
   const int digits = 1 << p.bits;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kSortThreads * ITEMS) + wave * (64 * ITEMS) + lane;
+  if (p.n == 0) return;  // the whole launch
+  uint32_t key[ITEMS], pos[ITEMS];
+  p.load_keys<ITEMS>(first, 64, key);
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int64_t n = first + i * 64 < p.n ? first + i * 64 : p.n - 1;
+    pos[i] = static_cast<uint32_t>(n);
+    if (!p.first) pos[i] = p.pos_in[n];
+  }
   for (int d = threadIdx.x; d < digits; d += kSortThreads) {
 #pragma unroll
     for (int w = 0; w < kSortWaves; ++w) cnt[w][d] = 0;
@@ -162,13 +190,7 @@ sort_scatter_kernel(SortPass p) {
     if (d < digits) start[d] = base + before[k];
     base += total[k];
   }
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kSortThreads * ITEMS) + wave * (64 * ITEMS) + lane;
-  uint32_t key[ITEMS], rank[ITEMS];
-#pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
-    const int64_t n = first + i * 64;
-    key[i] = n < p.n ? (p.first ? token_key(p.tokens, p.wide_ids, n, p.vocab, p.pad) : p.keys_in[n]) : 0u;
-  }
+  uint32_t rank[ITEMS];
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
     const bool valid = first + i * 64 < p.n;
@@ -202,7 +224,7 @@ sort_scatter_kernel(SortPass p) {
     if (n < p.n) {
       const uint32_t to = cnt[wave][(key[i] >> p.shift) & (digits - 1)] + rank[i];
       p.keys_out[to] = key[i];
-      p.pos_out[to] = p.first ? static_cast<uint32_t>(n) : p.pos_in[n];
+      p.pos_out[to] = pos[i];
       if (p.last && key[i] < static_cast<uint32_t>(p.vocab)) p.touched[key[i]] = 1;
     }
   }
@@ -327,9 +349,9 @@ embed_join_kernel(int64_t N, int64_t vocab, int D, const uint32_t* keys, float s
     uint32_t key = kNone;
     if (begins) {
       key = keys[p1 - 1];
+      const uint32_t next = keys[p1], own = keys[p0], before = keys[p0 > 0 ? p0 - 1 : 0];  // read together
       // it crosses, and does not come from an earlier piece
-      begins = key < static_cast<uint32_t>(vocab) && keys[p1] == key &&
-               !(p0 > 0 && keys[p0] == key && keys[p0 - 1] == key);
+      begins = key < static_cast<uint32_t>(vocab) && next == key && !(p0 > 0 && own == key && before == key);
     }
     int64_t last = piece;
     if (begins) {
@@ -413,7 +435,7 @@ Sort sort_of(int64_t n, int64_t vocab) {
   while ((vocab >> s.bits) > 0) ++s.bits;  // keys 0 .. vocab
   s.passes = (s.bits + 8) / 9;
   s.digit_bits = (s.bits + s.passes - 1) / s.passes;
-  s.items = n <= 65536 ? 8 : 32;  // at most 32 tiles' counts to add up, then tiles four times the size
+  s.items = n <= 65536 ? 4 : 16;  // at most 64 tiles' counts to add up, then tiles four times the size
   s.tiles = (n + kSortThreads * s.items - 1) / (kSortThreads * s.items);
   if (s.tiles < 1) s.tiles = 1;  // without tokens, one tile clears the flags
   return s;
@@ -531,8 +553,8 @@ sparc_status sparc_embedding_backward(int64_t n, int64_t vocab, int64_t dim, int
     p.bits = s.digit_bits;
     p.first = k == 0;
     p.last = k == s.passes - 1;
-    if (s.items == 8) em_sort_pass<8>(st, s.tiles, p);
-    else em_sort_pass<32>(st, s.tiles, p);
+    if (s.items == 4) em_sort_pass<4>(st, s.tiles, p);
+    else em_sort_pass<16>(st, s.tiles, p);
     cur ^= 1;
   }
   if (io_dtype == SPARC_F32) em_sums<float>(st, n, vocab, dim, keys[cur ^ 1], pos[cur ^ 1], touched, dy, scale, part, dweight);

@@ -16,7 +16,7 @@
 namespace sparc {
 namespace {
 
-constexpr int kMaxTensors = 128;      // per launch: 2.7 KB of kernel arguments
+constexpr int kMaxTensors = 160;      // per launch: 3.4 KB of kernel arguments
 constexpr int kPieceValues = 16384;
 constexpr int kMaxGroups = 1024;      // partial sums per launch
 constexpr int kThreads = 256;
