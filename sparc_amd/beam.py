@@ -33,6 +33,35 @@ def _like(states, planes):
     return [type(s)(next(at) for _ in s) if isinstance(s, (tuple, list)) else next(at) for s in states]
 
 
+def _fresh(planes):
+    """Contiguous tensors of the planes' shapes and dtypes: neighbours of one
+    shape share an allocation."""
+    out, i = [], 0
+    while i < len(planes):
+        shape, dtype, n = planes[i].shape, planes[i].dtype, 1
+        while i + n < len(planes) and planes[i + n].shape == shape and planes[i + n].dtype == dtype:
+            n += 1
+        out += torch.empty(n, *shape, dtype=dtype, device=planes[i].device).unbind(0)
+        i += n
+    return out
+
+
+def _check_out(planes, out):
+    if len(out) != len(planes):
+        raise ValueError(f"out_states has {len(out)} tensors for {len(planes)} states")
+    place = {}
+    for i, (o, p) in enumerate(zip(out, planes)):
+        if o is not p:
+            _lib.expect(o, p.shape, p.dtype, "out_states")
+        if not o.is_contiguous():
+            raise ValueError("out_states must be contiguous tensors")
+        if o.numel() and place.setdefault(o.data_ptr(), i) != i:
+            raise ValueError("two tensors of out_states are the same")
+    for i, p in enumerate(planes):
+        if place.get(p.data_ptr(), i) != i:
+            raise ValueError("a tensor of out_states is another one of the states")
+
+
 @torch.no_grad()
 def reorder_states(states: Sequence, parents: torch.Tensor, out_states: Sequence | None = None) -> list:
     """Every tensor's row b * K + k replaced by its row b * K + parents[b, k].
@@ -41,45 +70,37 @@ def reorder_states(states: Sequence, parents: torch.Tensor, out_states: Sequence
     ``SPARCMixer.step``, in a list; ``parents``: [B, K] int64, K up to 32.
     ``out_states``: the same structure to write to; it may be ``states`` itself
     (in place: rows that stay are neither read nor written), but no tensor of it
-    may overlap another of the states.  By default fresh tensors are returned.
-    A parent outside [0, K) gives a row of NaN."""
-    planes = _planes(states)
+    may overlap another of the states.  By default fresh tensors are returned;
+    those of one shape and dtype share an allocation.  A parent outside [0, K)
+    gives a row of NaN."""
     if parents.ndim != 2 or parents.dtype != torch.int64 or not 1 <= parents.shape[1] <= MAX_BEAMS:
         raise ValueError(f"parents must be [B, K] int64 with K from 1 to {MAX_BEAMS}, got {list(parents.shape)} "
                          f"{parents.dtype}")
+    return _reorder(states, parents.contiguous(), out_states)
+
+
+def _reorder(states, parents, out_states):
     B, K = parents.shape
+    planes = _planes(states)
+    rows = B * K
     for p in planes:
-        if p.ndim < 1 or p.shape[0] != B * K:
-            raise ValueError(f"states must have {B * K} rows (one per beam), got {list(p.shape)}")
+        if p.ndim < 1 or p.shape[0] != rows:
+            raise ValueError(f"states must have {rows} rows (one per beam), got {list(p.shape)}")
     dev = _lib.require_gpu(parents, *planes)
     if out_states is None:
-        out = [torch.empty_like(p, memory_format=torch.contiguous_format) for p in planes]
+        out = _fresh(planes)
     else:
         out = _planes(out_states)
-        if len(out) != len(planes):
-            raise ValueError(f"out_states has {len(out)} tensors for {len(planes)} states")
-        _lib.require_gpu(parents, *out)
-        place = {}
-        for o, p in zip(out, planes):
-            _lib.expect(o, p.shape, p.dtype, "out_states")
-            if not o.is_contiguous():
-                raise ValueError("out_states must be contiguous tensors")
-        for i, o in enumerate(out):
-            if o.numel() and place.setdefault(o.data_ptr(), i) != i:
-                raise ValueError("two tensors of out_states are the same")
-        for i, p in enumerate(planes):
-            if place.get(p.data_ptr(), i) != i:
-                raise ValueError("a tensor of out_states is another one of the states")
+        _check_out(planes, out)
+        if out_states is not states:
+            _lib.require_gpu(parents, *out)
     planes = [p.contiguous() for p in planes]
-    src, dst, row_bytes = array("Q"), array("Q"), array("q")
-    for p, o in zip(planes, out):
-        n = p.numel() // (B * K) * p.element_size() if B else 0
-        if n % 2:
+    row_bytes = [p.numel() // rows * p.element_size() for p in planes] if rows else [0] * len(planes)
+    for n in row_bytes:
+        if n & 1:
             raise ValueError("state rows must have an even number of bytes")
-        src.append(p.data_ptr())
-        dst.append(o.data_ptr())
-        row_bytes.append(n)
-    parents = parents.contiguous()
+    src, dst = array("Q", [p.data_ptr() for p in planes]), array("Q", [o.data_ptr() for o in out])
+    row_bytes = array("q", row_bytes)
     _lib.check(_lib.load().sparc_reorder_states(
         B, K, len(planes), src.buffer_info()[0], dst.buffer_info()[0], row_bytes.buffer_info()[0],
         parents.data_ptr(), _lib.stream_of(dev)), "sparc_reorder_states")
@@ -133,7 +154,7 @@ def beam_search_step(logits: torch.Tensor, scores: torch.Tensor, finished: torch
         B, K, V, stride, io, logits.data_ptr(), P(scores), P(finished), -1 if eos_id is None else eos_id, P(tokens),
         P(parents), P(new_scores), P(new_finished), P(ws), need, _lib.stream_of(dev)), "sparc_beam_step")
     if len(states):
-        states = reorder_states(states, parents, out_states)
+        states = _reorder(states, parents, out_states)
     return BeamStep(tokens, parents, new_scores, new_finished, list(states))
 
 

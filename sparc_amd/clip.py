@@ -42,30 +42,27 @@ def _call(fn_name, tensors, *args):
     once); the norm, [] float32."""
     lib = _lib.load()
     dev = _lib.require_gpu(*tensors)
-    seen, data, sizes, codes = set(), array("Q"), array("q"), array("i")
-    for t in tensors:
-        at = t.data_ptr()
-        if at in seen:
-            continue
-        seen.add(at)
-        data.append(at)
-        sizes.append(t.numel())
-        codes.append(_CODES[t.dtype])
+    data = [t.data_ptr() for t in tensors]
+    if len(set(data)) != len(data):
+        once = dict(zip(data, tensors))
+        data, tensors = list(once), list(once.values())
+    n = len(data)
+    sizes, codes = array("q", [t.numel() for t in tensors]), array("i", [_CODES[t.dtype] for t in tensors])
+    data = array("Q", data)
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    need = lib.sparc_grad_norm_workspace_bytes(len(data))
+    need = lib.sparc_grad_norm_workspace_bytes(n)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    _lib.check(getattr(lib, fn_name)(len(data), data.buffer_info()[0], sizes.buffer_info()[0], codes.buffer_info()[0],
-                                     *args, norm.data_ptr(), ws.data_ptr(), need, _lib.stream_of(dev)), fn_name)
+    _lib.check(getattr(lib, fn_name)(n, data.buffer_info()[0], sizes.buffer_info()[0], codes.buffer_info()[0], *args,
+                                     norm.data_ptr(), ws.data_ptr(), need, _lib.stream_of(dev)), fn_name)
     return norm
 
 
 def _checked(tensors):
-    tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
     for t in tensors:
-        if t.layout != torch.strided:
-            raise ValueError(f"gradients must be dense tensors, got layout {t.layout}")
         if t.dtype not in _CODES:
             raise TypeError(f"SPARC HIP kernels take float32 or bfloat16 tensors, got {t.dtype}")
+        if t.layout is not torch.strided:
+            raise ValueError(f"gradients must be dense tensors, got layout {t.layout}")
     return tensors
 
 
@@ -73,6 +70,7 @@ def grad_norm(tensors) -> torch.Tensor:
     """The L2 norm over all values of ``tensors`` (one or several, float32 and
     bfloat16 mixed, any shapes), a float32 scalar on their device.  Squares are
     summed in fp64 in a fixed order: no overflow, equal calls give equal bits."""
+    tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
     tensors = [t if _dense(t) else t.contiguous() for t in _checked(tensors)]
     return _call("sparc_grad_norm", tensors) if tensors else torch.zeros(())
 
@@ -91,12 +89,12 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     if math.isnan(max_norm) or max_norm < 0.0:
         raise ValueError(f"clip_grad_norm_ needs max_norm >= 0, got {max_norm}")
     parameters = [parameters] if torch.is_tensor(parameters) else parameters
-    grads = _checked([p.grad for p in parameters if p.grad is not None])
+    grads = _checked([g for g in [p.grad for p in parameters] if g is not None])
     if not grads:
         return torch.zeros(())
     copies = []
     for i, g in enumerate(grads):
-        if not _dense(g):
+        if not (g.is_contiguous() or _dense(g)):
             if _repeats(g):
                 raise ValueError("a gradient names one value more than once (an expanded view): it cannot be scaled "
                                  "in place")

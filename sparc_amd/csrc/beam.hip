@@ -227,7 +227,7 @@ struct Row {
   int64_t offset, V;
 
   __device__ __forceinline__ int64_t vectors() const { return V / VEC; }
-  __device__ __forceinline__ Vec<IO> load(int64_t j) const { return load_vec<IO>(logits, offset + j * VEC, VEC); }
+  __device__ __forceinline__ Vec<IO> load(int64_t j) const { return load_vec<IO, true>(logits, offset + j * VEC, VEC); }
   // the values behind the vectors, one per lane, -inf in the other lanes
   __device__ __forceinline__ float rest(int lane, int64_t& at) const {
     at = vectors() * VEC + lane;

@@ -95,23 +95,26 @@ __device__ __forceinline__ void store_value(uintptr_t at, float v) {
   if constexpr (sizeof(IO) == 4) *p = v;
   else *p = pack_bf16(v);
 }
+// Both passes stream the values (non-temporal): 0.9 GB are read at 6.6 TB/s
+// instead of 4.4, and the whole call takes 453 instead of 521 us; 512 MB 283
+// instead of 334, 32 MB 45 instead of 49.  Only values that lie in the
+// memory-side cache already are scaled faster without (128 MB: 86 against 101).
 template <typename IO>
 __device__ __forceinline__ void load_values(uintptr_t at, Vec<IO>& v) {
-  const auto u = *reinterpret_cast<const typename GlobalTypes<IO>::Four*>(at);
+  const auto u = __builtin_nontemporal_load(reinterpret_cast<const typename GlobalTypes<IO>::Four*>(at));
   __builtin_memcpy(&v, &u, 16);
 }
 template <typename IO>
 __device__ __forceinline__ void store_values(uintptr_t at, const Vec<IO>& v) {
   typename GlobalTypes<IO>::V4 u;
   __builtin_memcpy(&u, &v, 16);
-  *reinterpret_cast<typename GlobalTypes<IO>::Four*>(at) = u;
+  __builtin_nontemporal_store(u, reinterpret_cast<typename GlobalTypes<IO>::Four*>(at));
 }
 
 // Walks the bytes [at, end) of an array: four(a) for kInFlight whole 16-byte
 // vectors a, a + 16 kThreads, ..., vec(a) for each of the others, one(a) for the
 // values before the first aligned vector and behind the last
-constexpr int kInFlight = 4;
-template <typename IO, typename F1, typename FV, typename F4>
+template <typename IO, int kInFlight, typename F1, typename FV, typename F4>
 __device__ __forceinline__ void for_piece(uintptr_t at, uintptr_t end, F1&& one, FV&& vec, F4&& four) {
   constexpr uintptr_t kStep = 16 * kThreads;
   uintptr_t a = (at + 15) / 16 * 16;
@@ -136,7 +139,8 @@ __device__ __forceinline__ void add_vec(const Vec<IO>& raw, double& s0, double& 
 }
 template <typename IO>
 __device__ __forceinline__ void add_squares(uintptr_t at, uintptr_t end, double& s0, double& s1) {
-  for_piece<IO>(
+  constexpr int kInFlight = 4;
+  for_piece<IO, kInFlight>(
       at, end,
       [&](uintptr_t a) {
         const double v = load_value<IO>(a);
@@ -209,7 +213,8 @@ __device__ __forceinline__ Vec<IO> scaled(const Vec<IO>& raw, float f) {
 }
 template <typename IO>
 __device__ __forceinline__ void scale_piece(uintptr_t at, uintptr_t end, float f) {
-  for_piece<IO>(
+  constexpr int kInFlight = 2;  // 4: 329 against 318 us for 0.9 GB
+  for_piece<IO, kInFlight>(
       at, end, [&](uintptr_t a) { store_value<IO>(a, load_value<IO>(a) * f); },
       [&](uintptr_t a) {
         Vec<IO> r;
@@ -236,7 +241,7 @@ clip_kernel(TensorList l, const double* part, int n, float max_norm, float* norm
   list.load(l);
   const uint32_t pieces = l.first[l.count];
   for (uint32_t q = blockIdx.x; q < pieces; q += gridDim.x) {
-    const uint32_t p = pieces - 1 - q;  // the last read are the likeliest in the caches
+    const uint32_t p = pieces - 1 - q;  // backwards: what is still in a cache is what was read last
     list.piece(p, l.count, [&](uintptr_t at, uintptr_t end, bool narrow) {
       if (narrow) scale_piece<bf16>(at, end, f);
       else scale_piece<float>(at, end, f);

@@ -23,12 +23,17 @@ template <typename IO> struct Loose;  // 16 bytes at the alignment of a value
 template <> struct Loose<float> { typedef uint32_t T __attribute__((ext_vector_type(4), aligned(4))); };
 template <> struct Loose<bf16> { typedef uint32_t T __attribute__((ext_vector_type(4), aligned(2))); };
 
-template <typename IO>
+// STREAM: non-temporal, for values that a launch reads once and nothing else
+// will soon.
+template <typename IO, bool STREAM = false>
 __device__ __forceinline__ Vec<IO> load_vec(const void* base, int64_t index, int n) {
   Vec<IO> r;
   const IO* p = static_cast<const IO*>(base) + index;
   if (n >= kVec<IO>) {
-    const typename Loose<IO>::T u = *reinterpret_cast<const typename Loose<IO>::T*>(p);
+    const auto* v = reinterpret_cast<const typename Loose<IO>::T*>(p);
+    typename Loose<IO>::T u;
+    if constexpr (STREAM) u = __builtin_nontemporal_load(v);
+    else u = *v;
     __builtin_memcpy(&r, &u, sizeof(r));
   } else {
     IO e[kVec<IO>] = {};
@@ -39,13 +44,15 @@ __device__ __forceinline__ Vec<IO> load_vec(const void* base, int64_t index, int
   }
   return r;
 }
-template <typename IO>
+template <typename IO, bool STREAM = false>
 __device__ __forceinline__ void store_vec(void* base, int64_t index, int n, const Vec<IO>& r) {
   IO* p = static_cast<IO*>(base) + index;
   if (n >= kVec<IO>) {
     typename Loose<IO>::T u;
     __builtin_memcpy(&u, &r, sizeof(r));
-    *reinterpret_cast<typename Loose<IO>::T*>(p) = u;
+    auto* v = reinterpret_cast<typename Loose<IO>::T*>(p);
+    if constexpr (STREAM) __builtin_nontemporal_store(u, v);
+    else *v = u;
   } else {
     IO e[kVec<IO>];
     __builtin_memcpy(e, &r, sizeof(r));

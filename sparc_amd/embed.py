@@ -10,13 +10,14 @@ from . import _lib
 
 
 def _forward(tokens, weight, scale):
+    """The rows, of contiguous tensors."""
     lib = _lib.load()
     vocab, dim = weight.shape
-    y = torch.empty(*tokens.shape, dim, dtype=weight.dtype, device=weight.device)
-    P = _lib.ptr
+    dev = weight.device
+    y = torch.empty(*tokens.shape, dim, dtype=weight.dtype, device=dev)
     _lib.check(lib.sparc_embedding_forward(
-        tokens.numel(), vocab, dim, _lib.io_code(weight.dtype), tokens.element_size(), P(tokens), P(weight), scale,
-        P(y), _lib.stream_of(weight.device)), "sparc_embedding_forward")
+        tokens.numel(), vocab, dim, _lib.io_code(weight.dtype), tokens.element_size(), tokens.data_ptr(),
+        weight.data_ptr(), scale, y.data_ptr(), _lib.stream_of(dev)), "sparc_embedding_forward")
     return y
 
 
@@ -37,10 +38,9 @@ class _Embedding(torch.autograd.Function):
         dw = torch.empty(vocab, dim, dtype=dtype, device=dy.device)
         need = lib.sparc_embedding_workspace_bytes(n, vocab, dim)
         ws = torch.empty(need, dtype=torch.uint8, device=dy.device)
-        P = _lib.ptr
         _lib.check(lib.sparc_embedding_backward(
-            n, vocab, dim, _lib.io_code(dtype), tokens.element_size(), P(tokens), padding_id, P(dy), scale, P(dw),
-            P(ws), need, _lib.stream_of(dy.device)), "sparc_embedding_backward")
+            n, vocab, dim, _lib.io_code(dtype), tokens.element_size(), tokens.data_ptr(), padding_id, dy.data_ptr(),
+            scale, dw.data_ptr(), ws.data_ptr(), need, _lib.stream_of(dy.device)), "sparc_embedding_backward")
         return dw, None, None, None
 
 
@@ -55,7 +55,7 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
     a row of NaN and no gradient: the ids are not read back to be checked.
     The gradient's sums are fp32 in the order of the positions, rounded once,
     so equal calls give equal bits."""
-    if weight.ndim != 2 or 0 in weight.shape:
+    if weight.ndim != 2 or weight.numel() == 0:
         raise ValueError(f"embedding expects a table [V, D], got {list(weight.shape)}")
     if tokens.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"embedding takes int64 or int32 ids, got {tokens.dtype}")
@@ -67,7 +67,7 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
         padding_id = padding_idx % weight.shape[0]
     _lib.require_gpu(tokens, weight)
     tokens = tokens.contiguous()
-    if torch.is_grad_enabled() and weight.requires_grad:
+    if weight.requires_grad and torch.is_grad_enabled():
         return _Embedding.apply(weight, tokens, float(scale), padding_id)
     return _forward(tokens, weight.contiguous(), float(scale))
 

@@ -10,17 +10,22 @@ from . import _lib
 
 
 def _forward(x, weight, bias, eps, save):
+    """(y, mean and rstd [2, rows] or None, the parameters' dtype) of contiguous
+    tensors."""
     lib = _lib.load()
     D = x.shape[-1]
     rows = x.numel() // D
     y = torch.empty_like(x)
-    stats = torch.empty(2, rows, dtype=torch.float32, device=x.device) if save else None
-    P = _lib.ptr
-    pdtype = x.dtype if weight is None and bias is None else (weight if weight is not None else bias).dtype
+    pdtype = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
+    stats = mean = rstd = None
+    if save:
+        stats = torch.empty(2, rows, dtype=torch.float32, device=x.device)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * rows
     _lib.check(lib.sparc_layer_norm_forward(
-        rows, D, _lib.io_code(x.dtype), _lib.io_code(pdtype), P(x), P(weight), P(bias), eps, P(y),
-        stats.data_ptr() if save else None, stats.data_ptr() + 4 * rows if save else None,
-        _lib.stream_of(x.device)), "sparc_layer_norm_forward")
+        rows, D, _lib.io_code(x.dtype), _lib.io_code(pdtype), x.data_ptr(),
+        None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(), eps, y.data_ptr(),
+        mean, rstd, _lib.stream_of(x.device)), "sparc_layer_norm_forward")
     return y, stats, pdtype
 
 
@@ -47,10 +52,10 @@ class _LayerNorm(torch.autograd.Function):
         need = lib.sparc_layer_norm_workspace_bytes(rows, D) if want[1] or want[2] else 0
         ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
         P = _lib.ptr
+        mean = stats.data_ptr()
         _lib.check(lib.sparc_layer_norm_backward(
-            rows, D, _lib.io_code(x.dtype), _lib.io_code(ctx.pdtype), P(x), P(weight), stats.data_ptr(),
-            stats.data_ptr() + 4 * rows, P(dy), P(dx), P(dw), P(db), P(ws), need, _lib.stream_of(x.device)),
-            "sparc_layer_norm_backward")
+            rows, D, _lib.io_code(x.dtype), _lib.io_code(ctx.pdtype), x.data_ptr(), P(weight), mean, mean + 4 * rows,
+            dy.data_ptr(), P(dx), P(dw), P(db), P(ws), need, _lib.stream_of(x.device)), "sparc_layer_norm_backward")
         return dx, dw, db, None
 
 
@@ -64,21 +69,32 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     or None, in x's dtype or in float32.  The arithmetic is fp32 and every
     result is rounded once; the parameters' gradients are sums over rows in a
     fixed order, so equal calls give equal bits."""
-    if x.ndim < 1 or x.shape[-1] < 1:
+    D = x.shape[-1] if x.ndim else 0
+    if D < 1:
         raise ValueError(f"layer_norm expects [..., D] inputs with D > 0, got {list(x.shape)}")
     if not eps >= 0.0:
         raise ValueError(f"layer_norm needs eps >= 0, got {eps}")
-    _lib.io_code(x.dtype)
-    params = [(n, p) for n, p in (("weight", weight), ("bias", bias)) if p is not None]
-    for name, p in params:
-        if p.dtype not in (x.dtype, torch.float32) or p.dtype != params[0][1].dtype:
-            raise ValueError(f"{name} must be in the input's dtype or float32 (weight and bias alike), got {p.dtype}")
-        _lib.expect(p, (x.shape[-1],), p.dtype, name)
+    dtype = x.dtype
+    _lib.io_code(dtype)
+    grad = x.requires_grad
+    if weight is not None:
+        _param(weight, D, dtype, "weight")
+        grad = grad or weight.requires_grad
+    if bias is not None:
+        _param(bias, D, dtype, "bias")
+        grad = grad or bias.requires_grad
+        if weight is not None and weight.dtype != bias.dtype:
+            raise ValueError(f"weight and bias must be alike, got {weight.dtype} and {bias.dtype}")
     _lib.require_gpu(x, weight, bias)
-    if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for _, p in params)):
+    if grad and torch.is_grad_enabled():
         return _LayerNorm.apply(x, weight, bias, float(eps))
-    return _forward(x.contiguous(), *[None if p is None else p.contiguous() for p in (weight, bias)], float(eps),
-                    False)[0]
+    return _forward(x.contiguous(), None if weight is None else weight.contiguous(),
+                    None if bias is None else bias.contiguous(), float(eps), False)[0]
+
+
+def _param(p, D, dtype, name):
+    if p.ndim != 1 or p.numel() != D or p.dtype != dtype and p.dtype != torch.float32:
+        raise ValueError(f"{name} must be [{D}] in the input's dtype or float32, got {list(p.shape)} {p.dtype}")
 
 
 __all__ = ["layer_norm"]
