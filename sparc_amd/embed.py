@@ -30,6 +30,8 @@ class _Embedding(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        if torch.is_grad_enabled():
+            raise RuntimeError("embedding is not twice differentiable")
         tokens, = ctx.saved_tensors
         (vocab, dim), dtype, scale, padding_id = ctx.args
         lib = _lib.load()

@@ -5,7 +5,10 @@ Each block is pre-norm and residual:
     x <- x + out_proj(SPARCMixer(in_proj(rms_norm(x))))
 
 with ``in_proj`` d_model -> 2M and ``out_proj`` 2M -> d_model (M = d_model *
-N complex modes, so the mixer's width is 2M), and a final RMSNorm.  The
+N complex modes, so the mixer's width is 2M), and a final RMSNorm; with
+``norm="layer"`` every norm is a layer norm with a bias instead.  ``prefill``
+and ``step`` run a prompt and then one token at a time, carrying the mixers'
+states.  The
 projections are plain GEMMs (torch -> hipBLASLt on MI355X); the mixer is the
 fused HIP sequence path, with its two control dot products folded into the
 input projection (``fuse_projection``).  The reference ships the layer, not a network
@@ -23,6 +26,7 @@ from torch import nn
 from . import _lib
 from . import mixer as _mixer
 from .control import aligned16
+from .norm import layer_norm
 from .sparc import SPARCMixer
 
 # Fold the controls into the input projection (see mixer._ProjectedMixer);
@@ -85,11 +89,30 @@ def rms_norm(norm: nn.RMSNorm, x: torch.Tensor) -> torch.Tensor:
     return norm(x)
 
 
+def _make_norm(kind: str, d_model: int, eps: float) -> nn.Module:
+    if kind == "rms":
+        return nn.RMSNorm(d_model, eps=eps)
+    if kind == "layer":
+        return nn.LayerNorm(d_model, eps=eps)
+    raise ValueError(f"unknown norm {kind!r} (rms or layer)")
+
+
+def apply_norm(norm: nn.Module, x: torch.Tensor) -> torch.Tensor:
+    """``norm(x)`` through the library's kernels: ``layer_norm`` for an
+    nn.LayerNorm over the last dimension on the GPU, ``rms_norm`` for an
+    nn.RMSNorm."""
+    if isinstance(norm, nn.LayerNorm):
+        if x.is_cuda and x.dtype in (torch.float32, torch.bfloat16) and norm.normalized_shape == (x.shape[-1],):
+            return layer_norm(x, norm.weight, norm.bias, norm.eps)
+        return norm(x)
+    return rms_norm(norm, x)
+
+
 class SPARCBlock(nn.Module):
-    def __init__(self, d_model: int, n_states: int, eps: float = 1e-6):
+    def __init__(self, d_model: int, n_states: int, eps: float = 1e-6, norm: str = "rms"):
         super().__init__()
         modes = d_model * n_states
-        self.norm = nn.RMSNorm(d_model, eps=eps)
+        self.norm = _make_norm(norm, d_model, eps)
         self.in_proj = nn.Linear(d_model, 2 * modes, bias=False)
         self.mixer = SPARCMixer(2 * modes)
         self.out_proj = nn.Linear(2 * modes, d_model, bias=False)
@@ -97,7 +120,7 @@ class SPARCBlock(nn.Module):
             self.out_proj.weight.mul_(1.0 / (2 * modes) ** 0.5)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        xn = rms_norm(self.norm, x)
+        xn = apply_norm(self.norm, x)
         if fuse_projection and _mixer.get_mixer_path() != "composed" and \
                 _mixer.projected_fused_supported(xn, self.in_proj.weight):
             y, _ = _mixer.projected_sequence(self.mixer, xn, self.in_proj.weight)
@@ -105,19 +128,52 @@ class SPARCBlock(nn.Module):
             y, _ = self.mixer(self.in_proj(xn))
         return x + self.out_proj(y)
 
+    def prefill(self, x: torch.Tensor):
+        """(output, state) of a sequence [B, T, d_model]: the state is the
+        mixer's (re, im) after the last position, fp32 [B, M]."""
+        y, state = self.mixer(self.in_proj(apply_norm(self.norm, x)), return_cache=True)
+        return x + self.out_proj(y), state
+
+    def step(self, x: torch.Tensor, state):
+        """(output, new state) of one position [B, d_model]."""
+        y, state = self.mixer.step(self.in_proj(apply_norm(self.norm, x)), state, None)
+        return x + self.out_proj(y), state
+
 
 class SPARCStack(nn.Module):
     """``n_layers`` SPARC blocks on a [B, T, d_model] stream."""
 
-    def __init__(self, n_layers: int, d_model: int, n_states: int, eps: float = 1e-6):
+    def __init__(self, n_layers: int, d_model: int, n_states: int, eps: float = 1e-6, norm: str = "rms"):
         super().__init__()
-        self.blocks = nn.ModuleList(SPARCBlock(d_model, n_states, eps) for _ in range(n_layers))
-        self.norm = nn.RMSNorm(d_model, eps=eps)
+        self.blocks = nn.ModuleList(SPARCBlock(d_model, n_states, eps, norm) for _ in range(n_layers))
+        self.norm = _make_norm(norm, d_model, eps)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         for blk in self.blocks:
             x = blk(x)
-        return rms_norm(self.norm, x)
+        return apply_norm(self.norm, x)
+
+    def prefill(self, x: torch.Tensor):
+        """(output, states): ``forward`` and each block's state after the last
+        position."""
+        states = []
+        for blk in self.blocks:
+            x, state = blk.prefill(x)
+            states.append(state)
+        return apply_norm(self.norm, x), states
+
+    def step(self, x: torch.Tensor, states):
+        """(output, new states) of one position [B, d_model]."""
+        new = []
+        for blk, state in zip(self.blocks, states):
+            x, state = blk.step(x, state)
+            new.append(state)
+        return apply_norm(self.norm, x), new
+
+    def prepare_inference(self) -> None:
+        """The mixers' fused decode steps (``SPARCMixer.prepare_inference``)."""
+        for blk in self.blocks:
+            blk.mixer.prepare_inference()
 
 
 GEMM_TUNING_FILE = os.path.join(os.path.dirname(__file__), "tuning", "gemm_stack_gfx950.csv")
@@ -149,5 +205,5 @@ def rms_norm_reference(x: torch.Tensor, weight: torch.Tensor, eps: float) -> tor
     return F.rms_norm(x, (x.shape[-1],), weight, eps)
 
 
-__all__ = ["SPARCBlock", "SPARCStack", "rms_norm", "rms_norm_reference", "use_tuned_gemms", "use_default_gemms",
+__all__ = ["SPARCBlock", "SPARCStack", "apply_norm", "rms_norm", "rms_norm_reference", "use_tuned_gemms", "use_default_gemms",
            "GEMM_TUNING_FILE"]

@@ -208,8 +208,15 @@ def test_reorder_refuses_and_bad_parents():
     parents = torch.tensor([[0, 1, 2], [2, 2, 2]], device="cuda")
     with pytest.raises(ValueError, match="another one"):
         sparc_amd.reorder_states([a, b], parents, out_states=[b, a])
-    with pytest.raises(ValueError, match="the same"):
+    with pytest.raises(ValueError, match="another one"):
         sparc_amd.reorder_states([a, b], parents, out_states=[a, a])
+    with pytest.raises(ValueError, match="another one"):
+        sparc_amd.reorder_states([a, a], parents, out_states=[a, a])
+    wide = torch.randn(7, 8, device="cuda")
+    with pytest.raises(ValueError, match="another one"):
+        sparc_amd.reorder_states([wide[:6]], parents, out_states=[wide[1:]])
+    fresh = sparc_amd.reorder_states([a, a], parents)  # to other memory a state may come twice
+    assert torch.equal(fresh[0], fresh[1])
     with pytest.raises(ValueError, match="out_states"):
         sparc_amd.reorder_states([a], parents, out_states=[b[:5]])
     with pytest.raises(ValueError, match="tensors for"):
