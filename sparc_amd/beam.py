@@ -30,20 +30,16 @@ def _planes(states):
 def _like(states, planes):
     """``planes`` in the structure of ``states``."""
     at = iter(planes)
-    return [type(s)(next(at) for _ in s) if isinstance(s, (tuple, list)) else next(at) for s in states]
+    return [tuple([next(at) for _ in s]) if isinstance(s, (tuple, list)) else next(at) for s in states]
 
 
-def _fresh(planes):
-    """Contiguous tensors of the planes' shapes and dtypes: neighbours of one
-    shape share an allocation."""
-    out, i = [], 0
-    while i < len(planes):
-        shape, dtype, n = planes[i].shape, planes[i].dtype, 1
-        while i + n < len(planes) and planes[i + n].shape == shape and planes[i + n].dtype == dtype:
-            n += 1
-        out += torch.empty(n, *shape, dtype=dtype, device=planes[i].device).unbind(0)
-        i += n
-    return out
+def _fresh(planes, alike):
+    """Contiguous tensors of the planes' shapes and dtypes; those of one shape
+    and dtype (``alike``: all of them) share an allocation."""
+    if alike:
+        p = planes[0]
+        return torch.empty(len(planes), *p.shape, dtype=p.dtype, device=p.device).unbind(0)
+    return [torch.empty_like(p, memory_format=torch.contiguous_format) for p in planes]
 
 
 def _check_out(planes, out):
@@ -83,9 +79,9 @@ def reorder_states(states: Sequence, parents: torch.Tensor, out_states: Sequence
     ``SPARCMixer.step``, in a list; ``parents``: [B, K] int64, K up to 32.
     ``out_states``: the same structure to write to; it may be ``states`` itself
     (in place: rows that stay are neither read nor written), but no tensor of it
-    may overlap another of the states.  By default fresh tensors are returned;
-    those of one shape and dtype share an allocation.  A parent outside [0, K)
-    gives a row of NaN."""
+    may overlap another of the states.  By default fresh tensors are returned,
+    which share one allocation where all states are of one shape and dtype.  A
+    parent outside [0, K) gives a row of NaN."""
     if parents.ndim != 2 or parents.dtype != torch.int64 or not 1 <= parents.shape[1] <= MAX_BEAMS:
         raise ValueError(f"parents must be [B, K] int64 with K from 1 to {MAX_BEAMS}, got {list(parents.shape)} "
                          f"{parents.dtype}")
@@ -94,24 +90,34 @@ def reorder_states(states: Sequence, parents: torch.Tensor, out_states: Sequence
 
 def _reorder(states, parents, out_states):
     B, K = parents.shape
-    planes = _planes(states)
-    rows = B * K
-    for p in planes:
-        if p.ndim < 1 or p.shape[0] != rows:
-            raise ValueError(f"states must have {rows} rows (one per beam), got {list(p.shape)}")
-    dev = _lib.require_gpu(parents, *planes)
+    planes, rows, dev = _planes(states), B * K, parents.device
+    shapes = [p.shape for p in planes]
+    alike = shapes.count(shapes[0]) == len(shapes) if shapes else False
+    for shape in shapes[:1] if alike else shapes:
+        if not len(shape) or shape[0] != rows:
+            raise ValueError(f"states must have {rows} rows (one per beam), got {list(shape)}")
+    _lib.require_gpu(parents)
+    index = dev.index
+    if any([p.get_device() != index for p in planes]):
+        _lib.require_gpu(parents, *planes)
+    sizes = [p.element_size() for p in planes]
+    if alike:
+        dtype = planes[0].dtype
+        alike = all([p.dtype is dtype for p in planes])
     if out_states is None:
-        out = _fresh(planes)
+        out = _fresh(planes, alike)
     else:
         out = _planes(out_states)
         _check_out(planes, out)
         if out_states is not states:
             _lib.require_gpu(parents, *out)
-    planes = [p.contiguous() for p in planes]
-    row_bytes = [p.numel() // rows * p.element_size() for p in planes] if rows else [0] * len(planes)
-    for n in row_bytes:
-        if n & 1:
-            raise ValueError("state rows must have an even number of bytes")
+    planes = [p if p.is_contiguous() else p.contiguous() for p in planes]
+    if alike:
+        row_bytes = [planes[0].numel() // rows * sizes[0] if rows else 0] * len(planes)
+    else:
+        row_bytes = [p.numel() // rows * n if rows else 0 for p, n in zip(planes, sizes)]
+    if any([n & 1 for n in row_bytes]):
+        raise ValueError("state rows must have an even number of bytes")
     src, dst = array("Q", [p.data_ptr() for p in planes]), array("Q", [o.data_ptr() for o in out])
     row_bytes = array("q", row_bytes)
     _lib.check(_lib.load().sparc_reorder_states(
