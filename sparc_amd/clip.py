@@ -11,6 +11,7 @@ import torch
 
 from . import _lib
 
+_Tensor = torch.Tensor
 _CODES = {torch.float32: _lib.SPARC_F32, torch.bfloat16: _lib.SPARC_BF16}
 
 
@@ -41,13 +42,15 @@ def _call(fn_name, tensors, *args):
     """One library call over the tensors' values (a tensor given twice counts
     once); the norm, [] float32."""
     lib = _lib.load()
-    dev = _lib.require_gpu(*tensors)
-    data = [t.data_ptr() for t in tensors]
+    dev = tensors[0].device
+    if not tensors[0].is_cuda or len(set(map(_Tensor.get_device, tensors))) > 1:
+        _lib.require_gpu(*tensors)
+    data = list(map(_Tensor.data_ptr, tensors))
     if len(set(data)) != len(data):
         once = dict(zip(data, tensors))
         data, tensors = list(once), list(once.values())
     n = len(data)
-    sizes, codes = array("q", [t.numel() for t in tensors]), array("i", [_CODES[t.dtype] for t in tensors])
+    sizes, codes = array("q", map(_Tensor.numel, tensors)), array("i", [_CODES[t.dtype] for t in tensors])
     data = array("Q", data)
     norm = torch.empty((), dtype=torch.float32, device=dev)
     need = lib.sparc_grad_norm_workspace_bytes(n)
@@ -59,10 +62,10 @@ def _call(fn_name, tensors, *args):
 
 def _checked(tensors):
     for t in tensors:
-        if t.dtype not in _CODES:
-            raise TypeError(f"SPARC HIP kernels take float32 or bfloat16 tensors, got {t.dtype}")
         if t.layout is not torch.strided:
             raise ValueError(f"gradients must be dense tensors, got layout {t.layout}")
+        if t.dtype not in _CODES:
+            raise TypeError(f"SPARC HIP kernels take float32 or bfloat16 tensors, got {t.dtype}")
     return tensors
 
 
@@ -93,8 +96,8 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     if not grads:
         return torch.zeros(())
     copies = []
-    for i, g in enumerate(grads):
-        if not (g.is_contiguous() or _dense(g)):
+    for i, g in enumerate(grads if not all(map(_Tensor.is_contiguous, grads)) else ()):
+        if not _dense(g):
             if _repeats(g):
                 raise ValueError("a gradient names one value more than once (an expanded view): it cannot be scaled "
                                  "in place")

@@ -16,34 +16,33 @@
 namespace sparc {
 namespace {
 
-constexpr int kMaxTensors = 160;      // per launch: 3.4 KB of kernel arguments
+constexpr int kMaxTensors = 256;      // per launch: 3.6 KB of kernel arguments
 constexpr int kPieceValues = 16384;
 constexpr int kMaxGroups = 1024;      // partial sums per launch
 constexpr int kThreads = 256;
 
 struct TensorList {
   void* data[kMaxTensors];
-  int64_t size[kMaxTensors];
   uint32_t first[kMaxTensors + 1];    // first piece of each tensor
-  uint8_t bf16_values[kMaxTensors];
+  uint16_t last[kMaxTensors];         // values of its last piece, and kNarrow for bf16 values
   int count;
 };
+constexpr uint16_t kNarrow = 0x8000;
+static_assert(kPieceValues < kNarrow, "a piece's values beside the flag");
 
 // A launch's list in LDS: one trip to the kernel arguments for all threads,
 // where a search among them would make one for each of its steps.
 struct ListInLds {
   void* data[kMaxTensors];
-  int64_t size[kMaxTensors];
   uint32_t first[kMaxTensors + 1];
-  uint8_t bf16_values[kMaxTensors];
+  uint16_t last[kMaxTensors];
 
   __device__ __forceinline__ void load(const TensorList& l) {
     for (int i = threadIdx.x; i <= l.count; i += kThreads) {
       first[i] = l.first[i];
       if (i < l.count) {
         data[i] = l.data[i];
-        size[i] = l.size[i];
-        bf16_values[i] = l.bf16_values[i];
+        last[i] = l.last[i];
       }
     }
     __syncthreads();
@@ -61,12 +60,11 @@ struct ListInLds {
   template <typename F>
   __device__ __forceinline__ void piece(uint32_t p, int count, F&& f) const {
     const int t = __builtin_amdgcn_readfirstlane(tensor_of(p, count));
-    const int64_t lo = static_cast<int64_t>(p - first[t]) * kPieceValues;
-    const int64_t hi = lo + kPieceValues < size[t] ? lo + kPieceValues : size[t];
-    const bool narrow = bf16_values[t];
+    const bool narrow = last[t] & kNarrow;
+    const int64_t values = p + 1 < first[t + 1] ? kPieceValues : last[t] & (kNarrow - 1);
     const int size_of = narrow ? 2 : 4;
-    const uintptr_t base = reinterpret_cast<uintptr_t>(data[t]);
-    f(base + lo * size_of, base + hi * size_of, narrow);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(data[t]) + int64_t(p - first[t]) * kPieceValues * size_of;
+    f(at, at + values * size_of, narrow);
   }
 };
 
@@ -261,8 +259,8 @@ int64_t next_list(int64_t count, void* const* data, const int64_t* sizes, const 
   for (; at < count && l.count < kMaxTensors; ++at) {
     if (sizes[at] == 0) continue;
     l.data[l.count] = data[at];
-    l.size[l.count] = sizes[at];
-    l.bf16_values[l.count] = dtypes[at] == SPARC_BF16;
+    l.last[l.count] = static_cast<uint16_t>((sizes[at] - 1) % kPieceValues + 1) |
+                      (dtypes[at] == SPARC_BF16 ? kNarrow : uint16_t(0));
     l.first[l.count++] = pieces;
     pieces += static_cast<uint32_t>((sizes[at] + kPieceValues - 1) / kPieceValues);
   }

@@ -28,6 +28,11 @@ constexpr int kRowWaves = 4;       // forward, one wave per row: rows per workgr
 constexpr int kBwdRowWaves = 8;    // backward, one wave per row: rows in flight per workgroup
 constexpr int64_t kFewRows = 1024; // below this a forward workgroup holds one row: one per CU before two
 
+// columns from c on, as load_vec counts them
+__device__ __forceinline__ int left(int64_t D, int64_t c) {
+  return static_cast<int>(D - c < 64 ? D - c : 64);
+}
+
 // Sums of N values over the W waves that share a row, in every lane.  red: two
 // buffers used in turn (``turn``), so that one barrier per call is enough.
 template <int N, int W>
@@ -278,21 +283,32 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
 constexpr int kWideThreads = 1024;
 template <typename IO, typename PT>
 __global__ void __launch_bounds__(kWideThreads)
-layer_norm_fwd_wide_kernel(int64_t D, const void* x, const void* w, const void* b, float eps, void* y, float* mean,
-                           float* rstd, int64_t R) {
+layer_norm_fwd_wide_kernel(int64_t R, int64_t D, const void* x, const void* w, const void* b, float eps, void* y,
+                           float* mean, float* rstd) {
+  constexpr int V = kVec<IO>;
   __shared__ float red[2][1][kWideThreads / 64];
   int turn = 0;
   const float inv_d = 1.0f / static_cast<float>(D);
+  const int64_t c0 = static_cast<int64_t>(threadIdx.x) * V;
   for (int64_t row = blockIdx.x; row < R; row += gridDim.x) {
     const int64_t base = row * D;
-    float s[1] = {0.0f};
-    for (int64_t c = threadIdx.x; c < D; c += kWideThreads) s[0] += load1<IO>(x, base + c);
+    float s[1] = {0.0f}, v[V];
+    for (int64_t c = c0; c < D; c += kWideThreads * V) {
+      unpack<IO, V>(load_vec<IO>(x, base + c, left(D, c)), v);
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[0] += v[i];
+    }
     row_sums<1, kWideThreads / 64>(s, red, turn);
     const float mu = s[0] * inv_d;
     s[0] = 0.0f;
-    for (int64_t c = threadIdx.x; c < D; c += kWideThreads) {
-      const float d = load1<IO>(x, base + c) - mu;
-      s[0] = fmaf(d, d, s[0]);
+    for (int64_t c = c0; c < D; c += kWideThreads * V) {
+      const int n = left(D, c);
+      unpack<IO, V>(load_vec<IO>(x, base + c, n), v);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float d = i < n ? v[i] - mu : 0.0f;
+        s[0] = fmaf(d, d, s[0]);
+      }
     }
     row_sums<1, kWideThreads / 64>(s, red, turn);
     const float r = 1.0f / sqrtf(s[0] * inv_d + eps);
@@ -300,36 +316,63 @@ layer_norm_fwd_wide_kernel(int64_t D, const void* x, const void* w, const void* 
       mean[row] = mu;
       rstd[row] = r;
     }
-    for (int64_t c = threadIdx.x; c < D; c += kWideThreads) {
-      float o = (load1<IO>(x, base + c) - mu) * r;
-      if (w) o *= load1<PT>(w, c);
-      if (b) o += load1<PT>(b, c);
-      store1<IO>(y, base + c, o);
+    for (int64_t c = c0; c < D; c += kWideThreads * V) {
+      const int n = left(D, c);
+      float p[V], q[V];
+      unpack<IO, V>(load_vec<IO>(x, base + c, n), v);
+      if (w) load_f32<PT, V>(w, c, n, p);
+      if (b) load_f32<PT, V>(b, c, n, q);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        v[i] = (v[i] - mu) * r;
+        if (w) v[i] *= p[i];
+        if (b) v[i] += q[i];
+      }
+      store_vec<IO>(y, base + c, n, pack<IO, V>(v));
     }
   }
 }
 template <typename IO, typename PT>
 __global__ void __launch_bounds__(kWideThreads)
-layer_norm_dx_wide_kernel(int64_t D, const void* x, const void* w, const float* mean, const float* rstd,
-                          const void* dy, void* dx, int64_t R) {
+layer_norm_dx_wide_kernel(int64_t R, int64_t D, const void* x, const void* w, const float* mean, const float* rstd,
+                          const void* dy, void* dx) {
+  constexpr int V = kVec<IO>;
   __shared__ float red[2][2][kWideThreads / 64];
   int turn = 0;
   const float inv_d = 1.0f / static_cast<float>(D);
+  const int64_t c0 = static_cast<int64_t>(threadIdx.x) * V;
   for (int64_t row = blockIdx.x; row < R; row += gridDim.x) {
     const int64_t base = row * D;
     const float mu = mean[row], r = rstd[row];
-    float s[2] = {0.0f, 0.0f};
-    for (int64_t c = threadIdx.x; c < D; c += kWideThreads) {
-      const float g = load1<IO>(dy, base + c) * (w ? load1<PT>(w, c) : 1.0f);
-      s[0] += g;
-      s[1] = fmaf(g, (load1<IO>(x, base + c) - mu) * r, s[1]);
+    float s[2] = {0.0f, 0.0f}, g[V], xh[V];
+    // g and xhat of the columns from c on (behind the row g is 0)
+    const auto load = [&](int64_t c, int n) __attribute__((always_inline)) {
+      unpack<IO, V>(load_vec<IO>(dy, base + c, n), g);
+      unpack<IO, V>(load_vec<IO>(x, base + c, n), xh);
+      float p[V];
+      if (w) load_f32<PT, V>(w, c, n, p);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (w) g[i] *= p[i];
+        xh[i] = (xh[i] - mu) * r;
+      }
+    };
+    for (int64_t c = c0; c < D; c += kWideThreads * V) {
+      load(c, left(D, c));
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        s[0] += g[i];
+        s[1] = fmaf(g[i], xh[i], s[1]);
+      }
     }
     row_sums<2, kWideThreads / 64>(s, red, turn);
     const float m0 = s[0] * inv_d, m1 = s[1] * inv_d;
-    for (int64_t c = threadIdx.x; c < D; c += kWideThreads) {
-      const float g = load1<IO>(dy, base + c) * (w ? load1<PT>(w, c) : 1.0f);
-      const float xh = (load1<IO>(x, base + c) - mu) * r;
-      store1<IO>(dx, base + c, r * (fmaf(-xh, m1, g) - m0));
+    for (int64_t c = c0; c < D; c += kWideThreads * V) {
+      const int n = left(D, c);
+      load(c, n);
+#pragma unroll
+      for (int i = 0; i < V; ++i) g[i] = r * (fmaf(-xh[i], m1, g[i]) - m0);
+      store_vec<IO>(dx, base + c, n, pack<IO, V>(g));
     }
   }
 }
@@ -338,16 +381,30 @@ template <typename IO>
 __global__ void __launch_bounds__(256)
 layer_norm_params_wide_kernel(int64_t R, int64_t D, const void* x, const float* mean, const float* rstd,
                               const void* dy, float* dw_part, float* db_part) {
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  constexpr int V = kVec<IO>;
+  const int64_t c = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * V;
   if (c >= D) return;
-  float aw = 0.0f, ab = 0.0f;
+  const int n = left(D, c);
+  float aw[V], ab[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) { aw[i] = 0.0f; ab[i] = 0.0f; }
   for (int64_t row = blockIdx.y; row < R; row += gridDim.y) {
-    const float d = load1<IO>(dy, row * D + c);
-    aw = fmaf(d, (load1<IO>(x, row * D + c) - mean[row]) * rstd[row], aw);
-    ab += d;
+    float d[V], v[V];
+    unpack<IO, V>(load_vec<IO>(dy, row * D + c, n), d);
+    unpack<IO, V>(load_vec<IO>(x, row * D + c, n), v);
+    const float mu = mean[row], r = rstd[row];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      aw[i] = fmaf(d[i], (v[i] - mu) * r, aw[i]);
+      ab[i] += d[i];
+    }
   }
-  if (dw_part) dw_part[blockIdx.y * D + c] = aw;
-  if (db_part) db_part[blockIdx.y * D + c] = ab;
+#pragma unroll
+  for (int q = 0; q < V; q += 4) {
+    const int64_t at = blockIdx.y * D + c + q;
+    if (dw_part) store_vec<float>(dw_part, at, n - q, make_float4(aw[q], aw[q + 1], aw[q + 2], aw[q + 3]));
+    if (db_part) store_vec<float>(db_part, at, n - q, make_float4(ab[q], ab[q + 1], ab[q + 2], ab[q + 3]));
+  }
 }
 
 // out[c] = sum over the n partial rows: CW columns by 1024 / CW slices of rows
@@ -455,8 +512,8 @@ sparc_status ln_forward(hipStream_t st, int64_t R, int64_t D, const void* x, con
                          static_cast<int>(D), x, w, b, eps, y, mean, rstd);
   });
   if (!held)
-    hipLaunchKernelGGL((layer_norm_fwd_wide_kernel<IO, PT>), dim3(op_grid(R)), dim3(kWideThreads), 0, st, D, x, w, b,
-                       eps, y, mean, rstd, R);
+    hipLaunchKernelGGL((layer_norm_fwd_wide_kernel<IO, PT>), dim3(op_grid(R)), dim3(kWideThreads), 0, st, R, D, x, w, b,
+                       eps, y, mean, rstd);
   return op_launched("layer norm forward");
 }
 
@@ -480,14 +537,14 @@ sparc_status ln_backward(hipStream_t st, int64_t R, int64_t D, const void* x, co
   });
   if (!held) {
     if (dx)
-      hipLaunchKernelGGL((layer_norm_dx_wide_kernel<IO, PT>), dim3(op_grid(R)), dim3(kWideThreads), 0, st, D, x, w,
-                         mean, rstd, dy, dx, R);
+      hipLaunchKernelGGL((layer_norm_dx_wide_kernel<IO, PT>), dim3(op_grid(R)), dim3(kWideThreads), 0, st, R, D, x, w,
+                         mean, rstd, dy, dx);
     if (dw || db) {
       n = R < kWideSlices ? R : kWideSlices;
       if (dw && db) db_part = ws + n * D;
       hipLaunchKernelGGL((layer_norm_params_wide_kernel<IO>),
-                         dim3(static_cast<unsigned>((D + 255) / 256), static_cast<unsigned>(n)), dim3(256), 0, st, R, D,
-                         x, mean, rstd, dy, dw_part, db_part);
+                         dim3(static_cast<unsigned>((D - 1) / (256 * kVec<IO>) + 1), static_cast<unsigned>(n)),
+                         dim3(256), 0, st, R, D, x, mean, rstd, dy, dw_part, db_part);
     }
   }
   if (sparc_status s = op_launched("layer norm backward")) return s;
