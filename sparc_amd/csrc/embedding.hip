@@ -17,8 +17,9 @@
 // frequencies: a run of equal ids inside a piece is written to its row at
 // once; a run that crosses pieces leaves one fp32 partial row per piece,
 // joined in order by a second kernel.  Every sum has a fixed order, so dW does
-// not depend on timing, and every row of dW is written exactly once: rows
-// without tokens are cleared by further workgroups of the summing kernel.
+// not depend on timing.  The sort keeps few CUs busy and is bound by latency, so
+// further workgroups of its launches clear dW meanwhile, a share each; the rows
+// that tokens name are then written once more.
 
 #include "rows.h"
 
@@ -28,7 +29,7 @@ namespace {
 // Sorted positions per piece, all read at once.  8 against 16, the summing and
 // the joining kernel: 37 against 35 us for 32768 x 768 bf16 gradients, 43
 // against 48 us for 3711 x 1001 fp32 ones into 50001 rows, where the pieces are
-// few and the kernel's registers decide how many workgroups clear rows.
+// few.
 constexpr int kPiece = 8;
 constexpr int kSortThreads = 256;   // 4 waves per sort tile
 constexpr int kSortWaves = kSortThreads / 64;
@@ -93,14 +94,24 @@ struct SortPass {
   uint32_t* keys_out;
   uint32_t* pos_out;
   uint32_t* counts;       // [tiles][digits] of this pass
-  uint8_t* touched;       // [vocab]: cleared by the first count, set by the last scatter
   int64_t n;
   int shift, bits;
-  int first, last;
+  int first;
+  int tiles;              // sorting workgroups; those behind them clear
+  char* dw;               // this launch's share of dW, in bytes
+  int64_t dw_bytes;
 
-  // by thread ``at`` of ``step``; the flags' memory is a multiple of 256 bytes
-  __device__ __forceinline__ void clear_touched(int64_t at, int64_t step) const {
-    for (int64_t v = at; v * 16 < vocab; v += step) reinterpret_cast<uint4*>(touched)[v] = make_uint4(0, 0, 0, 0);
+  // by the workgroups behind the sorting ones
+  __device__ __forceinline__ void clear() const {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(dw);
+    const int64_t head = static_cast<int64_t>((16 - at % 16) % 16) < dw_bytes ? (16 - at % 16) % 16 : dw_bytes;
+    const int64_t vecs = (dw_bytes - head) / 16, tail = head + vecs * 16;
+    const int64_t step = static_cast<int64_t>(gridDim.x - tiles) * blockDim.x;
+    const int64_t t = static_cast<int64_t>(blockIdx.x - tiles) * blockDim.x + threadIdx.x;
+    uint4* const body = reinterpret_cast<uint4*>(dw + head);
+    for (int64_t v = t; v < vecs; v += step) body[v] = make_uint4(0, 0, 0, 0);
+    if (t < head) dw[t] = 0;
+    if (tail + t < dw_bytes) dw[tail + t] = 0;
   }
   // The keys of ITEMS positions from ``at`` on, ``step`` apart, all read at
   // once.  A key is the position's id, or vocab (behind every row) where it
@@ -134,21 +145,16 @@ template <int ITEMS>
 __global__ void __launch_bounds__(kSortThreads)
 sort_count_kernel(SortPass p) {
   __shared__ uint32_t hist[kMaxDigits];
+  if (static_cast<int>(blockIdx.x) >= p.tiles) return p.clear();
   const int digits = 1 << p.bits;
   for (int d = threadIdx.x; d < digits; d += kSortThreads) hist[d] = 0;
-  if (p.first) {
-    p.clear_touched(static_cast<int64_t>(blockIdx.x) * kSortThreads + threadIdx.x,
-                    static_cast<int64_t>(gridDim.x) * kSortThreads);
-  }
   __syncthreads();
   const int64_t base = static_cast<int64_t>(blockIdx.x) * (kSortThreads * ITEMS) + threadIdx.x;
-  if (p.n > 0) {
-    uint32_t key[ITEMS];
-    p.load_keys<ITEMS>(base, kSortThreads, key);
+  uint32_t key[ITEMS];
+  p.load_keys<ITEMS>(base, kSortThreads, key);
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
-      if (base + i * kSortThreads < p.n) atomicAdd(&hist[(key[i] >> p.shift) & (digits - 1)], 1u);
-  }
+  for (int i = 0; i < ITEMS; ++i)
+    if (base + i * kSortThreads < p.n) atomicAdd(&hist[(key[i] >> p.shift) & (digits - 1)], 1u);
   __syncthreads();
   for (int d = threadIdx.x; d < digits; d += kSortThreads)
     p.counts[static_cast<int64_t>(blockIdx.x) * digits + d] = hist[d];
@@ -164,10 +170,10 @@ sort_scatter_kernel(SortPass p) {
   __shared__ uint32_t cnt[kSortWaves][kMaxDigits];  // counts, then the waves' first places
   __shared__ uint32_t start[kMaxDigits];            // this tile's first place of each digit
   __shared__ uint32_t wsum[kSortWaves];
+  if (static_cast<int>(blockIdx.x) >= p.tiles) return p.clear();
   const int digits = 1 << p.bits;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * (kSortThreads * ITEMS) + wave * (64 * ITEMS) + lane;
-  if (p.n == 0) return;  // the whole launch
   uint32_t key[ITEMS], pos[ITEMS];
   p.load_keys<ITEMS>(first, 64, key);
 #pragma unroll
@@ -184,7 +190,7 @@ sort_scatter_kernel(SortPass p) {
   uint32_t before[2] = {0, 0}, total[2] = {0, 0};
   if (2 * static_cast<int>(threadIdx.x) < digits) {
     const uint2* counts = reinterpret_cast<const uint2*>(p.counts) + threadIdx.x;
-    const int tiles = gridDim.x, mine = blockIdx.x;
+    const int tiles = p.tiles, mine = blockIdx.x;
     for (int t0 = 0; t0 < tiles; t0 += 16) {
       uint2 c[16];
 #pragma unroll
@@ -252,7 +258,6 @@ sort_scatter_kernel(SortPass p) {
       const uint32_t to = cnt[wave][(key[i] >> p.shift) & (digits - 1)] + rank[i];
       p.keys_out[to] = key[i];
       p.pos_out[to] = pos[i];
-      if (p.last && key[i] < static_cast<uint32_t>(p.vocab)) p.touched[key[i]] = 1;
     }
   }
 }
@@ -265,6 +270,7 @@ sort_local_kernel(SortPass p, int pos_bits, int passes) {
   __shared__ uint32_t buf[kLocalThreads * ITEMS];
   __shared__ uint16_t cnt[kLocalWaves][kMaxDigits];
   __shared__ uint32_t wsum[kLocalWaves];
+  if (static_cast<int>(blockIdx.x) >= p.tiles) return p.clear();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int digits = 1 << p.bits, at = wave * 64 * ITEMS + lane, N = static_cast<int>(p.n);
   uint32_t v[ITEMS];
@@ -272,8 +278,6 @@ sort_local_kernel(SortPass p, int pos_bits, int passes) {
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i)  // what is behind the end stays behind all others
     v[i] = at + i * 64 < N ? v[i] << pos_bits | static_cast<uint32_t>(at + i * 64) : kNone;
-  p.clear_touched(threadIdx.x, kLocalThreads);
-  __threadfence();
   for (int pass = 0; pass < passes; ++pass) {
     const int shift = pos_bits + pass * p.bits;
     for (int d = threadIdx.x; d < kLocalWaves * kMaxDigits / 2; d += kLocalThreads)
@@ -333,10 +337,8 @@ sort_local_kernel(SortPass p, int pos_bits, int passes) {
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
     if (at + i * 64 < N) {
-      const uint32_t key = v[i] >> pos_bits;
-      p.keys_out[at + i * 64] = key;
+      p.keys_out[at + i * 64] = v[i] >> pos_bits;
       p.pos_out[at + i * 64] = v[i] & ((1u << pos_bits) - 1);
-      if (key < static_cast<uint32_t>(p.vocab)) p.touched[key] = 1;
     }
   }
 }
@@ -353,40 +355,17 @@ __device__ __forceinline__ void write_row(void* dw, int64_t row, int D, int c, c
   store_vec<IO>(dw, row * D + c, D - c, pack<IO, kVec<IO>>(o));
 }
 
-// Workgroups below sum_groups: pieces of sorted positions, a group of lpr lanes
-// per piece and block of lpr 16-byte vectors.  part: [pieces][2][D] fp32, the
-// partial sums of a run that goes on from the piece before (0) and of one that
-// begins here and goes on into the next (1).  The others clear rows of dW that
-// no token names.
+// A group of lanes per piece and block of columns.  part: [pieces][2][D] fp32,
+// the partial sums of a run that goes on from the piece before (0) and of one
+// that begins here and goes on into the next (1).
 template <typename IO>
 __global__ void __launch_bounds__(256)
-embed_sum_kernel(int64_t N, int64_t vocab, Jobs jb, int64_t sum_groups, const uint32_t* keys, const uint32_t* pos,
-                 const uint8_t* touched, const void* dy, float scale, float* part, void* dw) {
+embed_sum_kernel(int64_t N, int64_t vocab, Jobs jb, const uint32_t* keys, const uint32_t* pos, const void* dy,
+                 float scale, float* part, void* dw) {
   constexpr int V = kVec<IO>;
   const int D = jb.D;
-  const int64_t per = 256 / jb.lpr;
-  if (blockIdx.x >= sum_groups) {
-    constexpr int kFlags = 4;  // flags read together
-    const int64_t jobs = vocab * jb.blocks, step = (gridDim.x - sum_groups) * per;
-    const Vec<IO> zero = {};
-    for (int64_t job0 = (blockIdx.x - sum_groups) * per + threadIdx.x / jb.lpr; job0 < jobs; job0 += kFlags * step) {
-      int64_t v[kFlags];
-      int c[kFlags];
-      bool clear[kFlags];
-#pragma unroll
-      for (int u = 0; u < kFlags; ++u) {
-        const int64_t job = job0 + u * step < jobs ? job0 + u * step : job0;
-        v[u] = jb.row_of<V>(job, c[u]);
-        clear[u] = !touched[v[u]];
-      }
-#pragma unroll
-      for (int u = 0; u < kFlags; ++u)
-        if (clear[u] && c[u] < D) store_vec<IO>(dw, v[u] * D + c[u], D - c[u], zero);
-    }
-    return;
-  }
-  const int64_t pieces = (N + kPiece - 1) / kPiece, jobs = pieces * jb.blocks;
-  for (int64_t job = blockIdx.x * per + threadIdx.x / jb.lpr; job < jobs; job += sum_groups * per) {
+  const int64_t per = 256 / jb.lpr, pieces = (N + kPiece - 1) / kPiece, jobs = pieces * jb.blocks;
+  for (int64_t job = blockIdx.x * per + threadIdx.x / jb.lpr; job < jobs; job += gridDim.x * per) {
     int c;
     const int64_t piece = jb.row_of<V>(job, c);
     if (c >= D) continue;
@@ -434,7 +413,9 @@ embed_sum_kernel(int64_t N, int64_t vocab, Jobs jb, int64_t sum_groups, const ui
   }
 }
 
-// s += the rows a, a + 1, ... below b of the running partial sums, 4 columns
+// s += the rows a, a + 1, ... below b of the running partial sums, 4 columns.
+// (16 rows in flight: fewer workgroups at once, 17.6 us against 12.7 for 32768
+// positions.)
 __device__ __forceinline__ void add_parts(float (&s)[4], const float* part, int64_t a, int64_t b, int D, int c) {
   int64_t q = a;
   for (; q + 8 <= b; q += 8) {
@@ -476,13 +457,18 @@ embed_join_kernel(int64_t N, int64_t vocab, int D, const uint32_t* keys, float s
     }
     int64_t last = piece;
     if (begins) {
-      // pieces that begin with the key, 64 at a time: they are consecutive
-      for (;;) {
-        const int64_t q = last + 1 + lane;
-        const uint64_t same = __ballot(q < pieces && keys[q * kPiece] == key);
-        const int more = __popcll(same);
-        last += more;
-        if (more < 64) break;
+      // the last piece that begins with the key: those that do are consecutive.
+      // The next 64 first, then a search with 64 probes a time
+      const int64_t q = piece + 1 + lane;
+      last = piece + __popcll(__ballot(q < pieces && keys[q * kPiece] == key));
+      if (last == piece + 64) {
+        for (int64_t end = pieces; end - last > 1;) {  // ``last`` does, ``end`` does not
+          const int64_t step = (end - last + 63) / 64, probe = last + (lane + 1) * step;
+          const int more = __popcll(__ballot(probe < end && keys[probe * kPiece] == key));
+          const int64_t beyond = last + (more + 1) * step;
+          last += more * step;
+          end = beyond < end ? beyond : end;
+        }
       }
     }
     const bool is_long = begins && last - piece > kLongRun;
@@ -559,7 +545,6 @@ Sort sort_of(int64_t n, int64_t vocab) {
   s.digit_bits = (s.bits + s.passes - 1) / s.passes;
   s.items = n <= 65536 ? 4 : 16;  // at most 64 tiles' counts to add up, then tiles four times the size
   s.tiles = (n + kSortThreads * s.items - 1) / (kSortThreads * s.items);
-  if (s.tiles < 1) s.tiles = 1;  // without tokens, one tile clears the flags
   s.pos_bits = 1;
   while ((n - 1) >> s.pos_bits > 0) ++s.pos_bits;
   if (n < 1 || n > kLocalItems * kLocalThreads || s.bits + s.pos_bits > 32) s.pos_bits = 0;
@@ -575,8 +560,8 @@ Jobs em_jobs(int64_t dim, int v) {
   jb.blocks = static_cast<int>((vecs + jb.lpr - 1) / jb.lpr);
   return jb;
 }
-unsigned em_grid(const Jobs& jb, int64_t rows, int ahead) {
-  const int64_t per = 256 / jb.lpr * ahead;
+unsigned em_grid(const Jobs& jb, int64_t rows) {
+  const int64_t per = 256 / jb.lpr;
   return op_grid((rows * jb.blocks + per - 1) / per);
 }
 
@@ -584,29 +569,51 @@ template <typename IO>
 void em_forward(hipStream_t st, int64_t n, int64_t vocab, int64_t dim, const void* tokens, int id_bytes, const void* w,
                 float scale, void* y) {
   const Jobs jb = em_jobs(dim, kVec<IO>);
-  hipLaunchKernelGGL((embed_fwd_kernel<IO>), dim3(em_grid(jb, n, 1)), dim3(256), 0, st, n, vocab, jb, tokens,
+  hipLaunchKernelGGL((embed_fwd_kernel<IO>), dim3(em_grid(jb, n)), dim3(256), 0, st, n, vocab, jb, tokens,
                      id_bytes == 8, w, scale, y);
 }
+
+// The shares of dW that the launches of a sort clear, one behind the other, in
+// whole multiples of 256 bytes, and their grids.
+struct Clearing {
+  char* dw;
+  int64_t left;
+  int launches;
+
+  unsigned take(SortPass& p, int threads) {
+    int64_t share = (left / launches + 255) / 256 * 256;
+    if (launches == 1 || share > left) share = left;
+    p.dw = dw;
+    p.dw_bytes = share;
+    dw += share;
+    left -= share;
+    --launches;
+    const int64_t groups = (share / 16 + threads - 1) / threads, most = 4 * 256 * 1024 / threads;  // 4 per thread slot
+    return p.tiles + static_cast<unsigned>(share == 0 ? 0 : groups < 1 ? 1 : groups < most ? groups : most);
+  }
+};
 
 // A count and a scatter per pass; returns the buffer that holds the sorted
 // positions.  (The next pass's counts as atomic additions of the scatter, for
 // one launch less: 18 us instead of 6 + 3 at 32768 ids of natural frequencies,
 // whose commonest meet in a few counters.)
 template <int ITEMS>
-int em_sort(hipStream_t st, const Sort& s, SortPass p, uint32_t* const* keys, uint32_t* const* pos, uint32_t* counts) {
-  const dim3 grid(static_cast<unsigned>(s.tiles)), block(kSortThreads);
+int em_sort(hipStream_t st, const Sort& s, SortPass p, Clearing clear, uint32_t* const* keys, uint32_t* const* pos,
+            uint32_t* counts) {
   int cur = 0;
   p.counts = counts;
+  p.tiles = static_cast<int>(s.tiles);
   for (int k = 0; k < s.passes; ++k) {
     p.keys_in = keys[cur ^ 1];
     p.pos_in = pos[cur ^ 1];
     p.keys_out = keys[cur];
     p.pos_out = pos[cur];
-    p.last = k == s.passes - 1;
     p.shift = k * s.digit_bits;
     p.first = k == 0;
-    hipLaunchKernelGGL((sort_count_kernel<ITEMS>), grid, block, 0, st, p);
-    hipLaunchKernelGGL((sort_scatter_kernel<ITEMS>), grid, block, 0, st, p);
+    // the counts are over too soon to hide a share
+    hipLaunchKernelGGL((sort_count_kernel<ITEMS>), dim3(p.tiles), dim3(kSortThreads), 0, st, p);
+    const unsigned grid = clear.take(p, kSortThreads);
+    hipLaunchKernelGGL((sort_scatter_kernel<ITEMS>), dim3(grid), dim3(kSortThreads), 0, st, p);
     cur ^= 1;
   }
   return cur ^ 1;
@@ -614,12 +621,11 @@ int em_sort(hipStream_t st, const Sort& s, SortPass p, uint32_t* const* keys, ui
 
 template <typename IO>
 void em_sums(hipStream_t st, int64_t n, int64_t vocab, int64_t dim, const uint32_t* keys, const uint32_t* pos,
-             const uint8_t* touched, const void* dy, float scale, float* part, void* dw) {
+             const void* dy, float scale, float* part, void* dw) {
   const int64_t pieces = (n + kPiece - 1) / kPiece;
   const Jobs jb = em_jobs(dim, kVec<IO>);
-  const unsigned sum_groups = em_grid(jb, pieces, 1), clear = em_grid(jb, vocab, 4), most = 2048;
-  hipLaunchKernelGGL((embed_sum_kernel<IO>), dim3(sum_groups + (clear < most ? clear : most)), dim3(256), 0, st, n,
-                     vocab, jb, static_cast<int64_t>(sum_groups), keys, pos, touched, dy, scale, part, dw);
+  hipLaunchKernelGGL((embed_sum_kernel<IO>), dim3(em_grid(jb, pieces)), dim3(256), 0, st, n, vocab, jb, keys, pos, dy,
+                     scale, part, dw);
   if (pieces > 1) {
     const int64_t groups = (pieces + kJoinWaves - 1) / kJoinWaves, columns = (dim + 255) / 256;
     const dim3 grid(static_cast<unsigned>(groups < (1 << 18) ? groups : (1 << 18)),
@@ -656,7 +662,7 @@ size_t sparc_embedding_workspace_bytes(int64_t n, int64_t vocab, int64_t dim) {
   const Sort s = sort_of(n, vocab);
   const int64_t pieces = (n + kPiece - 1) / kPiece;
   return 4 * up256(n * sizeof(uint32_t)) + up256((s.tiles << s.digit_bits) * sizeof(uint32_t)) +
-         up256(vocab) + up256(static_cast<size_t>(pieces) * 2 * dim * sizeof(float)) + 256;
+         up256(static_cast<size_t>(pieces) * 2 * dim * sizeof(float)) + 256;
 }
 
 sparc_status sparc_embedding_backward(int64_t n, int64_t vocab, int64_t dim, int32_t io_dtype, int32_t id_bytes,
@@ -676,29 +682,34 @@ sparc_status sparc_embedding_backward(int64_t n, int64_t vocab, int64_t dim, int
   uint32_t* keys[2] = {reinterpret_cast<uint32_t*>(take(n * 4)), reinterpret_cast<uint32_t*>(take(n * 4))};
   uint32_t* pos[2] = {reinterpret_cast<uint32_t*>(take(n * 4)), reinterpret_cast<uint32_t*>(take(n * 4))};
   uint32_t* counts = reinterpret_cast<uint32_t*>(take((s.tiles << s.digit_bits) * 4));
-  uint8_t* touched = reinterpret_cast<uint8_t*>(take(vocab));
   float* part = reinterpret_cast<float*>(at);
   SortPass p{};
   p.tokens = tokens;
   p.wide_ids = id_bytes == 8;
   p.vocab = vocab;
   p.pad = padding_id;
-  p.touched = touched;
   p.n = n;
   p.bits = s.digit_bits;
+  Clearing clear{static_cast<char*>(dweight), vocab * dim * (io_dtype == SPARC_F32 ? 4 : 2), 1};
   int cur = 0;
+  if (n == 0) {
+    hipLaunchKernelGGL((sort_count_kernel<4>), dim3(clear.take(p, kSortThreads)), dim3(kSortThreads), 0, st, p);
+    return op_launched("embedding backward");
+  }
   if (s.pos_bits) {
     p.keys_out = keys[0];
     p.pos_out = pos[0];
     p.first = 1;
-    hipLaunchKernelGGL((sort_local_kernel<kLocalItems>), dim3(1), dim3(kLocalThreads), 0, st, p, s.pos_bits, s.passes);
-  } else if (s.items == 4) {
-    cur = em_sort<4>(st, s, p, keys, pos, counts);
+    p.tiles = 1;
+    hipLaunchKernelGGL((sort_local_kernel<kLocalItems>), dim3(clear.take(p, kLocalThreads)), dim3(kLocalThreads), 0, st,
+                       p, s.pos_bits, s.passes);
   } else {
-    cur = em_sort<16>(st, s, p, keys, pos, counts);
+    clear.launches = s.passes;
+    cur = s.items == 4 ? em_sort<4>(st, s, p, clear, keys, pos, counts)
+                       : em_sort<16>(st, s, p, clear, keys, pos, counts);
   }
-  if (io_dtype == SPARC_F32) em_sums<float>(st, n, vocab, dim, keys[cur], pos[cur], touched, dy, scale, part, dweight);
-  else em_sums<sparc::bf16>(st, n, vocab, dim, keys[cur], pos[cur], touched, dy, scale, part, dweight);
+  if (io_dtype == SPARC_F32) em_sums<float>(st, n, vocab, dim, keys[cur], pos[cur], dy, scale, part, dweight);
+  else em_sums<sparc::bf16>(st, n, vocab, dim, keys[cur], pos[cur], dy, scale, part, dweight);
   return op_launched("embedding backward");
 }
 

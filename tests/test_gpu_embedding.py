@@ -74,6 +74,12 @@ def test_many_tokens():
     _check(70001, 3, 8, F32, "same")
 
 
+def test_few_tokens_of_a_large_vocabulary():
+    """Ids and positions that do not fit into 32 bits together."""
+    _check(3000, (1 << 21) + 5, 1, F32, "uniform")
+    _check(4096, (1 << 19) + 5, 1, F32, "zipf")
+
+
 @pytest.mark.parametrize("pad", [0, 5, -1])
 def test_padding_and_id_types(pad):
     _check(700, 40, 33, F32, "zipf", pad=pad)
