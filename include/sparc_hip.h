@@ -634,7 +634,8 @@ sparc_status sparc_embedding_backward(int64_t n, int64_t vocab, int64_t dim, int
  * sizes[i] values of dtypes[i] (sparc_dtype) on the device.  norm [1] fp32 = the
  * L2 norm over all values, accumulated in fp64 in a fixed order (0 without
  * values).  sparc_clip_grad_norm then multiplies every value by max_norm /
- * (norm + 1e-6) where that is below 1 (or NaN), and writes nothing otherwise. */
+ * (norm + 1e-6) where that is below 1 (or NaN), and writes nothing otherwise;
+ * its tensors must not overlap. */
 size_t sparc_grad_norm_workspace_bytes(int64_t count);
 sparc_status sparc_grad_norm(int64_t count, void* const* tensors, const int64_t* sizes, const int32_t* dtypes,
                              float* norm, void* workspace, size_t workspace_bytes, sparc_stream_t stream);

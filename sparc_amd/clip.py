@@ -47,8 +47,8 @@ def _call(fn_name, tensors, *args):
         _lib.require_gpu(*tensors)
     data = list(map(_Tensor.data_ptr, tensors))
     if len(set(data)) != len(data):
-        once = dict(zip(data, tensors))
-        data, tensors = list(once), list(once.values())
+        tensors = list({(p, t.numel(), t.dtype): t for p, t in zip(data, tensors)}.values())
+        data = list(map(_Tensor.data_ptr, tensors))
     n = len(data)
     sizes, codes = array("q", map(_Tensor.numel, tensors)), array("i", [_CODES[t.dtype] for t in tensors])
     data = array("Q", data)
@@ -85,7 +85,8 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     returns ``norm`` (``torch.nn.utils.clip_grad_norm_`` for the L2 norm).
 
     Nothing waits for the device and nothing is read back; where the norm is
-    small enough no gradient is written.  A norm that is not finite goes into
+    small enough no gradient is written.  Gradients that overlap without being
+    the same are refused.  A norm that is not finite goes into
     the gradients as it does in torch: NaN for NaN, 0 (NaN for the infinite
     values) for infinity.  Parameters without a gradient are skipped."""
     max_norm = float(max_norm)

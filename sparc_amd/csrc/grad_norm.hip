@@ -11,6 +11,9 @@
 // order, so the norm does not depend on timing and no launch stands between;
 // where nothing is clipped they read nothing more.
 
+#include <algorithm>
+#include <new>
+
 #include "rows.h"
 
 namespace sparc {
@@ -289,6 +292,28 @@ sparc_status gn_check(int64_t count, void* const* data, const int64_t* sizes, co
   return SPARC_OK;
 }
 
+// Tensors that are scaled must not share values: two workgroups would scale them
+// at once.
+sparc_status check_apart(int64_t count, void* const* data, const int64_t* sizes, const int32_t* dtypes) {
+  struct Span { uintptr_t at, end; };
+  Span* spans = new (std::nothrow) Span[static_cast<size_t>(count) + 1];
+  if (!spans) return op_fail(SPARC_EINVAL, "gradient clipping: no host memory for the tensor list");
+  int64_t n = 0;
+  bool sorted = true;
+  for (int64_t i = 0; i < count; ++i) {
+    if (sizes[i] == 0) continue;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(data[i]);
+    spans[n] = Span{at, at + static_cast<uintptr_t>(sizes[i]) * (dtypes[i] == SPARC_BF16 ? 2 : 4)};
+    sorted = sorted && (n == 0 || spans[n - 1].at <= at);
+    ++n;
+  }
+  if (!sorted) std::sort(spans, spans + n, [](const Span& a, const Span& b) { return a.at < b.at; });
+  bool apart = true;
+  for (int64_t i = 1; i < n; ++i) apart = apart && spans[i - 1].end <= spans[i].at;
+  delete[] spans;
+  return apart ? SPARC_OK : op_fail(SPARC_EINVAL, "gradient clipping: two tensors overlap");
+}
+
 // the partial sums of all lists, one behind the other; their number
 int launch_sums(hipStream_t st, int64_t count, void* const* data, const int64_t* sizes, const int32_t* dtypes,
                 double* part) {
@@ -338,6 +363,7 @@ sparc_status sparc_clip_grad_norm(int64_t count, void* const* tensors, const int
                                   sparc_stream_t stream) {
   using namespace sparc;
   if (sparc_status s = gn_check(count, tensors, sizes, dtypes)) return s;
+  if (sparc_status s = check_apart(count, tensors, sizes, dtypes)) return s;
   if (!(max_norm >= 0.0f)) return op_fail(SPARC_EINVAL, "gradient clipping: max_norm must be >= 0");
   if (!norm) return op_fail(SPARC_EINVAL, "gradient clipping: NULL pointer");
   if (!workspace || workspace_bytes < sparc_grad_norm_workspace_bytes(count))

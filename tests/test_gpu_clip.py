@@ -70,7 +70,7 @@ def test_alignment_and_order():
     flat = torch.randn(5000, device="cuda").mul_(0.02)
     params[0].grad = flat.bfloat16()[3:1203].view(40, 30)
     params[1].grad = flat[1:2146].view(33, 65)
-    params[2].grad = flat[:1000].view(20, 50).t()
+    params[2].grad = flat[3000:4000].view(20, 50).t()
     wide = flat[:400].bfloat16().view(20, 20)
     params[3].grad = wide[:, 2:11]
     rest = wide.clone()
@@ -87,6 +87,25 @@ def test_a_gradient_given_twice_counts_once():
     norm = sparc_amd.clip_grad_norm_([params[0], params[0]], 0.1)
     assert abs(float(norm) - L.grad_norm([g.cpu()])) <= 1e-6
     assert ((params[0].grad - g * (0.1 / float(norm))).abs() <= 1e-6 * g.abs() + 1e-12).all()
+
+
+def test_gradients_that_overlap_are_refused():
+    """Two workgroups would scale the shared values at once."""
+    print("[case] clip overlap", flush=True)
+    params = _params([(40,), (20,), (30,)], [F32] * 3, 11)
+    flat = torch.ones(100, device="cuda")
+    for a, b, c in ((flat[:40], flat[30:50], flat[60:90]), (flat[60:100], flat[:20], flat[40:70]),
+                    (flat[:40], flat[:20], flat[50:80])):
+        for p, g in zip(params, (a, b, c)):
+            p.grad = g
+        with pytest.raises(RuntimeError, match="overlap"):
+            sparc_amd.clip_grad_norm_(params, 0.5)
+        assert abs(float(sparc_amd.grad_norm([a, b, c])) - math.sqrt(90.0)) <= 1e-5
+    assert torch.equal(flat, torch.ones_like(flat))
+    for p, g in zip(params, (flat[40:80], flat[20:40], None)):  # side by side, in any order
+        p.grad = g
+    sparc_amd.clip_grad_norm_(params, 0.5)
+    assert flat[80:].eq(1.0).all() and flat[:20].eq(1.0).all() and flat[20:80].lt(1.0).all()
 
 
 @pytest.mark.parametrize("scale", [1e-30, 1e30])
