@@ -33,6 +33,23 @@ __device__ __forceinline__ int left(int64_t D, int64_t c) {
   return static_cast<int>(D - c < 64 ? D - c : 64);
 }
 
+// Whether every vector of a row may be read whole: what the last one reads of
+// the next row is still inside the array.  Only the array's last rows read
+// short vectors then, whose branches would make every row wait for each load
+// in turn.
+__device__ __forceinline__ bool reads_whole(int64_t row, int64_t R, int D, int v) {
+  return (row + 1) * D + v - 1 <= R * D;
+}
+// zeros behind the first n values
+template <typename IO>
+__device__ __forceinline__ void keep_first(Vec<IO>& raw, int n) {
+  float v[kVec<IO>];
+  unpack<IO, kVec<IO>>(raw, v);
+#pragma unroll
+  for (int i = 0; i < kVec<IO>; ++i) v[i] = i < n ? v[i] : 0.0f;
+  raw = pack<IO, kVec<IO>>(v);
+}
+
 // Sums of N values over the W waves that share a row, in every lane.  red: two
 // buffers used in turn (``turn``), so that one barrier per call is enough.
 template <int N, int W>
@@ -67,20 +84,31 @@ layer_norm_fwd_kernel(int64_t R, int D, const void* x, const void* w, const void
   int turn = 0;
   const int t = W == 1 ? (threadIdx.x & 63) : threadIdx.x;
   const int64_t per = W == 1 ? blockDim.x >> 6 : 1;
-  const int64_t first = W == 1 ? blockIdx.x * per + (threadIdx.x >> 6) : blockIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int64_t first = W == 1 ? blockIdx.x * per + wave : blockIdx.x;
   const float inv_d = 1.0f / static_cast<float>(D);
   for (int64_t row = first; row < R; row += gridDim.x * per) {  // uniform over the waves of a row
     const int64_t base = row * D;
     Vec<IO> raw[NCH];
+    if (WHOLE || reads_whole(row, R, D, V)) {
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) {
-      const int c = (k * 64 * W + t) * V;
-      if (c < D) raw[k] = load_vec<IO>(x, base + c, WHOLE ? V : D - c);
+      for (int k = 0; k < NCH; ++k) {
+        const int c = (k * 64 * W + t) * V;
+        if (c < D) raw[k] = load_vec<IO>(x, base + c, V);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < NCH; ++k) {
+        const int c = (k * 64 * W + t) * V;
+        if (c < D) raw[k] = load_vec<IO>(x, base + c, D - c);
+      }
     }
     float s[1] = {0.0f};
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      if ((k * 64 * W + t) * V < D) {
+      const int c = (k * 64 * W + t) * V;
+      if (c < D) {
+        if (!WHOLE && D - c < V) keep_first<IO>(raw[k], D - c);
         float v[V];
         unpack<IO, V>(raw[k], v);
 #pragma unroll
@@ -186,12 +214,23 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
   const float inv_d = 1.0f / static_cast<float>(D);
   int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + (W == 1 ? wave : 0);
   const auto load_row = [&](int64_t at, Vec<IO> (&xo)[NCH], Vec<IO> (&dyo)[NCH]) __attribute__((always_inline)) {
+    if (WHOLE || reads_whole(at, R, D, V)) {
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) {
-      const int c = (k * 64 * W + t) * V;
-      if (c < D) {
-        xo[k] = load_vec<IO>(x, at * D + c, WHOLE ? V : D - c);
-        dyo[k] = load_vec<IO>(dy, at * D + c, WHOLE ? V : D - c);
+      for (int k = 0; k < NCH; ++k) {
+        const int c = (k * 64 * W + t) * V;
+        if (c < D) {
+          xo[k] = load_vec<IO>(x, at * D + c, V);
+          dyo[k] = load_vec<IO>(dy, at * D + c, V);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < NCH; ++k) {
+        const int c = (k * 64 * W + t) * V;
+        if (c < D) {
+          xo[k] = load_vec<IO>(x, at * D + c, D - c);
+          dyo[k] = load_vec<IO>(dy, at * D + c, D - c);
+        }
       }
     }
   };
@@ -205,7 +244,12 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      if ((k * 64 * W + t) * V < D) {  // behind a short vector dy is zero
+      const int c = (k * 64 * W + t) * V;
+      if (c < D) {
+        if (!WHOLE && D - c < V) {
+          keep_first<IO>(xr[k], D - c);
+          keep_first<IO>(dr[k], D - c);
+        }
         float xv[V], dv[V], p[V];
         unpack<IO, V>(xr[k], xv);
         unpack<IO, V>(dr[k], dv);
@@ -242,6 +286,9 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
         if constexpr (kAhead) {
           xr[k] = xn[k];
           dr[k] = dn[k];
+        } else if (WHOLE ? row + step < R : reads_whole(row + step, R, D, V)) {
+          xr[k] = load_vec<IO>(x, (row + step) * D + c, V);
+          dr[k] = load_vec<IO>(dy, (row + step) * D + c, V);
         } else if (row + step < R) {
           xr[k] = load_vec<IO>(x, (row + step) * D + c, n);
           dr[k] = load_vec<IO>(dy, (row + step) * D + c, n);
@@ -466,12 +513,19 @@ bool ln_form(int64_t D, F&& f) {
   return false;
 }
 
-// Workgroups of the backward = partial rows: enough to fill the GPU (256 CUs
-// of 16 waves at its registers), never more than rows need.
-int64_t bwd_groups(int64_t R, int rows_at_once, int waves) {
-  const int64_t need = (R + rows_at_once - 1) / rows_at_once;
-  const int64_t fill = 256 * 16 / waves;
-  return need < fill ? need : fill;
+// Workgroups of the backward = partial rows: never more than rows need, and
+// enough to fill the GPU: 256 CUs of 16 waves at its registers, of 8 with 4
+// vectors per lane, which keep as much in flight (8192 x 1000 fp32: 21 against
+// 25 us; 32768 x 768 bf16, 2 vectors: 41 against 31).  With a workgroup per row,
+// a partial row costs as much as a row: 2 of these at least for each, and 8
+// behind the first 512 (944 x 2827 bf16 with the sum of the partial rows: 19
+// against 24 us, 4096 x 2880: 24 against 26).
+int64_t bwd_groups(int64_t R, int nch, int waves_per_row) {
+  const int64_t need = waves_per_row == 1 ? (R + kBwdRowWaves - 1) / kBwdRowWaves : (R + 1) / 2;
+  const int64_t fill = 256 * (nch >= 4 && waves_per_row < 16 ? 8 : 16) / (waves_per_row == 1 ? kBwdRowWaves : waves_per_row);
+  int64_t n = need < fill ? need : fill;
+  if (waves_per_row > 1 && n > 512) n = R / 8 > 512 ? (R / 8 < n ? R / 8 : n) : 512;
+  return n;
 }
 constexpr int64_t kMostPartials = 1024;  // the largest bwd_groups (W = 4)
 constexpr int64_t kWideSlices = 64;
@@ -525,7 +579,7 @@ sparc_status ln_backward(hipStream_t st, int64_t R, int64_t D, const void* x, co
   int64_t n = 0;
   const bool held = ln_form<IO>(D, [&](auto NCH, auto W) {
     const int waves = W() > 1 ? W() : kBwdRowWaves;
-    n = bwd_groups(R, W() > 1 ? 1 : kBwdRowWaves, waves);
+    n = bwd_groups(R, NCH(), W());
     if (dw && db) db_part = ws + n * D;
     const dim3 grid(static_cast<unsigned>(n)), block(64 * waves);
     if (D % kVec<IO> == 0)
