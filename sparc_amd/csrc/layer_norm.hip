@@ -8,11 +8,10 @@
 // once.  The variance is the mean of squared differences from the mean, taken
 // from registers, so a large mean costs no precision.
 //
-// A row is held in registers by the waves that own it: one wave, or a
-// workgroup of 4 or 16 waves for wider rows, each lane NCH vectors of 16 bytes
-// (at any alignment; a width that is no multiple ends in a shorter one).  Rows
-// too wide for that are read again for each pass over them (the *_wide
-// kernels).  The backward keeps the columns' sums of dy xhat and dy in
+// A row is held in registers by the L lanes that own it, 8 to 64 of a wave or a
+// workgroup of 256 to 1024, each NCH vectors of 16 bytes (at any alignment; a
+// width that is no multiple ends in a shorter one).  Rows too wide for that are
+// read again for each pass over them (the *_wide kernels).  The backward keeps the columns' sums of dy xhat and dy in
 // registers over the rows that its waves walk, beside the weight (in LDS for
 // the widest rows, whose registers are full), reads the next row while it works
 // on one, and writes one partial row per workgroup; a second kernel adds the
@@ -24,9 +23,10 @@
 namespace sparc {
 namespace {
 
-constexpr int kRowWaves = 4;       // forward, one wave per row: rows per workgroup (1 with few rows)
-constexpr int kBwdRowWaves = 8;    // backward, one wave per row: rows in flight per workgroup
-constexpr int64_t kFewRows = 1024; // below this a forward workgroup holds one row: one per CU before two
+constexpr int kRowWaves = 4;       // forward, up to a wave per row: waves per workgroup (1 with few rows)
+constexpr int kBwdRowWaves = 8;    // backward, up to a wave per row: waves per workgroup
+template <int L> constexpr int kBwdRows = L <= 64 ? kBwdRowWaves * 64 / L : 1;
+constexpr int64_t kFewRows = 1024; // below this a forward workgroup is one wave or one row: one per CU before two
 
 // columns from c on, as load_vec counts them
 __device__ __forceinline__ int left(int64_t D, int64_t c) {
@@ -50,12 +50,14 @@ __device__ __forceinline__ void keep_first(Vec<IO>& raw, int n) {
   raw = pack<IO, kVec<IO>>(v);
 }
 
-// Sums of N values over the W waves that share a row, in every lane.  red: two
-// buffers used in turn (``turn``), so that one barrier per call is enough.
-template <int N, int W>
+// Sums of N values over the L lanes that share a row, in each of them.  With
+// W waves, red: two buffers used in turn (``turn``), so that one barrier per
+// call is enough.
+template <int L> constexpr int kWaves = L > 64 ? L / 64 : 1;
+template <int N, int L, int W = kWaves<L>>
 __device__ __forceinline__ void row_sums(float (&v)[N], float (*red)[N][W], int& turn) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = group_sum(v[i], 64);
+  for (int i = 0; i < N; ++i) v[i] = group_sum(v[i], L < 64 ? L : 64);
   if constexpr (W > 1) {
     const int wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0) {
@@ -75,38 +77,38 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float (*red)[N][W], int&
 }
 
 // WHOLE: D is a multiple of the vector, so that no element needs a mask
-template <typename IO, typename PT, int NCH, int W, bool WHOLE>
-__global__ void __launch_bounds__(W == 1 ? 64 * kRowWaves : 64 * W)
+template <typename IO, typename PT, int NCH, int L, bool WHOLE>
+__global__ void __launch_bounds__(L <= 64 ? 64 * kRowWaves : L)
 layer_norm_fwd_kernel(int64_t R, int D, const void* x, const void* w, const void* b, float eps, void* y, float* mean,
                       float* rstd) {
   constexpr int V = kVec<IO>;
-  __shared__ float red[2][1][W];
+  __shared__ float red[2][1][kWaves<L>];
   int turn = 0;
-  const int t = W == 1 ? (threadIdx.x & 63) : threadIdx.x;
-  const int64_t per = W == 1 ? blockDim.x >> 6 : 1;
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  const int64_t first = W == 1 ? blockIdx.x * per + wave : blockIdx.x;
+  const int t = threadIdx.x & (L - 1), per = L <= 64 ? blockDim.x / L : 1;
+  int64_t first = static_cast<int64_t>(blockIdx.x) * per;
+  if constexpr (L == 64) first += __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  else if constexpr (L < 64) first += threadIdx.x / L;
   const float inv_d = 1.0f / static_cast<float>(D);
-  for (int64_t row = first; row < R; row += gridDim.x * per) {  // uniform over the waves of a row
+  for (int64_t row = first; row < R; row += static_cast<int64_t>(gridDim.x) * per) {  // uniform over a row's lanes
     const int64_t base = row * D;
     Vec<IO> raw[NCH];
     if (WHOLE || reads_whole(row, R, D, V)) {
 #pragma unroll
       for (int k = 0; k < NCH; ++k) {
-        const int c = (k * 64 * W + t) * V;
+        const int c = (k * L + t) * V;
         if (c < D) raw[k] = load_vec<IO>(x, base + c, V);
       }
     } else {
 #pragma unroll
       for (int k = 0; k < NCH; ++k) {
-        const int c = (k * 64 * W + t) * V;
+        const int c = (k * L + t) * V;
         if (c < D) raw[k] = load_vec<IO>(x, base + c, D - c);
       }
     }
     float s[1] = {0.0f};
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      const int c = (k * 64 * W + t) * V;
+      const int c = (k * L + t) * V;
       if (c < D) {
         if (!WHOLE && D - c < V) keep_first<IO>(raw[k], D - c);
         float v[V];
@@ -115,12 +117,12 @@ layer_norm_fwd_kernel(int64_t R, int D, const void* x, const void* w, const void
         for (int i = 0; i < V; ++i) s[0] += v[i];
       }
     }
-    row_sums<1, W>(s, red, turn);
+    row_sums<1, L>(s, red, turn);
     const float mu = s[0] * inv_d;
     s[0] = 0.0f;
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      const int c = (k * 64 * W + t) * V;
+      const int c = (k * L + t) * V;
       if (c < D) {
         float v[V];
         unpack<IO, V>(raw[k], v);
@@ -131,7 +133,7 @@ layer_norm_fwd_kernel(int64_t R, int D, const void* x, const void* w, const void
         }
       }
     }
-    row_sums<1, W>(s, red, turn);
+    row_sums<1, L>(s, red, turn);
     const float r = 1.0f / sqrtf(s[0] * inv_d + eps);
     if (t == 0 && mean) {
       mean[row] = mu;
@@ -139,7 +141,7 @@ layer_norm_fwd_kernel(int64_t R, int D, const void* x, const void* w, const void
     }
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      const int c = (k * 64 * W + t) * V;
+      const int c = (k * L + t) * V;
       if (c < D) {
         const int n = WHOLE ? V : D - c;
         float v[V], o[V];
@@ -164,12 +166,13 @@ layer_norm_fwd_kernel(int64_t R, int D, const void* x, const void* w, const void
   }
 }
 
-template <typename IO, typename PT, int NCH, int W, bool WHOLE>
-__global__ void __launch_bounds__(W == 1 ? 64 * kBwdRowWaves : 64 * W)
+template <typename IO, typename PT, int NCH, int L, bool WHOLE>
+__global__ void __launch_bounds__(L <= 64 ? 64 * kBwdRowWaves : L)
 layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const float* mean, const float* rstd,
                       const void* dy, void* dx, float* dw_part, float* db_part) {
   constexpr int V = kVec<IO>;
-  constexpr int kRows = W == 1 ? kBwdRowWaves : 1;  // rows a workgroup works on at once
+  constexpr int W = kWaves<L>;
+  constexpr int kRows = kBwdRows<L>;                // rows a workgroup works on at once
   constexpr int NP = V / kVec<PT>;                  // parameter vectors per vector of a row
   constexpr bool kWeightInLds = W == 16;
   // the next row into registers of its own while this one is worked on; with
@@ -177,9 +180,9 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
   // of the next row is read once this row's is done with
   constexpr bool kAhead = NCH * V <= 16;
   __shared__ float red[2][2][W];
-  __shared__ Vec<PT> w_lds[kWeightInLds ? NCH * 64 * W * NP : 1];
+  __shared__ Vec<PT> w_lds[kWeightInLds ? NCH * L * NP : 1];
   int turn = 0;
-  const int t = W == 1 ? (threadIdx.x & 63) : threadIdx.x;
+  const int t = threadIdx.x & (L - 1), lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
   Vec<IO> xr[NCH], dr[NCH];
@@ -187,7 +190,7 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
   float aw[NCH][V], ab[NCH][V];
 #pragma unroll
   for (int k = 0; k < NCH; ++k) {
-    const int c = (k * 64 * W + t) * V;
+    const int c = (k * L + t) * V;
 #pragma unroll
     for (int i = 0; i < V; ++i) { aw[k][i] = 0.0f; ab[k][i] = 0.0f; }
 #pragma unroll
@@ -197,7 +200,7 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
       for (int i = 0; i < kVec<PT>; ++i) ones[i] = 1.0f;
       Vec<PT> p = pack<PT, kVec<PT>>(ones);
       if (w && c < D) p = load_vec<PT>(w, c + q * kVec<PT>, WHOLE ? kVec<PT> : D - c - q * kVec<PT>);
-      if constexpr (kWeightInLds) w_lds[(k * 64 * W + t) * NP + q] = p;  // read back by this thread only
+      if constexpr (kWeightInLds) w_lds[(k * L + t) * NP + q] = p;  // read back by this thread only
       else wr[k][q] = p;
     }
   }
@@ -205,19 +208,21 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
 #pragma unroll
     for (int q = 0; q < NP; ++q) {
       float f[kVec<PT>];
-      if constexpr (kWeightInLds) unpack<PT, kVec<PT>>(w_lds[(k * 64 * W + t) * NP + q], f);
+      if constexpr (kWeightInLds) unpack<PT, kVec<PT>>(w_lds[(k * L + t) * NP + q], f);
       else unpack<PT, kVec<PT>>(wr[k][q], f);
 #pragma unroll
       for (int i = 0; i < kVec<PT>; ++i) p[q * kVec<PT> + i] = f[i];
     }
   };
   const float inv_d = 1.0f / static_cast<float>(D);
-  int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + (W == 1 ? wave : 0);
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kRows;
+  if constexpr (L == 64) row += wave;
+  else if constexpr (L < 64) row += threadIdx.x / L;
   const auto load_row = [&](int64_t at, Vec<IO> (&xo)[NCH], Vec<IO> (&dyo)[NCH]) __attribute__((always_inline)) {
     if (WHOLE || reads_whole(at, R, D, V)) {
 #pragma unroll
       for (int k = 0; k < NCH; ++k) {
-        const int c = (k * 64 * W + t) * V;
+        const int c = (k * L + t) * V;
         if (c < D) {
           xo[k] = load_vec<IO>(x, at * D + c, V);
           dyo[k] = load_vec<IO>(dy, at * D + c, V);
@@ -226,7 +231,7 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
     } else {
 #pragma unroll
       for (int k = 0; k < NCH; ++k) {
-        const int c = (k * 64 * W + t) * V;
+        const int c = (k * L + t) * V;
         if (c < D) {
           xo[k] = load_vec<IO>(x, at * D + c, D - c);
           dyo[k] = load_vec<IO>(dy, at * D + c, D - c);
@@ -235,7 +240,7 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
     }
   };
   if (row < R) load_row(row, xr, dr);
-  for (; row < R; row += step) {  // uniform over the waves of a row
+  for (; row < R; row += step) {  // uniform over a row's lanes
     Vec<IO> xn[kAhead ? NCH : 1], dn[kAhead ? NCH : 1];
     if constexpr (kAhead) {
       if (row + step < R) load_row(row + step, xn, dn);
@@ -244,7 +249,7 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      const int c = (k * 64 * W + t) * V;
+      const int c = (k * L + t) * V;
       if (c < D) {
         if (!WHOLE && D - c < V) {
           keep_first<IO>(xr[k], D - c);
@@ -264,11 +269,11 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
         }
       }
     }
-    row_sums<2, W>(s, red, turn);
+    row_sums<2, L>(s, red, turn);
     const float m0 = s[0] * inv_d, m1 = s[1] * inv_d;
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      const int c = (k * 64 * W + t) * V;
+      const int c = (k * L + t) * V;
       if (c < D) {
         const int n = WHOLE ? V : D - c;
         if (dx) {
@@ -296,29 +301,34 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
       }
     }
   }
-  // one partial row per workgroup; with a wave per row, its waves' sums are
-  // added first, wave 0, 1, 2, ...
+  // one partial row per workgroup; where it has several rows in hand, their sums
+  // are added first, those of a wave and then wave 0, 1, 2, ...
   __shared__ float4 lds[W == 1 ? kBwdRowWaves - 1 : 1][V / 4][64];
   const auto write = [&](float (&a)[NCH][V], float* part) __attribute__((always_inline)) {
     const int64_t out = static_cast<int64_t>(blockIdx.x) * D;
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      const int c = (k * 64 * W + t) * V;
+      const int c = (k * L + t) * V;
 #pragma unroll
       for (int q = 0; q < V / 4; ++q) {
+#pragma unroll
+        for (int o = L; o < 64; o <<= 1) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) a[k][4 * q + i] += __shfl_xor(a[k][4 * q + i], o);
+        }
         float4 u = make_float4(a[k][4 * q], a[k][4 * q + 1], a[k][4 * q + 2], a[k][4 * q + 3]);
         if constexpr (W == 1) {
-          if (wave > 0) lds[wave - 1][q][t] = u;
+          if (wave > 0) lds[wave - 1][q][lane] = u;
           __syncthreads();
           if (wave == 0) {
             for (int v = 0; v < kBwdRowWaves - 1; ++v) {
-              const float4 o = lds[v][q][t];
+              const float4 o = lds[v][q][lane];
               u.x += o.x; u.y += o.y; u.z += o.z; u.w += o.w;
             }
           }
           __syncthreads();
         }
-        if ((W > 1 || wave == 0) && c + 4 * q < D) store_vec<float>(part, out + c + 4 * q, D - c - 4 * q, u);
+        if ((W > 1 || (wave == 0 && lane < L)) && c + 4 * q < D) store_vec<float>(part, out + c + 4 * q, D - c - 4 * q, u);
       }
     }
   };
@@ -345,7 +355,7 @@ layer_norm_fwd_wide_kernel(int64_t R, int64_t D, const void* x, const void* w, c
 #pragma unroll
       for (int i = 0; i < V; ++i) s[0] += v[i];
     }
-    row_sums<1, kWideThreads / 64>(s, red, turn);
+    row_sums<1, kWideThreads>(s, red, turn);
     const float mu = s[0] * inv_d;
     s[0] = 0.0f;
     for (int64_t c = c0; c < D; c += kWideThreads * V) {
@@ -357,7 +367,7 @@ layer_norm_fwd_wide_kernel(int64_t R, int64_t D, const void* x, const void* w, c
         s[0] = fmaf(d, d, s[0]);
       }
     }
-    row_sums<1, kWideThreads / 64>(s, red, turn);
+    row_sums<1, kWideThreads>(s, red, turn);
     const float r = 1.0f / sqrtf(s[0] * inv_d + eps);
     if (threadIdx.x == 0 && mean) {
       mean[row] = mu;
@@ -412,7 +422,7 @@ layer_norm_dx_wide_kernel(int64_t R, int64_t D, const void* x, const void* w, co
         s[1] = fmaf(g[i], xh[i], s[1]);
       }
     }
-    row_sums<2, kWideThreads / 64>(s, red, turn);
+    row_sums<2, kWideThreads>(s, red, turn);
     const float m0 = s[0] * inv_d, m1 = s[1] * inv_d;
     for (int64_t c = c0; c < D; c += kWideThreads * V) {
       const int n = left(D, c);
@@ -488,28 +498,65 @@ layer_norm_reduce_kernel(int n, int64_t D, const float* dw_part, const float* db
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-// f(NCH, W) for the narrowest form that holds a row of D columns in registers:
-// up to 16 columns per lane with 1 or 4 waves, 32 (16 in fp32) with 16 (the
-// backward holds two fp32 sums per column beside two rows of x and dy).
+// f(NCH, L) for the narrowest form that holds a row of D columns in registers, L
+// lanes with NCH vectors each, so that few lanes idle and as few waves as can
+// hold a row wait for one another (a wave per row: 88 us instead of 30 for
+// 300000 x 120 bf16; 1024 lanes with one vector each: 129 instead of 75 for
+// 20000 x 5000).  With few rows a lane's chain of vectors is what takes time: one
+// vector each up to 1024 lanes (4 x 2048 bf16: 2.7 us, 4 vectors in one wave 3.5).
 // False: wider than that.
 template <typename IO, typename F>
-bool ln_form(int64_t D, F&& f) {
-  constexpr int64_t P = 64 * kVec<IO>;  // columns per wave and vector
-  if (D <= P) return f(Int<1>{}, Int<1>{}), true;
-  if (D <= 2 * P) return f(Int<2>{}, Int<1>{}), true;
+bool fwd_form(int64_t R, int64_t D, F&& f) {
+  const int64_t vecs = (D + kVec<IO> - 1) / kVec<IO>;
+  if (R < kFewRows && vecs > 64 && vecs <= 256) return f(Int<1>{}, Int<256>{}), true;
+  if (R < kFewRows && vecs > 512 && vecs <= 1024) return f(Int<1>{}, Int<1024>{}), true;
+  if (vecs <= 8) return f(Int<1>{}, Int<8>{}), true;
+  if (vecs <= 16) return f(Int<1>{}, Int<16>{}), true;
+  if (vecs <= 32) return f(Int<1>{}, Int<32>{}), true;
+  if (vecs <= 64) return f(Int<1>{}, Int<64>{}), true;
+  if (vecs <= 96) return f(Int<3>{}, Int<32>{}), true;
+  if (vecs <= 128) return f(Int<2>{}, Int<64>{}), true;
+  if (vecs <= 192) return f(Int<3>{}, Int<64>{}), true;
+  if (vecs <= 256) return f(Int<4>{}, Int<64>{}), true;
+  if (vecs <= 512) return f(Int<2>{}, Int<256>{}), true;
+  if (vecs <= 768) return f(Int<3>{}, Int<256>{}), true;
+  if (vecs <= 1024) return f(Int<4>{}, Int<256>{}), true;
+  if (vecs <= 1536) return f(Int<3>{}, Int<512>{}), true;
+  if (vecs <= 2048) return f(Int<2>{}, Int<1024>{}), true;
+  if (vecs <= 3 * 1024) return f(Int<3>{}, Int<1024>{}), true;
+  if (vecs <= 4096) return f(Int<4>{}, Int<1024>{}), true;
+  return false;
+}
+// The backward holds two fp32 sums per column beside two rows of x and dy: up to
+// 16 columns per lane, 32 (16 in fp32) with 1024 lanes.
+template <typename IO, typename F>
+bool bwd_form(int64_t D, F&& f) {
+  const int64_t vecs = (D + kVec<IO> - 1) / kVec<IO>;
+  if (vecs <= 8) return f(Int<1>{}, Int<8>{}), true;
+  if (vecs <= 16) return f(Int<1>{}, Int<16>{}), true;
+  if (vecs <= 32) return f(Int<1>{}, Int<32>{}), true;
+  if (vecs <= 64) return f(Int<1>{}, Int<64>{}), true;
   if constexpr (sizeof(IO) == 4) {
-    if (D <= 3 * P) return f(Int<3>{}, Int<1>{}), true;
-    if (D <= 4 * P) return f(Int<4>{}, Int<1>{}), true;
+    if (vecs <= 96) return f(Int<3>{}, Int<32>{}), true;
   }
-  if (D <= 4 * P) return f(Int<1>{}, Int<4>{}), true;
-  if (D <= 8 * P) return f(Int<2>{}, Int<4>{}), true;
+  if (vecs <= 128) return f(Int<2>{}, Int<64>{}), true;
   if constexpr (sizeof(IO) == 4) {
-    if (D <= 16 * P) return f(Int<4>{}, Int<4>{}), true;
+    if (vecs <= 192) return f(Int<3>{}, Int<64>{}), true;
+    if (vecs <= 256) return f(Int<4>{}, Int<64>{}), true;
   }
-  if (D <= 16 * P) return f(Int<1>{}, Int<16>{}), true;
-  if (D <= 32 * P) return f(Int<2>{}, Int<16>{}), true;
-  if (D <= 48 * P) return f(Int<3>{}, Int<16>{}), true;
-  if (D <= 64 * P) return f(Int<4>{}, Int<16>{}), true;
+  if constexpr (sizeof(IO) == 2) {
+    if (vecs <= 256) return f(Int<1>{}, Int<256>{}), true;
+  }
+  if (vecs <= 512) return f(Int<2>{}, Int<256>{}), true;
+  if constexpr (sizeof(IO) == 4) {
+    if (vecs <= 768) return f(Int<3>{}, Int<256>{}), true;
+    if (vecs <= 1024) return f(Int<4>{}, Int<256>{}), true;
+  } else {
+    if (vecs <= 1024) return f(Int<1>{}, Int<1024>{}), true;
+  }
+  if (vecs <= 2048) return f(Int<2>{}, Int<1024>{}), true;
+  if (vecs <= 3 * 1024) return f(Int<3>{}, Int<1024>{}), true;
+  if (vecs <= 4096) return f(Int<4>{}, Int<1024>{}), true;
   return false;
 }
 
@@ -520,11 +567,12 @@ bool ln_form(int64_t D, F&& f) {
 // a partial row costs as much as a row: 2 of these at least for each, and 8
 // behind the first 512 (944 x 2827 bf16 with the sum of the partial rows: 19
 // against 24 us, 4096 x 2880: 24 against 26).
-int64_t bwd_groups(int64_t R, int nch, int waves_per_row) {
-  const int64_t need = waves_per_row == 1 ? (R + kBwdRowWaves - 1) / kBwdRowWaves : (R + 1) / 2;
-  const int64_t fill = 256 * (nch >= 4 && waves_per_row < 16 ? 8 : 16) / (waves_per_row == 1 ? kBwdRowWaves : waves_per_row);
+template <int NCH, int L>
+int64_t bwd_groups(int64_t R) {
+  const int64_t need = L <= 64 ? (R + kBwdRows<L> - 1) / kBwdRows<L> : (R + 1) / 2;
+  const int64_t fill = 256 * (NCH >= 4 && L < 1024 ? 8 : 16) / (L <= 64 ? kBwdRowWaves : kWaves<L>);
   int64_t n = need < fill ? need : fill;
-  if (waves_per_row > 1 && n > 512) n = R / 8 > 512 ? (R / 8 < n ? R / 8 : n) : 512;
+  if (L > 64 && n > 512) n = R / 8 > 512 ? (R / 8 < n ? R / 8 : n) : 512;
   return n;
 }
 constexpr int64_t kMostPartials = 1024;  // the largest bwd_groups (W = 4)
@@ -555,14 +603,14 @@ sparc_status ln_check(int64_t rows, int64_t cols, int32_t io, int32_t pt) {
 template <typename IO, typename PT>
 sparc_status ln_forward(hipStream_t st, int64_t R, int64_t D, const void* x, const void* w, const void* b, float eps,
                         void* y, float* mean, float* rstd) {
-  const bool held = ln_form<IO>(D, [&](auto NCH, auto W) {
-    const int per = W() > 1 ? 1 : (R < kFewRows ? 1 : kRowWaves);
-    const dim3 grid(op_grid((R + per - 1) / per)), block(64 * (W() > 1 ? W() : per));
+  const bool held = fwd_form<IO>(R, D, [&](auto NCH, auto L) {
+    const int threads = L() > 64 ? L() : (R < kFewRows ? 64 : 64 * kRowWaves), per = threads / L();
+    const dim3 grid(op_grid((R + per - 1) / per)), block(threads);
     if (D % kVec<IO> == 0)
-      hipLaunchKernelGGL((layer_norm_fwd_kernel<IO, PT, NCH(), W(), true>), grid, block, 0, st, R, static_cast<int>(D),
+      hipLaunchKernelGGL((layer_norm_fwd_kernel<IO, PT, NCH(), L(), true>), grid, block, 0, st, R, static_cast<int>(D),
                          x, w, b, eps, y, mean, rstd);
     else
-      hipLaunchKernelGGL((layer_norm_fwd_kernel<IO, PT, NCH(), W(), false>), grid, block, 0, st, R,
+      hipLaunchKernelGGL((layer_norm_fwd_kernel<IO, PT, NCH(), L(), false>), grid, block, 0, st, R,
                          static_cast<int>(D), x, w, b, eps, y, mean, rstd);
   });
   if (!held)
@@ -577,16 +625,15 @@ sparc_status ln_backward(hipStream_t st, int64_t R, int64_t D, const void* x, co
   float* dw_part = dw ? ws : nullptr;
   float* db_part = db ? ws : nullptr;  // behind dw's partial rows where there are any
   int64_t n = 0;
-  const bool held = ln_form<IO>(D, [&](auto NCH, auto W) {
-    const int waves = W() > 1 ? W() : kBwdRowWaves;
-    n = bwd_groups(R, NCH(), W());
+  const bool held = bwd_form<IO>(D, [&](auto NCH, auto L) {
+    n = bwd_groups<NCH(), L()>(R);
     if (dw && db) db_part = ws + n * D;
-    const dim3 grid(static_cast<unsigned>(n)), block(64 * waves);
+    const dim3 grid(static_cast<unsigned>(n)), block(L() > 64 ? L() : 64 * kBwdRowWaves);
     if (D % kVec<IO> == 0)
-      hipLaunchKernelGGL((layer_norm_bwd_kernel<IO, PT, NCH(), W(), true>), grid, block, 0, st, R, static_cast<int>(D),
+      hipLaunchKernelGGL((layer_norm_bwd_kernel<IO, PT, NCH(), L(), true>), grid, block, 0, st, R, static_cast<int>(D),
                          x, w, mean, rstd, dy, dx, dw_part, db_part);
     else
-      hipLaunchKernelGGL((layer_norm_bwd_kernel<IO, PT, NCH(), W(), false>), grid, block, 0, st, R,
+      hipLaunchKernelGGL((layer_norm_bwd_kernel<IO, PT, NCH(), L(), false>), grid, block, 0, st, R,
                          static_cast<int>(D), x, w, mean, rstd, dy, dx, dw_part, db_part);
   });
   if (!held) {
