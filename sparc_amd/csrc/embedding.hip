@@ -12,11 +12,11 @@
 // stand together in their order in the batch.  Up to 4096 positions one
 // workgroup sorts them in LDS, ids and positions packed into 32 bits; more of
 // them, or ids that do not fit beside the positions, take a counting and a
-// scattering launch per pass.  Pieces of
-// kPiece sorted positions are then summed side by side, whatever the ids'
-// frequencies: a run of equal ids inside a piece is written to its row at
-// once; a run that crosses pieces leaves one fp32 partial row per piece,
-// joined in order by a second kernel.  Every sum has a fixed order, so dW does
+// scattering launch per pass (and one between them with many tiles).  Pieces of
+// sorted positions are then summed side by side, whatever the ids' frequencies:
+// a run of equal ids inside a piece is written to its row at once; a run that
+// crosses pieces leaves one fp32 partial row per piece, joined in order by a
+// second kernel.  Every sum has a fixed order, so dW does
 // not depend on timing.  The sort keeps few CUs busy and is bound by latency, so
 // further workgroups of its launches clear dW meanwhile, a share each; the rows
 // that tokens name are then written once more.
@@ -26,11 +26,7 @@
 namespace sparc {
 namespace {
 
-// Sorted positions per piece, all read at once.  8 against 16, the summing and
-// the joining kernel: 37 against 35 us for 32768 x 768 bf16 gradients, 43
-// against 48 us for 3711 x 1001 fp32 ones into 50001 rows, where the pieces are
-// few.
-constexpr int kPiece = 8;
+constexpr int kBatch = 8;           // sorted positions that a lane reads at once
 constexpr int kSortThreads = 256;   // 4 waves per sort tile
 constexpr int kSortWaves = kSortThreads / 64;
 constexpr int kMaxDigits = 512;     // 9 bits
@@ -39,6 +35,9 @@ constexpr int kLocalWaves = kLocalThreads / 64;
 constexpr int kLocalItems = 4;      // per thread
 constexpr int kJoinWaves = 8;       // pieces per join workgroup
 constexpr int kLongRun = 16;        // pieces of a run that a whole join workgroup adds up
+// With more tiles than that a launch of its own sums their counts, else every
+// scattering workgroup does (65 tiles: 28 against 31 us; 256: 48 against 33).
+constexpr int kManyTiles = 96;
 constexpr uint32_t kNone = 0xffffffffu;
 
 // Jobs of a group of lpr lanes (a power of two up to 64): one block of lpr
@@ -94,6 +93,7 @@ struct SortPass {
   uint32_t* keys_out;
   uint32_t* pos_out;
   uint32_t* counts;       // [tiles][digits] of this pass
+  uint32_t* totals;       // [digits]; NULL: the counts are not yet summed over the tiles
   int64_t n;
   int shift, bits;
   int first;
@@ -160,6 +160,33 @@ sort_count_kernel(SortPass p) {
     p.counts[static_cast<int64_t>(blockIdx.x) * digits + d] = hist[d];
 }
 
+// With many tiles: turns each tile's counts into those of the tiles before it, and
+// leaves the digits' totals.  kScanDigits digits per workgroup, each by
+// kScanSlices slices of the tiles.
+constexpr int kScanDigits = 16;
+constexpr int kScanSlices = 64;
+__global__ void __launch_bounds__(kScanDigits * kScanSlices)
+sort_scan_kernel(SortPass p) {
+  __shared__ uint32_t sums[kScanSlices][kScanDigits];
+  const int digits = 1 << p.bits, d = threadIdx.x % kScanDigits, slice = threadIdx.x / kScanDigits;
+  const int digit = blockIdx.x * kScanDigits + d, each = (p.tiles + kScanSlices - 1) / kScanSlices;
+  const int t0 = slice * each, t1 = t0 + each < p.tiles ? t0 + each : p.tiles;
+  uint32_t* const at = p.counts + (digit < digits ? digit : 0);
+  uint32_t sum = 0;
+  for (int t = t0; t < t1; ++t) sum += at[static_cast<int64_t>(t) * digits];
+  sums[slice][d] = sum;
+  __syncthreads();
+  if (digit >= digits) return;
+  uint32_t before = 0;
+  for (int k = 0; k < slice; ++k) before += sums[k][d];
+  for (int t = t0; t < t1; ++t) {
+    const uint32_t own = at[static_cast<int64_t>(t) * digits];
+    at[static_cast<int64_t>(t) * digits] = before;
+    before += own;
+  }
+  if (slice == kScanSlices - 1) p.totals[digit] = before;
+}
+
 // Moves each tile's positions behind all positions of smaller digits and those
 // of its own digit in earlier tiles.  A wave ranks its 64 * ITEMS consecutive
 // positions 64 at a time: the lanes of equal digit are found by one ballot per
@@ -190,7 +217,15 @@ sort_scatter_kernel(SortPass p) {
   uint32_t before[2] = {0, 0}, total[2] = {0, 0};
   if (2 * static_cast<int>(threadIdx.x) < digits) {
     const uint2* counts = reinterpret_cast<const uint2*>(p.counts) + threadIdx.x;
-    const int tiles = p.tiles, mine = blockIdx.x;
+    const int tiles = p.totals ? 0 : p.tiles, mine = blockIdx.x;
+    if (p.totals) {
+      const uint2 b = counts[static_cast<int64_t>(mine) * (digits / 2)];
+      const uint2 all = reinterpret_cast<const uint2*>(p.totals)[threadIdx.x];
+      before[0] = b.x;
+      before[1] = b.y;
+      total[0] = all.x;
+      total[1] = all.y;
+    }
     for (int t0 = 0; t0 < tiles; t0 += 16) {
       uint2 c[16];
 #pragma unroll
@@ -364,66 +399,67 @@ __device__ __host__ __forceinline__ int64_t part_columns(int64_t D) { return (D 
 // one that begins here and goes on into the next (1).
 template <typename IO>
 __global__ void __launch_bounds__(256)
-embed_sum_kernel(int64_t N, int64_t vocab, Jobs jb, const uint32_t* keys, const uint32_t* pos, const void* dy,
+embed_sum_kernel(int64_t N, int piece_len, int64_t vocab, Jobs jb, const uint32_t* keys, const uint32_t* pos, const void* dy,
                  float scale, float* part, void* dw) {
   constexpr int V = kVec<IO>;
   const int D = jb.D;
   const int64_t last = N * D - V;  // where the gradient's last whole vector begins
-  const int64_t per = 256 / jb.lpr, pieces = (N + kPiece - 1) / kPiece, jobs = pieces * jb.blocks;
+  const int64_t per = 256 / jb.lpr, pieces = (N + piece_len - 1) / piece_len, jobs = pieces * jb.blocks;
   for (int64_t job = blockIdx.x * per + threadIdx.x / jb.lpr; job < jobs; job += gridDim.x * per) {
     int c;
     const int64_t piece = jb.row_of<V>(job, c);
     if (c >= D) continue;
-    const int64_t p0 = piece * kPiece;
-    const int n = N - p0 < kPiece ? static_cast<int>(N - p0) : kPiece;
-    uint32_t key[kPiece], at[kPiece];
-#pragma unroll
-    for (int i = 0; i < kPiece; ++i) {
-      const int64_t p = p0 + (i < n ? i : n - 1);
-      key[i] = keys[p];
-      at[i] = pos[p];
-    }
-#pragma unroll
-    for (int i = 0; i < kPiece; ++i) key[i] = i < n ? key[i] : kNone;
-    const uint32_t prev = p0 > 0 ? keys[p0 - 1] : kNone;
-    const uint32_t next = p0 + n < N ? keys[p0 + n] : kNone;
+    const int64_t p0 = piece * piece_len, p1 = p0 + piece_len < N ? p0 + piece_len : N;
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-    bool head = prev == key[0];  // the run in hand goes on from the piece before
-    // All rows at once, also those that take no part, and whole vectors, whose
-    // last values may be those of the next row: without a branch around them no
-    // load waits for another.
-    int64_t from[kPiece];
-    Vec<IO> raw[kPiece];
+    bool head = false;  // the run in hand goes on from the piece before
+    for (int64_t p = p0; p < p1; p += kBatch) {
+      uint32_t key[kBatch + 1], at[kBatch];
 #pragma unroll
-    for (int i = 0; i < kPiece; ++i) from[i] = static_cast<int64_t>(at[i]) * D + c;
-    if (key[0] < static_cast<uint32_t>(vocab) && last >= 0) {  // else none does
+      for (int i = 0; i <= kBatch; ++i) {
+        const int64_t q = p + i < N ? p + i : N - 1;
+        key[i] = keys[q];
+        if (i < kBatch) at[i] = pos[q];
+      }
+      if (p == p0) head = p0 > 0 && keys[p0 - 1] == key[0];
+      if (key[0] >= static_cast<uint32_t>(vocab)) break;  // those that take no part stand behind all others
 #pragma unroll
-      for (int i = 0; i < kPiece; ++i) raw[i] = load_vec<IO>(dy, from[i] < last ? from[i] : last, V);
-    }
+      for (int i = 1; i <= kBatch; ++i) key[i] = p + i < N ? key[i] : kNone;
+      // All rows at once, also those that take no part, and whole vectors, whose
+      // last values may be those of the next row: without a branch around them no
+      // load waits for another.
+      int64_t from[kBatch];
+      Vec<IO> raw[kBatch];
 #pragma unroll
-    for (int i = 0; i < kPiece; ++i) {
-      if (key[i] < static_cast<uint32_t>(vocab)) {  // what follows is vocab or kNone only
-        if (from[i] > last) raw[i] = load_vec<IO>(dy, from[i], D - c);
-        float v[V];
-        unpack<IO, V>(raw[i], v);
+      for (int i = 0; i < kBatch; ++i) from[i] = static_cast<int64_t>(at[i]) * D + c;
+      if (last >= 0) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) acc[k] += v[k];
-        const uint32_t after = i + 1 < kPiece && i + 1 < n ? key[i + 1 < kPiece ? i + 1 : i] : next;
-        const bool end = i + 1 == n;
-        if (end || after != key[i]) {
-          if (head || after == key[i]) {
-            float* to = part + (piece * 2 + (head ? 0 : 1)) * part_columns(D) + c;
+        for (int i = 0; i < kBatch; ++i) raw[i] = load_vec<IO>(dy, from[i] < last ? from[i] : last, V);
+      }
 #pragma unroll
-            for (int q = 0; q < V; q += 4)
-              if (c + q < D) *reinterpret_cast<float4*>(to + q) = make_float4(acc[q], acc[q + 1], acc[q + 2], acc[q + 3]);
-          } else {
-            write_row<IO>(dw, key[i], D, c, acc, scale);
+      for (int i = 0; i < kBatch; ++i) {
+        if (p + i < p1 && key[i] < static_cast<uint32_t>(vocab)) {
+          if (from[i] > last) raw[i] = load_vec<IO>(dy, from[i], D - c);
+          float v[V];
+          unpack<IO, V>(raw[i], v);
+#pragma unroll
+          for (int k = 0; k < V; ++k) acc[k] += v[k];
+          const bool more = key[i + 1] == key[i];
+          if (!more || p + i + 1 == p1) {
+            if (head || more) {
+              float* to = part + (piece * 2 + (head ? 0 : 1)) * part_columns(D) + c;
+#pragma unroll
+              for (int q = 0; q < V; q += 4)
+                if (c + q < D)
+                  *reinterpret_cast<float4*>(to + q) = make_float4(acc[q], acc[q + 1], acc[q + 2], acc[q + 3]);
+            } else {
+              write_row<IO>(dw, key[i], D, c, acc, scale);
+            }
+            head = false;
+#pragma unroll
+            for (int k = 0; k < V; ++k) acc[k] = 0.0f;
           }
-          head = false;
-#pragma unroll
-          for (int k = 0; k < V; ++k) acc[k] = 0.0f;
         }
       }
     }
@@ -458,15 +494,15 @@ __device__ __forceinline__ void add_parts(float (&s)[4], const float* part, int6
 // block of 256 columns.
 template <typename IO>
 __global__ void __launch_bounds__(64 * kJoinWaves)
-embed_join_kernel(int64_t N, int64_t vocab, int D, const uint32_t* keys, float scale, const float* part, void* dw) {
+embed_join_kernel(int64_t N, int piece_len, int64_t vocab, int D, const uint32_t* keys, float scale, const float* part, void* dw) {
   __shared__ float4 red[kJoinWaves][64];
   __shared__ int64_t long_first[kJoinWaves], long_last[kJoinWaves];
   __shared__ uint32_t long_key[kJoinWaves];
-  const int64_t pieces = (N + kPiece - 1) / kPiece;
+  const int64_t pieces = (N + piece_len - 1) / piece_len;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   for (int64_t piece0 = static_cast<int64_t>(blockIdx.x) * kJoinWaves; piece0 + 1 < pieces;
        piece0 += static_cast<int64_t>(gridDim.x) * kJoinWaves) {
-    const int64_t piece = piece0 + wave, p0 = piece * kPiece, p1 = p0 + kPiece;
+    const int64_t piece = piece0 + wave, p0 = piece * piece_len, p1 = p0 + piece_len;
     bool begins = piece + 1 < pieces;
     uint32_t key = kNone;
     if (begins) {
@@ -480,11 +516,11 @@ embed_join_kernel(int64_t N, int64_t vocab, int D, const uint32_t* keys, float s
       // the last piece that begins with the key: those that do are consecutive.
       // The next 64 first, then a search with 64 probes a time
       const int64_t q = piece + 1 + lane;
-      last = piece + __popcll(__ballot(q < pieces && keys[q * kPiece] == key));
+      last = piece + __popcll(__ballot(q < pieces && keys[q * piece_len] == key));
       if (last == piece + 64) {
         for (int64_t end = pieces; end - last > 1;) {  // ``last`` does, ``end`` does not
           const int64_t step = (end - last + 63) / 64, probe = last + (lane + 1) * step;
-          const int more = __popcll(__ballot(probe < end && keys[probe * kPiece] == key));
+          const int more = __popcll(__ballot(probe < end && keys[probe * piece_len] == key));
           const int64_t beyond = last + (more + 1) * step;
           last += more * step;
           end = beyond < end ? beyond : end;
@@ -563,7 +599,9 @@ Sort sort_of(int64_t n, int64_t vocab) {
   while ((vocab >> s.bits) > 0) ++s.bits;  // keys 0 .. vocab
   s.passes = (s.bits + 8) / 9;
   s.digit_bits = (s.bits + s.passes - 1) / s.passes;
-  s.items = n <= 65536 ? 4 : 16;  // at most 64 tiles' counts to add up, then tiles four times the size
+  // positions per thread: the whole sort of 524288 positions 41 us with 4, 49 with
+  // 16; of 2^22 169 and 130
+  s.items = n <= (1 << 20) ? 4 : 16;
   s.tiles = (n + kSortThreads * s.items - 1) / (kSortThreads * s.items);
   s.pos_bits = 1;
   while ((n - 1) >> s.pos_bits > 0) ++s.pos_bits;
@@ -623,6 +661,7 @@ int em_sort(hipStream_t st, const Sort& s, SortPass p, Clearing clear, uint32_t*
   int cur = 0;
   p.counts = counts;
   p.tiles = static_cast<int>(s.tiles);
+  if (s.tiles > kManyTiles) p.totals = counts + (s.tiles << s.digit_bits);
   for (int k = 0; k < s.passes; ++k) {
     p.keys_in = keys[cur ^ 1];
     p.pos_in = pos[cur ^ 1];
@@ -632,6 +671,9 @@ int em_sort(hipStream_t st, const Sort& s, SortPass p, Clearing clear, uint32_t*
     p.first = k == 0;
     // the counts are over too soon to hide a share
     hipLaunchKernelGGL((sort_count_kernel<ITEMS>), dim3(p.tiles), dim3(kSortThreads), 0, st, p);
+    if (p.totals)
+      hipLaunchKernelGGL(sort_scan_kernel, dim3(((1 << p.bits) + kScanDigits - 1) / kScanDigits),
+                         dim3(kScanDigits * kScanSlices), 0, st, p);
     const unsigned grid = clear.take(p, kSortThreads);
     hipLaunchKernelGGL((sort_scatter_kernel<ITEMS>), dim3(grid), dim3(kSortThreads), 0, st, p);
     cur ^= 1;
@@ -639,18 +681,29 @@ int em_sort(hipStream_t st, const Sort& s, SortPass p, Clearing clear, uint32_t*
   return cur ^ 1;
 }
 
+// Sorted positions per piece: as few as are read at once, unless the GPU (256 CUs
+// of 16 waves) is full with longer pieces too, whose partial rows are fewer and
+// long runs sooner joined (both kernels, 524288 rows of 64 bf16 values: 68 us in
+// pieces of 8, 41 in pieces of 32).
+int piece_of(int64_t n, int64_t dim) {
+  int piece = kBatch;
+  while (piece < 1024 && n * dim >= static_cast<int64_t>(2 * piece) << 20) piece *= 2;
+  return piece;
+}
+
 template <typename IO>
 void em_sums(hipStream_t st, int64_t n, int64_t vocab, int64_t dim, const uint32_t* keys, const uint32_t* pos,
              const void* dy, float scale, float* part, void* dw) {
-  const int64_t pieces = (n + kPiece - 1) / kPiece;
+  const int piece = piece_of(n, dim);
+  const int64_t pieces = (n + piece - 1) / piece;
   const Jobs jb = em_jobs(dim, kVec<IO>);
-  hipLaunchKernelGGL((embed_sum_kernel<IO>), dim3(em_grid(jb, pieces)), dim3(256), 0, st, n, vocab, jb, keys, pos, dy,
+  hipLaunchKernelGGL((embed_sum_kernel<IO>), dim3(em_grid(jb, pieces)), dim3(256), 0, st, n, piece, vocab, jb, keys, pos, dy,
                      scale, part, dw);
   if (pieces > 1) {
     const int64_t groups = (pieces + kJoinWaves - 1) / kJoinWaves, columns = (dim + 255) / 256;
     const dim3 grid(static_cast<unsigned>(groups < (1 << 18) ? groups : (1 << 18)),
                     static_cast<unsigned>(columns < 64 ? columns : 64));
-    hipLaunchKernelGGL((embed_join_kernel<IO>), grid, dim3(64 * kJoinWaves), 0, st, n, vocab, static_cast<int>(dim),
+    hipLaunchKernelGGL((embed_join_kernel<IO>), grid, dim3(64 * kJoinWaves), 0, st, n, piece, vocab, static_cast<int>(dim),
                        keys, scale, part, dw);
   }
 }
@@ -680,8 +733,8 @@ size_t sparc_embedding_workspace_bytes(int64_t n, int64_t vocab, int64_t dim) {
   using namespace sparc;
   if (em_check(n, vocab, dim, SPARC_F32, 8)) return 0;
   const Sort s = sort_of(n, vocab);
-  const int64_t pieces = (n + kPiece - 1) / kPiece;
-  return 4 * up256(n * sizeof(uint32_t)) + up256((s.tiles << s.digit_bits) * sizeof(uint32_t)) +
+  const int64_t piece = piece_of(n, dim), pieces = (n + piece - 1) / piece;
+  return 4 * up256(n * sizeof(uint32_t)) + up256(((s.tiles + 1) << s.digit_bits) * sizeof(uint32_t)) +
          up256(static_cast<size_t>(pieces) * 2 * part_columns(dim) * sizeof(float)) + 256;
 }
 
@@ -701,7 +754,7 @@ sparc_status sparc_embedding_backward(int64_t n, int64_t vocab, int64_t dim, int
   auto take = [&](size_t bytes) { char* p = at; at += up256(bytes); return p; };
   uint32_t* keys[2] = {reinterpret_cast<uint32_t*>(take(n * 4)), reinterpret_cast<uint32_t*>(take(n * 4))};
   uint32_t* pos[2] = {reinterpret_cast<uint32_t*>(take(n * 4)), reinterpret_cast<uint32_t*>(take(n * 4))};
-  uint32_t* counts = reinterpret_cast<uint32_t*>(take((s.tiles << s.digit_bits) * 4));
+  uint32_t* counts = reinterpret_cast<uint32_t*>(take(((s.tiles + 1) << s.digit_bits) * 4));
   float* part = reinterpret_cast<float*>(at);
   SortPass p{};
   p.tokens = tokens;

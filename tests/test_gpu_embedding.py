@@ -69,9 +69,18 @@ def test_sizes_and_frequencies(n, vocab, kind):
 
 
 def test_many_tokens():
-    """Past 65536 positions the sort takes larger tiles."""
+    """More positions than 64 tiles of the sort."""
     _check(70001, 1000, 8, F32, "zipf")
     _check(70001, 3, 8, F32, "same")
+
+
+@pytest.mark.parametrize("n,vocab,D,dtype,kind", [(100003, 1000, 400, BF16, "zipf"), (100003, 5000, 337, F32, "runs"),
+                                                  (60001, 3, 300, F32, "two"), (100003, 40, 336, BF16, "uniform"),
+                                                  (1100001, 3000, 16, F32, "zipf"), (99001, 300000, 9, F32, "uniform")])
+def test_long_batches(n, vocab, D, dtype, kind):
+    """Longer pieces with more work, the tiles' counts summed beforehand, and
+    past 2^20 positions larger tiles."""
+    _check(n, vocab, D, dtype, kind, seed=n)
 
 
 def test_few_tokens_of_a_large_vocabulary():

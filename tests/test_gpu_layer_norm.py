@@ -70,6 +70,19 @@ def test_wide_rows(D, dtype):
     _check(5, D, dtype, F32, seed=D)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("vectors", [1, 8, 9, 16, 17, 32, 33, 64, 65, 96, 97, 128, 129, 192, 193, 256, 257, 512, 513, 768,
+                                     769, 1024, 1025, 1536, 1537, 2048])
+def test_where_forms_meet(vectors, dtype):
+    """Rows of as many 16-byte vectors as a form holds, and of one value less or
+    more, with few rows and with many."""
+    print(f"[case] layer norm {vectors} vectors {dtype}", flush=True)
+    V = 4 if dtype == F32 else 8
+    _check(5, vectors * V, dtype, dtype, seed=vectors)
+    _check(3, vectors * V - 1, dtype, F32, seed=vectors)
+    _check(1030, vectors * V - V + 1, dtype, dtype, seed=vectors)
+
+
 @pytest.mark.parametrize("rows", [1, 2, 63, 1023, 1024, 4500])
 def test_row_counts(rows):
     print(f"[case] layer norm rows={rows}", flush=True)
