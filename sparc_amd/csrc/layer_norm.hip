@@ -116,7 +116,13 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float (*red)[N][W], int&
   }
 }
 
-// WHOLE: D is a multiple of the vector, so that no element needs a mask
+// The forward, a row per L lanes: one read and one write of each value, and bound
+// by them: 32768 x 768 bf16 22 us (50 MB read, 50 written: 4.6 TB/s), 8192 x 24576
+// 178 us (4.5 TB/s), 300000 x 64 16 us.  256 rows of 2048 take 3.5 us: the launch,
+// two reads one after the other and two sums over the row's lanes.  Rows that do
+// not begin at multiples of 16 bytes cost up to a third more in bf16 (20000 rows
+// of 5000 columns 75 us, of 5004 90, of 5001 105), next to nothing in fp32.
+// WHOLE: D is a multiple of the vector, so that no element needs a mask.
 template <typename IO, typename PT, int NCH, int L, bool WHOLE>
 __global__ void __launch_bounds__(L <= 64 ? 64 * kRowWaves : L)
 layer_norm_fwd_kernel(int64_t R, int D, const void* x, const void* w, const void* b, float eps, void* y, float* mean,
@@ -222,6 +228,10 @@ layer_norm_fwd_kernel(int64_t R, int D, const void* x, const void* w, const void
   }
 }
 
+// The backward: x and dy in, dx out, once each, and the partial rows beside them.
+// Memory again: 32768 x 768 bf16 31 us (102 MB read, 53 written: 5.0 TB/s), 8192 x
+// 24576 228 us (807 and 453: 5.5 TB/s); 3711 x 1001 fp32 13 us, a few rows per
+// wave, whose start and end count.
 template <typename IO, typename PT, int NCH, int L, bool WHOLE>
 __global__ void __launch_bounds__(L <= 64 ? 64 * kBwdRowWaves : L)
 layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const float* mean, const float* rstd,
@@ -384,7 +394,8 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
           }
           __syncthreads();
         }
-        if ((W > 1 || (wave == 0 && lane < L)) && c + 4 * q < D) store_vec<float>(part, out + c + 4 * q, D - c - 4 * q, u);
+        if ((W > 1 || (wave == 0 && lane < L)) && c + 4 * q < D)
+          store_vec<float>(part, out + c + 4 * q, D - c - 4 * q, u);
       }
     }
   };
@@ -392,7 +403,9 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
   if (db_part) write(ab, db_part);
 }
 
-// Rows of any width, read again for each pass over them.
+// Rows of any width, read again for each pass over them, mostly out of a cache:
+// 3172 x 40000 fp32 forward 306 us (1 GB: 3.3 TB/s); backward of 6009 x 16641 fp32
+// 289 us for dx and 153 for the sums over rows, which read x and dy once more.
 constexpr int kWideThreads = 1024;
 template <typename IO, typename PT>
 __global__ void __launch_bounds__(kWideThreads)
@@ -521,7 +534,8 @@ layer_norm_params_wide_kernel(int64_t R, int64_t D, const void* x, const float* 
 }
 
 // out[c] = sum over the n partial rows: CW columns by 1024 / CW slices of rows
-// per workgroup, the slices added in order.  blockIdx.y: dw, db.
+// per workgroup, the slices added in order.  blockIdx.y: dw, db.  4 us for 512
+// partial rows of 768 (a launch), 10 us for 256 of 24576 (50 MB).
 template <typename PT, int CW>
 __global__ void __launch_bounds__(1024)
 layer_norm_reduce_kernel(int n, int64_t D, const float* dw_part, const float* db_part, void* dw, void* db) {
@@ -641,7 +655,8 @@ constexpr int64_t kWideSlices = 64;
 template <typename PT>
 void launch_reduce(hipStream_t st, int64_t n, int64_t D, const float* dw_part, const float* db_part, void* dw,
                    void* db) {
-  // few columns: 16 of them per workgroup, so that more workgroups share the rows
+  // few columns: 16 of them per workgroup, so that more workgroups share the rows;
+  // many: 64, whole lines
   if (D < 8192)
     hipLaunchKernelGGL((layer_norm_reduce_kernel<PT, 16>), dim3(static_cast<unsigned>((D + 15) / 16), 2), dim3(1024), 0,
                        st, static_cast<int>(n), D, dw_part, db_part, dw, db);
