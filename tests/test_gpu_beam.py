@@ -106,6 +106,24 @@ def test_different_logits_of_equal_score_take_the_lowest_token():
         assert step.parents.tolist() == [[beam, beam]] and step.tokens.tolist() == [[first, first + 1]]
 
 
+@pytest.mark.parametrize("K", [1, 3, 11, 32])
+@pytest.mark.parametrize("V", [67, 5003, 70001])
+def test_rows_ranked_by_score(K, V):
+    """Logits of three values, apart by less than 2^-20 within each, under a score
+    of -4096 whose last place is 2^-11: three scores, the lowest tokens of the
+    best first, wherever in the row they stand."""
+    print(f"[case] beam ranked by score K={K} V={V}", flush=True)
+    g = torch.Generator().manual_seed(K * V)
+    level = (torch.randint(0, 3000, (2, K, V), generator=g) > 2990).float() + torch.randint(0, 2, (2, K, V), generator=g)
+    logits = level + torch.rand(2, K, V, generator=g) * 2.0 ** -21
+    scores = torch.full((2, K), -INF)
+    scores[0, 0] = scores[1, K - 1] = -4096.0
+    step = sparc_amd.beam_search_step(logits.cuda(), scores.cuda())
+    for b, beam in ((0, 0), (1, K - 1)):
+        assert step.parents[b].tolist() == [beam] * K
+        assert step.tokens[b].tolist() == torch.sort(-level[b, beam], stable=True).indices[:K].tolist()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 def test_masked_tokens(dtype):
     """-inf and the type's lowest value over most or all of the vocabulary."""
