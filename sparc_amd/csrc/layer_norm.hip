@@ -9,9 +9,8 @@
 // from registers, so a large mean costs no precision.
 //
 // A row is held in registers by the L lanes that own it, 8 to 64 of a wave or a
-// workgroup of 256 to 1024, each NCH vectors of 16 bytes (at any alignment; a
-// width that is no multiple ends in a shorter one).  Rows too wide for that are
-// read again for each pass over them (the *_wide kernels).  The backward keeps the columns' sums of dy xhat and dy in
+// workgroup of 256 to 1024, each NCH vectors of 16 bytes, at any alignment.  Rows
+// too wide for that are read again for each pass over them (the *_wide kernels).  The backward keeps the columns' sums of dy xhat and dy in
 // registers over the rows that its waves walk, beside the weight (in LDS for
 // the widest rows, whose registers are full), reads the next row while it works
 // on one, and writes one partial row per workgroup; a second kernel adds the
@@ -33,10 +32,40 @@ __device__ __forceinline__ int left(int64_t D, int64_t c) {
   return static_cast<int>(D - c < 64 ? D - c : 64);
 }
 
-// Whether every vector of a row may be read whole: what the last one reads of
-// the next row is still inside the array.  Only the array's last rows read
-// short vectors then, whose branches would make every row wait for each load
-// in turn.
+// How a row of D columns ends in vectors of V:
+//   kWhole  D is a multiple of V
+//   kLap    the last vector ends with the row and repeats some columns of the one
+//           before it, which count once in a sum over the row; both lanes come to
+//           the same values for them and store them both (D >= V)
+//   kShort  the last vector is short.  The branches of a short access make every
+//           load wait for the one before it, so all rows but the array's last ones
+//           read it whole, with values of the next row behind the end.
+enum Ends { kWhole, kLap, kShort };
+
+// The columns of vector k of a lane's NCH; those before kLast are whole, as the
+// forms are chosen.
+template <int NCH> constexpr int kLast = NCH <= 4 ? NCH - 1 : NCH - 2;
+template <int V, int NCH, int L, int E>
+struct Columns {
+  bool any;      // whether the row reaches the vector
+  int at, n;     // its first column and how many it has
+  int twice;     // of them repeated
+
+  __device__ __forceinline__ Columns(int k, int t, int D) {
+    const int c = (k * L + t) * V;
+    const bool last = k >= kLast<NCH>;
+    any = c < D;  // a branch for every vector, which keeps the registers of one from the next's
+    at = E == kLap && last && c > D - V ? D - V : c;
+    n = E == kShort && last && D - c < V ? D - c : V;
+    twice = c - at;
+  }
+  // value i of the vector in a sum over the row
+  __device__ __forceinline__ float once(int i, float v) const {
+    if constexpr (E == kLap) return i < twice ? 0.0f : v;
+    if constexpr (E == kShort) return i < n ? v : 0.0f;
+    return v;
+  }
+};
 __device__ __forceinline__ bool reads_whole(int64_t row, int64_t R, int D, int v) {
   return (row + 1) * D + v - 1 <= R * D;
 }
@@ -49,46 +78,6 @@ __device__ __forceinline__ void keep_first(Vec<IO>& raw, int n) {
   for (int i = 0; i < kVec<IO>; ++i) v[i] = i < n ? v[i] : 0.0f;
   raw = pack<IO, kVec<IO>>(v);
 }
-
-// The parameters of the V columns from c on of a row of D, in two steps: what is
-// read, without a branch around the loads where D >= V (the row's last vector is
-// read so that it ends with the row), and the values (zeros behind it).
-template <typename PT, int V>
-struct Params {
-  static constexpr int N = V / kVec<PT>;
-  Vec<PT> raw[N];
-
-  __device__ __forceinline__ void load(const void* w, int c, int D) {
-    if (D >= V) {
-      const int at = c < D - V ? c : D - V;
-#pragma unroll
-      for (int q = 0; q < N; ++q) raw[q] = load_vec<PT>(w, at + q * kVec<PT>, kVec<PT>);
-    } else {
-#pragma unroll
-      for (int q = 0; q < N; ++q) raw[q] = load_vec<PT>(w, c + q * kVec<PT>, D - c - q * kVec<PT>);
-    }
-  }
-  __device__ __forceinline__ void values(int c, int D, float (&p)[V]) const {
-#pragma unroll
-    for (int q = 0; q < N; ++q) {
-      float f[kVec<PT>];
-      unpack<PT, kVec<PT>>(raw[q], f);
-#pragma unroll
-      for (int i = 0; i < kVec<PT>; ++i) p[q * kVec<PT> + i] = f[i];
-    }
-    if (D >= V && c > D - V) {
-      const int by = c - (D - V);
-#pragma unroll
-      for (int s = 1; s < V; s <<= 1) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float up = i + s < V ? p[i + s < V ? i + s : i] : 0.0f;
-          p[i] = by & s ? up : p[i];
-        }
-      }
-    }
-  }
-};
 
 // Sums of N values over the L lanes that share a row, in each of them.  With
 // W waves, red: two buffers used in turn (``turn``), so that one barrier per
@@ -119,11 +108,11 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float (*red)[N][W], int&
 // The forward, a row per L lanes: one read and one write of each value, and bound
 // by them: 32768 x 768 bf16 22 us (50 MB read, 50 written: 4.6 TB/s), 8192 x 24576
 // 178 us (4.5 TB/s), 300000 x 64 16 us.  256 rows of 2048 take 3.5 us: the launch,
-// two reads one after the other and two sums over the row's lanes.  Rows that do
-// not begin at multiples of 16 bytes cost up to a third more in bf16 (20000 rows
-// of 5000 columns 75 us, of 5004 90, of 5001 105), next to nothing in fp32.
-// WHOLE: D is a multiple of the vector, so that no element needs a mask.
-template <typename IO, typename PT, int NCH, int L, bool WHOLE>
+// two reads one after the other and two sums over the row's lanes.  Rows that
+// begin at odd multiples of two bytes cost up to a third more (20000 bf16 rows of
+// 5000 columns 72 us, of 5001 93), since each access is split.  (kWhole in the
+// forward measured no faster than kLap.)
+template <typename IO, typename PT, int NCH, int L, int E>
 __global__ void __launch_bounds__(L <= 64 ? 64 * kRowWaves : L)
 layer_norm_fwd_kernel(int64_t R, int D, const void* x, const void* w, const void* b, float eps, void* y, float* mean,
                       float* rstd) {
@@ -138,43 +127,20 @@ layer_norm_fwd_kernel(int64_t R, int D, const void* x, const void* w, const void
   for (int64_t row = first; row < R; row += static_cast<int64_t>(gridDim.x) * per) {  // uniform over a row's lanes
     const int64_t base = row * D;
     Vec<IO> raw[NCH];
-    if (WHOLE || reads_whole(row, R, D, V)) {
 #pragma unroll
-      for (int k = 0; k < NCH; ++k) {
-        const int c = (k * L + t) * V;
-        if (c < D) raw[k] = load_vec<IO>(x, base + c, V);
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < NCH; ++k) {
-        const int c = (k * L + t) * V;
-        if (c < D) raw[k] = load_vec<IO>(x, base + c, D - c);
-      }
-    }
-    // Where rows end in a short vector, whose branch would make the parameters
-    // wait for one another, they are read here if registers are left for them
-    // (60000 x 1001 bf16: 47 us instead of 52; 20000 x 5001 with fp32 parameters,
-    // 48 registers: 140 instead of 116).
-    constexpr bool kEarly = !WHOLE && NCH * V * sizeof(PT) <= (L <= 64 ? 48 : 32);
-    Params<PT, V> wr[kEarly ? NCH : 1], br[kEarly ? NCH : 1];
-    if constexpr (kEarly) {
-#pragma unroll
-      for (int k = 0; k < NCH; ++k) {
-        const int c = (k * L + t) * V;
-        if (w && c < D) wr[k].load(w, c, D);
-        if (b && c < D) br[k].load(b, c, D);
-      }
+    for (int k = 0; k < NCH; ++k) {
+      const Columns<V, NCH, L, E> c(k, t, D);
+      if (c.any) raw[k] = load_vec<IO>(x, base + c.at, c.n);
     }
     float s[1] = {0.0f};
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      const int c = (k * L + t) * V;
-      if (c < D) {
-        if (!WHOLE && D - c < V) keep_first<IO>(raw[k], D - c);
+      const Columns<V, NCH, L, E> c(k, t, D);
+      if (c.any) {
         float v[V];
         unpack<IO, V>(raw[k], v);
 #pragma unroll
-        for (int i = 0; i < V; ++i) s[0] += v[i];
+        for (int i = 0; i < V; ++i) s[0] += c.once(i, v[i]);
       }
     }
     row_sums<1, L>(s, red, turn);
@@ -182,13 +148,13 @@ layer_norm_fwd_kernel(int64_t R, int D, const void* x, const void* w, const void
     s[0] = 0.0f;
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      const int c = (k * L + t) * V;
-      if (c < D) {
+      const Columns<V, NCH, L, E> c(k, t, D);
+      if (c.any) {
         float v[V];
         unpack<IO, V>(raw[k], v);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float d = WHOLE || i < D - c ? v[i] - mu : 0.0f;
+          const float d = c.once(i, v[i] - mu);
           s[0] = fmaf(d, d, s[0]);
         }
       }
@@ -201,28 +167,25 @@ layer_norm_fwd_kernel(int64_t R, int D, const void* x, const void* w, const void
     }
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      const int c = (k * L + t) * V;
-      if (c < D) {
-        const int n = WHOLE ? V : D - c;
+      const Columns<V, NCH, L, E> c(k, t, D);
+      if (c.any) {
         float v[V], o[V];
         unpack<IO, V>(raw[k], v);
 #pragma unroll
         for (int i = 0; i < V; ++i) o[i] = (v[i] - mu) * r;
         if (w) {
           float p[V];
-          if constexpr (kEarly) wr[k].values(c, D, p);
-          else load_f32<PT, V>(w, c, n, p);
+          load_f32<PT, V>(w, c.at, c.n, p);
 #pragma unroll
           for (int i = 0; i < V; ++i) o[i] *= p[i];
         }
         if (b) {
           float p[V];
-          if constexpr (kEarly) br[k].values(c, D, p);
-          else load_f32<PT, V>(b, c, n, p);
+          load_f32<PT, V>(b, c.at, c.n, p);
 #pragma unroll
           for (int i = 0; i < V; ++i) o[i] += p[i];
         }
-        store_vec<IO>(y, base + c, n, pack<IO, V>(o));
+        store_vec<IO>(y, base + c.at, c.n, pack<IO, V>(o));
       }
     }
   }
@@ -232,7 +195,7 @@ layer_norm_fwd_kernel(int64_t R, int D, const void* x, const void* w, const void
 // Memory again: 32768 x 768 bf16 31 us (102 MB read, 53 written: 5.0 TB/s), 8192 x
 // 24576 228 us (807 and 453: 5.5 TB/s); 3711 x 1001 fp32 13 us, a few rows per
 // wave, whose start and end count.
-template <typename IO, typename PT, int NCH, int L, bool WHOLE>
+template <typename IO, typename PT, int NCH, int L, int E>
 __global__ void __launch_bounds__(L <= 64 ? 64 * kBwdRowWaves : L)
 layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const float* mean, const float* rstd,
                       const void* dy, void* dx, float* dw_part, float* db_part) {
@@ -256,7 +219,7 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
   float aw[NCH][V], ab[NCH][V];
 #pragma unroll
   for (int k = 0; k < NCH; ++k) {
-    const int c = (k * L + t) * V;
+    const Columns<V, NCH, L, E> c(k, t, D);
 #pragma unroll
     for (int i = 0; i < V; ++i) { aw[k][i] = 0.0f; ab[k][i] = 0.0f; }
 #pragma unroll
@@ -265,7 +228,7 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
 #pragma unroll
       for (int i = 0; i < kVec<PT>; ++i) ones[i] = 1.0f;
       Vec<PT> p = pack<PT, kVec<PT>>(ones);
-      if (w && c < D) p = load_vec<PT>(w, c + q * kVec<PT>, WHOLE ? kVec<PT> : D - c - q * kVec<PT>);
+      if (w && c.any) p = load_vec<PT>(w, c.at + q * kVec<PT>, c.n - q * kVec<PT>);
       if constexpr (kWeightInLds) w_lds[(k * L + t) * NP + q] = p;  // read back by this thread only
       else wr[k][q] = p;
     }
@@ -285,22 +248,22 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
   if constexpr (L == 64) row += wave;
   else if constexpr (L < 64) row += threadIdx.x / L;
   const auto load_row = [&](int64_t at, Vec<IO> (&xo)[NCH], Vec<IO> (&dyo)[NCH]) __attribute__((always_inline)) {
-    if (WHOLE || reads_whole(at, R, D, V)) {
+    if (E != kShort || reads_whole(at, R, D, V)) {
 #pragma unroll
       for (int k = 0; k < NCH; ++k) {
-        const int c = (k * L + t) * V;
-        if (c < D) {
-          xo[k] = load_vec<IO>(x, at * D + c, V);
-          dyo[k] = load_vec<IO>(dy, at * D + c, V);
+        const Columns<V, NCH, L, E> c(k, t, D);
+        if (c.any) {
+          xo[k] = load_vec<IO>(x, at * D + c.at, V);
+          dyo[k] = load_vec<IO>(dy, at * D + c.at, V);
         }
       }
     } else {
 #pragma unroll
       for (int k = 0; k < NCH; ++k) {
-        const int c = (k * L + t) * V;
-        if (c < D) {
-          xo[k] = load_vec<IO>(x, at * D + c, D - c);
-          dyo[k] = load_vec<IO>(dy, at * D + c, D - c);
+        const Columns<V, NCH, L, E> c(k, t, D);
+        if (c.any) {
+          xo[k] = load_vec<IO>(x, at * D + c.at, c.n);
+          dyo[k] = load_vec<IO>(dy, at * D + c.at, c.n);
         }
       }
     }
@@ -315,11 +278,11 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      const int c = (k * L + t) * V;
-      if (c < D) {
-        if (!WHOLE && D - c < V) {
-          keep_first<IO>(xr[k], D - c);
-          keep_first<IO>(dr[k], D - c);
+      const Columns<V, NCH, L, E> c(k, t, D);
+      if (c.any) {
+        if (E == kShort && c.n < V) {
+          keep_first<IO>(xr[k], c.n);
+          keep_first<IO>(dr[k], c.n);
         }
         float xv[V], dv[V], p[V];
         unpack<IO, V>(xr[k], xv);
@@ -327,7 +290,7 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
         weight(k, p);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float xh = (xv[i] - mu) * r, g = dv[i] * p[i];
+          const float xh = (xv[i] - mu) * r, g = c.once(i, dv[i] * p[i]);
           s[0] += g;
           s[1] = fmaf(g, xh, s[1]);
           aw[k][i] = fmaf(dv[i], xh, aw[k][i]);
@@ -339,9 +302,8 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
     const float m0 = s[0] * inv_d, m1 = s[1] * inv_d;
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      const int c = (k * L + t) * V;
-      if (c < D) {
-        const int n = WHOLE ? V : D - c;
+      const Columns<V, NCH, L, E> c(k, t, D);
+      if (c.any) {
         if (dx) {
           float xv[V], dv[V], p[V], o[V];
           unpack<IO, V>(xr[k], xv);
@@ -352,17 +314,17 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
             const float xh = (xv[i] - mu) * r;
             o[i] = r * (fmaf(-xh, m1, dv[i] * p[i]) - m0);
           }
-          store_vec<IO>(dx, row * D + c, n, pack<IO, V>(o));
+          store_vec<IO>(dx, row * D + c.at, c.n, pack<IO, V>(o));
         }
         if constexpr (kAhead) {
           xr[k] = xn[k];
           dr[k] = dn[k];
-        } else if (WHOLE ? row + step < R : reads_whole(row + step, R, D, V)) {
-          xr[k] = load_vec<IO>(x, (row + step) * D + c, V);
-          dr[k] = load_vec<IO>(dy, (row + step) * D + c, V);
-        } else if (row + step < R) {
-          xr[k] = load_vec<IO>(x, (row + step) * D + c, n);
-          dr[k] = load_vec<IO>(dy, (row + step) * D + c, n);
+        } else if (E != kShort ? row + step < R : reads_whole(row + step, R, D, V)) {
+          xr[k] = load_vec<IO>(x, (row + step) * D + c.at, V);
+          dr[k] = load_vec<IO>(dy, (row + step) * D + c.at, V);
+        } else if (E == kShort && row + step < R) {
+          xr[k] = load_vec<IO>(x, (row + step) * D + c.at, c.n);
+          dr[k] = load_vec<IO>(dy, (row + step) * D + c.at, c.n);
         }
       }
     }
@@ -374,7 +336,7 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
     const int64_t out = static_cast<int64_t>(blockIdx.x) * D;
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      const int c = (k * L + t) * V;
+      const Columns<V, NCH, L, E> c(k, t, D);
 #pragma unroll
       for (int q = 0; q < V / 4; ++q) {
 #pragma unroll
@@ -394,8 +356,8 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
           }
           __syncthreads();
         }
-        if ((W > 1 || (wave == 0 && lane < L)) && c + 4 * q < D)
-          store_vec<float>(part, out + c + 4 * q, D - c - 4 * q, u);
+        if ((W > 1 || (wave == 0 && lane < L)) && c.any)
+          store_vec<float>(part, out + c.at + 4 * q, c.n - 4 * q, u);
       }
     }
   };
@@ -412,7 +374,7 @@ __global__ void __launch_bounds__(kWideThreads)
 layer_norm_fwd_wide_kernel(int64_t R, int64_t D, const void* x, const void* w, const void* b, float eps, void* y,
                            float* mean, float* rstd) {
   constexpr int V = kVec<IO>;
-  __shared__ float red[2][1][kWideThreads / 64];
+  __shared__ float red[2][1][kWaves<kWideThreads>];
   int turn = 0;
   const float inv_d = 1.0f / static_cast<float>(D);
   const int64_t c0 = static_cast<int64_t>(threadIdx.x) * V;
@@ -463,7 +425,7 @@ __global__ void __launch_bounds__(kWideThreads)
 layer_norm_dx_wide_kernel(int64_t R, int64_t D, const void* x, const void* w, const float* mean, const float* rstd,
                           const void* dy, void* dx) {
   constexpr int V = kVec<IO>;
-  __shared__ float red[2][2][kWideThreads / 64];
+  __shared__ float red[2][2][kWaves<kWideThreads>];
   int turn = 0;
   const float inv_d = 1.0f / static_cast<float>(D);
   const int64_t c0 = static_cast<int64_t>(threadIdx.x) * V;
@@ -641,6 +603,15 @@ bool bwd_form(int64_t D, F&& f) {
 // a partial row costs as much as a row: 2 of these at least for each, and 8
 // behind the first 512 (944 x 2827 bf16 with the sum of the partial rows: 19
 // against 24 us, 4096 x 2880: 24 against 26).
+// How rows of other widths than whole vectors end: with vectors that lap (20000 x
+// 5004 bf16, fp32 parameters 141 us, short ones 201; 300000 x 68 33 and 40; 60000 x
+// 701 57 and 73), but for 4 vectors in each of 1024 lanes, which have no registers
+// left for it (3944 x 25353: 224 and 178).
+template <int NCH, int L>
+constexpr int bwd_ends() {
+  return NCH >= 4 && L == 1024 ? kShort : kLap;
+}
+
 template <int NCH, int L>
 int64_t bwd_groups(int64_t R) {
   const int64_t need = L <= 64 ? (R + kBwdRows<L> - 1) / kBwdRows<L> : (R + 1) / 2;
@@ -681,12 +652,14 @@ sparc_status ln_forward(hipStream_t st, int64_t R, int64_t D, const void* x, con
   const bool held = fwd_form<IO>(R, D, [&](auto NCH, auto L) {
     const int threads = L() > 64 ? L() : (R < kFewRows ? 64 : 64 * kRowWaves), per = threads / L();
     const dim3 grid(op_grid((R + per - 1) / per)), block(threads);
-    if (D % kVec<IO> == 0)
-      hipLaunchKernelGGL((layer_norm_fwd_kernel<IO, PT, NCH(), L(), true>), grid, block, 0, st, R, static_cast<int>(D),
+    const auto launch = [&](auto E) {
+      hipLaunchKernelGGL((layer_norm_fwd_kernel<IO, PT, NCH(), L(), E()>), grid, block, 0, st, R, static_cast<int>(D),
                          x, w, b, eps, y, mean, rstd);
-    else
-      hipLaunchKernelGGL((layer_norm_fwd_kernel<IO, PT, NCH(), L(), false>), grid, block, 0, st, R,
-                         static_cast<int>(D), x, w, b, eps, y, mean, rstd);
+    };
+    if constexpr (L() == 8) {
+      if (D < kVec<IO>) return launch(Int<kShort>{});
+    }
+    launch(Int<kLap>{});
   });
   if (!held)
     hipLaunchKernelGGL((layer_norm_fwd_wide_kernel<IO, PT>), dim3(op_grid(R)), dim3(kWideThreads), 0, st, R, D, x, w, b,
@@ -704,12 +677,15 @@ sparc_status ln_backward(hipStream_t st, int64_t R, int64_t D, const void* x, co
     n = bwd_groups<NCH(), L()>(R);
     if (dw && db) db_part = ws + n * D;
     const dim3 grid(static_cast<unsigned>(n)), block(L() > 64 ? L() : 64 * kBwdRowWaves);
-    if (D % kVec<IO> == 0)
-      hipLaunchKernelGGL((layer_norm_bwd_kernel<IO, PT, NCH(), L(), true>), grid, block, 0, st, R, static_cast<int>(D),
+    const auto launch = [&](auto E) {
+      hipLaunchKernelGGL((layer_norm_bwd_kernel<IO, PT, NCH(), L(), E()>), grid, block, 0, st, R, static_cast<int>(D),
                          x, w, mean, rstd, dy, dx, dw_part, db_part);
-    else
-      hipLaunchKernelGGL((layer_norm_bwd_kernel<IO, PT, NCH(), L(), false>), grid, block, 0, st, R,
-                         static_cast<int>(D), x, w, mean, rstd, dy, dx, dw_part, db_part);
+    };
+    if constexpr (L() == 8) {
+      if (D < kVec<IO>) return launch(Int<kShort>{});
+    }
+    if (D % kVec<IO> == 0) return launch(Int<kWhole>{});
+    launch(Int<bwd_ends<NCH(), L()>()>{});
   });
   if (!held) {
     if (dx)
