@@ -342,9 +342,9 @@ struct SumExp {
 
 // 1024 rows of 131072 bf16 logits 62 us (269 MB, read once: 4.3 TB/s): some 10 us
 // of lists' starts and ends, and 5.3 TB/s between them; the VALU is 70 % busy, but a
-// maximum less per logit and a rescaling less per vector took no time out.  160 rows of 50001 fp32 ones 14 us, of which reading is 5: the sorts
-// and merges of the lists, a chain of some 60 exchanges per wave, are the rest;
-// 4 rows of 32768 6.6 us.
+// maximum less per logit and a rescaling less per vector took no time out.  160
+// rows of 50001 fp32 ones 14 us, of which reading is 5: the sorts and merges of the
+// lists, a chain of some 60 exchanges per wave, are the rest; 4 rows of 32768 6.6.
 // parts: [rows][spans] (maximum, sum of exp(x - maximum)); tops: [rows][spans][want] keys
 template <typename IO>
 __global__ void __launch_bounds__(64 * kScanWaves, 4)

@@ -10,12 +10,12 @@
 //
 // A row is held in registers by the L lanes that own it, 8 to 64 of a wave or a
 // workgroup of 256 to 1024, each NCH vectors of 16 bytes, at any alignment.  Rows
-// too wide for that are read again for each pass over them (the *_wide kernels).  The backward keeps the columns' sums of dy xhat and dy in
-// registers over the rows that its waves walk, beside the weight (in LDS for
-// the widest rows, whose registers are full), reads the next row while it works
-// on one, and writes one partial row per workgroup; a second kernel adds the
-// partial rows in a fixed order, so the parameters' gradients do not depend on
-// timing.
+// too wide for that are read again for each pass over them (the *_wide kernels).
+// The backward keeps the columns' sums of dy xhat and dy in registers over the
+// rows that its waves walk, beside the weight (in LDS for the widest rows, whose
+// registers are full), reads the next row while it works on one, and writes one
+// partial row per workgroup; a second kernel adds the partial rows in a fixed
+// order, so the parameters' gradients do not depend on timing.
 
 #include "rows.h"
 
