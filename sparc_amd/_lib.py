@@ -217,6 +217,22 @@ def load() -> ctypes.CDLL:
         return lib
 
 
+_native = None
+
+
+def native():
+    """The torch binding of the operators around the stack (csrc/native.cpp)."""
+    global _native
+    if _native is None:
+        load()
+        try:
+            from . import _native as module
+        except ImportError as e:
+            raise RuntimeError("sparc_amd's torch binding is not built: run `python -m sparc_amd.build`") from e
+        _native = module
+    return _native
+
+
 def check(status: int, what: str) -> None:
     if status != 0:
         msg = load().sparc_last_error().decode(errors="replace")

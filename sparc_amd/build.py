@@ -1,4 +1,5 @@
-"""Builds libsparc_hip.so (gfx950) in-tree with hipcc.
+"""Builds libsparc_hip.so (gfx950) in-tree with hipcc, and the torch binding of
+the operators around the stack (_native.so, host code over that library).
 
 ``python -m sparc_amd.build`` or ``sparc_amd.build.build()``.  Every call
 recompiles.  The objects are compiled in parallel, one process per source
@@ -10,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -20,6 +22,7 @@ LIB_NAME = "libsparc_hip.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 SOURCES = ["scan.hip", "pointwise.hip", "mixer.hip", "norm.hip", "fold.hip", "layer_norm.hip", "embedding.hip",
            "grad_norm.hip", "beam.hip"]
+NATIVE_PATH = os.path.join(HERE, "_native.so")
 # scan.hip compiles as SCAN_PARTS translation units (SPARC_SCAN_PART = 0..11:
 # the C ABI, then one per (transition, I/O dtype) launcher), in parallel
 SCAN_PARTS = 12
@@ -52,10 +55,35 @@ def _compile(job: tuple[str, int | None], build_dir: str, extra: list[str]) -> s
     defs = [] if part is None else [f"-DSPARC_SCAN_PART={part}"]
     cmd = [_hipcc(), *HIPCC_FLAGS, *defs, *extra, "-I", INCLUDE, "-I", CSRC, "-c",
            os.path.join(CSRC, src), "-o", obj]
+    _run(cmd, f"hipcc failed for {src}")
+    return obj
+
+
+def _compile_native(build_dir: str) -> str:
+    from torch.utils import cpp_extension
+    rocm = cpp_extension.ROCM_HOME or "/opt/rocm"
+    includes = [INCLUDE, *cpp_extension.include_paths(), sysconfig.get_paths()["include"],
+                os.path.join(rocm, "include")]
+    obj = os.path.join(build_dir, "native.o")
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+          *(flag for path in includes for flag in ("-isystem", path)),
+          "-c", os.path.join(CSRC, "native.cpp"), "-o", obj], "g++ failed for native.cpp")
+    return obj
+
+
+def _link_native(obj: str) -> None:
+    from torch.utils import cpp_extension
+    libs = [flag for path in cpp_extension.library_paths() for flag in ("-L", path)]
+    tmp = NATIVE_PATH + ".tmp"
+    _run(["g++", "-shared", obj, "-o", tmp, *libs, "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python",
+          "-L", HERE, f"-l:{LIB_NAME}", "-Wl,-rpath,$ORIGIN"], "linking the torch binding failed")
+    os.replace(tmp, NATIVE_PATH)
+
+
+def _run(cmd: list[str], what: str) -> None:
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
-        raise RuntimeError(f"hipcc failed for {src}:\n{proc.stdout}\n{proc.stderr}")
-    return obj
+        raise RuntimeError(f"{what}:\n{proc.stdout}\n{proc.stderr}")
 
 
 def build(verbose: bool = False, extra: list[str] | None = None) -> str:
@@ -66,15 +94,16 @@ def build(verbose: bool = False, extra: list[str] | None = None) -> str:
             for part in (range(SCAN_PARTS) if src == "scan.hip" else [None])]
     # the scan parts are the long ones: start them first
     with ThreadPoolExecutor(max_workers=min(len(jobs), os.cpu_count() or 4)) as pool:
+        native = pool.submit(_compile_native, build_dir)
         objs = list(pool.map(lambda j: _compile(j, build_dir, extra), jobs))
+        native_obj = native.result()
     tmp = LIB_PATH + ".tmp"
     cmd = [_hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", tmp]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f"link failed:\n{proc.stdout}\n{proc.stderr}")
+    _run(cmd, "link failed")
     os.replace(tmp, LIB_PATH)
+    _link_native(native_obj)
     if verbose:
-        print(f"built {LIB_PATH}")
+        print(f"built {LIB_PATH} and {NATIVE_PATH}")
     return LIB_PATH
 
 

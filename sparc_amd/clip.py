@@ -5,14 +5,12 @@ call takes every tensor."""
 from __future__ import annotations
 
 import math
-from array import array
 
 import torch
 
 from . import _lib
 
-_Tensor = torch.Tensor
-_CODES = {torch.float32: _lib.SPARC_F32, torch.bfloat16: _lib.SPARC_BF16}
+_DTYPES = (torch.float32, torch.bfloat16)
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -38,33 +36,11 @@ def _repeats(t: torch.Tensor) -> bool:
     return False
 
 
-def _call(fn_name, tensors, *args):
-    """One library call over the tensors' values (a tensor given twice counts
-    once); the norm, [] float32."""
-    lib = _lib.load()
-    dev = tensors[0].device
-    if not tensors[0].is_cuda or len(set(map(_Tensor.get_device, tensors))) > 1:
-        _lib.require_gpu(*tensors)
-    data = list(map(_Tensor.data_ptr, tensors))
-    if len(set(data)) != len(data):
-        tensors = list({(p, t.numel(), t.dtype): t for p, t in zip(data, tensors)}.values())
-        data = list(map(_Tensor.data_ptr, tensors))
-    n = len(data)
-    sizes, codes = array("q", map(_Tensor.numel, tensors)), array("i", [_CODES[t.dtype] for t in tensors])
-    data = array("Q", data)
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    need = lib.sparc_grad_norm_workspace_bytes(n)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    _lib.check(getattr(lib, fn_name)(n, data.buffer_info()[0], sizes.buffer_info()[0], codes.buffer_info()[0], *args,
-                                     norm.data_ptr(), ws.data_ptr(), need, _lib.stream_of(dev)), fn_name)
-    return norm
-
-
 def _checked(tensors):
     for t in tensors:
         if t.layout is not torch.strided:
             raise ValueError(f"gradients must be dense tensors, got layout {t.layout}")
-        if t.dtype not in _CODES:
+        if t.dtype not in _DTYPES:
             raise TypeError(f"SPARC HIP kernels take float32 or bfloat16 tensors, got {t.dtype}")
     return tensors
 
@@ -74,11 +50,14 @@ def grad_norm(tensors) -> torch.Tensor:
     bfloat16 mixed, any shapes), a float32 scalar on their device.  Squares are
     summed in fp64 in a fixed order: no overflow, equal calls give equal bits."""
     tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
-    tensors = [t if _dense(t) else t.contiguous() for t in _checked(tensors)]
-    return _call("sparc_grad_norm", tensors) if tensors else torch.zeros(())
+    if not tensors:
+        return torch.zeros(())
+    norm = _lib.native().grad_norm(tensors, None)
+    if norm is None:
+        norm = _dense_norm([t if _dense(t) else t.contiguous() for t in _checked(tensors)], None)
+    return norm
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     """Scale the gradients of ``parameters`` in place by
     ``min(1, max_norm / (norm + 1e-6))``, ``norm`` their common L2 norm before;
@@ -93,20 +72,32 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     if math.isnan(max_norm) or max_norm < 0.0:
         raise ValueError(f"clip_grad_norm_ needs max_norm >= 0, got {max_norm}")
     parameters = [parameters] if torch.is_tensor(parameters) else parameters
-    grads = _checked([g for g in [p.grad for p in parameters] if g is not None])
+    grads = [g for g in [p.grad for p in parameters] if g is not None]
     if not grads:
         return torch.zeros(())
+    norm = _lib.native().grad_norm(grads, max_norm)
+    if norm is not None:
+        return norm
     copies = []
-    for i, g in enumerate(grads if not all(map(_Tensor.is_contiguous, grads)) else ()):
+    for i, g in enumerate(_checked(grads)):
         if not _dense(g):
             if _repeats(g):
                 raise ValueError("a gradient names one value more than once (an expanded view): it cannot be scaled "
                                  "in place")
             grads[i] = g.contiguous()
             copies.append((g, grads[i]))
-    norm = _call("sparc_clip_grad_norm", grads, max_norm)
-    for g, c in copies:
-        g.copy_(c)
+    norm = _dense_norm(grads, max_norm)
+    with torch.no_grad():
+        for g, c in copies:
+            g.copy_(c)
+    return norm
+
+
+def _dense_norm(tensors, max_norm):
+    _lib.require_gpu(*tensors)
+    norm = _lib.native().grad_norm(tensors, max_norm)
+    if norm is None:
+        raise ValueError("gradients must be dense tensors")
     return norm
 
 

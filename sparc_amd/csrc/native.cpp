@@ -1,0 +1,312 @@
+// The torch binding of the operators around the stack: embedding, layer norm,
+// clipping, beam step.  Their calls are short, and what the host does for one is
+// most of the time of a small one: from Python through ctypes a lookup of 256 ids
+// took 7.6 us, from here 4.8; a beam step with 24 state planes 52 and 27; 64 ids
+// forward and gradient 45 to 87 and 34 to 56, because autograd runs a backward on a
+// thread of its own, where a node in Python costs it the interpreter beside the
+// launches.
+//
+// Every function checks what the kernels assume and returns None for arguments
+// that it does not take; the Python callers then say what is wrong with them.
+#include <set>
+#include <stdexcept>
+
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include "sparc_hip.h"
+
+namespace {
+
+using at::Tensor;
+using std::optional;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using Tensors = std::vector<Tensor>;
+
+sparc_stream_t stream_of(const Tensor& t) {
+  return reinterpret_cast<sparc_stream_t>(c10::hip::getCurrentHIPStream(t.device().index()).stream());
+}
+void check(sparc_status s, const char* what) {
+  if (s != SPARC_OK)
+    throw std::runtime_error(std::string(what) + " failed (sparc_status " + std::to_string(s) +
+                             "): " + sparc_last_error());
+}
+bool is_io(const Tensor& t) { return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16; }
+int32_t code_of(at::ScalarType t) { return t == at::kFloat ? SPARC_F32 : SPARC_BF16; }
+// whether t is a dense tensor on the device of the GPU tensor ``with``
+bool beside(const Tensor& t, const Tensor& with) {
+  return t.layout() == at::kStrided && t.is_cuda() && t.device() == with.device();
+}
+bool beside(const optional<Tensor>& t, const Tensor& with) { return !t || beside(*t, with); }
+void* address(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+Tensor scratch(size_t bytes, const Tensor& like) {
+  return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
+}
+Tensor contiguous(const optional<Tensor>& t) { return t ? t->contiguous() : Tensor(); }
+
+// ---------------------------------------------------------------------------
+// embedding
+// ---------------------------------------------------------------------------
+Tensor embedding_forward(const Tensor& tokens, const Tensor& weight, double scale) {
+  std::vector<int64_t> shape = tokens.sizes().vec();
+  shape.push_back(weight.size(1));
+  Tensor y = at::empty(shape, weight.options());
+  check(sparc_embedding_forward(tokens.numel(), weight.size(0), weight.size(1), code_of(weight.scalar_type()),
+                                static_cast<int32_t>(tokens.element_size()), tokens.data_ptr(), weight.data_ptr(),
+                                static_cast<float>(scale), y.data_ptr(), stream_of(weight)),
+        "sparc_embedding_forward");
+  return y;
+}
+
+struct Embedding : torch::autograd::Function<Embedding> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& tokens, double scale,
+                        int64_t padding_id) {
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["vocab"] = weight.size(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding_id"] = padding_id;
+    return embedding_forward(tokens, weight.contiguous(), scale);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (at::GradMode::is_enabled()) throw std::runtime_error("embedding is not twice differentiable");
+    const Tensor tokens = ctx->get_saved_variables()[0], dy = grads[0].contiguous();
+    const c10::DeviceGuard guard(dy.device());
+    const int64_t n = tokens.numel(), vocab = ctx->saved_data["vocab"].toInt(), dim = dy.size(-1);
+    Tensor dw = at::empty({vocab, dim}, dy.options());
+    const size_t need = sparc_embedding_workspace_bytes(n, vocab, dim);
+    const Tensor ws = scratch(need, dy);
+    check(sparc_embedding_backward(n, vocab, dim, code_of(dy.scalar_type()),
+                                   static_cast<int32_t>(tokens.element_size()), tokens.data_ptr(),
+                                   ctx->saved_data["padding_id"].toInt(), dy.data_ptr(),
+                                   static_cast<float>(ctx->saved_data["scale"].toDouble()), dw.data_ptr(),
+                                   ws.data_ptr(), need, stream_of(dy)),
+          "sparc_embedding_backward");
+    return {dw, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+optional<Tensor> embedding(const Tensor& tokens, const Tensor& weight, double scale, optional<int64_t> padding) {
+  if (weight.dim() != 2 || weight.numel() == 0 || !is_io(weight) || !beside(weight, weight) ||
+      (tokens.scalar_type() != at::kLong && tokens.scalar_type() != at::kInt) || !beside(tokens, weight))
+    return std::nullopt;
+  const int64_t vocab = weight.size(0);
+  if (padding && (*padding < -vocab || *padding >= vocab)) return std::nullopt;
+  const int64_t padding_id = !padding ? -1 : *padding < 0 ? *padding + vocab : *padding;
+  const c10::DeviceGuard guard(weight.device());
+  if (weight.requires_grad() && at::GradMode::is_enabled())
+    return Embedding::apply(weight, tokens.contiguous(), scale, padding_id);
+  return embedding_forward(tokens.contiguous(), weight.contiguous(), scale);
+}
+
+// ---------------------------------------------------------------------------
+// layer norm
+// ---------------------------------------------------------------------------
+// x, weight and bias contiguous, weight and bias perhaps undefined
+Tensor layer_norm_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps, float* mean,
+                          float* rstd) {
+  const Tensor& p = weight.defined() ? weight : bias.defined() ? bias : x;
+  const int64_t cols = x.size(-1);
+  Tensor y = at::empty_like(x);
+  check(sparc_layer_norm_forward(x.numel() / cols, cols, code_of(x.scalar_type()), code_of(p.scalar_type()),
+                                 x.data_ptr(), address(weight), address(bias), static_cast<float>(eps), y.data_ptr(),
+                                 mean, rstd, stream_of(x)),
+        "sparc_layer_norm_forward");
+  return y;
+}
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const optional<Tensor>& weight_in,
+                        const optional<Tensor>& bias_in, double eps) {
+    const Tensor x = x_in.contiguous(), weight = contiguous(weight_in), bias = contiguous(bias_in);
+    const int64_t rows = x.numel() / x.size(-1);
+    Tensor stats = at::empty({2, rows}, x.options().dtype(at::kFloat));
+    float* mean = stats.data_ptr<float>();
+    const Tensor& p = weight.defined() ? weight : bias.defined() ? bias : x;
+    ctx->save_for_backward({x, weight, stats});
+    ctx->saved_data["parameters"] = static_cast<int64_t>(p.scalar_type());
+    ctx->saved_data["bias"] = bias.defined();
+    return layer_norm_forward(x, weight, bias, eps, mean, mean + rows);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (at::GradMode::is_enabled()) throw std::runtime_error("layer_norm is not twice differentiable");
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &weight = saved[1], &stats = saved[2];
+    const Tensor dy = grads[0].contiguous();
+    const c10::DeviceGuard guard(x.device());
+    const int64_t cols = x.size(-1), rows = x.numel() / cols;
+    const auto type = static_cast<at::ScalarType>(ctx->saved_data["parameters"].toInt());
+    const auto gradient = [&](bool wanted) { return wanted ? at::empty({cols}, x.options().dtype(type)) : Tensor(); };
+    // the inputs are numbered without those that are not there
+    Tensor dx = ctx->needs_input_grad(0) ? at::empty_like(x) : Tensor();
+    Tensor dw = gradient(weight.defined() && ctx->needs_input_grad(1));
+    Tensor db = gradient(ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(weight.defined() ? 2 : 1));
+    const size_t need = dw.defined() || db.defined() ? sparc_layer_norm_workspace_bytes(rows, cols) : 0;
+    const Tensor ws = need ? scratch(need, x) : Tensor();
+    const float* mean = stats.data_ptr<float>();
+    check(sparc_layer_norm_backward(rows, cols, code_of(x.scalar_type()), code_of(type), x.data_ptr(), address(weight),
+                                    mean, mean + rows, dy.data_ptr(), address(dx), address(dw), address(db),
+                                    address(ws), need, stream_of(x)),
+          "sparc_layer_norm_backward");
+    return {dx, dw, db, Tensor()};
+  }
+};
+
+optional<Tensor> layer_norm(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias, double eps) {
+  if (x.dim() < 1 || x.size(-1) < 1 || !(eps >= 0.0) || !is_io(x) || !beside(x, x)) return std::nullopt;
+  for (const auto* p : {&weight, &bias}) {
+    if (*p && ((*p)->dim() != 1 || (*p)->numel() != x.size(-1) ||
+               ((*p)->scalar_type() != x.scalar_type() && (*p)->scalar_type() != at::kFloat) || !beside(**p, x)))
+      return std::nullopt;
+  }
+  if (weight && bias && weight->scalar_type() != bias->scalar_type()) return std::nullopt;
+  const c10::DeviceGuard guard(x.device());
+  const auto wants = [](const optional<Tensor>& t) { return t && t->requires_grad(); };
+  if ((x.requires_grad() || wants(weight) || wants(bias)) && at::GradMode::is_enabled())
+    return LayerNorm::apply(x, weight, bias, eps);
+  return layer_norm_forward(x.contiguous(), contiguous(weight), contiguous(bias), eps, nullptr, nullptr);
+}
+
+// ---------------------------------------------------------------------------
+// the gradients' norm
+// ---------------------------------------------------------------------------
+// A tensor given twice counts once.  max_norm: scale to it.
+optional<Tensor> grad_norm(const Tensors& tensors, optional<double> max_norm) {
+  if (tensors.empty()) return std::nullopt;
+  for (const Tensor& t : tensors)
+    if (!beside(t, tensors[0]) || !is_io(t) || !t.is_non_overlapping_and_dense()) return std::nullopt;
+  const size_t n = tensors.size();
+  const at::NoGradGuard no_grad;
+  using Key = std::tuple<void*, int64_t, int32_t>;
+  std::vector<void*> data;
+  std::vector<int64_t> sizes;
+  std::vector<int32_t> types;
+  std::set<Key> seen;
+  bool rising = true;  // addresses in order are no repeats: nothing to look up
+  for (size_t i = 1; i < n; ++i) rising = rising && tensors[i - 1].data_ptr() < tensors[i].data_ptr();
+  for (const Tensor& t : tensors) {
+    const Key key(t.data_ptr(), t.numel(), code_of(t.scalar_type()));
+    if (!rising && !seen.insert(key).second) continue;
+    data.push_back(std::get<0>(key));
+    sizes.push_back(std::get<1>(key));
+    types.push_back(std::get<2>(key));
+  }
+  const c10::DeviceGuard guard(tensors[0].device());
+  const int64_t count = static_cast<int64_t>(data.size());
+  Tensor norm = at::empty({}, tensors[0].options().dtype(at::kFloat));
+  const size_t need = sparc_grad_norm_workspace_bytes(count);
+  const Tensor ws = scratch(need, tensors[0]);
+  float* out = norm.data_ptr<float>();
+  if (max_norm)
+    check(sparc_clip_grad_norm(count, data.data(), sizes.data(), types.data(), static_cast<float>(*max_norm), out,
+                               ws.data_ptr(), need, stream_of(tensors[0])),
+          "sparc_clip_grad_norm");
+  else
+    check(sparc_grad_norm(count, data.data(), sizes.data(), types.data(), out, ws.data_ptr(), need,
+                          stream_of(tensors[0])),
+          "sparc_grad_norm");
+  return norm;
+}
+
+// ---------------------------------------------------------------------------
+// beam search
+// ---------------------------------------------------------------------------
+bool is_beams(const Tensor& t, int64_t B, int64_t K, at::ScalarType type, const Tensor& with) {
+  return t.dim() == 2 && t.size(0) == B && t.size(1) == K && t.scalar_type() == type && beside(t, with);
+}
+
+// (tokens, parents, scores, finished)
+optional<std::tuple<Tensor, Tensor, Tensor, optional<Tensor>>> beam_step(const Tensor& logits_in,
+                                                                         const Tensor& scores_in,
+                                                                         const optional<Tensor>& finished_in,
+                                                                         optional<int64_t> eos, int64_t most_beams) {
+  if (logits_in.dim() != 3 || !is_io(logits_in) || !beside(logits_in, logits_in)) return std::nullopt;
+  const int64_t B = logits_in.size(0), K = logits_in.size(1), V = logits_in.size(2);
+  if (K < 1 || K > most_beams || V < 1 || !is_beams(scores_in, B, K, at::kFloat, logits_in) ||
+      (finished_in && (!eos || !is_beams(*finished_in, B, K, at::kBool, logits_in))) ||
+      (eos && (*eos < 0 || *eos >= V)))
+    return std::nullopt;
+  const at::NoGradGuard no_grad;
+  const c10::DeviceGuard guard(logits_in.device());
+  Tensor logits = logits_in;
+  int64_t stride = K > 1 ? logits.stride(1) : B > 1 ? logits.stride(0) : V;
+  if ((V > 1 && logits.stride(2) != 1) || stride < V || (B > 1 && logits.stride(0) != K * stride)) {
+    logits = logits.contiguous();
+    stride = V;
+  }
+  const Tensor scores = scores_in.contiguous(), finished = contiguous(finished_in);
+  const auto make = [&](at::ScalarType type) { return at::empty({B, K}, scores.options().dtype(type)); };
+  Tensor tokens = make(at::kLong), parents = make(at::kLong), new_scores = make(at::kFloat);
+  optional<Tensor> new_finished;
+  if (eos) new_finished = make(at::kBool);
+  const size_t need = sparc_beam_workspace_bytes(B, K, V);
+  const Tensor ws = scratch(need, scores);
+  check(sparc_beam_step(B, K, V, stride, code_of(logits.scalar_type()), logits.data_ptr(), scores.data_ptr<float>(),
+                        static_cast<const uint8_t*>(address(finished)), eos ? *eos : -1, tokens.data_ptr<int64_t>(),
+                        parents.data_ptr<int64_t>(), new_scores.data_ptr<float>(),
+                        eos ? static_cast<uint8_t*>(new_finished->data_ptr()) : nullptr, ws.data_ptr(), need,
+                        stream_of(logits)),
+        "sparc_beam_step");
+  return std::make_tuple(tokens, parents, new_scores, new_finished);
+}
+
+// The planes in the parents' order: in ``out`` (of the planes' shapes, types and
+// contiguous; whether it overlaps them is checked by the caller), or in fresh
+// tensors, which share an allocation where all planes are alike.
+optional<Tensors> reorder(const Tensors& planes, const Tensor& parents_in, const optional<Tensors>& out) {
+  if (parents_in.dim() != 2 || parents_in.scalar_type() != at::kLong || !beside(parents_in, parents_in))
+    return std::nullopt;
+  const int64_t B = parents_in.size(0), K = parents_in.size(1), rows = B * K;
+  bool alike = true;
+  for (const Tensor& p : planes) {
+    if (!beside(p, parents_in) || p.dim() < 1 || p.size(0) != rows) return std::nullopt;
+    if (rows > 0 && p.numel() / rows * static_cast<int64_t>(p.element_size()) % 2) return std::nullopt;
+    alike = alike && p.scalar_type() == planes[0].scalar_type() && p.sizes() == planes[0].sizes();
+  }
+  if (planes.empty()) return Tensors();
+  const at::NoGradGuard no_grad;
+  const c10::DeviceGuard guard(parents_in.device());
+  const Tensor parents = parents_in.contiguous();
+  Tensors to;
+  if (out) {
+    to = *out;
+    if (to.size() != planes.size()) return std::nullopt;
+    for (size_t i = 0; i < to.size(); ++i)
+      if (!beside(to[i], parents) || to[i].scalar_type() != planes[i].scalar_type() ||
+          to[i].sizes() != planes[i].sizes() || !to[i].is_contiguous())
+        return std::nullopt;
+  } else if (alike) {
+    std::vector<int64_t> shape = planes[0].sizes().vec();
+    shape.insert(shape.begin(), static_cast<int64_t>(planes.size()));
+    to = at::empty(shape, planes[0].options()).unbind(0);
+  } else {
+    for (const Tensor& p : planes) to.push_back(at::empty(p.sizes(), p.options()));
+  }
+  Tensors from;  // kept until the launch is enqueued
+  std::vector<const void*> src;
+  std::vector<void*> dst;
+  std::vector<int64_t> bytes;
+  for (size_t i = 0; i < planes.size(); ++i) {
+    from.push_back(planes[i].contiguous());
+    src.push_back(from[i].data_ptr());
+    dst.push_back(to[i].data_ptr());
+    bytes.push_back(rows > 0 ? planes[i].numel() / rows * static_cast<int64_t>(planes[i].element_size()) : 0);
+  }
+  check(sparc_reorder_states(B, K, static_cast<int64_t>(planes.size()), src.data(), dst.data(), bytes.data(),
+                             parents.data_ptr<int64_t>(), stream_of(parents)),
+        "sparc_reorder_states");
+  return to;
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_native, m) {
+  m.def("embedding", &embedding);
+  m.def("layer_norm", &layer_norm);
+  m.def("grad_norm", &grad_norm);
+  m.def("beam_step", &beam_step);
+  m.def("reorder", &reorder);
+}
