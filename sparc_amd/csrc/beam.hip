@@ -623,6 +623,44 @@ reorder_in_place_kernel(Planes pl, int K, int batch, const int64_t* parents) {
   }
 }
 
+// The same where few workgroups would result: 64 accesses of all K rows per
+// workgroup, each of its 4 waves PW rows (4 PW >= K), so that no thread's chain of
+// accesses is long (2 x 30 beams, 2 planes of 640 bytes: 4.1 us, 8.2 with all rows
+// in a thread; 14 planes of 540 rows of 27 KB: 86 and 73).
+constexpr int kSplitWaves = 4;
+template <int B, int PW>
+__global__ void __launch_bounds__(64 * kSplitWaves)
+reorder_split_kernel(Planes pl, int K, int batch, const int64_t* parents) {
+  using T = typename Bytes<B>::T;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int64_t rb = pl.row_bytes[blockIdx.z], tile = static_cast<int64_t>(blockIdx.x) * (64 * B);
+  if (tile >= rb) return;
+  const uint32_t t = lane * B;
+  const bool in = tile + t < rb;
+  char* const plane = static_cast<char*>(pl.dst[blockIdx.z]) + tile;
+  for (int b = blockIdx.y; b < batch; b += gridDim.y) {
+    const int64_t own = parents[b * K + (lane < K ? lane : 0)];
+    const int from = own >= 0 && own < K ? static_cast<int>(own) : -1;
+    char* const col = plane + static_cast<int64_t>(b) * K * rb;
+    int p[PW];
+    T v[PW];
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+      const int k = i * kSplitWaves + wave;
+      p[i] = k < K ? __builtin_amdgcn_readlane(from, k) : k;
+      if (p[i] >= 0 && p[i] != k && in) v[i] = *reinterpret_cast<const T*>(col + p[i] * rb + t);
+    }
+    __syncthreads();  // all rows are read
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+      const int k = i * kSplitWaves + wave;
+      if (p[i] == k || !in) continue;
+      if (p[i] < 0) v[i] = ~T(0);
+      *reinterpret_cast<T*>(col + k * rb + t) = v[i];
+    }
+  }
+}
+
 // To other memory: rows blockIdx.y, + gridDim.y, ..., of plane blockIdx.z; a
 // workgroup copies kCopy accesses per thread of one row.
 constexpr int kCopy = 4;
@@ -682,11 +720,19 @@ template <int B>
 void launch_reorder(hipStream_t st, const Planes& pl, int count, int64_t widest, bool in_place, int K, int batch,
                     const int64_t* parents) {
   const int rows = in_place ? batch : batch * K, threads = !in_place && widest <= 64 * B * kCopy ? 64 : 256;
-  const int64_t tile = static_cast<int64_t>(threads) * B * (in_place ? 1 : kCopy);
+  const bool split = in_place && (widest + 256 * B - 1) / (256 * B) * rows * count < 1024;
+  const int64_t tile = static_cast<int64_t>(split ? 64 : threads) * B * (in_place ? 1 : kCopy);
   const dim3 grid(static_cast<unsigned>((widest + tile - 1) / tile), rows < 65535 ? rows : 65535, count);
   const dim3 block(threads);
   if (threads == 64) hipLaunchKernelGGL((reorder_copy_kernel<B, 64>), grid, block, 0, st, pl, K, rows, parents);
   else if (!in_place) hipLaunchKernelGGL((reorder_copy_kernel<B, 256>), grid, block, 0, st, pl, K, rows, parents);
+  else if (split && K <= 4)
+    hipLaunchKernelGGL((reorder_split_kernel<B, 1>), grid, block, 0, st, pl, K, batch, parents);
+  else if (split && K <= 8)
+    hipLaunchKernelGGL((reorder_split_kernel<B, 2>), grid, block, 0, st, pl, K, batch, parents);
+  else if (split && K <= 16)
+    hipLaunchKernelGGL((reorder_split_kernel<B, 4>), grid, block, 0, st, pl, K, batch, parents);
+  else if (split) hipLaunchKernelGGL((reorder_split_kernel<B, 8>), grid, block, 0, st, pl, K, batch, parents);
   else if (K <= 4) hipLaunchKernelGGL((reorder_in_place_kernel<B, 4>), grid, block, 0, st, pl, K, batch, parents);
   else if (K <= 8) hipLaunchKernelGGL((reorder_in_place_kernel<B, 8>), grid, block, 0, st, pl, K, batch, parents);
   else if (K <= 16) hipLaunchKernelGGL((reorder_in_place_kernel<B, 16>), grid, block, 0, st, pl, K, batch, parents);
