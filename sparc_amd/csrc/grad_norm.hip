@@ -3,7 +3,7 @@
 //
 // The tensors' addresses and sizes travel as kernel arguments (kMaxTensors per
 // launch), so a call copies nothing to the device and can be captured.  Each
-// tensor is cut into pieces of kPieceValues values; the workgroups of a launch
+// tensor is cut into pieces of 4096 to 16384 values; the workgroups of a launch
 // walk the pieces of all its tensors, and each leaves one partial sum of
 // squares.  The sums are kept in fp64: squares of fp32 values neither overflow
 // nor vanish there, and at the memory's rate the fp64 units are nearly idle.
@@ -20,7 +20,8 @@ namespace sparc {
 namespace {
 
 constexpr int kMaxTensors = 256;      // per launch: 3.6 KB of kernel arguments
-constexpr int kPieceValues = 16384;
+constexpr int kMostPiece = 16384;     // values of a piece at most
+constexpr int kLeastPiece = 4096;
 constexpr int kMaxGroups = 1024;      // partial sums per launch
 constexpr int kThreads = 256;
 
@@ -29,9 +30,10 @@ struct TensorList {
   uint32_t first[kMaxTensors + 1];    // first piece of each tensor
   uint16_t last[kMaxTensors];         // values of its last piece, and kNarrow for bf16 values
   int count;
+  int piece;                          // values of a piece
 };
 constexpr uint16_t kNarrow = 0x8000;
-static_assert(kPieceValues < kNarrow, "a piece's values beside the flag");
+static_assert(kMostPiece < kNarrow, "a piece's values beside the flag");
 
 // A launch's list in LDS: one trip to the kernel arguments for all threads,
 // where a search among them would make one for each of its steps.
@@ -61,12 +63,12 @@ struct ListInLds {
   }
   // f(first byte, end, whether bf16) for a piece
   template <typename F>
-  __device__ __forceinline__ void piece(uint32_t p, int count, F&& f) const {
+  __device__ __forceinline__ void piece(uint32_t p, int count, int piece_values, F&& f) const {
     const int t = __builtin_amdgcn_readfirstlane(tensor_of(p, count));
     const bool narrow = last[t] & kNarrow;
-    const int64_t values = p + 1 < first[t + 1] ? kPieceValues : last[t] & (kNarrow - 1);
+    const int64_t values = p + 1 < first[t + 1] ? piece_values : last[t] & (kNarrow - 1);
     const int size_of = narrow ? 2 : 4;
-    const uintptr_t at = reinterpret_cast<uintptr_t>(data[t]) + int64_t(p - first[t]) * kPieceValues * size_of;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(data[t]) + int64_t(p - first[t]) * piece_values * size_of;
     f(at, at + values * size_of, narrow);
   }
 };
@@ -173,8 +175,8 @@ __device__ __forceinline__ double group_total(double v, double* red) {
   return s;
 }
 
-// 909 MB of bf16 gradients in 133 tensors: 135 us (6.7 TB/s); 1.1 MB in 12: 6.4 us,
-// most of it the launch with its 3.6 KB of arguments and a trip to memory.
+// 909 MB of bf16 gradients in 133 tensors: 135 us (6.7 TB/s); 1.1 MB in 12: 5.4 us,
+// most of it the launch and three trips to memory, one after the other.
 __global__ void __launch_bounds__(kThreads)
 sum_squares_kernel(TensorList l, double* part) {
   __shared__ double red[kThreads / 64];
@@ -183,7 +185,7 @@ sum_squares_kernel(TensorList l, double* part) {
   double s0 = 0.0, s1 = 0.0;
   const uint32_t pieces = l.first[l.count];
   for (uint32_t p = blockIdx.x; p < pieces; p += gridDim.x) {
-    list.piece(p, l.count, [&](uintptr_t at, uintptr_t end, bool narrow) {
+    list.piece(p, l.count, l.piece, [&](uintptr_t at, uintptr_t end, bool narrow) {
       if (narrow) add_squares<bf16>(at, end, s0, s1);
       else add_squares<float>(at, end, s0, s1);
     });
@@ -233,7 +235,7 @@ __device__ __forceinline__ void scale_piece(uintptr_t at, uintptr_t end, float f
       });
 }
 
-// Reads and writes everything: 909 MB 317 us (5.7 TB/s), 1.1 MB 4.5 us; nothing
+// Reads and writes everything: 909 MB 317 us (5.7 TB/s), 1.1 MB 3.7 us; nothing
 // but the partial sums where nothing is clipped.
 __global__ void __launch_bounds__(kThreads)
 clip_kernel(TensorList l, const double* part, int n, float max_norm, float* norm) {
@@ -247,7 +249,7 @@ clip_kernel(TensorList l, const double* part, int n, float max_norm, float* norm
   const uint32_t pieces = l.first[l.count];
   for (uint32_t q = blockIdx.x; q < pieces; q += gridDim.x) {
     const uint32_t p = pieces - 1 - q;  // backwards: what is still in a cache is what was read last
-    list.piece(p, l.count, [&](uintptr_t at, uintptr_t end, bool narrow) {
+    list.piece(p, l.count, l.piece, [&](uintptr_t at, uintptr_t end, bool narrow) {
       if (narrow) scale_piece<bf16>(at, end, f);
       else scale_piece<float>(at, end, f);
     });
@@ -260,16 +262,17 @@ clip_kernel(TensorList l, const double* part, int n, float max_norm, float* norm
 // The next list of up to kMaxTensors tensors with values, from ``at`` on; where
 // they begin again is returned
 int64_t next_list(int64_t count, void* const* data, const int64_t* sizes, const int32_t* dtypes, int64_t at,
-                  TensorList& l) {
+                  int piece, TensorList& l) {
   l.count = 0;
+  l.piece = piece;
   uint32_t pieces = 0;
   for (; at < count && l.count < kMaxTensors; ++at) {
     if (sizes[at] == 0) continue;
     l.data[l.count] = data[at];
-    l.last[l.count] = static_cast<uint16_t>((sizes[at] - 1) % kPieceValues + 1) |
+    l.last[l.count] = static_cast<uint16_t>((sizes[at] - 1) % piece + 1) |
                       (dtypes[at] == SPARC_BF16 ? kNarrow : uint16_t(0));
     l.first[l.count++] = pieces;
-    pieces += static_cast<uint32_t>((sizes[at] + kPieceValues - 1) / kPieceValues);
+    pieces += static_cast<uint32_t>((sizes[at] + piece - 1) / piece);
   }
   l.first[l.count] = pieces;
   return at;
@@ -277,6 +280,17 @@ int64_t next_list(int64_t count, void* const* data, const int64_t* sizes, const 
 unsigned list_groups(const TensorList& l) {
   const uint32_t p = l.first[l.count];
   return p < kMaxGroups ? p : kMaxGroups;
+}
+
+// Values of a piece: few tensors' values are spread over more workgroups, down to
+// 4 accesses per thread (1.1 MB of fp32 in 12 tensors: 9 us for both launches
+// instead of 13)
+int piece_of(int64_t count, const int64_t* sizes) {
+  int64_t total = 0;
+  for (int64_t i = 0; i < count; ++i) total += sizes[i];
+  int piece = kLeastPiece;
+  while (piece < kMostPiece && total > static_cast<int64_t>(piece) * kMaxGroups) piece *= 2;
+  return piece;
 }
 
 sparc_status gn_check(int64_t count, void* const* data, const int64_t* sizes, const int32_t* dtypes) {
@@ -322,9 +336,10 @@ sparc_status check_apart(int64_t count, void* const* data, const int64_t* sizes,
 int launch_sums(hipStream_t st, int64_t count, void* const* data, const int64_t* sizes, const int32_t* dtypes,
                 double* part) {
   int n = 0;
+  const int piece = piece_of(count, sizes);
   TensorList l;
   for (int64_t at = 0; at < count;) {
-    at = next_list(count, data, sizes, dtypes, at, l);
+    at = next_list(count, data, sizes, dtypes, at, piece, l);
     if (l.count == 0) break;
     hipLaunchKernelGGL(sum_squares_kernel, dim3(list_groups(l)), dim3(kThreads), 0, st, l, part + n);
     n += static_cast<int>(list_groups(l));
@@ -377,10 +392,11 @@ sparc_status sparc_clip_grad_norm(int64_t count, void* const* tensors, const int
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   double* part = static_cast<double*>(workspace);
   const int n = launch_sums(st, count, tensors, sizes, dtypes, part);
+  const int piece = piece_of(count, sizes);
   TensorList l;
   bool any = false;
   for (int64_t at = 0; at < count;) {
-    at = next_list(count, tensors, sizes, dtypes, at, l);
+    at = next_list(count, tensors, sizes, dtypes, at, piece, l);
     if (l.count == 0) break;
     hipLaunchKernelGGL(clip_kernel, dim3(list_groups(l)), dim3(kThreads), 0, st, l, part, n, max_norm,
                        any ? nullptr : norm);
