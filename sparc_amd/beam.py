@@ -79,23 +79,22 @@ def reorder_states(states: Sequence, parents: torch.Tensor, out_states: Sequence
 
 def _reorder(states, parents, out_states):
     planes = _planes(states)
-    out = None
-    if out_states is not None:
-        out = _planes(out_states)
-        _check_out(planes, out)
+    out = None if out_states is None else planes if out_states is states else _planes(out_states)
     new = _lib.native().reorder(planes, parents, out)
     if new is None:
-        _refuse_states(planes, parents, out or ())
+        _refuse_states(planes, parents, out)
     return _like(states, new)
 
 
 def _refuse_states(planes, parents, out):
     """Raise what is wrong with the states."""
+    if out is not None:
+        _check_out(planes, out)
     rows = parents.numel()
     for p in planes:
         if not p.ndim or p.shape[0] != rows:
             raise ValueError(f"states must have {rows} rows (one per beam), got {list(p.shape)}")
-    _lib.require_gpu(parents, *planes, *out)
+    _lib.require_gpu(parents, *planes, *(out or ()))
     for p in planes:
         if rows and p.numel() // rows * p.element_size() % 2:
             raise ValueError("state rows must have an even number of bytes")
