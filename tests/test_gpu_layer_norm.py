@@ -178,3 +178,21 @@ def test_equal_calls_give_equal_bits_on_any_stream():
         again = torch.autograd.grad(sparc_amd.layer_norm(*leaves), leaves, dy)
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(p, q) for p, q in zip(first, again))
+
+
+@pytest.mark.parametrize("given", ["xwb", "xw", "xb", "x"])
+def test_gradients_of_some_inputs_only(given):
+    """Every choice of inputs that want a gradient, with parameters that are there
+    and not, and a gradient of y that is one row expanded."""
+    print(f"[case] layer norm gradients of some of {given}", flush=True)
+    x, w, b, _ = _case(9, 40, F32, F32, 3)
+    dy = torch.linspace(-1.0, 2.0, 40).expand(9, 40)
+    dx, dw, db = L.layer_norm_grads(x, w if "w" in given else None, 1e-5, dy)
+    want = {"x": dx, "w": dw, "b": db}
+    for pick in range(1, 1 << len(given)):
+        wanted = [n for i, n in enumerate(given) if pick >> i & 1]
+        t = {n: v.cuda().requires_grad_(n in wanted) for n, v in zip("xwb", (x, w, b)) if n in given}
+        y = sparc_amd.layer_norm(t["x"], t.get("w"), t.get("b"))
+        grads = torch.autograd.grad(y, [t[n] for n in wanted], dy[0].cuda().expand(9, 40))
+        for n, g in zip(wanted, grads):
+            _close(g, want[n], f"d{n} of {wanted}", scale=1.0 if n == "x" else 4.0)
