@@ -9,17 +9,17 @@
 //
 // The backward sorts the token positions by id (a stable radix sort, digits of
 // up to 9 bits: two passes up to 2^18 ids), so that the positions of one id
-// stand together in their order in the batch.  Up to 4096 positions one
-// workgroup sorts them in LDS, ids and positions packed into 32 bits; more of
-// them, or ids that do not fit beside the positions, take a counting and a
-// scattering launch per pass (and one between them with many tiles).  Pieces of
-// sorted positions are then summed side by side, whatever the ids' frequencies:
-// a run of equal ids inside a piece is written to its row at once; a run that
-// crosses pieces leaves one fp32 partial row per piece, joined in order by a
-// second kernel.  Every sum has a fixed order, so dW does
-// not depend on timing.  The sort keeps few CUs busy and is bound by latency, so
-// further workgroups of its launches clear dW meanwhile, a share each; the rows
-// that tokens name are then written once more.
+// stand together in their order in the batch.  Up to kFew positions one launch
+// does it all; up to 4096 one workgroup sorts them in LDS, ids and positions packed
+// into 32 bits; more of them, or ids that do not fit beside the positions, take a
+// counting and a scattering launch per pass (and one between them with many tiles).
+// Pieces of sorted positions are then summed side by side, whatever the ids'
+// frequencies: a run of equal ids inside a piece is written to its row at once; a
+// run that crosses pieces leaves one fp32 partial row per piece, joined in order by
+// a second kernel.  Every sum has a fixed order, so dW does not depend on timing.
+// The sort keeps few CUs busy and is bound by latency, so further workgroups of its
+// launches clear dW meanwhile, a share each; the rows that tokens name are then
+// written once more.
 
 #include "rows.h"
 
@@ -107,17 +107,20 @@ struct SortPass {
   char* dw;               // this launch's share of dW, in bytes
   int64_t dw_bytes;
 
-  // by the workgroups behind the sorting ones
-  __device__ __forceinline__ void clear() const {
+  // by the workgroups behind the sorting ones, a stretch each (1 GB: 207 us; every
+  // workgroup's stores spread over all of it 267)
+  __device__ __forceinline__ void clear() const { clear(blockIdx.x - tiles, gridDim.x - tiles); }
+  // by workgroup g of ``groups``
+  __device__ __forceinline__ void clear(int64_t g, int64_t groups) const {
     const uintptr_t at = reinterpret_cast<uintptr_t>(dw);
     const int64_t head = static_cast<int64_t>((16 - at % 16) % 16) < dw_bytes ? (16 - at % 16) % 16 : dw_bytes;
-    const int64_t vecs = (dw_bytes - head) / 16, tail = head + vecs * 16;
-    const int64_t step = static_cast<int64_t>(gridDim.x - tiles) * blockDim.x;
-    const int64_t t = static_cast<int64_t>(blockIdx.x - tiles) * blockDim.x + threadIdx.x;
+    const int64_t vecs = (dw_bytes - head) / 16, tail = head + vecs * 16, each = (vecs + groups - 1) / groups;
+    const int64_t end = (g + 1) * each < vecs ? (g + 1) * each : vecs;
+    const int t = threadIdx.x;
     uint4* const body = reinterpret_cast<uint4*>(dw + head);
-    for (int64_t v = t; v < vecs; v += step) body[v] = make_uint4(0, 0, 0, 0);
-    if (t < head) dw[t] = 0;
-    if (tail + t < dw_bytes) dw[tail + t] = 0;
+    for (int64_t v = g * each + t; v < end; v += blockDim.x) body[v] = make_uint4(0, 0, 0, 0);
+    if (g == 0 && t < head) dw[t] = 0;
+    if (g == 0 && tail + t < dw_bytes) dw[tail + t] = 0;
   }
   // The keys of ITEMS positions from ``at`` on, ``step`` apart, all read at
   // once.  A key is the position's id, or vocab (behind every row) where it
@@ -591,6 +594,80 @@ embed_join_kernel(int64_t N, int piece_len, int64_t vocab, int D, const uint32_t
 }
 
 // ---------------------------------------------------------------------------
+// few positions
+// ---------------------------------------------------------------------------
+// Up to kFew positions in one launch: every workgroup sorts them all (a position's
+// place is the number of those that come before it, N LDS reads), clears its share
+// of dW's rows and sums the runs of the ids among them, a wave per run and 64
+// vectors of columns.  64 positions of 64 columns: 6.4 us instead of 14.3 in three
+// launches, 128 of 768 with 32768 rows 16.7 and 21.4, and what two launches cost the
+// host; only 128 times the same id take longer, 23 and 14 (256: 45 and 14).
+constexpr int kFew = 128;
+constexpr int kFewThreads = 256;
+template <typename IO>
+__global__ void __launch_bounds__(kFewThreads)
+embed_few_kernel(SortPass p, int D, int64_t rows_each, const void* dy, float scale, void* dw) {
+  constexpr int V = kVec<IO>;
+  __shared__ uint32_t key_in[kFew], key[kFew], pos[kFew];
+  __shared__ int start[kFew], starts;
+  const int N = static_cast<int>(p.n), i = threadIdx.x;
+  if (i < N) {
+    uint32_t one[1];
+    p.load_keys<1>(i, 1, one);
+    key_in[i] = one[0];
+  }
+  if (i == 0) starts = 0;
+  const int64_t r0 = blockIdx.x * rows_each, r1 = r0 + rows_each < p.vocab ? r0 + rows_each : p.vocab;
+  p.dw = static_cast<char*>(dw) + r0 * D * sizeof(IO);
+  p.dw_bytes = (r1 - r0) * D * static_cast<int64_t>(sizeof(IO));
+  p.clear(0, 1);
+  __syncthreads();
+  if (i < N) {
+    const uint32_t own = key_in[i];
+    int at = 0;
+    for (int k = 0; k < N; ++k) at += key_in[k] < own || (key_in[k] == own && k < i);
+    key[at] = own;
+    pos[at] = i;
+  }
+  __syncthreads();
+  if (i < N && key[i] >= r0 && key[i] < r1 && (i == 0 || key[i - 1] != key[i])) start[atomicAdd(&starts, 1)] = i;
+  __syncthreads();  // behind the clearing too: the rows are written once more
+  const int lane = i & 63, wave = __builtin_amdgcn_readfirstlane(i >> 6);
+  const int blocks = (D + 64 * V - 1) / (64 * V), jobs = starts * blocks;
+  const int64_t last = p.n * D - V;
+  for (int job = wave; job < jobs; job += kFewThreads / 64) {
+    const int run = job / blocks, c = ((job - run * blocks) * 64 + lane) * V;
+    if (c >= D) continue;
+    const int a = start[run];
+    const uint32_t id = key[a];
+    float acc[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) acc[k] = 0.0f;
+    for (int q = a; q < N && key[q] == id; q += kBatch) {
+      int64_t from[kBatch];
+      Vec<IO> raw[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) from[k] = static_cast<int64_t>(pos[q + k < N ? q + k : N - 1]) * D + c;
+      if (last >= 0) {  // whole vectors, as above
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) raw[k] = load_vec<IO>(dy, from[k] < last ? from[k] : last, V);
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        if (q + k < N && key[q + k] == id) {
+          if (from[k] > last) raw[k] = load_vec<IO>(dy, from[k], D - c);
+          float v[V];
+          unpack<IO, V>(raw[k], v);
+#pragma unroll
+          for (int e = 0; e < V; ++e) acc[e] += v[e];
+        }
+      }
+    }
+    write_row<IO>(dw, id, D, c, acc, scale);
+  }
+}
+
+// ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
 sparc_status em_check(int64_t n, int64_t vocab, int64_t dim, int32_t io, int32_t id_bytes) {
@@ -737,6 +814,18 @@ void em_sums(hipStream_t st, int64_t n, int64_t vocab, int64_t dim, const uint32
   }
 }
 
+// As many workgroups as clear 16 KB each, and one for 4 positions at least, so that
+// a wave has one run
+template <typename IO>
+void em_few(hipStream_t st, const SortPass& p, int64_t dim, const void* dy, float scale, void* dw) {
+  const int64_t bytes = p.vocab * dim * static_cast<int64_t>(sizeof(IO));
+  int64_t groups = bytes / 16384 > p.n / 4 ? bytes / 16384 : p.n / 4;
+  groups = groups < 1 ? 1 : groups < 4096 ? groups : 4096;
+  const int64_t each = (p.vocab + groups - 1) / groups;
+  hipLaunchKernelGGL((embed_few_kernel<IO>), dim3(static_cast<unsigned>((p.vocab + each - 1) / each)),
+                     dim3(kFewThreads), 0, st, p, static_cast<int>(dim), each, dy, scale, dw);
+}
+
 }  // namespace
 }  // namespace sparc
 
@@ -796,6 +885,12 @@ sparc_status sparc_embedding_backward(int64_t n, int64_t vocab, int64_t dim, int
   int cur = 0;
   if (n == 0) {
     hipLaunchKernelGGL((sort_count_kernel<4>), dim3(clear.take(p, kSortThreads)), dim3(kSortThreads), 0, st, p);
+    return op_launched("embedding backward");
+  }
+  if (n <= kFew) {
+    p.first = 1;
+    if (io_dtype == SPARC_F32) em_few<float>(st, p, dim, dy, scale, dweight);
+    else em_few<sparc::bf16>(st, p, dim, dy, scale, dweight);
     return op_launched("embedding backward");
   }
   if (s.pos_bits) {

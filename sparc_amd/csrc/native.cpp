@@ -1,10 +1,10 @@
 // The torch binding of the operators around the stack: embedding, layer norm,
 // clipping, beam step.  Their calls are short, and what the host does for one is
 // most of the time of a small one: from Python through ctypes a lookup of 256 ids
-// took 7.6 us, from here 4.8; a beam step with 24 state planes 52 and 23; 64 ids
-// forward and gradient 45 to 87 and 34 to 56, because autograd runs a backward on a
-// thread of its own, where a node in Python costs it the interpreter beside the
-// launches.
+// took 7.6 us, from here 4.8; a beam step with 24 state planes 52 and 23; the layer
+// norm of 64 rows forward and backward 55 to 108 and 35 to 64, because autograd runs
+// a backward on a thread of its own, where a node in Python costs it the interpreter
+// beside the launches.
 //
 // Every function checks what the kernels assume and returns None for arguments
 // that it does not take; the Python callers then say what is wrong with them.

@@ -61,7 +61,8 @@ def test_widths(D, dtype):
     _check(300, 97, D, dtype, scale=math.sqrt(D), seed=D)
 
 
-@pytest.mark.parametrize("n,vocab", [(1, 1), (1, 500), (15, 9), (16, 9), (17, 9), (100, 1), (2048, 511), (2049, 512),
+@pytest.mark.parametrize("n,vocab", [(1, 1), (1, 500), (15, 9), (16, 9), (17, 9), (100, 1), (127, 300), (128, 40),
+                                     (129, 40), (2048, 511), (2049, 512),
                                      (5000, 32768), (5000, 300000)])
 @pytest.mark.parametrize("kind", ["zipf", "uniform", "same", "two", "runs"])
 def test_sizes_and_frequencies(n, vocab, kind):
