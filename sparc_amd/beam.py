@@ -68,7 +68,8 @@ def reorder_states(states: Sequence, parents: torch.Tensor, out_states: Sequence
     ``SPARCMixer.step``, in a list; ``parents``: [B, K] int64, K up to 32.
     ``out_states``: the same structure to write to; it may be ``states`` itself
     (in place: rows that stay are neither read nor written), but no tensor of it
-    may overlap another of the states.  By default fresh tensors are returned,
+    may overlap another of the states.  Outside ``torch.no_grad()`` a tensor
+    that requires grad is not written to.  By default fresh tensors are returned,
     which share one allocation where all states are of one shape and dtype.  A
     parent outside [0, K) gives a row of NaN."""
     if parents.ndim != 2 or parents.dtype != torch.int64 or not 1 <= parents.shape[1] <= MAX_BEAMS:

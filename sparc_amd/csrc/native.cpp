@@ -48,6 +48,12 @@ Tensor scratch(size_t bytes, const Tensor& like) {
   return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
 }
 Tensor contiguous(const optional<Tensor>& t) { return t ? t->contiguous() : Tensor(); }
+// Tensors that a call writes through their addresses: a backward that has saved one
+// must find that it is no longer what it was.  (Before the launch: torch refuses
+// inference tensors here, as in its own in-place operators.)
+void mark_written(const Tensors& tensors) {
+  for (const Tensor& t : tensors) t.unsafeGetTensorImpl()->bump_version();
+}
 
 // ---------------------------------------------------------------------------
 // embedding
@@ -196,6 +202,7 @@ optional<Tensor> grad_norm(const Tensors& tensors, optional<double> max_norm) {
     types.push_back(std::get<2>(key));
   }
   const c10::DeviceGuard guard(tensors[0].device());
+  if (max_norm) mark_written(tensors);
   const int64_t count = static_cast<int64_t>(data.size());
   Tensor norm = at::empty({}, tensors[0].options().dtype(at::kFloat));
   const size_t need = sparc_grad_norm_workspace_bytes(count);
@@ -308,6 +315,10 @@ optional<Tensors> reorder(const Tensors& planes, const Tensor& parents_in, const
     alike = alike && p.scalar_type() == planes[0].scalar_type() && p.sizes() == planes[0].sizes();
   }
   if (planes.empty()) return Tensors();
+  if (out && at::GradMode::is_enabled() &&
+      std::any_of(out->begin(), out->end(), [](const Tensor& t) { return t.requires_grad(); }))
+    throw std::runtime_error("reorder_states: a tensor of out_states requires grad, and writing to it has no backward: "
+                             "reorder it under torch.no_grad()");
   const at::NoGradGuard no_grad;
   const c10::DeviceGuard guard(parents_in.device());
   const Tensor parents = parents_in.contiguous();
@@ -320,6 +331,7 @@ optional<Tensors> reorder(const Tensors& planes, const Tensor& parents_in, const
           to[i].sizes() != planes[i].sizes() || !to[i].is_contiguous())
         return std::nullopt;
     if (!apart(planes, to)) return std::nullopt;
+    mark_written(to);
   } else if (alike) {
     to = fresh(planes.size(), planes[0]);
   } else {
