@@ -48,6 +48,17 @@ Tensor scratch(size_t bytes, const Tensor& like) {
   return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
 }
 Tensor contiguous(const optional<Tensor>& t) { return t ? t->contiguous() : Tensor(); }
+// No operator has a forward-mode derivative; without this a dual tensor that needs no
+// gradient would lose its tangent.  (Also under no_grad, which leaves that mode on.)
+void refuse_tangents(const char* what, std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    if (t && t->_fw_grad(0).defined())
+      throw std::runtime_error(std::string(what) + " has no forward-mode derivative");
+}
+void refuse_tangents(const char* what, const Tensors& tensors) {
+  for (const Tensor& t : tensors) refuse_tangents(what, {&t});
+}
+const Tensor* pointer(const optional<Tensor>& t) { return t ? &*t : nullptr; }
 // Tensors that a call writes through their addresses: a backward that has saved one
 // must find that it is no longer what it was.  (Before the launch: torch refuses
 // inference tensors here, as in its own in-place operators.)
@@ -103,6 +114,7 @@ optional<Tensor> embedding(const Tensor& tokens, const Tensor& weight, double sc
   const int64_t vocab = weight.size(0);
   if (padding && (*padding < -vocab || *padding >= vocab)) return std::nullopt;
   const int64_t padding_id = !padding ? -1 : *padding < 0 ? *padding + vocab : *padding;
+  refuse_tangents("embedding", {&weight});
   const c10::DeviceGuard guard(weight.device());
   if (weight.requires_grad() && at::GradMode::is_enabled())
     return Embedding::apply(weight, tokens.contiguous(), scale, padding_id);
@@ -170,6 +182,7 @@ optional<Tensor> layer_norm(const Tensor& x, const optional<Tensor>& weight, con
       return std::nullopt;
   }
   if (weight && bias && weight->scalar_type() != bias->scalar_type()) return std::nullopt;
+  refuse_tangents("layer_norm", {&x, pointer(weight), pointer(bias)});
   const c10::DeviceGuard guard(x.device());
   const auto wants = [](const optional<Tensor>& t) { return t && t->requires_grad(); };
   if ((x.requires_grad() || wants(weight) || wants(bias)) && at::GradMode::is_enabled())
@@ -185,6 +198,7 @@ optional<Tensor> grad_norm(const Tensors& tensors, optional<double> max_norm) {
   if (tensors.empty()) return std::nullopt;
   for (const Tensor& t : tensors)
     if (!beside(t, tensors[0]) || !is_io(t) || !t.is_non_overlapping_and_dense()) return std::nullopt;
+  refuse_tangents(max_norm ? "clip_grad_norm_" : "grad_norm", tensors);
   const size_t n = tensors.size();
   const at::NoGradGuard no_grad;
   using Key = std::tuple<void*, int64_t, int32_t>;
@@ -237,6 +251,7 @@ optional<std::tuple<Tensor, Tensor, Tensor, optional<Tensor>>> beam_step(const T
       (finished_in && (!eos || !is_beams(*finished_in, B, K, at::kBool, logits_in))) ||
       (eos && (*eos < 0 || *eos >= V)))
     return std::nullopt;
+  refuse_tangents("beam_search_step", {&logits_in, &scores_in});
   const at::NoGradGuard no_grad;
   const c10::DeviceGuard guard(logits_in.device());
   Tensor logits = logits_in;
@@ -315,6 +330,8 @@ optional<Tensors> reorder(const Tensors& planes, const Tensor& parents_in, const
     alike = alike && p.scalar_type() == planes[0].scalar_type() && p.sizes() == planes[0].sizes();
   }
   if (planes.empty()) return Tensors();
+  refuse_tangents("reorder_states", planes);
+  if (out) refuse_tangents("reorder_states", *out);
   if (out && at::GradMode::is_enabled() &&
       std::any_of(out->begin(), out->end(), [](const Tensor& t) { return t.requires_grad(); }))
     throw std::runtime_error("reorder_states: a tensor of out_states requires grad, and writing to it has no backward: "

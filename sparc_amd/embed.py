@@ -12,7 +12,8 @@ from . import _lib
 def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
               padding_idx: int | None = None) -> torch.Tensor:
     """``scale * weight[tokens]``, [*tokens.shape, D] in weight's dtype,
-    differentiable in ``weight`` (a dense gradient of its shape).
+    differentiable in ``weight`` (a dense gradient of its shape; once, and in
+    reverse mode only).
 
     ``tokens``: int64 or int32, any shape; ``weight``: [V, D], float32 or
     bfloat16.  ``padding_idx``: a row whose gradient is zero (its values are

@@ -13,7 +13,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
                eps: float = 1e-5) -> torch.Tensor:
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension
     (``torch.nn.functional.layer_norm``'s formula), differentiable in x, weight
-    and bias.
+    and bias (once, and in reverse mode only).
 
     ``x``: float32 or bfloat16, [..., D] for any D; ``weight`` and ``bias``: [D]
     or None, in x's dtype or in float32.  The arithmetic is fp32 and every

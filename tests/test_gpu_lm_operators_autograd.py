@@ -2,6 +2,7 @@
 as written, and what they have no derivative for is refused, never dropped."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import sparc_amd
 from oracle import lm_oracle as L
@@ -85,3 +86,56 @@ def test_clipping_under_no_grad_rules():
     norm = sparc_amd.clip_grad_norm_([w], 0.25)
     assert not norm.requires_grad
     assert ((w.grad.double() - want * (0.25 / (want.norm() + 1e-6))).abs() <= 2.0 ** -21 * want.abs()).all()
+
+
+# ---------------------------------------------------------------------------
+# what the operators have no rule for
+# ---------------------------------------------------------------------------
+NAMES = ("embedding", "layer_norm x", "layer_norm weight", "layer_norm bias", "grad_norm", "clip_grad_norm_",
+         "clip_grad_norm_ strided", "beam_search_step logits", "beam_search_step scores", "reorder_states",
+         "reorder_states into")
+
+
+def _calls(dual):
+    """Every operator with one input that ``dual`` makes of a tensor, over the
+    inputs."""
+    r = lambda *s: torch.randn(*s, device="cuda")  # noqa: E731
+    ids, parents = torch.tensor([1, 3], device="cuda"), torch.zeros(2, 3, dtype=torch.int64, device="cuda")
+    p = torch.nn.Parameter(torch.zeros(9, device="cuda"))
+
+    def clip():
+        p.grad = dual(r(9))
+        return sparc_amd.clip_grad_norm_([p], 0.5)
+
+    def strided_clip():
+        q = torch.nn.Parameter(torch.zeros(4, 3, device="cuda"))
+        q.grad = dual(r(4, 6))[:, ::2]
+        return sparc_amd.clip_grad_norm_([q], 0.5)
+
+    return {
+        "embedding": lambda: sparc_amd.embedding(ids, dual(r(5, 8))),
+        "layer_norm x": lambda: sparc_amd.layer_norm(dual(r(4, 8)), r(8), r(8)),
+        "layer_norm weight": lambda: sparc_amd.layer_norm(r(4, 8), dual(r(8)), r(8)),
+        "layer_norm bias": lambda: sparc_amd.layer_norm(r(4, 8), None, dual(r(8))),
+        "grad_norm": lambda: sparc_amd.grad_norm([r(3), dual(r(9))]),
+        "clip_grad_norm_": clip,
+        "clip_grad_norm_ strided": strided_clip,
+        "beam_search_step logits": lambda: sparc_amd.beam_search_step(dual(r(2, 3, 50)), r(2, 3)),
+        "beam_search_step scores": lambda: sparc_amd.beam_search_step(r(2, 3, 50), dual(r(2, 3))),
+        "reorder_states": lambda: sparc_amd.reorder_states([r(6, 4), dual(r(6, 8))], parents),
+        "reorder_states into": lambda: sparc_amd.reorder_states([r(6, 8)], parents, out_states=[dual(r(6, 8))]),
+    }
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_tangents_are_refused(name):
+    """No operator has a forward-mode derivative; a result without its tangent
+    would be a derivative of zero."""
+    print(f"[case] tangent {name}", flush=True)
+    with forward_ad.dual_level():
+        call = _calls(lambda t: forward_ad.make_dual(t, torch.ones_like(t)))[name]
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            call()
+    _calls(lambda t: t)[name]()
