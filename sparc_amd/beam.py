@@ -68,10 +68,12 @@ def reorder_states(states: Sequence, parents: torch.Tensor, out_states: Sequence
     ``SPARCMixer.step``, in a list; ``parents``: [B, K] int64, K up to 32.
     ``out_states``: the same structure to write to; it may be ``states`` itself
     (in place: rows that stay are neither read nor written), but no tensor of it
-    may overlap another of the states.  Outside ``torch.no_grad()`` a tensor
-    that requires grad is not written to.  By default fresh tensors are returned,
+    may overlap another of the states.  By default fresh tensors are returned,
     which share one allocation where all states are of one shape and dtype.  A
-    parent outside [0, K) gives a row of NaN."""
+    parent outside [0, K) gives a row of NaN.
+
+    There is no backward: outside ``torch.no_grad()`` tensors that require grad
+    are refused."""
     if parents.ndim != 2 or parents.dtype != torch.int64 or not 1 <= parents.shape[1] <= MAX_BEAMS:
         raise ValueError(f"parents must be [B, K] int64 with K from 1 to {MAX_BEAMS}, got {list(parents.shape)} "
                          f"{parents.dtype}")
@@ -118,7 +120,10 @@ def beam_search_step(logits: torch.Tensor, scores: torch.Tensor, finished: torch
     them NaN, and NaN ranks first, so that it shows.
 
     ``states``, ``out_states``: as in ``reorder_states``; the states come back
-    in the new beams' order.  Nothing waits for the device."""
+    in the new beams' order.  Nothing waits for the device.
+
+    There is no backward: outside ``torch.no_grad()`` tensors that require grad
+    are refused."""
     chosen = _lib.native().beam_step(logits, scores, finished, eos_id, MAX_BEAMS)
     if chosen is None:
         _refuse_step(logits, scores, finished, eos_id)

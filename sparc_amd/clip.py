@@ -48,7 +48,9 @@ def _checked(tensors):
 def grad_norm(tensors) -> torch.Tensor:
     """The L2 norm over all values of ``tensors`` (one or several, float32 and
     bfloat16 mixed, any shapes), a float32 scalar on their device.  Squares are
-    summed in fp64 in a fixed order: no overflow, equal calls give equal bits."""
+    summed in fp64 in a fixed order: no overflow, equal calls give equal bits.
+    There is no backward: outside ``torch.no_grad()`` tensors that require grad
+    are refused."""
     tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
     if not tensors:
         return torch.zeros(())
@@ -67,7 +69,8 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     small enough no gradient is written.  Gradients that overlap without being
     the same are refused.  A norm that is not finite goes into
     the gradients as it does in torch: NaN for NaN, 0 (NaN for the infinite
-    values) for infinity.  Parameters without a gradient are skipped."""
+    values) for infinity.  As in torch, the call is outside any graph, whatever
+    the grad mode.  Parameters without a gradient are skipped."""
     max_norm = float(max_norm)
     if math.isnan(max_norm) or max_norm < 0.0:
         raise ValueError(f"clip_grad_norm_ needs max_norm >= 0, got {max_norm}")

@@ -58,6 +58,17 @@ void refuse_tangents(const char* what, std::initializer_list<const Tensor*> tens
 void refuse_tangents(const char* what, const Tensors& tensors) {
   for (const Tensor& t : tensors) refuse_tangents(what, {&t});
 }
+// The same for calls without a backward: a graph must not end in them unnoticed.
+void refuse_gradients(const char* what, std::initializer_list<const Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : tensors)
+    if (t->requires_grad())
+      throw std::runtime_error(std::string(what) + " has no backward, and one of its tensors requires grad: call it "
+                               "under torch.no_grad() or on detached tensors");
+}
+void refuse_gradients(const char* what, const Tensors& tensors) {
+  for (const Tensor& t : tensors) refuse_gradients(what, {&t});
+}
 const Tensor* pointer(const optional<Tensor>& t) { return t ? &*t : nullptr; }
 // Tensors that a call writes through their addresses: a backward that has saved one
 // must find that it is no longer what it was.  (Before the launch: torch refuses
@@ -199,6 +210,7 @@ optional<Tensor> grad_norm(const Tensors& tensors, optional<double> max_norm) {
   for (const Tensor& t : tensors)
     if (!beside(t, tensors[0]) || !is_io(t) || !t.is_non_overlapping_and_dense()) return std::nullopt;
   refuse_tangents(max_norm ? "clip_grad_norm_" : "grad_norm", tensors);
+  if (!max_norm) refuse_gradients("grad_norm", tensors);
   const size_t n = tensors.size();
   const at::NoGradGuard no_grad;
   using Key = std::tuple<void*, int64_t, int32_t>;
@@ -252,6 +264,7 @@ optional<std::tuple<Tensor, Tensor, Tensor, optional<Tensor>>> beam_step(const T
       (eos && (*eos < 0 || *eos >= V)))
     return std::nullopt;
   refuse_tangents("beam_search_step", {&logits_in, &scores_in});
+  refuse_gradients("beam_search_step", {&logits_in, &scores_in});
   const at::NoGradGuard no_grad;
   const c10::DeviceGuard guard(logits_in.device());
   Tensor logits = logits_in;
@@ -331,11 +344,11 @@ optional<Tensors> reorder(const Tensors& planes, const Tensor& parents_in, const
   }
   if (planes.empty()) return Tensors();
   refuse_tangents("reorder_states", planes);
-  if (out) refuse_tangents("reorder_states", *out);
-  if (out && at::GradMode::is_enabled() &&
-      std::any_of(out->begin(), out->end(), [](const Tensor& t) { return t.requires_grad(); }))
-    throw std::runtime_error("reorder_states: a tensor of out_states requires grad, and writing to it has no backward: "
-                             "reorder it under torch.no_grad()");
+  refuse_gradients("reorder_states", planes);
+  if (out) {
+    refuse_tangents("reorder_states", *out);
+    refuse_gradients("reorder_states", *out);
+  }
   const at::NoGradGuard no_grad;
   const c10::DeviceGuard guard(parents_in.device());
   const Tensor parents = parents_in.contiguous();

@@ -139,3 +139,18 @@ def test_tangents_are_refused(name):
         with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
             call()
     _calls(lambda t: t)[name]()
+
+
+@pytest.mark.parametrize("name", ["grad_norm", "beam_search_step logits", "beam_search_step scores", "reorder_states"])
+def test_inputs_that_require_grad_are_refused(name):
+    """These calls have no backward: a graph that ends in them would lose its
+    gradient without a word."""
+    print(f"[case] graph into {name}", flush=True)
+    with pytest.raises(RuntimeError, match="no backward"):
+        _calls(lambda t: t.requires_grad_())[name]()
+    with pytest.raises(RuntimeError, match="no backward"):
+        _calls(lambda t: t.requires_grad_() * 2.0)[name]()
+    with torch.no_grad():
+        _calls(lambda t: t.requires_grad_())[name]()
+    with torch.inference_mode():
+        _calls(lambda t: t)[name]()
