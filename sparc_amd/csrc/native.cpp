@@ -13,6 +13,7 @@
 #include <stdexcept>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -48,6 +49,11 @@ Tensor scratch(size_t bytes, const Tensor& like) {
   return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
 }
 Tensor contiguous(const optional<Tensor>& t) { return t ? t->contiguous() : Tensor(); }
+// torch.jit.trace would record the allocation of a result and nothing that fills it.
+void refuse_tracing(const char* what) {
+  if (at::tracer::impl::is_dispatch_enabled())
+    throw std::runtime_error(std::string(what) + " cannot be traced");
+}
 // No operator has a forward-mode derivative; without this a dual tensor that needs no
 // gradient would lose its tangent.  (Also under no_grad, which leaves that mode on.)
 void refuse_tangents(const char* what, std::initializer_list<const Tensor*> tensors) {
@@ -119,6 +125,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
 };
 
 optional<Tensor> embedding(const Tensor& tokens, const Tensor& weight, double scale, optional<int64_t> padding) {
+  refuse_tracing("embedding");
   if (weight.dim() != 2 || weight.numel() == 0 || !is_io(weight) || !beside(weight, weight) ||
       (tokens.scalar_type() != at::kLong && tokens.scalar_type() != at::kInt) || !beside(tokens, weight))
     return std::nullopt;
@@ -186,6 +193,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 };
 
 optional<Tensor> layer_norm(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias, double eps) {
+  refuse_tracing("layer_norm");
   if (x.dim() < 1 || x.size(-1) < 1 || !(eps >= 0.0) || !is_io(x) || !beside(x, x)) return std::nullopt;
   for (const auto* p : {&weight, &bias}) {
     if (*p && ((*p)->dim() != 1 || (*p)->numel() != x.size(-1) ||
@@ -206,11 +214,13 @@ optional<Tensor> layer_norm(const Tensor& x, const optional<Tensor>& weight, con
 // ---------------------------------------------------------------------------
 // A tensor given twice counts once.  max_norm: scale to it.
 optional<Tensor> grad_norm(const Tensors& tensors, optional<double> max_norm) {
+  const char* const what = max_norm ? "clip_grad_norm_" : "grad_norm";
+  refuse_tracing(what);
   if (tensors.empty()) return std::nullopt;
   for (const Tensor& t : tensors)
     if (!beside(t, tensors[0]) || !is_io(t) || !t.is_non_overlapping_and_dense()) return std::nullopt;
-  refuse_tangents(max_norm ? "clip_grad_norm_" : "grad_norm", tensors);
-  if (!max_norm) refuse_gradients("grad_norm", tensors);
+  refuse_tangents(what, tensors);
+  if (!max_norm) refuse_gradients(what, tensors);
   const size_t n = tensors.size();
   const at::NoGradGuard no_grad;
   using Key = std::tuple<void*, int64_t, int32_t>;
@@ -257,6 +267,7 @@ optional<std::tuple<Tensor, Tensor, Tensor, optional<Tensor>>> beam_step(const T
                                                                          const Tensor& scores_in,
                                                                          const optional<Tensor>& finished_in,
                                                                          optional<int64_t> eos, int64_t most_beams) {
+  refuse_tracing("beam_search_step");
   if (logits_in.dim() != 3 || !is_io(logits_in) || !beside(logits_in, logits_in)) return std::nullopt;
   const int64_t B = logits_in.size(0), K = logits_in.size(1), V = logits_in.size(2);
   if (K < 1 || K > most_beams || V < 1 || !is_beams(scores_in, B, K, at::kFloat, logits_in) ||
@@ -333,6 +344,7 @@ bool apart(const Tensors& planes, const Tensors& out) {
 // contiguous), or in fresh tensors, which share an allocation where all planes are
 // alike.
 optional<Tensors> reorder(const Tensors& planes, const Tensor& parents_in, const optional<Tensors>& out) {
+  refuse_tracing("reorder_states");
   if (parents_in.dim() != 2 || parents_in.scalar_type() != at::kLong || !beside(parents_in, parents_in))
     return std::nullopt;
   const int64_t B = parents_in.size(0), K = parents_in.size(1), rows = B * K;

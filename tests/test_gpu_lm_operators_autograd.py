@@ -154,3 +154,19 @@ def test_inputs_that_require_grad_are_refused(name):
         _calls(lambda t: t.requires_grad_())[name]()
     with torch.inference_mode():
         _calls(lambda t: t)[name]()
+
+
+@pytest.mark.parametrize("name,grad", [("embedding", False), ("embedding", True), ("layer_norm x", False),
+                                       ("layer_norm x", True), ("grad_norm", False), ("clip_grad_norm_", False),
+                                       ("beam_search_step logits", False), ("reorder_states", False)])
+def test_tracing_is_refused(name, grad):
+    """A recorded call would be the allocation of its result and nothing that
+    fills it."""
+    print(f"[case] trace {name} grad={grad}", flush=True)
+
+    def traced(x):
+        out = _calls(lambda t: (t + 0.0 * x.detach()).requires_grad_(grad))[name]()
+        return out[0] if isinstance(out, (tuple, list)) else out
+
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(traced, (torch.zeros((), device="cuda"),), check_trace=False)
