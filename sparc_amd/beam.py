@@ -39,8 +39,8 @@ def _check_out(planes, out):
     for o, p in zip(out, planes):
         if o is not p:
             _lib.expect(o, p.shape, p.dtype, "out_states")
-        if not o.is_contiguous():
-            raise ValueError("out_states must be contiguous tensors")
+        if not o.is_contiguous() or o.is_conj() or o.is_neg():
+            raise ValueError("out_states must be contiguous tensors, no views that conjugate or negate")
         at, src, size = o.data_ptr(), p.data_ptr(), o.numel() * o.element_size()
         if size:
             spans.append((at, at + size, True))

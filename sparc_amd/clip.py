@@ -26,6 +26,16 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+def _copied(t: torch.Tensor) -> bool:
+    """Whether the kernels take a copy: of values with gaps, and of a view that
+    negates when it is read."""
+    return t.is_neg() or not _dense(t)
+
+
+def _copy(t: torch.Tensor) -> torch.Tensor:
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def _repeats(t: torch.Tensor) -> bool:
     """Whether the tensor may name one value more than once (an expanded view)."""
     reach = 0
@@ -56,7 +66,7 @@ def grad_norm(tensors) -> torch.Tensor:
         return torch.zeros(())
     norm = _lib.native().grad_norm(tensors, None)
     if norm is None:
-        norm = _dense_norm([t if _dense(t) else t.contiguous() for t in _checked(tensors)], None)
+        norm = _dense_norm([_copy(t) if _copied(t) else t for t in _checked(tensors)], None)
     return norm
 
 
@@ -83,11 +93,11 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
         return norm
     copies = []
     for i, g in enumerate(_checked(grads)):
-        if not _dense(g):
+        if _copied(g):
             if _repeats(g):
                 raise ValueError("a gradient names one value more than once (an expanded view): it cannot be scaled "
                                  "in place")
-            grads[i] = g.contiguous()
+            grads[i] = _copy(g)
             copies.append((g, grads[i]))
     norm = _dense_norm(grads, max_norm)
     with torch.no_grad():

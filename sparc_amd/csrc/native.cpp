@@ -48,7 +48,13 @@ void* address(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor scratch(size_t bytes, const Tensor& like) {
   return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
 }
-Tensor contiguous(const optional<Tensor>& t) { return t ? t->contiguous() : Tensor(); }
+// The values as they lie in memory: not those of a view that conjugates or negates
+// when torch reads it (z.conj(), and its imaginary part)
+bool is_literal(const Tensor& t) { return !t.is_conj() && !t.is_neg(); }
+Tensor contiguous(const Tensor& t) {
+  return is_literal(t) ? t.contiguous() : t.clone(at::MemoryFormat::Contiguous);
+}
+Tensor contiguous(const optional<Tensor>& t) { return t ? contiguous(*t) : Tensor(); }
 // torch.jit.trace would record the allocation of a result and nothing that fills it.
 void refuse_tracing(const char* what) {
   if (at::tracer::impl::is_dispatch_enabled())
@@ -104,11 +110,11 @@ struct Embedding : torch::autograd::Function<Embedding> {
     ctx->saved_data["vocab"] = weight.size(0);
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["padding_id"] = padding_id;
-    return embedding_forward(tokens, weight.contiguous(), scale);
+    return embedding_forward(tokens, contiguous(weight), scale);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (at::GradMode::is_enabled()) throw std::runtime_error("embedding is not twice differentiable");
-    const Tensor tokens = ctx->get_saved_variables()[0], dy = grads[0].contiguous();
+    const Tensor tokens = ctx->get_saved_variables()[0], dy = contiguous(grads[0]);
     const c10::DeviceGuard guard(dy.device());
     const int64_t n = tokens.numel(), vocab = ctx->saved_data["vocab"].toInt(), dim = dy.size(-1);
     Tensor dw = at::empty({vocab, dim}, dy.options());
@@ -135,8 +141,8 @@ optional<Tensor> embedding(const Tensor& tokens, const Tensor& weight, double sc
   refuse_tangents("embedding", {&weight});
   const c10::DeviceGuard guard(weight.device());
   if (weight.requires_grad() && at::GradMode::is_enabled())
-    return Embedding::apply(weight, tokens.contiguous(), scale, padding_id);
-  return embedding_forward(tokens.contiguous(), weight.contiguous(), scale);
+    return Embedding::apply(weight, contiguous(tokens), scale, padding_id);
+  return embedding_forward(contiguous(tokens), contiguous(weight), scale);
 }
 
 // ---------------------------------------------------------------------------
@@ -158,7 +164,7 @@ Tensor layer_norm_forward(const Tensor& x, const Tensor& weight, const Tensor& b
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const optional<Tensor>& weight_in,
                         const optional<Tensor>& bias_in, double eps) {
-    const Tensor x = x_in.contiguous(), weight = contiguous(weight_in), bias = contiguous(bias_in);
+    const Tensor x = contiguous(x_in), weight = contiguous(weight_in), bias = contiguous(bias_in);
     const int64_t rows = x.numel() / x.size(-1);
     Tensor stats = at::empty({2, rows}, x.options().dtype(at::kFloat));
     float* mean = stats.data_ptr<float>();
@@ -172,7 +178,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     if (at::GradMode::is_enabled()) throw std::runtime_error("layer_norm is not twice differentiable");
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1], &stats = saved[2];
-    const Tensor dy = grads[0].contiguous();
+    const Tensor dy = contiguous(grads[0]);
     const c10::DeviceGuard guard(x.device());
     const int64_t cols = x.size(-1), rows = x.numel() / cols;
     const auto type = static_cast<at::ScalarType>(ctx->saved_data["parameters"].toInt());
@@ -206,7 +212,7 @@ optional<Tensor> layer_norm(const Tensor& x, const optional<Tensor>& weight, con
   const auto wants = [](const optional<Tensor>& t) { return t && t->requires_grad(); };
   if ((x.requires_grad() || wants(weight) || wants(bias)) && at::GradMode::is_enabled())
     return LayerNorm::apply(x, weight, bias, eps);
-  return layer_norm_forward(x.contiguous(), contiguous(weight), contiguous(bias), eps, nullptr, nullptr);
+  return layer_norm_forward(contiguous(x), contiguous(weight), contiguous(bias), eps, nullptr, nullptr);
 }
 
 // ---------------------------------------------------------------------------
@@ -218,7 +224,8 @@ optional<Tensor> grad_norm(const Tensors& tensors, optional<double> max_norm) {
   refuse_tracing(what);
   if (tensors.empty()) return std::nullopt;
   for (const Tensor& t : tensors)
-    if (!beside(t, tensors[0]) || !is_io(t) || !t.is_non_overlapping_and_dense()) return std::nullopt;
+    if (!beside(t, tensors[0]) || !is_io(t) || !t.is_non_overlapping_and_dense() || !is_literal(t))
+      return std::nullopt;
   refuse_tangents(what, tensors);
   if (!max_norm) refuse_gradients(what, tensors);
   const size_t n = tensors.size();
@@ -280,11 +287,12 @@ optional<std::tuple<Tensor, Tensor, Tensor, optional<Tensor>>> beam_step(const T
   const c10::DeviceGuard guard(logits_in.device());
   Tensor logits = logits_in;
   int64_t stride = K > 1 ? logits.stride(1) : B > 1 ? logits.stride(0) : V;
-  if ((V > 1 && logits.stride(2) != 1) || stride < V || (B > 1 && logits.stride(0) != K * stride)) {
-    logits = logits.contiguous();
+  if (!is_literal(logits) || (V > 1 && logits.stride(2) != 1) || stride < V ||
+      (B > 1 && logits.stride(0) != K * stride)) {
+    logits = contiguous(logits);
     stride = V;
   }
-  const Tensor scores = scores_in.contiguous(), finished = contiguous(finished_in);
+  const Tensor scores = contiguous(scores_in), finished = contiguous(finished_in);
   const auto make = [&](at::ScalarType type) { return at::empty({B, K}, scores.options().dtype(type)); };
   Tensor tokens = make(at::kLong), parents = make(at::kLong), new_scores = make(at::kFloat);
   optional<Tensor> new_finished;
@@ -363,14 +371,14 @@ optional<Tensors> reorder(const Tensors& planes, const Tensor& parents_in, const
   }
   const at::NoGradGuard no_grad;
   const c10::DeviceGuard guard(parents_in.device());
-  const Tensor parents = parents_in.contiguous();
+  const Tensor parents = contiguous(parents_in);
   Tensors to;
   if (out) {
     to = *out;
     if (to.size() != planes.size()) return std::nullopt;
     for (size_t i = 0; i < to.size(); ++i)
       if (!beside(to[i], parents) || to[i].scalar_type() != planes[i].scalar_type() ||
-          to[i].sizes() != planes[i].sizes() || !to[i].is_contiguous())
+          to[i].sizes() != planes[i].sizes() || !to[i].is_contiguous() || !is_literal(to[i]))
         return std::nullopt;
     if (!apart(planes, to)) return std::nullopt;
     mark_written(to);
@@ -384,7 +392,7 @@ optional<Tensors> reorder(const Tensors& planes, const Tensor& parents_in, const
   std::vector<void*> dst;
   std::vector<int64_t> bytes;
   for (size_t i = 0; i < planes.size(); ++i) {
-    from.push_back(planes[i].contiguous());
+    from.push_back(contiguous(planes[i]));
     src.push_back(from[i].data_ptr());
     dst.push_back(to[i].data_ptr());
     bytes.push_back(rows > 0 ? planes[i].numel() / rows * static_cast<int64_t>(planes[i].element_size()) : 0);

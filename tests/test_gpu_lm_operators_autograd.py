@@ -1,5 +1,6 @@
 """The operators around the stack and autograd: what they write in place counts
-as written, and what they have no derivative for is refused, never dropped."""
+as written, and what they have no derivative for is refused, never dropped;
+views whose values are not those in memory are read as torch reads them."""
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -170,3 +171,47 @@ def test_tracing_is_refused(name, grad):
 
     with pytest.raises(RuntimeError, match="traced"):
         torch.jit.trace(traced, (torch.zeros((), device="cuda"),), check_trace=False)
+
+
+# ---------------------------------------------------------------------------
+# tensors whose values are not those in memory
+# ---------------------------------------------------------------------------
+def test_conjugated_and_negated_views():
+    """A view that negates when it is read (``z.conj()``, and its imaginary
+    part) is read as what it stands for, and not written."""
+    print("[case] conj and neg views", flush=True)
+    z = torch.randn(6, 5, dtype=torch.complex64, device="cuda")
+    parents = torch.tensor([[2, 1, 0], [0, 0, 1]], device="cuda")
+    rows = L.reorder(torch.arange(6), parents.cpu()).cuda()
+    assert z.conj().is_conj()
+    out, = sparc_amd.reorder_states([z.conj()], parents)
+    assert torch.equal(out, z.conj()[rows])
+    t = torch.randn(6, 8, device="cuda")
+    neg = torch._neg_view(t)
+    assert neg.is_neg() and neg.is_contiguous()
+    out, = sparc_amd.reorder_states([neg], parents)
+    assert torch.equal(out, -t[rows])
+    w, b = torch.randn(8, device="cuda"), torch.randn(8, device="cuda")
+    assert torch.equal(sparc_amd.layer_norm(neg, w, b), sparc_amd.layer_norm(-t, w, b))
+    assert torch.equal(sparc_amd.layer_norm(t, torch._neg_view(w), torch._neg_view(b)), sparc_amd.layer_norm(t, -w, -b))
+    x = t.clone().requires_grad_()
+    dx, = torch.autograd.grad(sparc_amd.layer_norm(x, w, b), x, torch._neg_view(t))
+    assert torch.equal(dx, torch.autograd.grad(sparc_amd.layer_norm(x, w, b), x, -t)[0])
+    ids = torch.tensor([1, 5], device="cuda")
+    assert torch.equal(sparc_amd.embedding(ids, neg), -t[ids])
+    assert torch.equal(sparc_amd.embedding(torch._neg_view(-ids), t), t[ids])
+    dw, = torch.autograd.grad(sparc_amd.embedding(ids, x), x, torch._neg_view(t[:2]))
+    assert torch.equal(dw[ids], -t[:2])
+    logits, scores = torch.randn(2, 3, 50, device="cuda"), -torch.rand(2, 3, device="cuda")
+    got = sparc_amd.beam_search_step(torch._neg_view(logits), torch._neg_view(-scores))
+    want = sparc_amd.beam_search_step(-logits, scores)
+    assert torch.equal(got.scores, want.scores) and torch.equal(got.tokens, want.tokens)
+    assert torch.equal(sparc_amd.grad_norm([neg]), sparc_amd.grad_norm([t]))
+    for view, plane in ((torch._neg_view(t.clone()), t), (z.clone().conj(), z)):
+        with pytest.raises(ValueError, match="out_states"):
+            sparc_amd.reorder_states([plane], parents, out_states=[view])
+    p = torch.nn.Parameter(torch.zeros(6, 8, device="cuda"))
+    p.grad = torch._neg_view(t.clone())
+    want = -t.double() * (0.5 / (t.double().norm() + 1e-6))
+    sparc_amd.clip_grad_norm_([p], 0.5)
+    assert ((p.grad.double() - want).abs() <= 2.0 ** -21 * want.abs()).all()
