@@ -26,16 +26,6 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-def _copied(t: torch.Tensor) -> bool:
-    """Whether the kernels take a copy: of values with gaps, and of a view that
-    negates when it is read."""
-    return t.is_neg() or not _dense(t)
-
-
-def _copy(t: torch.Tensor) -> torch.Tensor:
-    return t.clone(memory_format=torch.contiguous_format)
-
-
 def _repeats(t: torch.Tensor) -> bool:
     """Whether the tensor may name one value more than once (an expanded view)."""
     reach = 0
@@ -64,10 +54,8 @@ def grad_norm(tensors) -> torch.Tensor:
     tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
     if not tensors:
         return torch.zeros(())
-    norm = _lib.native().grad_norm(tensors, None)
-    if norm is None:
-        norm = _dense_norm([_copy(t) if _copied(t) else t for t in _checked(tensors)], None)
-    return norm
+    norm = _lib.native().grad_norm(tensors, None, False)
+    return _copied_norm(_checked(tensors), None) if norm is None else norm
 
 
 def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
@@ -76,9 +64,10 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     returns ``norm`` (``torch.nn.utils.clip_grad_norm_`` for the L2 norm).
 
     Nothing waits for the device and nothing is read back; where the norm is
-    small enough no gradient is written.  Gradients that overlap without being
-    the same are refused.  A norm that is not finite goes into
-    the gradients as it does in torch: NaN for NaN, 0 (NaN for the infinite
+    small enough no gradient is scaled.  Gradients with gaps between their
+    values are scaled in copies, which are written back always.  Gradients that
+    overlap without being the same are refused.  A norm that is not finite goes
+    into the gradients as it does in torch: NaN for NaN, 0 (NaN for the infinite
     values) for infinity.  As in torch, the call is outside any graph, whatever
     the grad mode.  Parameters without a gradient are skipped."""
     max_norm = float(max_norm)
@@ -88,30 +77,20 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     grads = [g for g in [p.grad for p in parameters] if g is not None]
     if not grads:
         return torch.zeros(())
-    norm = _lib.native().grad_norm(grads, max_norm)
+    norm = _lib.native().grad_norm(grads, max_norm, False)
     if norm is not None:
         return norm
-    copies = []
-    for i, g in enumerate(_checked(grads)):
-        if _copied(g):
-            if _repeats(g):
-                raise ValueError("a gradient names one value more than once (an expanded view): it cannot be scaled "
-                                 "in place")
-            grads[i] = _copy(g)
-            copies.append((g, grads[i]))
-    norm = _dense_norm(grads, max_norm)
-    with torch.no_grad():
-        for g, c in copies:
-            g.copy_(c)
-    return norm
+    for g in _checked(grads):
+        if not _dense(g) and _repeats(g):
+            raise ValueError("a gradient names one value more than once (an expanded view): it cannot be scaled in "
+                             "place")
+    return _copied_norm(grads, max_norm)
 
 
-def _dense_norm(tensors, max_norm):
+def _copied_norm(tensors, max_norm):
+    """By way of copies where the values are not in a row in memory."""
     _lib.require_gpu(*tensors)
-    norm = _lib.native().grad_norm(tensors, max_norm)
-    if norm is None:
-        raise ValueError("gradients must be dense tensors")
-    return norm
+    return _lib.native().grad_norm(tensors, max_norm, True)
 
 
 __all__ = ["grad_norm", "clip_grad_norm_"]

@@ -9,6 +9,7 @@
 // Every function checks what the kernels assume and returns None for arguments
 // that it does not take; the Python callers then say what is wrong with them.
 #include <algorithm>
+#include <map>
 #include <set>
 #include <stdexcept>
 
@@ -59,6 +60,12 @@ Tensor contiguous(const optional<Tensor>& t) { return t ? contiguous(*t) : Tenso
 void refuse_tracing(const char* what) {
   if (at::tracer::impl::is_dispatch_enabled())
     throw std::runtime_error(std::string(what) + " cannot be traced");
+}
+// Bytes from the first value of a tensor with values to behind its last
+int64_t reach_of(const Tensor& t) {
+  int64_t reach = 1;
+  for (int64_t d = 0; d < t.dim(); ++d) reach += (t.size(d) - 1) * t.stride(d);
+  return reach * static_cast<int64_t>(t.element_size());
 }
 // No operator has a forward-mode derivative; without this a dual tensor that needs no
 // gradient would lose its tangent.  (Also under no_grad, which leaves that mode on.)
@@ -218,47 +225,113 @@ optional<Tensor> layer_norm(const Tensor& x, const optional<Tensor>& weight, con
 // ---------------------------------------------------------------------------
 // the gradients' norm
 // ---------------------------------------------------------------------------
-// A tensor given twice counts once.  max_norm: scale to it.
-optional<Tensor> grad_norm(const Tensors& tensors, optional<double> max_norm) {
+// A tensor's values from its first one on: every sum of i step with i up to most
+struct Term { int64_t step, most; };
+// Whether such a sum over the terms from the k-th on is ``rest``; steps falling,
+// reach[k]: the largest sum from there on.  Strides that nest leave two or three
+// values of i to try; after ``tries`` it is taken to be.
+bool reaches(const std::vector<Term>& terms, const std::vector<int64_t>& reach, size_t k, int64_t rest, int& tries) {
+  if (k == terms.size() || --tries < 0) return true;
+  const Term& t = terms[k];
+  const int64_t behind = rest - reach[k + 1], least = behind > 0 ? (behind + t.step - 1) / t.step : 0;
+  for (int64_t i = std::min(t.most, rest / t.step); i >= least; --i)
+    if (reaches(terms, reach, k + 1, rest - i * t.step, tries)) return true;
+  return false;
+}
+// Whether a and b, which starts no sooner, share a byte.  With i and j counting in a
+// and b, and j from its end: a value of a lies where one of b does if sum i step + sum
+// j step = b - a + the length of b.
+bool share_memory(const Tensor& a, const Tensor& b) {
+  std::map<int64_t, int64_t, std::greater<>> most;
+  int64_t rest = static_cast<char*>(b.data_ptr()) - static_cast<char*>(a.data_ptr());
+  const auto add = [&](const Tensor& t, int64_t of_length) {
+    const auto dimension = [&](int64_t step, int64_t n) {
+      if (n > 1 && step > 0) most[step] += n - 1;
+      rest += of_length * (n - 1) * step;
+    };
+    const int64_t size_of = static_cast<int64_t>(t.element_size());
+    for (int64_t d = 0; d < t.dim(); ++d) dimension(t.stride(d) * size_of, t.size(d));
+    dimension(1, size_of);
+  };
+  add(a, 0);
+  add(b, 1);
+  std::vector<Term> terms;
+  for (const auto& [step, n] : most) terms.push_back({step, n});
+  std::vector<int64_t> reach(terms.size() + 1, 0);
+  for (size_t k = terms.size(); k-- > 0;) reach[k] = reach[k + 1] + terms[k].step * terms[k].most;
+  int tries = 1 << 14;
+  return rest <= reach[0] && reaches(terms, reach, 0, rest, tries);
+}
+// Tensors with gaps must not share values: each is scaled in a copy of its own.
+void check_apart(Tensors tensors) {
+  std::sort(tensors.begin(), tensors.end(), [](const Tensor& a, const Tensor& b) { return a.data_ptr() < b.data_ptr(); });
+  for (size_t i = 0; i < tensors.size(); ++i) {
+    const auto end = static_cast<char*>(tensors[i].data_ptr()) + reach_of(tensors[i]);
+    for (size_t j = i + 1; j < tensors.size() && tensors[j].data_ptr() < end; ++j)
+      if (share_memory(tensors[i], tensors[j])) throw std::runtime_error("gradient clipping: two tensors overlap");
+  }
+}
+
+// A tensor given twice counts once.  max_norm: scale to it.  copies: also tensors with
+// gaps between their values and views that negate, by way of a copy.
+optional<Tensor> grad_norm(const Tensors& tensors, optional<double> max_norm, bool copies) {
   const char* const what = max_norm ? "clip_grad_norm_" : "grad_norm";
   refuse_tracing(what);
   if (tensors.empty()) return std::nullopt;
+  const auto in_place = [](const Tensor& t) { return t.is_non_overlapping_and_dense() && is_literal(t); };
   for (const Tensor& t : tensors)
-    if (!beside(t, tensors[0]) || !is_io(t) || !t.is_non_overlapping_and_dense() || !is_literal(t))
-      return std::nullopt;
+    if (!beside(t, tensors[0]) || !is_io(t) || !(copies || in_place(t))) return std::nullopt;
   refuse_tangents(what, tensors);
   if (!max_norm) refuse_gradients(what, tensors);
   const size_t n = tensors.size();
   const at::NoGradGuard no_grad;
-  using Key = std::tuple<void*, int64_t, int32_t>;
+  const c10::DeviceGuard guard(tensors[0].device());
+  // values in a row in memory, in whatever order, are one array; others have a layout
+  using Key = std::tuple<void*, int64_t, int32_t, bool, std::vector<int64_t>>;
   std::vector<void*> data;
   std::vector<int64_t> sizes;
   std::vector<int32_t> types;
+  std::vector<std::pair<Tensor, Tensor>> copied;  // and their copies
+  Tensors distinct;                               // with values, where there are copies
   std::set<Key> seen;
-  bool rising = true;  // addresses in order are no repeats: nothing to look up
+  bool rising = !copies;  // addresses in order are no repeats: nothing to look up
   for (size_t i = 1; i < n; ++i) rising = rising && tensors[i - 1].data_ptr() < tensors[i].data_ptr();
   for (const Tensor& t : tensors) {
-    const Key key(t.data_ptr(), t.numel(), code_of(t.scalar_type()));
-    if (!rising && !seen.insert(key).second) continue;
-    data.push_back(std::get<0>(key));
-    sizes.push_back(std::get<1>(key));
-    types.push_back(std::get<2>(key));
+    const bool direct = !copies || in_place(t);
+    if (!rising) {
+      std::vector<int64_t> layout;
+      if (!direct) {
+        layout = t.sizes().vec();
+        layout.insert(layout.end(), t.strides().begin(), t.strides().end());
+      }
+      if (!seen.insert(Key(t.data_ptr(), t.numel(), code_of(t.scalar_type()), t.is_neg(), std::move(layout))).second)
+        continue;
+    }
+    if (!direct) copied.emplace_back(t, contiguous(t));
+    if (copies && t.numel() > 0) distinct.push_back(t);
+    data.push_back((direct ? t : copied.back().second).data_ptr());
+    sizes.push_back(t.numel());
+    types.push_back(code_of(t.scalar_type()));
   }
-  const c10::DeviceGuard guard(tensors[0].device());
-  if (max_norm) mark_written(tensors);
+  if (max_norm) {
+    check_apart(std::move(distinct));
+    mark_written(tensors);
+  }
   const int64_t count = static_cast<int64_t>(data.size());
   Tensor norm = at::empty({}, tensors[0].options().dtype(at::kFloat));
   const size_t need = sparc_grad_norm_workspace_bytes(count);
   const Tensor ws = scratch(need, tensors[0]);
   float* out = norm.data_ptr<float>();
-  if (max_norm)
+  if (max_norm) {
     check(sparc_clip_grad_norm(count, data.data(), sizes.data(), types.data(), static_cast<float>(*max_norm), out,
                                ws.data_ptr(), need, stream_of(tensors[0])),
           "sparc_clip_grad_norm");
-  else
+    for (const auto& [t, copy] : copied) t.copy_(copy);
+  } else {
     check(sparc_grad_norm(count, data.data(), sizes.data(), types.data(), out, ws.data_ptr(), need,
                           stream_of(tensors[0])),
           "sparc_grad_norm");
+  }
   return norm;
 }
 
@@ -334,9 +407,7 @@ bool apart(const Tensors& planes, const Tensors& out) {
     if (out[i].numel() == 0) continue;
     spans.emplace_back(at, at + out[i].nbytes(), true);
     if (src == at) continue;
-    int64_t reach = 1;
-    for (int64_t d = 0; d < planes[i].dim(); ++d) reach += (planes[i].size(d) - 1) * planes[i].stride(d);
-    spans.emplace_back(src, src + reach * planes[i].element_size(), false);
+    spans.emplace_back(src, src + reach_of(planes[i]), false);
   }
   std::sort(spans.begin(), spans.end());
   uintptr_t end = 0, written_end = 0;

@@ -5,6 +5,7 @@ Tolerances: squares are summed in fp64 and the norm is rounded once (2^-24; 4
 of them allowed); a scaled value is one fp32 product with a factor that is off
 by at most 2^-22, rounded once more in bf16 (2^-8)."""
 import math
+import random
 
 import pytest
 import torch
@@ -167,3 +168,105 @@ def test_matches_torch_and_replays_in_a_graph():
         want = sparc_amd.clip_grad_norm_(eager, 0.25)
         torch.cuda.synchronize()
         assert torch.equal(norm, want) and all(torch.equal(p.grad, q.grad) for p, q in zip(mine, eager))
+
+
+def _strided(*grads):
+    params = [torch.nn.Parameter(torch.zeros(g.shape, dtype=g.dtype, device="cuda")) for g in grads]
+    for p, g in zip(params, grads):
+        p.grad = g
+    return params
+
+
+def test_a_strided_gradient_given_twice_counts_once():
+    print("[case] clip strided twice", flush=True)
+    wide = torch.randn(20, 30, device="cuda")
+    before = wide.double()
+    want = before[:, 2:11].norm()
+    p, = _strided(wide[:, 2:11])
+    for params in ([p, p], _strided(wide[:, 2:11], wide[:, 2:11]), [p, *_strided(torch.zeros(7, device="cuda"))]):
+        wide.copy_(before)
+        assert abs(float(sparc_amd.grad_norm([q.grad for q in params])) - float(want)) <= 2.0 ** -22 * float(want)
+        norm = sparc_amd.clip_grad_norm_(params, 0.25)
+        assert abs(float(norm) - float(want)) <= 2.0 ** -22 * float(want)
+        ref = before.clone()
+        ref[:, 2:11] *= 0.25 / (want + 1e-6)
+        assert ((wide.double() - ref).abs() <= 2.0 ** -21 * ref.abs()).all()
+
+
+def test_strided_gradients_that_overlap_are_refused():
+    """And those that only lie between one another are not."""
+    print("[case] clip strided overlap", flush=True)
+    wide = torch.ones(20, 30, device="cuda")
+    flat = wide.view(-1)
+    for grads in ((wide[:, :6], wide[:, 3:9]), (wide[:, 3:9], wide[:, :6]), (wide[:, :6], wide[5:9, 2:4]),
+                  (wide[:, ::2], wide[:, ::3]), (wide[:, :6], wide[::3]), (wide[:, :6], wide[4:6]),
+                  (wide[2:, :6].t(), wide[:5, 5:9]), (flat[::7], flat[3::5]),
+                  (wide[:, :6], wide[:, 10:], wide[:, 5:9]), (wide[::2, ::3], flat[100:250])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            sparc_amd.clip_grad_norm_(_strided(*grads), 0.5)
+    assert torch.equal(wide, torch.ones_like(wide))
+    for grads in ((wide[:, :6], wide[:, 6:12], wide[:, 12:]), (wide[:, ::2], wide[:, 1::2]), (wide[::2], wide[1::2, 3:]),
+                  (wide[:10, :6], wide[10:]), (wide[:, :6].t(), wide[:, 6:9]), (flat[::6], flat[3::4]),
+                  (wide[::2, ::3], wide[1::2, 1::2], wide[::2, 1::3])):
+        wide.fill_(1.0)
+        inside = torch.zeros_like(wide)
+        for g in grads:
+            inside.as_strided(g.shape, g.stride(), g.storage_offset()).add_(1.0)
+        count = float(inside.sum())
+        norm = sparc_amd.clip_grad_norm_(_strided(*grads), 0.5)
+        assert abs(float(norm) - math.sqrt(count)) <= 2.0 ** -22 * math.sqrt(count)
+        want = torch.where(inside > 0, 0.5 / (math.sqrt(count) + 1e-6), 1.0).double()
+        assert ((wide.double() - want).abs() <= 2.0 ** -21).all()
+
+
+def test_strided_gradients_of_both_types():
+    """bf16 values between fp32 ones of the same memory, and the same bytes under
+    both types."""
+    print("[case] clip strided types", flush=True)
+    buf = torch.zeros(12, 16, device="cuda")
+    half = buf.view(BF16)  # [12, 32]
+    params = _strided(buf[:, :8], half[:, 16:20], half[:, 20::2])
+    for p in params:
+        p.grad.fill_(0.5)
+    _check(params, 0.125)
+    with pytest.raises(RuntimeError, match="overlap"):
+        sparc_amd.clip_grad_norm_(_strided(buf[:, :8], half[:, 15:20]), 0.5)
+
+
+@pytest.mark.parametrize("strides", [(5, 3), (10, 2), (0, 0)])
+def test_gradients_without_values_in_any_layout(strides):
+    print(f"[case] clip empty strides {strides}", flush=True)
+    empty = torch.zeros(60, device="cuda").as_strided((0, 5), strides)
+    params = _params([(40,)], [F32], 12) + _strided(empty)
+    want = L.grad_norm([params[0].grad.cpu()])
+    assert abs(float(sparc_amd.grad_norm([p.grad for p in params])) - want) <= 2.0 ** -22 * want
+    _check(params, 0.01)
+
+
+def test_overlaps_of_any_two_layouts():
+    """Views with 1 to 3 dimensions and any strides without repeats: refused where,
+    and only where, two of them name one value."""
+    print("[case] clip overlap of any layouts", flush=True)
+    r = random.Random(7)
+    base, index, overlapping = torch.zeros(400, device="cuda"), torch.arange(400), 0
+    for _ in range(400):
+        views = []
+        while len(views) < 2:
+            shape, strides, reach = [], [], 0
+            for _ in range(r.randint(1, 3)):
+                shape.append(r.randint(1, 5))
+                strides.append(reach + r.randint(1, 7))
+                reach += strides[-1] * (shape[-1] - 1)
+            if reach < 150:
+                order = r.sample(range(len(shape)), len(shape))
+                views.append(([shape[k] for k in order], [strides[k] for k in order], r.randint(0, 200)))
+        sets = [set(index.as_strided(*v).reshape(-1).tolist()) for v in views]
+        params = _strided(*[base.as_strided(*v) for v in views])
+        same = views[0] == views[1]
+        if sets[0] & sets[1] and not same:
+            overlapping += 1
+            with pytest.raises(RuntimeError, match="overlap"):
+                sparc_amd.clip_grad_norm_(params, 0.5)
+        else:
+            sparc_amd.clip_grad_norm_(params, 0.5)
+    assert 50 < overlapping < 350
