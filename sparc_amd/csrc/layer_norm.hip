@@ -290,7 +290,8 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
         weight(k, p);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float xh = (xv[i] - mu) * r, g = c.once(i, dv[i] * p[i]);
+          // xhat too is 0 behind a short row's end: 0 - mu may overflow times r
+          const float xh = E == kShort && i >= c.n ? 0.0f : (xv[i] - mu) * r, g = c.once(i, dv[i] * p[i]);
           s[0] += g;
           s[1] = fmaf(g, xh, s[1]);
           aw[k][i] = fmaf(dv[i], xh, aw[k][i]);
@@ -433,7 +434,7 @@ layer_norm_dx_wide_kernel(int64_t R, int64_t D, const void* x, const void* w, co
     const int64_t base = row * D;
     const float mu = mean[row], r = rstd[row];
     float s[2] = {0.0f, 0.0f}, g[V], xh[V];
-    // g and xhat of the columns from c on (behind the row g is 0)
+    // g and xhat of the columns from c on, 0 behind the row
     const auto load = [&](int64_t c, int n) __attribute__((always_inline)) {
       unpack<IO, V>(load_vec<IO>(dy, base + c, n), g);
       unpack<IO, V>(load_vec<IO>(x, base + c, n), xh);
@@ -442,7 +443,7 @@ layer_norm_dx_wide_kernel(int64_t R, int64_t D, const void* x, const void* w, co
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         if (w) g[i] *= p[i];
-        xh[i] = (xh[i] - mu) * r;
+        xh[i] = i < n ? (xh[i] - mu) * r : 0.0f;
       }
     };
     for (int64_t c = c0; c < D; c += kWideThreads * V) {

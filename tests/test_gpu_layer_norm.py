@@ -196,3 +196,20 @@ def test_gradients_of_some_inputs_only(given):
         grads = torch.autograd.grad(y, [t[n] for n in wanted], dy[0].cuda().expand(9, 40))
         for n, g in zip(wanted, grads):
             _close(g, want[n], f"d{n} of {wanted}", scale=1.0 if n == "x" else 4.0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("D", [1, 2, 3, 5, 7])
+def test_short_rows_of_large_values(D, dtype):
+    """mean * rstd overflows: nothing of that comes from behind a row's end.
+    Rows whose mean is exact are taken, so that xhat is 0."""
+    print(f"[case] layer norm short rows of large values D={D} {dtype}", flush=True)
+    x = torch.tensor([2.0 ** 121, -2.0 ** 122, 1.0])[:, None].expand(3, D).to(dtype).contiguous()
+    _, w, b, dy = _case(3, D, dtype, F32, D)
+    leaves = [t.cuda().requires_grad_() for t in (x, w, b)]
+    y = sparc_amd.layer_norm(*leaves)
+    assert torch.equal(y, leaves[2].detach().to(dtype).expand_as(y))
+    dx, dw, db = torch.autograd.grad(y, leaves, dy.cuda())
+    assert not dw.any()
+    _close(dx, L.layer_norm_grads(x, w, 1e-5, dy)[0], "dx")
+    _close(db, dy.double().sum(0), "db", scale=4.0)
