@@ -5,8 +5,11 @@
 //   dw = sum over rows of dy xhat,  db = sum over rows of dy
 // in fp32 arithmetic: x, y, dy, dx in the I/O type, w, b, dw, db in the
 // parameter type (the I/O type, or fp32 beside bf16 I/O), each output rounded
-// once.  The variance is the mean of squared differences from the mean, taken
-// from registers, so a large mean costs no precision.
+// once.  The mean is taken about the row's first value, and the mean difference from
+// it is corrected by what is left of the differences, beside the sum of their squares:
+// a sum of the values themselves would be off by some units of a large mean, which a
+// nearly constant row's variance does not outweigh.  What remains of a mean that is
+// large beside the deviations is its own rounding to fp32.
 //
 // A row is held in registers by the L lanes that own it, 8 to 64 of a wave or a
 // workgroup of 256 to 1024, each NCH vectors of 16 bytes, at any alignment.  Rows
@@ -105,6 +108,15 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float (*red)[N][W], int&
   }
 }
 
+// The mean and 1 / sqrt(variance + eps) of a row from the means of x - about and of its
+// square.  (An infinite variance stays so.)
+__device__ __forceinline__ void finish_stats(float about, float diff, float square, float eps, float& mean,
+                                             float& rstd) {
+  mean = about + diff;
+  const float shift = diff * diff;
+  rstd = 1.0f / sqrtf((shift < square ? square - shift : square) + eps);
+}
+
 // The forward, a row per L lanes: one read and one write of each value, and bound
 // by them: 32768 x 768 bf16 22 us (50 MB read, 50 written: 4.6 TB/s), 8192 x 24576
 // 178 us (4.5 TB/s), 300000 x 64 16 us.  256 rows of 2048 take 3.5 us: the launch,
@@ -117,7 +129,7 @@ __global__ void __launch_bounds__(L <= 64 ? 64 * kRowWaves : L)
 layer_norm_fwd_kernel(int64_t R, int D, const void* x, const void* w, const void* b, float eps, void* y, float* mean,
                       float* rstd) {
   constexpr int V = kVec<IO>;
-  __shared__ float red[2][1][kWaves<L>];
+  __shared__ float red[2][1][kWaves<L>], red2[2][2][kWaves<L>];
   int turn = 0;
   const int t = threadIdx.x & (L - 1), per = L <= 64 ? blockDim.x / L : 1;
   int64_t first = static_cast<int64_t>(blockIdx.x) * per;
@@ -126,6 +138,7 @@ layer_norm_fwd_kernel(int64_t R, int D, const void* x, const void* w, const void
   const float inv_d = 1.0f / static_cast<float>(D);
   for (int64_t row = first; row < R; row += static_cast<int64_t>(gridDim.x) * per) {  // uniform over a row's lanes
     const int64_t base = row * D;
+    const float first_value = load1<IO>(x, base);
     Vec<IO> raw[NCH];
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
@@ -140,12 +153,12 @@ layer_norm_fwd_kernel(int64_t R, int D, const void* x, const void* w, const void
         float v[V];
         unpack<IO, V>(raw[k], v);
 #pragma unroll
-        for (int i = 0; i < V; ++i) s[0] += c.once(i, v[i]);
+        for (int i = 0; i < V; ++i) s[0] = fmaf(c.once(i, v[i] - first_value), inv_d, s[0]);
       }
     }
     row_sums<1, L>(s, red, turn);
-    const float mu = s[0] * inv_d;
-    s[0] = 0.0f;
+    const float about = first_value + s[0];
+    float m[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       const Columns<V, NCH, L, E> c(k, t, D);
@@ -154,13 +167,15 @@ layer_norm_fwd_kernel(int64_t R, int D, const void* x, const void* w, const void
         unpack<IO, V>(raw[k], v);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float d = c.once(i, v[i] - mu);
-          s[0] = fmaf(d, d, s[0]);
+          const float d = c.once(i, v[i] - about);
+          m[0] += d;
+          m[1] = fmaf(d, d, m[1]);
         }
       }
     }
-    row_sums<1, L>(s, red, turn);
-    const float r = 1.0f / sqrtf(s[0] * inv_d + eps);
+    row_sums<2, L>(m, red2, turn);
+    float mu, r;
+    finish_stats(about, m[0] * inv_d, m[1] * inv_d, eps, mu, r);
     if (t == 0 && mean) {
       mean[row] = mu;
       rstd[row] = r;
@@ -375,32 +390,36 @@ __global__ void __launch_bounds__(kWideThreads)
 layer_norm_fwd_wide_kernel(int64_t R, int64_t D, const void* x, const void* w, const void* b, float eps, void* y,
                            float* mean, float* rstd) {
   constexpr int V = kVec<IO>;
-  __shared__ float red[2][1][kWaves<kWideThreads>];
+  __shared__ float red[2][1][kWaves<kWideThreads>], red2[2][2][kWaves<kWideThreads>];
   int turn = 0;
   const float inv_d = 1.0f / static_cast<float>(D);
   const int64_t c0 = static_cast<int64_t>(threadIdx.x) * V;
   for (int64_t row = blockIdx.x; row < R; row += gridDim.x) {
     const int64_t base = row * D;
+    const float first_value = load1<IO>(x, base);
     float s[1] = {0.0f}, v[V];
     for (int64_t c = c0; c < D; c += kWideThreads * V) {
-      unpack<IO, V>(load_vec<IO>(x, base + c, left(D, c)), v);
+      const int n = left(D, c);
+      unpack<IO, V>(load_vec<IO>(x, base + c, n), v);
 #pragma unroll
-      for (int i = 0; i < V; ++i) s[0] += v[i];
+      for (int i = 0; i < V; ++i) s[0] = fmaf(i < n ? v[i] - first_value : 0.0f, inv_d, s[0]);
     }
     row_sums<1, kWideThreads>(s, red, turn);
-    const float mu = s[0] * inv_d;
-    s[0] = 0.0f;
+    const float about = first_value + s[0];
+    float m[2] = {0.0f, 0.0f};
     for (int64_t c = c0; c < D; c += kWideThreads * V) {
       const int n = left(D, c);
       unpack<IO, V>(load_vec<IO>(x, base + c, n), v);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float d = i < n ? v[i] - mu : 0.0f;
-        s[0] = fmaf(d, d, s[0]);
+        const float d = i < n ? v[i] - about : 0.0f;
+        m[0] += d;
+        m[1] = fmaf(d, d, m[1]);
       }
     }
-    row_sums<1, kWideThreads>(s, red, turn);
-    const float r = 1.0f / sqrtf(s[0] * inv_d + eps);
+    row_sums<2, kWideThreads>(m, red2, turn);
+    float mu, r;
+    finish_stats(about, m[0] * inv_d, m[1] * inv_d, eps, mu, r);
     if (threadIdx.x == 0 && mean) {
       mean[row] = mu;
       rstd[row] = r;

@@ -213,3 +213,84 @@ def test_short_rows_of_large_values(D, dtype):
     assert not dw.any()
     _close(dx, L.layer_norm_grads(x, w, 1e-5, dy)[0], "dx")
     _close(db, dy.double().sum(0), "db", scale=4.0)
+
+
+def _off_by_the_mean(x, rstd):
+    """How far xhat may be off where the mean is rounded to fp32: half a unit in
+    its last place, and as much again for the sums behind it."""
+    return 2.0 ** -23 * x.double().mean(-1, keepdim=True).abs() * rstd
+
+
+@pytest.mark.parametrize("D", [3, 64, 200, 768, 1001, 5000, 16388, 24577, 33001, 50001])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_constant_rows_of_any_value(D, dtype):
+    """The mean of a constant row is its value, to the last bit: xhat and the
+    weight's gradient are 0, y is the bias, and rstd is 1 / sqrt(eps).  (A sum of
+    D values and a product with 1 / D, each rounded, are some units off.)"""
+    print(f"[case] layer norm constant rows D={D} {dtype}", flush=True)
+    values = [1000.7, 12345.67, 1e6 + 0.3, -1e6 - 0.3, 1e-3, 0.0, torch.finfo(dtype).min]
+    x = torch.tensor(values, dtype=torch.float64).to(dtype)[:, None].expand(len(values), D).contiguous()
+    _, w, b, dy = _case(len(values), D, dtype, F32, D)
+    leaves = [t.cuda().requires_grad_() for t in (x, w, b)]
+    y = sparc_amd.layer_norm(*leaves)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy.cuda())
+    assert torch.equal(y, leaves[2].detach().to(dtype).expand_as(y))
+    assert torch.equal(y, sparc_amd.layer_norm(*[t.detach() for t in leaves]))
+    assert not dw.any()
+    _close(dx, L.layer_norm_grads(x, w, 1e-5, dy)[0], "dx")
+    _close(db, dy.double().sum(0), "db", scale=4.0)
+
+
+@pytest.mark.parametrize("D", [200, 768, 1001, 5000, 16388, 33001])
+@pytest.mark.parametrize("mean", [1000.7, 12345.67, 1e6 + 0.3])
+def test_nearly_constant_rows(D, mean):
+    """A spread of some units in the values' last place: the variance is that of
+    the values, and xhat is off by no more than the mean's rounding to fp32.
+    dx = rstd (g - mean(g) - xhat mean(g xhat)) is then off by rstd e (|mean(g
+    xhat)| + |xhat| mean|g|), e the error of xhat, and dw by e times the sum of
+    |dy|."""
+    print(f"[case] layer norm nearly constant rows D={D} mean={mean}", flush=True)
+    _, w, b, dy = _case(8, D, F32, F32, D)
+    g = torch.Generator().manual_seed(D)
+    x = (mean + mean * 2.0 ** -21 * torch.randn(8, D, generator=g, dtype=torch.float64)).float()
+    x[0, 1:] = x[0, 0]
+    x[0, D // 2] = x[0, 0] * (1.0 + 2.0 ** -20)  # one value off
+    leaves = [t.cuda().requires_grad_() for t in (x, w, b)]
+    y = sparc_amd.layer_norm(*leaves)
+    dx, dw, _ = torch.autograd.grad(y, leaves, dy.cuda())
+    x64, g64 = x.double(), dy.double() * w.double()
+    rstd = 1.0 / torch.sqrt(x64.var(-1, correction=0, keepdim=True) + 1e-5)
+    xhat = (x64 - x64.mean(-1, keepdim=True)) * rstd
+    e = _off_by_the_mean(x, rstd)
+    want, (want_x, want_w, _) = L.layer_norm(x, w, b, 1e-5), L.layer_norm_grads(x, w, 1e-5, dy)
+
+    def held(got, ref, bound):
+        off = (got.detach().cpu().double() - ref).abs() - bound - 2.0 ** -17 * ref.abs().max()
+        assert off.max() <= 0.0, f"{off.max().item():.3g} over the bound"
+
+    held(y, want, e * w.double().abs())
+    along = (g64 * xhat).mean(-1, keepdim=True).abs()
+    held(dx, want_x, rstd * e * (along + xhat.abs() * g64.abs().mean(-1, keepdim=True)))
+    held(dw, want_w, (e * dy.double().abs()).sum(0))
+
+
+@pytest.mark.parametrize("D", [768, 16388, 32768, 40001])
+def test_one_value_far_from_the_others(D):
+    """At either end of the row and between: no sum about a value that is far off."""
+    print(f"[case] layer norm one far value D={D}", flush=True)
+    x, w, b, _ = _case(3, D, F32, F32, D)
+    x[0, 0] = x[1, D // 2] = x[2, D - 1] = 1e4
+    y = sparc_amd.layer_norm(x.cuda(), w.cuda(), b.cuda()).cpu().double()
+    want = L.layer_norm(x, w, b, 1e-5)
+    xhat = L.layer_norm(x, None, None, 1e-5)
+    assert ((y - want).abs() <= 2.0 ** -17 * (w.double().abs() * (1.0 + xhat.abs()) + b.double().abs())).all()
+
+
+@pytest.mark.parametrize("pdtype", ["same", F32], ids=["same", "f32"])
+@pytest.mark.parametrize("D,dtype", [(28000, F32), (32768, F32), (32769, F32), (40001, F32), (49152, BF16), (49153, BF16),
+                                     (60007, BF16)])
+def test_the_widest_rows(D, dtype, pdtype):
+    """On both sides of what a workgroup holds in registers."""
+    print(f"[case] layer norm D={D} {dtype} {pdtype}", flush=True)
+    _check(5, D, dtype, dtype if pdtype == "same" else pdtype, seed=D)
+    _check(70, D, dtype, F32, bias=False, seed=D + 1)
