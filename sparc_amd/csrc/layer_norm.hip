@@ -640,8 +640,14 @@ int64_t bwd_groups(int64_t R) {
   if (L > 64 && n > 512) n = R / 8 > 512 ? (R / 8 < n ? R / 8 : n) : 512;
   return n;
 }
-constexpr int64_t kMostPartials = 1024;  // the largest bwd_groups (W = 4)
 constexpr int64_t kWideSlices = 64;
+// The most partial rows that a backward of rows of D columns leaves
+template <typename IO>
+int64_t most_partials(int64_t D) {
+  int64_t n = kWideSlices;
+  bwd_form<IO>(D, [&](auto NCH, auto L) { n = bwd_groups<NCH(), L()>(INT32_MAX); });
+  return n;
+}
 
 template <typename PT>
 void launch_reduce(hipStream_t st, int64_t n, int64_t D, const float* dw_part, const float* db_part, void* dw,
@@ -752,7 +758,9 @@ sparc_status sparc_layer_norm_forward(int64_t rows, int64_t cols, int32_t io_dty
 size_t sparc_layer_norm_workspace_bytes(int64_t rows, int64_t cols) {
   using namespace sparc;
   if (ln_check(rows, cols, SPARC_F32, SPARC_F32)) return 0;
-  const int64_t n = rows < kMostPartials ? rows : kMostPartials;
+  int64_t n = most_partials<float>(cols);
+  if (most_partials<bf16>(cols) > n) n = most_partials<bf16>(cols);
+  if (rows < n) n = rows;
   return static_cast<size_t>(2 * n) * static_cast<size_t>(cols) * sizeof(float) + 256;
 }
 

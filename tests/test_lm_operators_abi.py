@@ -208,3 +208,14 @@ def test_oracle_gradients_against_differences():
     dw, u = L.embedding_grad(tokens, 5, dy, 3.0), r(5, 3)
     diff = sum(s * (L.embedding(tokens, table + s * u, 3.0) * dy).nansum() for s in (1, -1)) / 2
     assert abs(float(diff - (dw * u).sum())) < 1e-12
+
+
+def test_layer_norm_workspace_holds_the_partial_rows():
+    """Two partial rows for each workgroup that the widths' forms launch, not more:
+    512 for rows of a wave, 1024 for 4 waves, 256 for 16, 64 for rows that no
+    workgroup holds."""
+    need = _lib.load().sparc_layer_norm_workspace_bytes
+    for rows, cols, partials in ((1 << 20, 768, 512), (1 << 20, 1536, 1024), (8192, 24576, 256), (70000, 32768, 256),
+                                 (9000, 131072, 64), (40, 131072, 40), (10, 24576, 10)):
+        assert need(rows, cols) <= 2 * partials * cols * 4 + 256, (rows, cols)
+        assert need(rows, cols) >= 2 * min(partials, rows // 2) * cols * 4, (rows, cols)
