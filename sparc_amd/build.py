@@ -96,12 +96,13 @@ def build(verbose: bool = False, extra: list[str] | None = None) -> str:
     with ThreadPoolExecutor(max_workers=min(len(jobs), os.cpu_count() or 4)) as pool:
         native = pool.submit(_compile_native, build_dir)
         objs = list(pool.map(lambda j: _compile(j, build_dir, extra), jobs))
-        native_obj = native.result()
-    tmp = LIB_PATH + ".tmp"
-    cmd = [_hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", tmp]
-    _run(cmd, "link failed")
-    os.replace(tmp, LIB_PATH)
-    _link_native(native_obj)
+        # the library does not need the binding: it is there for other callers where
+        # torch's headers or g++ are not
+        tmp = LIB_PATH + ".tmp"
+        cmd = [_hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", tmp]
+        _run(cmd, "link failed")
+        os.replace(tmp, LIB_PATH)
+        _link_native(native.result())
     if verbose:
         print(f"built {LIB_PATH} and {NATIVE_PATH}")
     return LIB_PATH
