@@ -28,11 +28,15 @@ from .stack import SPARCStack
 class SPARCLanguageModel(nn.Module):
     """Logits [B, T, vocab] of ids [B, T].  The embedding is scaled by
     sqrt(d_model) and its table is the output projection too; ``padding_idx``
-    takes no gradient from the lookup."""
+    takes no gradient from the lookup (negative counts from the end)."""
 
     def __init__(self, vocab: int, n_layers: int, d_model: int, n_states: int, padding_idx: int | None = None,
                  norm: str = "layer"):
         super().__init__()
+        if padding_idx is not None:
+            if not -vocab <= padding_idx < vocab:
+                raise ValueError(f"padding_idx {padding_idx} is outside the vocabulary of {vocab}")
+            padding_idx %= vocab  # the id itself: targets are compared with it
         self.weight = nn.Parameter(torch.randn(vocab, d_model) * d_model ** -0.5)
         self.scale = math.sqrt(d_model)
         self.padding_idx = padding_idx

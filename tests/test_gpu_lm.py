@@ -115,3 +115,18 @@ def test_norm_kinds():
         stack.SPARCStack(1, 16, 4, norm="batch")
     s = stack.SPARCStack(1, 16, 4)
     assert isinstance(s.norm, torch.nn.RMSNorm) and isinstance(s.blocks[0].norm, torch.nn.RMSNorm)
+
+
+def test_padding_counted_from_the_end():
+    """padding_idx=-1 is the last id, for the lookup and for the targets."""
+    print("[case] lm padding from the end", flush=True)
+    tokens = torch.randint(0, 20, (3, 12), generator=torch.Generator().manual_seed(4))
+    tokens[:, 8:] = 19
+    tokens = tokens.cuda()
+    results = []
+    for pad in (19, -1):
+        m = _model(20, 1, 16, 4, padding_idx=pad)
+        loss, norm = lm.train_step(m, torch.optim.SGD(m.parameters(), lr=0.0), tokens, max_norm=1.0)
+        results.append((float(loss), float(norm), [p.grad.clone() for p in m.parameters() if p.grad is not None]))
+    assert results[0][:2] == results[1][:2]
+    assert all(torch.equal(a, b) for a, b in zip(results[0][2], results[1][2]))

@@ -219,3 +219,11 @@ def test_layer_norm_workspace_holds_the_partial_rows():
                                  (9000, 131072, 64), (40, 131072, 40), (10, 24576, 10)):
         assert need(rows, cols) <= 2 * partials * cols * 4 + 256, (rows, cols)
         assert need(rows, cols) >= 2 * min(partials, rows // 2) * cols * 4, (rows, cols)
+
+
+def test_language_model_refuses_padding_outside_the_vocabulary():
+    from sparc_amd import lm
+    for bad in (7, -8):
+        with pytest.raises(ValueError, match="padding_idx"):
+            lm.SPARCLanguageModel(7, 1, 16, 4, padding_idx=bad)
+    assert lm.SPARCLanguageModel(7, 1, 16, 4, padding_idx=-7).padding_idx == 0
