@@ -64,7 +64,7 @@ def train_step(model: SPARCLanguageModel, optimizer: torch.optim.Optimizer, toke
     gradient norm before clipping), both on the device."""
     logits = model(tokens[:, :-1])
     ignore = -100 if model.padding_idx is None else model.padding_idx
-    loss = F.cross_entropy(logits.flatten(0, 1).float(), tokens[:, 1:].reshape(-1), ignore_index=ignore)
+    loss = F.cross_entropy(logits.flatten(0, 1).float(), tokens[:, 1:].reshape(-1).long(), ignore_index=ignore)
     optimizer.zero_grad(set_to_none=True)
     loss.backward()
     norm = clip_grad_norm_(model.parameters(), max_norm)

@@ -130,3 +130,13 @@ def test_padding_counted_from_the_end():
         results.append((float(loss), float(norm), [p.grad.clone() for p in m.parameters() if p.grad is not None]))
     assert results[0][:2] == results[1][:2]
     assert all(torch.equal(a, b) for a, b in zip(results[0][2], results[1][2]))
+
+
+def test_ids_of_32_bits_train():
+    print("[case] lm int32 ids", flush=True)
+    tokens = torch.randint(0, 20, (2, 9), generator=torch.Generator().manual_seed(4)).cuda()
+    losses = []
+    for ids in (tokens, tokens.int()):
+        m = _model(20, 1, 16, 4)
+        losses.append(float(lm.train_step(m, torch.optim.SGD(m.parameters(), lr=0.0), ids, max_norm=1.0)[0]))
+    assert losses[0] == losses[1]
