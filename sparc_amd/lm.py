@@ -85,17 +85,14 @@ def beam_search(model: SPARCLanguageModel, prompt: torch.Tensor, beams: int, ste
     logits = logits.repeat_interleave(beams, dim=0)
     scores = torch.full((B, beams), -math.inf, device=prompt.device)
     scores[:, 0] = 0.0  # one hypothesis so far
-    finished, ids = None, None
+    finished = None
+    ids = torch.empty(B, beams, 0, dtype=torch.int64, device=prompt.device)
     for k in range(steps):
         # the states are this loop's own, so they are reordered in place
         step = beam_search_step(logits.view(B, beams, V), scores, finished=finished, eos_id=eos_id, states=states,
                                 out_states=states)
         scores, finished, states = step.scores, step.finished, step.states
-        last = step.tokens[..., None]
-        if ids is None:
-            ids = last
-        else:
-            ids = torch.cat((ids.gather(1, step.parents[..., None].expand(-1, -1, k)), last), dim=-1)
+        ids = torch.cat((ids.gather(1, step.parents[..., None].expand(-1, -1, k)), step.tokens[..., None]), dim=-1)
         if k + 1 < steps:
             logits, states = model.step(step.tokens.reshape(-1), states)
     return ids, scores

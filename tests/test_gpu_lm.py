@@ -140,3 +140,12 @@ def test_ids_of_32_bits_train():
         m = _model(20, 1, 16, 4)
         losses.append(float(lm.train_step(m, torch.optim.SGD(m.parameters(), lr=0.0), ids, max_norm=1.0)[0]))
     assert losses[0] == losses[1]
+
+
+@pytest.mark.parametrize("beams", [1, 3])
+def test_beam_search_of_no_steps(beams):
+    print(f"[case] lm beam search of no steps, {beams} beams", flush=True)
+    m = _model(20, 1, 16, 4)
+    ids, scores = lm.beam_search(m, torch.ones(2, 3, dtype=torch.int64, device="cuda"), beams, 0)
+    assert ids.shape == (2, beams, 0) and ids.dtype == torch.int64 and ids.is_cuda
+    assert scores.tolist() == [[0.0] + [-math.inf] * (beams - 1)] * 2
