@@ -53,8 +53,10 @@ class SPARCLanguageModel(nn.Module):
         h, states = self.stack.prefill(self.embed(tokens))
         return F.linear(h[:, -1], self.weight), states
 
+    @torch.no_grad()
     def step(self, tokens: torch.Tensor, states):
-        """(logits [B, vocab], new states) after one more id each, [B]."""
+        """(logits [B, vocab], new states) after one more id each, [B]; no
+        gradient, like the mixers' steps."""
         h, states = self.stack.step(self.embed(tokens), states)
         return F.linear(h, self.weight), states
 

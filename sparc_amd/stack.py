@@ -134,8 +134,10 @@ class SPARCBlock(nn.Module):
         y, state = self.mixer(self.in_proj(apply_norm(self.norm, x)), return_cache=True)
         return x + self.out_proj(y), state
 
+    @torch.no_grad()
     def step(self, x: torch.Tensor, state):
-        """(output, new state) of one position [B, d_model]."""
+        """(output, new state) of one position [B, d_model]; no gradient, like the
+        mixer's step."""
         y, state = self.mixer.step(self.in_proj(apply_norm(self.norm, x)), state, None)
         return x + self.out_proj(y), state
 
@@ -162,8 +164,9 @@ class SPARCStack(nn.Module):
             states.append(state)
         return apply_norm(self.norm, x), states
 
+    @torch.no_grad()
     def step(self, x: torch.Tensor, states):
-        """(output, new states) of one position [B, d_model]."""
+        """(output, new states) of one position [B, d_model]; no gradient."""
         new = []
         for blk, state in zip(self.blocks, states):
             x, state = blk.step(x, state)

@@ -149,3 +149,18 @@ def test_beam_search_of_no_steps(beams):
     ids, scores = lm.beam_search(m, torch.ones(2, 3, dtype=torch.int64, device="cuda"), beams, 0)
     assert ids.shape == (2, beams, 0) and ids.dtype == torch.int64 and ids.is_cuda
     assert scores.tolist() == [[0.0] + [-math.inf] * (beams - 1)] * 2
+
+
+def test_steps_have_no_gradient():
+    """The mixers' step has none, so what is around them has none either: the
+    gradient of the projections alone would be a wrong one."""
+    print("[case] lm steps and gradients", flush=True)
+    m = _model(20, 2, 16, 4)
+    tokens = torch.ones(2, 3, dtype=torch.int64, device="cuda")
+    with torch.no_grad():
+        _, states = m.prefill(tokens)
+    x = torch.randn(2, 16, device="cuda", requires_grad=True)
+    logits, new = m.step(tokens[:, 0], states)
+    for out in (logits, m.stack.step(x, states)[0], m.stack.blocks[0].step(x, states[0])[0]):
+        assert not out.requires_grad
+    assert not any(p.requires_grad for s in new for p in s)
