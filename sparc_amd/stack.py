@@ -97,12 +97,22 @@ def _make_norm(kind: str, d_model: int, eps: float) -> nn.Module:
     raise ValueError(f"unknown norm {kind!r} (rms or layer)")
 
 
+def _is_observed(module: nn.Module) -> bool:
+    """Whether a call of the module does more than its forward (hooks, of its own
+    or of all modules)."""
+    m = nn.modules.module
+    return any((module._forward_hooks, module._forward_pre_hooks, module._backward_hooks, module._backward_pre_hooks,
+                m._global_forward_hooks, m._global_forward_pre_hooks, m._global_backward_hooks,
+                m._global_backward_pre_hooks))
+
+
 def apply_norm(norm: nn.Module, x: torch.Tensor) -> torch.Tensor:
     """``norm(x)`` through the library's kernels: ``layer_norm`` for an
     nn.LayerNorm over the last dimension on the GPU, ``rms_norm`` for an
-    nn.RMSNorm."""
+    nn.RMSNorm.  A layer norm with hooks, or of a class of its own, is called."""
     if isinstance(norm, nn.LayerNorm):
-        if x.is_cuda and x.dtype in (torch.float32, torch.bfloat16) and norm.normalized_shape == (x.shape[-1],):
+        if (type(norm) is nn.LayerNorm and not _is_observed(norm) and x.is_cuda
+                and x.dtype in (torch.float32, torch.bfloat16) and norm.normalized_shape == (x.shape[-1],)):
             return layer_norm(x, norm.weight, norm.bias, norm.eps)
         return norm(x)
     return rms_norm(norm, x)

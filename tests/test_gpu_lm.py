@@ -164,3 +164,33 @@ def test_steps_have_no_gradient():
     for out in (logits, m.stack.step(x, states)[0], m.stack.blocks[0].step(x, states[0])[0]):
         assert not out.requires_grad
     assert not any(p.requires_grad for s in new for p in s)
+
+
+@pytest.mark.parametrize("kind", ["forward", "pre", "backward", "global", "subclass"])
+def test_a_norm_is_called_with_its_hooks(kind):
+    print(f"[case] layer norm module hooks {kind}", flush=True)
+    seen = []
+    norm = torch.nn.LayerNorm(16).cuda()
+    x = torch.randn(3, 16, device="cuda", requires_grad=True)
+    handle = None
+    if kind == "forward":
+        handle = norm.register_forward_hook(lambda mod, args, y: y + 1.0)
+    elif kind == "pre":
+        handle = norm.register_forward_pre_hook(lambda mod, args: (args[0] * torch.arange(16.0, device="cuda"),))
+    elif kind == "backward":
+        handle = norm.register_full_backward_hook(lambda mod, gx, gy: seen.append(gy))
+    elif kind == "global":
+        handle = torch.nn.modules.module.register_module_forward_hook(lambda mod, args, y: y + 1.0)
+    else:
+        class Centred(torch.nn.LayerNorm):
+            def forward(self, x):
+                return x - x.mean(-1, keepdim=True)
+        norm = Centred(16).cuda()
+    try:
+        y, want = stack.apply_norm(norm, x), norm(x)
+        y.sum().backward()
+    finally:
+        if handle is not None:
+            handle.remove()
+    torch.testing.assert_close(y, want, rtol=1e-5, atol=1e-5)
+    assert len(seen) == (1 if kind == "backward" else 0)
