@@ -264,3 +264,28 @@ def test_step_with_states_and_streams():
             assert torch.equal(p.cpu(), L.reorder(q.cpu(), step.parents.cpu()))
     empty = sparc_amd.beam_search_step(x[:0], s[:0])
     assert empty.tokens.shape == (0, 4)
+
+
+@pytest.mark.parametrize("dtype,width", [(F32, 1028), (F32, 257), (BF16, 257)], ids=["16", "4", "2"])
+@pytest.mark.parametrize("K", [1, 3, 4, 7, 8, 13, 16, 32])
+def test_reorder_in_place_of_many_rows(K, dtype, width):
+    """More workgroups than the GPU runs at once, at each width of access."""
+    print(f"[case] reorder in place K={K} {dtype} {width}", flush=True)
+    g = torch.Generator().manual_seed(K)
+    B = 300
+    parents = torch.randint(0, K, (B, K), generator=g)
+    parents[0] = torch.arange(K)
+    parents[1] = torch.arange(K).flip(0)
+    states = [tuple(torch.randn(B * K, width, generator=g).to(dtype).cuda() for _ in range(2)) for _ in range(2)]
+    want = [tuple(L.reorder(p.cpu(), parents) for p in s) for s in states]
+    out = sparc_amd.reorder_states(states, parents.cuda(), out_states=states)
+    for a, b, s in zip(out, want, states):
+        for x, y, q in zip(a, b, s):
+            assert x.data_ptr() == q.data_ptr() and torch.equal(x.cpu(), y)
+    bad = parents.clone()
+    bad[5, K - 1], bad[7, 0] = K, -1
+    kept = states[0][0].clone()
+    sparc_amd.reorder_states(states, bad.cuda(), out_states=states)
+    ok = ((bad >= 0) & (bad < K)).reshape(-1)
+    rows = L.reorder(torch.arange(B * K), bad.clamp(0, K - 1))
+    assert torch.equal(states[0][0][ok.cuda()], kept[rows[ok].cuda()]) and states[0][0][~ok.cuda()].isnan().all()

@@ -157,3 +157,29 @@ def test_equal_calls_give_equal_bits():
     leaf = w.requires_grad_()
     grads = [torch.autograd.grad(sparc_amd.embedding(tokens, leaf), [leaf], dy)[0] for _ in range(3)]
     assert torch.equal(grads[0], grads[1]) and torch.equal(grads[0], grads[2])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("D", [1, 7, 64, 513, 1001, 2056])
+@pytest.mark.parametrize("n", [1, 5, 127, 128, 129])
+def test_few_positions(n, D, dtype):
+    """Rows of one and of several blocks of columns, whole vectors and not, with
+    every kind of id."""
+    _check(n, 90, D, dtype, "zipf", scale=math.sqrt(D), seed=n)
+    _check(n, 90, D, dtype, "same", pad=-1, ids=torch.int32, seed=n)
+    _check(n, 90, D, dtype, "same", pad=3, seed=n)
+    _check(n, 4099, D, dtype, "uniform", pad=11, ids=torch.int32, seed=n)
+    _check(n, 7, D, dtype, "runs", pad=2, seed=n)
+
+
+def test_few_positions_outside_the_table():
+    """And equal calls give equal bits."""
+    print("[case] embedding few positions", flush=True)
+    g = torch.Generator().manual_seed(6)
+    for dtype in (F32, BF16):
+        tokens = torch.randint(-3, 44, (100,), generator=g)
+        w, dy = torch.randn(40, 1001, generator=g).to(dtype), torch.randn(100, 1001, generator=g).to(dtype)
+        leaf = w.cuda().requires_grad_()
+        grads = [torch.autograd.grad(sparc_amd.embedding(tokens.cuda(), leaf), leaf, dy.cuda())[0] for _ in range(3)]
+        _close(grads[0], L.embedding_grad(tokens, 40, dy, 1.0), "dw")
+        assert torch.equal(grads[0], grads[1]) and torch.equal(grads[0], grads[2])

@@ -93,3 +93,37 @@ def test_second_differentiation_is_refused():
     ids = torch.zeros(3, dtype=torch.int64, device="cuda")
     with pytest.raises(RuntimeError, match="twice differentiable"):
         torch.autograd.grad(sparc_amd.embedding(ids, x).square().sum(), x, create_graph=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_embedding_of_few_ids_graph(dtype):
+    print(f"[case] embedding graph n=100 {dtype}", flush=True)
+
+    def make(seed):
+        g = _gen(seed)
+        return [torch.randint(0, 500, (100,), device="cuda", generator=g),
+                torch.randn(500, 700, device="cuda", generator=g).to(dtype).requires_grad_(),
+                torch.randn(100, 700, device="cuda", generator=g).to(dtype)]
+
+    def run(i):
+        y = sparc_amd.embedding(i[0], i[1], scale=2.0)
+        return [y.detach(), *torch.autograd.grad(y, [i[1]], i[2])]
+
+    _replays(make, run)
+
+
+def test_states_in_place_graph():
+    """The beam step with its states reordered in place, many rows and few."""
+    print("[case] states in place graph", flush=True)
+    for B, width in ((3, 333), (300, 1028)):
+        def make(seed):
+            g = _gen(seed)
+            r = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+            return [r(B, 4, 500), -r(B, 4).abs(), *[r(4 * B, width) for _ in range(4)]]
+
+        def run(i):
+            states = [(i[2], i[3]), (i[4], i[5])]
+            step = sparc_amd.beam_search_step(i[0], i[1], states=states, out_states=states)
+            return [step.tokens, step.parents, step.scores, *i[2:]]
+
+        _replays(make, run)

@@ -103,3 +103,21 @@ def test_beam_and_states_beyond_32_bits():
         assert torch.equal(out[r], plane[rows[r]])
     sparc_amd.reorder_states([plane], parents, out_states=[plane])
     assert torch.equal(out, plane)
+
+
+def test_few_ids_of_a_table_beyond_32_bits():
+    vocab, D, n = 300_001, 8_192, 100
+    print(f"[case] embedding {n} of {vocab} x {D}", flush=True)
+    w = torch.empty(vocab, D, dtype=BF16, device="cuda").normal_().requires_grad_()
+    tokens = torch.randint(0, vocab, (n,), generator=torch.Generator().manual_seed(3))
+    tokens[:5] = torch.tensor([0, vocab - 1, vocab - 1, 262_143, 262_144])
+    dy = torch.empty(n, D, dtype=BF16, device="cuda").normal_()
+    y = sparc_amd.embedding(tokens.cuda(), w)
+    dw, = torch.autograd.grad(y, [w], dy)
+    assert torch.equal(y, w.detach()[tokens.cuda()])
+    named = tokens.unique()
+    want = torch.zeros(len(named), D, dtype=torch.float64)
+    want.index_add_(0, torch.searchsorted(named, tokens), dy.cpu().double())
+    got = dw[named.cuda()].cpu().double()
+    assert ((got - want).abs() <= want.abs() * 2.0 ** -8 + 1e-6).all()
+    assert int((dw != 0).any(dim=1).sum()) == len(named)
