@@ -35,30 +35,11 @@ def _like(states, planes):
 def _check_out(planes, out):
     if len(out) != len(planes):
         raise ValueError(f"out_states has {len(out)} tensors for {len(planes)} states")
-    spans = []  # (first byte, end, whether it is written)
     for o, p in zip(out, planes):
         if o is not p:
             _lib.expect(o, p.shape, p.dtype, "out_states")
         if not o.is_contiguous() or o.is_conj() or o.is_neg():
             raise ValueError("out_states must be contiguous tensors, no views that conjugate or negate")
-        at, src, size = o.data_ptr(), p.data_ptr(), o.numel() * o.element_size()
-        if size:
-            spans.append((at, at + size, True))
-            if src != at:
-                spans.append((src, src + _reach(p), False))
-    spans.sort()
-    end, written_end = 0, 0
-    for first, last, written in spans:
-        if first < (end if written else written_end):
-            raise ValueError("a tensor of out_states overlaps another one, or another one of the states")
-        end = max(end, last)
-        if written:
-            written_end = max(written_end, last)
-
-
-def _reach(t):
-    """Bytes from a tensor's first value to behind its last."""
-    return (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
 
 
 def reorder_states(states: Sequence, parents: torch.Tensor, out_states: Sequence | None = None) -> list:

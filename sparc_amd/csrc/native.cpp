@@ -7,7 +7,9 @@
 // beside the launches.
 //
 // Every function checks what the kernels assume and returns None for arguments
-// that it does not take; the Python callers then say what is wrong with them.
+// that it does not take; the Python callers then say what is wrong with them.  What
+// torch would lose track of is refused here: tensors that require grad where there is
+// no backward, tangents, tracing, and memory that is shared with what is written.
 #include <algorithm>
 #include <map>
 #include <set>
@@ -451,7 +453,8 @@ optional<Tensors> reorder(const Tensors& planes, const Tensor& parents_in, const
       if (!beside(to[i], parents) || to[i].scalar_type() != planes[i].scalar_type() ||
           to[i].sizes() != planes[i].sizes() || !to[i].is_contiguous() || !is_literal(to[i]))
         return std::nullopt;
-    if (!apart(planes, to)) return std::nullopt;
+    if (!apart(planes, to))
+      throw pybind11::value_error("a tensor of out_states overlaps another one, or another one of the states");
     mark_written(to);
   } else if (alike) {
     to = fresh(planes.size(), planes[0]);
