@@ -584,10 +584,12 @@ sparc_status sparc_rms_norm_backward(int64_t rows, int64_t cols, int32_t io_dtyp
  * param_dtype (io_dtype, or F32 beside BF16 I/O), each NULL where there is
  * none; mean, rstd [rows] fp32, written where given (both or neither; the
  * backward needs them).  Per row, in fp32 arithmetic: mu = mean(x), rstd =
- * 1 / sqrt(mean((x - mu)^2) + eps), y = (x - mu) rstd weight + bias.  Pointers
- * are aligned to their values; 16-byte alignment (and cols a multiple of 16
- * bytes) takes the widest accesses.  No counterpart in the reference, which
- * ships the layer, not a network: torch.nn.LayerNorm's formula. */
+ * 1 / sqrt(mean((x - mu)^2) + eps), y = (x - mu) rstd weight + bias; the mean
+ * of a constant row is its value.  Pointers are aligned to their values:
+ * accesses are 16 bytes wide at any alignment, slower by up to a third where
+ * BF16 rows begin at odd multiples of two bytes.  No counterpart in the
+ * reference, which ships the layer, not a network: torch.nn.LayerNorm's
+ * formula. */
 sparc_status sparc_layer_norm_forward(int64_t rows, int64_t cols, int32_t io_dtype, int32_t param_dtype, const void* x,
                                       const void* weight, const void* bias, float eps, void* y, float* mean,
                                       float* rstd, sparc_stream_t stream);

@@ -118,12 +118,14 @@ __device__ __forceinline__ void finish_stats(float about, float diff, float squa
 }
 
 // The forward, a row per L lanes: one read and one write of each value, and bound
-// by them: 32768 x 768 bf16 22 us (50 MB read, 50 written: 4.6 TB/s), 8192 x 24576
-// 178 us (4.5 TB/s), 300000 x 64 16 us.  256 rows of 2048 take 3.5 us: the launch,
-// two reads one after the other and two sums over the row's lanes.  Rows that
-// begin at odd multiples of two bytes cost up to a third more (20000 bf16 rows of
-// 5000 columns 72 us, of 5001 93), since each access is split.  (kWhole in the
-// forward measured no faster than kLap.)
+// by them: 32768 x 768 bf16 20 us (50 MB read, 50 written: 5.0 TB/s), 300000 x 64
+// 16 us.  Where one workgroup fills a CU its arithmetic is not hidden: 8192 x 24576
+// 192 us at best (4.2 TB/s; 180 with a mean that is not taken about the first value,
+// smaller rows 1 to 4 % less).  256 rows of 2048 take 3.6 us: the launch, two reads
+// one after the other and two sums over the row's lanes.  Rows that begin at odd
+// multiples of two bytes cost up to a third more (20000 bf16 rows of 5000 columns 73
+// us, of 5001 94), since each access is split.  (kWhole in the forward measured no
+// faster than kLap.)
 template <typename IO, typename PT, int NCH, int L, int E>
 __global__ void __launch_bounds__(L <= 64 ? 64 * kRowWaves : L)
 layer_norm_fwd_kernel(int64_t R, int D, const void* x, const void* w, const void* b, float eps, void* y, float* mean,
@@ -382,8 +384,8 @@ layer_norm_bwd_kernel(int64_t R, int D, const void* x, const void* w, const floa
 }
 
 // Rows of any width, read again for each pass over them, mostly out of a cache:
-// 3172 x 40000 fp32 forward 306 us (1 GB: 3.3 TB/s); backward of 6009 x 16641 fp32
-// 289 us for dx and 153 for the sums over rows, which read x and dy once more.
+// 3172 x 40000 fp32 forward 302 us (1 GB: 3.4 TB/s); backward of 6009 x 16641 fp32
+// 291 us for dx and 157 for the sums over rows, which read x and dy once more.
 constexpr int kWideThreads = 1024;
 template <typename IO, typename PT>
 __global__ void __launch_bounds__(kWideThreads)
@@ -623,15 +625,6 @@ bool bwd_form(int64_t D, F&& f) {
 // a partial row costs as much as a row: 2 of these at least for each, and 8
 // behind the first 512 (944 x 2827 bf16 with the sum of the partial rows: 19
 // against 24 us, 4096 x 2880: 24 against 26).
-// How rows of other widths than whole vectors end: with vectors that lap (20000 x
-// 5004 bf16, fp32 parameters 141 us, short ones 201; 300000 x 68 33 and 40; 60000 x
-// 701 57 and 73), but for 4 vectors in each of 1024 lanes, which have no registers
-// left for it (3944 x 25353: 224 and 178).
-template <int NCH, int L>
-constexpr int bwd_ends() {
-  return NCH >= 4 && L == 1024 ? kShort : kLap;
-}
-
 template <int NCH, int L>
 int64_t bwd_groups(int64_t R) {
   const int64_t need = L <= 64 ? (R + kBwdRows<L> - 1) / kBwdRows<L> : (R + 1) / 2;
@@ -639,6 +632,14 @@ int64_t bwd_groups(int64_t R) {
   int64_t n = need < fill ? need : fill;
   if (L > 64 && n > 512) n = R / 8 > 512 ? (R / 8 < n ? R / 8 : n) : 512;
   return n;
+}
+// How rows of other widths than whole vectors end: with vectors that lap (20000 x
+// 5004 bf16, fp32 parameters 141 us, short ones 201; 300000 x 68 33 and 40; 60000 x
+// 701 57 and 73), but for 4 vectors in each of 1024 lanes, which have no registers
+// left for it (3944 x 25353: 224 and 178).
+template <int NCH, int L>
+constexpr int bwd_ends() {
+  return NCH >= 4 && L == 1024 ? kShort : kLap;
 }
 constexpr int64_t kWideSlices = 64;
 // The most partial rows that a backward of rows of D columns leaves
