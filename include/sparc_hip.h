@@ -673,6 +673,110 @@ sparc_status sparc_reorder_states(int64_t batch, int64_t beams, int64_t count, c
                                   void* const* dst, const int64_t* row_bytes, const int64_t* parents,
                                   sparc_stream_t stream);
 
+/* ---- Norms and rotation of queries and keys --------------------------------
+ * For each head of q [batch, length, q_heads, head_dim] and k [.., k_heads, ..]
+ * (io_dtype; strides in values, the last dimension's is 1; k_heads may be 0):
+ *   y = R (x rstd weight),   rstd = 1 / sqrt(mean(x^2) + eps)
+ * with weights [head_dim] in param_dtype (io_dtype, or F32 beside BF16; NULL:
+ * ones).  R turns the pairs of the first rotary_dim values (i and i + rotary_dim /
+ * 2, or with interleaved 2 i and 2 i + 1) by the angles whose cosines and sines
+ * are the row of table [table_rows, rotary_dim] fp32 (cosines, then sines) at the
+ * token's position: positions [batch, length] int64, or NULL: its index.  A
+ * position outside the table gives NaN.  yq, yk contiguous, in io_dtype;
+ * arithmetic in fp32, rounded once.  No counterpart in the reference. */
+typedef struct sparc_rotary_desc {
+  int64_t batch, length, q_heads, k_heads, head_dim, rotary_dim, table_rows;
+  int64_t q_stride[3], k_stride[3]; /* batch, time, head */
+  int32_t io_dtype, param_dtype, interleaved;
+  float eps;
+} sparc_rotary_desc;
+
+sparc_status sparc_qk_norm_rotary_forward(const sparc_rotary_desc* desc, const void* q, const void* k,
+                                          const void* q_weight, const void* k_weight, const float* table,
+                                          const int64_t* positions, void* yq, void* yk, sparc_stream_t stream);
+
+/* Workspace bytes of the backward (0: invalid desc). */
+size_t sparc_qk_norm_rotary_workspace_bytes(const sparc_rotary_desc* desc);
+
+/* The backward given dyq, dyk (contiguous, io_dtype): dq, dk (contiguous) and the
+ * weights' gradients [head_dim] in param_dtype, sums over all heads of a kind in a
+ * fixed order; each NULL where it is not wanted (without weights' gradients no
+ * workspace is needed). */
+sparc_status sparc_qk_norm_rotary_backward(const sparc_rotary_desc* desc, const void* q, const void* k,
+                                           const void* q_weight, const void* k_weight, const float* table,
+                                           const int64_t* positions, const void* dyq, const void* dyk, void* dq,
+                                           void* dk, void* dq_weight, void* dk_weight, void* workspace,
+                                           size_t workspace_bytes, sparc_stream_t stream);
+
+/* ---- Linear attention with a decay for each head ---------------------------
+ * Per batch row b and head h, with a = exp(log_decay[h]):
+ *   S_t = a S_(t-1) + k_t v_t^T  (key_dim x value_dim),   o_t = scale q_t S_t.
+ * q [batch, length, heads, key_dim], k [.., kv_heads, key_dim] and v [..,
+ * kv_heads, value_dim] in io_dtype, heads a multiple of kv_heads (query head h
+ * reads key head h / (heads / kv_heads)), with the strides given in values (the
+ * last dimension's is 1); o [batch, length, heads, value_dim] contiguous.
+ * log_decay [heads] fp32, at most 0 (-inf: no memory).  lengths [batch] int64 or
+ * NULL: the steps that a row has, cut to [0, length]; behind them k, v and q are
+ * not read, o is zero and the state stays.  state_in, state_out [batch, heads,
+ * key_dim, value_dim] fp32, contiguous; state_in NULL: zero, state_out NULL: not
+ * wanted.  key_dim and value_dim from 1 to 256.  Products are fp32 or bf16 matrix
+ * instructions with fp32 sums; where a state, a score or a decayed value enters a
+ * bf16 product it does so as a sum of two or three bf16 values.  Results are
+ * rounded once, and equal calls give equal bits.  No counterpart in the
+ * reference, whose states are vectors (one value per mode). */
+typedef struct sparc_linear_desc {
+  int64_t batch, length, heads, kv_heads, key_dim, value_dim;
+  int32_t io_dtype;
+  float scale;
+  int64_t q_stride[3], k_stride[3], v_stride[3]; /* batch, time, head */
+} sparc_linear_desc;
+
+/* Workspace bytes of the forward, or with backward != 0 of the backward (0 may be
+ * all that it needs; an invalid desc gives 0). */
+size_t sparc_linear_attention_workspace_bytes(const sparc_linear_desc* desc, int backward);
+sparc_status sparc_linear_attention_forward(const sparc_linear_desc* desc, const void* q, const void* k, const void* v,
+                                            const float* log_decay, const int64_t* lengths, const float* state_in,
+                                            void* o, float* state_out, void* workspace, size_t workspace_bytes,
+                                            sparc_stream_t stream);
+
+/* Gradients of q, k, v and (dstate_in not NULL) state_in, given do [batch, length,
+ * heads, value_dim] and (not NULL) dstate_out.  dq, dk, dv are contiguous, in
+ * io_dtype, zero behind a row's length; those of a shared head are sums over its
+ * query heads in a fixed order.  log_decay has no gradient. */
+sparc_status sparc_linear_attention_backward(const sparc_linear_desc* desc, const void* q, const void* k,
+                                             const void* v, const float* log_decay, const int64_t* lengths,
+                                             const float* state_in, const void* d_o, const float* dstate_out, void* dq,
+                                             void* dk, void* dv, float* dstate_in, void* workspace,
+                                             size_t workspace_bytes, sparc_stream_t stream);
+
+/* One step (desc->length is 1, the time strides are not used): o [batch, heads,
+ * value_dim] and the new state, which may be state_in itself. */
+sparc_status sparc_linear_attention_step(const sparc_linear_desc* desc, const void* q, const void* k, const void* v,
+                                         const float* log_decay, const float* state_in, void* o, float* state_out,
+                                         sparc_stream_t stream);
+
+/* ---- Gated linear unit ------------------------------------------------------
+ * y = act(x Wg^T) * (x Wu^T): x [rows, dim], gate and up weights [hidden, dim], y
+ * [rows, hidden], all contiguous, in io_dtype, aligned to their values.  activation:
+ * 0 x sigmoid(x), 1 x Phi(x) (the normal distribution's), 2 max(x, 0), 3 sigmoid(x).
+ * Products are matrix instructions with fp32 sums; the activation and the product
+ * with the other projection are fp32, rounded once.  No counterpart in the
+ * reference. */
+sparc_status sparc_gated_forward(int64_t rows, int64_t dim, int64_t hidden, int32_t io_dtype, int32_t activation,
+                                 const void* x, const void* gate_weight, const void* up_weight, void* y,
+                                 sparc_stream_t stream);
+
+/* Workspace bytes of the backward (0: invalid sizes, or none needed). */
+size_t sparc_gated_workspace_bytes(int64_t rows, int64_t dim, int64_t hidden, int32_t io_dtype);
+
+/* The backward given dy [rows, hidden]: dx (NULL: not wanted) and both weights'
+ * gradients (both or neither), overwritten.  The projections are computed again; the
+ * gradients of both are rounded to io_dtype once before the products with them. */
+sparc_status sparc_gated_backward(int64_t rows, int64_t dim, int64_t hidden, int32_t io_dtype, int32_t activation,
+                                  const void* x, const void* gate_weight, const void* up_weight, const void* dy,
+                                  void* dx, void* dgate_weight, void* dup_weight, void* workspace,
+                                  size_t workspace_bytes, sparc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -73,6 +73,16 @@ EXPORTED_SYMBOLS = (
     "sparc_beam_workspace_bytes",
     "sparc_beam_step",
     "sparc_reorder_states",
+    "sparc_qk_norm_rotary_forward",
+    "sparc_qk_norm_rotary_workspace_bytes",
+    "sparc_qk_norm_rotary_backward",
+    "sparc_linear_attention_workspace_bytes",
+    "sparc_linear_attention_forward",
+    "sparc_linear_attention_backward",
+    "sparc_linear_attention_step",
+    "sparc_gated_forward",
+    "sparc_gated_workspace_bytes",
+    "sparc_gated_backward",
     "sparc_last_error",
     "sparc_version",
 )
@@ -88,6 +98,28 @@ class ScanDesc(ctypes.Structure):
         ("io_dtype", ctypes.c_int32),
         ("gate_dtype", ctypes.c_int32),
         ("flags", ctypes.c_int32),
+    ]
+
+
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("batch", "length", "q_heads", "k_heads", "head_dim", "rotary_dim",
+                                              "table_rows")] + [
+        ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("io_dtype", ctypes.c_int32),
+        ("param_dtype", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+    ]
+
+
+class LinearDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("batch", "length", "heads", "kv_heads", "key_dim", "value_dim")] + [
+        ("io_dtype", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("v_stride", ctypes.c_int64 * 3),
     ]
 
 
@@ -209,6 +241,27 @@ def load() -> ctypes.CDLL:
         lib.sparc_beam_step.restype = ctypes.c_int
         lib.sparc_reorder_states.argtypes = [_I64, _I64, _I64, _P, _P, _P, _P, _P]
         lib.sparc_reorder_states.restype = ctypes.c_int
+        R, L = ctypes.POINTER(RotaryDesc), ctypes.POINTER(LinearDesc)
+        lib.sparc_qk_norm_rotary_forward.argtypes = [R] + [_P] * 9
+        lib.sparc_qk_norm_rotary_forward.restype = ctypes.c_int
+        lib.sparc_qk_norm_rotary_workspace_bytes.argtypes = [R]
+        lib.sparc_qk_norm_rotary_workspace_bytes.restype = _SZ
+        lib.sparc_qk_norm_rotary_backward.argtypes = [R] + [_P] * 13 + [_SZ, _P]
+        lib.sparc_qk_norm_rotary_backward.restype = ctypes.c_int
+        lib.sparc_linear_attention_workspace_bytes.argtypes = [L, ctypes.c_int]
+        lib.sparc_linear_attention_workspace_bytes.restype = _SZ
+        lib.sparc_linear_attention_forward.argtypes = [L] + [_P] * 9 + [_SZ, _P]
+        lib.sparc_linear_attention_forward.restype = ctypes.c_int
+        lib.sparc_linear_attention_backward.argtypes = [L] + [_P] * 13 + [_SZ, _P]
+        lib.sparc_linear_attention_backward.restype = ctypes.c_int
+        lib.sparc_linear_attention_step.argtypes = [L] + [_P] * 8
+        lib.sparc_linear_attention_step.restype = ctypes.c_int
+        lib.sparc_gated_forward.argtypes = [_I64] * 3 + [_I32] * 2 + [_P] * 5
+        lib.sparc_gated_forward.restype = ctypes.c_int
+        lib.sparc_gated_workspace_bytes.argtypes = [_I64] * 3 + [_I32]
+        lib.sparc_gated_workspace_bytes.restype = _SZ
+        lib.sparc_gated_backward.argtypes = [_I64] * 3 + [_I32] * 2 + [_P] * 8 + [_SZ, _P]
+        lib.sparc_gated_backward.restype = ctypes.c_int
         lib.sparc_last_error.argtypes = []
         lib.sparc_last_error.restype = ctypes.c_char_p
         lib.sparc_version.argtypes = []

@@ -21,7 +21,8 @@ INCLUDE = os.path.join(ROOT, "include")
 LIB_NAME = "libsparc_hip.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 SOURCES = ["scan.hip", "pointwise.hip", "mixer.hip", "norm.hip", "fold.hip", "layer_norm.hip", "embedding.hip",
-           "grad_norm.hip", "beam.hip"]
+           "grad_norm.hip", "beam.hip", "rotary.hip", "linear_attention.hip", "gated.hip"]
+NATIVE_SOURCES = ["native.cpp", "native_block.cpp"]
 NATIVE_PATH = os.path.join(HERE, "_native.so")
 # scan.hip compiles as SCAN_PARTS translation units (SPARC_SCAN_PART = 0..11:
 # the C ABI, then one per (transition, I/O dtype) launcher), in parallel
@@ -59,23 +60,28 @@ def _compile(job: tuple[str, int | None], build_dir: str, extra: list[str]) -> s
     return obj
 
 
-def _compile_native(build_dir: str) -> str:
+def _compile_native(build_dir: str) -> list[str]:
     from torch.utils import cpp_extension
     rocm = cpp_extension.ROCM_HOME or "/opt/rocm"
     includes = [INCLUDE, *cpp_extension.include_paths(), sysconfig.get_paths()["include"],
                 os.path.join(rocm, "include")]
-    obj = os.path.join(build_dir, "native.o")
-    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-          *(flag for path in includes for flag in ("-isystem", path)),
-          "-c", os.path.join(CSRC, "native.cpp"), "-o", obj], "g++ failed for native.cpp")
-    return obj
+
+    def compile_one(src):
+        obj = os.path.join(build_dir, os.path.splitext(src)[0] + ".o")
+        _run(["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-D__HIP_PLATFORM_AMD__=1",
+              "-DUSE_ROCM=1", *(flag for path in includes for flag in ("-isystem", path)),
+              "-c", os.path.join(CSRC, src), "-o", obj], f"g++ failed for {src}")
+        return obj
+
+    with ThreadPoolExecutor(max_workers=len(NATIVE_SOURCES)) as pool:
+        return list(pool.map(compile_one, NATIVE_SOURCES))
 
 
-def _link_native(obj: str) -> None:
+def _link_native(objs: list[str]) -> None:
     from torch.utils import cpp_extension
     libs = [flag for path in cpp_extension.library_paths() for flag in ("-L", path)]
     tmp = NATIVE_PATH + ".tmp"
-    _run(["g++", "-shared", obj, "-o", tmp, *libs, "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python",
+    _run(["g++", "-shared", *objs, "-o", tmp, *libs, "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python",
           "-L", HERE, f"-l:{LIB_NAME}", "-Wl,-rpath,$ORIGIN"], "linking the torch binding failed")
     os.replace(tmp, NATIVE_PATH)
 

@@ -1,0 +1,640 @@
+// Linear attention with a decay for each head (include/sparc_hip.h): the chunked form
+// over a sequence, its gradients, and the recurrent form for one step.
+//
+// With a chunk of C steps that enters with the state S (key_dim x value_dim):
+//   o_i  = a^(i+1) q_i S + sum over j <= i of a^(i-j) (q_i . k_j) v_j
+//   S'   = a^C S + sum over j of a^(C-1-j) k_j v_j^T
+// and the gradients are the same sums with other operands:
+//   dq   = the forward of (do, v, k) with the states transposed;
+//   dk   = the reversed sequence's of (v, do, q), dv that of (k, q, do), where the
+//          state R is the gradient of the state before a step: it enters a step
+//          undecayed (dS_t = R_(t+1) + q_t do_t^T) and leaves it decayed (R_t = a
+//          dS_t), so the powers are a^i and a^(C-j) in place of a^(i+1) and a^(C-1-j).
+// One kernel therefore does all four, and the backward is three problems of a launch.
+#include "matrix.h"
+
+namespace sparc {
+namespace {
+
+// ---------------------------------------------------------------------------
+// the chunked form
+// ---------------------------------------------------------------------------
+// Rows of one operand: strides in values, query heads that share one of its heads
+struct Rows {
+  const void* p;
+  int64_t sb, st, sh;
+  int group;
+};
+struct Problem {
+  Rows q, k, v;
+  void* o;              // [B, T, H, V] contiguous, in the I/O type or (o_f32) in fp32
+  const float* s_in;    // element (k, n) of chain c at c K V + k in_k + n in_n; NULL: zero
+  float* s_out;         // the same with out_k, out_n; NULL: not wanted
+  float* seg;           // [chains, segments, K, V]: what a segment adds, then what it enters with
+  int in_k, in_n, out_k, out_n;
+  int K, V, v_tiles;
+  int extra;            // 1: the state is decayed before a step, 0: after it
+  int reverse, o_f32;
+  float intra, inter, update;  // factors of the scores, of q S, of what is added to S
+};
+struct Problems {
+  Problem p[3];
+  const float* decay;      // log a, per head
+  const int64_t* lengths;  // NULL: T
+  int64_t T, seg_len;
+  int H, segments;
+  int blocks[3];           // workgroups of each problem
+};
+
+// a^n for l2 = log2 a (-inf: a is zero)
+__device__ __forceinline__ float power(float l2, int n) {
+  return n == 0 ? 1.0f : __builtin_amdgcn_exp2f(l2 * static_cast<float>(n));
+}
+// log2 a; a decay above 1 is not one: it is taken as no number
+__device__ __forceinline__ float log2_decay(const float* decay, int h) {
+  return decay[h] * 1.4426950408889634f;
+}
+__device__ __forceinline__ int64_t steps_of(const Problems& a, int64_t b) {
+  if (!a.lengths) return a.T;
+  const int64_t n = a.lengths[b];
+  return n < 0 ? 0 : n < a.T ? n : a.T;
+}
+
+// Values of each operand that a bf16 product takes: the state and the scores as two
+// bf16 values (2^-17 of their size), what is added to the state as three (2^-25), so
+// that the state keeps 24 bits over any number of chunks.
+template <typename IO> constexpr int kStateParts = sizeof(IO) == 2 ? 2 : 1;
+template <typename IO> constexpr int kScoreParts = sizeof(IO) == 2 ? 2 : 1;
+template <typename IO> constexpr int kAddedParts = sizeof(IO) == 2 ? 3 : 1;
+
+// Steps of a chunk, by the type and the padded key width
+template <typename IO, int KP> constexpr int kChunk = sizeof(IO) == 2 && KP < 256 ? 64 : 32;
+
+template <typename IO, int KP, int NV> struct Tiles {
+  static constexpr int C = kChunk<IO, KP>;
+  static constexpr int VT = 64 * NV;                   // value columns of a workgroup
+  static constexpr int KS = KP + 16 / sizeof(IO);      // row strides: 16 bytes more, so
+  static constexpr int VS = VT + 16 / sizeof(IO);      // that rows begin in other banks
+  static constexpr int PS = C + 16 / sizeof(IO);
+};
+
+// A workgroup of four waves: one chain (batch row and head), 64 NV value columns, one
+// segment of steps.  Each wave keeps the state of its 16 NV columns in registers.
+// OUT: with outputs; else only what the segment adds to the state.
+template <typename IO, int KP, int NV, bool OUT>
+__global__ __launch_bounds__(256, 2) void linear_kernel(const Problems a) {
+  using W = Tiles<IO, KP, NV>;
+  constexpr int C = W::C, KT = KP / 16, NT = C / 16, VEC = kVec<IO>;
+  constexpr int SP = kStateParts<IO>, PP = kScoreParts<IO>, AP = kAddedParts<IO>;
+  __shared__ __attribute__((aligned(16))) IO lq[OUT ? C * W::KS : 1];
+  __shared__ __attribute__((aligned(16))) IO lk[C * W::KS];
+  __shared__ __attribute__((aligned(16))) IO lv[C * W::VS];
+  __shared__ __attribute__((aligned(16))) IO lp[OUT ? PP : 1][OUT ? C * W::PS : 1];
+
+  int block = blockIdx.x, which = 0;
+  while (which < 2 && block >= a.blocks[which]) block -= a.blocks[which++];
+  const Problem& p = a.p[which];
+  block = xcd_swizzle(block, a.blocks[which]);
+  const int seg = block % a.segments, v_tile = block / a.segments % p.v_tiles;
+  const int chain = block / a.segments / p.v_tiles, h = chain % a.H;
+  const int64_t b = chain / a.H;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, quad = 4 * (lane >> 4);
+  const int64_t steps = steps_of(a, b), first = seg * a.seg_len;
+  const int64_t last = first + a.seg_len < a.T ? first + a.seg_len : a.T, end = last < steps ? last : steps;
+  const float l2 = log2_decay(a.decay, h);
+  const int v0 = v_tile * W::VT, w0 = wave * 16 * NV;  // first column of the workgroup, of the wave within it
+
+  const IO* gq = static_cast<const IO*>(p.q.p) + b * p.q.sb + (h / p.q.group) * p.q.sh;
+  const IO* gk = static_cast<const IO*>(p.k.p) + b * p.k.sb + (h / p.k.group) * p.k.sh;
+  const IO* gv = static_cast<const IO*>(p.v.p) + b * p.v.sb + (h / p.v.group) * p.v.sh;
+  const auto place = [&](int64_t t) { return p.reverse && t < steps ? steps - 1 - t : t; };
+
+  // the state: s[i][n] holds rows 16 i + quad + r of column v0 + w0 + 16 n + col
+  f32x4 s[KT][NV];
+  const int64_t state = static_cast<int64_t>(chain) * p.K * p.V;
+  const auto each_state = [&](auto&& f) {
+#pragma unroll
+    for (int i = 0; i < KT; ++i)
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = 16 * i + quad + r, c = v0 + w0 + 16 * n + col;
+          if (row < p.K && c < p.V) f(i, n, r, row, c);
+        }
+  };
+#pragma unroll
+  for (int i = 0; i < KT; ++i)
+#pragma unroll
+    for (int n = 0; n < NV; ++n) s[i][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  if constexpr (OUT) {
+    if (a.segments > 1) {
+      const float* from = p.seg + (static_cast<int64_t>(chain) * a.segments + seg) * p.K * p.V;
+      each_state([&](int i, int n, int r, int row, int c) { s[i][n][r] = from[row * p.V + c]; });
+    } else if (p.s_in) {
+      each_state([&](int i, int n, int r, int row, int c) { s[i][n][r] = p.s_in[state + row * p.in_k + c * p.in_n]; });
+    }
+  }
+
+  // vectors of a chunk, read while the chunk before it is worked on
+  constexpr int QN = C * KP / VEC / 256, VN = C * W::VT / VEC / 256;
+  static_assert(QN * 256 * VEC == C * KP && VN * 256 * VEC == C * W::VT, "whole vectors per thread");
+  Vec<IO> rq[OUT ? QN : 1], rk[QN], rv[VN];
+  const auto fetch = [&](int64_t t0) {
+    const auto rows = [&](const IO* base, int64_t st, int width, int from, int tile, Vec<IO>* r, auto count) {
+#pragma unroll
+      for (int i = 0; i < count; ++i) {
+        const int e = tid + 256 * i, row = e / (tile / VEC), c = from + e % (tile / VEC) * VEC;
+        const int64_t t = t0 + row;
+        r[i] = load_vec<IO>(base, place(t) * st + c, t < end ? width - c : 0);
+      }
+    };
+    if constexpr (OUT) rows(gq, p.q.st, p.K, 0, KP, rq, Int<QN>());
+    rows(gk, p.k.st, p.K, 0, KP, rk, Int<QN>());
+    rows(gv, p.v.st, p.V, v0, W::VT, rv, Int<VN>());
+  };
+  const auto put = [&] {
+    const auto rows = [&](IO* lds, int stride, int tile, const Vec<IO>* r, auto count) {
+#pragma unroll
+      for (int i = 0; i < count; ++i) {
+        const int e = tid + 256 * i;
+        *reinterpret_cast<Vec<IO>*>(lds + e / (tile / VEC) * stride + e % (tile / VEC) * VEC) = r[i];
+      }
+    };
+    if constexpr (OUT) rows(lq, W::KS, KP, rq, Int<QN>());
+    rows(lk, W::KS, KP, rk, Int<QN>());
+    rows(lv, W::VS, W::VT, rv, Int<VN>());
+  };
+  // four outputs of column tile n at step t
+  const auto emit = [&](int64_t t, int n, f32x4 x) {
+    const int c = v0 + w0 + 16 * n + quad;
+    const int64_t at = ((b * a.T + place(t)) * a.H + h) * p.V + c;
+    if (p.o_f32) store_quad(static_cast<float*>(p.o) + at, p.V - c, x);
+    else store_quad(static_cast<IO*>(p.o) + at, p.V - c, x);
+  };
+
+  if (first < end) fetch(first);
+  for (int64_t t0 = first; t0 < end; t0 += C) {
+    const int have = static_cast<int>(end - t0 < C ? end - t0 : C);
+    __syncthreads();  // the chunk before is no longer read
+    put();
+    __syncthreads();
+    if (t0 + C < end) fetch(t0 + C);
+
+    f32x4 acc[OUT ? NV : 1][OUT ? NT : 1];
+    if constexpr (OUT) {
+      // scores of 16 queries per wave: decayed, zero for later keys
+      const int qt = wave % NT;
+#pragma unroll
+      for (int step = 0; step < NT * NT / 4; ++step) {
+        const int kt = wave / NT + step * (4 / NT);
+        if (kt > (qt | 1)) continue;  // not read
+        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (kt <= qt) {
+#pragma unroll
+          for (int c = 0; c < KP; c += 32)
+            x = mma(read_rows(lk, W::KS, 16 * kt, c), read_rows(lq, W::KS, 16 * qt, c), x);
+        }
+        float y[8];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int n = 16 * (qt - kt) + col - quad - r;
+          y[r] = n < 0 ? 0.0f : x[r] * (p.intra * power(l2, n));
+          y[4 + r] = 0.0f;
+        }
+        Frag<IO> parts[PP];
+        split(y, parts);
+#pragma unroll
+        for (int n = 0; n < PP; ++n)
+          *reinterpret_cast<Quad<IO>*>(&lp[n][(16 * qt + col) * W::PS + 16 * kt + quad]) = parts[n].q[0];
+      }
+      // q S
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int i = 0; i < NT; ++i) acc[n][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < KT; c += 2) {
+        Frag<IO> sf[NV][SP];
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+          const float x[8] = {s[c][n][0],     s[c][n][1],     s[c][n][2],     s[c][n][3],
+                              s[c + 1][n][0], s[c + 1][n][1], s[c + 1][n][2], s[c + 1][n][3]};
+          split(x, sf[n]);
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          const Frag<IO> q = read_rows(lq, W::KS, 16 * i, 16 * c);
+#pragma unroll
+          for (int n = 0; n < NV; ++n)
+#pragma unroll
+            for (int m = SP - 1; m >= 0; --m) acc[n][i] = mma(sf[n][m], q, acc[n][i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const float f = p.inter * power(l2, 16 * i + col + p.extra);
+#pragma unroll
+        for (int n = 0; n < NV; ++n) acc[n][i] *= f;
+      }
+    }
+    const float whole = power(l2, have);
+#pragma unroll
+    for (int i = 0; i < KT; ++i)
+#pragma unroll
+      for (int n = 0; n < NV; ++n) s[i][n] *= whole;
+    if constexpr (OUT) __syncthreads();  // the scores are there
+#pragma unroll
+    for (int j = 0; j < C; j += 32) {
+      Frag<IO> vf[NV];
+#pragma unroll
+      for (int n = 0; n < NV; ++n) vf[n] = read_columns(lv, W::VS, j, w0 + 16 * n);
+      if constexpr (OUT) {
+        // a value that is not finite must not reach earlier steps of its block as 0 v
+        uint32_t odd = 0;
+#pragma unroll
+        for (int n = 0; n < NV; ++n) odd |= odd_bits(vf[n]);
+        const bool apart = __any(odd != 0);
+        if (apart) {
+#pragma unroll
+          for (int i = j / 16; i < j / 16 + 2; ++i)
+            for (int e = 0; e < 32; ++e) {
+              if (j + e > 16 * i + col) continue;
+              float x = 0.0f;
+#pragma unroll
+              for (int m = 0; m < PP; ++m) x += widen(lp[m][(16 * i + col) * W::PS + j + e]);
+#pragma unroll
+              for (int n = 0; n < NV; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  acc[n][i][r] = fmaf(x, widen(lv[(j + e) * W::VS + w0 + 16 * n + quad + r]), acc[n][i][r]);
+            }
+        }
+#pragma unroll
+        for (int i = j / 16; i < NT; ++i) {
+          if (apart && i < j / 16 + 2) continue;
+#pragma unroll
+          for (int m = PP - 1; m >= 0; --m) {
+            const Frag<IO> pf = read_rows(lp[m], W::PS, 16 * i, j);
+#pragma unroll
+            for (int n = 0; n < NV; ++n) acc[n][i] = mma(vf[n], pf, acc[n][i]);
+          }
+        }
+      }
+      // the state's share of these steps
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int n = have - p.extra - (j + 16 * (e / 4) + quad + e % 4);
+        f[e] = p.update * power(l2, n < 0 ? 0 : n);
+      }
+      Frag<IO> added[NV][AP];
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        float x[8];
+        widen(vf[n], x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] *= f[e];
+        split(x, added[n]);
+      }
+#pragma unroll
+      for (int i = 0; i < KT; ++i) {
+        const Frag<IO> kf = read_columns(lk, W::KS, j, 16 * i);
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+#pragma unroll
+          for (int m = AP - 1; m >= 0; --m) s[i][n] = mma(kf, added[n][m], s[i][n]);
+      }
+    }
+    if constexpr (OUT) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const int64_t t = t0 + 16 * i + col;
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+          if (t < end) emit(t, n, acc[n][i]);
+      }
+    }
+  }
+  if constexpr (OUT) {  // steps that a row does not have
+    for (int64_t t = (end > first ? end : first) + col; t < last; t += 16)
+#pragma unroll
+      for (int n = 0; n < NV; ++n) emit(t, n, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+    if (a.segments == 1 && p.s_out)
+      each_state([&](int i, int n, int r, int row, int c) { p.s_out[state + row * p.out_k + c * p.out_n] = s[i][n][r]; });
+  } else {
+    float* to = p.seg + (static_cast<int64_t>(chain) * a.segments + seg) * p.K * p.V;
+    each_state([&](int i, int n, int r, int row, int c) { to[row * p.V + c] = s[i][n][r]; });
+  }
+}
+
+// What each segment enters with, from what each adds; and the last state.  One thread
+// per value of a chain's state.
+__global__ __launch_bounds__(256) void linear_join_kernel(const Problems a, int which) {
+  const Problem& p = a.p[which];
+  const int size = p.K * p.V;
+  const int blocks = (size + 255) / 256;  // of a chain
+  const int64_t chain = blockIdx.x / blocks;
+  const int e = blockIdx.x % blocks * 256 + threadIdx.x;
+  if (e >= size) return;
+  const int row = e / p.V, c = e % p.V;
+  const int64_t steps = steps_of(a, chain / a.H);
+  const float l2 = log2_decay(a.decay, static_cast<int>(chain % a.H));
+  float s = p.s_in ? p.s_in[chain * size + row * p.in_k + c * p.in_n] : 0.0f;
+  float* seg = p.seg + chain * a.segments * size + e;
+  for (int n = 0; n < a.segments; ++n) {
+    const int64_t left = steps - n * a.seg_len;
+    const float f = power(l2, static_cast<int>(left < 0 ? 0 : left < a.seg_len ? left : a.seg_len));
+    const float add = seg[static_cast<int64_t>(n) * size];
+    seg[static_cast<int64_t>(n) * size] = s;
+    s = f * s + add;
+  }
+  if (p.s_out) p.s_out[chain * size + row * p.out_k + c * p.out_n] = s;
+}
+
+// Sums over the query heads of a shared head: [rows, G, m, D] fp32 to [rows, G, D]
+template <typename IO>
+__global__ __launch_bounds__(256) void linear_shared_kernel(const float* in, IO* out, int64_t total, int m, int D) {
+  for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < total;
+       e += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t head = e / D;
+    const float* p = in + head * m * D + (e - head * D);
+    float s = 0.0f;
+    for (int i = 0; i < m; ++i) s += p[static_cast<int64_t>(i) * D];
+    if constexpr (sizeof(IO) == 4) out[e] = s;
+    else out[e].bits = pack_bf16(s);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// one step
+// ---------------------------------------------------------------------------
+// A workgroup: one chain, 64 value columns; 16 lanes of four columns, 16 groups of rows.
+template <typename IO>
+__global__ __launch_bounds__(256) void linear_step_kernel(const Rows q, const Rows k, const Rows v, const float* decay,
+                                                          const float* s_in, float* s_out, void* o, int H, int K,
+                                                          int V, int v_tiles, float scale) {
+  __shared__ float lq[256], lk[256];
+  __shared__ f32x4 sums[16][17];
+  const int chain = blockIdx.x / v_tiles, h = chain % H;
+  const int64_t b = chain / H;
+  const int tid = threadIdx.x, lane = tid & 15, group = tid >> 4, c = blockIdx.x % v_tiles * 64 + 4 * lane;
+  if (tid < K) {
+    float x[1];
+    unpack<IO, 1>(load_raw<IO, 1>(q.p, b * q.sb + (h / q.group) * q.sh + tid), x);
+    lq[tid] = x[0] * scale;
+    unpack<IO, 1>(load_raw<IO, 1>(k.p, b * k.sb + (h / k.group) * k.sh + tid), x);
+    lk[tid] = x[0];
+  }
+  const float a = expf(decay[h]);
+  float x[4] = {};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (c + i < V) {
+      float y[1];
+      unpack<IO, 1>(load_raw<IO, 1>(v.p, b * v.sb + (h / v.group) * v.sh + c + i), y);
+      x[i] = y[0];
+    }
+  __syncthreads();
+  f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int row = group; row < K; row += 16) {
+    const int64_t at = (static_cast<int64_t>(chain) * K + row) * V + c;
+    float s[4];
+    unpack<float, 4>(load_vec<float>(s_in, at, V - c), s);
+    f32x4 n;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n[i] = fmaf(a, s[i], lk[row] * x[i]);
+    store_quad(s_out + at, V - c, n);
+    sum += lq[row] * n;
+  }
+  sums[group][lane] = sum;
+  __syncthreads();
+  if (group == 0) {
+    for (int i = 1; i < 16; ++i) sum += sums[i][lane];
+    store_quad(static_cast<IO*>(o) + static_cast<int64_t>(chain) * V + c, V - c, sum);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+const char* fault_of(const sparc_linear_desc* d) {
+  if (!d) return "linear attention: desc is NULL";
+  if (d->batch < 0 || d->length < 0) return "linear attention: batch and length must not be negative";
+  if (d->heads < 1 || d->kv_heads < 1 || d->heads % d->kv_heads) return "linear attention: heads must be a positive multiple of kv_heads";
+  if (d->key_dim < 1 || d->key_dim > 256 || d->value_dim < 1 || d->value_dim > 256)
+    return "linear attention: key_dim and value_dim must be from 1 to 256";
+  if (d->io_dtype != SPARC_F32 && d->io_dtype != SPARC_BF16) return "linear attention: io_dtype must be F32 or BF16";
+  // grids and chain numbers are 32-bit
+  if (d->heads > (1 << 20) || d->batch > (1 << 22) || d->batch * d->heads > (1 << 22) || d->length > (1LL << 31))
+    return "linear attention: too large";
+  return nullptr;
+}
+
+int padded(int64_t k) { return k <= 32 ? 32 : k <= 64 ? 64 : k <= 128 ? 128 : 256; }
+// column tiles of 16 per wave
+int tiles_per_wave(int64_t k, int64_t v) { return padded(k) < 256 && v > 64 ? 2 : 1; }
+
+struct Plan {
+  int segments;
+  int64_t seg_len;
+};
+// Time is cut into segments where the chains alone are too few workgroups.
+Plan plan_of(const sparc_linear_desc* d, int64_t k, int64_t v, int problems) {
+  const int64_t chunk = d->io_dtype == SPARC_BF16 && padded(k) < 256 ? 64 : 32;
+  const int64_t width = 64 * tiles_per_wave(k, v), groups = d->batch * d->heads * ((v + width - 1) / width) * problems;
+  const int64_t most = d->length / (4 * chunk);  // segments of four chunks at least
+  int64_t n = groups >= 384 || groups < 1 ? 1 : (1024 + groups - 1) / groups;
+  if (n > most) n = most;
+  if (n < 1) n = 1;
+  int64_t len = (d->length + n - 1) / n;
+  len = (len + chunk - 1) / chunk * chunk;
+  if (len < chunk) len = chunk;
+  n = d->length > 0 ? (d->length + len - 1) / len : 1;
+  return {static_cast<int>(n), len};
+}
+size_t segment_bytes(const sparc_linear_desc* d, const Plan& plan) {
+  return plan.segments > 1 ? up256(sizeof(float) * d->batch * d->heads * plan.segments * d->key_dim * d->value_dim) : 0;
+}
+
+template <typename IO, int KP, int NV> void launch(Problems& a, int n, int64_t chains, hipStream_t stream) {
+  int total = 0;
+  for (int i = 0; i < 3; ++i) a.blocks[i] = 0;
+  for (int i = 0; i < n; ++i) {
+    a.p[i].v_tiles = (a.p[i].V + 64 * NV - 1) / (64 * NV);
+    a.blocks[i] = static_cast<int>(chains * a.p[i].v_tiles * a.segments);
+    total += a.blocks[i];
+  }
+  if (total == 0) return;
+  if (a.segments > 1) {
+    linear_kernel<IO, KP, NV, false><<<total, 256, 0, stream>>>(a);
+    for (int i = 0; i < n; ++i)
+      linear_join_kernel<<<static_cast<unsigned>((a.p[i].K * a.p[i].V + 255) / 256 * chains), 256, 0, stream>>>(a, i);
+  }
+  linear_kernel<IO, KP, NV, true><<<total, 256, 0, stream>>>(a);
+}
+// All problems have the same padded widths
+template <typename IO> void launch_io(Problems& a, int n, int64_t chains, hipStream_t stream) {
+  const int k = padded(a.p[0].K), nv = tiles_per_wave(a.p[0].K, a.p[0].V);
+  if (k == 256) launch<IO, 256, 1>(a, n, chains, stream);
+  else if (k == 128) nv == 2 ? launch<IO, 128, 2>(a, n, chains, stream) : launch<IO, 128, 1>(a, n, chains, stream);
+  else if (k == 64) nv == 2 ? launch<IO, 64, 2>(a, n, chains, stream) : launch<IO, 64, 1>(a, n, chains, stream);
+  else nv == 2 ? launch<IO, 32, 2>(a, n, chains, stream) : launch<IO, 32, 1>(a, n, chains, stream);
+}
+void launch_all(int32_t io, Problems& a, int n, int64_t chains, hipStream_t stream) {
+  if (io == SPARC_BF16) launch_io<bf16>(a, n, chains, stream);
+  else launch_io<float>(a, n, chains, stream);
+}
+
+Rows rows_of(const void* p, const int64_t* stride, int64_t group) {
+  return {p, stride[0], stride[1], stride[2], static_cast<int>(group)};
+}
+// Whether the problems of the backward (dq with the two widths exchanged, dk too) fit one launch
+bool alike(const sparc_linear_desc* d) {
+  return padded(d->key_dim) == padded(d->value_dim) &&
+         tiles_per_wave(d->key_dim, d->value_dim) == tiles_per_wave(d->value_dim, d->key_dim);
+}
+struct BackwardPlan {
+  Plan qk, v;  // of dq and dk, of dv
+  size_t seg_qk, seg_v, shared_k, shared_v, total;
+};
+BackwardPlan backward_plan(const sparc_linear_desc* d) {
+  BackwardPlan r;
+  const bool one = alike(d);
+  r.qk = plan_of(d, d->value_dim, d->key_dim, one ? 3 : 2);
+  r.v = one ? r.qk : plan_of(d, d->key_dim, d->value_dim, 1);
+  r.seg_qk = segment_bytes(d, r.qk);
+  r.seg_v = segment_bytes(d, r.v);
+  const bool shared = d->heads > d->kv_heads;
+  const int64_t rows = d->batch * d->length * d->heads;
+  r.shared_k = shared ? up256(sizeof(float) * rows * d->key_dim) : 0;
+  r.shared_v = shared ? up256(sizeof(float) * rows * d->value_dim) : 0;
+  r.total = 2 * r.seg_qk + r.seg_v + r.shared_k + r.shared_v;
+  return r;
+}
+
+sparc_status check_desc(const sparc_linear_desc* d) {
+  const char* fault = fault_of(d);
+  return fault ? op_fail(SPARC_EINVAL, fault) : SPARC_OK;
+}
+
+}  // namespace
+}  // namespace sparc
+
+using namespace sparc;
+
+extern "C" {
+
+size_t sparc_linear_attention_workspace_bytes(const sparc_linear_desc* d, int backward) {
+  if (fault_of(d) || d->batch == 0) return 0;
+  if (backward) return backward_plan(d).total;
+  return segment_bytes(d, plan_of(d, d->key_dim, d->value_dim, 1));
+}
+
+sparc_status sparc_linear_attention_forward(const sparc_linear_desc* d, const void* q, const void* k, const void* v,
+                                            const float* log_decay, const int64_t* lengths, const float* state_in,
+                                            void* o, float* state_out, void* workspace, size_t workspace_bytes,
+                                            sparc_stream_t stream) {
+  if (const sparc_status s = check_desc(d)) return s;
+  if (d->batch == 0) return SPARC_OK;
+  if ((d->length > 0 && (!q || !k || !v || !o)) || !log_decay)
+    return op_fail(SPARC_EINVAL, "linear attention: a tensor is NULL");
+  const Plan plan = plan_of(d, d->key_dim, d->value_dim, 1);
+  if (workspace_bytes < segment_bytes(d, plan) || (plan.segments > 1 && !workspace))
+    return op_fail(SPARC_EWORKSPACE, "linear attention: workspace missing or too small");
+  const int K = static_cast<int>(d->key_dim), V = static_cast<int>(d->value_dim);
+  const int64_t group = d->heads / d->kv_heads;
+  Problems a = {};
+  a.p[0] = {rows_of(q, d->q_stride, 1), rows_of(k, d->k_stride, group), rows_of(v, d->v_stride, group), o, state_in,
+            state_out, static_cast<float*>(workspace), V, 1, V, 1, K, V, 0, 1, 0, 0, d->scale, d->scale, 1.0f};
+  a.decay = log_decay;
+  a.lengths = lengths;
+  a.T = d->length;
+  a.seg_len = plan.seg_len;
+  a.H = static_cast<int>(d->heads);
+  a.segments = plan.segments;
+  launch_all(d->io_dtype, a, 1, d->batch * d->heads, reinterpret_cast<hipStream_t>(stream));
+  return op_launched("sparc_linear_attention_forward");
+}
+
+sparc_status sparc_linear_attention_backward(const sparc_linear_desc* d, const void* q, const void* k, const void* v,
+                                             const float* log_decay, const int64_t* lengths, const float* state_in,
+                                             const void* d_o, const float* dstate_out, void* dq, void* dk, void* dv,
+                                             float* dstate_in, void* workspace, size_t workspace_bytes,
+                                             sparc_stream_t stream_) {
+  if (const sparc_status s = check_desc(d)) return s;
+  if (d->batch == 0) return SPARC_OK;
+  if ((d->length > 0 && (!q || !k || !v || !d_o || !dq || !dk || !dv)) || !log_decay)
+    return op_fail(SPARC_EINVAL, "linear attention: a tensor is NULL");
+  const BackwardPlan plan = backward_plan(d);
+  if (workspace_bytes < plan.total || (plan.total > 0 && !workspace))
+    return op_fail(SPARC_EWORKSPACE, "linear attention: workspace missing or too small");
+  const hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+  char* ws = static_cast<char*>(workspace);
+  float* const seg_q = reinterpret_cast<float*>(ws);
+  float* const seg_k = reinterpret_cast<float*>(ws + plan.seg_qk);
+  float* const seg_v = reinterpret_cast<float*>(ws + 2 * plan.seg_qk);
+  float* const all_k = reinterpret_cast<float*>(ws + 2 * plan.seg_qk + plan.seg_v);
+  float* const all_v = reinterpret_cast<float*>(ws + 2 * plan.seg_qk + plan.seg_v + plan.shared_k);
+  const int K = static_cast<int>(d->key_dim), V = static_cast<int>(d->value_dim);
+  const int64_t group = d->heads / d->kv_heads, H = d->heads, T = d->length, chains = d->batch * H;
+  const int64_t o_stride[3] = {T * H * V, H * V, V};
+  const Rows rq = rows_of(q, d->q_stride, 1), rk = rows_of(k, d->k_stride, group), rv = rows_of(v, d->v_stride, group);
+  const Rows ro = rows_of(d_o, o_stride, 1);
+  const int shared = group > 1;
+  Problems a = {};
+  // states of dq and dk are transposed: element (n, k) of the problem is (k, n) of the tensor
+  a.p[0] = {ro, rv, rk, dq, state_in, nullptr, seg_q, 1, V, 1, V, V, K, 0, 1, 0, 0, d->scale, d->scale, 1.0f};
+  a.p[1] = {rv, ro, rq, shared ? all_k : dk, dstate_out, nullptr, seg_k, 1, V, 1, V, V, K, 0, 0, 1, shared, d->scale, 1.0f, d->scale};
+  a.p[2] = {rk, rq, ro, shared ? all_v : dv, dstate_out, dstate_in, seg_v, V, 1, V, 1, K, V, 0, 0, 1, shared, d->scale, 1.0f, d->scale};
+  a.decay = log_decay;
+  a.lengths = lengths;
+  a.T = T;
+  a.H = static_cast<int>(H);
+  a.seg_len = plan.qk.seg_len;
+  a.segments = plan.qk.segments;
+  if (alike(d)) {
+    launch_all(d->io_dtype, a, 3, chains, stream);
+  } else {
+    launch_all(d->io_dtype, a, 2, chains, stream);
+    a.p[0] = a.p[2];
+    a.seg_len = plan.v.seg_len;
+    a.segments = plan.v.segments;
+    launch_all(d->io_dtype, a, 1, chains, stream);
+  }
+  if (shared && T > 0) {
+    const auto sum = [&](const float* in, void* out, int64_t D) {
+      const int64_t total = d->batch * T * d->kv_heads * D;
+      const unsigned grid = op_grid((total + 255) / 256);
+      const int m = static_cast<int>(group), n = static_cast<int>(D);
+      if (d->io_dtype == SPARC_BF16) linear_shared_kernel<<<grid, 256, 0, stream>>>(in, static_cast<bf16*>(out), total, m, n);
+      else linear_shared_kernel<<<grid, 256, 0, stream>>>(in, static_cast<float*>(out), total, m, n);
+    };
+    sum(all_k, dk, K);
+    sum(all_v, dv, V);
+  }
+  return op_launched("sparc_linear_attention_backward");
+}
+
+sparc_status sparc_linear_attention_step(const sparc_linear_desc* d, const void* q, const void* k, const void* v,
+                                         const float* log_decay, const float* state_in, void* o, float* state_out,
+                                         sparc_stream_t stream_) {
+  if (const sparc_status s = check_desc(d)) return s;
+  if (d->length != 1) return op_fail(SPARC_EINVAL, "linear attention: a step has length 1");
+  if (d->batch == 0) return SPARC_OK;
+  if (!q || !k || !v || !log_decay || !state_in || !o || !state_out)
+    return op_fail(SPARC_EINVAL, "linear attention: a tensor is NULL");
+  const hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+  const int64_t group = d->heads / d->kv_heads;
+  const Rows rq = rows_of(q, d->q_stride, 1), rk = rows_of(k, d->k_stride, group), rv = rows_of(v, d->v_stride, group);
+  const int H = static_cast<int>(d->heads), K = static_cast<int>(d->key_dim), V = static_cast<int>(d->value_dim);
+  const int v_tiles = (V + 63) / 64;
+  const unsigned grid = static_cast<unsigned>(d->batch * d->heads * v_tiles);
+  if (d->io_dtype == SPARC_BF16)
+    linear_step_kernel<bf16><<<grid, 256, 0, stream>>>(rq, rk, rv, log_decay, state_in, state_out, o, H, K, V, v_tiles, d->scale);
+  else
+    linear_step_kernel<float><<<grid, 256, 0, stream>>>(rq, rk, rv, log_decay, state_in, state_out, o, H, K, V, v_tiles, d->scale);
+  return op_launched("sparc_linear_attention_step");
+}
+
+}  // extern "C"

@@ -1,0 +1,358 @@
+// RMS norms of queries and keys for each head, and the rotation by their positions in
+// the same pass (include/sparc_hip.h):
+//   y = R(position) (x rstd w),   rstd = 1 / sqrt(mean(x^2) + eps)
+// and with g = R^T dy:  dx = rstd (g w - xhat mean(g w xhat)),  dw = sum of g xhat.
+//
+// Bound by memory: a head (a row) lives in registers of a few lanes, so forward and
+// backward read it once.  A lane holds both values of each pair that is rotated.
+#include "rows.h"
+
+namespace sparc {
+namespace {
+
+struct Side {  // queries or keys
+  const void* x;
+  int64_t sb, st, sh;  // strides in values
+  const void* w;       // NULL: ones
+  const void* dy;      // contiguous, like y and dx
+  void* out;           // y or dx
+  float* partial;      // [blocks, D]: sums of g xhat (NULL: not wanted)
+  int heads, blocks;
+  int64_t rows;
+};
+struct RotaryArgs {
+  Side side[2];
+  const float* table;        // [table_rows, R]: cosines, sines
+  const int64_t* positions;  // [B, T] or NULL: t
+  int64_t table_rows;
+  int T, D, R, lanes, params_f32;
+  float eps;
+};
+
+// W values at the alignment of one
+template <typename T, int W> __device__ __forceinline__ void load_few(const void* base, int64_t index, float (&o)[W]) {
+  struct __attribute__((packed, aligned(sizeof(T)))) Bits { T v[W]; };
+  const Bits bits = *reinterpret_cast<const Bits*>(static_cast<const T*>(base) + index);
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    if constexpr (sizeof(T) == 4) o[i] = bits.v[i];
+    else o[i] = bf16_bits_to_float(bits.v[i].bits);
+  }
+}
+template <typename T, int W> __device__ __forceinline__ void store_few(void* base, int64_t index, const float (&x)[W]) {
+  struct __attribute__((packed, aligned(sizeof(T)))) Bits { T v[W]; } bits;
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    if constexpr (sizeof(T) == 4) bits.v[i] = x[i];
+    else bits.v[i].bits = pack_bf16(x[i]);
+  }
+  *reinterpret_cast<Bits*>(static_cast<T*>(base) + index) = bits;
+}
+
+// A unit: W values and the W that they are paired with (for interleaved pairs the 2 W
+// values in a row).  Units of a lane, for heads of up to 512 values:
+template <int W> constexpr int kUnits = W >= 4 ? 1 : W == 2 ? 2 : 4;
+
+template <typename IO, int W, bool INTER, bool BACK>
+__global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
+  constexpr int U = kUnits<W>;
+  const bool keys = static_cast<int>(blockIdx.x) >= a.side[0].blocks;
+  const Side& s = a.side[keys];
+  const int block = blockIdx.x - (keys ? a.side[0].blocks : 0);
+  const int tid = threadIdx.x, lane = tid & (a.lanes - 1), group = tid / a.lanes, groups = 256 / a.lanes;
+  const int half = a.R / 2;
+  const float nan = __uint_as_float(0x7fc00000u);
+
+  // where a lane's units lie, and the weights there
+  int at[U][2];
+  bool turns[U], there[U], second[U];
+  float w[U][2 * W], sums[U][2 * W];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int first = (lane + u * a.lanes) * W;  // of the unit's pairs
+    there[u] = 2 * first < a.D;
+    turns[u] = first < half;
+    at[u][0] = !INTER && turns[u] ? first : 2 * first;
+    at[u][1] = !INTER && turns[u] ? half + first : 2 * first + W;
+    second[u] = there[u] && at[u][1] < a.D;  // a head of odd width ends with one value
+#pragma unroll
+    for (int i = 0; i < 2 * W; ++i) sums[u][i] = 0.0f, w[u][i] = 1.0f;
+    if (s.w) {
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+          if (m ? second[u] : there[u]) {
+            const int e = at[u][m] + i;
+            float y[1];
+            if (a.params_f32) load_few<float, 1>(s.w, e, y);
+            else load_few<IO, 1>(s.w, e, y);
+            w[u][m * W + i] = y[0];
+          }
+    }
+  }
+  // a unit's two halves from or to memory, in pairs: o[i] belongs to o[W + i]
+  const auto load = [&](const void* p, int64_t base, int u, float (&o)[2 * W]) {
+    float lo[W] = {}, hi[W] = {};
+    if (there[u]) load_few<IO, W>(p, base + at[u][0], lo);
+    if (second[u]) load_few<IO, W>(p, base + at[u][1], hi);
+#pragma unroll
+    for (int i = 0; i < W; ++i) o[i] = lo[i], o[W + i] = hi[i];
+  };
+  // INTER: values 2 i and 2 i + 1 are a pair
+  const auto first_of = [](int i) { return INTER ? 2 * i : i; };
+  const auto second_of = [](int i) { return INTER ? 2 * i + 1 : W + i; };
+
+  for (int64_t row = static_cast<int64_t>(block) * groups + group; row < s.rows;
+       row += static_cast<int64_t>(s.blocks) * groups) {
+    const uint32_t token = static_cast<uint32_t>(row) / static_cast<uint32_t>(s.heads);
+    const uint32_t head = static_cast<uint32_t>(row) - token * s.heads;
+    const uint32_t b = token / static_cast<uint32_t>(a.T), t = token - b * a.T;
+    const int64_t from = b * s.sb + t * s.st + head * s.sh, to = row * a.D;
+    const int64_t position = a.positions ? a.positions[token] : t;
+    const bool known = position >= 0 && position < a.table_rows;
+    float x[U][2 * W], g[U][2 * W], cs[U][W], sn[U][W];
+    float square = 0.0f;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      load(s.x, from, u, x[u]);
+      if constexpr (BACK) load(s.dy, to, u, g[u]);
+#pragma unroll
+      for (int i = 0; i < W; ++i) cs[u][i] = 1.0f, sn[u][i] = 0.0f;
+      if (turns[u] && known) {
+        const int64_t angle = position * a.R + (lane + u * a.lanes) * W;
+        load_few<float, W>(a.table, angle, cs[u]);
+        load_few<float, W>(a.table, angle + half, sn[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 2 * W; ++i) square = fmaf(x[u][i], x[u][i], square);
+    for (int m = 1; m < a.lanes; m *= 2) square += __shfl_xor(square, m);
+    const float rstd = known ? rsqrtf(square / static_cast<float>(a.D) + a.eps) : nan;
+    float along = 0.0f;
+    if constexpr (BACK) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          float &p = g[u][first_of(i)], &q = g[u][second_of(i)];
+          const float c = p * cs[u][i] + q * sn[u][i], d = q * cs[u][i] - p * sn[u][i];
+          p = c, q = d;
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * W; ++i) {
+          x[u][i] *= rstd;
+          sums[u][i] = fmaf(g[u][i], x[u][i], sums[u][i]);
+          g[u][i] *= w[u][i];
+          along = fmaf(g[u][i], x[u][i], along);
+        }
+      }
+      for (int m = 1; m < a.lanes; m *= 2) along += __shfl_xor(along, m);
+      along /= static_cast<float>(a.D);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float y[2 * W];
+      if constexpr (BACK) {
+#pragma unroll
+        for (int i = 0; i < 2 * W; ++i) y[i] = rstd * (g[u][i] - x[u][i] * along);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2 * W; ++i) y[i] = x[u][i] * rstd * w[u][i];
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          float &p = y[first_of(i)], &q = y[second_of(i)];
+          const float c = p * cs[u][i] - q * sn[u][i], d = q * cs[u][i] + p * sn[u][i];
+          p = c, q = d;
+        }
+      }
+      float lo[W], hi[W];
+#pragma unroll
+      for (int i = 0; i < W; ++i) lo[i] = y[i], hi[i] = y[W + i];
+      if (s.out && there[u]) store_few<IO, W>(s.out, to + at[u][0], lo);
+      if (s.out && second[u]) store_few<IO, W>(s.out, to + at[u][1], hi);
+    }
+  }
+  if constexpr (BACK) {
+    if (!s.partial) return;
+    __shared__ float part[256][2 * W * U + 1];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 2 * W; ++i) part[tid][u * 2 * W + i] = sums[u][i];
+    __syncthreads();
+    if (group == 0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < 2 * W; ++i) {
+          float sum = 0.0f;
+          for (int m = 0; m < groups; ++m) sum += part[m * a.lanes + lane][u * 2 * W + i];
+          if (i < W ? there[u] : second[u])
+            s.partial[static_cast<int64_t>(block) * a.D + (i < W ? at[u][0] + i : at[u][1] + i - W)] = sum;
+        }
+    }
+  }
+}
+
+// dw[c] = the sum of the workgroups' partial rows, in order
+struct RotarySums {
+  const float* in[2];
+  void* out[2];
+  int rows[2], D, f32;
+};
+__global__ __launch_bounds__(256) void rotary_sum_kernel(const RotarySums a) {
+  __shared__ float part[8][33];
+  const int which = blockIdx.y, c = blockIdx.x * 32 + (threadIdx.x & 31), group = threadIdx.x >> 5;
+  if (!a.out[which]) return;
+  float sum = 0.0f;
+  if (c < a.D)
+    for (int r = group; r < a.rows[which]; r += 8) sum += a.in[which][static_cast<int64_t>(r) * a.D + c];
+  part[group][threadIdx.x & 31] = sum;
+  __syncthreads();
+  if (group || c >= a.D) return;
+  for (int m = 1; m < 8; ++m) sum += part[m][threadIdx.x & 31];
+  if (a.f32) static_cast<float*>(a.out[which])[c] = sum;
+  else static_cast<bf16*>(a.out[which])[c].bits = pack_bf16(sum);
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+constexpr int kBackBlocks = 1024;
+
+const char* fault_of(const sparc_rotary_desc* d) {
+  if (!d) return "qk_norm_rotary: desc is NULL";
+  if (d->batch < 0 || d->length < 0 || d->q_heads < 1 || d->k_heads < 0)
+    return "qk_norm_rotary: batch and length must not be negative, q_heads must be positive";
+  if (d->head_dim < 1 || d->head_dim > 512) return "qk_norm_rotary: head_dim must be from 1 to 512";
+  if (d->rotary_dim < 0 || d->rotary_dim > d->head_dim || d->rotary_dim % 2)
+    return "qk_norm_rotary: rotary_dim must be even and at most head_dim";
+  if (d->table_rows < 0) return "qk_norm_rotary: table_rows must not be negative";
+  if (d->io_dtype != SPARC_F32 && d->io_dtype != SPARC_BF16) return "qk_norm_rotary: io_dtype must be F32 or BF16";
+  if (d->param_dtype != d->io_dtype && d->param_dtype != SPARC_F32)
+    return "qk_norm_rotary: parameters must be in io_dtype or F32";
+  if (!(d->eps >= 0.0f)) return "qk_norm_rotary: eps must be >= 0";
+  const int64_t most = 1LL << 31;
+  if (d->batch >= most || d->length >= most || d->q_heads >= most || d->k_heads >= most ||
+      (d->batch > 0 && d->length > 0 &&
+       (d->length >= most / d->batch || d->q_heads >= most / (d->batch * d->length) ||
+        d->k_heads >= most / (d->batch * d->length))))
+    return "qk_norm_rotary: too large";
+  return nullptr;
+}
+int width_of(const sparc_rotary_desc* d) {
+  for (int w = d->io_dtype == SPARC_BF16 ? 8 : 4; w > 1; w /= 2)
+    if (d->head_dim % (2 * w) == 0 && d->rotary_dim % (2 * w) == 0) return w;
+  return 1;
+}
+template <typename IO, int W, bool BACK> void rotary_launch(const RotaryArgs& a, bool inter, hipStream_t stream) {
+  const int grid = a.side[0].blocks + a.side[1].blocks;
+  if (inter) rotary_kernel<IO, W, true, BACK><<<grid, 256, 0, stream>>>(a);
+  else rotary_kernel<IO, W, false, BACK><<<grid, 256, 0, stream>>>(a);
+}
+template <bool BACK> void rotary_dispatch(const sparc_rotary_desc* d, RotaryArgs& a, hipStream_t stream) {
+  const int w = width_of(d);
+  const bool inter = d->interleaved != 0;
+  if (d->io_dtype == SPARC_BF16) {
+    if (w == 8) rotary_launch<bf16, 8, BACK>(a, inter, stream);
+    else if (w == 4) rotary_launch<bf16, 4, BACK>(a, inter, stream);
+    else if (w == 2) rotary_launch<bf16, 2, BACK>(a, inter, stream);
+    else rotary_launch<bf16, 1, BACK>(a, inter, stream);
+  } else {
+    if (w == 4) rotary_launch<float, 4, BACK>(a, inter, stream);
+    else if (w == 2) rotary_launch<float, 2, BACK>(a, inter, stream);
+    else rotary_launch<float, 1, BACK>(a, inter, stream);
+  }
+}
+// Everything but the sides' tensors; ``most``: workgroups at most
+RotaryArgs rotary_args(const sparc_rotary_desc* d, const float* table, const int64_t* positions, int64_t most) {
+  RotaryArgs a = {};
+  const int w = width_of(d);
+  const int64_t units = (d->head_dim + 2 * w - 1) / (2 * w);
+  a.lanes = 1;
+  while (a.lanes < 64 && a.lanes < units) a.lanes *= 2;
+  const int64_t tokens = d->batch * d->length, groups = 256 / a.lanes;
+  const int64_t heads[2] = {d->q_heads, d->k_heads}, all = tokens * (d->q_heads + d->k_heads);
+  for (int i = 0; i < 2; ++i) {
+    Side& s = a.side[i];
+    const int64_t* stride = i ? d->k_stride : d->q_stride;
+    s.sb = stride[0], s.st = stride[1], s.sh = stride[2];
+    s.heads = static_cast<int>(heads[i]);
+    s.rows = tokens * heads[i];
+    int64_t blocks = (s.rows + groups - 1) / groups;
+    const int64_t share = all ? (most * s.rows + all - 1) / all : 0;
+    if (blocks > share) blocks = share;
+    s.blocks = static_cast<int>(blocks);
+  }
+  a.table = table;
+  a.positions = positions;
+  a.table_rows = d->table_rows;
+  a.T = static_cast<int>(d->length);
+  a.D = static_cast<int>(d->head_dim);
+  a.R = static_cast<int>(d->rotary_dim);
+  a.params_f32 = d->param_dtype == SPARC_F32;
+  a.eps = d->eps;
+  return a;
+}
+
+}  // namespace
+}  // namespace sparc
+
+using namespace sparc;
+
+extern "C" {
+
+sparc_status sparc_qk_norm_rotary_forward(const sparc_rotary_desc* d, const void* q, const void* k,
+                                          const void* q_weight, const void* k_weight, const float* table,
+                                          const int64_t* positions, void* yq, void* yk, sparc_stream_t stream) {
+  if (const char* fault = fault_of(d)) return op_fail(SPARC_EINVAL, fault);
+  if (d->batch == 0 || d->length == 0) return SPARC_OK;
+  if (!q || !yq || (d->k_heads > 0 && (!k || !yk)) || (d->rotary_dim > 0 && d->table_rows > 0 && !table))
+    return op_fail(SPARC_EINVAL, "qk_norm_rotary: a tensor is NULL");
+  RotaryArgs a = rotary_args(d, table, positions, 1 << 16);
+  a.side[0].x = q, a.side[0].w = q_weight, a.side[0].out = yq;
+  a.side[1].x = k, a.side[1].w = k_weight, a.side[1].out = yk;
+  rotary_dispatch<false>(d, a, reinterpret_cast<hipStream_t>(stream));
+  return op_launched("sparc_qk_norm_rotary_forward");
+}
+
+size_t sparc_qk_norm_rotary_workspace_bytes(const sparc_rotary_desc* d) {
+  if (fault_of(d)) return 0;
+  return up256(sizeof(float) * (kBackBlocks + 2) * d->head_dim);
+}
+
+sparc_status sparc_qk_norm_rotary_backward(const sparc_rotary_desc* d, const void* q, const void* k,
+                                           const void* q_weight, const void* k_weight, const float* table,
+                                           const int64_t* positions, const void* dyq, const void* dyk, void* dq,
+                                           void* dk, void* dq_weight, void* dk_weight, void* workspace,
+                                           size_t workspace_bytes, sparc_stream_t stream_) {
+  if (const char* fault = fault_of(d)) return op_fail(SPARC_EINVAL, fault);
+  const hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+  const int64_t tokens = d->batch * d->length;
+  if (tokens > 0 && (!q || !dyq || (d->k_heads > 0 && (!k || !dyk)) || (d->rotary_dim > 0 && d->table_rows > 0 && !table)))
+    return op_fail(SPARC_EINVAL, "qk_norm_rotary: a tensor is NULL");
+  const bool sums = dq_weight || dk_weight;
+  if (sums && (!workspace || workspace_bytes < sparc_qk_norm_rotary_workspace_bytes(d)))
+    return op_fail(SPARC_EWORKSPACE, "qk_norm_rotary: workspace missing or too small");
+  RotaryArgs a = rotary_args(d, table, positions, kBackBlocks);
+  float* const partial = static_cast<float*>(workspace);
+  a.side[0].x = q, a.side[0].w = q_weight, a.side[0].dy = dyq, a.side[0].out = dq;
+  a.side[1].x = k, a.side[1].w = k_weight, a.side[1].dy = dyk, a.side[1].out = dk;
+  if (dq_weight) a.side[0].partial = partial;
+  if (dk_weight) a.side[1].partial = partial + static_cast<int64_t>(a.side[0].blocks) * d->head_dim;
+  if (tokens > 0) rotary_dispatch<true>(d, a, stream);
+  if (sums) {
+    const RotarySums r = {{partial, partial + static_cast<int64_t>(a.side[0].blocks) * d->head_dim},
+                          {dq_weight, dk_weight},
+                          {a.side[0].blocks, a.side[1].blocks},
+                          a.D,
+                          a.params_f32};
+    rotary_sum_kernel<<<dim3((a.D + 31) / 32, 2), 256, 0, stream>>>(r);
+  }
+  return op_launched("sparc_qk_norm_rotary_backward");
+}
+
+}  // extern "C"
