@@ -46,13 +46,12 @@ struct Problems {
   int blocks[3];           // workgroups of each problem
 };
 
-// a^n for l2 = log2 a (-inf: a is zero)
-__device__ __forceinline__ float power(float l2, int n) {
-  return n == 0 ? 1.0f : __builtin_amdgcn_exp2f(l2 * static_cast<float>(n));
-}
-// log2 a; a decay above 1 is not one: it is taken as no number
+// a^n for l2 = log2 a, n >= 0
+__device__ __forceinline__ float power(float l2, float n) { return __builtin_amdgcn_exp2f(l2 * n); }
+// log2 a.  Where a is zero a number so low that its powers are, but that of 0.
 __device__ __forceinline__ float log2_decay(const float* decay, int h) {
-  return decay[h] * 1.4426950408889634f;
+  const float d = decay[h] * 1.4426950408889634f;
+  return d < -1e30f ? -1e30f : d;
 }
 __device__ __forceinline__ int64_t steps_of(const Problems& a, int64_t b) {
   if (!a.lengths) return a.T;
@@ -70,21 +69,104 @@ template <typename IO> constexpr int kAddedParts = sizeof(IO) == 2 ? 3 : 1;
 // Steps of a chunk, by the type and the padded key width
 template <typename IO, int KP> constexpr int kChunk = sizeof(IO) == 2 && KP < 256 ? 64 : 32;
 
-template <typename IO, int KP, int NV> struct Tiles {
+// NW: waves, each with NV tiles of 16 value columns
+template <typename IO, int KP, int NW, int NV> struct Tiles {
   static constexpr int C = kChunk<IO, KP>;
-  static constexpr int VT = 64 * NV;                   // value columns of a workgroup
+  static constexpr int VT = 16 * NW * NV;              // value columns of a workgroup
   static constexpr int KS = KP + 16 / sizeof(IO);      // row strides: 16 bytes more, so
   static constexpr int VS = VT + 16 / sizeof(IO);      // that rows begin in other banks
   static constexpr int PS = C + 16 / sizeof(IO);
 };
 
-// A workgroup of four waves: one chain (batch row and head), 64 NV value columns, one
+// An offset that no buffer reaches: loads there give zero, stores are dropped.
+constexpr uint32_t kNowhere = 0x80000000u;
+
+// One operand's rows of a chunk on their way to LDS: TILE columns from ``from`` on of
+// rows of ``width`` values.  A thread reads 16-byte vectors of one column position
+// through a buffer that ends with the chunk's last row, so that nothing needs a
+// condition (a branch around a load makes the loads wait for one another): what lies
+// behind the last row or the last column is zero.  The vector that a row's end would
+// cut is read so that it ends with the row, and shifted.
+template <typename IO, int C, int TILE, int THREADS> struct Stage {
+  static constexpr int VEC = kVec<IO>, PER = TILE / VEC, SIZE = sizeof(IO);
+  static constexpr int STEP = THREADS / PER < C ? THREADS / PER : C, N = C / STEP;
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+  u4 r[N];
+  const IO* p;      // uniform: the chain's step 0
+  int64_t gap;      // values from a step's row to the next one's
+  uint32_t at;      // the thread's bytes in a row
+  int width, lack;  // columns that its vector lies further left than it should
+  bool down;        // steps go down in memory
+
+  static __device__ __forceinline__ int row() { return static_cast<int>(threadIdx.x) / PER; }
+  __device__ __forceinline__ void begin(const Rows& o, int64_t b, int h, int width_, int from, bool reverse,
+                                        int64_t steps) {
+    const int c = from + static_cast<int>(threadIdx.x) % PER * VEC;
+    width = width_;
+    const int left = c + VEC <= width ? c : width > VEC ? width - VEC : 0;
+    lack = c - left;
+    at = lack < VEC && row() < C ? static_cast<uint32_t>(left * SIZE) : kNowhere;
+    p = static_cast<const IO*>(o.p) + b * o.sb + (h / o.group) * o.sh + (reverse ? (steps - 1) * o.st : 0);
+    gap = o.st;
+    down = reverse;
+  }
+  // the rows of steps t0 .. t0 + have - 1
+  __device__ __forceinline__ void fetch(int64_t t0, int have) {
+    const IO* const low = down ? p - (t0 + have - 1) * gap : p + t0 * gap;
+    const auto buffer = make_rsrc(low, static_cast<uint32_t>(((have - 1) * gap + width) * SIZE));
+    const uint32_t bytes = static_cast<uint32_t>(gap) * SIZE;
+    const uint32_t first = at + bytes * static_cast<uint32_t>(down ? have - 1 - row() : row());
+    if (width < VEC) {  // value by value: a vector would end behind the last row
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint32_t on = bytes * static_cast<uint32_t>(i * STEP), to = down ? first - on : first + on;
+        r[i] = u4{0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          const uint32_t one = k < width ? to + k * SIZE : kNowhere;
+          if constexpr (SIZE == 4) r[i][k] = __builtin_amdgcn_raw_buffer_load_b32(buffer, one, 0, 0);
+          else r[i][k / 2] |= static_cast<uint32_t>(__builtin_amdgcn_raw_buffer_load_b16(buffer, one, 0, 0)) << (16 * (k % 2));
+        }
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t on = bytes * static_cast<uint32_t>(i * STEP);
+      r[i] = __builtin_amdgcn_raw_buffer_load_b128(buffer, down ? first - on : first + on, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void put(IO* lds, int stride) {
+    if (THREADS / PER > C && row() >= C) return;  // fewer vectors than threads
+    IO* const to = lds + row() * stride + static_cast<int>(threadIdx.x) % PER * VEC;
+    if (width % VEC) {
+      const int words = lack * SIZE / 4, odd = lack * SIZE % 4;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const u4 u = r[i];
+        uint32_t w[5];
+#pragma unroll
+        for (int k = 0; k < 5; ++k) {
+          w[k] = 0;
+#pragma unroll
+          for (int m = k; m < 4; ++m) w[k] = words == m - k ? u[m] : w[k];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r[i][k] = odd ? w[k] >> 16 | w[k + 1] << 16 : w[k];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) *reinterpret_cast<u4*>(to + i * STEP * stride) = r[i];
+  }
+};
+
+// A workgroup of NW waves: one chain (batch row and head), 16 NW NV value columns, one
 // segment of steps.  Each wave keeps the state of its 16 NV columns in registers.
 // OUT: with outputs; else only what the segment adds to the state.
-template <typename IO, int KP, int NV, bool OUT>
-__global__ __launch_bounds__(256, 2) void linear_kernel(const Problems a) {
-  using W = Tiles<IO, KP, NV>;
-  constexpr int C = W::C, KT = KP / 16, NT = C / 16, VEC = kVec<IO>;
+template <typename IO, int KP, int NW, int NV, bool OUT>
+__global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(const Problems a) {
+  using W = Tiles<IO, KP, NW, NV>;
+  constexpr int C = W::C, KT = KP / 16, NT = C / 16, THREADS = 64 * NW;
   constexpr int SP = kStateParts<IO>, PP = kScoreParts<IO>, AP = kAddedParts<IO>;
   __shared__ __attribute__((aligned(16))) IO lq[OUT ? C * W::KS : 1];
   __shared__ __attribute__((aligned(16))) IO lk[C * W::KS];
@@ -98,16 +180,12 @@ __global__ __launch_bounds__(256, 2) void linear_kernel(const Problems a) {
   const int seg = block % a.segments, v_tile = block / a.segments % p.v_tiles;
   const int chain = block / a.segments / p.v_tiles, h = chain % a.H;
   const int64_t b = chain / a.H;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, quad = 4 * (lane >> 4);
+  const int lane = threadIdx.x & 63, col = lane & 15, quad = 4 * (lane >> 4);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t steps = steps_of(a, b), first = seg * a.seg_len;
   const int64_t last = first + a.seg_len < a.T ? first + a.seg_len : a.T, end = last < steps ? last : steps;
   const float l2 = log2_decay(a.decay, h);
   const int v0 = v_tile * W::VT, w0 = wave * 16 * NV;  // first column of the workgroup, of the wave within it
-
-  const IO* gq = static_cast<const IO*>(p.q.p) + b * p.q.sb + (h / p.q.group) * p.q.sh;
-  const IO* gk = static_cast<const IO*>(p.k.p) + b * p.k.sb + (h / p.k.group) * p.k.sh;
-  const IO* gv = static_cast<const IO*>(p.v.p) + b * p.v.sb + (h / p.v.group) * p.v.sh;
-  const auto place = [&](int64_t t) { return p.reverse && t < steps ? steps - 1 - t : t; };
 
   // the state: s[i][n] holds rows 16 i + quad + r of column v0 + w0 + 16 n + col
   f32x4 s[KT][NV];
@@ -120,7 +198,7 @@ __global__ __launch_bounds__(256, 2) void linear_kernel(const Problems a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int row = 16 * i + quad + r, c = v0 + w0 + 16 * n + col;
-          if (row < p.K && c < p.V) f(i, n, r, row, c);
+          if (row < p.K && c < p.V) s[i][n][r] = f(s[i][n][r], row, c);
         }
   };
 #pragma unroll
@@ -130,65 +208,87 @@ __global__ __launch_bounds__(256, 2) void linear_kernel(const Problems a) {
   if constexpr (OUT) {
     if (a.segments > 1) {
       const float* from = p.seg + (static_cast<int64_t>(chain) * a.segments + seg) * p.K * p.V;
-      each_state([&](int i, int n, int r, int row, int c) { s[i][n][r] = from[row * p.V + c]; });
+      each_state([&](float, int row, int c) { return from[row * p.V + c]; });
     } else if (p.s_in) {
-      each_state([&](int i, int n, int r, int row, int c) { s[i][n][r] = p.s_in[state + row * p.in_k + c * p.in_n]; });
+      each_state([&](float, int row, int c) { return p.s_in[state + row * p.in_k + c * p.in_n]; });
     }
   }
 
-  // vectors of a chunk, read while the chunk before it is worked on
-  constexpr int QN = C * KP / VEC / 256, VN = C * W::VT / VEC / 256;
-  static_assert(QN * 256 * VEC == C * KP && VN * 256 * VEC == C * W::VT, "whole vectors per thread");
-  Vec<IO> rq[OUT ? QN : 1], rk[QN], rv[VN];
+  Stage<IO, C, KP, THREADS> sq, sk;
+  Stage<IO, C, W::VT, THREADS> sv;
+  const int64_t rows = steps < 1 ? 1 : steps;
+  if constexpr (OUT) sq.begin(p.q, b, h, p.K, 0, p.reverse, rows);
+  sk.begin(p.k, b, h, p.K, 0, p.reverse, rows);
+  sv.begin(p.v, b, h, p.V, v0, p.reverse, rows);
+  const auto have_at = [&](int64_t t0) { return static_cast<int>(end - t0 < C ? end - t0 : C); };
   const auto fetch = [&](int64_t t0) {
-    const auto rows = [&](const IO* base, int64_t st, int width, int from, int tile, Vec<IO>* r, auto count) {
+    const int have = have_at(t0);
+    if constexpr (OUT) sq.fetch(t0, have);
+    sk.fetch(t0, have);
+    sv.fetch(t0, have);
+  };
+  // outputs of columns c4 .. c4 + 3 of steps t0 + 16 i + col, ``count`` steps from t0 on
+  const int64_t o_gap = static_cast<int64_t>(a.H) * p.V;
+  const auto emit = [&](int64_t t0, int count, bool down, int c4, const auto& x, auto tiles) {
+    const int size = p.o_f32 ? 4 : sizeof(IO);
+    const int64_t low = down ? steps - t0 - count : t0;
+    const auto buffer = make_rsrc(static_cast<char*>(p.o) + ((b * a.T + low) * o_gap + h * p.V) * size,
+                                  static_cast<uint32_t>(((count - 1) * o_gap + p.V) * size));
+    const auto each = [&](auto&& store) {
 #pragma unroll
-      for (int i = 0; i < count; ++i) {
-        const int e = tid + 256 * i, row = e / (tile / VEC), c = from + e % (tile / VEC) * VEC;
-        const int64_t t = t0 + row;
-        r[i] = load_vec<IO>(base, place(t) * st + c, t < end ? width - c : 0);
+      for (int i = 0; i < tiles; ++i) {
+        const int k = 16 * i + col;
+        const uint32_t at = static_cast<uint32_t>((down ? count - 1 - k : k) * static_cast<int>(o_gap) + c4) * size;
+        store(x[i], k < count && c4 < p.V ? at : kNowhere);
       }
     };
-    if constexpr (OUT) rows(gq, p.q.st, p.K, 0, KP, rq, Int<QN>());
-    rows(gk, p.k.st, p.K, 0, KP, rk, Int<QN>());
-    rows(gv, p.v.st, p.V, v0, W::VT, rv, Int<VN>());
-  };
-  const auto put = [&] {
-    const auto rows = [&](IO* lds, int stride, int tile, const Vec<IO>* r, auto count) {
+    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+    if (p.V % 4) {
+      each([&](const f32x4& y, uint32_t to) {
 #pragma unroll
-      for (int i = 0; i < count; ++i) {
-        const int e = tid + 256 * i;
-        *reinterpret_cast<Vec<IO>*>(lds + e / (tile / VEC) * stride + e % (tile / VEC) * VEC) = r[i];
-      }
-    };
-    if constexpr (OUT) rows(lq, W::KS, KP, rq, Int<QN>());
-    rows(lk, W::KS, KP, rk, Int<QN>());
-    rows(lv, W::VS, W::VT, rv, Int<VN>());
+        for (int r = 0; r < 4; ++r) {
+          const uint32_t one = c4 + r < p.V ? to + r * size : kNowhere;
+          if (size == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(y[r]), buffer, one, 0, 0);
+          else __builtin_amdgcn_raw_buffer_store_b16(pack_bf16(y[r]), buffer, one, 0, 0);
+        }
+      });
+    } else if (size == 4) {
+      each([&](const f32x4& y, uint32_t to) {
+        const float f[4] = {y[0], y[1], y[2], y[3]};
+        buffer_store_f32<4, 0>(buffer, to, f);
+      });
+    } else {
+      each([&](const f32x4& y, uint32_t to) {
+        __builtin_amdgcn_raw_buffer_store_b64(u2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])}, buffer, to, 0, 0);
+      });
+    }
   };
-  // four outputs of column tile n at step t
-  const auto emit = [&](int64_t t, int n, f32x4 x) {
-    const int c = v0 + w0 + 16 * n + quad;
-    const int64_t at = ((b * a.T + place(t)) * a.H + h) * p.V + c;
-    if (p.o_f32) store_quad(static_cast<float*>(p.o) + at, p.V - c, x);
-    else store_quad(static_cast<IO*>(p.o) + at, p.V - c, x);
-  };
+  // powers of the decay: steps of a lane within a tile as fp32 numbers
+  const float ahead = static_cast<float>(col - quad), lane_col = static_cast<float>(col);
+  float leave[4];  // a^(15 - quad - r)
+#pragma unroll
+  for (int r = 0; r < 4; ++r) leave[r] = power(l2, static_cast<float>(15 - quad - r));
+  const float leave16 = power(l2, 16.0f);
+  constexpr int ST = NT * NT > NW ? NT * NT / NW : 1;  // score tiles of a wave
+  const int qt = wave % NT;
 
   if (first < end) fetch(first);
   for (int64_t t0 = first; t0 < end; t0 += C) {
-    const int have = static_cast<int>(end - t0 < C ? end - t0 : C);
+    const int have = have_at(t0);
     __syncthreads();  // the chunk before is no longer read
-    put();
+    if constexpr (OUT) sq.put(lq, W::KS);
+    sk.put(lk, W::KS);
+    sv.put(lv, W::VS);
     __syncthreads();
     if (t0 + C < end) fetch(t0 + C);
 
     f32x4 acc[OUT ? NV : 1][OUT ? NT : 1];
     if constexpr (OUT) {
-      // scores of 16 queries per wave: decayed, zero for later keys
-      const int qt = wave % NT;
+      // scores of 16 queries with some tiles of keys: decayed, zero for later keys
 #pragma unroll
-      for (int step = 0; step < NT * NT / 4; ++step) {
-        const int kt = wave / NT + step * (4 / NT);
-        if (kt > (qt | 1)) continue;  // not read
+      for (int m = 0; m < ST; ++m) {
+        const int kt = wave / NT + m * (NW > NT ? NW / NT : 1);
+        if (kt > (qt | 1)) continue;  // not read (and waves without a tile)
         f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
         if (kt <= qt) {
 #pragma unroll
@@ -198,8 +298,9 @@ __global__ __launch_bounds__(256, 2) void linear_kernel(const Problems a) {
         float y[8];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int n = 16 * (qt - kt) + col - quad - r;
-          y[r] = n < 0 ? 0.0f : x[r] * (p.intra * power(l2, n));
+          const float n = ahead + static_cast<float>(16 * (qt - kt) - r);
+          const float f = p.intra * power(l2, n < 0.0f ? 0.0f : n);
+          y[r] = n < 0.0f ? 0.0f : x[r] * f;
           y[4 + r] = 0.0f;
         }
         Frag<IO> parts[PP];
@@ -230,15 +331,16 @@ __global__ __launch_bounds__(256, 2) void linear_kernel(const Problems a) {
 #pragma unroll
             for (int m = SP - 1; m >= 0; --m) acc[n][i] = mma(sf[n][m], q, acc[n][i]);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        const float f = p.inter * power(l2, 16 * i + col + p.extra);
+        const float f = p.inter * power(l2, lane_col + static_cast<float>(16 * i + p.extra));
 #pragma unroll
         for (int n = 0; n < NV; ++n) acc[n][i] *= f;
       }
     }
-    const float whole = power(l2, have);
+    const float whole = power(l2, static_cast<float>(have));
 #pragma unroll
     for (int i = 0; i < KT; ++i)
 #pragma unroll
@@ -258,6 +360,7 @@ __global__ __launch_bounds__(256, 2) void linear_kernel(const Problems a) {
         if (apart) {
 #pragma unroll
           for (int i = j / 16; i < j / 16 + 2; ++i)
+#pragma unroll 1
             for (int e = 0; e < 32; ++e) {
               if (j + e > 16 * i + col) continue;
               float x = 0.0f;
@@ -283,10 +386,16 @@ __global__ __launch_bounds__(256, 2) void linear_kernel(const Problems a) {
       }
       // the state's share of these steps
       float f[8];
+      if (have == C) {
+        const float block = p.update * power(l2, static_cast<float>(C - 32 - j + 1 - p.extra));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int n = have - p.extra - (j + 16 * (e / 4) + quad + e % 4);
-        f[e] = p.update * power(l2, n < 0 ? 0 : n);
+        for (int e = 0; e < 8; ++e) f[e] = e < 4 ? leave[e % 4] * (block * leave16) : leave[e % 4] * block;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int n = have - p.extra - (j + 16 * (e / 4) + quad + e % 4);
+          f[e] = p.update * power(l2, static_cast<float>(n < 0 ? 0 : n));
+        }
       }
       Frag<IO> added[NV][AP];
 #pragma unroll
@@ -304,27 +413,25 @@ __global__ __launch_bounds__(256, 2) void linear_kernel(const Problems a) {
         for (int n = 0; n < NV; ++n)
 #pragma unroll
           for (int m = AP - 1; m >= 0; --m) s[i][n] = mma(kf, added[n][m], s[i][n]);
+        if (i % 2) __builtin_amdgcn_sched_barrier(0);
       }
     }
     if constexpr (OUT) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const int64_t t = t0 + 16 * i + col;
-#pragma unroll
-        for (int n = 0; n < NV; ++n)
-          if (t < end) emit(t, n, acc[n][i]);
-      }
+      for (int n = 0; n < NV; ++n) emit(t0, have, p.reverse, v0 + w0 + 16 * n + quad, acc[n], Int<NT>());
     }
   }
   if constexpr (OUT) {  // steps that a row does not have
-    for (int64_t t = (end > first ? end : first) + col; t < last; t += 16)
+    const f32x4 zero[1] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+    for (int64_t t = end > first ? end : first; t < last; t += 16)
 #pragma unroll
-      for (int n = 0; n < NV; ++n) emit(t, n, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+      for (int n = 0; n < NV; ++n)
+        emit(t, static_cast<int>(last - t < 16 ? last - t : 16), false, v0 + w0 + 16 * n + quad, zero, Int<1>());
     if (a.segments == 1 && p.s_out)
-      each_state([&](int i, int n, int r, int row, int c) { p.s_out[state + row * p.out_k + c * p.out_n] = s[i][n][r]; });
+      each_state([&](float x, int row, int c) { return p.s_out[state + row * p.out_k + c * p.out_n] = x; });
   } else {
     float* to = p.seg + (static_cast<int64_t>(chain) * a.segments + seg) * p.K * p.V;
-    each_state([&](int i, int n, int r, int row, int c) { to[row * p.V + c] = s[i][n][r]; });
+    each_state([&](float x, int row, int c) { return to[row * p.V + c] = x; });
   }
 }
 
@@ -344,7 +451,7 @@ __global__ __launch_bounds__(256) void linear_join_kernel(const Problems a, int 
   float* seg = p.seg + chain * a.segments * size + e;
   for (int n = 0; n < a.segments; ++n) {
     const int64_t left = steps - n * a.seg_len;
-    const float f = power(l2, static_cast<int>(left < 0 ? 0 : left < a.seg_len ? left : a.seg_len));
+    const float f = power(l2, static_cast<float>(left < 0 ? 0 : left < a.seg_len ? left : a.seg_len));
     const float add = seg[static_cast<int64_t>(n) * size];
     seg[static_cast<int64_t>(n) * size] = s;
     s = f * s + add;
@@ -425,15 +532,21 @@ const char* fault_of(const sparc_linear_desc* d) {
   if (d->key_dim < 1 || d->key_dim > 256 || d->value_dim < 1 || d->value_dim > 256)
     return "linear attention: key_dim and value_dim must be from 1 to 256";
   if (d->io_dtype != SPARC_F32 && d->io_dtype != SPARC_BF16) return "linear attention: io_dtype must be F32 or BF16";
+  // a chunk's rows lie one behind the other, within 2^31 bytes
+  const int64_t* const strides[3] = {d->q_stride, d->k_stride, d->v_stride};
+  for (int i = 0; i < 3; ++i)
+    if (d->length > 1 && (strides[i][1] < (i < 2 ? d->key_dim : d->value_dim) || strides[i][1] >= (1LL << 23)))
+      return "linear attention: time strides must be at least a row's values, and less than 2^23";
+  if (d->heads * (d->key_dim > d->value_dim ? d->key_dim : d->value_dim) >= (1LL << 23)) return "linear attention: too large";
   // grids and chain numbers are 32-bit
-  if (d->heads > (1 << 20) || d->batch > (1 << 22) || d->batch * d->heads > (1 << 22) || d->length > (1LL << 31))
+  if (d->batch > (1 << 22) || d->batch * d->heads > (1 << 22) || d->length > (1LL << 31))
     return "linear attention: too large";
   return nullptr;
 }
 
 int padded(int64_t k) { return k <= 32 ? 32 : k <= 64 ? 64 : k <= 128 ? 128 : 256; }
-// column tiles of 16 per wave
-int tiles_per_wave(int64_t k, int64_t v) { return padded(k) < 256 && v > 64 ? 2 : 1; }
+// value columns of a workgroup
+int columns_of(int64_t v) { return v > 64 ? 128 : 64; }
 
 struct Plan {
   int segments;
@@ -442,7 +555,7 @@ struct Plan {
 // Time is cut into segments where the chains alone are too few workgroups.
 Plan plan_of(const sparc_linear_desc* d, int64_t k, int64_t v, int problems) {
   const int64_t chunk = d->io_dtype == SPARC_BF16 && padded(k) < 256 ? 64 : 32;
-  const int64_t width = 64 * tiles_per_wave(k, v), groups = d->batch * d->heads * ((v + width - 1) / width) * problems;
+  const int64_t width = columns_of(v), groups = d->batch * d->heads * ((v + width - 1) / width) * problems;
   const int64_t most = d->length / (4 * chunk);  // segments of four chunks at least
   int64_t n = groups >= 384 || groups < 1 ? 1 : (1024 + groups - 1) / groups;
   if (n > most) n = most;
@@ -457,29 +570,37 @@ size_t segment_bytes(const sparc_linear_desc* d, const Plan& plan) {
   return plan.segments > 1 ? up256(sizeof(float) * d->batch * d->heads * plan.segments * d->key_dim * d->value_dim) : 0;
 }
 
-template <typename IO, int KP, int NV> void launch(Problems& a, int n, int64_t chains, hipStream_t stream) {
+template <typename IO, int KP, int NW, int NV> void launch(Problems& a, int n, int64_t chains, hipStream_t stream) {
+  constexpr int VT = Tiles<IO, KP, NW, NV>::VT;
   int total = 0;
   for (int i = 0; i < 3; ++i) a.blocks[i] = 0;
   for (int i = 0; i < n; ++i) {
-    a.p[i].v_tiles = (a.p[i].V + 64 * NV - 1) / (64 * NV);
+    a.p[i].v_tiles = (a.p[i].V + VT - 1) / VT;
     a.blocks[i] = static_cast<int>(chains * a.p[i].v_tiles * a.segments);
     total += a.blocks[i];
   }
   if (total == 0) return;
   if (a.segments > 1) {
-    linear_kernel<IO, KP, NV, false><<<total, 256, 0, stream>>>(a);
+    linear_kernel<IO, KP, NW, NV, false><<<total, 64 * NW, 0, stream>>>(a);
     for (int i = 0; i < n; ++i)
       linear_join_kernel<<<static_cast<unsigned>((a.p[i].K * a.p[i].V + 255) / 256 * chains), 256, 0, stream>>>(a, i);
   }
-  linear_kernel<IO, KP, NV, true><<<total, 256, 0, stream>>>(a);
+  linear_kernel<IO, KP, NW, NV, true><<<total, 64 * NW, 0, stream>>>(a);
 }
 // All problems have the same padded widths
 template <typename IO> void launch_io(Problems& a, int n, int64_t chains, hipStream_t stream) {
-  const int k = padded(a.p[0].K), nv = tiles_per_wave(a.p[0].K, a.p[0].V);
-  if (k == 256) launch<IO, 256, 1>(a, n, chains, stream);
-  else if (k == 128) nv == 2 ? launch<IO, 128, 2>(a, n, chains, stream) : launch<IO, 128, 1>(a, n, chains, stream);
-  else if (k == 64) nv == 2 ? launch<IO, 64, 2>(a, n, chains, stream) : launch<IO, 64, 1>(a, n, chains, stream);
-  else nv == 2 ? launch<IO, 32, 2>(a, n, chains, stream) : launch<IO, 32, 1>(a, n, chains, stream);
+  const int k = padded(a.p[0].K);
+  if (columns_of(a.p[0].V) == 64) {
+    if (k == 256) launch<IO, 256, 4, 1>(a, n, chains, stream);
+    else if (k == 128) launch<IO, 128, 4, 1>(a, n, chains, stream);
+    else if (k == 64) launch<IO, 64, 4, 1>(a, n, chains, stream);
+    else launch<IO, 32, 4, 1>(a, n, chains, stream);
+  } else {
+    if (k == 256) launch<IO, 256, 8, 1>(a, n, chains, stream);
+    else if (k == 128) launch<IO, 128, 4, 2>(a, n, chains, stream);
+    else if (k == 64) launch<IO, 64, 4, 2>(a, n, chains, stream);
+    else launch<IO, 32, 4, 2>(a, n, chains, stream);
+  }
 }
 void launch_all(int32_t io, Problems& a, int n, int64_t chains, hipStream_t stream) {
   if (io == SPARC_BF16) launch_io<bf16>(a, n, chains, stream);
@@ -492,7 +613,7 @@ Rows rows_of(const void* p, const int64_t* stride, int64_t group) {
 // Whether the problems of the backward (dq with the two widths exchanged, dk too) fit one launch
 bool alike(const sparc_linear_desc* d) {
   return padded(d->key_dim) == padded(d->value_dim) &&
-         tiles_per_wave(d->key_dim, d->value_dim) == tiles_per_wave(d->value_dim, d->key_dim);
+         columns_of(d->key_dim) == columns_of(d->value_dim);
 }
 struct BackwardPlan {
   Plan qk, v;  // of dq and dk, of dv

@@ -12,6 +12,11 @@ namespace {
 Tensor rows_of(const Tensor& t) {
   return is_literal(t) && (t.stride(-1) == 1 || t.size(-1) <= 1) ? t : contiguous(t);
 }
+// The same for sequences [B, T, H, D], where the rows of one head lie apart and not too far
+Tensor steps_of(const Tensor& t) {
+  const bool fits = t.size(1) <= 1 || (t.stride(1) >= t.size(3) && t.stride(1) < (1 << 23));
+  return fits ? rows_of(t) : t.clone(at::MemoryFormat::Contiguous);
+}
 void strides_of(const Tensor& t, int64_t (&stride)[3]) {  // [B, T, H, D]
   for (int i = 0; i < 3; ++i) stride[i] = t.stride(i);
 }
@@ -164,7 +169,7 @@ struct Linear : torch::autograd::Function<Linear> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
                                const optional<Tensor>& state, const Tensor& decay, const optional<Tensor>& lengths,
                                double scale) {
-    const LinearCall c = linear_call(rows_of(q), rows_of(k), rows_of(v), contiguous(decay), contiguous(state),
+    const LinearCall c = linear_call(steps_of(q), steps_of(k), steps_of(v), contiguous(decay), contiguous(state),
                                      contiguous(lengths), scale);
     ctx->save_for_backward({c.q, c.k, c.v, c.decay, c.state, c.lengths});
     ctx->saved_data["scale"] = scale;
@@ -233,7 +238,7 @@ optional<std::tuple<Tensor, Tensor>> linear_attention(const Tensor& q, const Ten
     const variable_list y = Linear::apply(q, k, v, state, decay, lengths, scale);
     return std::make_tuple(y[0], y[1]);
   }
-  return linear_forward(linear_call(rows_of(q), rows_of(k), rows_of(v), contiguous(decay), contiguous(state),
+  return linear_forward(linear_call(steps_of(q), steps_of(k), steps_of(v), contiguous(decay), contiguous(state),
                                     contiguous(lengths), scale));
 }
 
