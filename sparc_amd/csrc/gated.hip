@@ -60,12 +60,13 @@ constexpr int kTile = 128;
 
 template <typename IO, int KIND, bool PA, bool QA>
 __global__ __launch_bounds__(256, 2) void product_kernel(const ProductArgs a) {
-  constexpr int BK = 32, VEC = kVec<IO>, PAD = 16 / sizeof(IO);
+  constexpr int BK = 32, VEC = kVec<IO>;
   constexpr bool DUAL = KIND != PRODUCT;
   // [tile rows][BK], or ACROSS [BK][tile rows]
-  constexpr int PS = PA ? kTile + PAD : BK + PAD, QS = QA ? kTile + PAD : BK + PAD;
-  __shared__ __attribute__((aligned(16))) IO lp[PA ? BK * PS : kTile * PS];
-  __shared__ __attribute__((aligned(16))) IO lq[QA ? BK * QS : kTile * QS];
+  using LP = Panel<IO, PA ? kTile : BK, PA>;
+  using LQ = Panel<IO, QA ? kTile : BK, QA>;
+  __shared__ __attribute__((aligned(16))) IO lp[(PA ? BK : kTile) * LP::kStride];
+  __shared__ __attribute__((aligned(16))) IO lq[(QA ? BK : kTile) * LQ::kStride];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, quad = 4 * (lane >> 4);
   constexpr int PT = DUAL ? kTile / 2 : kTile;
   const int64_t p0 = static_cast<int64_t>(blockIdx.x) * PT, q0 = static_cast<int64_t>(blockIdx.y) * kTile;
@@ -93,12 +94,12 @@ __global__ __launch_bounds__(256, 2) void product_kernel(const ProductArgs a) {
       }
     }
   };
-  const auto put = [&](IO* lds, int stride, auto across, const Vec<IO>(&r)[N]) {
+  const auto put = [&](IO* lds, auto across, const Vec<IO>(&r)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int e = tid + 256 * i;
-      constexpr int per = (decltype(across)::value ? kTile : BK) / VEC;
-      *reinterpret_cast<Vec<IO>*>(lds + e / per * stride + e % per * VEC) = r[i];
+      constexpr int cols = decltype(across)::value ? kTile : BK, per = cols / VEC;
+      *reinterpret_cast<Vec<IO>*>(lds + Panel<IO, cols, decltype(across)::value>::at(e / per, e % per * VEC)) = r[i];
     }
   };
   using PAcross = std::integral_constant<bool, PA>;
@@ -117,17 +118,17 @@ __global__ __launch_bounds__(256, 2) void product_kernel(const ProductArgs a) {
   fetch_both(k0);
   for (int64_t k = k0; k < k1; k += BK) {
     __syncthreads();
-    put(lp, PS, PAcross(), rp);
-    put(lq, QS, QAcross(), rq);
+    put(lp, PAcross(), rp);
+    put(lq, QAcross(), rq);
     __syncthreads();
     if (k + BK < k1) fetch_both(k + BK);
     Frag<IO> fp[4], fq[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if constexpr (PA) fp[i] = read_columns(lp, PS, 0, wp + 16 * i);
-      else fp[i] = read_rows(lp, PS, wp + 16 * i, 0);
-      if constexpr (QA) fq[i] = read_columns(lq, QS, 0, wq + 16 * i);
-      else fq[i] = read_rows(lq, QS, wq + 16 * i, 0);
+      if constexpr (PA) fp[i] = read_columns<LP>(lp, 0, wp + 16 * i);
+      else fp[i] = read_rows<LP>(lp, wp + 16 * i, 0);
+      if constexpr (QA) fq[i] = read_columns<LQ>(lq, 0, wq + 16 * i);
+      else fq[i] = read_rows<LQ>(lq, wq + 16 * i, 0);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)

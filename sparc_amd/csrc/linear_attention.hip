@@ -73,9 +73,10 @@ template <typename IO, int KP> constexpr int kChunk = sizeof(IO) == 2 && KP < 25
 template <typename IO, int KP, int NW, int NV> struct Tiles {
   static constexpr int C = kChunk<IO, KP>;
   static constexpr int VT = 16 * NW * NV;              // value columns of a workgroup
-  static constexpr int KS = KP + 16 / sizeof(IO);      // row strides: 16 bytes more, so
-  static constexpr int VS = VT + 16 / sizeof(IO);      // that rows begin in other banks
-  static constexpr int PS = C + 16 / sizeof(IO);
+  using Q = Panel<IO, KP, false>;
+  using K = Panel<IO, KP, true>;
+  using V = Panel<IO, VT, true>;
+  using P = Panel<IO, C, false>;
 };
 
 // An offset that no buffer reaches: loads there give zero, stores are dropped.
@@ -136,9 +137,8 @@ template <typename IO, int C, int TILE, int THREADS> struct Stage {
       r[i] = __builtin_amdgcn_raw_buffer_load_b128(buffer, down ? first - on : first + on, 0, 0);
     }
   }
-  __device__ __forceinline__ void put(IO* lds, int stride) {
+  template <typename L> __device__ __forceinline__ void put(IO* lds) {
     if (THREADS / PER > C && row() >= C) return;  // fewer vectors than threads
-    IO* const to = lds + row() * stride + static_cast<int>(threadIdx.x) % PER * VEC;
     if (width % VEC) {
       const int words = lack * SIZE / 4, odd = lack * SIZE % 4;
 #pragma unroll
@@ -156,7 +156,8 @@ template <typename IO, int C, int TILE, int THREADS> struct Stage {
       }
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i) *reinterpret_cast<u4*>(to + i * STEP * stride) = r[i];
+    for (int i = 0; i < N; ++i)
+      *reinterpret_cast<u4*>(lds + L::at(row() + i * STEP, static_cast<int>(threadIdx.x) % PER * VEC)) = r[i];
   }
 };
 
@@ -168,10 +169,10 @@ __global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(
   using W = Tiles<IO, KP, NW, NV>;
   constexpr int C = W::C, KT = KP / 16, NT = C / 16, THREADS = 64 * NW;
   constexpr int SP = kStateParts<IO>, PP = kScoreParts<IO>, AP = kAddedParts<IO>;
-  __shared__ __attribute__((aligned(16))) IO lq[OUT ? C * W::KS : 1];
-  __shared__ __attribute__((aligned(16))) IO lk[C * W::KS];
-  __shared__ __attribute__((aligned(16))) IO lv[C * W::VS];
-  __shared__ __attribute__((aligned(16))) IO lp[OUT ? PP : 1][OUT ? C * W::PS : 1];
+  __shared__ __attribute__((aligned(16))) IO lq[OUT ? C * W::Q::kStride : 1];
+  __shared__ __attribute__((aligned(16))) IO lk[C * W::K::kStride];
+  __shared__ __attribute__((aligned(16))) IO lv[C * W::V::kStride];
+  __shared__ __attribute__((aligned(16))) IO lp[OUT ? PP : 1][OUT ? C * W::P::kStride : 1];
 
   int block = blockIdx.x, which = 0;
   while (which < 2 && block >= a.blocks[which]) block -= a.blocks[which++];
@@ -187,7 +188,7 @@ __global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(
   const float l2 = log2_decay(a.decay, h);
   const int v0 = v_tile * W::VT, w0 = wave * 16 * NV;  // first column of the workgroup, of the wave within it
 
-  // the state: s[i][n] holds rows 16 i + quad + r of column v0 + w0 + 16 n + col
+  // the state: s[i][n] holds rows tile_row(i, quad, r) of column v0 + w0 + 16 n + col
   f32x4 s[KT][NV];
   const int64_t state = static_cast<int64_t>(chain) * p.K * p.V;
   const auto each_state = [&](auto&& f) {
@@ -197,7 +198,7 @@ __global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(
       for (int n = 0; n < NV; ++n)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int row = 16 * i + quad + r, c = v0 + w0 + 16 * n + col;
+          const int row = tile_row<IO>(i, quad, r), c = v0 + w0 + 16 * n + col;
           if (row < p.K && c < p.V) s[i][n][r] = f(s[i][n][r], row, c);
         }
   };
@@ -265,10 +266,11 @@ __global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(
   };
   // powers of the decay: steps of a lane within a tile as fp32 numbers
   const float ahead = static_cast<float>(col - quad), lane_col = static_cast<float>(col);
-  float leave[4];  // a^(15 - quad - r)
+  constexpr int kHalf = sizeof(IO) == 2 ? 4 : 16;  // from a fragment's first four steps to the others
+  float leave[4];  // a^(31 - step) of those
 #pragma unroll
-  for (int r = 0; r < 4; ++r) leave[r] = power(l2, static_cast<float>(15 - quad - r));
-  const float leave16 = power(l2, 16.0f);
+  for (int r = 0; r < 4; ++r) leave[r] = power(l2, static_cast<float>(31 - step_of<IO>(quad, 4 + r)));
+  const float leave_half = power(l2, static_cast<float>(kHalf));
   constexpr int ST = NT * NT > NW ? NT * NT / NW : 1;  // score tiles of a wave
   const int qt = wave % NT;
 
@@ -276,9 +278,9 @@ __global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(
   for (int64_t t0 = first; t0 < end; t0 += C) {
     const int have = have_at(t0);
     __syncthreads();  // the chunk before is no longer read
-    if constexpr (OUT) sq.put(lq, W::KS);
-    sk.put(lk, W::KS);
-    sv.put(lv, W::VS);
+    if constexpr (OUT) sq.template put<typename W::Q>(lq);
+    sk.template put<typename W::K>(lk);
+    sv.template put<typename W::V>(lv);
     __syncthreads();
     if (t0 + C < end) fetch(t0 + C);
 
@@ -293,7 +295,7 @@ __global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(
         if (kt <= qt) {
 #pragma unroll
           for (int c = 0; c < KP; c += 32)
-            x = mma(read_rows(lk, W::KS, 16 * kt, c), read_rows(lq, W::KS, 16 * qt, c), x);
+            x = mma(read_rows<typename W::K>(lk, 16 * kt, c), read_rows<typename W::Q>(lq, 16 * qt, c), x);
         }
         float y[8];
 #pragma unroll
@@ -307,7 +309,7 @@ __global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(
         split(y, parts);
 #pragma unroll
         for (int n = 0; n < PP; ++n)
-          *reinterpret_cast<Quad<IO>*>(&lp[n][(16 * qt + col) * W::PS + 16 * kt + quad]) = parts[n].q[0];
+          *reinterpret_cast<Quad<IO>*>(&lp[n][W::P::at(16 * qt + col, 16 * kt + quad)]) = parts[n].q[0];
       }
       // q S
 #pragma unroll
@@ -325,13 +327,12 @@ __global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(
         }
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          const Frag<IO> q = read_rows(lq, W::KS, 16 * i, 16 * c);
+          const Frag<IO> q = read_rows<typename W::Q>(lq, 16 * i, 16 * c);
 #pragma unroll
-          for (int n = 0; n < NV; ++n)
+          for (int m = SP - 1; m >= 0; --m)
 #pragma unroll
-            for (int m = SP - 1; m >= 0; --m) acc[n][i] = mma(sf[n][m], q, acc[n][i]);
+            for (int n = 0; n < NV; ++n) acc[n][i] = mma(sf[n][m], q, acc[n][i]);
         }
-        __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
@@ -350,7 +351,7 @@ __global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(
     for (int j = 0; j < C; j += 32) {
       Frag<IO> vf[NV];
 #pragma unroll
-      for (int n = 0; n < NV; ++n) vf[n] = read_columns(lv, W::VS, j, w0 + 16 * n);
+      for (int n = 0; n < NV; ++n) vf[n] = read_columns<typename W::V>(lv, j, w0 + 16 * n);
       if constexpr (OUT) {
         // a value that is not finite must not reach earlier steps of its block as 0 v
         uint32_t odd = 0;
@@ -365,12 +366,12 @@ __global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(
               if (j + e > 16 * i + col) continue;
               float x = 0.0f;
 #pragma unroll
-              for (int m = 0; m < PP; ++m) x += widen(lp[m][(16 * i + col) * W::PS + j + e]);
+              for (int m = 0; m < PP; ++m) x += widen(lp[m][W::P::at(16 * i + col, j + e)]);
 #pragma unroll
               for (int n = 0; n < NV; ++n)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                  acc[n][i][r] = fmaf(x, widen(lv[(j + e) * W::VS + w0 + 16 * n + quad + r]), acc[n][i][r]);
+                  acc[n][i][r] = fmaf(x, widen(lv[W::V::at(j + e, w0 + 16 * n + quad + r)]), acc[n][i][r]);
             }
         }
 #pragma unroll
@@ -378,7 +379,7 @@ __global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(
           if (apart && i < j / 16 + 2) continue;
 #pragma unroll
           for (int m = PP - 1; m >= 0; --m) {
-            const Frag<IO> pf = read_rows(lp[m], W::PS, 16 * i, j);
+            const Frag<IO> pf = read_rows<typename W::P>(lp[m], 16 * i, j);
 #pragma unroll
             for (int n = 0; n < NV; ++n) acc[n][i] = mma(vf[n], pf, acc[n][i]);
           }
@@ -389,11 +390,11 @@ __global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(
       if (have == C) {
         const float block = p.update * power(l2, static_cast<float>(C - 32 - j + 1 - p.extra));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = e < 4 ? leave[e % 4] * (block * leave16) : leave[e % 4] * block;
+        for (int e = 0; e < 8; ++e) f[e] = e < 4 ? leave[e % 4] * (block * leave_half) : leave[e % 4] * block;
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int n = have - p.extra - (j + 16 * (e / 4) + quad + e % 4);
+          const int n = have - p.extra - (j + step_of<IO>(quad, e));
           f[e] = p.update * power(l2, static_cast<float>(n < 0 ? 0 : n));
         }
       }
@@ -408,12 +409,11 @@ __global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(
       }
 #pragma unroll
       for (int i = 0; i < KT; ++i) {
-        const Frag<IO> kf = read_columns(lk, W::KS, j, 16 * i);
+        const Frag<IO> kf = read_tile_columns<typename W::K>(lk, j, i);
 #pragma unroll
-        for (int n = 0; n < NV; ++n)
+        for (int m = AP - 1; m >= 0; --m)
 #pragma unroll
-          for (int m = AP - 1; m >= 0; --m) s[i][n] = mma(kf, added[n][m], s[i][n]);
-        if (i % 2) __builtin_amdgcn_sched_barrier(0);
+          for (int n = 0; n < NV; ++n) s[i][n] = mma(kf, added[n][m], s[i][n]);
       }
     }
     if constexpr (OUT) {

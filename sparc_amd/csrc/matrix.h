@@ -1,13 +1,13 @@
 // Operands of the matrix instructions (16x16 results in fp32), for fp32 and bf16
 // values in one form.
 //
-// A fragment holds, for lane l of a wave, the eight values at 32 consecutive indices
-// of the contraction that lie at 16 h + 4 (l / 16) + i (h < 2, i < 4) of row (or
-// column) l % 16.  Both operands of a product are held in this order, so the order in
-// which the instruction itself numbers the contraction does not matter.  A result has
-// rows 4 (l / 16) + i of column l % 16 in lane l: two results, one above the other,
-// are a fragment of the operand whose contraction runs over their rows, without any
-// exchange between lanes.
+// A fragment holds, for lane l of a wave, eight of 32 consecutive indices of the
+// contraction of row (or column) l % 16: bf16 those from 8 (l / 16) on, fp32 16 h + 4
+// (l / 16) + i (h < 2, i < 4).  Both operands of a product are held in this order, so
+// the order in which the instruction itself numbers the contraction does not matter.
+// A result has rows 4 (l / 16) + i of column l % 16 in lane l.  Two results are a
+// fragment of the operand whose contraction runs over their rows, without any exchange
+// between lanes, if their rows stand for the indices that tile_row gives.
 #ifndef SPARC_MATRIX_H
 #define SPARC_MATRIX_H
 
@@ -25,7 +25,7 @@ template <typename IO> struct QuadOf;  // four values
 template <> struct QuadOf<bf16> { typedef s16x4 T; };
 template <> struct QuadOf<float> { typedef f32x4 T; };
 template <typename IO> using Quad = typename QuadOf<IO>::T;
-template <typename IO> struct Frag { Quad<IO> q[2]; };
+template <typename IO> struct alignas(16) Frag { Quad<IO> q[2]; };
 
 // c + a b over the 32 indices of the contraction
 __device__ __forceinline__ f32x4 mma(const Frag<bf16>& a, const Frag<bf16>& b, f32x4 c) {
@@ -40,35 +40,61 @@ __device__ __forceinline__ f32x4 mma(const Frag<float>& a, const Frag<float>& b,
   return c;
 }
 
-// Rows row0 + l % 16 of an LDS array whose rows lie ``stride`` values apart (a multiple
-// of a quad), the contraction from column col0 on
-template <typename IO> __device__ __forceinline__ Frag<IO> read_rows(const IO* lds, int stride, int row0, int col0) {
-  const int lane = threadIdx.x & 63;
-  const IO* p = lds + (row0 + (lane & 15)) * stride + col0 + 4 * (lane >> 4);
+// Index of the contraction (of 32) that element e of a fragment is, quad = 4 (l / 16)
+template <typename IO> __device__ __forceinline__ constexpr int step_of(int quad, int e) {
+  return sizeof(IO) == 2 ? 2 * quad + e : 16 * (e / 4) + quad + e % 4;
+}
+// Index that row quad + r of the i-th result stands for
+template <typename IO> __device__ __forceinline__ constexpr int tile_row(int i, int quad, int r) {
+  return sizeof(IO) == 2 ? 32 * (i / 2) + 2 * quad + 4 * (i % 2) + r : 16 * i + quad + r;
+}
+
+// Rows of COLS values in LDS, longer by some bytes so that a wave's accesses spread over
+// the banks: 16 bytes where rows are read along them, 32 where bf16 columns are read
+// across them (4 rows of 16 columns then lie in different banks).
+template <typename IO, int COLS, bool ACROSS> struct Panel {
+  static constexpr int kStride = COLS + (sizeof(IO) == 2 && ACROSS ? 32 : 16) / sizeof(IO);
+  static __device__ __forceinline__ int at(int row, int col) { return row * kStride + col; }
+};
+
+// Rows row0 + l % 16, the contraction from column col0 on (multiples of 16 and 32)
+template <typename L, typename IO> __device__ __forceinline__ Frag<IO> read_rows(const IO* lds, int row0, int col0) {
+  const int lane = threadIdx.x & 63, row = row0 + (lane & 15);
   Frag<IO> f;
-  f.q[0] = *reinterpret_cast<const Quad<IO>*>(p);
-  f.q[1] = *reinterpret_cast<const Quad<IO>*>(p + 16);
+  if constexpr (sizeof(IO) == 2) {
+    f = *reinterpret_cast<const Frag<IO>*>(lds + L::at(row, col0 + 8 * (lane >> 4)));
+  } else {
+    const IO* p = lds + L::at(row, col0 + 4 * (lane >> 4));
+    f.q[0] = *reinterpret_cast<const Quad<IO>*>(p);
+    f.q[1] = *reinterpret_cast<const Quad<IO>*>(p + 16);
+  }
   return f;
 }
-// Columns col0 + l % 16, the contraction over the rows from row0 on
-__device__ __forceinline__ Frag<bf16> read_columns(const bf16* lds, int stride, int row0, int col0) {
+// 16 columns, of which lane l gets column_of(l % 16), four at a time in a row; the
+// contraction over the rows from row0 on (a multiple of 32)
+template <typename L, typename IO, typename F>
+__device__ __forceinline__ Frag<IO> gather_columns(const IO* lds, int row0, F&& column_of) {
   const int lane = threadIdx.x & 63;
-  // 16 lanes exchange a block of 4 rows x 16 columns that they read in quads of a row
-  const bf16* p = lds + (row0 + 4 * (lane >> 4) + ((lane & 15) >> 2)) * stride + col0 + 4 * (lane & 3);
-  Frag<bf16> f;
-  f.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p));
-  f.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 16 * stride));
+  Frag<IO> f;
+  if constexpr (sizeof(IO) == 2) {
+    // 16 lanes exchange a block of 4 rows x 16 columns that they read in quads of a row
+    const int row = row0 + 8 * (lane >> 4) + ((lane & 15) >> 2), col = column_of(4 * (lane & 3));
+    f.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds + L::at(row, col)));
+    f.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds + L::at(row + 4, col)));
+  } else {
+    const IO* p = lds + L::at(row0 + 4 * (lane >> 4), column_of(lane & 15));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f.q[e / 4][e % 4] = p[(16 * (e / 4) + e % 4) * L::kStride];
+  }
   return f;
 }
-__device__ __forceinline__ Frag<float> read_columns(const float* lds, int stride, int row0, int col0) {
-  const int lane = threadIdx.x & 63;
-  const float* p = lds + (row0 + 4 * (lane >> 4)) * stride + col0 + (lane & 15);
-  Frag<float> f;
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f.q[h][i] = p[(16 * h + i) * stride];
-  return f;
+// Columns col0 + l % 16
+template <typename L, typename IO> __device__ __forceinline__ Frag<IO> read_columns(const IO* lds, int row0, int col0) {
+  return gather_columns<L>(lds, row0, [&](int m) { return col0 + m; });
+}
+// The columns that the rows of the i-th result stand for
+template <typename L, typename IO> __device__ __forceinline__ Frag<IO> read_tile_columns(const IO* lds, int row0, int i) {
+  return gather_columns<L>(lds, row0, [&](int m) { return tile_row<IO>(i, m & ~3, m & 3); });
 }
 
 // fp32 values as a sum of N fragments: N bf16 values hold 8 N bits of each (a value
