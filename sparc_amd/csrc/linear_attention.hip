@@ -59,12 +59,30 @@ __device__ __forceinline__ int64_t steps_of(const Problems& a, int64_t b) {
   return n < 0 ? 0 : n < a.T ? n : a.T;
 }
 
+// The value, which the compiler takes for another one each time: what is computed from
+// it in a loop is computed there, and is not kept in registers that the loop needs.
+__device__ __forceinline__ float anew(float x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+__device__ __forceinline__ int anew(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+__device__ __forceinline__ uint32_t anew(uint32_t x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // Values of each operand that a bf16 product takes: the state and the scores as two
-// bf16 values (2^-17 of their size), what is added to the state as three (2^-25), so
-// that the state keeps 24 bits over any number of chunks.
+// bf16 values (2^-17 of their size); what is added to the state as three (2^-25) where
+// the state is a result (EXACT), and as two where it only passes through to results in
+// bf16.
 template <typename IO> constexpr int kStateParts = sizeof(IO) == 2 ? 2 : 1;
 template <typename IO> constexpr int kScoreParts = sizeof(IO) == 2 ? 2 : 1;
-template <typename IO> constexpr int kAddedParts = sizeof(IO) == 2 ? 3 : 1;
+
+// An offset that no buffer reaches: loads there give zero, stores are dropped.
+constexpr uint32_t kNowhere = 0x80000000u;
 
 // Steps of a chunk, by the type and the padded key width
 template <typename IO, int KP> constexpr int kChunk = sizeof(IO) == 2 && KP < 256 ? 64 : 32;
@@ -79,16 +97,13 @@ template <typename IO, int KP, int NW, int NV> struct Tiles {
   using P = Panel<IO, C, false>;
 };
 
-// An offset that no buffer reaches: loads there give zero, stores are dropped.
-constexpr uint32_t kNowhere = 0x80000000u;
-
 // One operand's rows of a chunk on their way to LDS: TILE columns from ``from`` on of
 // rows of ``width`` values.  A thread reads 16-byte vectors of one column position
 // through a buffer that ends with the chunk's last row, so that nothing needs a
 // condition (a branch around a load makes the loads wait for one another): what lies
 // behind the last row or the last column is zero.  The vector that a row's end would
 // cut is read so that it ends with the row, and shifted.
-template <typename IO, int C, int TILE, int THREADS> struct Stage {
+template <typename IO, int C, int TILE, int THREADS, bool WHOLE> struct Stage {
   static constexpr int VEC = kVec<IO>, PER = TILE / VEC, SIZE = sizeof(IO);
   static constexpr int STEP = THREADS / PER < C ? THREADS / PER : C, N = C / STEP;
   typedef uint32_t u4 __attribute__((ext_vector_type(4)));
@@ -113,34 +128,31 @@ template <typename IO, int C, int TILE, int THREADS> struct Stage {
   }
   // the rows of steps t0 .. t0 + have - 1
   __device__ __forceinline__ void fetch(int64_t t0, int have) {
+    if (!WHOLE && width < VEC) return;
     const IO* const low = down ? p - (t0 + have - 1) * gap : p + t0 * gap;
     const auto buffer = make_rsrc(low, static_cast<uint32_t>(((have - 1) * gap + width) * SIZE));
     const uint32_t bytes = static_cast<uint32_t>(gap) * SIZE;
     const uint32_t first = at + bytes * static_cast<uint32_t>(down ? have - 1 - row() : row());
-    if (width < VEC) {  // value by value: a vector would end behind the last row
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const uint32_t on = bytes * static_cast<uint32_t>(i * STEP), to = down ? first - on : first + on;
-        r[i] = u4{0, 0, 0, 0};
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          const uint32_t one = k < width ? to + k * SIZE : kNowhere;
-          if constexpr (SIZE == 4) r[i][k] = __builtin_amdgcn_raw_buffer_load_b32(buffer, one, 0, 0);
-          else r[i][k / 2] |= static_cast<uint32_t>(__builtin_amdgcn_raw_buffer_load_b16(buffer, one, 0, 0)) << (16 * (k % 2));
-        }
-      }
-      return;
-    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const uint32_t on = bytes * static_cast<uint32_t>(i * STEP);
       r[i] = __builtin_amdgcn_raw_buffer_load_b128(buffer, down ? first - on : first + on, 0, 0);
     }
   }
-  template <typename L> __device__ __forceinline__ void put(IO* lds) {
+  template <typename L> __device__ __forceinline__ void put(IO* lds, int64_t t0, int have) {
+    if (!WHOLE && width < VEC) {  // rows shorter than a vector, value by value
+#pragma unroll 1
+      for (int e = threadIdx.x; e < C * TILE; e += THREADS) {
+        const int k = e / TILE, c = e % TILE;
+        IO x = {};
+        if (c < width && k < have) x = p[(t0 + k) * (down ? -gap : gap) + c];
+        lds[L::at(k, c)] = x;
+      }
+      return;
+    }
     if (THREADS / PER > C && row() >= C) return;  // fewer vectors than threads
-    if (width % VEC) {
-      const int words = lack * SIZE / 4, odd = lack * SIZE % 4;
+    if (!WHOLE && width % VEC) {
+      const int far = anew(lack * SIZE), words = far / 4, odd = far % 4;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const u4 u = r[i];
@@ -163,12 +175,15 @@ template <typename IO, int C, int TILE, int THREADS> struct Stage {
 
 // A workgroup of NW waves: one chain (batch row and head), 16 NW NV value columns, one
 // segment of steps.  Each wave keeps the state of its 16 NV columns in registers.
-// OUT: with outputs; else only what the segment adds to the state.
-template <typename IO, int KP, int NW, int NV, bool OUT>
-__global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(const Problems a) {
+// OUT: with outputs; else only what the segment adds to the state.  WHOLE: keys as wide
+// as the tile, values that tiles divide and outputs in the I/O type; the other paths
+// cost registers that the kernel for 128 x 128 needs (they spilled:
+// 65536 steps of 16 heads 640 us with them, 555 without).
+template <typename IO, int KP, int NW, int NV, bool OUT, bool EXACT, bool WHOLE>
+__global__ __launch_bounds__(64 * NW, KP * NV >= 128 ? 2 : 3) void linear_kernel(const Problems a) {
   using W = Tiles<IO, KP, NW, NV>;
   constexpr int C = W::C, KT = KP / 16, NT = C / 16, THREADS = 64 * NW;
-  constexpr int SP = kStateParts<IO>, PP = kScoreParts<IO>, AP = kAddedParts<IO>;
+  constexpr int SP = kStateParts<IO>, PP = kScoreParts<IO>, AP = sizeof(IO) == 4 ? 1 : EXACT ? 3 : 2;
   __shared__ __attribute__((aligned(16))) IO lq[OUT ? C * W::Q::kStride : 1];
   __shared__ __attribute__((aligned(16))) IO lk[C * W::K::kStride];
   __shared__ __attribute__((aligned(16))) IO lv[C * W::V::kStride];
@@ -185,44 +200,58 @@ __global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t steps = steps_of(a, b), first = seg * a.seg_len;
   const int64_t last = first + a.seg_len < a.T ? first + a.seg_len : a.T, end = last < steps ? last : steps;
-  const float l2 = log2_decay(a.decay, h);
+  const float l2_once = log2_decay(a.decay, h);
   const int v0 = v_tile * W::VT, w0 = wave * 16 * NV;  // first column of the workgroup, of the wave within it
 
   // the state: s[i][n] holds rows tile_row(i, quad, r) of column v0 + w0 + 16 n + col
   f32x4 s[KT][NV];
   const int64_t state = static_cast<int64_t>(chain) * p.K * p.V;
-  const auto each_state = [&](auto&& f) {
+  // f(the value, its offset in bytes for these strides, or one that no buffer reaches)
+  const auto each_state = [&](int of_k, int of_n, auto&& f) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < KT; ++i)
+    for (int n = 0; n < NV; ++n) {
+      const int c = v0 + w0 + 16 * n + col;
 #pragma unroll
-      for (int n = 0; n < NV; ++n)
+      for (int i = 0; i < KT; ++i) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int row = tile_row<IO>(i, quad, r), c = v0 + w0 + 16 * n + col;
-          if (row < p.K && c < p.V) s[i][n][r] = f(s[i][n][r], row, c);
+          const int row = tile_row<IO>(i, quad, r);
+          s[i][n][r] = f(s[i][n][r], row < p.K && c < p.V ? static_cast<uint32_t>(4 * (row * of_k + c * of_n)) : kNowhere);
         }
+        __builtin_amdgcn_sched_barrier(0);  // offsets of few values at a time
+      }
+    }
+  };
+  const auto read_state = [&](const float* from, int of_k, int of_n) __attribute__((always_inline)) {
+    const auto buffer = make_rsrc(from, static_cast<uint32_t>(4 * p.K * p.V));
+    each_state(of_k, of_n, [&](float, uint32_t at) __attribute__((always_inline)) {
+      return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(buffer, at, 0, 0));
+    });
+  };
+  const auto write_state = [&](float* to, int of_k, int of_n) __attribute__((always_inline)) {
+    const auto buffer = make_rsrc(to, static_cast<uint32_t>(4 * p.K * p.V));
+    each_state(of_k, of_n, [&](float x, uint32_t at) __attribute__((always_inline)) {
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x), buffer, at, 0, 0);
+      return x;
+    });
   };
 #pragma unroll
   for (int i = 0; i < KT; ++i)
 #pragma unroll
     for (int n = 0; n < NV; ++n) s[i][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   if constexpr (OUT) {
-    if (a.segments > 1) {
-      const float* from = p.seg + (static_cast<int64_t>(chain) * a.segments + seg) * p.K * p.V;
-      each_state([&](float, int row, int c) { return from[row * p.V + c]; });
-    } else if (p.s_in) {
-      each_state([&](float, int row, int c) { return p.s_in[state + row * p.in_k + c * p.in_n]; });
-    }
+    if (a.segments > 1) read_state(p.seg + (static_cast<int64_t>(chain) * a.segments + seg) * p.K * p.V, p.V, 1);
+    else if (p.s_in) read_state(p.s_in + state, p.in_k, p.in_n);
   }
 
-  Stage<IO, C, KP, THREADS> sq, sk;
-  Stage<IO, C, W::VT, THREADS> sv;
+  Stage<IO, C, KP, THREADS, WHOLE> sq, sk;
+  Stage<IO, C, W::VT, THREADS, WHOLE> sv;
   const int64_t rows = steps < 1 ? 1 : steps;
   if constexpr (OUT) sq.begin(p.q, b, h, p.K, 0, p.reverse, rows);
   sk.begin(p.k, b, h, p.K, 0, p.reverse, rows);
   sv.begin(p.v, b, h, p.V, v0, p.reverse, rows);
-  const auto have_at = [&](int64_t t0) { return static_cast<int>(end - t0 < C ? end - t0 : C); };
-  const auto fetch = [&](int64_t t0) {
+  const auto have_at = [&](int64_t t0) __attribute__((always_inline)) { return static_cast<int>(end - t0 < C ? end - t0 : C); };
+  const auto fetch = [&](int64_t t0) __attribute__((always_inline)) {
     const int have = have_at(t0);
     if constexpr (OUT) sq.fetch(t0, have);
     sk.fetch(t0, have);
@@ -230,22 +259,21 @@ __global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(
   };
   // outputs of columns c4 .. c4 + 3 of steps t0 + 16 i + col, ``count`` steps from t0 on
   const int64_t o_gap = static_cast<int64_t>(a.H) * p.V;
-  const auto emit = [&](int64_t t0, int count, bool down, int c4, const auto& x, auto tiles) {
-    const int size = p.o_f32 ? 4 : sizeof(IO);
+  const auto emit = [&](int64_t t0, int count, bool down, int c4, const auto& x, auto tiles) __attribute__((always_inline)) {
+    const int size = !WHOLE && p.o_f32 ? 4 : sizeof(IO);
     const int64_t low = down ? steps - t0 - count : t0;
     const auto buffer = make_rsrc(static_cast<char*>(p.o) + ((b * a.T + low) * o_gap + h * p.V) * size,
                                   static_cast<uint32_t>(((count - 1) * o_gap + p.V) * size));
-    const auto each = [&](auto&& store) {
+    const uint32_t step = static_cast<uint32_t>(o_gap) * size;
+    const uint32_t at = anew(static_cast<uint32_t>(down ? count - 1 - col : col) * step + c4 * size);
+    const auto each = [&](auto&& store) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < tiles; ++i) {
-        const int k = 16 * i + col;
-        const uint32_t at = static_cast<uint32_t>((down ? count - 1 - k : k) * static_cast<int>(o_gap) + c4) * size;
-        store(x[i], k < count && c4 < p.V ? at : kNowhere);
-      }
+      for (int i = 0; i < tiles; ++i)
+        store(x[i], 16 * i + col < count && c4 < p.V ? (down ? at - 16 * i * step : at + 16 * i * step) : kNowhere);
     };
     typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-    if (p.V % 4) {
-      each([&](const f32x4& y, uint32_t to) {
+    if (!WHOLE && p.V % 4) {
+      each([&](const f32x4& y, uint32_t to) __attribute__((always_inline)) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const uint32_t one = c4 + r < p.V ? to + r * size : kNowhere;
@@ -254,12 +282,12 @@ __global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(
         }
       });
     } else if (size == 4) {
-      each([&](const f32x4& y, uint32_t to) {
+      each([&](const f32x4& y, uint32_t to) __attribute__((always_inline)) {
         const float f[4] = {y[0], y[1], y[2], y[3]};
         buffer_store_f32<4, 0>(buffer, to, f);
       });
     } else {
-      each([&](const f32x4& y, uint32_t to) {
+      each([&](const f32x4& y, uint32_t to) __attribute__((always_inline)) {
         __builtin_amdgcn_raw_buffer_store_b64(u2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])}, buffer, to, 0, 0);
       });
     }
@@ -269,34 +297,44 @@ __global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(
   constexpr int kHalf = sizeof(IO) == 2 ? 4 : 16;  // from a fragment's first four steps to the others
   float leave[4];  // a^(31 - step) of those
 #pragma unroll
-  for (int r = 0; r < 4; ++r) leave[r] = power(l2, static_cast<float>(31 - step_of<IO>(quad, 4 + r)));
-  const float leave_half = power(l2, static_cast<float>(kHalf));
-  constexpr int ST = NT * NT > NW ? NT * NT / NW : 1;  // score tiles of a wave
-  const int qt = wave % NT;
+  for (int r = 0; r < 4; ++r) leave[r] = power(l2_once, static_cast<float>(31 - step_of<IO>(quad, 4 + r)));
+  const float leave_half = power(l2_once, static_cast<float>(kHalf));
+  constexpr int TILES = NT * (NT + 1) / 2;  // of scores: a tile of queries with its own and earlier keys
+  static_assert(NT <= 4, "the tiles' numbers");
+  if constexpr (OUT) {  // the tile of keys behind an even tile of queries is read and stays zero
+    if (wave < NT / 2)
+#pragma unroll
+      for (int n = 0; n < PP; ++n)
+        *reinterpret_cast<Quad<IO>*>(&lp[n][W::P::at(32 * wave + col, 32 * wave + 16 + quad)]) = Quad<IO>{};
+  }
 
-  if (first < end) fetch(first);
+  const auto put = [&](int64_t t0) __attribute__((always_inline)) {
+    const int have = have_at(t0);
+    if constexpr (OUT) sq.template put<typename W::Q>(lq, t0, have);
+    sk.template put<typename W::K>(lk, t0, have);
+    sv.template put<typename W::V>(lv, t0, have);
+  };
+  if (first < end) {
+    fetch(first);
+    put(first);
+  }
   for (int64_t t0 = first; t0 < end; t0 += C) {
     const int have = have_at(t0);
-    __syncthreads();  // the chunk before is no longer read
-    if constexpr (OUT) sq.template put<typename W::Q>(lq);
-    sk.template put<typename W::K>(lk);
-    sv.template put<typename W::V>(lv);
-    __syncthreads();
-    if (t0 + C < end) fetch(t0 + C);
+    const float l2 = anew(l2_once);
+    __syncthreads();  // the chunk is there
 
     f32x4 acc[OUT ? NV : 1][OUT ? NT : 1];
     if constexpr (OUT) {
-      // scores of 16 queries with some tiles of keys: decayed, zero for later keys
+      // scores of 16 queries with 16 keys, decayed, zero for later keys
 #pragma unroll
-      for (int m = 0; m < ST; ++m) {
-        const int kt = wave / NT + m * (NW > NT ? NW / NT : 1);
-        if (kt > (qt | 1)) continue;  // not read (and waves without a tile)
+      for (int m = 0; m < (TILES + NW - 1) / NW; ++m) {
+        const int tile = wave + m * NW;
+        if (tile >= TILES) break;
+        const int qt = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, kt = tile - qt * (qt + 1) / 2;
         f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (kt <= qt) {
 #pragma unroll
-          for (int c = 0; c < KP; c += 32)
-            x = mma(read_rows<typename W::K>(lk, 16 * kt, c), read_rows<typename W::Q>(lq, 16 * qt, c), x);
-        }
+        for (int c = 0; c < KP; c += 32)
+          x = mma(read_rows<typename W::K>(lk, 16 * kt, c), read_rows<typename W::Q>(lq, 16 * qt, c), x);
         float y[8];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -347,6 +385,8 @@ __global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(
 #pragma unroll
       for (int n = 0; n < NV; ++n) s[i][n] *= whole;
     if constexpr (OUT) __syncthreads();  // the scores are there
+    // early enough for the rows to arrive, and late enough that q S needs no registers
+    if (t0 + C < end) fetch(t0 + C);
 #pragma unroll
     for (int j = 0; j < C; j += 32) {
       Frag<IO> vf[NV];
@@ -356,8 +396,8 @@ __global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(
         // a value that is not finite must not reach earlier steps of its block as 0 v
         uint32_t odd = 0;
 #pragma unroll
-        for (int n = 0; n < NV; ++n) odd |= odd_bits(vf[n]);
-        const bool apart = __any(odd != 0);
+        for (int n = 0; n < NV; ++n) odd = see(odd, vf[n]);
+        const bool apart = __any(is_odd<IO>(odd));
         if (apart) {
 #pragma unroll
           for (int i = j / 16; i < j / 16 + 2; ++i)
@@ -414,8 +454,13 @@ __global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(
         for (int m = AP - 1; m >= 0; --m)
 #pragma unroll
           for (int n = 0; n < NV; ++n) s[i][n] = mma(kf, added[n][m], s[i][n]);
+        if (i % 2) __builtin_amdgcn_sched_barrier(0);  // fragments of two tiles at a time: no more registers
       }
     }
+    // Outputs are stored after the next chunk's rows have arrived: memory operations
+    // end in order, and a wait for the rows must not wait for the stores.
+    __syncthreads();  // the chunk is no longer read
+    if (t0 + C < end) put(t0 + C);
     if constexpr (OUT) {
 #pragma unroll
       for (int n = 0; n < NV; ++n) emit(t0, have, p.reverse, v0 + w0 + 16 * n + quad, acc[n], Int<NT>());
@@ -427,11 +472,9 @@ __global__ __launch_bounds__(64 * NW, KP * NV < 128 ? 3 : 2) void linear_kernel(
 #pragma unroll
       for (int n = 0; n < NV; ++n)
         emit(t, static_cast<int>(last - t < 16 ? last - t : 16), false, v0 + w0 + 16 * n + quad, zero, Int<1>());
-    if (a.segments == 1 && p.s_out)
-      each_state([&](float x, int row, int c) { return p.s_out[state + row * p.out_k + c * p.out_n] = x; });
+    if (a.segments == 1 && p.s_out) write_state(p.s_out + state, p.out_k, p.out_n);
   } else {
-    float* to = p.seg + (static_cast<int64_t>(chain) * a.segments + seg) * p.K * p.V;
-    each_state([&](float x, int row, int c) { return to[row * p.V + c] = x; });
+    write_state(p.seg + (static_cast<int64_t>(chain) * a.segments + seg) * p.K * p.V, p.V, 1);
   }
 }
 
@@ -552,12 +595,17 @@ struct Plan {
   int segments;
   int64_t seg_len;
 };
-// Time is cut into segments where the chains alone are too few workgroups.
+// Time is cut into segments where the chains alone leave most of the GPU idle: into as
+// many as the workgroups that it holds at once.  A second pass over keys and values,
+// and the states between the passes, cost about as much as two thirds of idle CUs (16 x
+// 2048 steps of 12 heads of 64, 192 workgroups of 768: 94 us in one pass, 79 with 4
+// segments; the gradients of 8 x 4096 steps of 8 heads of 128, 192 of 512: 400 in one
+// pass, 447 with 4 segments, 487 with 3).
 Plan plan_of(const sparc_linear_desc* d, int64_t k, int64_t v, int problems) {
   const int64_t chunk = d->io_dtype == SPARC_BF16 && padded(k) < 256 ? 64 : 32;
   const int64_t width = columns_of(v), groups = d->batch * d->heads * ((v + width - 1) / width) * problems;
-  const int64_t most = d->length / (4 * chunk);  // segments of four chunks at least
-  int64_t n = groups >= 384 || groups < 1 ? 1 : (1024 + groups - 1) / groups;
+  const int64_t slots = padded(k) * (width / 64) >= 128 ? 512 : 768, most = d->length / (4 * chunk);
+  int64_t n = groups < 1 || 3 * groups >= slots ? 1 : slots / groups;
   if (n > most) n = most;
   if (n < 1) n = 1;
   int64_t len = (d->length + n - 1) / n;
@@ -580,12 +628,25 @@ template <typename IO, int KP, int NW, int NV> void launch(Problems& a, int n, i
     total += a.blocks[i];
   }
   if (total == 0) return;
+  bool exact = false, whole = true;
+  for (int i = 0; i < n; ++i) {
+    exact = exact || (a.segments == 1 && a.p[i].s_out);  // with segments the joined states are the results
+    whole = whole && a.p[i].K == KP && a.p[i].V % VT == 0 && !a.p[i].o_f32;
+  }
   if (a.segments > 1) {
-    linear_kernel<IO, KP, NW, NV, false><<<total, 64 * NW, 0, stream>>>(a);
+    if (whole) linear_kernel<IO, KP, NW, NV, false, true, true><<<total, 64 * NW, 0, stream>>>(a);
+    else linear_kernel<IO, KP, NW, NV, false, true, false><<<total, 64 * NW, 0, stream>>>(a);
     for (int i = 0; i < n; ++i)
       linear_join_kernel<<<static_cast<unsigned>((a.p[i].K * a.p[i].V + 255) / 256 * chains), 256, 0, stream>>>(a, i);
   }
-  linear_kernel<IO, KP, NW, NV, true><<<total, 64 * NW, 0, stream>>>(a);
+  constexpr bool kOne = sizeof(IO) == 4;  // fp32 products are exact either way
+  if (whole) {
+    if (exact) linear_kernel<IO, KP, NW, NV, true, true, true><<<total, 64 * NW, 0, stream>>>(a);
+    else linear_kernel<IO, KP, NW, NV, true, kOne, true><<<total, 64 * NW, 0, stream>>>(a);
+  } else {
+    if (exact) linear_kernel<IO, KP, NW, NV, true, true, false><<<total, 64 * NW, 0, stream>>>(a);
+    else linear_kernel<IO, KP, NW, NV, true, kOne, false><<<total, 64 * NW, 0, stream>>>(a);
+  }
 }
 // All problems have the same padded widths
 template <typename IO> void launch_io(Problems& a, int n, int64_t chains, hipStream_t stream) {

@@ -138,19 +138,28 @@ __device__ __forceinline__ void widen(const Frag<float>& f, float (&x)[8]) {
   for (int i = 0; i < 8; ++i) x[i] = f.q[i / 4][i % 4];
 }
 
-// Bits that are set where a value is infinite or no number
-__device__ __forceinline__ uint32_t odd_bits(const Frag<bf16>& f) {
-  uint32_t u[4], odd = 0;
+// Whether a value of the fragments that top has seen is infinite or no number: the
+// largest exponent is kept, of bf16 two at a time
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t see(uint32_t top, const Frag<bf16>& f) {
+  uint32_t u[4];
   __builtin_memcpy(u, &f, sizeof(u));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) odd |= ((u[i] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-  return odd;
+  for (int i = 0; i < 4; ++i)
+    top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top),
+                                                                 __builtin_bit_cast(u16x2, u[i] & 0x7fff7fffu)));
+  return top;
 }
-__device__ __forceinline__ uint32_t odd_bits(const Frag<float>& f) {
-  uint32_t odd = 0;
+__device__ __forceinline__ uint32_t see(uint32_t top, const Frag<float>& f) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) odd |= ((__float_as_uint(f.q[i / 4][i % 4]) & 0x7f800000u) + 0x00800000u) & 0x80000000u;
-  return odd;
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t u = __float_as_uint(f.q[i / 4][i % 4]) & 0x7fffffffu;
+    top = top > u ? top : u;
+  }
+  return top;
+}
+template <typename IO> __device__ __forceinline__ bool is_odd(uint32_t top) {
+  return sizeof(IO) == 4 ? top >= 0x7f800000u : (top & 0xffffu) >= 0x7f80u || top >= 0x7f800000u;
 }
 
 // n (at most 4) values to p, rounded to OUT
