@@ -6,8 +6,8 @@
 // All of them are matrix products: out[q][p] = sum over k of Q[q][k] P[p][k].  A launch
 // makes g and u of a tile together and leaves y, or (the backward computes them again
 // instead of keeping them: nothing of the width of the block is saved, and dg and du
-// come from unrounded g and u) dg and du, side by side in one matrix G of 2 F columns.
-// Then dx = G [Wg; Wu] and [dWg; dWu] = G^T x are one product each.
+// come from unrounded g and u) dg and du.  dx is one launch over both contractions, the
+// weights' gradients are one launch of two products.
 #include "matrix.h"
 
 namespace sparc {
@@ -15,8 +15,11 @@ namespace {
 
 enum Act : int { ACT_SILU = 0, ACT_GELU = 1, ACT_RELU = 2, ACT_SIGMOID = 3 };
 
-// act(g), and its derivative
-__device__ __forceinline__ float act_of(int act, float g, float& slope) {
+// act(g), and its derivative.  For results in bf16 the sigmoid is that of the hardware's
+// base-2 exponential and reciprocal (some 2^-21 of its value; the library's take 30
+// instructions more for each value, and a tile of 256 x 256 results is computed in
+// little more time than its activations were).
+template <typename IO> __device__ __forceinline__ float act_of(int act, float g, float& slope) {
   if (act == ACT_RELU) {
     slope = g > 0.0f ? 1.0f : 0.0f;
     return g > 0.0f ? g : g * 0.0f;  // NaN stays
@@ -26,7 +29,7 @@ __device__ __forceinline__ float act_of(int act, float g, float& slope) {
     slope = phi + g * expf(-0.5f * g * g) * 0.39894228040143268f;
     return g * phi;
   }
-  const float sig = 1.0f / (1.0f + expf(-g));
+  const float sig = sizeof(IO) == 2 ? __builtin_amdgcn_rcpf(1.0f + fast_exp(-g)) : 1.0f / (1.0f + expf(-g));
   if (act == ACT_SIGMOID) {
     slope = sig * (1.0f - sig);
     return sig;
@@ -36,154 +39,292 @@ __device__ __forceinline__ float act_of(int act, float g, float& slope) {
 }
 
 // An operand: rows r (the result's p or q) and the contraction k; element (r, k) at
-// r ld + k, or (ACROSS) at k ld + r.  Two parts: rows (or, ACROSS, values of the
-// contraction) from ``cut`` on are those of p1.
+// r ld + k, or (ACROSS) at k ld + r.  Of two parts each has a tensor of its own.
 struct Operand {
-  const void *p0, *p1;
-  int64_t ld;
-  int64_t cut;
+  const void* p[2];
+  int64_t ld, rows;
 };
 struct ProductArgs {
   Operand P, Q;
-  int64_t np, nq, nk;  // sizes of the result and of the contraction
-  void *out0, *out1;   // rows q from out_cut on are those of out1
-  int64_t out_ld, out_cut;
-  const void* dy;      // GATED_BACK: [nq, F]
-  int act;
-  int64_t k_split;     // contraction of one workgroup; partial sums in fp32 where it is shorter than nk
-  float* partial;      // [splits, nq, np]
+  int64_t nk;             // contraction of a part
+  int p_tiles, q_tiles;   // workgroups; in PAIR and of a gated product each side's own tiles
+  void* out[2];           // [rows q, rows p], row stride out_ld
+  int64_t out_ld;
+  const void* dy;         // GATED_BACK: [Q.rows, P.rows]
+  int act, parts;
+  int64_t k_split;        // contraction of one workgroup (one part); shorter than nk: partial sums
+  float* partial;         // [splits, sides, Q.rows, P.rows]
 };
 
-enum Kind : int { GATED = 0, GATED_BACK = 1, PRODUCT = 2 };
+// GATED: both parts of P at once, out[0] = act(.) * (.).  GATED_BACK: out[0] and out[1]
+// the gradients of both projections.  PARTS: the sum over both parts.  PAIR: a product
+// for each part of Q.
+enum Kind : int { GATED = 0, GATED_BACK = 1, PARTS = 2, PAIR = 3 };
 
-constexpr int kTile = 128;
+// An offset that no buffer reaches: loads there give zero.
+constexpr uint32_t kNowhere = 0x80000000u;
 
-template <typename IO, int KIND, bool PA, bool QA>
-__global__ __launch_bounds__(256, 2) void product_kernel(const ProductArgs a) {
-  constexpr int BK = 32, VEC = kVec<IO>;
-  constexpr bool DUAL = KIND != PRODUCT;
-  // [tile rows][BK], or ACROSS [BK][tile rows]
-  using LP = Panel<IO, PA ? kTile : BK, PA>;
-  using LQ = Panel<IO, QA ? kTile : BK, QA>;
-  __shared__ __attribute__((aligned(16))) IO lp[(PA ? BK : kTile) * LP::kStride];
-  __shared__ __attribute__((aligned(16))) IO lq[(QA ? BK : kTile) * LQ::kStride];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, quad = 4 * (lane >> 4);
-  constexpr int PT = DUAL ? kTile / 2 : kTile;
-  const int64_t p0 = static_cast<int64_t>(blockIdx.x) * PT, q0 = static_cast<int64_t>(blockIdx.y) * kTile;
-  const int64_t k0 = blockIdx.z * a.k_split, k1 = k0 + a.k_split < a.nk ? k0 + a.k_split : a.nk;
+// Bytes 2 and 3 of b and a: their upper halves, truncated to bf16, a's below
+__device__ __forceinline__ uint32_t upper_halves(uint32_t a, uint32_t b) {
+  return __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
 
-  constexpr int N = kTile * BK / VEC / 256;
-  Vec<IO> rp[N], rq[N];
-  const auto fetch = [&](const Operand& o, auto across, auto dual, int64_t r0, int64_t rows, int64_t k, Vec<IO>(&r)[N]) {
+// LINES x COLS values of an operand on their way from memory to LDS, through a buffer
+// that ends with the last line, so that no load is under a condition: what lies behind
+// the last line or column is zero.  A vector that the columns' end would cut is read so
+// that it ends with them, and shifted.  fp32 values become the sum of three bf16 values
+// (truncated, then the rest truncated, then the rest, which is exact: 8 bits each).
+// WHOLE: no vector is cut.
+template <typename IO, int LINES, int COLS, int THREADS, bool ACROSS, bool WHOLE> struct Feed {
+  static constexpr int VEC = kVec<IO>, PER = COLS / VEC, SIZE = sizeof(IO), STEP = THREADS / PER, N = LINES / STEP;
+  static constexpr int PARTS = SIZE == 2 ? 1 : 3;
+  using L = Panel<bf16, COLS, ACROSS>;
+  static constexpr int kSize = LINES * L::kStride;  // of one part
+  static_assert(THREADS % PER == 0 && LINES % STEP == 0, "whole vectors per thread");
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+  u4 r[N];
+  int lack;
+
+  static __device__ __forceinline__ int line() { return static_cast<int>(threadIdx.x) / PER; }
+  static __device__ __forceinline__ int column() { return static_cast<int>(threadIdx.x) % PER * VEC; }
+  // Columns up to ``end`` of lines of ``size`` values; at(i) is the byte of line(i)'s
+  // first column in the buffer, or kNowhere.
+  template <typename F>
+  __device__ __forceinline__ void fetch(__amdgpu_buffer_rsrc_t buffer, int64_t end, int64_t size, F&& at) {
+    fetch_by(end, size, [&](int) __attribute__((always_inline)) { return buffer; }, at);
+  }
+  template <typename B, typename F>
+  __device__ __forceinline__ void fetch_by(int64_t end, int64_t size, B&& buffer, F&& at) {
+    const int64_t c = column();
+    const int64_t left = WHOLE || c + VEC <= end || size < VEC ? c : end - VEC;
+    lack = static_cast<int>(c - left);
+    const bool there = lack < VEC && c < end;
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = one(buffer(i), at(i), there, left, end, size);
+  }
+  static __device__ __forceinline__ u4 one(__amdgpu_buffer_rsrc_t buffer, uint32_t line_at, bool there, int64_t left,
+                                           int64_t end, int64_t size) {
+    const uint32_t first = there && line_at < kNowhere ? line_at + static_cast<uint32_t>(left * SIZE) : kNowhere;
+    if (WHOLE || size >= VEC) return __builtin_amdgcn_raw_buffer_load_b128(buffer, first, 0, 0);
+    // lines shorter than a vector, value by value: a vector would end behind the last one
+    u4 u = {0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const uint32_t from = left + k < end ? first + k * SIZE : kNowhere;
+      if constexpr (SIZE == 4) u[k] = __builtin_amdgcn_raw_buffer_load_b32(buffer, from, 0, 0);
+      else u[k / 2] |= static_cast<uint32_t>(__builtin_amdgcn_raw_buffer_load_b16(buffer, from, 0, 0)) << (16 * (k % 2));
+    }
+    return u;
+  }
+  __device__ __forceinline__ void put(bf16* lds, bool ragged) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int e = tid + 256 * i;
-      if constexpr (decltype(across)::value) {
-        const int line = e / (kTile / VEC), c = e % (kTile / VEC) * VEC;
-        const int64_t kk = k + line;
-        const void* p = kk < o.cut ? o.p0 : o.p1;
-        r[i] = load_vec<IO>(p, (kk < o.cut ? kk : kk - o.cut) * o.ld + r0 + c,
-                            kk < k1 ? static_cast<int>(rows - r0 - c < VEC ? rows - r0 - c : VEC) : 0);
+      u4 u = r[i];
+      if (!WHOLE && ragged) {
+        const int words = lack * SIZE / 4, odd = lack * SIZE % 4;
+        uint32_t w[5];
+#pragma unroll
+        for (int k = 0; k < 5; ++k) {
+          w[k] = 0;
+#pragma unroll
+          for (int m = k; m < 4; ++m) w[k] = words == m - k ? u[m] : w[k];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) u[k] = odd ? w[k] >> 16 | w[k + 1] << 16 : w[k];
+      }
+      bf16* const to = lds + L::at(line() + i * STEP, column());
+      if constexpr (SIZE == 2) {
+        *reinterpret_cast<u4*>(to) = u;
       } else {
-        const int line = e / (BK / VEC), c = e % (BK / VEC) * VEC;
-        // DUAL: of 64 lines, 32 of the gate's rows, then the same 32 of the other's
-        const bool other = decltype(dual)::value && (line & 32);
-        const int64_t row = r0 + (decltype(dual)::value ? (line >> 6) * 32 + (line & 31) : line);
-        r[i] = load_vec<IO>(other ? o.p1 : o.p0, row * o.ld + k + c,
-                            row < rows ? static_cast<int>(k1 - k - c < VEC ? k1 - k - c : VEC) : 0);
+        float x[4];
+#pragma unroll
+        for (int part = 0; part < 3; ++part) {
+          typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+          *reinterpret_cast<u2*>(to + part * kSize) = u2{upper_halves(u[0], u[1]), upper_halves(u[2], u[3])};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            x[k] = __uint_as_float(u[k]) - __uint_as_float(u[k] & 0xffff0000u);
+            u[k] = __float_as_uint(x[k]);
+          }
+        }
       }
     }
-  };
-  const auto put = [&](IO* lds, auto across, const Vec<IO>(&r)[N]) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int e = tid + 256 * i;
-      constexpr int cols = decltype(across)::value ? kTile : BK, per = cols / VEC;
-      *reinterpret_cast<Vec<IO>*>(lds + Panel<IO, cols, decltype(across)::value>::at(e / per, e % per * VEC)) = r[i];
+  }
+};
+
+// TP x TQ results by WP x WQ waves; BK values of the contraction at a time, in BUFFERS
+// places in LDS.
+template <typename IO, int KIND, bool PA, bool QA, int TP, int TQ, int WP, int WQ, int BK, int BUFFERS, bool WHOLE>
+__global__ __launch_bounds__(64 * WP * WQ, 2) void product_kernel(const ProductArgs a) {
+  constexpr bool DUAL = KIND == GATED || KIND == GATED_BACK;
+  constexpr int THREADS = 64 * WP * WQ, VEC = kVec<IO>, SIZE = sizeof(IO);
+  constexpr int LP = TP / WP, LQ = TQ / WQ, MP = LP / 16, MQ = LQ / 16;  // a wave's results, and in tiles
+  constexpr int PT = DUAL ? TP / 2 : TP;
+  using FP = Feed<IO, PA ? BK : TP, PA ? TP : BK, THREADS, PA, WHOLE>;
+  using FQ = Feed<IO, QA ? BK : TQ, QA ? TQ : BK, THREADS, QA, WHOLE>;
+  constexpr int SP = FP::kSize * FP::PARTS, SQ = FQ::kSize * FQ::PARTS, SUM = FP::PARTS;
+  __shared__ __attribute__((aligned(16))) bf16 lds[BUFFERS * (SP + SQ)];
+
+  const int lane = threadIdx.x & 63, col = lane & 15, quad = 4 * (lane >> 4);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wp = wave % WP * LP, wq = wave / WP * LQ;
+  // neighbouring workgroups of an XCD: eight tiles of q beside all of p
+  const int sides = KIND == PAIR ? 2 : 1;
+  const int per_split = a.p_tiles * a.q_tiles * sides, id = xcd_swizzle(blockIdx.x, gridDim.x);
+  const int split = id / per_split, rest = id % per_split;
+  const int all_q = a.q_tiles * sides, group = rest / (8 * a.p_tiles), first_q = 8 * group;
+  const int here = all_q - first_q < 8 ? all_q - first_q : 8, within = rest - 8 * group * a.p_tiles;
+  const int q_tile = first_q + within % here, p_tile = within / here;
+  const int side = KIND == PAIR ? q_tile / a.q_tiles : 0;
+  const int64_t p0 = static_cast<int64_t>(p_tile) * PT, q0 = static_cast<int64_t>(q_tile - side * a.q_tiles) * TQ;
+  const int64_t k0 = split * a.k_split, k1 = k0 + a.k_split < a.nk ? k0 + a.k_split : a.nk;
+
+  FP fp;
+  FQ fq;
+  // a tile's lines of the contraction from k on, or its rows
+  const auto fetch = [&](auto& feed, const Operand& o, auto across, auto dual, int64_t r0, int64_t k, int part)
+                         __attribute__((always_inline)) {
+    using F = std::remove_reference_t<decltype(feed)>;
+    if constexpr (decltype(across)::value) {
+      const int lines = static_cast<int>(k1 - k < BK ? k1 - k : BK);
+      // a vector's start may have to move left of the tile: offsets count from the lines' start
+      const auto buffer = make_rsrc(static_cast<const IO*>(o.p[part]) + k * o.ld,
+                                    static_cast<uint32_t>(((lines - 1) * o.ld + o.rows) * SIZE));
+      feed.fetch(buffer, o.rows - r0, o.rows, [&](int i) __attribute__((always_inline)) {
+        return static_cast<uint32_t>((F::line() + i * F::STEP) * o.ld + r0) * SIZE;
+      });
+    } else {
+      const int64_t rows = o.rows - r0 < TP + TQ ? o.rows - r0 : TP + TQ;
+      const auto buffer_of = [&](int which) __attribute__((always_inline)) {
+        return make_rsrc(static_cast<const IO*>(o.p[which]) + r0 * o.ld,
+                         static_cast<uint32_t>(((rows - 1) * o.ld + a.nk) * SIZE));
+      };
+      const auto at = [&](int row) __attribute__((always_inline)) {
+        return row < rows ? static_cast<uint32_t>(row * o.ld + k) * SIZE : kNowhere;
+      };
+      if constexpr (decltype(dual)::value) {
+        // of a wave's lines one half is of the first part, the other of the second; the
+        // lines of one load are of one of them
+        const auto gate = buffer_of(0), up = buffer_of(1);
+        feed.fetch_by(k1 - k, a.nk, [&](int i) __attribute__((always_inline)) {
+          return __builtin_amdgcn_readfirstlane(F::line() + i * F::STEP) / (LP / 2) % 2 ? up : gate;
+        }, [&](int i) __attribute__((always_inline)) {
+          const int line = F::line() + i * F::STEP;
+          return at(line / LP * (LP / 2) + line % (LP / 2));
+        });
+      } else {
+        feed.fetch(buffer_of(part), k1 - k, a.nk, [&](int i) __attribute__((always_inline)) {
+          return at(F::line() + i * F::STEP);
+        });
+      }
     }
   };
   using PAcross = std::integral_constant<bool, PA>;
   using QAcross = std::integral_constant<bool, QA>;
   using Dual = std::integral_constant<bool, DUAL>;
-  const int wp = (wave & 1) * 64, wq = (wave >> 1) * 64;
-  f32x4 acc[4][4];  // [p][q] tiles
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  const auto fetch_both = [&](int64_t k) {
-    fetch(a.P, PAcross(), Dual(), p0, a.np, k, rp);
-    fetch(a.Q, QAcross(), std::false_type(), q0, a.nq, k, rq);
+  const auto fetch_both = [&](int64_t k, int part) __attribute__((always_inline)) {
+    fetch(fp, a.P, PAcross(), Dual(), p0, k, part);
+    fetch(fq, a.Q, QAcross(), std::false_type(), q0, k, KIND == PAIR ? side : part);
   };
-  fetch_both(k0);
-  for (int64_t k = k0; k < k1; k += BK) {
-    __syncthreads();
-    put(lp, PAcross(), rp);
-    put(lq, QAcross(), rq);
-    __syncthreads();
-    if (k + BK < k1) fetch_both(k + BK);
-    Frag<IO> fp[4], fq[4];
+  const auto put_both = [&](int place, int64_t k) __attribute__((always_inline)) {
+    const bool tail = k1 - k < BK && (k1 - k) % VEC != 0 && a.nk >= VEC;
+    fp.put(lds + place * (SP + SQ), PA ? p0 + TP > a.P.rows && a.P.rows % VEC != 0 && a.P.rows >= VEC : tail);
+    fq.put(lds + place * (SP + SQ) + SP, QA ? q0 + TQ > a.Q.rows && a.Q.rows % VEC != 0 && a.Q.rows >= VEC : tail);
+  };
+  f32x4 acc[MP][MQ];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (PA) fp[i] = read_columns<LP>(lp, 0, wp + 16 * i);
-      else fp[i] = read_rows<LP>(lp, wp + 16 * i, 0);
-      if constexpr (QA) fq[i] = read_columns<LQ>(lq, 0, wq + 16 * i);
-      else fq[i] = read_rows<LQ>(lq, wq + 16 * i, 0);
+  for (int i = 0; i < MP; ++i)
+#pragma unroll
+    for (int j = 0; j < MQ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const auto multiply = [&](int place) __attribute__((always_inline)) {
+    const bf16* const lp = lds + place * (SP + SQ);
+    const bf16* const lq = lp + SP;
+#pragma unroll
+    for (int c = 0; c < BK; c += 32) {
+      Frag<bf16> p[SUM][MP], q[SUM][MQ];
+#pragma unroll
+      for (int n = 0; n < SUM; ++n) {
+#pragma unroll
+        for (int i = 0; i < MP; ++i) {
+          if constexpr (PA) p[n][i] = read_columns<typename FP::L>(lp + n * FP::kSize, c, wp + 16 * i);
+          else p[n][i] = read_rows<typename FP::L>(lp + n * FP::kSize, wp + 16 * i, c);
+        }
+#pragma unroll
+        for (int j = 0; j < MQ; ++j) {
+          if constexpr (QA) q[n][j] = read_columns<typename FQ::L>(lq + n * FQ::kSize, c, wq + 16 * j);
+          else q[n][j] = read_rows<typename FQ::L>(lq + n * FQ::kSize, wq + 16 * j, c);
+        }
+      }
+      // of three parts each the six products that reach the 24 bits, the small ones first
+#pragma unroll
+      for (int order = SUM - 1; order >= 0; --order)
+#pragma unroll
+        for (int n = 0; n <= order; ++n)
+#pragma unroll
+          for (int i = 0; i < MP; ++i)
+#pragma unroll
+            for (int j = 0; j < MQ; ++j) acc[i][j] = mma(p[n][i], q[order - n][j], acc[i][j]);
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = mma(fp[i], fq[j], acc[i][j]);
+  };
+  // steps: all of one part, then all of the next
+  const int per_part = static_cast<int>((k1 - k0 + BK - 1) / BK), steps = per_part * (KIND == PARTS ? a.parts : 1);
+  const auto k_of = [&](int step) { return k0 + static_cast<int64_t>(step % per_part) * BK; };
+  const auto part_of = [&](int step) { return step / per_part; };
+  fetch_both(k0, 0);
+  if constexpr (BUFFERS == 2) {
+    put_both(0, k0);
+    if (steps > 1) fetch_both(k_of(1), part_of(1));
+    for (int step = 0; step < steps; ++step) {
+      __syncthreads();  // this step's place is filled, and the other one no longer read
+      if (step + 1 < steps) {
+        put_both((step + 1) & 1, k_of(step + 1));
+        if (step + 2 < steps) fetch_both(k_of(step + 2), part_of(step + 2));
+      }
+      multiply(step & 1);
+    }
+  } else {
+    for (int step = 0; step < steps; ++step) {
+      __syncthreads();
+      put_both(0, k_of(step));
+      __syncthreads();
+      if (step + 1 < steps) fetch_both(k_of(step + 1), part_of(step + 1));
+      multiply(0);
+    }
   }
-  if constexpr (DUAL) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t q = q0 + wq + 16 * j + col;
-      if (q >= a.nq) continue;
+  for (int j = 0; j < MQ; ++j) {
+    const int64_t q = q0 + wq + 16 * j + col;
+    if (q >= a.Q.rows) continue;
+    if constexpr (DUAL) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < MP / 2; ++i) {
         const int64_t p = p0 + wp / 2 + 16 * i + quad;
-        const int n = static_cast<int>(a.np - p < 4 ? a.np - p : 4);
+        const int n = static_cast<int>(a.P.rows - p < 4 ? a.P.rows - p : 4);
         if (n <= 0) continue;
         f32x4 slope, h;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           float d;
-          h[r] = act_of(a.act, acc[i][j][r], d);
+          h[r] = act_of<IO>(a.act, acc[i][j][r], d);
           slope[r] = d;
         }
+        const int64_t at = q * a.out_ld + p;
         if constexpr (KIND == GATED) {
-          store_quad(static_cast<IO*>(a.out0) + q * a.out_ld + p, n, h * acc[i + 2][j]);
+          store_quad(static_cast<IO*>(a.out[0]) + at, n, h * acc[i + MP / 2][j]);
         } else {
-          f32x4 dy = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (r < n) {
-              float y[1];
-              unpack<IO, 1>(load_raw<IO, 1>(a.dy, q * a.np + p + r), y);
-              dy[r] = y[0];
-            }
-          store_quad(static_cast<IO*>(a.out0) + q * a.out_ld + p, n, dy * acc[i + 2][j] * slope);
-          store_quad(static_cast<IO*>(a.out0) + q * a.out_ld + a.np + p, n, dy * h);
+          const f32x4 dy = load_quad(static_cast<const IO*>(a.dy) + q * a.P.rows + p, n);
+          store_quad(static_cast<IO*>(a.out[0]) + at, n, dy * acc[i + MP / 2][j] * slope);
+          store_quad(static_cast<IO*>(a.out[1]) + at, n, dy * h);
         }
       }
-    }
-  } else {
+    } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t q = q0 + wq + 16 * j + col;
-      if (q >= a.nq) continue;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < MP; ++i) {
         const int64_t p = p0 + wp + 16 * i + quad;
-        const int n = static_cast<int>(a.np - p < 4 ? a.np - p : 4);
+        const int n = static_cast<int>(a.P.rows - p < 4 ? a.P.rows - p : 4);
         if (n <= 0) continue;
-        if (a.partial) {
-          store_quad(a.partial + (blockIdx.z * a.nq + q) * a.np + p, n, acc[i][j]);
-        } else {
-          IO* out = static_cast<IO*>(q < a.out_cut ? a.out0 : a.out1);
-          store_quad(out + (q < a.out_cut ? q : q - a.out_cut) * a.out_ld + p, n, acc[i][j]);
-        }
+        if (a.partial) store_quad(a.partial + ((split * sides + side) * a.Q.rows + q) * a.P.rows + p, n, acc[i][j]);
+        else store_quad(static_cast<IO*>(a.out[side]) + q * a.out_ld + p, n, acc[i][j]);
       }
     }
   }
@@ -209,80 +350,111 @@ __global__ __launch_bounds__(256) void product_sum_kernel(const float* partial, 
 // ---------------------------------------------------------------------------
 const char* fault_of(int64_t rows, int64_t dim, int64_t hidden, int32_t io, int32_t act) {
   if (rows < 0 || dim < 1 || hidden < 1) return "gated linear unit: rows must not be negative, dim and hidden positive";
-  if (rows >= (1LL << 31) || dim >= (1LL << 31) || hidden >= (1LL << 30)) return "gated linear unit: too large";
+  // a tile's lines lie within 2^31 bytes
+  if (rows >= (1LL << 31) || dim >= (1LL << 20) || hidden >= (1LL << 20)) return "gated linear unit: too large";
   if (io != SPARC_F32 && io != SPARC_BF16) return "gated linear unit: io_dtype must be F32 or BF16";
   if (act < ACT_SILU || act > ACT_SIGMOID) return "gated linear unit: unknown activation";
   return nullptr;
 }
 size_t size_of(int32_t io) { return io == SPARC_BF16 ? 2 : 4; }
 
-// Parts of the contraction over the rows in the weights' gradient: as many as fill the GPU
-int splits_of(int64_t rows, int64_t dim, int64_t hidden) {
-  const int64_t tiles = ((dim + kTile - 1) / kTile) * ((2 * hidden + kTile - 1) / kTile);
-  int64_t n = (512 + tiles - 1) / tiles, most = rows / 512;
-  if (n > most) n = most;
-  return static_cast<int>(n < 1 ? 1 : n > 64 ? 64 : n);
+int64_t tiles(int64_t n, int64_t tile) { return (n + tile - 1) / tile; }
+
+// Tiles of a product: large ones where there are enough of them for every CU, else
+// smaller ones, two to a CU.
+bool large_tiles(int32_t io, int64_t np, int64_t nq) {
+  return io == SPARC_BF16 && tiles(np, 256) * tiles(nq, 256) >= 192;
 }
+
 struct GatedPlan {
-  int splits;
-  int64_t k_split;
+  int splits;        // parts of the contraction over the rows in the weights' gradients
+  int64_t k_split, g_ld;
   size_t g, partial;
 };
 GatedPlan gated_plan(int64_t rows, int64_t dim, int64_t hidden, int32_t io) {
   GatedPlan p;
-  p.splits = splits_of(rows, dim, hidden);
-  p.k_split = ((rows + p.splits - 1) / p.splits + 31) / 32 * 32;
-  if (p.k_split < 32) p.k_split = 32;
-  p.splits = static_cast<int>((rows + p.k_split - 1) / p.k_split);
+  const bool large = io == SPARC_BF16 && rows >= 4096 && dim >= 192 && hidden >= 192;
+  const int64_t tile = large ? 256 : 128, slots = large ? 256 : 512;
+  const int64_t count = tiles(dim, tile) * tiles(hidden, tile) * 2;
+  int64_t n = slots / count, most = rows / 512;
+  if (n > most) n = most;
+  n = n < 1 ? 1 : n > 64 ? 64 : n;
+  p.k_split = tiles(tiles(rows, n), 64) * 64;
+  if (p.k_split < 64) p.k_split = 64;
+  p.splits = static_cast<int>(tiles(rows, p.k_split));
   if (p.splits < 1) p.splits = 1;
-  p.g = up256(2 * rows * hidden * size_of(io));
+  p.g_ld = tiles(hidden, 8) * 8;  // whole vectors, whatever the width
+  p.g = up256(rows * p.g_ld * size_of(io));
   p.partial = p.splits > 1 ? up256(sizeof(float) * p.splits * 2 * hidden * dim) : 0;
   return p;
 }
-dim3 grid_of(int64_t np, int64_t nq, int tile_p, int splits) {
-  return dim3(static_cast<unsigned>((np + tile_p - 1) / tile_p), static_cast<unsigned>((nq + kTile - 1) / kTile),
-              static_cast<unsigned>(splits));
+
+template <typename IO, int KIND, bool PA, bool QA, int TP, int TQ, int WP, int WQ, int BK, int BUFFERS, bool WHOLE>
+void product_tiled(ProductArgs& a, hipStream_t stream) {
+  constexpr bool DUAL = KIND == GATED || KIND == GATED_BACK;
+  a.p_tiles = static_cast<int>(tiles(a.P.rows, DUAL ? TP / 2 : TP));
+  a.q_tiles = static_cast<int>(tiles(a.Q.rows, TQ));
+  const int64_t count = static_cast<int64_t>(a.p_tiles) * a.q_tiles * (KIND == PAIR ? 2 : 1) * tiles(a.nk, a.k_split);
+  product_kernel<IO, KIND, PA, QA, TP, TQ, WP, WQ, BK, BUFFERS, WHOLE><<<static_cast<unsigned>(count), 64 * WP * WQ, 0, stream>>>(a);
+}
+template <typename IO, int KIND, bool PA, bool QA> void product(ProductArgs& a, bool large, hipStream_t stream) {
+  constexpr int VEC = 16 / sizeof(IO);
+  // no vector of a line is cut by the line's end
+  const bool whole = (PA && QA ? true : a.nk % VEC == 0) && (!PA || a.P.rows % VEC == 0) && (!QA || a.Q.rows % VEC == 0);
+  if constexpr (sizeof(IO) == 2) {
+    if (!whole) product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 64, 2, false>(a, stream);
+    else if (large) product_tiled<IO, KIND, PA, QA, 256, 256, 4, 2, 64, 2, true>(a, stream);
+    else product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 64, 2, true>(a, stream);
+  } else {
+    if (whole) product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 32, 1, true>(a, stream);
+    else product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 32, 1, false>(a, stream);
+  }
 }
 
 template <typename IO>
-void gated_run(int64_t rows, int64_t dim, int64_t hidden, int act, const void* x, const void* wg, const void* wu,
-               const void* dy, void* y, hipStream_t stream) {
+void gated_run(int32_t io, int64_t rows, int64_t dim, int64_t hidden, int act, const void* x, const void* wg,
+               const void* wu, const void* dy, void* out0, void* out1, int64_t out_ld, hipStream_t stream) {
   ProductArgs a = {};
-  a.P = {wg, wu, dim, hidden};
-  a.Q = {x, x, dim, rows};
-  a.np = hidden, a.nq = rows, a.nk = a.k_split = dim;
-  a.out0 = y;
+  a.P = {{wg, wu}, dim, hidden};
+  a.Q = {{x, x}, dim, rows};
+  a.nk = a.k_split = dim;
+  a.out[0] = out0, a.out[1] = out1;
+  a.out_ld = out_ld;
   a.dy = dy;
   a.act = act;
-  a.out_ld = dy ? 2 * hidden : hidden;
-  const dim3 grid = grid_of(hidden, rows, kTile / 2, 1);
-  if (dy) product_kernel<IO, GATED_BACK, false, false><<<grid, 256, 0, stream>>>(a);
-  else product_kernel<IO, GATED, false, false><<<grid, 256, 0, stream>>>(a);
+  a.parts = 1;
+  const bool large = large_tiles(io, 2 * hidden, rows);
+  if (dy) product<IO, GATED_BACK, false, false>(a, large, stream);
+  else product<IO, GATED, false, false>(a, large, stream);
 }
 template <typename IO>
-void gated_grads(int64_t rows, int64_t dim, int64_t hidden, const void* x, const void* wg, const void* wu, const void* g,
-                 void* dx, void* dwg, void* dwu, float* partial, const GatedPlan& plan, hipStream_t stream) {
+void gated_grads(int32_t io, int64_t rows, int64_t dim, int64_t hidden, const void* x, const void* wg, const void* wu,
+                 const void* dg, const void* du, void* dx, void* dwg, void* dwu, float* partial, const GatedPlan& plan,
+                 hipStream_t stream) {
   if (dx) {
     ProductArgs a = {};
-    a.P = {wg, wu, dim, hidden};
-    a.Q = {g, g, 2 * hidden, 2 * hidden};
-    a.np = dim, a.nq = rows, a.nk = a.k_split = 2 * hidden;
-    a.out0 = a.out1 = dx;
-    a.out_ld = dim, a.out_cut = rows;
-    product_kernel<IO, PRODUCT, true, false><<<grid_of(dim, rows, kTile, 1), 256, 0, stream>>>(a);
+    a.P = {{wg, wu}, dim, dim};
+    a.Q = {{dg, du}, plan.g_ld, rows};
+    a.nk = a.k_split = hidden;
+    a.out[0] = a.out[1] = dx;
+    a.out_ld = dim;
+    a.parts = 2;
+    product<IO, PARTS, true, false>(a, large_tiles(io, dim, rows), stream);
   }
   if (dwg) {
     ProductArgs a = {};
-    a.P = {x, x, dim, rows};
-    a.Q = {g, g, 2 * hidden, rows};
-    a.np = dim, a.nq = 2 * hidden, a.nk = rows, a.k_split = plan.k_split;
-    a.out0 = dwg, a.out1 = dwu;
-    a.out_ld = dim, a.out_cut = hidden;
+    a.P = {{x, x}, dim, dim};
+    a.Q = {{dg, du}, plan.g_ld, hidden};
+    a.nk = rows > 0 ? rows : 1;
+    a.k_split = plan.k_split;
+    a.out[0] = dwg, a.out[1] = dwu;
+    a.out_ld = dim;
+    a.parts = 1;
     a.partial = plan.splits > 1 ? partial : nullptr;
-    product_kernel<IO, PRODUCT, true, true><<<grid_of(dim, 2 * hidden, kTile, plan.splits), 256, 0, stream>>>(a);
-    if (plan.splits > 1)
+    if (rows > 0) product<IO, PAIR, true, true>(a, plan.k_split >= 512 && large_tiles(io, dim, 2 * hidden * plan.splits), stream);
+    if (rows == 0 || plan.splits > 1)
       product_sum_kernel<IO><<<op_grid((2 * hidden * dim + 255) / 256), 256, 0, stream>>>(
-          partial, plan.splits, hidden * dim, static_cast<IO*>(dwg), static_cast<IO*>(dwu));
+          partial, rows > 0 ? plan.splits : 0, hidden * dim, static_cast<IO*>(dwg), static_cast<IO*>(dwu));
   }
 }
 
@@ -300,15 +472,17 @@ sparc_status sparc_gated_forward(int64_t rows, int64_t dim, int64_t hidden, int3
   if (rows == 0) return SPARC_OK;
   if (!x || !gate_weight || !up_weight || !y) return op_fail(SPARC_EINVAL, "gated linear unit: a tensor is NULL");
   const hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
-  if (io_dtype == SPARC_BF16) gated_run<bf16>(rows, dim, hidden, activation, x, gate_weight, up_weight, nullptr, y, stream);
-  else gated_run<float>(rows, dim, hidden, activation, x, gate_weight, up_weight, nullptr, y, stream);
+  if (io_dtype == SPARC_BF16)
+    gated_run<bf16>(io_dtype, rows, dim, hidden, activation, x, gate_weight, up_weight, nullptr, y, nullptr, hidden, stream);
+  else
+    gated_run<float>(io_dtype, rows, dim, hidden, activation, x, gate_weight, up_weight, nullptr, y, nullptr, hidden, stream);
   return op_launched("sparc_gated_forward");
 }
 
 size_t sparc_gated_workspace_bytes(int64_t rows, int64_t dim, int64_t hidden, int32_t io_dtype) {
   if (fault_of(rows, dim, hidden, io_dtype, 0)) return 0;
   const GatedPlan p = gated_plan(rows, dim, hidden, io_dtype);
-  return p.g + p.partial;
+  return 2 * p.g + p.partial;
 }
 
 sparc_status sparc_gated_backward(int64_t rows, int64_t dim, int64_t hidden, int32_t io_dtype, int32_t activation,
@@ -319,16 +493,17 @@ sparc_status sparc_gated_backward(int64_t rows, int64_t dim, int64_t hidden, int
   if ((rows > 0 && (!x || !dy)) || !gate_weight || !up_weight || !dgate_weight != !dup_weight)
     return op_fail(SPARC_EINVAL, "gated linear unit: a tensor is NULL");
   const GatedPlan plan = gated_plan(rows, dim, hidden, io_dtype);
-  if (rows > 0 && (!workspace || workspace_bytes < plan.g + plan.partial))
+  if (rows > 0 && (!workspace || workspace_bytes < 2 * plan.g + plan.partial))
     return op_fail(SPARC_EWORKSPACE, "gated linear unit: workspace missing or too small");
   const hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
   char* const ws = static_cast<char*>(workspace);
-  float* const partial = reinterpret_cast<float*>(ws + plan.g);
+  void *const dg = ws, *const du = ws + plan.g;
+  float* const partial = reinterpret_cast<float*>(ws + 2 * plan.g);
   const auto go = [&](auto type) {
     using IO = decltype(type);
-    if (rows > 0) gated_run<IO>(rows, dim, hidden, activation, x, gate_weight, up_weight, dy, ws, stream);
-    gated_grads<IO>(rows, dim, hidden, x, gate_weight, up_weight, ws, rows > 0 ? dx : nullptr, dgate_weight, dup_weight,
-                    partial, plan, stream);
+    if (rows > 0) gated_run<IO>(io_dtype, rows, dim, hidden, activation, x, gate_weight, up_weight, dy, dg, du, plan.g_ld, stream);
+    gated_grads<IO>(io_dtype, rows, dim, hidden, x, gate_weight, up_weight, dg, du, rows > 0 ? dx : nullptr, dgate_weight,
+                    dup_weight, partial, plan, stream);
   };
   if (io_dtype == SPARC_BF16) go(bf16());
   else go(float());

@@ -186,6 +186,27 @@ template <typename OUT> __device__ __forceinline__ void store_quad(OUT* p, int n
   }
 }
 
+// n (at most 4) values from p, the others zero
+template <typename IN> __device__ __forceinline__ f32x4 load_quad(const IN* p, int n) {
+  f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (n >= 4) {
+    if constexpr (sizeof(IN) == 4) {
+      typedef f32x4 loose __attribute__((aligned(4)));
+      v = *reinterpret_cast<const loose*>(p);
+    } else {
+      typedef uint32_t loose __attribute__((ext_vector_type(2), aligned(2)));
+      const loose u = *reinterpret_cast<const loose*>(p);
+      v = f32x4{__uint_as_float(u[0] << 16), __uint_as_float(u[0] & 0xffff0000u), __uint_as_float(u[1] << 16),
+                __uint_as_float(u[1] & 0xffff0000u)};
+    }
+    return v;
+  }
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    if (i < n) v[i] = widen(p[i]);
+  return v;
+}
+
 }  // namespace
 }  // namespace sparc
 
