@@ -51,9 +51,9 @@ struct ProductArgs {
   void* out[2];           // [rows q, rows p], row stride out_ld
   int64_t out_ld;
   const void* dy;         // GATED_BACK: [Q.rows, P.rows]
-  int act, parts;
-  int64_t k_split;        // contraction of one workgroup (one part); shorter than nk: partial sums
-  float* partial;         // [splits, sides, Q.rows, P.rows]
+  int act;
+  int split_steps;        // steps of the contraction (over all parts) of one workgroup
+  float* partial;         // [splits, sides, Q.rows, P.rows]; NULL: one workgroup does all
 };
 
 // GATED: both parts of P at once, out[0] = act(.) * (.).  GATED_BACK: out[0] and out[1]
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void product_kernel(const ProductA
   const int q_tile = first_q + within % here, p_tile = within / here;
   const int side = KIND == PAIR ? q_tile / a.q_tiles : 0;
   const int64_t p0 = static_cast<int64_t>(p_tile) * PT, q0 = static_cast<int64_t>(q_tile - side * a.q_tiles) * TQ;
-  const int64_t k0 = split * a.k_split, k1 = k0 + a.k_split < a.nk ? k0 + a.k_split : a.nk;
+  const int64_t k1 = a.nk;
 
   FP fp;
   FQ fq;
@@ -222,74 +222,128 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void product_kernel(const ProductA
   using PAcross = std::integral_constant<bool, PA>;
   using QAcross = std::integral_constant<bool, QA>;
   using Dual = std::integral_constant<bool, DUAL>;
-  const auto fetch_both = [&](int64_t k, int part) __attribute__((always_inline)) {
+  const auto fetch_p = [&](int64_t k, int part) __attribute__((always_inline)) {
     fetch(fp, a.P, PAcross(), Dual(), p0, k, part);
+  };
+  const auto fetch_q = [&](int64_t k, int part) __attribute__((always_inline)) {
     fetch(fq, a.Q, QAcross(), std::false_type(), q0, k, KIND == PAIR ? side : part);
   };
-  const auto put_both = [&](int place, int64_t k) __attribute__((always_inline)) {
-    const bool tail = k1 - k < BK && (k1 - k) % VEC != 0 && a.nk >= VEC;
-    fp.put(lds + place * (SP + SQ), PA ? p0 + TP > a.P.rows && a.P.rows % VEC != 0 && a.P.rows >= VEC : tail);
-    fq.put(lds + place * (SP + SQ) + SP, QA ? q0 + TQ > a.Q.rows && a.Q.rows % VEC != 0 && a.Q.rows >= VEC : tail);
+  const auto tail = [&](int64_t k) { return k1 - k < BK && (k1 - k) % VEC != 0 && a.nk >= VEC; };
+  const auto put_p = [&](int place, int64_t k) __attribute__((always_inline)) {
+    fp.put(lds + place * (SP + SQ), PA ? p0 + TP > a.P.rows && a.P.rows % VEC != 0 && a.P.rows >= VEC : tail(k));
+  };
+  const auto put_q = [&](int place, int64_t k) __attribute__((always_inline)) {
+    fq.put(lds + place * (SP + SQ) + SP, QA ? q0 + TQ > a.Q.rows && a.Q.rows % VEC != 0 && a.Q.rows >= VEC : tail(k));
   };
   f32x4 acc[MP][MQ];
 #pragma unroll
   for (int i = 0; i < MP; ++i)
 #pragma unroll
     for (int j = 0; j < MQ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  const auto multiply = [&](int place) __attribute__((always_inline)) {
+  Frag<bf16> p[SUM][MP], q[SUM][MQ];
+  // fragments of 32 values of the contraction, c of a place's BK on
+  const auto read = [&](int place, int c) __attribute__((always_inline)) {
     const bf16* const lp = lds + place * (SP + SQ);
     const bf16* const lq = lp + SP;
 #pragma unroll
-    for (int c = 0; c < BK; c += 32) {
-      Frag<bf16> p[SUM][MP], q[SUM][MQ];
+    for (int n = 0; n < SUM; ++n) {
 #pragma unroll
-      for (int n = 0; n < SUM; ++n) {
-#pragma unroll
-        for (int i = 0; i < MP; ++i) {
-          if constexpr (PA) p[n][i] = read_columns<typename FP::L>(lp + n * FP::kSize, c, wp + 16 * i);
-          else p[n][i] = read_rows<typename FP::L>(lp + n * FP::kSize, wp + 16 * i, c);
-        }
-#pragma unroll
-        for (int j = 0; j < MQ; ++j) {
-          if constexpr (QA) q[n][j] = read_columns<typename FQ::L>(lq + n * FQ::kSize, c, wq + 16 * j);
-          else q[n][j] = read_rows<typename FQ::L>(lq + n * FQ::kSize, wq + 16 * j, c);
-        }
+      for (int i = 0; i < MP; ++i) {
+        if constexpr (PA) p[n][i] = read_columns<typename FP::L>(lp + n * FP::kSize, c, wp + 16 * i);
+        else p[n][i] = read_rows<typename FP::L>(lp + n * FP::kSize, wp + 16 * i, c);
       }
-      // of three parts each the six products that reach the 24 bits, the small ones first
 #pragma unroll
-      for (int order = SUM - 1; order >= 0; --order)
-#pragma unroll
-        for (int n = 0; n <= order; ++n)
-#pragma unroll
-          for (int i = 0; i < MP; ++i)
-#pragma unroll
-            for (int j = 0; j < MQ; ++j) acc[i][j] = mma(p[n][i], q[order - n][j], acc[i][j]);
+      for (int j = 0; j < MQ; ++j) {
+        if constexpr (QA) q[n][j] = read_columns<typename FQ::L>(lq + n * FQ::kSize, c, wq + 16 * j);
+        else q[n][j] = read_rows<typename FQ::L>(lq + n * FQ::kSize, wq + 16 * j, c);
+      }
     }
   };
+  // of three parts each the six products that reach the 24 bits, the small ones first
+  const auto multiply = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int order = SUM - 1; order >= 0; --order)
+#pragma unroll
+      for (int n = 0; n <= order; ++n)
+#pragma unroll
+        for (int i = 0; i < MP; ++i)
+#pragma unroll
+          for (int j = 0; j < MQ; ++j) acc[i][j] = mma(p[n][i], q[order - n][j], acc[i][j]);
+  };
   // steps: all of one part, then all of the next
-  const int per_part = static_cast<int>((k1 - k0 + BK - 1) / BK), steps = per_part * (KIND == PARTS ? a.parts : 1);
-  const auto k_of = [&](int step) { return k0 + static_cast<int64_t>(step % per_part) * BK; };
-  const auto part_of = [&](int step) { return step / per_part; };
-  fetch_both(k0, 0);
+  const int per_part = static_cast<int>((a.nk + BK - 1) / BK), all = per_part * (KIND == PARTS ? 2 : 1);
+  const int begin = split * a.split_steps, end = begin + a.split_steps < all ? begin + a.split_steps : all;
+  const int count = end - begin;
+  // Goes from step to step and stays at the last one: what is fetched and put behind it
+  // is not read, and without conditions a wait for some rows waits for no later ones.
+  struct Walk {
+    int64_t k;
+    int part, left;
+    __device__ __forceinline__ void next(int64_t nk) {
+      if (left <= 1) return;
+      --left;
+      k += BK;
+      if (KIND == PARTS && k >= nk) k = 0, ++part;
+    }
+  };
+  Walk at = {static_cast<int64_t>(begin % per_part) * BK, begin / per_part, count}, put_at = at;
   if constexpr (BUFFERS == 2) {
-    put_both(0, k0);
-    if (steps > 1) fetch_both(k_of(1), part_of(1));
-    for (int step = 0; step < steps; ++step) {
+    // Places take turns: while a step is multiplied, the rows of the next go from
+    // registers to the other place, and those of the one after it are fetched.
+    fetch_p(at.k, at.part);
+    fetch_q(at.k, at.part);
+    put_p(0, put_at.k);
+    put_q(0, put_at.k);
+    at.next(a.nk);
+    fetch_p(at.k, at.part);
+    fetch_q(at.k, at.part);
+    for (int step = 0; step < count; ++step) {
+      const int place = step & 1;
       __syncthreads();  // this step's place is filled, and the other one no longer read
-      if (step + 1 < steps) {
-        put_both((step + 1) & 1, k_of(step + 1));
-        if (step + 2 < steps) fetch_both(k_of(step + 2), part_of(step + 2));
+#pragma unroll
+      for (int c = 0; c < BK; c += 32) {
+        if (c == BK / 64 * 32) {
+          put_at.next(a.nk);
+          at.next(a.nk);
+          put_p(1 - place, put_at.k);
+          put_q(1 - place, put_at.k);
+          fetch_p(at.k, at.part);
+          fetch_q(at.k, at.part);
+        }
+        read(place, c);
+        multiply();
       }
-      multiply(step & 1);
     }
   } else {
-    for (int step = 0; step < steps; ++step) {
+    fetch_p(at.k, at.part);
+    fetch_q(at.k, at.part);
+    for (int step = 0; step < count; ++step) {
       __syncthreads();
-      put_both(0, k_of(step));
+      put_p(0, put_at.k);
+      put_q(0, put_at.k);
       __syncthreads();
-      if (step + 1 < steps) fetch_both(k_of(step + 1), part_of(step + 1));
-      multiply(0);
+      put_at.next(a.nk);
+      at.next(a.nk);
+      fetch_p(at.k, at.part);
+      fetch_q(at.k, at.part);
+#pragma unroll
+      for (int c = 0; c < BK; c += 32) {
+        read(0, c);
+        multiply();
+      }
     }
+  }
+  // all of dy first: a wait for a load behind a store waits for the store too
+  f32x4 dys[KIND == GATED_BACK ? MP / 2 : 1][KIND == GATED_BACK ? MQ : 1];
+  if constexpr (KIND == GATED_BACK) {
+#pragma unroll
+    for (int j = 0; j < MQ; ++j)
+#pragma unroll
+      for (int i = 0; i < MP / 2; ++i) {
+        const int64_t q = q0 + wq + 16 * j + col, p = p0 + wp / 2 + 16 * i + quad;
+        const int n = q < a.Q.rows ? static_cast<int>(a.P.rows - p < 4 ? a.P.rows - p : 4) : 0;
+        dys[i][j] = load_quad(static_cast<const IO*>(a.dy) + q * a.P.rows + p, n);
+      }
   }
 #pragma unroll
   for (int j = 0; j < MQ; ++j) {
@@ -312,7 +366,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void product_kernel(const ProductA
         if constexpr (KIND == GATED) {
           store_quad(static_cast<IO*>(a.out[0]) + at, n, h * acc[i + MP / 2][j]);
         } else {
-          const f32x4 dy = load_quad(static_cast<const IO*>(a.dy) + q * a.P.rows + p, n);
+          const f32x4 dy = dys[i][j];
           store_quad(static_cast<IO*>(a.out[0]) + at, n, dy * acc[i + MP / 2][j] * slope);
           store_quad(static_cast<IO*>(a.out[1]) + at, n, dy * h);
         }
@@ -332,9 +386,8 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void product_kernel(const ProductA
 
 // The sum of the partial products, in order
 template <typename IO>
-__global__ __launch_bounds__(256) void product_sum_kernel(const float* partial, int splits, int64_t half, IO* out0,
-                                                          IO* out1) {
-  const int64_t total = 2 * half;
+__global__ __launch_bounds__(256) void product_sum_kernel(const float* partial, int splits, int64_t total, int64_t half,
+                                                          IO* out0, IO* out1) {
   for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < total;
        e += static_cast<int64_t>(gridDim.x) * 256) {
     float s = 0.0f;
@@ -359,55 +412,69 @@ const char* fault_of(int64_t rows, int64_t dim, int64_t hidden, int32_t io, int3
 size_t size_of(int32_t io) { return io == SPARC_BF16 ? 2 : 4; }
 
 int64_t tiles(int64_t n, int64_t tile) { return (n + tile - 1) / tile; }
+int step_of(int32_t io) { return io == SPARC_BF16 ? 64 : 32; }
 
-// Tiles of a product: large ones where there are enough of them for every CU, else
-// smaller ones, two to a CU.
-bool large_tiles(int32_t io, int64_t np, int64_t nq) {
-  return io == SPARC_BF16 && tiles(np, 256) * tiles(nq, 256) >= 192;
+// How a product is cut: into large tiles where they are enough for most CUs, into small
+// ones, two to a CU, else; and its contraction into as many splits as fill the GPU, each
+// of eight steps at least.
+struct Cut {
+  bool large;
+  int splits, split_steps;
+};
+Cut cut_of(int32_t io, bool whole, int64_t np, int64_t nq, int64_t nk, int parts, bool may_split) {
+  Cut c;
+  const int64_t steps = tiles(nk, step_of(io)) * parts, most = may_split && steps >= 16 ? steps / 8 : 1;
+  const int64_t big = tiles(np, 256) * tiles(nq, 256), small = tiles(np, 128) * tiles(nq, 128);
+  c.large = io == SPARC_BF16 && whole && big * most >= 192;
+  const int64_t count = c.large ? big : small, slots = c.large ? 256 : 512;
+  int64_t n = count > 0 ? slots / count : 1;
+  if (n > most) n = most;
+  if (n > 64) n = 64;
+  if (n < 1) n = 1;
+  c.split_steps = static_cast<int>(tiles(steps, n));
+  if (c.split_steps < 1) c.split_steps = 1;
+  c.splits = static_cast<int>(tiles(steps, c.split_steps));
+  if (c.splits < 1) c.splits = 1;
+  return c;
 }
+// Whether no line's end cuts a vector, for lines of these lengths
+bool is_whole(int32_t io, int64_t m, int64_t n = 0) { return io == SPARC_BF16 ? (m | n) % 8 == 0 : (m | n) % 4 == 0; }
 
 struct GatedPlan {
-  int splits;        // parts of the contraction over the rows in the weights' gradients
-  int64_t k_split, g_ld;
-  size_t g, partial;
+  Cut dx, dw;
+  int64_t g_ld;
+  size_t g, partial;  // bytes of dg, and as many of du; of the partial sums, which dx and the weights' share
 };
 GatedPlan gated_plan(int64_t rows, int64_t dim, int64_t hidden, int32_t io) {
   GatedPlan p;
-  const bool large = io == SPARC_BF16 && rows >= 4096 && dim >= 192 && hidden >= 192;
-  const int64_t tile = large ? 256 : 128, slots = large ? 256 : 512;
-  const int64_t count = tiles(dim, tile) * tiles(hidden, tile) * 2;
-  int64_t n = slots / count, most = rows / 512;
-  if (n > most) n = most;
-  n = n < 1 ? 1 : n > 64 ? 64 : n;
-  p.k_split = tiles(tiles(rows, n), 64) * 64;
-  if (p.k_split < 64) p.k_split = 64;
-  p.splits = static_cast<int>(tiles(rows, p.k_split));
-  if (p.splits < 1) p.splits = 1;
+  p.dx = cut_of(io, is_whole(io, dim, hidden), dim, rows, hidden, 2, true);
+  p.dw = cut_of(io, is_whole(io, dim, hidden), dim, 2 * hidden, rows, 1, true);
   p.g_ld = tiles(hidden, 8) * 8;  // whole vectors, whatever the width
   p.g = up256(rows * p.g_ld * size_of(io));
-  p.partial = p.splits > 1 ? up256(sizeof(float) * p.splits * 2 * hidden * dim) : 0;
+  const size_t x = p.dx.splits > 1 ? sizeof(float) * p.dx.splits * rows * dim : 0;
+  const size_t w = p.dw.splits > 1 ? sizeof(float) * p.dw.splits * 2 * hidden * dim : 0;
+  p.partial = up256(x > w ? x : w);
   return p;
 }
 
 template <typename IO, int KIND, bool PA, bool QA, int TP, int TQ, int WP, int WQ, int BK, int BUFFERS, bool WHOLE>
-void product_tiled(ProductArgs& a, hipStream_t stream) {
+void product_tiled(ProductArgs& a, int splits, hipStream_t stream) {
   constexpr bool DUAL = KIND == GATED || KIND == GATED_BACK;
   a.p_tiles = static_cast<int>(tiles(a.P.rows, DUAL ? TP / 2 : TP));
   a.q_tiles = static_cast<int>(tiles(a.Q.rows, TQ));
-  const int64_t count = static_cast<int64_t>(a.p_tiles) * a.q_tiles * (KIND == PAIR ? 2 : 1) * tiles(a.nk, a.k_split);
+  const int64_t count = static_cast<int64_t>(a.p_tiles) * a.q_tiles * (KIND == PAIR ? 2 : 1) * splits;
   product_kernel<IO, KIND, PA, QA, TP, TQ, WP, WQ, BK, BUFFERS, WHOLE><<<static_cast<unsigned>(count), 64 * WP * WQ, 0, stream>>>(a);
 }
-template <typename IO, int KIND, bool PA, bool QA> void product(ProductArgs& a, bool large, hipStream_t stream) {
-  constexpr int VEC = 16 / sizeof(IO);
-  // no vector of a line is cut by the line's end
-  const bool whole = (PA && QA ? true : a.nk % VEC == 0) && (!PA || a.P.rows % VEC == 0) && (!QA || a.Q.rows % VEC == 0);
+template <typename IO, int KIND, bool PA, bool QA>
+void product(ProductArgs& a, const Cut& cut, bool whole, hipStream_t stream) {
+  a.split_steps = cut.split_steps;
   if constexpr (sizeof(IO) == 2) {
-    if (!whole) product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 64, 2, false>(a, stream);
-    else if (large) product_tiled<IO, KIND, PA, QA, 256, 256, 4, 2, 64, 2, true>(a, stream);
-    else product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 64, 2, true>(a, stream);
+    if (!whole) product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 64, 2, false>(a, cut.splits, stream);
+    else if (cut.large) product_tiled<IO, KIND, PA, QA, 256, 256, 4, 2, 64, 2, true>(a, cut.splits, stream);
+    else product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 64, 2, true>(a, cut.splits, stream);
   } else {
-    if (whole) product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 32, 1, true>(a, stream);
-    else product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 32, 1, false>(a, stream);
+    if (whole) product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 32, 1, true>(a, cut.splits, stream);
+    else product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 32, 1, false>(a, cut.splits, stream);
   }
 }
 
@@ -417,44 +484,48 @@ void gated_run(int32_t io, int64_t rows, int64_t dim, int64_t hidden, int act, c
   ProductArgs a = {};
   a.P = {{wg, wu}, dim, hidden};
   a.Q = {{x, x}, dim, rows};
-  a.nk = a.k_split = dim;
+  a.nk = dim;
   a.out[0] = out0, a.out[1] = out1;
   a.out_ld = out_ld;
   a.dy = dy;
   a.act = act;
-  a.parts = 1;
-  const bool large = large_tiles(io, 2 * hidden, rows);
-  if (dy) product<IO, GATED_BACK, false, false>(a, large, stream);
-  else product<IO, GATED, false, false>(a, large, stream);
+  const bool whole = is_whole(io, dim);
+  const Cut cut = cut_of(io, whole, 2 * hidden, rows, dim, 1, false);
+  if (dy) product<IO, GATED_BACK, false, false>(a, cut, whole, stream);
+  else product<IO, GATED, false, false>(a, cut, whole, stream);
+}
+template <typename IO>
+void sum_partial(const float* partial, int splits, int64_t total, int64_t half, void* out0, void* out1, hipStream_t stream) {
+  product_sum_kernel<IO><<<op_grid((total + 255) / 256), 256, 0, stream>>>(partial, splits, total, half,
+                                                                           static_cast<IO*>(out0), static_cast<IO*>(out1));
 }
 template <typename IO>
 void gated_grads(int32_t io, int64_t rows, int64_t dim, int64_t hidden, const void* x, const void* wg, const void* wu,
                  const void* dg, const void* du, void* dx, void* dwg, void* dwu, float* partial, const GatedPlan& plan,
                  hipStream_t stream) {
+  const bool whole = is_whole(io, dim, hidden);
   if (dx) {
     ProductArgs a = {};
     a.P = {{wg, wu}, dim, dim};
     a.Q = {{dg, du}, plan.g_ld, rows};
-    a.nk = a.k_split = hidden;
+    a.nk = hidden;
     a.out[0] = a.out[1] = dx;
     a.out_ld = dim;
-    a.parts = 2;
-    product<IO, PARTS, true, false>(a, large_tiles(io, dim, rows), stream);
+    a.partial = plan.dx.splits > 1 ? partial : nullptr;
+    product<IO, PARTS, true, false>(a, plan.dx, whole, stream);
+    if (a.partial) sum_partial<IO>(partial, plan.dx.splits, rows * dim, rows * dim, dx, dx, stream);
   }
   if (dwg) {
     ProductArgs a = {};
     a.P = {{x, x}, dim, dim};
     a.Q = {{dg, du}, plan.g_ld, hidden};
-    a.nk = rows > 0 ? rows : 1;
-    a.k_split = plan.k_split;
+    a.nk = rows;
     a.out[0] = dwg, a.out[1] = dwu;
     a.out_ld = dim;
-    a.parts = 1;
-    a.partial = plan.splits > 1 ? partial : nullptr;
-    if (rows > 0) product<IO, PAIR, true, true>(a, plan.k_split >= 512 && large_tiles(io, dim, 2 * hidden * plan.splits), stream);
-    if (rows == 0 || plan.splits > 1)
-      product_sum_kernel<IO><<<op_grid((2 * hidden * dim + 255) / 256), 256, 0, stream>>>(
-          partial, rows > 0 ? plan.splits : 0, hidden * dim, static_cast<IO*>(dwg), static_cast<IO*>(dwu));
+    a.partial = plan.dw.splits > 1 ? partial : nullptr;
+    if (rows > 0) product<IO, PAIR, true, true>(a, plan.dw, whole, stream);
+    if (rows == 0 || a.partial)
+      sum_partial<IO>(partial, rows > 0 ? plan.dw.splits : 0, 2 * hidden * dim, hidden * dim, dwg, dwu, stream);
   }
 }
 

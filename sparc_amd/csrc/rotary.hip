@@ -10,6 +10,13 @@
 namespace sparc {
 namespace {
 
+// Heads whose rows a lane holds at once where there are enough of them: the angles of a
+// token are read once for all of them (they are twice a bf16 head's bytes), and more
+// loads are in flight.
+// The backward holds both x and dy, and fewer heads (32768 tokens of 24 heads of 64 bf16:
+// forward 59 us with one head at once, 43 with 4).
+template <bool BACK> constexpr int kHeads = BACK ? 2 : 4;
+
 struct Side {  // queries or keys
   const void* x;
   int64_t sb, st, sh;  // strides in values
@@ -17,15 +24,15 @@ struct Side {  // queries or keys
   const void* dy;      // contiguous, like y and dx
   void* out;           // y or dx
   float* partial;      // [blocks, D]: sums of g xhat (NULL: not wanted)
-  int heads, blocks;
-  int64_t rows;
+  int heads, blocks, chunks;  // chunks: groups of heads of a token
+  int64_t units;              // chunks of all tokens
 };
 struct RotaryArgs {
   Side side[2];
   const float* table;        // [table_rows, R]: cosines, sines
   const int64_t* positions;  // [B, T] or NULL: t
   int64_t table_rows;
-  int T, D, R, lanes, params_f32;
+  int T, D, R, lanes, params_f32, several;
   float eps;
 };
 
@@ -50,18 +57,41 @@ template <typename T, int W> __device__ __forceinline__ void store_few(void* bas
 }
 
 // A unit: W values and the W that they are paired with (for interleaved pairs the 2 W
-// values in a row).  Units of a lane, for heads of up to 512 values:
+// values in a row).  A lane has U units; heads of up to 512 values have at most 64 lanes
+// of so many:
 template <int W> constexpr int kUnits = W >= 4 ? 1 : W == 2 ? 2 : 4;
 
-template <typename IO, int W, bool INTER, bool BACK>
+// W values at the alignment of one, as they lie in memory
+template <typename T, int W> struct __attribute__((packed, aligned(sizeof(T)))) Few { T v[W]; };
+template <int W> __device__ __forceinline__ void widen(const Few<float, W>& f, float* o) {
+#pragma unroll
+  for (int i = 0; i < W; ++i) o[i] = f.v[i];
+}
+template <int W> __device__ __forceinline__ void widen(const Few<bf16, W>& f, float* o) {
+#pragma unroll
+  for (int i = 0; i < W; ++i) o[i] = bf16_bits_to_float(f.v[i].bits);
+}
+
+// The sum over groups of ``lanes`` neighbours, in all of them
+__device__ __forceinline__ float sum_lanes(float x, int lanes) {
+  if (lanes > 1) x += dpp_mov<kDppXor1>(0.0f, x);
+  if (lanes > 2) x += dpp_mov<kDppXor2>(0.0f, x);
+  if (lanes > 4) x += dpp_mov<kDppHalfMirror>(0.0f, x);
+  if (lanes > 8) x += dpp_mov<kDppRowMirror>(0.0f, x);
+  if (lanes > 16) x += __shfl_xor(x, 16);
+  if (lanes > 32) x += __shfl_xor(x, 32);
+  return x;
+}
+
+// HB: heads at once
+template <typename IO, int W, int U, bool INTER, bool BACK, int HB>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
-  constexpr int U = kUnits<W>;
   const bool keys = static_cast<int>(blockIdx.x) >= a.side[0].blocks;
   const Side& s = a.side[keys];
   const int block = blockIdx.x - (keys ? a.side[0].blocks : 0);
   const int tid = threadIdx.x, lane = tid & (a.lanes - 1), group = tid / a.lanes, groups = 256 / a.lanes;
   const int half = a.R / 2;
-  const float nan = __uint_as_float(0x7fc00000u);
+  const float nan = __uint_as_float(0x7fc00000u), inverse = 1.0f / static_cast<float>(a.D);
 
   // where a lane's units lie, and the weights there
   int at[U][2];
@@ -91,32 +121,60 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
           }
     }
   }
-  // a unit's two halves from or to memory, in pairs: o[i] belongs to o[W + i]
-  const auto load = [&](const void* p, int64_t base, int u, float (&o)[2 * W]) {
-    float lo[W] = {}, hi[W] = {};
-    if (there[u]) load_few<IO, W>(p, base + at[u][0], lo);
-    if (second[u]) load_few<IO, W>(p, base + at[u][1], hi);
+  // a unit's two halves, in pairs: o[i] belongs to o[W + i], or (INTER: the 2 W values in
+  // a row) o[2 i] to o[2 i + 1]
+  // Nothing is read under a condition (a branch around a load makes the loads wait for
+  // one another): a lane without a unit reads the head's first values and drops them, and
+  // behind the last head the last one is read again.
+  using Bits = Few<IO, W>;
+  bool whole = true;
 #pragma unroll
-    for (int i = 0; i < W; ++i) o[i] = lo[i], o[W + i] = hi[i];
+  for (int u = 0; u < U; ++u) {
+    whole = whole && second[u];
+    if (!there[u]) at[u][0] = 0;
+    if (!second[u]) at[u][1] = 0;
+  }
+  whole = __all(whole);
+  const auto load = [&](const void* p, int64_t base, int u, Bits (&o)[2]) {
+    const IO* const q = static_cast<const IO*>(p) + base;
+    o[0] = *reinterpret_cast<const Bits*>(q + at[u][0]);
+    o[1] = *reinterpret_cast<const Bits*>(q + at[u][1]);
   };
-  // INTER: values 2 i and 2 i + 1 are a pair
+  const auto values = [&](const Bits (&o)[2], int u, float* x) {
+    widen(o[0], x);
+    widen(o[1], x + W);
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        x[i] = there[u] ? x[i] : 0.0f;
+        x[W + i] = second[u] ? x[W + i] : 0.0f;
+      }
+    }
+  };
   const auto first_of = [](int i) { return INTER ? 2 * i : i; };
   const auto second_of = [](int i) { return INTER ? 2 * i + 1 : W + i; };
 
-  for (int64_t row = static_cast<int64_t>(block) * groups + group; row < s.rows;
-       row += static_cast<int64_t>(s.blocks) * groups) {
-    const uint32_t token = static_cast<uint32_t>(row) / static_cast<uint32_t>(s.heads);
-    const uint32_t head = static_cast<uint32_t>(row) - token * s.heads;
+  for (int64_t unit = static_cast<int64_t>(block) * groups + group; unit < s.units;
+       unit += static_cast<int64_t>(s.blocks) * groups) {
+    const uint32_t token = static_cast<uint32_t>(unit) / static_cast<uint32_t>(s.chunks);
+    const int head0 = static_cast<int>(static_cast<uint32_t>(unit) - token * s.chunks) * HB;
     const uint32_t b = token / static_cast<uint32_t>(a.T), t = token - b * a.T;
-    const int64_t from = b * s.sb + t * s.st + head * s.sh, to = row * a.D;
+    const int64_t from = b * s.sb + t * s.st + head0 * s.sh;
+    const int64_t to = (static_cast<int64_t>(token) * s.heads + head0) * a.D;
     const int64_t position = a.positions ? a.positions[token] : t;
     const bool known = position >= 0 && position < a.table_rows;
-    float x[U][2 * W], g[U][2 * W], cs[U][W], sn[U][W];
-    float square = 0.0f;
+    Bits xs[HB][U][2], gs[BACK ? HB : 1][U][2];
+    float cs[U][W], sn[U][W];
+#pragma unroll
+    for (int k = 0; k < HB; ++k)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int h = head0 + k < s.heads ? k : s.heads - 1 - head0;
+        load(s.x, from + h * s.sh, u, xs[k][u]);
+        if constexpr (BACK) load(s.dy, to + h * a.D, u, gs[k][u]);
+      }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      load(s.x, from, u, x[u]);
-      if constexpr (BACK) load(s.dy, to, u, g[u]);
 #pragma unroll
       for (int i = 0; i < W; ++i) cs[u][i] = 1.0f, sn[u][i] = 0.0f;
       if (turns[u] && known) {
@@ -126,53 +184,62 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
       }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int i = 0; i < 2 * W; ++i) square = fmaf(x[u][i], x[u][i], square);
-    for (int m = 1; m < a.lanes; m *= 2) square += __shfl_xor(square, m);
-    const float rstd = known ? rsqrtf(square / static_cast<float>(a.D) + a.eps) : nan;
-    float along = 0.0f;
-    if constexpr (BACK) {
+    for (int k = 0; k < HB; ++k) {
+      float x[U][2 * W], g[U][2 * W];
+      float square = 0.0f;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
+        values(xs[k][u], u, x[u]);
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-          float &p = g[u][first_of(i)], &q = g[u][second_of(i)];
-          const float c = p * cs[u][i] + q * sn[u][i], d = q * cs[u][i] - p * sn[u][i];
-          p = c, q = d;
-        }
-#pragma unroll
-        for (int i = 0; i < 2 * W; ++i) {
-          x[u][i] *= rstd;
-          sums[u][i] = fmaf(g[u][i], x[u][i], sums[u][i]);
-          g[u][i] *= w[u][i];
-          along = fmaf(g[u][i], x[u][i], along);
-        }
+        for (int i = 0; i < 2 * W; ++i) square = fmaf(x[u][i], x[u][i], square);
       }
-      for (int m = 1; m < a.lanes; m *= 2) along += __shfl_xor(along, m);
-      along /= static_cast<float>(a.D);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float y[2 * W];
+      square = sum_lanes(square, a.lanes);
+      const float rstd = known ? rsqrtf(fmaf(square, inverse, a.eps)) : nan;
+      float along = 0.0f;
       if constexpr (BACK) {
 #pragma unroll
-        for (int i = 0; i < 2 * W; ++i) y[i] = rstd * (g[u][i] - x[u][i] * along);
-      } else {
+        for (int u = 0; u < U; ++u) {
+          values(gs[k][u], u, g[u]);
 #pragma unroll
-        for (int i = 0; i < 2 * W; ++i) y[i] = x[u][i] * rstd * w[u][i];
+          for (int i = 0; i < W; ++i) {
+            float &p = g[u][first_of(i)], &q = g[u][second_of(i)];
+            const float c = p * cs[u][i] + q * sn[u][i], d = q * cs[u][i] - p * sn[u][i];
+            p = c, q = d;
+          }
+          const bool real = head0 + k < s.heads;  // (else 0 NaN could reach the sums)
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-          float &p = y[first_of(i)], &q = y[second_of(i)];
-          const float c = p * cs[u][i] - q * sn[u][i], d = q * cs[u][i] + p * sn[u][i];
-          p = c, q = d;
+          for (int i = 0; i < 2 * W; ++i) {
+            x[u][i] *= rstd;
+            sums[u][i] = real ? fmaf(g[u][i], x[u][i], sums[u][i]) : sums[u][i];
+            g[u][i] *= w[u][i];
+            along = fmaf(g[u][i], x[u][i], along);
+          }
         }
+        along = sum_lanes(along, a.lanes) * inverse;
       }
-      float lo[W], hi[W];
+      if (head0 + k >= s.heads || !s.out) continue;
 #pragma unroll
-      for (int i = 0; i < W; ++i) lo[i] = y[i], hi[i] = y[W + i];
-      if (s.out && there[u]) store_few<IO, W>(s.out, to + at[u][0], lo);
-      if (s.out && second[u]) store_few<IO, W>(s.out, to + at[u][1], hi);
+      for (int u = 0; u < U; ++u) {
+        float y[2 * W];
+        if constexpr (BACK) {
+#pragma unroll
+          for (int i = 0; i < 2 * W; ++i) y[i] = rstd * (g[u][i] - x[u][i] * along);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2 * W; ++i) y[i] = x[u][i] * rstd * w[u][i];
+#pragma unroll
+          for (int i = 0; i < W; ++i) {
+            float &p = y[first_of(i)], &q = y[second_of(i)];
+            const float c = p * cs[u][i] - q * sn[u][i], d = q * cs[u][i] + p * sn[u][i];
+            p = c, q = d;
+          }
+        }
+        float lo[W], hi[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) lo[i] = y[i], hi[i] = y[W + i];
+        if (there[u]) store_few<IO, W>(s.out, to + k * a.D + at[u][0], lo);
+        if (second[u]) store_few<IO, W>(s.out, to + k * a.D + at[u][1], hi);
+      }
     }
   }
   if constexpr (BACK) {
@@ -203,17 +270,19 @@ struct RotarySums {
   void* out[2];
   int rows[2], D, f32;
 };
-__global__ __launch_bounds__(256) void rotary_sum_kernel(const RotarySums a) {
-  __shared__ float part[8][33];
-  const int which = blockIdx.y, c = blockIdx.x * 32 + (threadIdx.x & 31), group = threadIdx.x >> 5;
+__global__ __launch_bounds__(1024) void rotary_sum_kernel(const RotarySums a) {
+  __shared__ float part[32][33];
+  const int which = blockIdx.y, col = threadIdx.x & 31, c = blockIdx.x * 32 + col, group = threadIdx.x >> 5;
   if (!a.out[which]) return;
   float sum = 0.0f;
-  if (c < a.D)
-    for (int r = group; r < a.rows[which]; r += 8) sum += a.in[which][static_cast<int64_t>(r) * a.D + c];
-  part[group][threadIdx.x & 31] = sum;
+  if (c < a.D) {
+#pragma unroll 8
+    for (int r = group; r < a.rows[which]; r += 32) sum += a.in[which][static_cast<int64_t>(r) * a.D + c];
+  }
+  part[group][col] = sum;
   __syncthreads();
   if (group || c >= a.D) return;
-  for (int m = 1; m < 8; ++m) sum += part[m][threadIdx.x & 31];
+  for (int m = 1; m < 32; ++m) sum += part[m][col];
   if (a.f32) static_cast<float*>(a.out[which])[c] = sum;
   else static_cast<bf16*>(a.out[which])[c].bits = pack_bf16(sum);
 }
@@ -248,10 +317,15 @@ int width_of(const sparc_rotary_desc* d) {
     if (d->head_dim % (2 * w) == 0 && d->rotary_dim % (2 * w) == 0) return w;
   return 1;
 }
-template <typename IO, int W, bool BACK> void rotary_launch(const RotaryArgs& a, bool inter, hipStream_t stream) {
+template <typename IO, int W, int U, bool BACK, int HB> void rotary_pairs(const RotaryArgs& a, bool inter, hipStream_t stream) {
   const int grid = a.side[0].blocks + a.side[1].blocks;
-  if (inter) rotary_kernel<IO, W, true, BACK><<<grid, 256, 0, stream>>>(a);
-  else rotary_kernel<IO, W, false, BACK><<<grid, 256, 0, stream>>>(a);
+  if (inter) rotary_kernel<IO, W, U, true, BACK, HB><<<grid, 256, 0, stream>>>(a);
+  else rotary_kernel<IO, W, U, false, BACK, HB><<<grid, 256, 0, stream>>>(a);
+}
+template <typename IO, int W, bool BACK> void rotary_launch(const RotaryArgs& a, bool inter, hipStream_t stream) {
+  if (a.several) rotary_pairs<IO, W, 1, BACK, kHeads<BACK>>(a, inter, stream);
+  else if (a.D <= 128 * W) rotary_pairs<IO, W, 1, BACK, 1>(a, inter, stream);
+  else rotary_pairs<IO, W, kUnits<W>, BACK, 1>(a, inter, stream);
 }
 template <bool BACK> void rotary_dispatch(const sparc_rotary_desc* d, RotaryArgs& a, hipStream_t stream) {
   const int w = width_of(d);
@@ -268,22 +342,27 @@ template <bool BACK> void rotary_dispatch(const sparc_rotary_desc* d, RotaryArgs
   }
 }
 // Everything but the sides' tensors; ``most``: workgroups at most
-RotaryArgs rotary_args(const sparc_rotary_desc* d, const float* table, const int64_t* positions, int64_t most) {
+RotaryArgs rotary_args(const sparc_rotary_desc* d, const float* table, const int64_t* positions, int64_t most, bool back) {
   RotaryArgs a = {};
   const int w = width_of(d);
   const int64_t units = (d->head_dim + 2 * w - 1) / (2 * w);
   a.lanes = 1;
   while (a.lanes < 64 && a.lanes < units) a.lanes *= 2;
   const int64_t tokens = d->batch * d->length, groups = 256 / a.lanes;
-  const int64_t heads[2] = {d->q_heads, d->k_heads}, all = tokens * (d->q_heads + d->k_heads);
+  const int64_t heads[2] = {d->q_heads, d->k_heads};
+  // several heads at once where a lane group for each head would be many more than the GPU holds
+  a.several = tokens * (d->q_heads + d->k_heads) * a.lanes >= (1 << 20) && units <= 64;
+  const int64_t hb = a.several ? (back ? kHeads<true> : kHeads<false>) : 1, chunks[2] = {(heads[0] + hb - 1) / hb, (heads[1] + hb - 1) / hb};
+  const int64_t all = tokens * (chunks[0] + chunks[1]);
   for (int i = 0; i < 2; ++i) {
     Side& s = a.side[i];
     const int64_t* stride = i ? d->k_stride : d->q_stride;
     s.sb = stride[0], s.st = stride[1], s.sh = stride[2];
     s.heads = static_cast<int>(heads[i]);
-    s.rows = tokens * heads[i];
-    int64_t blocks = (s.rows + groups - 1) / groups;
-    const int64_t share = all ? (most * s.rows + all - 1) / all : 0;
+    s.chunks = static_cast<int>(chunks[i]);
+    s.units = tokens * chunks[i];
+    int64_t blocks = (s.units + groups - 1) / groups;
+    const int64_t share = all ? (most * s.units + all - 1) / all : 0;
     if (blocks > share) blocks = share;
     s.blocks = static_cast<int>(blocks);
   }
@@ -312,7 +391,7 @@ sparc_status sparc_qk_norm_rotary_forward(const sparc_rotary_desc* d, const void
   if (d->batch == 0 || d->length == 0) return SPARC_OK;
   if (!q || !yq || (d->k_heads > 0 && (!k || !yk)) || (d->rotary_dim > 0 && d->table_rows > 0 && !table))
     return op_fail(SPARC_EINVAL, "qk_norm_rotary: a tensor is NULL");
-  RotaryArgs a = rotary_args(d, table, positions, 1 << 16);
+  RotaryArgs a = rotary_args(d, table, positions, 1 << 16, false);
   a.side[0].x = q, a.side[0].w = q_weight, a.side[0].out = yq;
   a.side[1].x = k, a.side[1].w = k_weight, a.side[1].out = yk;
   rotary_dispatch<false>(d, a, reinterpret_cast<hipStream_t>(stream));
@@ -337,7 +416,7 @@ sparc_status sparc_qk_norm_rotary_backward(const sparc_rotary_desc* d, const voi
   const bool sums = dq_weight || dk_weight;
   if (sums && (!workspace || workspace_bytes < sparc_qk_norm_rotary_workspace_bytes(d)))
     return op_fail(SPARC_EWORKSPACE, "qk_norm_rotary: workspace missing or too small");
-  RotaryArgs a = rotary_args(d, table, positions, kBackBlocks);
+  RotaryArgs a = rotary_args(d, table, positions, kBackBlocks, true);
   float* const partial = static_cast<float*>(workspace);
   a.side[0].x = q, a.side[0].w = q_weight, a.side[0].dy = dyq, a.side[0].out = dq;
   a.side[1].x = k, a.side[1].w = k_weight, a.side[1].dy = dyk, a.side[1].out = dk;
@@ -350,7 +429,7 @@ sparc_status sparc_qk_norm_rotary_backward(const sparc_rotary_desc* d, const voi
                           {a.side[0].blocks, a.side[1].blocks},
                           a.D,
                           a.params_f32};
-    rotary_sum_kernel<<<dim3((a.D + 31) / 32, 2), 256, 0, stream>>>(r);
+    rotary_sum_kernel<<<dim3((a.D + 31) / 32, 2), 1024, 0, stream>>>(r);
   }
   return op_launched("sparc_qk_norm_rotary_backward");
 }

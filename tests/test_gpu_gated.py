@@ -60,7 +60,8 @@ def _run(x, wg, wu, dy, act, shape=None):
 
 
 SHAPES = [(1, 1, 1), (1, 8, 8), (3, 5, 7), (16, 32, 64), (17, 33, 65), (128, 64, 64), (129, 96, 200), (5, 1000, 3),
-          (1, 256, 513), (300, 40, 31), (64, 512, 256), (256, 128, 128), (700, 136, 72), (2000, 24, 40)]
+          (1, 256, 513), (300, 40, 31), (64, 512, 256), (256, 128, 128), (700, 136, 72), (2000, 24, 40),
+          (6000, 520, 1032)]  # the last one in large tiles, all products split
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], **IDS)
