@@ -72,17 +72,6 @@ template <int W> __device__ __forceinline__ void widen(const Few<bf16, W>& f, fl
   for (int i = 0; i < W; ++i) o[i] = bf16_bits_to_float(f.v[i].bits);
 }
 
-// The sum over groups of ``lanes`` neighbours, in all of them
-__device__ __forceinline__ float sum_lanes(float x, int lanes) {
-  if (lanes > 1) x += dpp_mov<kDppXor1>(0.0f, x);
-  if (lanes > 2) x += dpp_mov<kDppXor2>(0.0f, x);
-  if (lanes > 4) x += dpp_mov<kDppHalfMirror>(0.0f, x);
-  if (lanes > 8) x += dpp_mov<kDppRowMirror>(0.0f, x);
-  if (lanes > 16) x += __shfl_xor(x, 16);
-  if (lanes > 32) x += __shfl_xor(x, 32);
-  return x;
-}
-
 // HB: heads at once
 template <typename IO, int W, int U, bool INTER, bool BACK, int HB>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
@@ -193,7 +182,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
 #pragma unroll
         for (int i = 0; i < 2 * W; ++i) square = fmaf(x[u][i], x[u][i], square);
       }
-      square = sum_lanes(square, a.lanes);
+      square = group_sum(square, a.lanes);
       const float rstd = known ? rsqrtf(fmaf(square, inverse, a.eps)) : nan;
       float along = 0.0f;
       if constexpr (BACK) {
@@ -215,7 +204,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
             along = fmaf(g[u][i], x[u][i], along);
           }
         }
-        along = sum_lanes(along, a.lanes) * inverse;
+        along = group_sum(along, a.lanes) * inverse;
       }
       if (head0 + k >= s.heads || !s.out) continue;
 #pragma unroll

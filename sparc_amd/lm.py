@@ -28,10 +28,11 @@ from .stack import SPARCStack
 class SPARCLanguageModel(nn.Module):
     """Logits [B, T, vocab] of ids [B, T].  The embedding is scaled by
     sqrt(d_model) and its table is the output projection too; ``padding_idx``
-    takes no gradient from the lookup (negative counts from the end)."""
+    takes no gradient from the lookup (negative counts from the end).  ``stack``:
+    further options of ``SPARCStack`` (``mixer``, ``heads``, ``feed_forward``, ...)."""
 
     def __init__(self, vocab: int, n_layers: int, d_model: int, n_states: int, padding_idx: int | None = None,
-                 norm: str = "layer"):
+                 norm: str = "layer", **stack):
         super().__init__()
         if padding_idx is not None:
             if not -vocab <= padding_idx < vocab:
@@ -40,7 +41,7 @@ class SPARCLanguageModel(nn.Module):
         self.weight = nn.Parameter(torch.randn(vocab, d_model) * d_model ** -0.5)
         self.scale = math.sqrt(d_model)
         self.padding_idx = padding_idx
-        self.stack = SPARCStack(n_layers, d_model, n_states, norm=norm)
+        self.stack = SPARCStack(n_layers, d_model, n_states, norm=norm, **stack)
 
     def embed(self, tokens: torch.Tensor) -> torch.Tensor:
         return embedding(tokens, self.weight, scale=self.scale, padding_idx=self.padding_idx)
@@ -108,11 +109,15 @@ def main(argv=None) -> None:
     ap.add_argument("--layers", type=int, default=2)
     ap.add_argument("--d-model", type=int, default=64)
     ap.add_argument("--states", type=int, default=8)
+    ap.add_argument("--mixer", choices=("sparc", "linear"), default="sparc")
+    ap.add_argument("--heads", type=int, default=4, help="of linear attention")
+    ap.add_argument("--feed-forward", type=int, default=0, help="values of a gated feed-forward half (0: none)")
     ap.add_argument("--steps", type=int, default=200)
     ap.add_argument("--beams", type=int, default=4)
     a = ap.parse_args(argv)
     torch.manual_seed(0)
-    model = SPARCLanguageModel(a.vocab, a.layers, a.d_model, a.states).cuda()
+    model = SPARCLanguageModel(a.vocab, a.layers, a.d_model, a.states, mixer=a.mixer, heads=a.heads,
+                               feed_forward=a.feed_forward).cuda()
     optimizer = torch.optim.AdamW(model.parameters(), lr=3e-3)
     for i in range(a.steps):
         start, by = torch.randint(0, a.vocab, (32, 1)), torch.randint(1, 4, (32, 1))

@@ -6,7 +6,10 @@ Each block is pre-norm and residual:
 
 with ``in_proj`` d_model -> 2M and ``out_proj`` 2M -> d_model (M = d_model *
 N complex modes, so the mixer's width is 2M), and a final RMSNorm; with
-``norm="layer"`` every norm is a layer norm with a bias instead.  ``prefill``
+``norm="layer"`` every norm is a layer norm with a bias instead.  With
+``mixer="linear"`` the blocks mix tokens by linear attention with a decay for each
+head instead (``LinearAttentionBlock``), and ``feed_forward=F`` puts a gated
+feed-forward half of F values behind either mixer.  ``prefill``
 and ``step`` run a prompt and then one token at a time, carrying the mixers'
 states.  The
 projections are plain GEMMs (torch -> hipBLASLt on MI355X); the mixer is the
@@ -25,7 +28,9 @@ from torch import nn
 
 from . import _lib
 from . import mixer as _mixer
+from .attention import linear_attention, linear_attention_step, qk_norm_rotary, rotary_table
 from .control import aligned16
+from .feed_forward import gated_linear_unit
 from .norm import layer_norm
 from .sparc import SPARCMixer
 
@@ -118,8 +123,107 @@ def apply_norm(norm: nn.Module, x: torch.Tensor) -> torch.Tensor:
     return rms_norm(norm, x)
 
 
-class SPARCBlock(nn.Module):
-    def __init__(self, d_model: int, n_states: int, eps: float = 1e-6, norm: str = "rms"):
+class GatedFeedForward(nn.Module):
+    """down(act(gate(x)) * up(x)): ``gated_linear_unit`` and the projection back."""
+
+    def __init__(self, d_model: int, hidden: int, activation: str = "silu"):
+        super().__init__()
+        self.gate = nn.Linear(d_model, hidden, bias=False)
+        self.up = nn.Linear(d_model, hidden, bias=False)
+        self.down = nn.Linear(hidden, d_model, bias=False)
+        self.activation = activation
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return self.down(gated_linear_unit(x, self.gate.weight, self.up.weight, self.activation))
+
+
+class _Block(nn.Module):
+    """What blocks of either mixer share: the feed-forward half behind it."""
+
+    def _make_feed_forward(self, d_model: int, hidden: int, norm: str, eps: float) -> None:
+        if hidden:
+            self.ff_norm = _make_norm(norm, d_model, eps)
+            self.ff = GatedFeedForward(d_model, hidden)
+
+    def _feed_forward(self, x: torch.Tensor) -> torch.Tensor:
+        return x + self.ff(apply_norm(self.ff_norm, x)) if hasattr(self, "ff") else x
+
+    def prepare_inference(self) -> None:
+        """What a decode step needs once."""
+
+
+class LinearAttentionBlock(_Block):
+    """A pre-norm residual block of linear attention: queries, keys and values of one
+    projection, the norms of queries and keys with the rotation by their positions
+    (``qk_norm_rotary``), ``linear_attention`` with a decay for each head from 32 steps
+    of memory to 4096, a norm of each head's output, and the projection back.  The
+    state of a row is (S [heads, D, D] fp32, position); positions reach
+    ``max_length``."""
+
+    def __init__(self, d_model: int, heads: int, kv_heads: int | None = None, eps: float = 1e-6, norm: str = "rms",
+                 feed_forward: int = 0, max_length: int = 65536):
+        super().__init__()
+        kv_heads = heads if kv_heads is None else kv_heads
+        if heads < 1 or kv_heads < 1 or d_model % heads or heads % kv_heads or d_model // heads % 2:
+            raise ValueError(f"d_model {d_model} must be an even multiple of the {heads} heads, and these a multiple of "
+                             f"the {kv_heads} key heads")
+        self.heads, self.kv_heads, self.head_dim, self.eps = heads, kv_heads, d_model // heads, eps
+        self.norm = _make_norm(norm, d_model, eps)
+        self.qkv = nn.Linear(d_model, (heads + 2 * kv_heads) * self.head_dim, bias=False)
+        self.q_weight = nn.Parameter(torch.ones(self.head_dim))
+        self.k_weight = nn.Parameter(torch.ones(self.head_dim))
+        self.head_norm = nn.RMSNorm(self.head_dim, eps=eps)
+        self.out_proj = nn.Linear(d_model, d_model, bias=False)
+        decay = torch.log1p(-torch.exp2(-5.0 - 7.0 * torch.arange(heads) / max(1, heads - 1)))
+        self.register_buffer("log_decay", decay, persistent=False)
+        self.register_buffer("table", rotary_table(max_length, self.head_dim), persistent=False)
+        self._make_feed_forward(d_model, feed_forward, norm, eps)
+
+    def _apply(self, fn, recurse=True):
+        # the operators take both in fp32, whatever the parameters are converted to
+        decay, table = self.log_decay, self.table
+        super()._apply(fn, recurse)
+        if self.log_decay.dtype != torch.float32:
+            self.log_decay, self.table = (t.to(self.log_decay.device) for t in (decay, table))
+        return self
+
+    def _heads(self, x: torch.Tensor):
+        """(q, k, v) [B, T, heads, D] of the block's input, before norms and rotation."""
+        both = self.qkv(apply_norm(self.norm, x))
+        sizes = [self.heads, self.kv_heads, self.kv_heads]
+        return [p.unflatten(-1, (-1, self.head_dim)) for p in both.split([n * self.head_dim for n in sizes], dim=-1)]
+
+    def _out(self, x: torch.Tensor, o: torch.Tensor) -> torch.Tensor:
+        return self._feed_forward(x + self.out_proj(rms_norm(self.head_norm, o).flatten(-2)))
+
+    def _attend(self, x: torch.Tensor):
+        if x.shape[1] > self.table.shape[0]:
+            raise ValueError(f"{x.shape[1]} positions are more than max_length {self.table.shape[0]}")
+        q, k, v = self._heads(x)
+        q, k = qk_norm_rotary(q, k, self.q_weight, self.k_weight, self.table, eps=self.eps)
+        o, state = linear_attention(q, k, v, self.log_decay)
+        return self._out(x, o), state
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return self._attend(x)[0]
+
+    def prefill(self, x: torch.Tensor):
+        """(output, state) of a sequence [B, T, d_model]."""
+        y, state = self._attend(x)
+        return y, (state, torch.full((x.shape[0],), x.shape[1], dtype=torch.int64, device=x.device))
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, state):
+        """(output, new state) of one position [B, d_model]; no gradient."""
+        s, position = state
+        q, k, v = self._heads(x[:, None])
+        q, k = qk_norm_rotary(q, k, self.q_weight, self.k_weight, self.table, position[:, None], eps=self.eps)
+        o, s = linear_attention_step(q[:, 0], k[:, 0], v[:, 0], self.log_decay, s)
+        return self._out(x, o), (s, position + 1)
+
+
+class SPARCBlock(_Block):
+    def __init__(self, d_model: int, n_states: int, eps: float = 1e-6, norm: str = "rms", feed_forward: int = 0):
         super().__init__()
         modes = d_model * n_states
         self.norm = _make_norm(norm, d_model, eps)
@@ -128,6 +232,7 @@ class SPARCBlock(nn.Module):
         self.out_proj = nn.Linear(2 * modes, d_model, bias=False)
         with torch.no_grad():  # keep the residual stream's scale at init
             self.out_proj.weight.mul_(1.0 / (2 * modes) ** 0.5)
+        self._make_feed_forward(d_model, feed_forward, norm, eps)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         xn = apply_norm(self.norm, x)
@@ -136,28 +241,45 @@ class SPARCBlock(nn.Module):
             y, _ = _mixer.projected_sequence(self.mixer, xn, self.in_proj.weight)
         else:
             y, _ = self.mixer(self.in_proj(xn))
-        return x + self.out_proj(y)
+        return self._feed_forward(x + self.out_proj(y))
 
     def prefill(self, x: torch.Tensor):
         """(output, state) of a sequence [B, T, d_model]: the state is the
         mixer's (re, im) after the last position, fp32 [B, M]."""
         y, state = self.mixer(self.in_proj(apply_norm(self.norm, x)), return_cache=True)
-        return x + self.out_proj(y), state
+        return self._feed_forward(x + self.out_proj(y)), state
 
     @torch.no_grad()
     def step(self, x: torch.Tensor, state):
         """(output, new state) of one position [B, d_model]; no gradient, like the
         mixer's step."""
         y, state = self.mixer.step(self.in_proj(apply_norm(self.norm, x)), state, None)
-        return x + self.out_proj(y), state
+        return self._feed_forward(x + self.out_proj(y)), state
+
+    def prepare_inference(self) -> None:
+        """The mixer's fused decode step."""
+        self.mixer.prepare_inference()
 
 
 class SPARCStack(nn.Module):
-    """``n_layers`` SPARC blocks on a [B, T, d_model] stream."""
+    """``n_layers`` blocks on a [B, T, d_model] stream: SPARC blocks, or with
+    ``mixer="linear"`` ``LinearAttentionBlock`` of ``heads`` (and ``kv_heads``) heads,
+    which have no use for ``n_states``; each with a gated feed-forward half of
+    ``feed_forward`` values where that is not 0."""
 
-    def __init__(self, n_layers: int, d_model: int, n_states: int, eps: float = 1e-6, norm: str = "rms"):
+    def __init__(self, n_layers: int, d_model: int, n_states: int, eps: float = 1e-6, norm: str = "rms",
+                 mixer: str = "sparc", heads: int | None = None, kv_heads: int | None = None, feed_forward: int = 0,
+                 max_length: int = 65536):
         super().__init__()
-        self.blocks = nn.ModuleList(SPARCBlock(d_model, n_states, eps, norm) for _ in range(n_layers))
+        if mixer == "sparc":
+            make = lambda: SPARCBlock(d_model, n_states, eps, norm, feed_forward)
+        elif mixer == "linear":
+            if heads is None:
+                raise ValueError("linear attention needs heads")
+            make = lambda: LinearAttentionBlock(d_model, heads, kv_heads, eps, norm, feed_forward, max_length)
+        else:
+            raise ValueError(f"unknown mixer {mixer!r} (sparc or linear)")
+        self.blocks = nn.ModuleList(make() for _ in range(n_layers))
         self.norm = _make_norm(norm, d_model, eps)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
@@ -186,7 +308,7 @@ class SPARCStack(nn.Module):
     def prepare_inference(self) -> None:
         """The mixers' fused decode steps (``SPARCMixer.prepare_inference``)."""
         for blk in self.blocks:
-            blk.mixer.prepare_inference()
+            blk.prepare_inference()
 
 
 GEMM_TUNING_FILE = os.path.join(os.path.dirname(__file__), "tuning", "gemm_stack_gfx950.csv")
@@ -218,5 +340,5 @@ def rms_norm_reference(x: torch.Tensor, weight: torch.Tensor, eps: float) -> tor
     return F.rms_norm(x, (x.shape[-1],), weight, eps)
 
 
-__all__ = ["SPARCBlock", "SPARCStack", "apply_norm", "rms_norm", "rms_norm_reference", "use_tuned_gemms", "use_default_gemms",
+__all__ = ["SPARCBlock", "LinearAttentionBlock", "GatedFeedForward", "SPARCStack", "apply_norm", "rms_norm", "rms_norm_reference", "use_tuned_gemms", "use_default_gemms",
            "GEMM_TUNING_FILE"]

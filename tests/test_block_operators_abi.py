@@ -53,14 +53,16 @@ def test_rotary_entry_points_check_pointers():
 
 def _linear(**kw):
     d = dict(batch=2, length=3, heads=4, kv_heads=2, key_dim=16, value_dim=8, io_dtype=0, scale=1.0)
-    return ctypes.byref(_lib.LinearDesc(**{**d, **kw}))
+    far = (ctypes.c_int64 * 3)(1 << 20, 1 << 12, 256)
+    return ctypes.byref(_lib.LinearDesc(**{**d, "q_stride": far, "k_stride": far, "v_stride": far, **kw}))
 
 
 @pytest.mark.parametrize("kw,msg", [
     (dict(batch=-1), b"negative"), (dict(length=-1), b"negative"), (dict(heads=0), b"multiple"),
     (dict(kv_heads=3), b"multiple"), (dict(kv_heads=0), b"multiple"), (dict(key_dim=0), b"1 to 256"),
     (dict(value_dim=257), b"1 to 256"), (dict(io_dtype=4), b"io_dtype"), (dict(batch=1 << 23), b"too large"),
-    (dict(length=1 << 33), b"too large"),
+    (dict(length=1 << 33), b"too large"), (dict(q_stride=(ctypes.c_int64 * 3)(0, 15, 1)), b"time strides"),
+    (dict(v_stride=(ctypes.c_int64 * 3)(0, 1 << 23, 1)), b"time strides"),
 ])
 def test_linear_attention_entry_points_validate(kw, msg):
     lib = _lib.load()
@@ -171,3 +173,13 @@ def test_gated_linear_unit_refuses():
     _raises(TypeError, "float32 or bfloat16", call, x.half(), w.half(), w.half())
     _raises(ValueError, "alike", call, x, w.bfloat16(), w)
     _raises(RuntimeError, "GPU tensors", call, x, w, w)
+
+
+def test_stack_refuses():
+    from sparc_amd.stack import LinearAttentionBlock, SPARCStack
+    _raises(ValueError, "unknown mixer", SPARCStack, 1, 32, 2, mixer="other")
+    _raises(ValueError, "needs heads", SPARCStack, 1, 32, 2, mixer="linear")
+    _raises(ValueError, "multiple", LinearAttentionBlock, 30, heads=4)
+    _raises(ValueError, "multiple", LinearAttentionBlock, 32, heads=4, kv_heads=3)
+    _raises(ValueError, "even multiple", LinearAttentionBlock, 12, heads=4)
+    assert len(SPARCStack(2, 32, 2, mixer="linear", heads=2, feed_forward=16, max_length=4).blocks) == 2

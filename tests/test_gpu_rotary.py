@@ -81,6 +81,7 @@ SHAPES = [  # B, T, H, G, D, R
     (1, 1, 1, 1, 1, 0), (2, 3, 2, 1, 2, 2), (2, 5, 3, 2, 7, 4), (1, 40, 4, 4, 64, 64), (2, 9, 6, 1, 128, 128),
     (3, 17, 5, 2, 90, 42), (1, 6, 2, 2, 256, 64), (2, 3, 1, 1, 512, 512), (1, 7, 2, 1, 511, 510), (2, 4, 12, 3, 80, 32),
     (1, 11, 3, 3, 36, 20), (1, 300, 2, 2, 40, 40),
+    (2, 10000, 5, 2, 20, 12),  # enough for several heads at once, with heads left over
 ]
 
 
