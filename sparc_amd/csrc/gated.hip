@@ -64,11 +64,6 @@ enum Kind : int { GATED = 0, GATED_BACK = 1, PARTS = 2, PAIR = 3 };
 // An offset that no buffer reaches: loads there give zero.
 constexpr uint32_t kNowhere = 0x80000000u;
 
-// Bytes 2 and 3 of b and a: their upper halves, truncated to bf16, a's below
-__device__ __forceinline__ uint32_t upper_halves(uint32_t a, uint32_t b) {
-  return __builtin_amdgcn_perm(b, a, 0x07060302u);
-}
-
 // LINES x COLS values of an operand on their way from memory to LDS, through a buffer
 // that ends with the last line, so that no load is under a condition: what lies behind
 // the last line or column is zero.  A vector that the columns' end would cut is read so

@@ -75,9 +75,9 @@ __device__ __forceinline__ uint32_t anew(uint32_t x) {
 }
 
 // Values of each operand that a bf16 product takes: the state and the scores as two
-// bf16 values (2^-17 of their size); what is added to the state as three (2^-25) where
-// the state is a result (EXACT), and as two where it only passes through to results in
-// bf16.
+// bf16 values (all but 2^-15 of each); what is added to the state as three (all 24 bits)
+// where the state is a result (EXACT), and as two where it only passes through to
+// results in bf16.
 template <typename IO> constexpr int kStateParts = sizeof(IO) == 2 ? 2 : 1;
 template <typename IO> constexpr int kScoreParts = sizeof(IO) == 2 ? 2 : 1;
 

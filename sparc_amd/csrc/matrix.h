@@ -97,21 +97,26 @@ template <typename L, typename IO> __device__ __forceinline__ Frag<IO> read_tile
   return gather_columns<L>(lds, row0, [&](int m) { return tile_row<IO>(i, m & ~3, m & 3); });
 }
 
-// fp32 values as a sum of N fragments: N bf16 values hold 8 N bits of each (a value
-// that is not finite becomes NaN for N > 1)
+// Bytes 2 and 3 of a and b, a's below: both truncated to bf16
+__device__ __forceinline__ uint32_t upper_halves(uint32_t a, uint32_t b) {
+  return __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+// fp32 values as a sum of N fragments.  Each part is what is left of the value, truncated
+// to bf16: 8 bits of it, so that two parts hold 16 bits and three all 24.  (A value that
+// is infinite becomes NaN for N > 1.)
 template <int N> __device__ __forceinline__ void split(const float (&x)[8], Frag<bf16> (&f)[N]) {
-  float r[8];
+  uint32_t r[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = x[i];
+  for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(x[i]);
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     uint32_t u[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      u[i] = pack_bf16x2(r[2 * i], r[2 * i + 1]);
+      u[i] = upper_halves(r[2 * i], r[2 * i + 1]);
       if (n + 1 < N) {
-        r[2 * i] -= __uint_as_float(u[i] << 16);
-        r[2 * i + 1] -= __uint_as_float(u[i] & 0xffff0000u);
+        r[2 * i] = __float_as_uint(__uint_as_float(r[2 * i]) - __uint_as_float(r[2 * i] & 0xffff0000u));
+        r[2 * i + 1] = __float_as_uint(__uint_as_float(r[2 * i + 1]) - __uint_as_float(r[2 * i + 1] & 0xffff0000u));
       }
     }
     __builtin_memcpy(&f[n], u, sizeof(u));

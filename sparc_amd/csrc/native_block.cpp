@@ -17,8 +17,11 @@ Tensor steps_of(const Tensor& t) {
   const bool fits = t.size(1) <= 1 || (t.stride(1) >= t.size(3) && t.stride(1) < (1 << 23));
   return fits ? rows_of(t) : t.clone(at::MemoryFormat::Contiguous);
 }
-void strides_of(const Tensor& t, int64_t (&stride)[3]) {  // [B, T, H, D]
-  for (int i = 0; i < 3; ++i) stride[i] = t.stride(i);
+void strides_of(const Tensor& t, int64_t (&stride)[3]) {  // [B, T, H, D], or one step's [B, H, D]
+  const bool one = t.dim() == 3;
+  stride[0] = t.stride(0);
+  stride[1] = one ? 0 : t.stride(1);
+  stride[2] = t.stride(one ? 1 : 2);
 }
 bool wants(const Tensor& t) { return t.requires_grad(); }
 bool wants(const optional<Tensor>& t) { return t && t->requires_grad(); }
@@ -142,8 +145,8 @@ LinearCall linear_call(const Tensor& q, const Tensor& k, const Tensor& v, const 
                        const Tensor& lengths, double scale) {
   LinearCall c{q, k, v, decay, state, lengths, {}};
   sparc_linear_desc& d = c.desc;
-  d.batch = q.size(0), d.length = q.size(1), d.heads = q.size(2), d.key_dim = q.size(3);
-  d.kv_heads = k.size(2), d.value_dim = v.size(3);
+  d.batch = q.size(0), d.length = q.dim() == 3 ? 1 : q.size(1), d.heads = q.size(-2), d.key_dim = q.size(-1);
+  d.kv_heads = k.size(-2), d.value_dim = v.size(-1);
   d.io_dtype = code_of(q.scalar_type());
   d.scale = static_cast<float>(scale);
   strides_of(q, d.q_stride);
@@ -262,7 +265,7 @@ optional<std::tuple<Tensor, Tensor>> linear_attention_step(const Tensor& q_in, c
   refuse_gradients(what, {&q_in, &k_in, &v_in, &decay_in, &state_in, pointer(out)});
   const at::NoGradGuard no_grad;
   const c10::DeviceGuard guard(q_in.device());
-  const Tensor q = rows_of(q_in).unsqueeze(1), k = rows_of(k_in).unsqueeze(1), v = rows_of(v_in).unsqueeze(1);
+  const Tensor q = rows_of(q_in), k = rows_of(k_in), v = rows_of(v_in);
   const Tensor decay = contiguous(decay_in), state = contiguous(state_in);
   if (out) {
     const bool same = out->data_ptr() == state_in.data_ptr() && state_in.is_contiguous();
@@ -274,7 +277,7 @@ optional<std::tuple<Tensor, Tensor>> linear_attention_step(const Tensor& q_in, c
   Tensor after = out ? *out : at::empty(state.sizes(), state.options());
   const double scale = scale_in ? *scale_in : 1.0 / std::sqrt(static_cast<double>(q.size(-1)));
   const LinearCall c = linear_call(q, k, v, decay, state, Tensor(), scale);
-  Tensor o = at::empty({q.size(0), q.size(2), v.size(3)}, q.options());
+  Tensor o = at::empty({q.size(0), q.size(1), v.size(2)}, q.options());
   check(sparc_linear_attention_step(&c.desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), floats(decay), floats(state),
                                     o.data_ptr(), after.data_ptr<float>(), stream_of(q)),
         "sparc_linear_attention_step");

@@ -5,8 +5,8 @@ Tolerances.  All results are sums of products with factors that are not negative
 sum of the terms' sizes.  A chain of n roundings of fp32 is off by n 2^-24 A at most;
 here n counts a dot product over the head (K or V), the steps that a value passes
 (T), and 64 for the powers and the rest.  With bfloat16 inputs the state, the scores
-and decayed values enter products as two or three bfloat16 values, good to 2^-16 of
-each: another 2^-14 A.  A result in bfloat16 is rounded once: 2^-8 of its value."""
+and decayed values enter products as two or three bfloat16 values, truncated to 2^-15
+of each or better, two of them for a term at most: another 2^-14 A.  A result in bfloat16 is rounded once: 2^-8 of its value."""
 import pytest
 import torch
 
