@@ -148,11 +148,13 @@ template <typename IO, int LINES, int COLS, int THREADS, bool ACROSS, bool WHOLE
 };
 
 // TP x TQ results by WP x WQ waves; BK values of the contraction at a time, in BUFFERS
-// places in LDS.
-template <typename IO, int KIND, bool PA, bool QA, int TP, int TQ, int WP, int WQ, int BK, int BUFFERS, bool WHOLE>
-__global__ __launch_bounds__(64 * WP * WQ, 2) void product_kernel(const ProductArgs a) {
+// places in LDS.  KS: groups of so many waves that share the BK values and are added up
+// at the end, where tiles are small and one group would leave a SIMD one wave (256 rows
+// of 2048 on 8192: 39.1 -> 33.6 us).
+template <typename IO, int KIND, bool PA, bool QA, int TP, int TQ, int WP, int WQ, int KS, int BK, int BUFFERS, bool WHOLE>
+__global__ __launch_bounds__(64 * WP * WQ * KS, 2) void product_kernel(const ProductArgs a) {
   constexpr bool DUAL = KIND == GATED || KIND == GATED_BACK;
-  constexpr int THREADS = 64 * WP * WQ, VEC = kVec<IO>, SIZE = sizeof(IO);
+  constexpr int THREADS = 64 * WP * WQ * KS, VEC = kVec<IO>, SIZE = sizeof(IO);
   constexpr int LP = TP / WP, LQ = TQ / WQ, MP = LP / 16, MQ = LQ / 16;  // a wave's results, and in tiles
   constexpr int PT = DUAL ? TP / 2 : TP;
   using FP = Feed<IO, PA ? BK : TP, PA ? TP : BK, THREADS, PA, WHOLE>;
@@ -161,7 +163,8 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void product_kernel(const ProductA
   __shared__ __attribute__((aligned(16))) bf16 lds[BUFFERS * (SP + SQ)];
 
   const int lane = threadIdx.x & 63, col = lane & 15, quad = 4 * (lane >> 4);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % (WP * WQ);
+  const int share = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / (WP * WQ);  // of the BK values
   const int wp = wave % WP * LP, wq = wave / WP * LQ;
   // neighbouring workgroups of an XCD: eight tiles of q beside all of p
   const int sides = KIND == PAIR ? 2 : 1;
@@ -294,18 +297,23 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void product_kernel(const ProductA
     fetch_q(at.k, at.part);
     for (int step = 0; step < count; ++step) {
       const int place = step & 1;
+      const auto next = [&]() __attribute__((always_inline)) {
+        put_at.next(a.nk);
+        at.next(a.nk);
+        put_p(1 - place, put_at.k);
+        put_q(1 - place, put_at.k);
+        fetch_p(at.k, at.part);
+        fetch_q(at.k, at.part);
+      };
       __syncthreads();  // this step's place is filled, and the other one no longer read
 #pragma unroll
-      for (int c = 0; c < BK; c += 32) {
-        if (c == BK / 64 * 32) {
-          put_at.next(a.nk);
-          at.next(a.nk);
-          put_p(1 - place, put_at.k);
-          put_q(1 - place, put_at.k);
-          fetch_p(at.k, at.part);
-          fetch_q(at.k, at.part);
-        }
-        read(place, c);
+      for (int c = 0; c < BK; c += 32 * KS) {
+        // the other place is filled in the middle of a step: before it the rows would be
+        // waited for at once, and no matrix instruction would run meanwhile
+        const bool fill = c == (KS == 1 ? BK / 64 * 32 : 0);
+        if (fill && KS == 1) next();
+        read(place, c + 32 * share);
+        if (fill && KS > 1) next();
         multiply();
       }
     }
@@ -322,11 +330,28 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void product_kernel(const ProductA
       fetch_p(at.k, at.part);
       fetch_q(at.k, at.part);
 #pragma unroll
-      for (int c = 0; c < BK; c += 32) {
-        read(0, c);
+      for (int c = 0; c < BK; c += 32 * KS) {
+        read(0, c + 32 * share);
         multiply();
       }
     }
+  }
+  if constexpr (KS > 1) {
+    static_assert(KS == 2 && sizeof(lds) >= sizeof(float) * TP * TQ, "the second group's results pass through LDS");
+    f32x4* const sums = reinterpret_cast<f32x4*>(lds) + wave * MP * MQ * 64 + lane;
+    __syncthreads();
+    if (share == 1) {
+#pragma unroll
+      for (int i = 0; i < MP; ++i)
+#pragma unroll
+        for (int j = 0; j < MQ; ++j) sums[(i * MQ + j) * 64] = acc[i][j];
+    }
+    __syncthreads();
+    if (share == 1) return;
+#pragma unroll
+    for (int i = 0; i < MP; ++i)
+#pragma unroll
+      for (int j = 0; j < MQ; ++j) acc[i][j] += sums[(i * MQ + j) * 64];
   }
   // all of dy first: a wait for a load behind a store waits for the store too
   f32x4 dys[KIND == GATED_BACK ? MP / 2 : 1][KIND == GATED_BACK ? MQ : 1];
@@ -452,24 +477,35 @@ GatedPlan gated_plan(int64_t rows, int64_t dim, int64_t hidden, int32_t io) {
   return p;
 }
 
-template <typename IO, int KIND, bool PA, bool QA, int TP, int TQ, int WP, int WQ, int BK, int BUFFERS, bool WHOLE>
+template <typename IO, int KIND, bool PA, bool QA, int TP, int TQ, int WP, int WQ, int KS, int BK, int BUFFERS, bool WHOLE>
 void product_tiled(ProductArgs& a, int splits, hipStream_t stream) {
   constexpr bool DUAL = KIND == GATED || KIND == GATED_BACK;
   a.p_tiles = static_cast<int>(tiles(a.P.rows, DUAL ? TP / 2 : TP));
   a.q_tiles = static_cast<int>(tiles(a.Q.rows, TQ));
   const int64_t count = static_cast<int64_t>(a.p_tiles) * a.q_tiles * (KIND == PAIR ? 2 : 1) * splits;
-  product_kernel<IO, KIND, PA, QA, TP, TQ, WP, WQ, BK, BUFFERS, WHOLE><<<static_cast<unsigned>(count), 64 * WP * WQ, 0, stream>>>(a);
+  product_kernel<IO, KIND, PA, QA, TP, TQ, WP, WQ, KS, BK, BUFFERS, WHOLE><<<static_cast<unsigned>(count), 64 * WP * WQ * KS, 0, stream>>>(a);
 }
 template <typename IO, int KIND, bool PA, bool QA>
 void product(ProductArgs& a, const Cut& cut, bool whole, hipStream_t stream) {
   a.split_steps = cut.split_steps;
+  constexpr bool DUAL = KIND == GATED || KIND == GATED_BACK;
+  if constexpr (DUAL && sizeof(IO) == 2) {
+    // A few rows, for which the weights' way is all the time: tiles so small that most
+    // CUs have one, all of them under way at once, each step of a whole 256 bytes of a
+    // row (weights of 8192 x 2048 for 1 row 28.0 -> 16.6 us, for 64 30.7 -> 17.7, for
+    // 128 31.5 -> 25.8; for 256, where they no longer are, 33.9 instead of 44.5).
+    if (whole && tiles(a.P.rows, 32) * tiles(a.Q.rows, 64) <= 512) {
+      product_tiled<IO, KIND, PA, QA, 64, 64, 2, 2, 2, 128, 2, true>(a, 1, stream);
+      return;
+    }
+  }
   if constexpr (sizeof(IO) == 2) {
-    if (!whole) product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 64, 2, false>(a, cut.splits, stream);
-    else if (cut.large) product_tiled<IO, KIND, PA, QA, 256, 256, 4, 2, 64, 2, true>(a, cut.splits, stream);
-    else product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 64, 2, true>(a, cut.splits, stream);
+    if (!whole) product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 1, 64, 2, false>(a, cut.splits, stream);
+    else if (cut.large) product_tiled<IO, KIND, PA, QA, 256, 256, 4, 2, 1, 64, 2, true>(a, cut.splits, stream);
+    else product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 2, 64, 2, true>(a, cut.splits, stream);
   } else {
-    if (whole) product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 32, 1, true>(a, cut.splits, stream);
-    else product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 32, 1, false>(a, cut.splits, stream);
+    if (whole) product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 1, 32, 1, true>(a, cut.splits, stream);
+    else product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 1, 32, 1, false>(a, cut.splits, stream);
   }
 }
 
