@@ -714,7 +714,7 @@ sparc_status sparc_qk_norm_rotary_backward(const sparc_rotary_desc* desc, const 
  * q [batch, length, heads, key_dim], k [.., kv_heads, key_dim] and v [..,
  * kv_heads, value_dim] in io_dtype, heads a multiple of kv_heads (query head h
  * reads key head h / (heads / kv_heads)), with the strides given in values (the
- * last dimension's is 1; that of time at least a row's values and less than 2^23,
+ * last dimension's is 1; that of time at least a row's values and less than 2^22,
  * where length is more than 1); o [batch, length, heads, value_dim] contiguous.
  * log_decay [heads] fp32, at most 0 (-inf: no memory).  lengths [batch] int64 or
  * NULL: the steps that a row has, cut to [0, length]; behind them k, v and q are

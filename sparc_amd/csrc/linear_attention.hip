@@ -575,12 +575,13 @@ const char* fault_of(const sparc_linear_desc* d) {
   if (d->key_dim < 1 || d->key_dim > 256 || d->value_dim < 1 || d->value_dim > 256)
     return "linear attention: key_dim and value_dim must be from 1 to 256";
   if (d->io_dtype != SPARC_F32 && d->io_dtype != SPARC_BF16) return "linear attention: io_dtype must be F32 or BF16";
-  // a chunk's rows lie one behind the other, within 2^31 bytes
+  // a chunk's rows, and those of threads beside it, lie within 2^30 bytes: kNowhere and
+  // as much more or less stays outside
   const int64_t* const strides[3] = {d->q_stride, d->k_stride, d->v_stride};
   for (int i = 0; i < 3; ++i)
-    if (d->length > 1 && (strides[i][1] < (i < 2 ? d->key_dim : d->value_dim) || strides[i][1] >= (1LL << 23)))
-      return "linear attention: time strides must be at least a row's values, and less than 2^23";
-  if (d->heads * (d->key_dim > d->value_dim ? d->key_dim : d->value_dim) >= (1LL << 23)) return "linear attention: too large";
+    if (d->length > 1 && (strides[i][1] < (i < 2 ? d->key_dim : d->value_dim) || strides[i][1] >= (1LL << 22)))
+      return "linear attention: time strides must be at least a row's values, and less than 2^22";
+  if (d->heads * (d->key_dim > d->value_dim ? d->key_dim : d->value_dim) >= (1LL << 22)) return "linear attention: too large";
   // grids and chain numbers are 32-bit
   if (d->batch > (1 << 22) || d->batch * d->heads > (1 << 22) || d->length > (1LL << 31))
     return "linear attention: too large";

@@ -14,7 +14,7 @@ Tensor rows_of(const Tensor& t) {
 }
 // The same for sequences [B, T, H, D], where the rows of one head lie apart and not too far
 Tensor steps_of(const Tensor& t) {
-  const bool fits = t.size(1) <= 1 || (t.stride(1) >= t.size(3) && t.stride(1) < (1 << 23));
+  const bool fits = t.size(1) <= 1 || (t.stride(1) >= t.size(3) && t.stride(1) < (1 << 22));
   return fits ? rows_of(t) : t.clone(at::MemoryFormat::Contiguous);
 }
 void strides_of(const Tensor& t, int64_t (&stride)[3]) {  // [B, T, H, D], or one step's [B, H, D]

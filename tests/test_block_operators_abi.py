@@ -62,7 +62,7 @@ def _linear(**kw):
     (dict(kv_heads=3), b"multiple"), (dict(kv_heads=0), b"multiple"), (dict(key_dim=0), b"1 to 256"),
     (dict(value_dim=257), b"1 to 256"), (dict(io_dtype=4), b"io_dtype"), (dict(batch=1 << 23), b"too large"),
     (dict(length=1 << 33), b"too large"), (dict(q_stride=(ctypes.c_int64 * 3)(0, 15, 1)), b"time strides"),
-    (dict(v_stride=(ctypes.c_int64 * 3)(0, 1 << 23, 1)), b"time strides"),
+    (dict(v_stride=(ctypes.c_int64 * 3)(0, 1 << 22, 1)), b"time strides"),
 ])
 def test_linear_attention_entry_points_validate(kw, msg):
     lib = _lib.load()

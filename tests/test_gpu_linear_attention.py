@@ -115,6 +115,22 @@ def test_strides(layout, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], **IDS)
+@pytest.mark.parametrize("stride", [(1 << 22) - 1, 1 << 22, (1 << 23) + 8])
+def test_steps_that_lie_far_apart(stride, dtype):
+    """At the largest stride that is read in place and behind it: the plain call's bits."""
+    T, K, V = 70, 30, 24
+    s, do, _ = _case(1, T, 2, 1, K, V, dtype, seed=stride)
+    s = {n: x.cuda() for n, x in s.items()}
+    far = dict(s)
+    for n in ("q", "k", "v"):
+        h, d = s[n].shape[2:]
+        far[n] = torch.full((stride * (T - 1) + h * d,), float("nan"), dtype=dtype, device="cuda").as_strided(
+            (1, T, h, d), (stride * T, stride, d, 1)).copy_(s[n])
+    got, want = (_all(sparc_amd.linear_attention, x, do.cuda(), None, False) for x in (far, s))
+    assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], **IDS)
 @pytest.mark.parametrize("state", [False, True])
 def test_lengths(state, dtype):
     lengths = [0, 1, 64, 65, 100, 1000, -3]
