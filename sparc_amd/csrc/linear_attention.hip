@@ -479,9 +479,9 @@ __global__ __launch_bounds__(64 * NW, KP * NV >= 128 ? 2 : 3) void linear_kernel
 }
 
 // What each segment enters with, from what each adds; and the last state.  One thread
-// per value of a chain's state.
-__global__ __launch_bounds__(256) void linear_join_kernel(const Problems a, int which) {
-  const Problem& p = a.p[which];
+// per value of a chain's state of a problem (blockIdx.y); their states are equally large.
+__global__ __launch_bounds__(256) void linear_join_kernel(const Problems a) {
+  const Problem& p = a.p[blockIdx.y];
   const int size = p.K * p.V;
   const int blocks = (size + 255) / 256;  // of a chain
   const int64_t chain = blockIdx.x / blocks;
@@ -492,12 +492,18 @@ __global__ __launch_bounds__(256) void linear_join_kernel(const Problems a, int 
   const float l2 = log2_decay(a.decay, static_cast<int>(chain % a.H));
   float s = p.s_in ? p.s_in[chain * size + row * p.in_k + c * p.in_n] : 0.0f;
   float* seg = p.seg + chain * a.segments * size + e;
-  for (int n = 0; n < a.segments; ++n) {
-    const int64_t left = steps - n * a.seg_len;
-    const float f = power(l2, static_cast<float>(left < 0 ? 0 : left < a.seg_len ? left : a.seg_len));
-    const float add = seg[static_cast<int64_t>(n) * size];
-    seg[static_cast<int64_t>(n) * size] = s;
-    s = f * s + add;
+  constexpr int N = 8;  // loads at a time: a store between them would keep them apart
+  for (int n0 = 0; n0 < a.segments; n0 += N) {
+    float add[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) add[i] = n0 + i < a.segments ? seg[static_cast<int64_t>(n0 + i) * size] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int64_t left = steps - (n0 + i) * a.seg_len;
+      const float f = power(l2, static_cast<float>(left < 0 ? 0 : left < a.seg_len ? left : a.seg_len));
+      if (n0 + i < a.segments) seg[static_cast<int64_t>(n0 + i) * size] = s;
+      s = n0 + i < a.segments ? f * s + add[i] : s;
+    }
   }
   if (p.s_out) p.s_out[chain * size + row * p.out_k + c * p.out_n] = s;
 }
@@ -593,6 +599,7 @@ int padded(int64_t k) { return k <= 32 ? 32 : k <= 64 ? 64 : k <= 128 ? 128 : 25
 int columns_of(int64_t v) { return v > 64 ? 128 : 64; }
 
 struct Plan {
+  int keys, columns;  // padded keys and value columns of a workgroup
   int segments;
   int64_t seg_len;
 };
@@ -601,19 +608,31 @@ struct Plan {
 // and the states between the passes, cost about as much as two thirds of idle CUs (16 x
 // 2048 steps of 12 heads of 64, 192 workgroups of 768: 94 us in one pass, 79 with 4
 // segments; the gradients of 8 x 4096 steps of 8 heads of 128, 192 of 512: 400 in one
-// pass, 447 with 4 segments, 487 with 3).
-Plan plan_of(const sparc_linear_desc* d, int64_t k, int64_t v, int problems) {
-  const int64_t chunk = d->io_dtype == SPARC_BF16 && padded(k) < 256 ? 64 : 32;
-  const int64_t width = columns_of(v), groups = d->batch * d->heads * ((v + width - 1) / width) * problems;
-  const int64_t slots = padded(k) * (width / 64) >= 128 ? 512 : 768, most = d->length / (4 * chunk);
+// pass, 447 with 4 segments, 487 with 3).  Where chains are few or short, the length of
+// a segment's chain is what counts: against segments of four chunks at least, 2 x 1000
+// steps of 4 heads of 64 take 22.5 us instead of 34, 4096 of 8 heads of 128 45 (of one
+// chunk 52: 512 workgroups, and 64 states to join) instead of 50.
+int64_t groups_of(const sparc_linear_desc* d, int columns, int64_t v) {
+  return d->batch * d->heads * ((v + columns - 1) / columns);
+}
+int64_t slots_of(int keys, int columns) { return keys * (columns / 64) >= 128 ? 512 : 768; }
+Plan plan_of(const sparc_linear_desc* d, int keys, int columns, int64_t groups) {
+  const int64_t chunk = d->io_dtype == SPARC_BF16 && keys < 256 ? 64 : 32;
+  const int64_t slots = slots_of(keys, columns), chunks = d->length / chunk;
   int64_t n = groups < 1 || 3 * groups >= slots ? 1 : slots / groups;
+  // segments of a chunk while every workgroup has a CU, of two at least else
+  const int64_t most = groups < 1 || chunks / 2 > 256 / groups ? chunks / 2 : chunks < 256 / groups ? chunks : 256 / groups;
   if (n > most) n = most;
   if (n < 1) n = 1;
   int64_t len = (d->length + n - 1) / n;
   len = (len + chunk - 1) / chunk * chunk;
   if (len < chunk) len = chunk;
   n = d->length > 0 ? (d->length + len - 1) / len : 1;
-  return {static_cast<int>(n), len};
+  return {keys, columns, static_cast<int>(n), len};
+}
+Plan plan_of(const sparc_linear_desc* d, int64_t k, int64_t v, int problems) {
+  const int columns = columns_of(v);
+  return plan_of(d, padded(k), columns, groups_of(d, columns, v) * problems);
 }
 size_t segment_bytes(const sparc_linear_desc* d, const Plan& plan) {
   return plan.segments > 1 ? up256(sizeof(float) * d->batch * d->heads * plan.segments * d->key_dim * d->value_dim) : 0;
@@ -637,8 +656,7 @@ template <typename IO, int KP, int NW, int NV> void launch(Problems& a, int n, i
   if (a.segments > 1) {
     if (whole) linear_kernel<IO, KP, NW, NV, false, true, true><<<total, 64 * NW, 0, stream>>>(a);
     else linear_kernel<IO, KP, NW, NV, false, true, false><<<total, 64 * NW, 0, stream>>>(a);
-    for (int i = 0; i < n; ++i)
-      linear_join_kernel<<<static_cast<unsigned>((a.p[i].K * a.p[i].V + 255) / 256 * chains), 256, 0, stream>>>(a, i);
+    linear_join_kernel<<<dim3(static_cast<unsigned>((a.p[0].K * a.p[0].V + 255) / 256 * chains), n), 256, 0, stream>>>(a);
   }
   constexpr bool kOne = sizeof(IO) == 4;  // fp32 products are exact either way
   if (whole) {
@@ -649,10 +667,9 @@ template <typename IO, int KP, int NW, int NV> void launch(Problems& a, int n, i
     else linear_kernel<IO, KP, NW, NV, true, kOne, false><<<total, 64 * NW, 0, stream>>>(a);
   }
 }
-// All problems have the same padded widths
-template <typename IO> void launch_io(Problems& a, int n, int64_t chains, hipStream_t stream) {
-  const int k = padded(a.p[0].K);
-  if (columns_of(a.p[0].V) == 64) {
+template <typename IO> void launch_io(const Plan& plan, Problems& a, int n, int64_t chains, hipStream_t stream) {
+  const int k = plan.keys;
+  if (plan.columns == 64) {
     if (k == 256) launch<IO, 256, 4, 1>(a, n, chains, stream);
     else if (k == 128) launch<IO, 128, 4, 1>(a, n, chains, stream);
     else if (k == 64) launch<IO, 64, 4, 1>(a, n, chains, stream);
@@ -664,28 +681,35 @@ template <typename IO> void launch_io(Problems& a, int n, int64_t chains, hipStr
     else launch<IO, 32, 4, 2>(a, n, chains, stream);
   }
 }
-void launch_all(int32_t io, Problems& a, int n, int64_t chains, hipStream_t stream) {
-  if (io == SPARC_BF16) launch_io<bf16>(a, n, chains, stream);
-  else launch_io<float>(a, n, chains, stream);
+void launch_all(int32_t io, const Plan& plan, Problems& a, int n, int64_t chains, hipStream_t stream) {
+  a.seg_len = plan.seg_len;
+  a.segments = plan.segments;
+  if (io == SPARC_BF16) launch_io<bf16>(plan, a, n, chains, stream);
+  else launch_io<float>(plan, a, n, chains, stream);
 }
 
 Rows rows_of(const void* p, const int64_t* stride, int64_t group) {
   return {p, stride[0], stride[1], stride[2], static_cast<int>(group)};
 }
-// Whether the problems of the backward (dq with the two widths exchanged, dk too) fit one launch
-bool alike(const sparc_linear_desc* d) {
-  return padded(d->key_dim) == padded(d->value_dim) &&
-         columns_of(d->key_dim) == columns_of(d->value_dim);
-}
+// The backward's problems (dq with the two widths exchanged, dk too) are one launch
+// where they are padded alike, and where all of them, padded to the larger keys, are on
+// the GPU at once: what idle CUs do costs nothing (3 x 1237 steps of 6 heads, keys of 40
+// and values of 72 in fp32: 111 -> 80 us; but keys of 32 beside values of 200, padded
+// from 32 to 256, 126 -> 139, so at most to twice their width).
 struct BackwardPlan {
-  Plan qk, v;  // of dq and dk, of dv
+  bool one;
+  Plan qk, v;  // of dq and dk (or of all), of dv
   size_t seg_qk, seg_v, shared_k, shared_v, total;
 };
 BackwardPlan backward_plan(const sparc_linear_desc* d) {
   BackwardPlan r;
-  const bool one = alike(d);
-  r.qk = plan_of(d, d->value_dim, d->key_dim, one ? 3 : 2);
-  r.v = one ? r.qk : plan_of(d, d->key_dim, d->value_dim, 1);
+  const int64_t K = d->key_dim, V = d->value_dim;
+  const int keys = padded(K > V ? K : V), columns = columns_of(K < V ? K : V);
+  const int64_t groups = 2 * groups_of(d, columns, K) + groups_of(d, columns, V);
+  r.one = (padded(K) == padded(V) && columns_of(K) == columns_of(V)) ||
+          (keys <= 2 * padded(K < V ? K : V) && groups <= slots_of(keys, columns));
+  r.qk = r.one ? plan_of(d, keys, columns, groups) : plan_of(d, V, K, 2);
+  r.v = r.one ? r.qk : plan_of(d, K, V, 1);
   r.seg_qk = segment_bytes(d, r.qk);
   r.seg_v = segment_bytes(d, r.v);
   const bool shared = d->heads > d->kv_heads;
@@ -733,10 +757,8 @@ sparc_status sparc_linear_attention_forward(const sparc_linear_desc* d, const vo
   a.decay = log_decay;
   a.lengths = lengths;
   a.T = d->length;
-  a.seg_len = plan.seg_len;
   a.H = static_cast<int>(d->heads);
-  a.segments = plan.segments;
-  launch_all(d->io_dtype, a, 1, d->batch * d->heads, reinterpret_cast<hipStream_t>(stream));
+  launch_all(d->io_dtype, plan, a, 1, d->batch * d->heads, reinterpret_cast<hipStream_t>(stream));
   return op_launched("sparc_linear_attention_forward");
 }
 
@@ -774,16 +796,10 @@ sparc_status sparc_linear_attention_backward(const sparc_linear_desc* d, const v
   a.lengths = lengths;
   a.T = T;
   a.H = static_cast<int>(H);
-  a.seg_len = plan.qk.seg_len;
-  a.segments = plan.qk.segments;
-  if (alike(d)) {
-    launch_all(d->io_dtype, a, 3, chains, stream);
-  } else {
-    launch_all(d->io_dtype, a, 2, chains, stream);
+  launch_all(d->io_dtype, plan.qk, a, plan.one ? 3 : 2, chains, stream);
+  if (!plan.one) {
     a.p[0] = a.p[2];
-    a.seg_len = plan.v.seg_len;
-    a.segments = plan.v.segments;
-    launch_all(d->io_dtype, a, 1, chains, stream);
+    launch_all(d->io_dtype, plan.v, a, 1, chains, stream);
   }
   if (shared && T > 0) {
     const auto sum = [&](const float* in, void* out, int64_t D) {
