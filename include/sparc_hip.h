@@ -761,8 +761,9 @@ sparc_status sparc_linear_attention_step(const sparc_linear_desc* desc, const vo
  * [rows, hidden], all contiguous, in io_dtype, aligned to their values.  activation:
  * 0 x sigmoid(x), 1 x Phi(x) (the normal distribution's), 2 max(x, 0), 3 sigmoid(x).
  * Products are matrix instructions with fp32 sums; the activation and the product
- * with the other projection are fp32, rounded once.  No counterpart in the
- * reference. */
+ * with the other projection are fp32, rounded once.  (F32 values are multiplied as
+ * sums of three bf16 values, all 24 bits of them: an infinite one gives NaN.)  No
+ * counterpart in the reference. */
 sparc_status sparc_gated_forward(int64_t rows, int64_t dim, int64_t hidden, int32_t io_dtype, int32_t activation,
                                  const void* x, const void* gate_weight, const void* up_weight, void* y,
                                  sparc_stream_t stream);

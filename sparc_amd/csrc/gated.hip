@@ -22,7 +22,7 @@ enum Act : int { ACT_SILU = 0, ACT_GELU = 1, ACT_RELU = 2, ACT_SIGMOID = 3 };
 template <typename IO> __device__ __forceinline__ float act_of(int act, float g, float& slope) {
   if (act == ACT_RELU) {
     slope = g > 0.0f ? 1.0f : 0.0f;
-    return g > 0.0f ? g : g * 0.0f;  // NaN stays
+    return g < 0.0f ? 0.0f : g;  // NaN stays
   }
   if (act == ACT_GELU) {
     const float phi = 0.5f * erfcf(g * -0.70710678118654752f);

@@ -18,7 +18,8 @@ def gated_linear_unit(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: tor
     ``x``: [..., D]; the weights: [F, D] as in ``torch.nn.Linear``, all float32 or
     all bfloat16, of any sizes; ``activation``: "silu" (x sigmoid(x)), "gelu" (x
     Phi(x), exact), "relu" or "sigmoid".  Sums are fp32, and the activation and the
-    product are computed from unrounded projections and rounded once.  Nothing but
+    product are computed from unrounded projections and rounded once (an infinite
+    float32 input gives NaN: it is multiplied in parts).  Nothing but
     the inputs is kept for the backward, which computes the projections again;
     their gradients are rounded to the inputs' dtype once before they are
     multiplied with x and the weights."""

@@ -97,6 +97,21 @@ def test_large_and_odd_values():
         torch.testing.assert_close(leaf.grad.cpu().double()[ok], ref.grad[ok], rtol=1e-5, atol=1e-30)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], **IDS)
+def test_a_projection_that_overflows(dtype):
+    """relu of -inf is zero, and so are its gradients."""
+    x, wg, wu = (torch.tensor([[v]], dtype=dtype, device="cuda").requires_grad_() for v in (-3e38, 10.0, 1e-38))
+    y = sparc_amd.gated_linear_unit(x, wg, wu, activation="relu")
+    y.sum().backward()
+    assert not y.any() and not x.grad.any() and not wg.grad.any() and not wu.grad.any()
+
+
+@pytest.mark.parametrize("rows", [1, 64, 65, 128, 129, 256])
+def test_few_rows_over_wide_weights(rows):
+    """Tiles of every size, whatever the rows."""
+    _run(*_case(rows, 136, 2056, BF16, seed=rows), "silu")
+
+
 def test_views_some_gradients_and_equal_bits():
     x, wg, wu, dy = _case(150, 72, 56, BF16, seed=7)
     x, wg, wu, dy = x.cuda(), wg.cuda(), wu.cuda(), dy.cuda()
