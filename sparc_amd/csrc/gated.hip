@@ -149,8 +149,10 @@ template <typename IO, int LINES, int COLS, int THREADS, bool ACROSS, bool WHOLE
 
 // TP x TQ results by WP x WQ waves; BK values of the contraction at a time, in BUFFERS
 // places in LDS.  KS: groups of so many waves that share the BK values and are added up
-// at the end, where tiles are small and one group would leave a SIMD one wave (256 rows
-// of 2048 on 8192: 39.1 -> 33.6 us).
+// at the end, where tiles are small and more waves would each have fewer results for what
+// they read (1 row of 2048 on 8192 in fp32: 53 us with eight waves beside one another, 41
+// with two groups of four).  Tiles of 128 have eight waves rather than four, which leave
+// a SIMD one each (1500 rows of 768 on 2048 29.5 -> 24.8 us, 256 of 3549 on 4105 78 -> 63).
 template <typename IO, int KIND, bool PA, bool QA, int TP, int TQ, int WP, int WQ, int KS, int BK, int BUFFERS, bool WHOLE>
 __global__ __launch_bounds__(64 * WP * WQ * KS, 2) void product_kernel(const ProductArgs a) {
   constexpr bool DUAL = KIND == GATED || KIND == GATED_BACK;
@@ -310,10 +312,9 @@ __global__ __launch_bounds__(64 * WP * WQ * KS, 2) void product_kernel(const Pro
       for (int c = 0; c < BK; c += 32 * KS) {
         // the other place is filled in the middle of a step: before it the rows would be
         // waited for at once, and no matrix instruction would run meanwhile
-        const bool fill = c == (KS == 1 ? BK / 64 * 32 : 0);
-        if (fill && KS == 1) next();
+        if (KS == 1 && c == BK / 64 * 32) next();
         read(place, c + 32 * share);
-        if (fill && KS > 1) next();
+        if (KS > 1 && c == 0) next();
         multiply();
       }
     }
@@ -432,7 +433,9 @@ const char* fault_of(int64_t rows, int64_t dim, int64_t hidden, int32_t io, int3
 size_t size_of(int32_t io) { return io == SPARC_BF16 ? 2 : 4; }
 
 int64_t tiles(int64_t n, int64_t tile) { return (n + tile - 1) / tile; }
-int step_of(int32_t io) { return io == SPARC_BF16 ? 64 : 32; }
+// values of the contraction that splits are counted in
+template <typename IO> constexpr int kStep = sizeof(IO) == 2 ? 64 : 32;
+int step_of(int32_t io) { return io == SPARC_BF16 ? kStep<bf16> : kStep<float>; }
 
 // How a product is cut: into large tiles where they are enough for most CUs, into small
 // ones, two to a CU, else; and its contraction into as many splits as fill the GPU, each
@@ -480,6 +483,7 @@ GatedPlan gated_plan(int64_t rows, int64_t dim, int64_t hidden, int32_t io) {
 template <typename IO, int KIND, bool PA, bool QA, int TP, int TQ, int WP, int WQ, int KS, int BK, int BUFFERS, bool WHOLE>
 void product_tiled(ProductArgs& a, int splits, hipStream_t stream) {
   constexpr bool DUAL = KIND == GATED || KIND == GATED_BACK;
+  static_assert(DUAL || BK == kStep<IO>, "a split begins at a step of its own");  // (and a dual product has none)
   a.p_tiles = static_cast<int>(tiles(a.P.rows, DUAL ? TP / 2 : TP));
   a.q_tiles = static_cast<int>(tiles(a.Q.rows, TQ));
   const int64_t count = static_cast<int64_t>(a.p_tiles) * a.q_tiles * (KIND == PAIR ? 2 : 1) * splits;
@@ -489,23 +493,30 @@ template <typename IO, int KIND, bool PA, bool QA>
 void product(ProductArgs& a, const Cut& cut, bool whole, hipStream_t stream) {
   a.split_steps = cut.split_steps;
   constexpr bool DUAL = KIND == GATED || KIND == GATED_BACK;
-  if constexpr (DUAL && sizeof(IO) == 2) {
+  if constexpr (DUAL) {
     // A few rows, for which the weights' way is all the time: tiles so small that most
     // CUs have one, all of them under way at once, each step of a whole 256 bytes of a
     // row (weights of 8192 x 2048 for 1 row 28.0 -> 16.6 us, for 64 30.7 -> 17.7, for
-    // 128 31.5 -> 25.8; for 256, where they no longer are, 33.9 instead of 44.5).
-    if (whole && tiles(a.P.rows, 32) * tiles(a.Q.rows, 64) <= 512) {
-      product_tiled<IO, KIND, PA, QA, 64, 64, 2, 2, 2, 128, 2, true>(a, 1, stream);
+    // 128 31.5 -> 25.8; for 256, where they no longer are, 33.9 instead of 44.5; in fp32
+    // for 1 row 121 -> 41; 14 rows of 3549 on 4105 bf16 73 -> 30).
+    if (tiles(a.P.rows, 32) * tiles(a.Q.rows, 64) <= 512) {
+      if constexpr (sizeof(IO) == 2) {
+        if (whole) product_tiled<IO, KIND, PA, QA, 64, 64, 2, 2, 2, 128, 2, true>(a, 1, stream);
+        else product_tiled<IO, KIND, PA, QA, 64, 64, 2, 2, 2, 128, 2, false>(a, 1, stream);
+      } else {
+        if (whole) product_tiled<IO, KIND, PA, QA, 64, 64, 2, 2, 2, 64, 2, true>(a, 1, stream);
+        else product_tiled<IO, KIND, PA, QA, 64, 64, 2, 2, 2, 64, 2, false>(a, 1, stream);
+      }
       return;
     }
   }
   if constexpr (sizeof(IO) == 2) {
-    if (!whole) product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 1, 64, 2, false>(a, cut.splits, stream);
+    if (!whole) product_tiled<IO, KIND, PA, QA, 128, 128, 4, 2, 1, 64, 2, false>(a, cut.splits, stream);
     else if (cut.large) product_tiled<IO, KIND, PA, QA, 256, 256, 4, 2, 1, 64, 2, true>(a, cut.splits, stream);
-    else product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 2, 64, 2, true>(a, cut.splits, stream);
+    else product_tiled<IO, KIND, PA, QA, 128, 128, 4, 2, 1, 64, 2, true>(a, cut.splits, stream);
   } else {
-    if (whole) product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 1, 32, 1, true>(a, cut.splits, stream);
-    else product_tiled<IO, KIND, PA, QA, 128, 128, 2, 2, 1, 32, 1, false>(a, cut.splits, stream);
+    if (whole) product_tiled<IO, KIND, PA, QA, 128, 128, 4, 2, 1, 32, 1, true>(a, cut.splits, stream);
+    else product_tiled<IO, KIND, PA, QA, 128, 128, 4, 2, 1, 32, 1, false>(a, cut.splits, stream);
   }
 }
 
