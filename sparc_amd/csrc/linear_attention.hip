@@ -11,6 +11,14 @@
 //          undecayed (dS_t = R_(t+1) + q_t do_t^T) and leaves it decayed (R_t = a
 //          dS_t), so the powers are a^i and a^(C-j) in place of a^(i+1) and a^(C-1-j).
 // One kernel therefore does all four, and the backward is three problems of a launch.
+//
+// The state stays in the matrix instructions' accumulators of a wave for its whole chain,
+// and every row is read once (with time segments keys and values twice).  What bounds a
+// chain is neither memory nor the matrix instructions but one chunk after the other: load,
+// scores, the split of scores and state into bf16 parts, products, update (65536 steps of
+// 16 heads of 128 x 128 bf16: 130 us for the states of 32 segments, 17 to join them, 290
+// for the outputs, at 3.9 TB/s, the matrix instructions busy 27 % and the VALU 36 % of the
+// time; the gradients of 8 x 4096 steps of 8 heads 345 us, 192 workgroups on 256 CUs).
 #include "matrix.h"
 
 namespace sparc {
@@ -178,7 +186,8 @@ template <typename IO, int C, int TILE, int THREADS, bool WHOLE> struct Stage {
 // OUT: with outputs; else only what the segment adds to the state.  WHOLE: keys as wide
 // as the tile, values that tiles divide and outputs in the I/O type; the other paths
 // cost registers that the kernel for 128 x 128 needs (they spilled:
-// 65536 steps of 16 heads 640 us with them, 555 without).
+// 65536 steps of 16 heads 609 us with them, 527 without; the gradients of 8 x 4096 steps
+// of 8 heads 470 and 337).
 template <typename IO, int KP, int NW, int NV, bool OUT, bool EXACT, bool WHOLE>
 __global__ __launch_bounds__(64 * NW, KP * NV >= 128 ? 2 : 3) void linear_kernel(const Problems a) {
   using W = Tiles<IO, KP, NW, NV>;
@@ -526,6 +535,8 @@ __global__ __launch_bounds__(256) void linear_shared_kernel(const float* in, IO*
 // one step
 // ---------------------------------------------------------------------------
 // A workgroup: one chain, 64 value columns; 16 lanes of four columns, 16 groups of rows.
+// Bound by the state, read and written once (256 rows of 16 heads of 128 x 128: 86 us for
+// 537 MB, 6.2 TB/s; 1 row: 5 us, two trips to memory).
 template <typename IO>
 __global__ __launch_bounds__(256) void linear_step_kernel(const Rows q, const Rows k, const Rows v, const float* decay,
                                                           const float* s_in, float* s_out, void* o, int H, int K,
@@ -606,9 +617,9 @@ struct Plan {
 // Time is cut into segments where the chains alone leave most of the GPU idle: into as
 // many as the workgroups that it holds at once.  A second pass over keys and values,
 // and the states between the passes, cost about as much as two thirds of idle CUs (16 x
-// 2048 steps of 12 heads of 64, 192 workgroups of 768: 94 us in one pass, 79 with 4
-// segments; the gradients of 8 x 4096 steps of 8 heads of 128, 192 of 512: 400 in one
-// pass, 447 with 4 segments, 487 with 3).  Where chains are few or short, the length of
+// 2048 steps of 12 heads of 64, 192 workgroups of 768: 94 us in one pass, 80 with 4
+// segments; the gradients of 8 x 4096 steps of 8 heads of 128, 192 of 512: 337 in one
+// pass, 427 with 2 segments, 397 with 4).  Where chains are few or short, the length of
 // a segment's chain is what counts: against segments of four chunks at least, 2 x 1000
 // steps of 4 heads of 64 take 22.5 us instead of 34, 4096 of 8 heads of 128 45 (of one
 // chunk 52: 512 workgroups, and 64 states to join) instead of 50.
