@@ -686,9 +686,18 @@ template <typename IO> void launch_io(const Plan& plan, Problems& a, int n, int6
     else if (k == 64) launch<IO, 64, 4, 1>(a, n, chains, stream);
     else launch<IO, 32, 4, 1>(a, n, chains, stream);
   } else {
+    // Where no CU has a second workgroup the columns go to eight waves rather than four,
+    // two to a SIMD (the gradients of 8 x 4096 steps of 8 heads of 128 x 128 bf16, 192
+    // workgroups: 338 -> 304 us; 65536 steps of 16 heads, 512: 513 and 541).
+    int64_t groups = 0;
+    for (int i = 0; i < n; ++i) groups += chains * ((a.p[i].V + 127) / 128) * a.segments;
+    const bool few = groups <= 256;
     if (k == 256) launch<IO, 256, 8, 1>(a, n, chains, stream);
+    else if (k == 128 && few) launch<IO, 128, 8, 1>(a, n, chains, stream);
     else if (k == 128) launch<IO, 128, 4, 2>(a, n, chains, stream);
+    else if (k == 64 && few) launch<IO, 64, 8, 1>(a, n, chains, stream);
     else if (k == 64) launch<IO, 64, 4, 2>(a, n, chains, stream);
+    else if (few) launch<IO, 32, 8, 1>(a, n, chains, stream);
     else launch<IO, 32, 4, 2>(a, n, chains, stream);
   }
 }

@@ -99,6 +99,14 @@ def test_against_the_recurrence(shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], **IDS)
+@pytest.mark.parametrize("K,V", [(32, 128), (64, 72), (64, 128), (128, 128), (100, 128)])
+def test_many_chains(K, V, dtype):
+    """More workgroups than CUs."""
+    s, do, ds = _case(33, 70, 8, 8, K, V, dtype, seed=K + V, state=True)
+    _run(s, do, ds, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], **IDS)
 @pytest.mark.parametrize("T", [257, 1000])
 def test_long_enough_for_segments(T, dtype):
     """Few chains over many chunks are cut into segments, with a ragged end."""
