@@ -18,7 +18,7 @@
 // scores, the split of scores and state into bf16 parts, products, update (65536 steps of
 // 16 heads of 128 x 128 bf16: 130 us for the states of 32 segments, 17 to join them, 290
 // for the outputs, at 3.9 TB/s, the matrix instructions busy 27 % and the VALU 36 % of the
-// time; the gradients of 8 x 4096 steps of 8 heads 345 us, 192 workgroups on 256 CUs).
+// time; the gradients of 8 x 4096 steps of 8 heads 290 us, 192 workgroups on 256 CUs).
 #include "matrix.h"
 
 namespace sparc {
@@ -186,8 +186,7 @@ template <typename IO, int C, int TILE, int THREADS, bool WHOLE> struct Stage {
 // OUT: with outputs; else only what the segment adds to the state.  WHOLE: keys as wide
 // as the tile, values that tiles divide and outputs in the I/O type; the other paths
 // cost registers that the kernel for 128 x 128 needs (they spilled:
-// 65536 steps of 16 heads 609 us with them, 527 without; the gradients of 8 x 4096 steps
-// of 8 heads 470 and 337).
+// 65536 steps of 16 heads 609 us with them, 527 without).
 template <typename IO, int KP, int NW, int NV, bool OUT, bool EXACT, bool WHOLE>
 __global__ __launch_bounds__(64 * NW, KP * NV >= 128 ? 2 : 3) void linear_kernel(const Problems a) {
   using W = Tiles<IO, KP, NW, NV>;
@@ -618,7 +617,7 @@ struct Plan {
 // many as the workgroups that it holds at once.  A second pass over keys and values,
 // and the states between the passes, cost about as much as two thirds of idle CUs (16 x
 // 2048 steps of 12 heads of 64, 192 workgroups of 768: 94 us in one pass, 80 with 4
-// segments; the gradients of 8 x 4096 steps of 8 heads of 128, 192 of 512: 337 in one
+// segments; the gradients of 8 x 4096 steps of 8 heads of 128, 192 of 512: 300 in one
 // pass, 427 with 2 segments, 397 with 4).  Where chains are few or short, the length of
 // a segment's chain is what counts: against segments of four chunks at least, 2 x 1000
 // steps of 4 heads of 64 take 22.5 us instead of 34, 4096 of 8 heads of 128 45 (of one
