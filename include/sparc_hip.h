@@ -773,7 +773,8 @@ size_t sparc_gated_workspace_bytes(int64_t rows, int64_t dim, int64_t hidden, in
 
 /* The backward given dy [rows, hidden]: dx (NULL: not wanted) and both weights'
  * gradients (both or neither), overwritten.  The projections are computed again; the
- * gradients of both are rounded to io_dtype once before the products with them. */
+ * gradients of both are rounded to io_dtype once before the products with them (in
+ * BF16 up to 2^28 rows x dim x hidden to a sum of two values, all but 2^-16 of them). */
 sparc_status sparc_gated_backward(int64_t rows, int64_t dim, int64_t hidden, int32_t io_dtype, int32_t activation,
                                   const void* x, const void* gate_weight, const void* up_weight, const void* dy,
                                   void* dx, void* dgate_weight, void* dup_weight, void* workspace,

@@ -47,16 +47,17 @@ template <typename IO> __device__ __forceinline__ float act_of(int act, float g,
 }
 
 // An operand: rows r (the result's p or q) and the contraction k; element (r, k) at
-// r ld + k, or (ACROSS) at k ld + r.  Of two parts each has a tensor of its own.
+// r ld + k, or (ACROSS) at k ld + r.  Each part has a tensor of its own.
 struct Operand {
-  const void* p[2];
+  const void* p[4];
   int64_t ld, rows;
 };
 struct ProductArgs {
   Operand P, Q;
   int64_t nk;             // contraction of a part
+  int parts;              // PARTS: of the contraction; PAIR: of each product's
   int p_tiles, q_tiles;   // workgroups; in PAIR and of a gated product each side's own tiles
-  void* out[2];           // [rows q, rows p], row stride out_ld
+  void* out[4];           // [rows q, rows p], row stride out_ld; GATED_BACK: [2], [3] what rounding took (or NULL)
   int64_t out_ld;
   const void* dy;         // GATED_BACK: [Q.rows, P.rows]
   int act;
@@ -65,9 +66,20 @@ struct ProductArgs {
 };
 
 // GATED: both parts of P at once, out[0] = act(.) * (.).  GATED_BACK: out[0] and out[1]
-// the gradients of both projections.  PARTS: the sum over both parts.  PAIR: a product
-// for each part of Q.
+// the gradients of both projections.  PARTS: the sum over all parts.  PAIR: a product
+// for each of two tensors of Q, and over every second part.
 enum Kind : int { GATED = 0, GATED_BACK = 1, PARTS = 2, PAIR = 3 };
+
+// What rounding to bf16 takes from values (nothing where that is not finite)
+__device__ __forceinline__ f32x4 rest_of(const f32x4& x) {
+  f32x4 y;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const float rest = x[r] - bf16_bits_to_float(pack_bf16(x[r]));
+    y[r] = fabsf(rest) < __builtin_inff() ? rest : 0.0f;
+  }
+  return y;
+}
 
 // An offset that no buffer reaches: loads there give zero.
 constexpr uint32_t kNowhere = 0x80000000u;
@@ -234,7 +246,7 @@ __global__ __launch_bounds__(64 * WP * WQ * KS, 2) void product_kernel(const Pro
     fetch(fp, a.P, PAcross(), Dual(), p0, k, part);
   };
   const auto fetch_q = [&](int64_t k, int part) __attribute__((always_inline)) {
-    fetch(fq, a.Q, QAcross(), std::false_type(), q0, k, KIND == PAIR ? side : part);
+    fetch(fq, a.Q, QAcross(), std::false_type(), q0, k, KIND == PAIR ? side + 2 * part : part);
   };
   const auto tail = [&](int64_t k) { return k1 - k < BK && (k1 - k) % VEC != 0 && a.nk >= VEC; };
   const auto put_p = [&](int place, int64_t k) __attribute__((always_inline)) {
@@ -279,7 +291,7 @@ __global__ __launch_bounds__(64 * WP * WQ * KS, 2) void product_kernel(const Pro
           for (int j = 0; j < MQ; ++j) acc[i][j] = mma(p[n][i], q[order - n][j], acc[i][j]);
   };
   // steps: all of one part, then all of the next
-  const int per_part = static_cast<int>((a.nk + BK - 1) / BK), all = per_part * (KIND == PARTS ? 2 : 1);
+  const int per_part = static_cast<int>((a.nk + BK - 1) / BK), all = per_part * (DUAL ? 1 : a.parts);
   const int begin = split * a.split_steps, end = begin + a.split_steps < all ? begin + a.split_steps : all;
   const int count = end - begin;
   // Goes from step to step and stays at the last one: what is fetched and put behind it
@@ -291,7 +303,7 @@ __global__ __launch_bounds__(64 * WP * WQ * KS, 2) void product_kernel(const Pro
       if (left <= 1) return;
       --left;
       k += BK;
-      if (KIND == PARTS && k >= nk) k = 0, ++part;
+      if ((KIND == PARTS || KIND == PAIR) && k >= nk) k = 0, ++part;
     }
   };
   Walk at = {static_cast<int64_t>(begin % per_part) * BK, begin / per_part, count}, put_at = at;
@@ -396,8 +408,13 @@ __global__ __launch_bounds__(64 * WP * WQ * KS, 2) void product_kernel(const Pro
           store_quad(static_cast<IO*>(a.out[0]) + at, n, h * acc[i + MP / 2][j]);
         } else {
           const f32x4 dy = dys[i][j];
-          store_quad(static_cast<IO*>(a.out[0]) + at, n, dy * acc[i + MP / 2][j] * slope);
-          store_quad(static_cast<IO*>(a.out[1]) + at, n, dy * h);
+          const f32x4 dg = dy * acc[i + MP / 2][j] * slope, du = dy * h;
+          store_quad(static_cast<IO*>(a.out[0]) + at, n, dg);
+          store_quad(static_cast<IO*>(a.out[1]) + at, n, du);
+          if (sizeof(IO) == 2 && a.out[2]) {
+            store_quad(static_cast<IO*>(a.out[2]) + at, n, rest_of(dg));
+            store_quad(static_cast<IO*>(a.out[3]) + at, n, rest_of(du));
+          }
         }
       }
     } else {
@@ -471,15 +488,26 @@ Cut cut_of(int32_t io, bool whole, int64_t np, int64_t nq, int64_t nk, int parts
 // Whether no line's end cuts a vector, for lines of these lengths
 bool is_whole(int32_t io, int64_t m, int64_t n = 0) { return io == SPARC_BF16 ? (m | n) % 8 == 0 : (m | n) % 4 == 0; }
 
+// dg and du are rounded to bf16 for the products with them, which makes their results'
+// errors 1.4 times as large as one rounding's.  Where launches take the time rather than
+// the products, what the rounding took is multiplied too, and the errors are one
+// rounding's (the backward's kernels of 32 rows of 64 on 96 17.6 -> 21.6 us, of 1000 of
+// 256 on 1024 42 -> 50, behind some 50 of autograd; at 32768 rows of 768 on 2048 it
+// would be another 500 beside 1050).
+constexpr int64_t kRestUpTo = 1LL << 28;  // rows x dim x hidden
+
 struct GatedPlan {
   Cut dx, dw;
   int64_t g_ld;
-  size_t g, partial;  // bytes of dg, and as many of du; of the partial sums, which dx and the weights' share
+  int parts;             // of dg and du: 2 with what rounding took
+  size_t g, partial;     // bytes of a part of dg or du; of the partial sums, which dx and the weights' share
+  size_t all() const { return 2 * parts * g + partial; }
 };
 GatedPlan gated_plan(int64_t rows, int64_t dim, int64_t hidden, int32_t io) {
   GatedPlan p;
-  p.dx = cut_of(io, is_whole(io, dim, hidden), dim, rows, hidden, 2, true);
-  p.dw = cut_of(io, is_whole(io, dim, hidden), dim, 2 * hidden, rows, 1, true);
+  p.parts = io == SPARC_BF16 && rows <= kRestUpTo / (dim * hidden) ? 2 : 1;
+  p.dx = cut_of(io, is_whole(io, dim, hidden), dim, rows, hidden, 2 * p.parts, true);
+  p.dw = cut_of(io, is_whole(io, dim, hidden), dim, 2 * hidden, rows, p.parts, true);
   p.g_ld = tiles(hidden, 8) * 8;  // whole vectors, whatever the width
   p.g = up256(rows * p.g_ld * size_of(io));
   const size_t x = p.dx.splits > 1 ? sizeof(float) * p.dx.splits * rows * dim : 0;
@@ -530,12 +558,12 @@ void product(ProductArgs& a, const Cut& cut, bool whole, hipStream_t stream) {
 
 template <typename IO>
 void gated_run(int32_t io, int64_t rows, int64_t dim, int64_t hidden, int act, const void* x, const void* wg,
-               const void* wu, const void* dy, void* out0, void* out1, int64_t out_ld, hipStream_t stream) {
+               const void* wu, const void* dy, void* const (&out)[4], int64_t out_ld, hipStream_t stream) {
   ProductArgs a = {};
   a.P = {{wg, wu}, dim, hidden};
   a.Q = {{x, x}, dim, rows};
   a.nk = dim;
-  a.out[0] = out0, a.out[1] = out1;
+  for (int i = 0; i < 4; ++i) a.out[i] = out[i];
   a.out_ld = out_ld;
   a.dy = dy;
   a.act = act;
@@ -551,14 +579,15 @@ void sum_partial(const float* partial, int splits, int64_t total, int64_t half, 
 }
 template <typename IO>
 void gated_grads(int32_t io, int64_t rows, int64_t dim, int64_t hidden, const void* x, const void* wg, const void* wu,
-                 const void* dg, const void* du, void* dx, void* dwg, void* dwu, float* partial, const GatedPlan& plan,
+                 void* const (&g)[4], void* dx, void* dwg, void* dwu, float* partial, const GatedPlan& plan,
                  hipStream_t stream) {
   const bool whole = is_whole(io, dim, hidden);
   if (dx) {
     ProductArgs a = {};
-    a.P = {{wg, wu}, dim, dim};
-    a.Q = {{dg, du}, plan.g_ld, rows};
+    a.P = {{wg, wu, wg, wu}, dim, dim};
+    a.Q = {{g[0], g[1], g[2], g[3]}, plan.g_ld, rows};
     a.nk = hidden;
+    a.parts = 2 * plan.parts;
     a.out[0] = a.out[1] = dx;
     a.out_ld = dim;
     a.partial = plan.dx.splits > 1 ? partial : nullptr;
@@ -568,8 +597,9 @@ void gated_grads(int32_t io, int64_t rows, int64_t dim, int64_t hidden, const vo
   if (dwg) {
     ProductArgs a = {};
     a.P = {{x, x}, dim, dim};
-    a.Q = {{dg, du}, plan.g_ld, hidden};
+    a.Q = {{g[0], g[1], g[2], g[3]}, plan.g_ld, hidden};
     a.nk = rows;
+    a.parts = plan.parts;
     a.out[0] = dwg, a.out[1] = dwu;
     a.out_ld = dim;
     a.partial = plan.dw.splits > 1 ? partial : nullptr;
@@ -594,16 +624,16 @@ sparc_status sparc_gated_forward(int64_t rows, int64_t dim, int64_t hidden, int3
   if (!x || !gate_weight || !up_weight || !y) return op_fail(SPARC_EINVAL, "gated linear unit: a tensor is NULL");
   const hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
   if (io_dtype == SPARC_BF16)
-    gated_run<bf16>(io_dtype, rows, dim, hidden, activation, x, gate_weight, up_weight, nullptr, y, nullptr, hidden, stream);
+    gated_run<bf16>(io_dtype, rows, dim, hidden, activation, x, gate_weight, up_weight, nullptr, {y}, hidden, stream);
   else
-    gated_run<float>(io_dtype, rows, dim, hidden, activation, x, gate_weight, up_weight, nullptr, y, nullptr, hidden, stream);
+    gated_run<float>(io_dtype, rows, dim, hidden, activation, x, gate_weight, up_weight, nullptr, {y}, hidden, stream);
   return op_launched("sparc_gated_forward");
 }
 
 size_t sparc_gated_workspace_bytes(int64_t rows, int64_t dim, int64_t hidden, int32_t io_dtype) {
   if (fault_of(rows, dim, hidden, io_dtype, 0)) return 0;
   const GatedPlan p = gated_plan(rows, dim, hidden, io_dtype);
-  return 2 * p.g + p.partial;
+  return p.all();
 }
 
 sparc_status sparc_gated_backward(int64_t rows, int64_t dim, int64_t hidden, int32_t io_dtype, int32_t activation,
@@ -614,16 +644,16 @@ sparc_status sparc_gated_backward(int64_t rows, int64_t dim, int64_t hidden, int
   if ((rows > 0 && (!x || !dy)) || !gate_weight || !up_weight || !dgate_weight != !dup_weight)
     return op_fail(SPARC_EINVAL, "gated linear unit: a tensor is NULL");
   const GatedPlan plan = gated_plan(rows, dim, hidden, io_dtype);
-  if (rows > 0 && (!workspace || workspace_bytes < 2 * plan.g + plan.partial))
+  if (rows > 0 && (!workspace || workspace_bytes < plan.all()))
     return op_fail(SPARC_EWORKSPACE, "gated linear unit: workspace missing or too small");
   const hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
   char* const ws = static_cast<char*>(workspace);
-  void *const dg = ws, *const du = ws + plan.g;
-  float* const partial = reinterpret_cast<float*>(ws + 2 * plan.g);
+  void* const g[4] = {ws, ws + plan.g, plan.parts == 2 ? ws + 2 * plan.g : nullptr, plan.parts == 2 ? ws + 3 * plan.g : nullptr};
+  float* const partial = reinterpret_cast<float*>(ws + 2 * plan.parts * plan.g);
   const auto go = [&](auto type) {
     using IO = decltype(type);
-    if (rows > 0) gated_run<IO>(io_dtype, rows, dim, hidden, activation, x, gate_weight, up_weight, dy, dg, du, plan.g_ld, stream);
-    gated_grads<IO>(io_dtype, rows, dim, hidden, x, gate_weight, up_weight, dg, du, rows > 0 ? dx : nullptr, dgate_weight,
+    if (rows > 0) gated_run<IO>(io_dtype, rows, dim, hidden, activation, x, gate_weight, up_weight, dy, g, plan.g_ld, stream);
+    gated_grads<IO>(io_dtype, rows, dim, hidden, x, gate_weight, up_weight, g, rows > 0 ? dx : nullptr, dgate_weight,
                     dup_weight, partial, plan, stream);
   };
   if (io_dtype == SPARC_BF16) go(bf16());

@@ -5,7 +5,8 @@ terms' sizes.  The activations' slopes are at most 1.13 and change by at most 0.
 unit, so y is off by 1.2 e_g |u| + |act| e_u, and what the gradients are made of, dg
 = dy u act'(g) and du = dy act(g), by |dy| (1.2 e_u + 0.8 |u| e_g) and 1.2 |dy| e_g;
 16 further roundings each.  With bfloat16 inputs both are rounded before their
-products (2^-8 each), and so is every result (2^-8)."""
+products (2^-8 each; in small calls what that leaves is multiplied too, 2^-16), and so
+is every result (2^-8)."""
 import pytest
 import torch
 
@@ -25,7 +26,7 @@ def _case(N, D, F, dtype, seed):
     return r(N, D).to(dtype), (r(F, D) * D ** -0.5).to(dtype), (r(F, D) * D ** -0.5).to(dtype), r(N, F).to(dtype)
 
 
-def _run(x, wg, wu, dy, act, shape=None):
+def _run(x, wg, wu, dy, act, shape=None, rest=2.0 ** -8):
     dtype = x.dtype
     half = 2.0 ** -8 if dtype == BF16 else U
     X, G, W, DY = (t.double() for t in (x, wg, wu, dy))
@@ -43,7 +44,7 @@ def _run(x, wg, wu, dy, act, shape=None):
     edg = DY.abs() * (1.2 * eu + 0.8 * u.abs() * eg) + 16 * U * (DY * u).abs() * 1.2
     edu = 1.2 * DY.abs() * eg + 16 * U * du.abs()
     if dtype == BF16:
-        edg, edu = edg + half * dg.abs(), edu + half * du.abs()
+        edg, edu = edg + rest * dg.abs(), edu + rest * du.abs()
     want = {"y": (y, ey),
             "dx": (dg @ G + du @ W, edg @ G.abs() + edu @ W.abs() + (2 * F + 8) * U * (dg.abs() @ G.abs() + du.abs() @ W.abs())),
             "dwg": (dg.T @ X, edg.T @ X.abs() + (N + 72) * U * (dg.abs().T @ X.abs())),
@@ -104,6 +105,12 @@ def test_a_projection_that_overflows(dtype):
     y = sparc_amd.gated_linear_unit(x, wg, wu, activation="relu")
     y.sum().backward()
     assert not y.any() and not x.grad.any() and not wg.grad.any() and not wu.grad.any()
+
+
+@pytest.mark.parametrize("shape", [(2, 59, 3183), (32, 64, 96), (150, 416, 2272), (1001, 256, 1000), (700, 72, 4000)],
+                         ids=str)
+def test_small_calls_lose_nothing_between_their_products(shape):
+    _run(*_case(*shape, BF16, seed=sum(shape)), "silu", rest=2.0 ** -16)
 
 
 @pytest.mark.parametrize("rows", [1, 64, 65, 128, 129, 256])
