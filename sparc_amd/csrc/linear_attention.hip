@@ -109,8 +109,9 @@ template <typename IO, int KP, int NW, int NV> struct Tiles {
 // rows of ``width`` values.  A thread reads 16-byte vectors of one column position
 // through a buffer that ends with the chunk's last row, so that nothing needs a
 // condition (a branch around a load makes the loads wait for one another): what lies
-// behind the last row or the last column is zero.  The vector that a row's end would
-// cut is read so that it ends with the row, and shifted.
+// behind the last row (rows lie a row's width apart or more) or the last column is
+// zero.  The vector that a row's end would cut is read so that it ends with the row,
+// and shifted.
 template <typename IO, int C, int TILE, int THREADS, bool WHOLE> struct Stage {
   static constexpr int VEC = kVec<IO>, PER = TILE / VEC, SIZE = sizeof(IO);
   static constexpr int STEP = THREADS / PER < C ? THREADS / PER : C, N = C / STEP;
@@ -707,8 +708,11 @@ void launch_all(int32_t io, const Plan& plan, Problems& a, int n, int64_t chains
   else launch_io<float>(plan, a, n, chains, stream);
 }
 
-Rows rows_of(const void* p, const int64_t* stride, int64_t group) {
-  return {p, stride[0], stride[1], stride[2], static_cast<int>(group)};
+// A row of ``width`` values for each step.  A chunk's absent steps are read as zero because
+// they lie behind its last row, which takes a time stride of a row's width or more: one
+// step, whose stride may be anything, gets that width.
+Rows rows_of(const sparc_linear_desc* d, const void* p, const int64_t* stride, int64_t width, int64_t group) {
+  return {p, stride[0], d->length == 1 ? width : stride[1], stride[2], static_cast<int>(group)};
 }
 // The backward's problems (dq with the two widths exchanged, dk too) are one launch
 // where they are padded alike, and where all of them, padded to the larger keys, are on
@@ -771,8 +775,9 @@ sparc_status sparc_linear_attention_forward(const sparc_linear_desc* d, const vo
   const int K = static_cast<int>(d->key_dim), V = static_cast<int>(d->value_dim);
   const int64_t group = d->heads / d->kv_heads;
   Problems a = {};
-  a.p[0] = {rows_of(q, d->q_stride, 1), rows_of(k, d->k_stride, group), rows_of(v, d->v_stride, group), o, state_in,
-            state_out, static_cast<float*>(workspace), V, 1, V, 1, K, V, 0, 1, 0, 0, d->scale, d->scale, 1.0f};
+  a.p[0] = {rows_of(d, q, d->q_stride, K, 1), rows_of(d, k, d->k_stride, K, group),
+            rows_of(d, v, d->v_stride, V, group), o, state_in, state_out, static_cast<float*>(workspace),
+            V, 1, V, 1, K, V, 0, 1, 0, 0, d->scale, d->scale, 1.0f};
   a.decay = log_decay;
   a.lengths = lengths;
   a.T = d->length;
@@ -803,8 +808,8 @@ sparc_status sparc_linear_attention_backward(const sparc_linear_desc* d, const v
   const int K = static_cast<int>(d->key_dim), V = static_cast<int>(d->value_dim);
   const int64_t group = d->heads / d->kv_heads, H = d->heads, T = d->length, chains = d->batch * H;
   const int64_t o_stride[3] = {T * H * V, H * V, V};
-  const Rows rq = rows_of(q, d->q_stride, 1), rk = rows_of(k, d->k_stride, group), rv = rows_of(v, d->v_stride, group);
-  const Rows ro = rows_of(d_o, o_stride, 1);
+  const Rows rq = rows_of(d, q, d->q_stride, K, 1), rk = rows_of(d, k, d->k_stride, K, group);
+  const Rows rv = rows_of(d, v, d->v_stride, V, group), ro = rows_of(d, d_o, o_stride, V, 1);
   const int shared = group > 1;
   Problems a = {};
   // states of dq and dk are transposed: element (n, k) of the problem is (k, n) of the tensor
@@ -844,8 +849,9 @@ sparc_status sparc_linear_attention_step(const sparc_linear_desc* d, const void*
     return op_fail(SPARC_EINVAL, "linear attention: a tensor is NULL");
   const hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
   const int64_t group = d->heads / d->kv_heads;
-  const Rows rq = rows_of(q, d->q_stride, 1), rk = rows_of(k, d->k_stride, group), rv = rows_of(v, d->v_stride, group);
   const int H = static_cast<int>(d->heads), K = static_cast<int>(d->key_dim), V = static_cast<int>(d->value_dim);
+  const Rows rq = rows_of(d, q, d->q_stride, K, 1), rk = rows_of(d, k, d->k_stride, K, group);
+  const Rows rv = rows_of(d, v, d->v_stride, V, group);
   const int v_tiles = (V + 63) / 64;
   const unsigned grid = static_cast<unsigned>(d->batch * d->heads * v_tiles);
   if (d->io_dtype == SPARC_BF16)
