@@ -722,9 +722,10 @@ sparc_status sparc_qk_norm_rotary_backward(const sparc_rotary_desc* desc, const 
  * key_dim, value_dim] fp32, contiguous; state_in NULL: zero, state_out NULL: not
  * wanted.  key_dim and value_dim from 1 to 256.  Products are fp32 or bf16 matrix
  * instructions with fp32 sums; where a state, a score or a decayed value enters a
- * bf16 product it does so as a sum of two or three bf16 values.  Results are
- * rounded once, and equal calls give equal bits.  No counterpart in the
- * reference, whose states are vectors (one value per mode). */
+ * bf16 product it does so as a sum of two bf16 values (all but 2^-17 of it; an
+ * infinite one becomes NaN), and what is added to a state that is written as one of
+ * three (all of it).  Results are rounded once, and equal calls give equal bits.
+ * No counterpart in the reference, whose states are vectors (one value per mode). */
 typedef struct sparc_linear_desc {
   int64_t batch, length, heads, kv_heads, key_dim, value_dim;
   int32_t io_dtype;

@@ -95,10 +95,12 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     and the state is that after the last step there is.
 
     Differentiable in q, k, v and state (once, and in reverse mode only); nothing
-    but the inputs is kept for it.  Sums and states are fp32; bfloat16 inputs are
-    multiplied as they are, and what is computed on the way (scores, decayed values,
-    the state) enters a product as two or three bfloat16 values, so results are those
-    of fp32 arithmetic rounded once.  Equal calls give equal bits."""
+    but the inputs is kept for it.  Sums and states are fp32, and results are rounded
+    once.  bfloat16 inputs are multiplied as they are; what is computed on the way
+    enters a product with them as a sum of bfloat16 values: what is added to a state
+    that is returned as three, which hold all of it, the rest (scores, the state where
+    it is read, decayed values) as two, which hold all but 2^-17 (an infinite one of
+    these becomes NaN).  Equal calls give equal bits."""
     y = _lib.native().linear_attention(q, k, v, log_decay, state, scale, lengths)
     return y if y is not None else _refuse_linear(q, k, v, log_decay, state, lengths, 4)
 

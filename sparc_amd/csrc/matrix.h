@@ -101,9 +101,10 @@ template <typename L, typename IO> __device__ __forceinline__ Frag<IO> read_tile
 __device__ __forceinline__ uint32_t upper_halves(uint32_t a, uint32_t b) {
   return __builtin_amdgcn_perm(b, a, 0x07060302u);
 }
-// fp32 values as a sum of N fragments.  Each part is what is left of the value, truncated
-// to bf16: 8 bits of it, so that two parts hold 16 bits and three all 24.  (A value that
-// is infinite becomes NaN for N > 1.)
+// fp32 values as a sum of N fragments.  Two parts are rounded to nearest: of a value
+// from 1 to 2 the first leaves 2^-8 at most, of which the second leaves 2^-17 (truncated
+// they would leave 2^-15, and always on the same side).  Three are truncated, 8 bits
+// each, and hold all 24.  (A value that is infinite becomes NaN for N > 1.)
 template <int N> __device__ __forceinline__ void split(const float (&x)[8], Frag<bf16> (&f)[N]) {
   uint32_t r[8];
 #pragma unroll
@@ -113,10 +114,12 @@ template <int N> __device__ __forceinline__ void split(const float (&x)[8], Frag
     uint32_t u[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      u[i] = upper_halves(r[2 * i], r[2 * i + 1]);
+      uint32_t &a = r[2 * i], &b = r[2 * i + 1];
+      u[i] = N == 2 ? pack_bf16x2(__uint_as_float(a), __uint_as_float(b)) : upper_halves(a, b);
       if (n + 1 < N) {
-        r[2 * i] = __float_as_uint(__uint_as_float(r[2 * i]) - __uint_as_float(r[2 * i] & 0xffff0000u));
-        r[2 * i + 1] = __float_as_uint(__uint_as_float(r[2 * i + 1]) - __uint_as_float(r[2 * i + 1] & 0xffff0000u));
+        const uint32_t low = N == 2 ? u[i] << 16 : a & 0xffff0000u, high = N == 2 ? u[i] & 0xffff0000u : b & 0xffff0000u;
+        a = __float_as_uint(__uint_as_float(a) - __uint_as_float(low));
+        b = __float_as_uint(__uint_as_float(b) - __uint_as_float(high));
       }
     }
     __builtin_memcpy(&f[n], u, sizeof(u));
