@@ -103,12 +103,12 @@ def _make_norm(kind: str, d_model: int, eps: float) -> nn.Module:
 
 
 def _is_observed(module: nn.Module) -> bool:
-    """Whether a call of the module does more than its forward (hooks, of its own
-    or of all modules)."""
+    """Whether a call of the module does more than its class's forward (hooks, of its
+    own or of all modules; a forward of its own)."""
     m = nn.modules.module
-    return any((module._forward_hooks, module._forward_pre_hooks, module._backward_hooks, module._backward_pre_hooks,
-                m._global_forward_hooks, m._global_forward_pre_hooks, m._global_backward_hooks,
-                m._global_backward_pre_hooks))
+    return any(("forward" in vars(module), module._forward_hooks, module._forward_pre_hooks, module._backward_hooks,
+                module._backward_pre_hooks, m._global_forward_hooks, m._global_forward_pre_hooks,
+                m._global_backward_hooks, m._global_backward_pre_hooks))
 
 
 def apply_norm(norm: nn.Module, x: torch.Tensor) -> torch.Tensor:
@@ -123,18 +123,33 @@ def apply_norm(norm: nn.Module, x: torch.Tensor) -> torch.Tensor:
     return rms_norm(norm, x)
 
 
+def _only_multiplies(module: nn.Module) -> bool:
+    """Whether a call of the module is the product with its weight and nothing more,
+    so that an operator may take the weight in place of the call."""
+    return type(module) is nn.Linear and module.bias is None and not _is_observed(module)
+
+
+_ACTIVATIONS = {"silu": F.silu, "gelu": F.gelu, "relu": F.relu, "sigmoid": torch.sigmoid}
+
+
 class GatedFeedForward(nn.Module):
-    """down(act(gate(x)) * up(x)): ``gated_linear_unit`` and the projection back."""
+    """down(act(gate(x)) * up(x)): ``gated_linear_unit`` and the projection back.  Where
+    ``gate`` or ``up`` does more than multiply by its weight (hooks, a bias, a module
+    put in its place), both are called."""
 
     def __init__(self, d_model: int, hidden: int, activation: str = "silu"):
         super().__init__()
         self.gate = nn.Linear(d_model, hidden, bias=False)
         self.up = nn.Linear(d_model, hidden, bias=False)
         self.down = nn.Linear(hidden, d_model, bias=False)
+        if activation not in _ACTIVATIONS:
+            raise ValueError(f"unknown activation {activation!r} ({', '.join(_ACTIVATIONS)})")
         self.activation = activation
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return self.down(gated_linear_unit(x, self.gate.weight, self.up.weight, self.activation))
+        if _only_multiplies(self.gate) and _only_multiplies(self.up):
+            return self.down(gated_linear_unit(x, self.gate.weight, self.up.weight, self.activation))
+        return self.down(_ACTIVATIONS[self.activation](self.gate(x)) * self.up(x))
 
 
 class _Block(nn.Module):
