@@ -80,15 +80,26 @@ class _RMSNorm(torch.autograd.Function):
         return dx.view(dy.shape), dw.to(ctx.wdtype), None
 
 
+def _is_observed(module: nn.Module) -> bool:
+    """Whether a call of the module does more than its class's forward (hooks, of its
+    own or of all modules; a forward of its own)."""
+    m = nn.modules.module
+    return any(("forward" in vars(module), module._forward_hooks, module._forward_pre_hooks, module._backward_hooks,
+                module._backward_pre_hooks, m._global_forward_hooks, m._global_forward_pre_hooks,
+                m._global_backward_hooks, m._global_backward_pre_hooks))
+
+
 def rms_norm(norm: nn.RMSNorm, x: torch.Tensor) -> torch.Tensor:
     """``norm(x)`` through the library's RMSNorm kernels when ``fused_norm``
     is set and the shape allows (GPU tensors, float32 or bfloat16 with the
     weight in the same dtype, a last dimension that is a multiple of 8 up to
-    4096), else torch's."""
+    4096), else torch's.  A norm with hooks, or of a class of its own, is called."""
+    if type(norm) is not nn.RMSNorm or _is_observed(norm):
+        return norm(x)
     D = x.shape[-1]
     w = norm.weight
     if (fused_norm and x.is_cuda and x.dtype in (torch.float32, torch.bfloat16) and w is not None
-            and w.dtype == x.dtype and D % 8 == 0 and D <= 4096 and x.numel() > 0):
+            and w.dtype == x.dtype and w.shape == (D,) and D % 8 == 0 and D <= 4096 and x.numel() > 0):
         eps = norm.eps if norm.eps is not None else torch.finfo(x.dtype).eps
         return _RMSNorm.apply(x, w, eps)
     return norm(x)
@@ -102,19 +113,10 @@ def _make_norm(kind: str, d_model: int, eps: float) -> nn.Module:
     raise ValueError(f"unknown norm {kind!r} (rms or layer)")
 
 
-def _is_observed(module: nn.Module) -> bool:
-    """Whether a call of the module does more than its class's forward (hooks, of its
-    own or of all modules; a forward of its own)."""
-    m = nn.modules.module
-    return any(("forward" in vars(module), module._forward_hooks, module._forward_pre_hooks, module._backward_hooks,
-                module._backward_pre_hooks, m._global_forward_hooks, m._global_forward_pre_hooks,
-                m._global_backward_hooks, m._global_backward_pre_hooks))
-
-
 def apply_norm(norm: nn.Module, x: torch.Tensor) -> torch.Tensor:
     """``norm(x)`` through the library's kernels: ``layer_norm`` for an
     nn.LayerNorm over the last dimension on the GPU, ``rms_norm`` for an
-    nn.RMSNorm.  A layer norm with hooks, or of a class of its own, is called."""
+    nn.RMSNorm.  A norm with hooks, or of a class of its own, is called."""
     if isinstance(norm, nn.LayerNorm):
         if (type(norm) is nn.LayerNorm and not _is_observed(norm) and x.is_cuda
                 and x.dtype in (torch.float32, torch.bfloat16) and norm.normalized_shape == (x.shape[-1],)):

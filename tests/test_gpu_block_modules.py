@@ -110,3 +110,34 @@ def test_changed_projections_of_a_feed_forward_half(kind, name):
 def test_unknown_activations_are_refused():
     with pytest.raises(ValueError, match="activation"):
         stack.GatedFeedForward(D, HIDDEN, "tanh").cuda()(torch.zeros(1, D, device="cuda"))
+
+
+@pytest.mark.parametrize("kind", ["forward hook", "pre hook", "backward hook", "global hook", "own forward", "subclass",
+                                  "another module"])
+def test_an_rms_norm_is_called_with_its_hooks(kind):
+    print(f"[case] rms norm, {kind}", flush=True)
+    torch.manual_seed(2)
+    block, seen = stack.LinearAttentionBlock(D, heads=4, max_length=8).cuda(), []
+    if kind == "subclass":
+        class Centred(nn.RMSNorm):
+            def forward(self, x):
+                return super().forward(x - x.mean(-1, keepdim=True))
+        block.head_norm, handle = Centred(D // 4).cuda(), None
+    elif kind == "another module":
+        block.head_norm, handle = nn.Tanh(), None
+    else:
+        handle = _change(block, "head_norm", kind, seen)
+    _both(lambda x: stack.apply_norm(block.head_norm, x), lambda x: block.head_norm(x),
+          torch.randn(3, 5, D // 4, device="cuda"), handle)
+    assert len(seen) == (2 if kind == "backward hook" else 0)
+
+
+@pytest.mark.parametrize("mixer", ["sparc", "linear"])
+def test_a_stack_calls_every_norm_that_is_observed(mixer):
+    torch.manual_seed(3)
+    model = stack.SPARCStack(2, D, 2, mixer=mixer, heads=4, feed_forward=HIDDEN, max_length=8).cuda()
+    norms, seen = [m for m in model.modules() if isinstance(m, nn.RMSNorm)], []
+    for m in norms:
+        m.register_forward_hook(lambda mod, args, y: seen.append(mod))
+    model(torch.randn(2, 8, D, device="cuda"))
+    assert set(seen) == set(norms) and len(seen) == len(norms) == (7 if mixer == "linear" else 5)
