@@ -35,7 +35,8 @@ from .norm import layer_norm
 from .sparc import SPARCMixer
 
 # Fold the controls into the input projection (see mixer._ProjectedMixer);
-# False runs the projection and the module separately.
+# False runs the projection and the module separately, as do hooks on either and
+# modules of other classes.
 fuse_projection = True
 # RMSNorm through sparc_rms_norm_forward / _backward where the shape allows
 # (rms_norm below); False keeps torch's RMSNorm.
@@ -253,7 +254,8 @@ class SPARCBlock(_Block):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         xn = apply_norm(self.norm, x)
-        if fuse_projection and _mixer.get_mixer_path() != "composed" and \
+        if fuse_projection and _mixer.get_mixer_path() != "composed" and _only_multiplies(self.in_proj) and \
+                type(self.mixer) is SPARCMixer and not _is_observed(self.mixer) and \
                 _mixer.projected_fused_supported(xn, self.in_proj.weight):
             y, _ = _mixer.projected_sequence(self.mixer, xn, self.in_proj.weight)
         else:

@@ -141,3 +141,20 @@ def test_a_stack_calls_every_norm_that_is_observed(mixer):
         m.register_forward_hook(lambda mod, args, y: seen.append(mod))
     model(torch.randn(2, 8, D, device="cuda"))
     assert set(seen) == set(norms) and len(seen) == len(norms) == (7 if mixer == "linear" else 5)
+
+
+@pytest.mark.parametrize("kind,name", [(kind, "in_proj") for kind in KINDS] + [
+    (kind, "mixer") for kind in ("pre hook", "backward hook", "own forward")])
+def test_changed_modules_of_a_sparc_block(kind, name):
+    """A fused call takes the projection and the mixer together where neither does more."""
+    print(f"[case] {kind} at {name}", flush=True)
+    torch.manual_seed(4)
+    block, seen = stack.SPARCBlock(D, 2).cuda(), []
+    if name == "mixer" and kind == "own forward":
+        inner, handle = block.mixer.forward, None
+        block.mixer.forward = lambda x, return_cache=False: inner(-x, return_cache)
+    else:
+        handle = _change(block, name, kind, seen)
+    _both(block, lambda x: x + block.out_proj(block.mixer(block.in_proj(block.norm(x)))[0]),
+          torch.randn(2, 16, D, device="cuda"), handle)
+    assert len(seen) == (2 if kind == "backward hook" else 0)
