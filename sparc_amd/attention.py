@@ -25,6 +25,22 @@ def rotary_table(length: int, dim: int, base: float = 10000.0, device=None) -> t
     return torch.cat((angle.cos(), angle.sin()), dim=-1).float()
 
 
+def keep_reach(positions: torch.Tensor, reach: int | None) -> torch.Tensor:
+    """``positions``, with how far they reach at most (the steps behind them) kept on
+    the host beside them, so that a limit is checked without waiting for the device.
+    It holds until the tensor is written; an inference tensor, which does not count
+    its writes, keeps none."""
+    if reach is not None and not positions.is_inference():
+        positions.reach = (reach, positions._version)
+    return positions
+
+
+def reach_of(positions: torch.Tensor) -> int | None:
+    """What ``keep_reach`` has kept beside the tensor, or None."""
+    reach, version = getattr(positions, "reach", (None, None))
+    return reach if version is not None and positions._version == version else None
+
+
 def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
                    table: torch.Tensor, positions: torch.Tensor | None = None, interleaved: bool = False,
                    eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:

@@ -9,6 +9,7 @@ from typing import NamedTuple, Sequence
 import torch
 
 from . import _lib
+from .attention import keep_reach, reach_of
 
 MAX_BEAMS = 32
 
@@ -64,9 +65,13 @@ def reorder_states(states: Sequence, parents: torch.Tensor, out_states: Sequence
 def _reorder(states, parents, out_states):
     planes = _planes(states)
     out = None if out_states is None else planes if out_states is states else _planes(out_states)
+    reaches = [reach_of(p) for p in planes]  # of positions, whatever their order
     new = _lib.native().reorder(planes, parents, out)
     if new is None:
         _refuse_states(planes, parents, out)
+    for reach, one in zip(reaches, new):
+        if reach is not None:
+            keep_reach(one, reach)
     return _like(states, new)
 
 

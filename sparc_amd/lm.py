@@ -80,7 +80,11 @@ def beam_search(model: SPARCLanguageModel, prompt: torch.Tensor, beams: int, ste
     """The ``beams`` best continuations of each prompt row [B, T] by ``steps``
     ids: (ids [B, beams, steps], scores [B, beams]), best first.  With
     ``eos_id`` a hypothesis that has ended keeps its score and repeats
-    ``eos_id``.  Nothing waits for the device between the steps."""
+    ``eos_id``.  Nothing waits for the device between the steps.  A prompt and
+    steps of more positions than the stack's ``max_length`` are refused."""
+    limit, positions = model.stack.max_length, prompt.shape[1] + max(steps - 1, 0)
+    if limit is not None and positions > limit:
+        raise ValueError(f"{positions} positions are more than max_length {limit}")
     model.stack.prepare_inference()
     logits, states = model.prefill(prompt)
     B, V = logits.shape

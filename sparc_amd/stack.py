@@ -28,7 +28,8 @@ from torch import nn
 
 from . import _lib
 from . import mixer as _mixer
-from .attention import linear_attention, linear_attention_step, qk_norm_rotary, rotary_table
+from .attention import (keep_reach, linear_attention, linear_attention_step, qk_norm_rotary, reach_of,
+                        rotary_table)
 from .control import aligned16
 from .feed_forward import gated_linear_unit
 from .norm import layer_norm
@@ -176,7 +177,10 @@ class LinearAttentionBlock(_Block):
     (``qk_norm_rotary``), ``linear_attention`` with a decay for each head from 32 steps
     of memory to 4096, a norm of each head's output, and the projection back.  The
     state of a row is (S [heads, D, D] fp32, position); positions reach
-    ``max_length``."""
+    ``max_length``, and a prompt or a step behind it is refused.  (How far positions
+    reach is kept on the host beside their tensor, and ``step`` and ``reorder_states``
+    hand it on.  Positions that a program has made or written itself, copies among
+    them, are not checked: behind ``max_length`` outputs and states are NaN.)"""
 
     def __init__(self, d_model: int, heads: int, kv_heads: int | None = None, eps: float = 1e-6, norm: str = "rms",
                  feed_forward: int = 0, max_length: int = 65536):
@@ -205,6 +209,10 @@ class LinearAttentionBlock(_Block):
             self.log_decay, self.table = (t.to(self.log_decay.device) for t in (decay, table))
         return self
 
+    @property
+    def max_length(self) -> int:
+        return self.table.shape[0]
+
     def _heads(self, x: torch.Tensor):
         """(q, k, v) [B, T, heads, D] of the block's input, before norms and rotation."""
         both = self.qkv(apply_norm(self.norm, x))
@@ -215,8 +223,8 @@ class LinearAttentionBlock(_Block):
         return self._feed_forward(x + self.out_proj(rms_norm(self.head_norm, o).flatten(-2)))
 
     def _attend(self, x: torch.Tensor):
-        if x.shape[1] > self.table.shape[0]:
-            raise ValueError(f"{x.shape[1]} positions are more than max_length {self.table.shape[0]}")
+        if x.shape[1] > self.max_length:
+            raise ValueError(f"{x.shape[1]} positions are more than max_length {self.max_length}")
         q, k, v = self._heads(x)
         q, k = qk_norm_rotary(q, k, self.q_weight, self.k_weight, self.table, eps=self.eps)
         o, state = linear_attention(q, k, v, self.log_decay)
@@ -228,16 +236,23 @@ class LinearAttentionBlock(_Block):
     def prefill(self, x: torch.Tensor):
         """(output, state) of a sequence [B, T, d_model]."""
         y, state = self._attend(x)
-        return y, (state, torch.full((x.shape[0],), x.shape[1], dtype=torch.int64, device=x.device))
+        with torch.inference_mode(False):
+            position = torch.full((x.shape[0],), x.shape[1], dtype=torch.int64, device=x.device)
+        return y, (state, keep_reach(position, x.shape[1]))
 
     @torch.no_grad()
     def step(self, x: torch.Tensor, state):
         """(output, new state) of one position [B, d_model]; no gradient."""
         s, position = state
+        reach = reach_of(position)
+        if reach is not None and reach >= self.max_length:
+            raise ValueError(f"{reach + 1} positions are more than max_length {self.max_length}")
         q, k, v = self._heads(x[:, None])
         q, k = qk_norm_rotary(q, k, self.q_weight, self.k_weight, self.table, position[:, None], eps=self.eps)
         o, s = linear_attention_step(q[:, 0], k[:, 0], v[:, 0], self.log_decay, s)
-        return self._out(x, o), (s, position + 1)
+        with torch.inference_mode(False):
+            position = position + 1
+        return self._out(x, o), (s, position if reach is None else keep_reach(position, reach + 1))
 
 
 class SPARCBlock(_Block):
@@ -300,6 +315,11 @@ class SPARCStack(nn.Module):
             raise ValueError(f"unknown mixer {mixer!r} (sparc or linear)")
         self.blocks = nn.ModuleList(make() for _ in range(n_layers))
         self.norm = _make_norm(norm, d_model, eps)
+
+    @property
+    def max_length(self) -> int | None:
+        """The positions that all blocks have, or None where there is no limit."""
+        return min((blk.max_length for blk in self.blocks if isinstance(blk, LinearAttentionBlock)), default=None)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         for blk in self.blocks:
