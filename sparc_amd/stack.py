@@ -180,10 +180,12 @@ class LinearAttentionBlock(_Block):
     ``max_length``, and a prompt or a step behind it is refused.  (How far positions
     reach is kept on the host beside their tensor, and ``step`` and ``reorder_states``
     hand it on.  Positions that a program has made or written itself, copies among
-    them, are not checked: behind ``max_length`` outputs and states are NaN.)"""
+    them, are not checked: behind ``max_length`` outputs and states are NaN.)
+    ``table``: the positions' ``rotary_table(max_length, D)``, where other blocks have
+    it already."""
 
     def __init__(self, d_model: int, heads: int, kv_heads: int | None = None, eps: float = 1e-6, norm: str = "rms",
-                 feed_forward: int = 0, max_length: int = 65536):
+                 feed_forward: int = 0, max_length: int = 65536, table: torch.Tensor | None = None):
         super().__init__()
         kv_heads = heads if kv_heads is None else kv_heads
         if heads < 1 or kv_heads < 1 or d_model % heads or heads % kv_heads or d_model // heads % 2:
@@ -198,7 +200,8 @@ class LinearAttentionBlock(_Block):
         self.out_proj = nn.Linear(d_model, d_model, bias=False)
         decay = torch.log1p(-torch.exp2(-5.0 - 7.0 * torch.arange(heads) / max(1, heads - 1)))
         self.register_buffer("log_decay", decay, persistent=False)
-        self.register_buffer("table", rotary_table(max_length, self.head_dim), persistent=False)
+        self.register_buffer("table", rotary_table(max_length, self.head_dim) if table is None else table,
+                             persistent=False)
         self._make_feed_forward(d_model, feed_forward, norm, eps)
 
     def _apply(self, fn, recurse=True):
@@ -310,11 +313,24 @@ class SPARCStack(nn.Module):
         elif mixer == "linear":
             if heads is None:
                 raise ValueError("linear attention needs heads")
-            make = lambda: LinearAttentionBlock(d_model, heads, kv_heads, eps, norm, feed_forward, max_length)
+            # one table of angles for all of them (33 MB at 65536 positions and heads of 128)
+            make = lambda: LinearAttentionBlock(d_model, heads, kv_heads, eps, norm, feed_forward, max_length,
+                                                self.blocks[0].table if len(self.blocks) else None)
         else:
             raise ValueError(f"unknown mixer {mixer!r} (sparc or linear)")
-        self.blocks = nn.ModuleList(make() for _ in range(n_layers))
+        self.blocks = nn.ModuleList()
+        for _ in range(n_layers):
+            self.blocks.append(make())
         self.norm = _make_norm(norm, d_model, eps)
+
+    def _apply(self, fn, recurse=True):
+        # torch moves the buffers block by block: tables that were one are made one again
+        blocks = [blk for blk in self.blocks if isinstance(blk, LinearAttentionBlock)]
+        before, after = [blk.table for blk in blocks], {}
+        super()._apply(fn, recurse)
+        for blk, table in zip(blocks, before):
+            blk.table = after.setdefault(id(table), blk.table)
+        return self
 
     @property
     def max_length(self) -> int | None:
