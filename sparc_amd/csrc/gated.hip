@@ -12,10 +12,10 @@
 // Bound by what feeds the matrix instructions from LDS (a step of 64 values of a tile of
 // 256 x 256 takes 192 KB of reads there, about as long as its products), and where the
 // contraction is short by a tile's first loads and its results, which nothing overlaps
-// with one tile to a CU.  bf16, forward: 8192 x 4096 on 4096 590 us (930 TFLOP/s), 32768 x
-// 768 on 2048 280 us (740 TFLOP/s) and the projections' gradients 390; 256 rows of 2048 on
-// 8192 31 us, 1 row 16 us (67 MB of weights, 4.1 TB/s).  fp32: 1237 x 1001 on 2731 106 us
-// (128 TFLOP/s as one product's, 770 as the six bf16 ones).
+// with one tile to a CU.  bf16, forward, in long runs: 8192 x 4096 on 4096 484 us (1.14
+// PFLOP/s), 32768 x 768 on 2048 247 us (0.83 PFLOP/s; the whole backward 789); 256 rows of
+// 2048 on 8192 28 us, 1 row 14 us (67 MB of weights, 4.8 TB/s).  fp32: 1237 x 1001 on 2731
+// 91 us (148 TFLOP/s as one product's, 890 as the six bf16 ones).
 #include "matrix.h"
 
 namespace sparc {
@@ -24,9 +24,11 @@ namespace {
 enum Act : int { ACT_SILU = 0, ACT_GELU = 1, ACT_RELU = 2, ACT_SIGMOID = 3 };
 
 // act(g), and its derivative.  For results in bf16 the sigmoid is that of the hardware's
-// base-2 exponential and reciprocal (some 2^-21 of its value; the library's take 30
-// instructions more for each value, and a tile of 256 x 256 results is computed in
-// little more time than its activations were).
+// base-2 exponential and reciprocal: off by some 2^-22 of its value, and for negative g
+// by |g| 2^-24 more, what rounding the exponent |g| / ln 2 leaves (2^-17 at g = -80,
+// where a result's rounding is 2^-8).  The library's functions take 30 instructions more
+// for each value, and a tile of 256 x 256 results is computed in little more time than
+// its activations were.
 template <typename IO> __device__ __forceinline__ float act_of(int act, float g, float& slope) {
   if (act == ACT_RELU) {
     slope = g > 0.0f ? 1.0f : 0.0f;
@@ -489,11 +491,14 @@ Cut cut_of(int32_t io, bool whole, int64_t np, int64_t nq, int64_t nk, int parts
 bool is_whole(int32_t io, int64_t m, int64_t n = 0) { return io == SPARC_BF16 ? (m | n) % 8 == 0 : (m | n) % 4 == 0; }
 
 // dg and du are rounded to bf16 for the products with them, which makes their results'
-// errors 1.4 times as large as one rounding's.  Where launches take the time rather than
-// the products, what the rounding took is multiplied too, and the errors are one
-// rounding's (the backward's kernels of 32 rows of 64 on 96 17.6 -> 21.6 us, of 1000 of
-// 256 on 1024 42 -> 50, behind some 50 of autograd; at 32768 rows of 768 on 2048 it
-// would be another 500 beside 1050).
+// errors 1.4 times as large as one rounding's: 0.00235 of the gradients instead of
+// 0.00166 (two library products that keep the projections in bf16: 0.0034 to 0.0039).
+// Where launches take the time rather than the products, what the rounding took is
+// multiplied too, and the errors are one rounding's: the backward's kernels of 32 rows of
+// 64 on 96 17.6 -> 21.6 us, of 1000 of 256 on 1024, at the border, 42 -> 50, behind some
+// 50 of autograd.  Above it the products would be as many again as dx and the weights
+// take: 512 rows of 1024 on 1024 38 -> 52 us, 512 of 1024 on 4096 64 -> 110, 2048 of
+// 2048 on 8192 436 -> 660, 32768 of 768 on 2048 789 -> 1312.
 constexpr int64_t kRestUpTo = 1LL << 28;  // rows x dim x hidden
 
 struct GatedPlan {

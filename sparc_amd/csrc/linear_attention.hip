@@ -16,9 +16,10 @@
 // and every row is read once (with time segments keys and values twice).  What bounds a
 // chain is neither memory nor the matrix instructions but one chunk after the other: load,
 // scores, the split of scores and state into bf16 parts, products, update (65536 steps of
-// 16 heads of 128 x 128 bf16: 130 us for the states of 32 segments, 17 to join them, 290
-// for the outputs, at 3.9 TB/s, the matrix instructions busy 27 % and the VALU 36 % of the
-// time; the gradients of 8 x 4096 steps of 8 heads 290 us, 192 workgroups on 256 CUs).
+// 16 heads of 128 x 128 bf16: 134 us for the states of 32 segments, 17 to join them, 321
+// for the outputs, at 3.6 TB/s, the matrix instructions busy 25 % and the VALU 33 % of the
+// time, 423 in long runs; the gradients of 8 x 4096 steps of 8 heads 300 us, 192
+// workgroups on 256 CUs).
 #include "matrix.h"
 
 namespace sparc {
