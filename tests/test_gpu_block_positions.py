@@ -99,3 +99,33 @@ def test_beam_search_ends_at_max_length():
     assert lm.beam_search(model, full, beams=2, steps=0)[0].shape == (1, 2, 0)
     sparc = lm.SPARCLanguageModel(20, 1, 32, 1).cuda()
     assert lm.beam_search(sparc, prompt, beams=2, steps=5)[1].isfinite().all()
+
+
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode], ids=["no_grad", "inference"])
+def test_a_captured_step(mode):
+    """Replays read positions from the state's tensors, which the host does not follow:
+    the last one's angles are there, and behind it outputs are NaN."""
+    stack = _stack(feed_forward=48)
+    x = torch.randn(2, LENGTH + 1, 32, device="cuda")
+    with mode():
+        want = stack(x[:, :LENGTH])
+        _, states = stack.prefill(x[:, :3])
+        token = x[:, 3].clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):  # what the first call allocates
+            stack.step(token, states)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y, new = stack.step(token, states)
+        for t in range(3, LENGTH + 1):
+            token.copy_(x[:, t])
+            graph.replay()
+            for old, fresh in zip(states, new):
+                for a, b in zip(old, fresh):
+                    a.copy_(b)
+            if t < LENGTH:
+                torch.testing.assert_close(y, want[:, t], rtol=1e-4, atol=1e-4)
+            else:
+                assert y.isnan().all()
