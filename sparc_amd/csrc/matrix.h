@@ -104,7 +104,8 @@ __device__ __forceinline__ uint32_t upper_halves(uint32_t a, uint32_t b) {
 // fp32 values as a sum of N fragments.  Two parts are rounded to nearest: of a value
 // from 1 to 2 the first leaves 2^-8 at most, of which the second leaves 2^-17 (truncated
 // they would leave 2^-15, and always on the same side).  Three are truncated, 8 bits
-// each, and hold all 24.  (A value that is infinite becomes NaN for N > 1.)
+// each, and hold all 24.  (A value that is infinite, or that two parts round to it,
+// which takes 3.39e38, becomes NaN for N > 1.)
 template <int N> __device__ __forceinline__ void split(const float (&x)[8], Frag<bf16> (&f)[N]) {
   uint32_t r[8];
 #pragma unroll
